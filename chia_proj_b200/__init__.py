@@ -32,5 +32,13 @@ from .ops import (  # noqa: F401
     tile_plan,
     visible_pairs,
 )
+from .paged import (  # noqa: F401
+    PageStep,
+    cache_append,
+    new_cache,
+    page_tables,
+    paged_attention,
+    release_pages,
+)
 from ._native import ChiaError  # noqa: F401
 from . import flex  # noqa: F401,E402

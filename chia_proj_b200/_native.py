@@ -1,4 +1,5 @@
-"""ctypes binding of ``libchia_attn.so`` (declared in ``include/chia_attn.h``).
+"""ctypes binding of ``libchia_attn.so`` (declared in ``include/chia_attn.h``
+and ``include/chia_paged.h``).
 
 The library is built in-tree by ``chia_proj_b200.build`` and loaded from
 ``chia_proj_b200/_lib/``. There is no fallback: if the library is missing or
@@ -9,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -31,6 +33,8 @@ STATUS = {
     4: "CHIA_ERR_LAUNCH",
     5: "CHIA_ERR_DEVICE_TIMEOUT",
     6: "CHIA_ERR_NO_DEVICE",
+    8: "CHIA_ERR_BAD_INDEX",
+    16: "CHIA_ERR_NO_PAGES",
 }
 
 EXPORTED_SYMBOLS = (
@@ -103,6 +107,132 @@ class AttnGrads(ctypes.Structure):
     ]
 
 
+# ---- the paged 8-bit K/V cache (include/chia_paged.h)
+PAGED_ABI_VERSION = 1
+CACHE_E4M3, CACHE_INT8 = 0, 1
+BAD_INDEX, NO_PAGES = 8, 16
+
+PAGED_SYMBOLS = (
+    "chia_page_tables",
+    "chia_release_pages",
+    "chia_cache_append",
+    "chia_paged_attn",
+    "chia_paged_attn_workspace_bytes",
+)
+
+
+class TablesParams(ctypes.Structure):
+    """Mirror of ``chia_tables_params_t`` (include/chia_paged.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("ring_size", ctypes.c_int64),
+        ("max_tokens", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_state", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p),
+        ("new_seq_lens", ctypes.c_void_p),
+        ("new_free_state", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AppendParams(ctypes.Structure):
+    """Mirror of ``chia_append_params_t`` (include/chia_paged.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("num_pages", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2),
+        ("slots", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class PagedParams(ctypes.Structure):
+    """Mirror of ``chia_paged_params_t`` (include/chia_paged.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("mod", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_q", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("num_pages", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("o_stride", ctypes.c_int64 * 2),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("head_param", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("sig_bias", ctypes.c_float),
+        ("out_scale", ctypes.c_float),
+        ("win_left", ctypes.c_int64),
+        ("win_right", ctypes.c_int64),
+        ("block", ctypes.c_int64),
+        ("prefix", ctypes.c_int64),
+        ("dilation", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("wait_limit_ns", ctypes.c_uint64),
+    ]
+
+
+def packer(struct_type):
+    """``struct.Struct(...).pack`` for a ctypes structure of this file: all
+    fields in one call, which is several times quicker than setting them one by
+    one. Arrays take one value an element."""
+    codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_uint64: "Q", ctypes.c_float: "f",
+             ctypes.c_void_p: "Q"}
+    fmt = ""
+    for _, t in struct_type._fields_:
+        fmt += codes[t._type_] * t._length_ if hasattr(t, "_length_") else codes[t]
+    s = struct.Struct("@" + fmt)
+    assert s.size == ctypes.sizeof(struct_type), struct_type
+    return s.pack
+
+
 class ChiaError(RuntimeError):
     """A non-zero ``chia_status`` returned by the library."""
 
@@ -153,6 +283,11 @@ def load() -> ctypes.CDLL:
             lib.chia_attn_status_string.restype = ctypes.c_char_p
             lib.chia_attn_abi_version.argtypes = []
             lib.chia_attn_abi_version.restype = ctypes.c_int
+            for name in PAGED_SYMBOLS[:4]:  # the parameters as the bytes of their struct
+                getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+                getattr(lib, name).restype = ctypes.c_int
+            lib.chia_paged_attn_workspace_bytes.argtypes = [ctypes.c_char_p]
+            lib.chia_paged_attn_workspace_bytes.restype = ctypes.c_int64
             if lib.chia_attn_abi_version() != ABI_VERSION:
                 raise ImportError(f"{LIB_PATH}: ABI version mismatch")
             _lib = lib

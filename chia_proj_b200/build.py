@@ -2,7 +2,8 @@
 
     python -m chia_proj_b200.build [--force] [--verbose]
 
-The library is a plain shared object with C linkage (``include/chia_attn.h``);
+The library is a plain shared object with C linkage (``include/chia_attn.h``,
+``include/chia_paged.h``);
 it links the CUDA runtime statically and fetches ``cuTensorMapEncodeTiled``
 from the driver at run time, so it needs no libcuda at link time.
 """
@@ -12,19 +13,22 @@ from __future__ import annotations
 import argparse
 import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "_lib", "libchia_attn.so")
+OBJ = os.path.join(HERE, "_lib", "_build")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
+    "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     "-cudart", "static",
 ]
 
@@ -41,8 +45,8 @@ def sources():
 
 
 def _deps():
-    return sources() + sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + [
-        os.path.join(ROOT, "include", "chia_attn.h")]
+    return sources() + sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + sorted(
+        glob.glob(os.path.join(ROOT, "include", "*.h")))
 
 
 def up_to_date() -> bool:
@@ -52,17 +56,46 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(d) <= t for d in _deps())
 
 
+def _headers(src: str, seen=None):
+    """The headers of this repository that ``src`` includes, directly or not."""
+    seen = set() if seen is None else seen
+    with open(src) as f:
+        names = re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M)
+    for n in names:
+        p = os.path.normpath(os.path.join(os.path.dirname(src), n))
+        if os.path.exists(p) and p not in seen:
+            seen.add(p)
+            _headers(p, seen)
+    return seen
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if any source is newer; returns its path."""
+    """Compile the library if any source is newer; returns its path. Each
+    source file is an object of its own, compiled only when it or one of its
+    headers changed, several at a time."""
     if not force and up_to_date():
         return OUT
     os.makedirs(os.path.dirname(OUT), exist_ok=True)
+    os.makedirs(OBJ, exist_ok=True)
+    nvcc = _nvcc()
+
+    def compile_one(src: str) -> str:
+        obj = os.path.join(OBJ, os.path.basename(src) + ".o")
+        newest = max(os.path.getmtime(p) for p in (src, *_headers(src)))
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) >= newest:
+            return obj
+        cmd = [nvcc, *NVCC_FLAGS, "-c", "-I", os.path.join(ROOT, "include"), "-o", obj + ".tmp", src]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+        os.replace(obj + ".tmp", obj)
+        return obj
+
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        objects = list(pool.map(compile_one, sources()))
     tmp = OUT + ".tmp"
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-o", tmp, *sources()]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", tmp, *objects], check=True)
     os.replace(tmp, OUT)
     return OUT
 

@@ -22,6 +22,7 @@
 #include <mutex>
 
 #include "../../include/chia_attn.h"
+#include "../../include/chia_paged.h"
 #include "bwd_sm100.cuh"
 #include "decode_sm100.cuh"
 #include "fmha2_sm100.cuh"
@@ -703,6 +704,8 @@ const char *chia_attn_status_string(int status) {
     case CHIA_ERR_LAUNCH: return "kernel launch or tensor-map encoding failed";
     case CHIA_ERR_DEVICE_TIMEOUT: return "bounded device wait expired";
     case CHIA_ERR_NO_DEVICE: return "no usable sm_100 device";
+    case CHIA_ERR_BAD_INDEX: return "length, page, slot or offset out of range";
+    case CHIA_ERR_NO_PAGES: return "a request was not served: no free page, or its table row is full";
   }
   return "unknown status";
 }

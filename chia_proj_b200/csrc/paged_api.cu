@@ -1,0 +1,283 @@
+// paged_api.cu -- extern "C" entry points of the paged 8-bit K/V cache
+// (include/chia_paged.h): argument checks, choice of the kernel, launch. No
+// allocation, no synchronisation.
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/chia_paged.h"
+#include "cache_sm100.cuh"
+#include "paged_attn_sm100.cuh"
+
+namespace {
+
+constexpr int64_t kI32 = 0x7fffffffLL;
+
+bool aligned(const void *p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+bool page_ok(int64_t p) { return p == 16 || p == 32 || p == 64 || p == 128; }
+
+// The current device's number of SMs; CHIA_ERR_NO_DEVICE where it is no sm_100.
+int device_sms(int &sms) {
+  int dev = 0, major = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+      major != 10 ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1)
+    return CHIA_ERR_NO_DEVICE;
+  return CHIA_OK;
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? CHIA_OK : CHIA_ERR_LAUNCH; }
+
+// ---------------------------------------------------------------------- tables
+int tables_args(const chia_tables_params_t *p, bool release, chia::TablesArgs &a) {
+  if (p == nullptr || p->abi_version != CHIA_PAGED_ABI_VERSION) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!page_ok(p->page_size)) return CHIA_ERR_UNSUPPORTED;
+  if (p->batch < 1 || p->batch > (1 << 24) || p->table_width < 1 || p->table_width > kI32 ||
+      p->table_stride < p->table_width || p->ring_size < 1 || p->ring_size > kI32 ||
+      p->max_tokens < 0 || p->max_tokens > kI32)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if (!p->seq_lens || !p->new_lens || !p->block_table || !p->free_pages || !p->free_state ||
+      !p->new_seq_lens || !p->new_free_state)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if (!release && (!p->cu_q || (p->max_tokens > 0 && (!p->slots || !p->positions))))
+    return CHIA_ERR_INVALID_ARGUMENT;
+  // the kernels read them while they write the new ones
+  if (p->new_seq_lens == p->seq_lens || p->new_free_state == p->free_state)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  for (const void *q : {static_cast<const void *>(p->seq_lens), static_cast<const void *>(p->new_lens),
+                        static_cast<const void *>(p->block_table),
+                        static_cast<const void *>(p->free_pages),
+                        static_cast<const void *>(p->free_state), static_cast<const void *>(p->slots),
+                        static_cast<const void *>(p->positions), static_cast<const void *>(p->cu_q),
+                        static_cast<const void *>(p->new_seq_lens),
+                        static_cast<const void *>(p->new_free_state),
+                        static_cast<const void *>(p->status)})
+    if (!aligned(q, 4)) return CHIA_ERR_MISALIGNED;
+  a.seq_lens = p->seq_lens;
+  a.new_lens = p->new_lens;
+  a.free_state = p->free_state;
+  a.block_table = p->block_table;
+  a.free_pages = p->free_pages;
+  a.slots = p->slots;
+  a.positions = p->positions;
+  a.cu_q = p->cu_q;
+  a.new_seq_lens = p->new_seq_lens;
+  a.new_free_state = p->new_free_state;
+  a.status = p->status;
+  a.table_stride = p->table_stride;
+  a.batch = static_cast<int32_t>(p->batch);
+  a.width = static_cast<int32_t>(p->table_width);
+  a.ring = static_cast<int32_t>(p->ring_size);
+  a.max_tokens = static_cast<int32_t>(p->max_tokens);
+  a.page = p->page_size;
+  return CHIA_OK;
+}
+
+// CTAs of the tables' kernels: one for each kTablesThreads items, one wave at most.
+int tables_grid(int64_t items, int sms) {
+  const int64_t n = (items + chia::kTablesThreads - 1) / chia::kTablesThreads;
+  return static_cast<int>(n < 1 ? 1 : n > sms ? sms : n);
+}
+
+// ---------------------------------------------------------------------- append
+int check_append(const chia_append_params_t *p) {
+  if (p == nullptr || p->abi_version != CHIA_PAGED_ABI_VERSION) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->dtype != CHIA_DTYPE_BF16 && p->dtype != CHIA_DTYPE_F16) return CHIA_ERR_UNSUPPORTED;
+  if (p->cache_dtype != CHIA_CACHE_E4M3 && p->cache_dtype != CHIA_CACHE_INT8)
+    return CHIA_ERR_UNSUPPORTED;
+  if ((p->head_dim != 64 && p->head_dim != 128) || !page_ok(p->page_size))
+    return CHIA_ERR_UNSUPPORTED;
+  if (p->heads_kv < 1 || p->heads_kv > 65535 || p->tokens < 0 || p->tokens > kI32 ||
+      p->num_pages < 1 || p->num_pages > kI32 / p->page_size)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->tokens > 0 && (!p->k || !p->v || !p->slots)) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!p->k_cache || !p->v_cache || !p->k_scale || !p->v_scale) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->k_cache, 16) ||
+      !aligned(p->v_cache, 16) || !aligned(p->slots, 4) || !aligned(p->k_scale, 4) ||
+      !aligned(p->v_scale, 4) || !aligned(p->status, 4))
+    return CHIA_ERR_MISALIGNED;
+  for (const int64_t *s : {p->k_stride, p->v_stride})
+    for (int d = 0; d < 2; ++d) {
+      if (s[d] < 0) return CHIA_ERR_INVALID_ARGUMENT;
+      if (s[d] % 8 != 0) return CHIA_ERR_MISALIGNED;
+    }
+  return CHIA_OK;
+}
+
+template <int D, bool BF16, int CT>
+int launch_append(const chia::AppendArgs &a, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads_kv), 2);
+  chia::cache_append_kernel<D, BF16, CT><<<grid, 128, 0, s>>>(a);
+  return launched();
+}
+
+// ------------------------------------------------------------------- attention
+int check_paged(const chia_paged_params_t *p) {
+  if (p == nullptr || p->abi_version != CHIA_PAGED_ABI_VERSION) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->dtype != CHIA_DTYPE_BF16 && p->dtype != CHIA_DTYPE_F16) return CHIA_ERR_UNSUPPORTED;
+  if (p->cache_dtype != CHIA_CACHE_E4M3 && p->cache_dtype != CHIA_CACHE_INT8)
+    return CHIA_ERR_UNSUPPORTED;
+  if ((p->head_dim != 64 && p->head_dim != 128) || !page_ok(p->page_size))
+    return CHIA_ERR_UNSUPPORTED;
+  if (p->norm < CHIA_NORM_SOFTMAX || p->norm > CHIA_NORM_RELU) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->mod < CHIA_MOD_NONE || p->mod > CHIA_MOD_TEMP) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->norm != CHIA_NORM_SOFTMAX && p->mod != CHIA_MOD_NONE) return CHIA_ERR_UNSUPPORTED;
+  if (p->heads < 1 || p->heads > (1 << 20) || p->heads_kv < 1 || p->heads % p->heads_kv != 0 ||
+      p->max_q < 1 || p->batch < 1 || p->batch > (1 << 24) || p->tokens < 0 || p->tokens > kI32 ||
+      p->num_pages < 1 || p->num_pages > kI32 / p->page_size || p->table_width < 1 ||
+      p->table_width > kI32 / p->page_size || p->table_stride < p->table_width)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->cu_q == nullptr && p->tokens % p->batch != 0) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->win_left < -1 || p->win_right < -1 || p->block < 0 || p->prefix < 0 || p->dilation < 1)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->tokens > 0 && (!p->q || !p->o)) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!p->k_cache || !p->v_cache || !p->k_scale || !p->v_scale || !p->block_table || !p->seq_lens)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if ((p->mod == CHIA_MOD_ALIBI || p->mod == CHIA_MOD_TEMP) && p->head_param == nullptr)
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->mod == CHIA_MOD_SOFTCAP && !(p->softcap > 0.f)) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!std::isfinite(p->scale) || !std::isfinite(p->sig_bias) || !std::isfinite(p->out_scale))
+    return CHIA_ERR_INVALID_ARGUMENT;
+  if (!aligned(p->q, 16) || !aligned(p->o, 16) || !aligned(p->k_cache, 16) ||
+      !aligned(p->v_cache, 16) || !aligned(p->k_scale, 4) || !aligned(p->v_scale, 4) ||
+      !aligned(p->block_table, 4) || !aligned(p->seq_lens, 4) || !aligned(p->cu_q, 4) ||
+      !aligned(p->lse, 4) || !aligned(p->head_param, 4) || !aligned(p->status, 4))
+    return CHIA_ERR_MISALIGNED;
+  for (const int64_t *s : {p->q_stride, p->o_stride})
+    for (int d = 0; d < 2; ++d) {
+      if (s[d] < 0) return CHIA_ERR_INVALID_ARGUMENT;
+      if (s[d] % 8 != 0) return CHIA_ERR_MISALIGNED;
+    }
+  return CHIA_OK;
+}
+
+int kind_of(const chia_paged_params_t *p) {
+  if (p->norm == CHIA_NORM_SIGMOID) return chia::KIND_SIGMOID;
+  if (p->norm == CHIA_NORM_RELU) return chia::KIND_RELU;
+  switch (p->mod) {
+    case CHIA_MOD_SOFTCAP: return chia::KIND_SOFTCAP;
+    case CHIA_MOD_ALIBI: return chia::KIND_ALIBI;
+    default: return chia::KIND_SOFTMAX;  // NONE and TEMP
+  }
+}
+
+template <int D, bool BF16, int CT>
+int launch_paged(const chia::PagedArgs &a, int kind, cudaStream_t s) {
+  const int64_t warps = static_cast<int64_t>(a.tokens) * a.heads;
+  if ((warps + 3) / 4 > kI32) return CHIA_ERR_UNSUPPORTED;
+  chia::paged_rows_kernel<D, BF16, CT><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, s>>>(a, kind);
+  return launched();
+}
+
+// Calls f.template operator()<D, BF16, CT>() for the call's types.
+#define CHIA_BY_TYPE(p, FN, ...)                                                          \
+  ((p)->head_dim == 128                                                                   \
+       ? ((p)->dtype == CHIA_DTYPE_BF16                                                   \
+              ? ((p)->cache_dtype == CHIA_CACHE_E4M3 ? FN<128, true, 0>(__VA_ARGS__)      \
+                                                     : FN<128, true, 1>(__VA_ARGS__))     \
+              : ((p)->cache_dtype == CHIA_CACHE_E4M3 ? FN<128, false, 0>(__VA_ARGS__)     \
+                                                     : FN<128, false, 1>(__VA_ARGS__)))   \
+       : ((p)->dtype == CHIA_DTYPE_BF16                                                   \
+              ? ((p)->cache_dtype == CHIA_CACHE_E4M3 ? FN<64, true, 0>(__VA_ARGS__)       \
+                                                     : FN<64, true, 1>(__VA_ARGS__))      \
+              : ((p)->cache_dtype == CHIA_CACHE_E4M3 ? FN<64, false, 0>(__VA_ARGS__)      \
+                                                     : FN<64, false, 1>(__VA_ARGS__))))
+
+}  // namespace
+
+extern "C" {
+
+int chia_page_tables(const chia_tables_params_t *p, void *stream) {
+  chia::TablesArgs a{};
+  int rc = tables_args(p, false, a), sms = 0;
+  if (rc != CHIA_OK || (rc = device_sms(sms)) != CHIA_OK) return rc;
+  chia::page_tables_kernel<<<tables_grid(p->max_tokens, sms), chia::kTablesThreads, 0,
+                             static_cast<cudaStream_t>(stream)>>>(a);
+  return launched();
+}
+
+int chia_release_pages(const chia_tables_params_t *p, void *stream) {
+  chia::TablesArgs a{};
+  int rc = tables_args(p, true, a), sms = 0;
+  if (rc != CHIA_OK || (rc = device_sms(sms)) != CHIA_OK) return rc;
+  chia::release_pages_kernel<<<tables_grid(p->ring_size, sms), chia::kTablesThreads, 0,
+                               static_cast<cudaStream_t>(stream)>>>(a);
+  return launched();
+}
+
+int chia_cache_append(const chia_append_params_t *p, void *stream) {
+  int rc = check_append(p), sms = 0;
+  if (rc != CHIA_OK || (rc = device_sms(sms)) != CHIA_OK) return rc;
+  if (p->tokens == 0) return CHIA_OK;
+  chia::AppendArgs a{};
+  a.k = p->k;
+  a.v = p->v;
+  a.k_st = p->k_stride[0], a.k_sh = p->k_stride[1];
+  a.v_st = p->v_stride[0], a.v_sh = p->v_stride[1];
+  a.slots = p->slots;
+  a.k_cache = static_cast<uint8_t *>(p->k_cache);
+  a.v_cache = static_cast<uint8_t *>(p->v_cache);
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.status = p->status;
+  a.tokens = static_cast<int32_t>(p->tokens);
+  a.heads_kv = p->heads_kv;
+  a.page = p->page_size;
+  a.num_pages = p->num_pages;
+  return CHIA_BY_TYPE(p, launch_append, a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t chia_paged_attn_workspace_bytes(const chia_paged_params_t *p) {
+  if (check_paged(p) != CHIA_OK) return -1;
+  return 256;
+}
+
+int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
+  int rc = check_paged(p), sms = 0;
+  if (rc != CHIA_OK) return rc;
+  const int64_t need = chia_paged_attn_workspace_bytes(p);
+  if (p->workspace == nullptr || p->workspace_bytes < need) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!aligned(p->workspace, 256)) return CHIA_ERR_MISALIGNED;
+  if ((rc = device_sms(sms)) != CHIA_OK) return rc;
+  if (p->tokens == 0) return CHIA_OK;
+  chia::PagedArgs a{};
+  a.q = p->q;
+  a.o = p->o;
+  a.q_st = p->q_stride[0], a.q_sh = p->q_stride[1];
+  a.o_st = p->o_stride[0], a.o_sh = p->o_stride[1];
+  a.k_cache = static_cast<const uint8_t *>(p->k_cache);
+  a.v_cache = static_cast<const uint8_t *>(p->v_cache);
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.block_table = p->block_table;
+  a.seq_lens = p->seq_lens;
+  a.cu_q = p->cu_q;
+  a.table_stride = p->table_stride;
+  a.lse = p->norm == CHIA_NORM_SOFTMAX ? p->lse : nullptr;
+  a.head_param = (p->mod == CHIA_MOD_ALIBI || p->mod == CHIA_MOD_TEMP) ? p->head_param : nullptr;
+  a.mask.left = p->win_left;
+  a.mask.right = p->win_right;
+  a.mask.block = p->block;
+  a.mask.prefix = p->prefix;
+  a.mask.dil = p->dilation;
+  a.score_scale = p->scale;
+  a.softcap = p->softcap;
+  a.sig_bias = p->sig_bias;
+  a.out_scale = p->out_scale;
+  a.heads = p->heads;
+  a.heads_kv = p->heads_kv;
+  a.group = p->heads / p->heads_kv;
+  a.batch = static_cast<int32_t>(p->batch);
+  a.tokens = static_cast<int32_t>(p->tokens);
+  a.page = p->page_size;
+  a.width = static_cast<int32_t>(p->table_width);
+  a.num_pages = p->num_pages;
+  a.status = p->status;
+  const int kind = kind_of(p);
+  return CHIA_BY_TYPE(p, launch_paged, a, kind, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,538 @@
+"""The operators of the paged 8-bit K/V cache on the GPU against plain 64-bit restatements (``paged_oracle.py``).
+
+Tables and cache contents are compared exactly. Tolerances of the attention, element by element: the output is
+rounded once to its type (at most 2^-9 relative for bf16, 2^-12 for fp16, 2^-24 absolute where fp16 is subnormal);
+P may be rounded to 16 bits with 11 significant ones before P V (2^-12 of each term; the sum of the terms' sizes is
+the oracle's ``mass``); the exponential, hyperbolic tangent and reciprocal in fp32 and the products' fp32 sums stay
+under 2^-14 of a term for the scores used here (|s| < 64). Twice their sum is allowed: 2^-8 |o| (2^-11) + 2^-10 mass.
+"""
+
+import math
+
+import pytest
+import torch
+
+import chia_proj_b200 as cp
+import paged_oracle as po
+
+pytestmark = pytest.mark.gpu
+E4M3, I8 = torch.float8_e4m3fn, torch.int8
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda):
+    yield
+    cp.check_device_status(0)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+# ---------------------------------------------------------------------- tables
+def run_tables(lens, new, width, page, ring, state, max_tokens, stride=None):
+    B = len(lens)
+    table = torch.full((B, stride or width), 7777, dtype=torch.int32)
+    nxt = 100000
+    for b, n in enumerate(lens):
+        for p in range(min(po.pages_for(n, page), width)):
+            table[b, p] = nxt
+            nxt += 1
+    host = table[:, :width].tolist()
+    dev = table.cuda()
+    view = dev[:, :width]
+    args = [ints(lens), ints(new), view, ints(ring), ints(state)]
+    keep = [a.clone() for a in args]
+    got = cp.page_tables(*args, page_size=page, max_tokens=max_tokens)
+    want = po.tables(lens, new, host, ring, state, page, max_tokens)
+    assert got.slots.tolist() == want[0]
+    assert got.positions.tolist() == want[1]
+    assert got.cu_q.tolist() == want[2]
+    assert got.seq_lens.tolist() == want[3]
+    assert got.free_state.tolist() == want[4]
+    assert view.tolist() == want[5]
+    if stride:
+        assert (dev[:, width:] == 7777).all()
+    for i in (0, 1, 3, 4):
+        assert torch.equal(args[i], keep[i])
+    return want[6]
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("B,most", [(1, 1), (1, 300), (7, 40), (64, 1), (1023, 3), (1024, 1), (1025, 2), (2500, 5)])
+def test_tables(cuda, B, most, page):
+    g = torch.Generator().manual_seed(B * 1000 + page + most)
+    lens = torch.randint(0, 4 * page, (B,), generator=g).tolist()
+    new = torch.randint(0, most + 1, (B,), generator=g).tolist()
+    lens[0] = page  # a full last page
+    new[-1] = most
+    need = sum(po.pages_for(n + m, page) - po.pages_for(n, page) for n, m in zip(lens, new))
+    ring = torch.randperm(need + 5, generator=g).tolist()
+    width = max(po.pages_for(n + m, page) for n, m in zip(lens, new))
+    head = len(ring) - 1  # wraps round
+    assert run_tables(lens, new, width, page, ring, [head, need + 3], sum(new) + 9, stride=width + 3)
+    assert run_tables(lens, new, width, page, ring, [head, need], sum(new))
+
+
+def test_tables_without_pages_left(cuda):
+    # 2 pages: the first request takes one, the second needs two and gets none, the third needs none
+    assert not run_tables([0, 0, 5, 0], [3, 20, 2, 1], 4, 16, [9, 8, 7], [1, 2], 26)
+    with pytest.raises(cp.ChiaError, match="NO_PAGES"):
+        cp.check_device_status(0)
+    # a full row: the others are served
+    assert not run_tables([30, 32, 0], [5, 1, 16], 2, 16, [4, 5, 6], [0, 3], 22)
+    with pytest.raises(cp.ChiaError, match="NO_PAGES"):
+        cp.check_device_status(0)
+
+
+def test_tables_bad_values_are_reported(cuda):
+    t = cp.page_tables(ints([-5, 3]), ints([2, 1]), ints([[1, 2], [3, 4]]), ints([5, 6, 7]), ints([0, 3]), page_size=16,
+                       max_tokens=3)
+    assert t.cu_q.tolist() == [0, 0, 1] and t.slots.tolist() == [3 * 16 + 3, -1, -1]
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+    t = cp.page_tables(ints([0]), ints([4]), ints([[1]]), ints([5]), ints([3, 1]), page_size=16, max_tokens=4)
+    assert t.slots.tolist() == [-1] * 4  # a ring head outside the ring: nothing is handed out
+    with pytest.raises(cp.ChiaError):
+        cp.check_device_status(0)
+    t = cp.page_tables(ints([0]), ints([4]), ints([[1]]), ints([5]), ints([0, 1]), page_size=16, max_tokens=3)
+    assert t.slots.tolist() == [80, 81, 82] and t.cu_q.tolist() == [0, 4]  # more tokens than max_tokens
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+
+
+@pytest.mark.parametrize("B", [1, 5, 1500])
+def test_release_and_take_again(cuda, B):
+    g = torch.Generator().manual_seed(B)
+    page, width = 16, 6
+    lens = torch.randint(0, width * page + 1, (B,), generator=g).tolist()
+    done = torch.randint(0, 2, (B,), generator=g).tolist()
+    done[-1] = 1
+    held = [po.pages_for(n, page) for n in lens]
+    perm = torch.randperm(sum(held) + 4, generator=g).tolist()
+    table, at = [], 0
+    for h in held:
+        table.append(perm[at:at + h] + [0] * (width - h))
+        at += h
+    N = len(perm)
+    ring = [-1] * N
+    for i, p in enumerate(perm[at:]):
+        ring[(N - 2 + i) % N] = p
+    dev_ring, dev_table = ints(ring), ints(table)
+    lens2, state2 = cp.release_pages(ints(done), ints(lens), dev_table, dev_ring, ints([N - 2, 4]), page_size=page)
+    back = [p for b in range(B) if done[b] for p in table[b][:held[b]]]
+    want = list(ring)
+    for i, p in enumerate(back):
+        want[(N - 2 + 4 + i) % N] = p
+    assert dev_ring.tolist() == want
+    assert lens2.tolist() == [0 if d else n for d, n in zip(done, lens)]
+    assert state2.tolist() == [N - 2, 4 + len(back)]
+    # and they are handed out again
+    n_back = min(width * page, (4 + len(back)) * page)
+    new = [0] * B
+    new[-1] = n_back
+    t = cp.page_tables(lens2, ints(new), dev_table, dev_ring, state2, page_size=page, max_tokens=n_back)
+    first = [want[(N - 2 + i) % N] for i in range(po.pages_for(n_back, page))]
+    assert t.slots.tolist() == [first[i // page] * page + i % page for i in range(n_back)]
+
+
+# ---------------------------------------------------------------------- append
+def make_cache(pages, hkv, page, D, ct, g, empty=False):
+    """Cache tensors on the GPU holding random bytes under power-of-two scales."""
+    def one():
+        x = torch.randn(pages, hkv, page, D, generator=g) * 150 / (1 if ct == E4M3 else 3)
+        q = x.clamp(-448, 448).to(ct) if ct == E4M3 else x.round().clamp(-127, 127).to(ct)
+        s = 2.0 ** torch.randint(-9, -4, (pages, hkv), generator=g).float()
+        return q, s
+    (k, ks), (v, vs) = one(), one()
+    return [t.cuda() for t in (k, v, ks, vs)]
+
+
+def check_append(k, v, slots, cache):
+    want = [(c.double().cpu(), c.dtype) for c in cache[:2]]
+    scales = [s.double().cpu() for s in cache[2:]]
+    cp.cache_append(k, v, ints(slots), *cache)
+    for x, w, s, c, cs in zip((k, v), want, scales, cache[:2], cache[2:]):
+        po.append(x.cpu(), slots, w, s)
+        assert torch.equal(cs.double().cpu(), s)
+        assert torch.equal(torch.nan_to_num(c.double().cpu(), nan=1e9), torch.nan_to_num(w[0], nan=1e9))
+
+
+@pytest.mark.parametrize("D,dtype,ct,page,hkv", [
+    (128, BF16, E4M3, 64, 8), (128, F16, E4M3, 16, 1), (64, BF16, E4M3, 128, 3), (64, F16, I8, 32, 2),
+    (128, BF16, I8, 128, 4), (128, F16, I8, 16, 5), (64, BF16, I8, 64, 1), (64, F16, E4M3, 64, 7)])
+@pytest.mark.parametrize("size", [0.05, 1.0, 900.0])
+def test_append(cuda, D, dtype, ct, page, hkv, size):
+    """Runs of every kind: one token into a page that holds some, a page's end and the next one's beginning, whole
+    pages, a page's first token, skipped tokens; small, ordinary and large values beside the scales that are there."""
+    g = torch.Generator().manual_seed(D + page + hkv)
+    cache = make_cache(12, hkv, page, D, ct, g)
+    runs = [(3, 5, 1), (7, page - 2, 2), (1, 0, page), (9, 0, 3), (4, 1, page - 1), (0, page - 1, 1), (11, 0, 1)]
+    slots = []
+    for p, off, n in runs:
+        slots += [p * page + off + i for i in range(n)]
+        slots += [-1] * (p % 2)
+    T = len(slots)
+    qkv = (torch.randn(T, 3 * hkv + 2, D, generator=g) * size).to(dtype).cuda()
+    qkv[T // 2] *= 8
+    check_append(qkv[:, 1:1 + hkv], qkv[:, 2 * hkv:3 * hkv], slots, cache)
+    # again: nothing grows any more
+    before = [c.clone() for c in cache]
+    cp.cache_append(qkv[:, 1:1 + hkv], qkv[:, 2 * hkv:3 * hkv], ints(slots), *cache)
+    for a, b in zip(before, cache):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("ct", [E4M3, I8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_special_values(cuda, ct, dtype):
+    g = torch.Generator().manual_seed(5)
+    page, D = 16, 64
+    x = torch.randn(6 * page, 2, D, generator=g).to(dtype)
+    x[3, 0, 5] = math.inf
+    x[4, 0, 6] = -math.inf
+    x[5, 1, 7] = math.nan
+    x[page:2 * page] = 0  # a page of zeros: the smallest scale
+    x[2 * page:3 * page] = math.inf  # nothing finite in the page
+    top = po.TOP[ct]
+    x[3 * page] = torch.tensor(top).to(dtype)  # exactly the largest value (bf16: 127 and 448 are exact)
+    x[3 * page + 1:4 * page] *= 0.01
+    x[4 * page:5 * page] *= 2.0 ** -14  # small ones
+    x[5 * page:] = torch.finfo(dtype).max
+    cache = make_cache(6, 2, page, D, ct, g)
+    x = x.cuda()
+    check_append(x, x.flip(0).contiguous(), list(range(6 * page)), cache)
+    check_append(x[:1], x[:1] * 3, [page + 7], cache)  # a token that needs a larger scale than a page of zeros has
+
+
+def test_append_grows_a_page_step_by_step(cuda):
+    """One token at a time, each larger than those before: the page is re-expressed at every step."""
+    for ct in (E4M3, I8):
+        g = torch.Generator().manual_seed(9)
+        cache = make_cache(2, 3, 32, 128, ct, g)
+        for i in range(32):
+            x = (torch.randn(1, 3, 128, generator=g) * 1.3 ** i).to(BF16).cuda()
+            check_append(x, x * -0.5, [32 + i], cache)
+
+
+@pytest.mark.parametrize("T,hkv", [(1, 1), (1, 8), (257, 8), (4100, 2), (700, 16)])
+def test_append_long(cuda, T, hkv):
+    g = torch.Generator().manual_seed(T)
+    page, D = 64, 128
+    off = 37
+    pages = po.pages_for(off + T, page)
+    perm = torch.randperm(pages, generator=g).tolist()
+    slots = [perm[(off + t) // page] * page + (off + t) % page for t in range(T)]
+    cache = make_cache(pages, hkv, page, D, E4M3, g)
+    x = torch.randn(T, 2 * hkv, D, generator=g).to(BF16).cuda()
+    check_append(x[:, :hkv], x[:, hkv:], slots, cache)
+
+
+def test_append_slots_out_of_range(cuda):
+    g = torch.Generator().manual_seed(3)
+    cache = make_cache(4, 2, 16, 64, E4M3, g)
+    x = torch.randn(5, 2, 64, generator=g).to(BF16).cuda()
+    check_append(x, x, [5, 4 * 16, 4 * 16 + 1, 2 ** 31 - 1, 17], cache)
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+    cp.cache_append(x[:0], x[:0], ints([]), *cache)  # no tokens
+
+
+# ------------------------------------------------------------------- attention
+def setup(lens, counts, H, hkv, D, page, ct, dtype, seed=0, spare=3, qsize=1.0):
+    g = torch.Generator().manual_seed(seed)
+    need = [po.pages_for(n, page) for n in lens]
+    total = sum(need) + spare
+    perm = torch.randperm(total, generator=g).tolist()
+    W = max(1, max(need)) + 1
+    table, at = [], 0
+    for n in need:
+        table.append(perm[at:at + n] + [2 ** 30] * (W - n))  # entries that nothing may read
+        at += n
+    k, v, ks, vs = make_cache(total, hkv, page, D, ct, g)
+    q = (torch.randn(sum(counts), H, D, generator=g) * qsize).to(dtype).cuda()
+    cu = [0]
+    for c in counts:
+        cu.append(cu[-1] + c)
+    # what lies past a request's keys may be anything
+    for b, n in enumerate(lens):
+        if n % page:
+            p = table[b][n // page]
+            for c in (k, v):
+                c.view(torch.uint8)[p, :, n % page:] = 0x7f if ct == E4M3 else 0x80
+    for p in perm[at:]:
+        k.view(torch.uint8)[p] = 0x7f
+        v.view(torch.uint8)[p] = 0xff
+        vs[p] = math.nan
+        ks[p] = math.inf
+    return q, k, v, ks, vs, table, cu
+
+
+def check_attention(lens, counts, H, hkv, D, page, ct, dtype, *, seed=0, cu=True, qsize=1.0, **kw):
+    mask = kw.pop("mask", cp.CAUSAL)
+    max_q = kw.pop("max_q", None)
+    q, k, v, ks, vs, table, offs = setup(lens, counts, H, hkv, D, page, ct, dtype, seed, qsize=qsize)
+    softmax = kw.get("norm", "softmax") == "softmax"
+    got = cp.paged_attention(q, k, v, ks, vs, ints(table), ints(lens), ints(offs) if cu else None, max_q=max_q,
+                             mask=mask, return_lse=softmax, **kw)
+    got, lse = got if softmax else (got, None)
+    okw = dict(kw)
+    out, want_lse, mass = po.attention(q.cpu(), k.cpu(), v.cpu(), ks.cpu(), vs.cpu(), table, lens, offs, mask=mask, **okw)
+    err = (got.double().cpu() - out).abs()
+    tol = 2.0 ** (-8 if dtype == BF16 else -11) * out.abs() + 2.0 ** -10 * mass + 2.0 ** -23
+    assert torch.isfinite(got).all()
+    assert (err <= tol).all(), (float((err - tol).max()), float((err / tol).max()))
+    if softmax:
+        none = torch.isinf(want_lse)
+        assert torch.equal(torch.isinf(lse.cpu()), none)
+        assert ((lse.double().cpu() - want_lse).abs()[~none] <= 2.0 ** -12).all()
+    return got
+
+
+KINDS = {
+    "plain": {}, "softcap": dict(mod="softcap", softcap=20.0), "alibi": dict(mod="alibi"), "temp": dict(mod="temp"),
+    "sigmoid": dict(norm="sigmoid", sig_bias=-3.0), "relu": dict(norm="relu", out_scale=0.01),
+}
+
+
+def kind_args(kind, H):
+    kw = dict(KINDS[kind])
+    if kind == "alibi":
+        kw["head_param"] = cp.alibi_slopes_geometric(H)
+    if kind == "temp":
+        kw["head_param"] = cp.reference_temps(H)
+    return kw
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("D,dtype,ct,page", [(128, BF16, E4M3, 64), (64, F16, I8, 16), (128, F16, E4M3, 128),
+                                             (64, BF16, E4M3, 32), (128, BF16, I8, 16)])
+def test_decode(cuda, kind, D, dtype, ct, page):
+    check_attention([1, 300, 0, 64, 129, 15], [1] * 6, 8, 2, D, page, ct, dtype, cu=False, **kind_args(kind, 8))
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 7, 8, 12, 16, 24, 32, 40])
+def test_head_groups(cuda, group):
+    check_attention([77, 200], [1, 1], 2 * group, 2, 128, 64, E4M3, BF16)
+
+
+@pytest.mark.parametrize("counts", [[2, 5], [9, 33], [1, 70], [150, 1], [260, 0], [0, 3]])
+@pytest.mark.parametrize("kind", ["plain", "softcap", "sigmoid", "relu"])
+def test_several_queries(cuda, counts, kind):
+    check_attention([300, 75], counts, 8, 2, 128, 64, E4M3, BF16, **kind_args(kind, 8))
+    check_attention([300, 75], counts, 4, 4, 64, 16, I8, F16, max_q=max(counts), **kind_args(kind, 4))
+
+
+MASKS = {
+    "full": cp.FULL, "causal": cp.CAUSAL, "window": cp.Mask(left=20, right=0), "window 1": cp.Mask(left=0, right=0),
+    "local": cp.Mask(left=70, right=2), "ahead": cp.Mask(left=-1, right=3), "prefix": cp.Mask(left=10, right=0, prefix=33),
+    "block": cp.Mask(left=-1, right=0, block=48), "dilated": cp.Mask(left=-1, right=0, dilation=4),
+    "all": cp.Mask(left=100, right=1, block=96, prefix=5, dilation=3),
+}
+
+
+@pytest.mark.parametrize("name", list(MASKS))
+@pytest.mark.parametrize("counts", [[1, 1, 1], [6, 3, 17], [90, 130, 1]])
+def test_masks(cuda, name, counts):
+    lens = [max(n, c) for n, c in zip([150, 333, 40], counts)]
+    check_attention(lens, counts, 4, 2, 64, 32, E4M3, BF16, mask=MASKS[name])
+    check_attention(lens, counts, 8, 1, 128, 64, I8, F16, mask=MASKS[name], mod="alibi",
+                    head_param=cp.alibi_slopes_geometric(8))
+
+
+def test_rows_without_keys(cuda):
+    """More queries than keys, no keys, no queries, a window before the first key."""
+    got = check_attention([3, 0, 5, 0], [6, 2, 0, 1], 4, 2, 128, 16, E4M3, BF16)
+    assert not got[:3].any() and not got[6:].any()
+    check_attention([3, 40], [6, 40], 4, 2, 128, 16, E4M3, BF16, mask=cp.FULL)
+    check_attention([40, 90], [1, 2], 4, 2, 64, 16, I8, F16, mask=cp.Mask(left=5, right=0, block=7))
+
+
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 1000, 4097])
+def test_lengths(cuda, n):
+    check_attention([n], [1], 4, 1, 128, 16, E4M3, BF16)
+    check_attention([n, n + 1], [min(n, 3), 1], 8, 2, 64, 128, I8, BF16)
+
+
+def test_many_requests(cuda):
+    g = torch.Generator().manual_seed(2)
+    lens = torch.randint(0, 90, (700,), generator=g).tolist()
+    check_attention(lens, [1] * 700, 2, 1, 64, 16, E4M3, BF16)
+    check_attention([5000, 3, 0, 900] * 3, [1, 2, 1, 4] * 3, 4, 2, 128, 64, E4M3, BF16, max_q=1)
+
+
+def test_large_and_small_scales(cuda):
+    """Scales far from one another in one request; P and V stay within the range of their 16-bit forms."""
+    for ct in (E4M3, I8):
+        q, k, v, ks, vs, table, cu = setup([200, 64], [1, 2], 4, 2, 128, 16, ct, BF16)
+        live = torch.tensor([p for r, n in zip(table, (200, 64)) for p in r[:po.pages_for(n, 16)]], device="cuda")
+        vs[live] = 2.0 ** torch.randint(-60, 20, vs[live].shape, generator=torch.Generator().manual_seed(1)).float().cuda()
+        ks[live] = 2.0 ** torch.randint(-30, -6, ks[live].shape, generator=torch.Generator().manual_seed(2)).float().cuda()
+        for kw in ({}, dict(norm="relu"), dict(norm="sigmoid")):
+            got = cp.paged_attention(q, k, v, ks, vs, ints(table), ints([200, 64]), ints(cu), **kw)
+            out, _, mass = po.attention(q.cpu(), k.cpu(), v.cpu(), ks.cpu(), vs.cpu(), table, [200, 64], cu,
+                                        mask=cp.CAUSAL, **kw)
+            top = mass.amax((0, 2), keepdim=True)  # P is kept relative to the largest scale of its head's pages
+            err = (got.double().cpu() - out).abs()
+            assert (err <= 2.0 ** -8 * out.abs() + 2.0 ** -10 * mass + 2.0 ** -20 * top).all()
+
+
+def test_hidden_keys_do_not_matter(cuda):
+    """NaN and infinities, in values and scales, where the mask hides them: not a bit changes."""
+    mask = cp.Mask(left=40, right=0)
+    for counts in ([1, 1], [3, 20], [100, 150]):
+        q, k, v, ks, vs, table, cu = setup([500, 300], counts, 8, 2, 128, 16, E4M3, BF16)
+        run = lambda: cp.paged_attention(q, k, v, ks, vs, ints(table), ints([500, 300]), ints(cu), mask=mask)  # noqa: E731
+        a = run()
+        for b, n in enumerate((500, 300)):
+            first = n - counts[b] - 40  # the first key that any query sees
+            for p in range(first // 16):
+                for c in (k, v):
+                    c.view(torch.uint8)[table[b][p]] = 0x7f
+                ks[table[b][p]] = math.nan
+                vs[table[b][p]] = math.inf
+            k.view(torch.uint8)[table[b][first // 16], :, :first % 16] = 0x7f
+            v.view(torch.uint8)[table[b][first // 16], :, :first % 16] = 0xff
+        assert torch.equal(a, run())
+
+
+def test_dilated_nan(cuda):
+    q, k, v, ks, vs, table, cu = setup([130], [1], 4, 2, 64, 16, E4M3, BF16)
+    mask = cp.Mask(left=-1, right=0, dilation=5)
+    a = cp.paged_attention(q, k, v, ks, vs, ints(table), ints([130]), ints(cu), mask=mask)
+    for j in range(130):
+        if (129 - j) % 5:
+            k.view(torch.uint8)[table[0][j // 16], :, j % 16] = 0x7f
+            v.view(torch.uint8)[table[0][j // 16], :, j % 16] = 0x7f
+    assert torch.equal(a, cp.paged_attention(q, k, v, ks, vs, ints(table), ints([130]), ints(cu), mask=mask))
+
+
+def test_same_bits_again_and_by_schedule(cuda):
+    q, k, v, ks, vs, table, cu = setup([9000, 100, 2500], [1, 2, 1], 16, 2, 128, 64, E4M3, BF16)
+    args = (q, k, v, ks, vs, ints(table), ints([9000, 100, 2500]), ints(cu))
+    a = cp.paged_attention(*args)
+    for _ in range(3):
+        assert torch.equal(a, cp.paged_attention(*args))
+
+
+def test_strides_out_and_rows_nobody_owns(cuda):
+    q, k, v, ks, vs, table, cu = setup([70, 33], [2, 1], 8, 2, 128, 16, E4M3, BF16)
+    want = cp.paged_attention(q, k, v, ks, vs, ints(table), ints([70, 33]), ints(cu))
+    wide = torch.randn(5, 20, 128, dtype=BF16, device="cuda")
+    wide[:3, 4:12] = q
+    out = torch.full((5, 9, 128), 3.0, dtype=BF16, device="cuda")
+    t2 = torch.full((2, 40), -9, dtype=torch.int32, device="cuda")
+    t2[:, :len(table[0])] = ints(table)
+    got = cp.paged_attention(wide[:, 4:12], k, v, ks, vs, t2[:, :len(table[0])], ints([70, 33]), ints(cu),
+                             out=out[:, :8], max_q=2)
+    assert got.data_ptr() == out.data_ptr()
+    assert torch.equal(out[:3, :8], want) and (out[3:] == 3).all() and (out[:, 8] == 3).all()
+    # a layout that the kernels do not take is copied first
+    odd = torch.empty(3, 8, 132, dtype=BF16, device="cuda")[..., :128]
+    odd.copy_(q)
+    assert torch.equal(cp.paged_attention(odd, k, v, ks, vs, ints(table), ints([70, 33]), ints(cu)), want)
+
+
+def test_bad_pages_and_lengths_are_reported(cuda):
+    q, k, v, ks, vs, table, cu = setup([70, 33], [1, 1], 8, 2, 128, 16, E4M3, BF16)
+    good = cp.paged_attention(q, k, v, ks, vs, ints(table), ints([70, 33]), ints(cu))
+    for page in (-1, k.shape[0], 2 ** 31 - 1):
+        bad = [list(r) for r in table]
+        bad[0][2] = page
+        got = cp.paged_attention(q, k, v, ks, vs, ints(bad), ints([70, 33]), ints(cu))
+        assert torch.equal(got[1], good[1])
+        with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+            cp.check_device_status(0)
+    short = ints(table)[:, :3].contiguous()
+    for lens in ([2 ** 31 - 1, 33], [-4, 33]):
+        got = cp.paged_attention(q, k, v, ks, vs, short, ints(lens), ints(cu))
+        assert torch.equal(got[1], good[1])
+        with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+            cp.check_device_status(0)
+    for offs in ([0, 2 ** 30, 2], [0, -7, 2], [-3, 1, 2], [0, 1, 9]):
+        cp.paged_attention(q, k, v, ks, vs, ints(table), ints([70, 33]), ints(offs))
+        torch.cuda.synchronize()
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+    assert torch.equal(cp.paged_attention(q, k, v, ks, vs, ints(table), ints([70, 33]), ints(cu)), good)
+
+
+def test_other_streams_and_a_graph(cuda):
+    q, k, v, ks, vs, table, cu = setup([5000, 100], [1, 1], 8, 2, 128, 64, E4M3, BF16)
+    args = (q, k, v, ks, vs, ints(table), ints([5000, 100]), ints(cu))
+    want = cp.paged_attention(*args)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(cp.paged_attention(*args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    out = torch.empty_like(want)
+    lens, new = ints([4999, 99]), ints([1, 1])
+    ring, state, tab = ints([0, 1]), ints([0, 2]), ints(table)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step = cp.page_tables(lens, new, tab, ring, state, page_size=64, max_tokens=2)
+        cp.paged_attention(q, k, v, ks, vs, tab, step.seq_lens, step.cu_q, max_q=1, out=out)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_cache_beyond_32_bit_offsets(cuda):
+    """Pages whose bytes lie past 2^32."""
+    page, hkv, D = 128, 4, 128
+    pages = 2 ** 32 // (page * hkv * D) + 40
+    k = torch.empty(pages, hkv, page, D, dtype=torch.uint8, device="cuda").view(E4M3)
+    v = torch.empty(pages, hkv, page, D, dtype=torch.uint8, device="cuda").view(E4M3)
+    ks, vs = (torch.zeros(pages, hkv, device="cuda") for _ in range(2))
+    T = 300
+    table = [[pages - 1, 3, pages - 7]]
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(T, 2 * hkv, D, generator=g).to(BF16).cuda()
+    slots = [table[0][t // page] * page + t % page for t in range(T)]
+    cp.cache_append(x[:, :hkv], x[:, hkv:], ints(slots), k, v, ks, vs)
+    q = torch.randn(2, 8, D, generator=g).to(BF16).cuda()
+    got = cp.paged_attention(q, k, v, ks, vs, ints(table), ints([T]), ints([0, 2]))
+    rows = torch.tensor(table[0], device="cuda")
+    small = [t[rows].contiguous() for t in (k.view(torch.uint8), v.view(torch.uint8), ks, vs)]
+    want = cp.paged_attention(q, small[0].view(E4M3), small[1].view(E4M3), small[2], small[3], ints([[0, 1, 2]]),
+                              ints([T]), ints([0, 2]))
+    assert torch.equal(got, want) and want.float().abs().max() > 0.01
+
+
+def test_a_step_end_to_end(cuda):
+    """Prompts in, then tokens one by one, in 8 bits: near the same attention over what was written in 16."""
+    g = torch.Generator().manual_seed(4)
+    H, hkv, D, page, B, W = 8, 2, 128, 64, 3, 5
+    cache = cp.new_cache(16, hkv, D, page_size=page)
+    lens, table = ints([0] * B), torch.zeros(B, W, dtype=torch.int32, device="cuda")
+    ring, state = ints(list(range(15, -1, -1))), ints([5, 16])
+    hist = [([], []) for _ in range(B)]
+    for new in [[70, 1, 130], [1, 1, 1], [1, 1, 1], [5, 0, 2], [1, 1, 1]]:
+        T = sum(new)
+        q = torch.randn(T, H, D, generator=g).to(BF16).cuda()
+        k, v = (torch.randn(T, hkv, D, generator=g).to(BF16).cuda() for _ in range(2))
+        step = cp.page_tables(lens, ints(new), table, ring, state, page_size=page, max_tokens=T)
+        cp.cache_append(k, v, step.slots, *cache)
+        out = cp.paged_attention(q, *cache, table, step.seq_lens, step.cu_q, max_q=max(new))
+        lens, state = step.seq_lens, step.free_state
+        at = 0
+        for b, n in enumerate(new):
+            hist[b][0].append(k[at:at + n])
+            hist[b][1].append(v[at:at + n])
+            if n:
+                kk, vv = (torch.cat(x).transpose(0, 1)[None] for x in hist[b])
+                ref = cp.attention(q[at:at + n].transpose(0, 1)[None], kk, vv,
+                                   mask=cp.Mask(left=-1, right=kk.shape[2] - n))
+                ref = ref[0].transpose(0, 1).float()
+                rel = (out[at:at + n].float() - ref).norm() / ref.norm()
+                assert rel < 0.06, rel  # e4m3: 2^-4 relative at most, about 2.6% rms in K and in V
+            at += n
+    assert lens.tolist() == [78, 4, 135] and state.tolist()[1] == 16 - (2 + 1 + 3)
