@@ -1,18 +1,22 @@
 // paged_api.cu -- extern "C" entry points of the paged 8-bit K/V cache
 // (include/chia_paged.h): argument checks, choice of the kernel, launch. No
 // allocation, no synchronisation.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <cmath>
 #include <cstdint>
+#include <mutex>
 
 #include "../../include/chia_paged.h"
 #include "cache_sm100.cuh"
-#include "paged_attn_sm100.cuh"
+#include "paged_split_sm100.cuh"
 
 namespace {
 
 constexpr int64_t kI32 = 0x7fffffffLL;
+constexpr uint64_t kDefaultTimeoutNs = 2000000000ull;  // 2 s a wait
 
 bool aligned(const void *p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
@@ -131,6 +135,7 @@ int check_paged(const chia_paged_params_t *p) {
       p->table_width > kI32 / p->page_size || p->table_stride < p->table_width)
     return CHIA_ERR_INVALID_ARGUMENT;
   if (p->cu_q == nullptr && p->tokens % p->batch != 0) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->num_pages * p->heads_kv > kI32) return CHIA_ERR_UNSUPPORTED;
   if (p->win_left < -1 || p->win_right < -1 || p->block < 0 || p->prefix < 0 || p->dilation < 1)
     return CHIA_ERR_INVALID_ARGUMENT;
   if (p->tokens > 0 && (!p->q || !p->o)) return CHIA_ERR_INVALID_ARGUMENT;
@@ -164,15 +169,71 @@ int kind_of(const chia_paged_params_t *p) {
   }
 }
 
-template <int D, bool BF16, int CT>
-int launch_paged(const chia::PagedArgs &a, int kind, cudaStream_t s) {
-  const int64_t warps = static_cast<int64_t>(a.tokens) * a.heads;
-  if ((warps + 3) / 4 > kI32) return CHIA_ERR_UNSUPPORTED;
-  chia::paged_rows_kernel<D, BF16, CT><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, s>>>(a, kind);
-  return launched();
+// Rows of a unit: row tiles of 8 a warp, warps that share a key tile, and
+// requests' rows that a unit takes. A warp with two row tiles converts each
+// key once for 16 rows; beyond that more warps convert the same keys, which
+// costs issue slots and no HBM traffic.
+struct RowPlan {
+  int tiles, groups;
+  int rows() const { return 8 * tiles * groups; }
+};
+RowPlan row_plan(const chia_paged_params_t *p) {
+  const int64_t rows = static_cast<int64_t>(p->max_q) * (p->heads / p->heads_kv);
+  if (rows <= 8) return {1, 1};
+  if (rows <= 16) return {2, 1};
+  return rows <= 32 ? RowPlan{2, 2} : RowPlan{2, 4};
 }
 
-// Calls f.template operator()<D, BF16, CT>() for the call's types.
+// Workspace: the tickets, then the partial results of two units a CTA.
+constexpr int64_t kTicketBytes = 4096;
+struct SplitPlan {
+  RowPlan rows;
+  int grid;
+  int64_t off_ml, bytes;
+};
+int split_plan(const chia_paged_params_t *p, int sms, SplitPlan &pl) {
+  pl.rows = row_plan(p);
+  pl.grid = 2 * sms;
+  if (pl.grid * 4 > kTicketBytes) return CHIA_ERR_UNSUPPORTED;
+  const int64_t rows = 2ll * pl.grid * pl.rows.rows();
+  pl.off_ml = kTicketBytes + rows * p->head_dim * 4;
+  pl.bytes = (pl.off_ml + rows * 8 + 255) / 256 * 256;
+  return CHIA_OK;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault,
+                                         &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// A cache as (head_dim, page_size, pages * heads) bytes; a box is `rows` tokens
+// of one page and head, swizzled over their own width.
+bool encode_cache(CUtensorMap *map, const void *base, const chia_paged_params_t *p, int rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t D = p->head_dim, P = p->page_size;
+  const cuuint64_t dims[3] = {D, P, static_cast<cuuint64_t>(p->num_pages) * p->heads_kv};
+  const cuuint64_t strides[2] = {D, P * D};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(D), static_cast<cuuint32_t>(rows), 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE,
+            D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int32_t clamp30(int64_t v) { return static_cast<int32_t>(v > (1 << 30) ? (1 << 30) : v); }
+
+// FN<D, BF16, CT>(...) for the call's types.
 #define CHIA_BY_TYPE(p, FN, ...)                                                          \
   ((p)->head_dim == 128                                                                   \
        ? ((p)->dtype == CHIA_DTYPE_BF16                                                   \
@@ -232,24 +293,36 @@ int chia_cache_append(const chia_append_params_t *p, void *stream) {
 
 int64_t chia_paged_attn_workspace_bytes(const chia_paged_params_t *p) {
   if (check_paged(p) != CHIA_OK) return -1;
-  return 256;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1)
+    sms = 148;  // host-only callers (no GPU): size for a B200
+  SplitPlan pl;
+  return split_plan(p, sms, pl) == CHIA_OK ? pl.bytes : -1;
 }
 
 int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
-  int rc = check_paged(p), sms = 0;
+  int rc = check_paged(p), sms = 0, dev = 0;
   if (rc != CHIA_OK) return rc;
-  const int64_t need = chia_paged_attn_workspace_bytes(p);
-  if (p->workspace == nullptr || p->workspace_bytes < need) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->workspace == nullptr) return CHIA_ERR_INVALID_ARGUMENT;
   if (!aligned(p->workspace, 256)) return CHIA_ERR_MISALIGNED;
+  // (a workspace for no device is too small for any)
+  if (p->workspace_bytes <= kTicketBytes) return CHIA_ERR_INVALID_ARGUMENT;
   if ((rc = device_sms(sms)) != CHIA_OK) return rc;
+  if (cudaGetDevice(&dev) != cudaSuccess) return CHIA_ERR_NO_DEVICE;
+  SplitPlan pl;
+  if ((rc = split_plan(p, sms, pl)) != CHIA_OK) return rc;
+  if (p->workspace_bytes < pl.bytes) return CHIA_ERR_INVALID_ARGUMENT;
   if (p->tokens == 0) return CHIA_OK;
+  CUtensorMap mk, mv;
+  const int box = p->page_size < 32 ? p->page_size : 32;
+  if (!encode_cache(&mk, p->k_cache, p, box) || !encode_cache(&mv, p->v_cache, p, box))
+    return CHIA_ERR_LAUNCH;
   chia::PagedArgs a{};
   a.q = p->q;
   a.o = p->o;
   a.q_st = p->q_stride[0], a.q_sh = p->q_stride[1];
   a.o_st = p->o_stride[0], a.o_sh = p->o_stride[1];
-  a.k_cache = static_cast<const uint8_t *>(p->k_cache);
-  a.v_cache = static_cast<const uint8_t *>(p->v_cache);
   a.k_scale = p->k_scale;
   a.v_scale = p->v_scale;
   a.block_table = p->block_table;
@@ -258,11 +331,11 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   a.table_stride = p->table_stride;
   a.lse = p->norm == CHIA_NORM_SOFTMAX ? p->lse : nullptr;
   a.head_param = (p->mod == CHIA_MOD_ALIBI || p->mod == CHIA_MOD_TEMP) ? p->head_param : nullptr;
-  a.mask.left = p->win_left;
-  a.mask.right = p->win_right;
-  a.mask.block = p->block;
-  a.mask.prefix = p->prefix;
-  a.mask.dil = p->dilation;
+  a.left = clamp30(p->win_left);
+  a.right = clamp30(p->win_right);
+  a.block = clamp30(p->block);
+  a.prefix = clamp30(p->prefix);
+  a.dil = clamp30(p->dilation);
   a.score_scale = p->scale;
   a.softcap = p->softcap;
   a.sig_bias = p->sig_bias;
@@ -270,14 +343,40 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   a.heads = p->heads;
   a.heads_kv = p->heads_kv;
   a.group = p->heads / p->heads_kv;
-  a.batch = static_cast<int32_t>(p->batch);
   a.tokens = static_cast<int32_t>(p->tokens);
   a.page = p->page_size;
   a.width = static_cast<int32_t>(p->table_width);
-  a.num_pages = p->num_pages;
+  a.num_pages = static_cast<int32_t>(p->num_pages);
+  a.q_each = static_cast<int32_t>(p->tokens / p->batch);
+  a.row_groups = pl.rows.groups;
+  a.bf16 = p->dtype == CHIA_DTYPE_BF16;
   a.status = p->status;
+  uint8_t *ws = static_cast<uint8_t *>(p->workspace);
+  a.tickets = reinterpret_cast<int32_t *>(ws);
+  a.part_o = reinterpret_cast<float *>(ws + kTicketBytes);
+  a.part_ml = reinterpret_cast<float *>(ws + pl.off_ml);
+  a.timeout_ns = p->wait_limit_ns > 0 ? p->wait_limit_ns : kDefaultTimeoutNs;
+  a.drain_ns = kDefaultTimeoutNs;
   const int kind = kind_of(p);
-  return CHIA_BY_TYPE(p, launch_paged, a, kind, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int64_t b = 0; b < p->batch; b += chia::kSplitMaxBatch) {
+    const int64_t n = p->batch - b < chia::kSplitMaxBatch ? p->batch - b : chia::kSplitMaxBatch;
+    a.batch = static_cast<int32_t>(n);
+    a.seq_lens = p->seq_lens + b;
+    a.cu_q = p->cu_q != nullptr ? p->cu_q + b : nullptr;
+    a.token0 = static_cast<int32_t>(b * a.q_each);
+    a.block_table = p->block_table + b * p->table_stride;
+    const cudaError_t e =
+        p->head_dim == 128
+            ? (p->cache_dtype == CHIA_CACHE_E4M3
+                   ? chia::launch_split<128, chia::CACHE_E4M3>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s)
+                   : chia::launch_split<128, chia::CACHE_INT8>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s))
+            : (p->cache_dtype == CHIA_CACHE_E4M3
+                   ? chia::launch_split<64, chia::CACHE_E4M3>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s)
+                   : chia::launch_split<64, chia::CACHE_INT8>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s));
+    if (e != cudaSuccess) return CHIA_ERR_LAUNCH;
+  }
+  return CHIA_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,4 @@
+// The split kernels of head size 128 over an e4m3 cache.
+#include "paged_split_sm100.cuh"
+
+CHIA_INSTANTIATE_SPLIT(128, chia::CACHE_E4M3)
