@@ -169,35 +169,26 @@ int kind_of(const chia_paged_params_t *p) {
   }
 }
 
-// Rows of a unit: row tiles of 8 a warp, warps that share a key tile, and
-// requests' rows that a unit takes. A warp with two row tiles converts each
-// key once for 16 rows; beyond that more warps convert the same keys, which
-// costs issue slots and no HBM traffic.
-struct RowPlan {
-  int tiles, groups;
-  int rows() const { return 8 * tiles * groups; }
-};
-RowPlan row_plan(const chia_paged_params_t *p) {
-  const int64_t rows = static_cast<int64_t>(p->max_q) * (p->heads / p->heads_kv);
-  if (rows <= 8) return {1, 1};
-  if (rows <= 16) return {2, 1};
-  return rows <= 32 ? RowPlan{2, 2} : RowPlan{2, 4};
-}
-
-// Workspace: the tickets, then the partial results of two units a CTA.
+// Workspace: the tickets, then the parts of two units a CTA and of one a worker.
 constexpr int64_t kTicketBytes = 4096;
 struct SplitPlan {
-  RowPlan rows;
-  int grid;
+  int tiles;  // rows of a unit: 8 (as many as most groups of heads have) or 16
+  int grid;   // one CTA an SM
   int64_t off_ml, bytes;
 };
 int split_plan(const chia_paged_params_t *p, int sms, SplitPlan &pl) {
-  pl.rows = row_plan(p);
-  pl.grid = 2 * sms;
-  if (pl.grid * 4 > kTicketBytes) return CHIA_ERR_UNSUPPORTED;
-  const int64_t rows = 2ll * pl.grid * pl.rows.rows();
-  pl.off_ml = kTicketBytes + rows * p->head_dim * 4;
-  pl.bytes = (pl.off_ml + rows * 8 + 255) / 256 * 256;
+  const int64_t group = p->heads / p->heads_kv;
+  pl.tiles = p->max_q * group <= 8 ? 1 : 2;
+  pl.grid = sms;
+  // the line of tiles is counted in 32 bits
+  const int64_t rows = 8 * pl.tiles;
+  const double line = static_cast<double>(p->heads_kv) * (p->tokens * group / rows + p->batch + 1) *
+                      (p->table_width * p->page_size / 32 + 2);
+  if (pl.grid * 4 > kTicketBytes || p->tokens * p->heads > kI32 || line > kI32)
+    return CHIA_ERR_UNSUPPORTED;
+  const int64_t slots = (2 + chia::kSplitWarps) * pl.grid * rows;
+  pl.off_ml = kTicketBytes + slots * p->head_dim * 4;
+  pl.bytes = (pl.off_ml + slots * 8 + 255) / 256 * 256;
   return CHIA_OK;
 }
 
@@ -348,7 +339,6 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   a.width = static_cast<int32_t>(p->table_width);
   a.num_pages = static_cast<int32_t>(p->num_pages);
   a.q_each = static_cast<int32_t>(p->tokens / p->batch);
-  a.row_groups = pl.rows.groups;
   a.bf16 = p->dtype == CHIA_DTYPE_BF16;
   a.status = p->status;
   uint8_t *ws = static_cast<uint8_t *>(p->workspace);
@@ -369,11 +359,11 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
     const cudaError_t e =
         p->head_dim == 128
             ? (p->cache_dtype == CHIA_CACHE_E4M3
-                   ? chia::launch_split<128, chia::CACHE_E4M3>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s)
-                   : chia::launch_split<128, chia::CACHE_INT8>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s))
+                   ? chia::launch_split<128, chia::CACHE_E4M3>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s)
+                   : chia::launch_split<128, chia::CACHE_INT8>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s))
             : (p->cache_dtype == CHIA_CACHE_E4M3
-                   ? chia::launch_split<64, chia::CACHE_E4M3>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s)
-                   : chia::launch_split<64, chia::CACHE_INT8>(mk, mv, a, kind, pl.rows.tiles, pl.grid, dev, s));
+                   ? chia::launch_split<64, chia::CACHE_E4M3>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s)
+                   : chia::launch_split<64, chia::CACHE_INT8>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s));
     if (e != cudaSuccess) return CHIA_ERR_LAUNCH;
   }
   return CHIA_OK;

@@ -2,18 +2,17 @@
 // cache: decode steps and drafted tokens.
 //
 // Every key and value byte is read once and used by group * queries rows, so
-// the work is bound by HBM as long as nothing else is in its way. The grid is
-// one wave of CTAs; all (request, K/V head, block of rows) units with their
-// 32-key tiles form one line of tiles, of which each CTA takes an equal piece,
-// whatever the lengths. A unit that is cut by CTAs' borders leaves partial
-// results, and the last CTA to finish merges them in a fixed order.
-//
-// A CTA: four compute warps and one that loads. The load warp looks up 32
-// tiles' pages and scales at a time, a tile a lane, and keeps a ring of tiles
-// in flight by TMA (tiled copies with a swizzle that keeps the reads below free
-// of bank conflicts). A tile is consumed by one compute warp alone (or by one
-// warp of each row group), with its own running maximum, sum and output: no
-// barrier between warps until the unit ends.
+// the work is bound by HBM as long as nothing else is in its way. All (request,
+// K/V head, block of up to 16 rows) units with their 32-key tiles form one line
+// of tiles. A worker is a warp: one CTA of eight an SM, and each takes an equal
+// piece of the line whatever the lengths, a unit counting as kUnitCost tiles
+// more than it has (its queries, its output). A worker has a ring of its own,
+// which its lane 0 fills by TMA (tiled copies with a swizzle that keeps the
+// reads below free of bank conflicts), after it looked up 32 tiles' pages and
+// scales at a time, a tile a lane. So no warp waits for another until all of a
+// CTA's are done. A unit within one worker's piece goes straight to the output;
+// units that are cut leave parts, which the CTA merges in shared memory, and the
+// last CTA of a unit merges the CTAs' parts, always in the order of the line.
 //
 // A tile is computed transposed, keys and channels on the 16-row side of
 // m16n8k16 and query rows on the 8-column side, so that a group of up to eight
@@ -55,17 +54,18 @@ struct PagedArgs {
   int32_t num_pages;
   int32_t q_each;     // queries of a request where cu_q is null
   int32_t token0;     // first token of request 0 where cu_q is null
-  int32_t row_groups; // 1, 2 or 4: compute warps that share a tile
   int32_t bf16;       // type of q and o
   int32_t *tickets;   // [gridDim.x], zero between launches
-  float *part_o;      // [2 gridDim.x][rows][D]
-  float *part_ml;     // [2 gridDim.x][rows][2]
+  float *part_o;      // [10 gridDim.x][rows][D]: two parts a CTA, then one a worker
+  float *part_ml;     // [10 gridDim.x][rows][2]
   int32_t *status;
   uint64_t timeout_ns, drain_ns;
 };
 
 constexpr int kSplitMaxBatch = 1024;  // requests of one launch (prefix sums in shared memory)
-constexpr int kSplitThreads = 160;
+constexpr int kSplitWarps = 8;
+constexpr int kSplitThreads = 32 * kSplitWarps;
+constexpr int kUnitCost = 4;  // what a unit costs beside its tiles, in tiles
 
 // Queries and keys of request b, checked: [t0, t0 + n) of q, keys [0, len).
 struct Request {
@@ -149,10 +149,6 @@ __device__ __forceinline__ bool split_wait(uint32_t bar, uint32_t parity, volati
   return true;
 }
 
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar,
                                             int c0, int c1, int c2) {
   asm volatile(
@@ -167,237 +163,266 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <int D, int NT>
 struct SplitConfig {
-  static constexpr int TK = 32;                     // keys of a tile
-  static constexpr int STAGE = 2 * TK * D;          // bytes: K, then V
-  static constexpr int NST = (NT == 1 ? 10 : 8) * (128 / D);  // 80 or 64 KB of tiles
-  static constexpr int ROWS = 8 * NT;               // rows of a row group
-  static constexpr int PITCH = D + 4;               // floats of a row in the merge buffer
-  static constexpr int MERGE = 4 * ROWS * (PITCH + 2) * 4;
-  static constexpr int SCALES = 64;                 // tiles whose scales are held
-  static constexpr int SMEM = 1024 + NST * STAGE + MERGE + SCALES * 16;
+  static constexpr int TK = 32;                   // keys of a tile
+  static constexpr int STAGE = 2 * TK * D;        // bytes: K, then V
+  static constexpr int NST = 3 * (128 / D);       // stages of a worker: 24 KB of tiles
+  static constexpr int ROWS = 8 * NT;             // rows of a unit
+  static constexpr int PITCH = D + 4;             // floats of a row in the merge buffer
+  static constexpr int SCALES = 64;               // tiles whose scales a worker holds
+  static constexpr int RING = kSplitWarps * NST * STAGE;
+  static constexpr int SMEM = 1024 + RING + kSplitWarps * SCALES * 16;
+  static_assert(kSplitWarps * ROWS * PITCH * 4 <= RING, "the parts fit the spent ring");
 };
 
-// Grid: at most two CTAs an SM. KIND: score modification and normaliser.
+// A unit: rows [row0, row0 + rows) of a request's queries with one K/V head.
+struct Unit {
+  int t0, row0, rows, hk;  // first token of the request
+  long long cost;          // where it begins in the line, in cost
+  int n;                   // its tiles
+};
+
+// A row's four channels, normalised, to the output; the first also writes the log-sum-exp.
+template <int KIND>
+__device__ __forceinline__ void split_store(const PagedArgs &a, const Unit &u, int r, int c, float x0,
+                                            float x1, float x2, float x3, float M, float L) {
+  constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
+  float f = 1.f;
+  if (SOFTMAX) f = L > 0.f ? 1.f / L : L;  // (a NaN stays)
+  if (KIND == KIND_RELU) f = a.out_scale * ptx::ex2(M);
+  const int hh = u.hk * a.group + (u.row0 + r) % a.group;
+  const int64_t tok = u.t0 + (u.row0 + r) / a.group;
+  uint16_t *dst = static_cast<uint16_t *>(a.o) + tok * a.o_st + hh * a.o_sh + c;
+  x0 *= f, x1 *= f, x2 *= f, x3 *= f;
+  *reinterpret_cast<uint2 *>(dst) =
+      a.bf16 ? make_uint2(ptx::pack_bf16(x0, x1), ptx::pack_bf16(x2, x3))
+             : make_uint2(ptx::pack_f16(x0, x1), ptx::pack_f16(x2, x3));
+  if (SOFTMAX && a.lse != nullptr && c == 0)
+    a.lse[tok * a.heads + hh] =
+        L > 0.f ? (M + __log2f(L)) * 0.6931471805599453f : L == 0.f ? -INFINITY : L;
+}
+
+// KIND: score modification and normaliser.
 template <int D, int CT, int NT, int KIND>
-__global__ void __launch_bounds__(kSplitThreads, 2)
+__global__ void __launch_bounds__(kSplitThreads, 1)
 paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const PagedArgs a) {
   using C = SplitConfig<D, NT>;
   constexpr int TK = C::TK, NST = C::NST, ROWS = C::ROWS, PITCH = C::PITCH;
   constexpr int H = D / 64;   // 16-byte pieces of a key row a lane
   constexpr int MT = D / 16;  // channel tiles of the output
-  constexpr bool SOFTMAX = KIND == KIND_SOFTMAX || KIND == KIND_SOFTCAP || KIND == KIND_ALIBI;
-  constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+  constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
+  constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ uint8_t dyn[];
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
-  float *mo = reinterpret_cast<float *>(sm + NST * C::STAGE);  // [4][ROWS][PITCH]
-  float *mml = mo + 4 * ROWS * PITCH;                          // [4][ROWS][2]
-  float4 *scales = reinterpret_cast<float4 *>(mml + 4 * ROWS * 2);  // ks, vs of keys 0-15, 16-31
-  __shared__ long long pre[kSplitMaxBatch + 1];
-  __shared__ long long wsum[5];
-  __shared__ __align__(8) uint64_t bars[2 * NST];
+  float *parts = reinterpret_cast<float *>(sm);  // [warps][ROWS][PITCH], in the spent ring
+  __shared__ int tiles_pre[kSplitMaxBatch + 1], units_pre[kSplitMaxBatch + 1];
+  __shared__ int wsum[kSplitWarps][2];
+  __shared__ __align__(8) uint64_t bars[kSplitWarps * NST];
+  __shared__ float part_ml[kSplitWarps][ROWS][2];
+  __shared__ Unit s_head[kSplitWarps], s_end[kSplitWarps];
+  __shared__ int s_has_head[kSplitWarps], s_has_end[kSplitWarps];  // end: 1 begun here, 2 before
   __shared__ volatile int abort_flag;
-  __shared__ int s_last;
+  // A unit's parts in this CTA: what workers first..last have of it. `before`,
+  // `after`: it began in an earlier CTA, goes on in a later one.
+  struct Group {
+    int first, last;
+    bool before, after, last_is_head;
+  };
+  __shared__ Group s_group[kSplitWarps + 1];
+  __shared__ int s_groups, s_last[2];
 
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int RG = a.row_groups, KW = 4 / RG, RPB = ROWS * RG;
-  const uint32_t ring = ptx::smem_u32(sm), bar0 = ptx::smem_u32(bars);
-  auto full = [&](int s) { return bar0 + 8 * s; };
-  auto empty = [&](int s) { return bar0 + 8 * (NST + s); };
-  if (t < NST) {
-    ptx::mbar_init(full(t), 1);
-    ptx::mbar_init(empty(t), RG);
-  }
-  if (t == 0) abort_flag = 0;
-  if (t == 128) {
+  const int gid = lane >> 2, tig = lane & 3;
+  const uint32_t bar0 = ptx::smem_u32(bars) + warp * NST * 8;
+  const uint32_t ring = ptx::smem_u32(sm) + warp * NST * C::STAGE;
+  float4 *scales = reinterpret_cast<float4 *>(sm + C::RING) + warp * C::SCALES;  // ks, vs of
+                                                                                 // keys 0-15, 16-31
+  if (t < kSplitWarps * NST) ptx::mbar_init(ptx::smem_u32(bars) + 8 * t, 1);
+  if (t == 0) {
+    abort_flag = 0;
     ptx::tma_prefetch_desc(&mk);
     ptx::tma_prefetch_desc(&mv);
   }
 
-  // ---- the line of tiles: pre[b] is where request b's begin
+  // ---- the line: tiles and units before each request
   {
     const int per = (a.batch + kSplitThreads - 1) / kSplitThreads;
     const int b0 = t * per, b1 = min(a.batch, b0 + per);
-    long long sum = 0;
+    int nt = 0, nu = 0;
     bool bad = false;
     for (int b = b0; b < b1; ++b) {
       const Request r = request_of(a, b, bad);
-      long long n = 0;
-      if (r.n > 0)
-        n = static_cast<long long>(tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len).n) * a.heads_kv *
-            ((static_cast<long long>(r.n) * a.group + RPB - 1) / RPB);
-      pre[b + 1] = n;
-      sum += n;
+      int n = 0, u = 0;
+      if (r.n > 0) {
+        u = (r.n * a.group + ROWS - 1) / ROWS * a.heads_kv;
+        n = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len).n * u;
+      }
+      tiles_pre[b + 1] = n;
+      units_pre[b + 1] = u;
+      nt += n;
+      nu += u;
     }
     if (bad && blockIdx.x == 0) report(a.status, kStatusBadIndex);
-    long long inc = sum;
+    int it = nt, iu = nu;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += u;
+      const int x = __shfl_up_sync(0xffffffffu, it, d), y = __shfl_up_sync(0xffffffffu, iu, d);
+      if (lane >= d) it += x, iu += y;
     }
-    if (lane == 31) wsum[warp] = inc;
+    if (lane == 31) wsum[warp][0] = it, wsum[warp][1] = iu;
     ptx::fence_barrier_init();
     __syncthreads();
-    long long at = inc - sum;
-    for (int w = 0; w < warp; ++w) at += wsum[w];
+    it -= nt, iu -= nu;
+    for (int w = 0; w < warp; ++w) it += wsum[w][0], iu += wsum[w][1];
     for (int b = b0; b < b1; ++b) {
-      at += pre[b + 1];
-      pre[b + 1] = at;
+      it += tiles_pre[b + 1], iu += units_pre[b + 1];
+      tiles_pre[b + 1] = it, units_pre[b + 1] = iu;
     }
-    if (t == 0) pre[0] = 0;
+    if (t == 0) tiles_pre[0] = units_pre[0] = 0;
     __syncthreads();
   }
-  const long long total = pre[a.batch];
-  // no more CTAs than give each compute warp a tile
-  long long ctas = (total + KW - 1) / KW;
+  auto cost_before = [&](int b) {
+    return tiles_pre[b] + static_cast<long long>(kUnitCost) * units_pre[b];
+  };
+  const long long total = cost_before(a.batch);
+  long long ctas = (total + kSplitWarps - 1) / kSplitWarps;
   if (ctas > gridDim.x) ctas = gridDim.x;
   if (blockIdx.x >= ctas) return;
-  const long long c0 = total * blockIdx.x / ctas, c1 = total * (blockIdx.x + 1) / ctas;
-  auto request_at = [&](long long g) {  // the request of tile g
+  const long long workers = ctas * kSplitWarps;
+  // Worker w begins at cost total * w / workers. A border within the cost of a
+  // unit's own counts as its first tile.
+  auto tile_at = [&](long long w) {
+    const long long x = total * w / workers;
+    if (x >= total) return tiles_pre[a.batch];
     int lo = 0, hi = a.batch;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (pre[mid] <= g)
+      if (cost_before(mid) <= x)
         lo = mid;
       else
         hi = mid;
     }
-    return lo;
+    const int units = units_pre[lo + 1] - units_pre[lo];
+    const int n = (tiles_pre[lo + 1] - tiles_pre[lo]) / units;
+    const int in = static_cast<int>(x - cost_before(lo));
+    const int u = in / (n + kUnitCost);
+    return tiles_pre[lo] + u * n + max(0, in - u * (n + kUnitCost) - kUnitCost);
   };
+  // the CTA that has tile k of a unit
+  auto cta_of = [&](const Unit &u, int k) {
+    return static_cast<int>(((u.cost + kUnitCost + k + 1) * workers - 1) / total / kSplitWarps);
+  };
+  const int me = blockIdx.x * kSplitWarps + warp;
+  const int c0 = tile_at(me), c1 = tile_at(me + 1);
+  const int nk = c1 - c0;  // tiles of this worker
+  if (lane == 0) s_has_head[warp] = s_has_end[warp] = 0;
+  auto head_o = [&](int w) { return a.part_o + (2ll * gridDim.x + w) * ROWS * D; };
+  auto head_ml = [&](int w) { return a.part_ml + (2ll * gridDim.x + w) * ROWS * 2; };
+  auto rings_spent = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
 
-  if (warp == 4) {
-    // ================================================= the load warp
-    long long seq = 0;  // tiles issued
-    bool ok = true;
-    for (long long base = c0; base < c1 && ok; base += 32) {
-      const int n = static_cast<int>(min(32ll, c1 - base));
-      int row0 = -1, row1 = -1, tok = 0;  // rows of the tensor map (page * heads_kv + head)
-      float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (lane < n) {
-        const long long g = base + lane;
-        const int b = request_at(g);
-        bool bad = false;
-        const Request r = request_of(a, b, bad);
-        const Tiles tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
-        const long long in = g - pre[b];
-        const int nrb = (r.n * a.group + RPB - 1) / RPB;
-        const int hk = static_cast<int>(in / tl.n) / nrb;
-        const int key = tl.key_tile(static_cast<int>(in % tl.n)) * TK;
-        const int32_t *table = a.block_table + b * a.table_stride;
-        tok = key % a.page;
-        int p0 = -1, p1 = -1;
-        if (key < r.len) p0 = table[key / a.page];
-        if (a.page == 16 && key + 16 < r.len) p1 = table[key / 16 + 1];
-        if (key < r.len) {
-          if (p0 < 0 || p0 >= a.num_pages)
-            bad = true, p0 = -1;
-          else
-            row0 = p0 * a.heads_kv + hk;
-        }
-        if (a.page == 16 && key + 16 < r.len) {
-          if (p1 < 0 || p1 >= a.num_pages)
-            bad = true, p1 = -1;
-          else
-            row1 = p1 * a.heads_kv + hk;
-        }
-        if (bad) report(a.status, kStatusBadIndex);
+  // ---- loads
+  int row0 = -1, row1 = -1, tok = 0;  // of tile 32 * (issued / 32) + lane: rows of the tensor map
+  auto look_up = [&](int k) {         // (page * heads_kv + head), first token; the scales go to
+    row0 = row1 = -1;                 // shared memory
+    float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (k + lane < nk) {
+      const int g = c0 + k + lane;
+      const int b = last_not_above(tiles_pre, a.batch, g);
+      bool bad = false;
+      const Request r = request_of(a, b, bad);
+      const Tiles tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
+      const int nrb = (r.n * a.group + ROWS - 1) / ROWS;
+      const int in = g - tiles_pre[b], u = in / tl.n;
+      const int hk = u / nrb, key = tl.key_tile(in - u * tl.n) * TK;
+      const int32_t *table = a.block_table + b * a.table_stride;
+      tok = key % a.page;
+      if (key < r.len) {
+        const int pg = table[key / a.page];
+        if (pg < 0 || pg >= a.num_pages)
+          bad = true;
+        else
+          row0 = pg * a.heads_kv + hk;
       }
-      auto issue = [&](int i) {  // wait for the stage, start its copies
-        const int stage = static_cast<int>((seq + i) % NST);
-        const uint32_t par = static_cast<uint32_t>((seq + i) / NST) & 1u;
-        if (!split_wait(empty(stage), par ^ 1u, &abort_flag, a)) return false;
-        const int r0 = __shfl_sync(0xffffffffu, row0, i), r1 = __shfl_sync(0xffffffffu, row1, i);
-        const int tk = __shfl_sync(0xffffffffu, tok, i);
-        if (lane == 0) {
-          const uint32_t dst = ring + stage * C::STAGE;
-          const int rows = a.page == 16 ? 16 : TK;
-          mbar_expect_tx(full(stage), ((r0 >= 0) + (r1 >= 0)) * 2 * rows * D);
-          if (r0 >= 0) {
-            tma_load_3d(dst, &mk, full(stage), 0, tk, r0);
-            tma_load_3d(dst + TK * D, &mv, full(stage), 0, tk, r0);
-          }
-          if (r1 >= 0) {
-            tma_load_3d(dst + 16 * D, &mk, full(stage), 0, 0, r1);
-            tma_load_3d(dst + TK * D + 16 * D, &mv, full(stage), 0, 0, r1);
-          }
-        }
-        return true;
-      };
-      // the first copies leave before the scales are here
-      const int early = min(n, NST);
-      int done = 0;
-      for (; done < early && ok; ++done) ok = issue(done);
+      if (a.page == 16 && key + 16 < r.len) {
+        const int pg = table[key / 16 + 1];
+        if (pg < 0 || pg >= a.num_pages)
+          bad = true;
+        else
+          row1 = pg * a.heads_kv + hk;
+      }
+      if (bad) report(a.status, kStatusBadIndex);
       if (row0 >= 0) sc.x = a.k_scale[row0], sc.y = a.v_scale[row0];
       if (a.page != 16)
         sc.z = sc.x, sc.w = sc.y;
       else if (row1 >= 0)
         sc.z = a.k_scale[row1], sc.w = a.v_scale[row1];
-      scales[(seq + lane) % C::SCALES] = sc;
-      __syncwarp();
-      if (!ok) --done;
-      if (lane == 0)
-        for (int i = 0; i < done; ++i) ptx::mbar_arrive(full((seq + i) % NST));
-      for (int i = early; i < n && ok; ++i) {
-        ok = issue(i);
-        if (ok) {
-          if (lane == 0) ptx::mbar_arrive(full((seq + i) % NST));
-          ++done;
-        }
-      }
-      seq += done;
     }
-    // no copy of this CTA is in flight when it exits
-    PagedArgs d = a;
-    d.timeout_ns = a.drain_ns;
-    int none = 0;
-    for (long long i = seq > NST ? seq - NST : 0; i < seq; ++i)
-      split_wait(full(i % NST), static_cast<uint32_t>(i / NST) & 1u, &none, d);
-    return;
-  }
+    scales[(k + lane) % C::SCALES] = sc;  // (those of 64 tiles ago are long used)
+    __syncwarp();
+  };
+  auto issue = [&](int k) {  // start the copies of tile k, whose stage is free
+    if (k >= nk) return;
+    if (k % 32 == 0) look_up(k);
+    const int r0 = __shfl_sync(0xffffffffu, row0, k % 32);
+    const int r1 = __shfl_sync(0xffffffffu, row1, k % 32);
+    const int tk = __shfl_sync(0xffffffffu, tok, k % 32);
+    if (lane == 0) {
+      const uint32_t dst = ring + (k % NST) * C::STAGE, bar = bar0 + 8 * (k % NST);
+      const int rows = a.page == 16 ? 16 : TK;
+      ptx::mbar_arrive_expect_tx(bar, ((r0 >= 0) + (r1 >= 0)) * 2 * rows * D);
+      if (r0 >= 0) {
+        tma_load_3d(dst, &mk, bar, 0, tk, r0);
+        tma_load_3d(dst + TK * D, &mv, bar, 0, tk, r0);
+      }
+      if (r1 >= 0) {
+        tma_load_3d(dst + 16 * D, &mk, bar, 0, 0, r1);
+        tma_load_3d(dst + TK * D + 16 * D, &mv, bar, 0, 0, r1);
+      }
+    }
+  };
+  for (int k = 0; k < NST; ++k) issue(k);
 
-  // =================================================== compute warps
-  const int gid = lane >> 2, tig = lane & 3;
-  const int rg = warp % RG, kw = warp / RG;
-  long long seq = 0;
-  for (long long g = c0; g < c1;) {
-    const int b = request_at(g);
+  // ---- units of the piece
+  bool aborted = false, has_end = false;
+  for (int k = 0; k < nk;) {
+    const int g = c0 + k;
+    const int b = last_not_above(tiles_pre, a.batch, g);
     bool bad = false;
     const Request rq = request_of(a, b, bad);
     const int p0 = rq.len - rq.n;
     const Tiles tl = tiles_of<TK>(a, p0, rq.len - 1, rq.len);
-    const long long in = g - pre[b];
-    const int nrows_all = rq.n * a.group;
-    const int nrb = (nrows_all + RPB - 1) / RPB;
-    const int ut0 = static_cast<int>(in % tl.n), u = static_cast<int>(in / tl.n);
-    const int hk = u / nrb, rb = u % nrb;
-    const long long ustart = g - ut0, uend = ustart + tl.n;
-    const int nt = static_cast<int>(min(uend, c1) - g);
-    const int row_base = rb * RPB;                       // rows of this unit: [row_base, row_end)
-    const int row_end = min(nrows_all, row_base + RPB);
+    const int nrows_all = rq.n * a.group, nrb = (nrows_all + ROWS - 1) / ROWS;
+    const int in = g - tiles_pre[b], u = in / tl.n, ut0 = in - u * tl.n;
+    const int nt = min(tl.n - ut0, nk - k);
+    Unit un;
+    un.t0 = rq.t0;
+    un.row0 = (u % nrb) * ROWS;
+    un.rows = min(ROWS, nrows_all - un.row0);
+    un.hk = u / nrb;
+    un.cost = cost_before(b) + static_cast<long long>(u) * (tl.n + kUnitCost);
+    un.n = tl.n;
     // all rows of the unit see keys [lo_max, hi_min]; none sees one outside [lo_min, hi_max]
     int lo_min, lo_max, hi_min, hi_max;
-    band32(a, p0 + row_base / a.group, rq.len, lo_min, hi_min);
-    band32(a, p0 + (row_end - 1) / a.group, rq.len, lo_max, hi_max);
+    band32(a, p0 + un.row0 / a.group, rq.len, lo_min, hi_min);
+    band32(a, p0 + (un.row0 + un.rows - 1) / a.group, rq.len, lo_max, hi_max);
     const int pf = min(a.prefix, rq.len);
 
-    // ---- Q: row rg * ROWS + 8 n + gid, channels 16 (H tig + h) + 4 s .. + 3 of step (h, s)
+    // ---- Q: row 8 n + gid, channels 16 (H tig + h) + 4 s .. + 3 of step (h, s)
     uint32_t qf[NT][H * 4][2];
     float rowmul[NT][2], slope[NT][2];  // rows 8 n + 2 tig + e, as in the columns of S^T
     int posn[NT][2];
     uint32_t real = 0;  // bit 2 n + e: that row exists
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int row = row_base + rg * ROWS + 8 * n + gid;
+      const int rr = 8 * n + gid, row = un.row0 + rr;
       uint4 raw[H * 2];
-      if (row < row_end) {
+      if (rr < un.rows) {
         const uint16_t *src = static_cast<const uint16_t *>(a.q) +
                               static_cast<int64_t>(rq.t0 + row / a.group) * a.q_st +
-                              (hk * a.group + row % a.group) * a.q_sh + H * 16 * tig;
+                              (un.hk * a.group + row % a.group) * a.q_sh + H * 16 * tig;
 #pragma unroll
         for (int c = 0; c < H * 2; ++c) raw[c] = *reinterpret_cast<const uint4 *>(src + 8 * c);
       } else {
@@ -427,15 +452,14 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         get(w, x);
         qf[n][w / 2][w % 2] = ptx::pack_f16(x.x * up, x.y * up);
       }
-      const int src_row = row_base + rg * ROWS + 8 * n + 2 * tig;
       const float down = pow2f(e - 14);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float f = __shfl_sync(0xffffffffu, down, (2 * tig + x) * 4);
-        const int r = min(src_row + x, row_end - 1);
-        const float hp = a.head_param != nullptr ? a.head_param[hk * a.group + r % a.group] : 1.f;
+        const int r = min(8 * n + 2 * tig + x, un.rows - 1) + un.row0;
+        const float hp = a.head_param != nullptr ? a.head_param[un.hk * a.group + r % a.group] : 1.f;
         posn[n][x] = p0 + r / a.group;
-        real |= (src_row + x < row_end ? 1u : 0u) << (2 * n + x);
+        real |= (8 * n + 2 * tig + x < un.rows ? 1u : 0u) << (2 * n + x);
         float mul = a.score_scale * f;
         slope[n][x] = 0.f;
         if (KIND == KIND_SOFTMAX) mul *= LOG2E * hp;
@@ -454,13 +478,21 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       l_run[n][0] = l_run[n][1] = 0.f;
     }
 
-    for (int i = (kw - static_cast<int>(seq % KW) + KW) % KW; i < nt; i += KW) {
-      const int stage = static_cast<int>((seq + i) % NST);
-      const uint32_t par = static_cast<uint32_t>((seq + i) / NST) & 1u;
-      if (!split_wait(full(stage), par, &abort_flag, a)) break;
+    for (int i = 0; i < nt && !aborted; ++i) {
+      const int kk = k + i, stage = kk % NST;
+      if (!split_wait(bar0 + 8 * stage, (kk / NST) & 1, &abort_flag, a)) {
+        // leave no copy in flight: the ring's memory is used again, and the CTA may exit
+        PagedArgs d = a;
+        d.timeout_ns = a.drain_ns;
+        int none = 0;
+        for (int j = kk; j < min(nk, kk + NST); ++j)
+          split_wait(bar0 + 8 * (j % NST), (j / NST) & 1, &none, d);
+        aborted = true;
+        break;
+      }
       __syncwarp();
       const int j0 = tl.key_tile(ut0 + i) * TK;
-      float4 sc = scales[(seq + i) % C::SCALES];
+      float4 sc = scales[kk % C::SCALES];
       const uint32_t kst = ring + stage * C::STAGE, vst = kst + TK * D;
       const bool all = a.dil == 1 ? (j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf
                                   : j0 + TK <= pf;
@@ -691,108 +723,171 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(empty(stage));
+      __syncwarp();  // all lanes are done with the stage
+      issue(kk + NST);
     }
-    seq += nt;
+    k += nt;
 
-    // ---------------- merge the key warps
+    // ---------------- the unit's result, or this worker's part of it
+    const bool begun = ut0 == 0, ended = ut0 + nt == tl.n;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float l = l_run[n][e];
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-        const int r = 8 * n + 2 * tig + e;
-        float *dst = mo + (warp * ROWS + r) * PITCH + 2 * gid;
+        for (int d = 4; d < 32; d <<= 1)
+          l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], d);
+    if (begun && ended) {
 #pragma unroll
-        for (int c = 0; c < MT; ++c)
-          *reinterpret_cast<float2 *>(dst + 16 * c) =
-              make_float2(o[c][n][e] * vref, o[c][n][2 + e] * vref);
-        if (gid == 0) {
-          mml[(warp * ROWS + r) * 2] = m_run[n][e];
-          mml[(warp * ROWS + r) * 2 + 1] = l;
-        }
-      }
-    bar_compute();
-    const bool whole = ustart >= c0 && uend <= c1;
-    const int64_t slot = 2ll * blockIdx.x + (ustart < c0 ? 0 : 1);
-    const int rows = row_end - row_base;
-    auto store = [&](int r, int c4, float4 acc, float M, float L) {  // a row's four channels
-      float f = 1.f;
-      if (SOFTMAX) f = L > 0.f ? 1.f / L : L;  // (a NaN stays)
-      if (KIND == KIND_RELU) f = a.out_scale * ptx::ex2(M);
-      const int qi = (row_base + r) / a.group, hh = hk * a.group + (row_base + r) % a.group;
-      const int64_t tok = rq.t0 + qi;
-      uint16_t *dst = static_cast<uint16_t *>(a.o) + tok * a.o_st + hh * a.o_sh + 4 * c4;
-      acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-      *reinterpret_cast<uint2 *>(dst) =
-          a.bf16 ? make_uint2(ptx::pack_bf16(acc.x, acc.y), ptx::pack_bf16(acc.z, acc.w))
-                 : make_uint2(ptx::pack_f16(acc.x, acc.y), ptx::pack_f16(acc.z, acc.w));
-      if (SOFTMAX && a.lse != nullptr && c4 == 0)
-        a.lse[tok * a.heads + hh] = L > 0.f ? (M + __log2f(L)) * LN2 : L == 0.f ? -INFINITY : L;
-    };
-    for (int e = t; e < rows * (D / 4); e += 128) {
-      const int r = e / (D / 4), c4 = e % (D / 4);
-      const int w0 = r / ROWS, rr = r % ROWS;  // warps w0, w0 + RG, ...
-      float M = -INFINITY, L = 0.f;
-      for (int k = 0; k < KW; ++k) M = fmaxf(M, mml[((w0 + k * RG) * ROWS + rr) * 2]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = 0; k < KW; ++k) {
-        const int w = (w0 + k * RG) * ROWS + rr;
-        const float wt = ptx::ex2(mml[w * 2] - (M == -INFINITY ? 0.f : M));
-        const float4 x = *reinterpret_cast<const float4 *>(mo + w * PITCH + 4 * c4);
-        L = fmaf(wt, mml[w * 2 + 1], L);
-        acc.x = fmaf(wt, x.x, acc.x);
-        acc.y = fmaf(wt, x.y, acc.y);
-        acc.z = fmaf(wt, x.z, acc.z);
-        acc.w = fmaf(wt, x.w, acc.w);
-      }
-      if (whole) {
-        store(r, c4, acc, M, L);
-      } else {
-        *reinterpret_cast<float4 *>(a.part_o + (slot * RPB + r) * D + 4 * c4) = acc;
-        if (c4 == 0)
-          *reinterpret_cast<float2 *>(a.part_ml + (slot * RPB + r) * 2) = make_float2(M, L);
-      }
-    }
-    if (!whole) {
-      // ---------------- the last of the unit's CTAs merges its parts, in their order
-      auto cta_of = [&](long long x) { return static_cast<int>(((x + 1) * ctas - 1) / total); };
-      const int first = cta_of(ustart), last = cta_of(uend - 1);
-      __threadfence();
-      bar_compute();
-      if (t == 0)  // counts up to the number of parts and wraps to zero
-        s_last = atomicInc(reinterpret_cast<unsigned *>(a.tickets) + first,
-                           static_cast<unsigned>(last - first)) ==
-                 static_cast<unsigned>(last - first);
-      bar_compute();
-      if (s_last) {
-        __threadfence();
-        for (int e = t; e < rows * (D / 4); e += 128) {
-          const int r = e / (D / 4), c4 = e % (D / 4);
-          auto part = [&](int c) { return (2ll * c + (c == first ? 1 : 0)) * RPB + r; };
-          float M = -INFINITY, L = 0.f;
-          for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(a.part_ml + part(c) * 2));
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int c = first; c <= last; ++c) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part(c) * 2));
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part(c) * D + 4 * c4));
-            const float wt = ptx::ex2(ml.x - (M == -INFINITY ? 0.f : M));
-            L = fmaf(wt, ml.y, L);
-            acc.x = fmaf(wt, x.x, acc.x);
-            acc.y = fmaf(wt, x.y, acc.y);
-            acc.z = fmaf(wt, x.z, acc.z);
-            acc.w = fmaf(wt, x.w, acc.w);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 8 * n + 2 * tig + e;
+#pragma unroll
+          for (int c = 0; c < MT; ++c) {
+            // lanes of even and odd gid exchange, so that each has four channels of a row
+            const float x0 = o[c][n][e] * vref, x1 = o[c][n][2 + e] * vref;
+            const float y0 = __shfl_xor_sync(0xffffffffu, x0, 4), y1 = __shfl_xor_sync(0xffffffffu, x1, 4);
+            if (((gid ^ c) & 1) == 0 && r < un.rows) {
+              if (gid & 1)
+                split_store<KIND>(a, un, r, 16 * c + 2 * (gid - 1), y0, y1, x0, x1, m_run[n][e],
+                                  l_run[n][e]);
+              else
+                split_store<KIND>(a, un, r, 16 * c + 2 * gid, x0, x1, y0, y1, m_run[n][e], l_run[n][e]);
+            }
           }
-          store(r, c4, acc, M, L);
         }
+    } else {
+      // A unit that goes on after this piece ends the worker's work: its part
+      // waits for the other workers' in shared memory, in the rings once all
+      // are spent. One that ended here began before: to the workspace.
+      float *po = head_o(me), *pm = head_ml(me);
+      int pitch = D;
+      if (!ended) {
+        has_end = true;
+        if (lane == 0) s_end[warp] = un, s_has_end[warp] = begun ? 1 : 2;
+        po = parts + warp * ROWS * PITCH;
+        pm = &part_ml[warp][0][0];
+        pitch = PITCH;
+        rings_spent();
+      } else if (lane == 0) {
+        s_head[warp] = un, s_has_head[warp] = 1;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 8 * n + 2 * tig + e;
+#pragma unroll
+          for (int c = 0; c < MT; ++c)
+            *reinterpret_cast<float2 *>(po + r * pitch + 16 * c + 2 * gid) =
+                make_float2(o[c][n][e] * vref, o[c][n][2 + e] * vref);
+          if (gid == 0) *reinterpret_cast<float2 *>(pm + 2 * r) = make_float2(m_run[n][e], l_run[n][e]);
+        }
+    }
+  }
+  if (!has_end) rings_spent();
+  __syncthreads();
+
+  // ================ the parts of this CTA's workers, in the order of the line
+  if (t == 0) {
+    int n = 0;
+    bool open = false;
+    Group gr;
+    for (int w = 0; w < kSplitWarps; ++w) {
+      if (s_has_head[w]) {  // closes the open group, or one begun in an earlier CTA
+        if (!open) gr.first = w, gr.before = true;
+        gr.last = w, gr.last_is_head = true, gr.after = false;
+        s_group[n++] = gr;
+        open = false;
+      }
+      if (s_has_end[w]) {
+        if (!open) gr.first = w, gr.before = s_has_end[w] == 2;
+        open = true;
+        gr.last = w, gr.last_is_head = false, gr.after = true;
       }
     }
-    bar_compute();  // the merge buffer is free again
-    g += nt;
+    if (open) s_group[n++] = gr;
+    s_groups = n;
+    s_last[0] = s_last[1] = 0;
+  }
+  __syncthreads();
+  const int groups = s_groups;
+  auto unit_of = [&](const Group &gr) -> const Unit & {
+    return gr.last_is_head ? s_head[gr.last] : s_end[gr.last];
+  };
+  auto add = [&](float4 &acc, float &L, float wt, const float4 &x, float l) {
+    L = fmaf(wt, l, L);
+    acc.x = fmaf(wt, x.x, acc.x);
+    acc.y = fmaf(wt, x.y, acc.y);
+    acc.z = fmaf(wt, x.z, acc.z);
+    acc.w = fmaf(wt, x.w, acc.w);
+  };
+  constexpr int ITEMS = ROWS * (D / 4);  // of a unit: a row's four channels each
+  for (int e = t; e < groups * ITEMS; e += kSplitThreads) {
+    const Group &gr = s_group[e / ITEMS];
+    const Unit &un = unit_of(gr);
+    const int r = e % ITEMS / (D / 4), c4 = e % (D / 4);
+    if (r >= un.rows) continue;
+    auto ml = [&](int w) {
+      return w == gr.last && gr.last_is_head
+                 ? __ldcg(reinterpret_cast<const float2 *>(head_ml(blockIdx.x * kSplitWarps + w)) + r)
+                 : make_float2(part_ml[w][r][0], part_ml[w][r][1]);
+    };
+    auto has = [&](int w) { return s_has_end[w] || (w == gr.last && gr.last_is_head); };
+    float M = -INFINITY, L = 0.f;
+    for (int w = gr.first; w <= gr.last; ++w)
+      if (has(w)) M = fmaxf(M, ml(w).x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = gr.first; w <= gr.last; ++w) {
+      if (!has(w)) continue;
+      const float2 x = ml(w);
+      const float4 v =
+          w == gr.last && gr.last_is_head
+              ? __ldcg(reinterpret_cast<const float4 *>(head_o(blockIdx.x * kSplitWarps + w) + r * D) + c4)
+              : *reinterpret_cast<const float4 *>(parts + (w * ROWS + r) * PITCH + 4 * c4);
+      add(acc, L, ptx::ex2(x.x - (M == -INFINITY ? 0.f : M)), v, x.y);
+    }
+    if (!gr.before && !gr.after) {
+      split_store<KIND>(a, un, r, 4 * c4, acc.x, acc.y, acc.z, acc.w, M, L);
+    } else {
+      const int64_t slot = 2ll * blockIdx.x + (gr.before ? 0 : 1);
+      *reinterpret_cast<float4 *>(a.part_o + (slot * ROWS + r) * D + 4 * c4) = acc;
+      if (c4 == 0) *reinterpret_cast<float2 *>(a.part_ml + (slot * ROWS + r) * 2) = make_float2(M, L);
+    }
+  }
+  if (groups == 0 || !(s_group[0].before || s_group[groups - 1].after)) return;
+
+  // ================ the last CTA of a unit merges the CTAs' parts, in their order
+  __threadfence();
+  __syncthreads();
+  if (t < 2 && (t == 0 ? s_group[0].before : s_group[groups - 1].after && !s_group[groups - 1].before)) {
+    const Unit &un = unit_of(s_group[t == 0 ? 0 : groups - 1]);
+    const unsigned first = cta_of(un, 0), parts_less_1 = cta_of(un, un.n - 1) - first;
+    // counts the unit's CTAs and wraps to zero
+    s_last[t] = atomicInc(reinterpret_cast<unsigned *>(a.tickets) + first, parts_less_1) == parts_less_1;
+  }
+  __syncthreads();
+  for (int x = 0; x < 2; ++x) {
+    if (!s_last[x]) continue;
+    __threadfence();
+    const Unit &un = unit_of(s_group[x == 0 ? 0 : groups - 1]);
+    const int first = cta_of(un, 0), last = cta_of(un, un.n - 1);
+    for (int e = t; e < un.rows * (D / 4); e += kSplitThreads) {
+      const int r = e / (D / 4), c4 = e % (D / 4);
+      auto part = [&](int c) { return (2ll * c + (c == first ? 1 : 0)) * ROWS + r; };
+      float M = -INFINITY, L = 0.f;
+#pragma unroll 4
+      for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(a.part_ml + part(c) * 2));
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int c = first; c <= last; ++c) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part(c) * 2));
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part(c) * D + 4 * c4));
+        add(acc, L, ptx::ex2(ml.x - (M == -INFINITY ? 0.f : M)), v, ml.y);
+      }
+      split_store<KIND>(a, un, r, 4 * c4, acc.x, acc.y, acc.z, acc.w, M, L);
+    }
   }
 }
 
