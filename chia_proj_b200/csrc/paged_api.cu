@@ -183,7 +183,7 @@ int split_plan(const chia_paged_params_t *p, int sms, SplitPlan &pl) {
   // the line of tiles is counted in 32 bits
   const int64_t rows = 8 * pl.tiles;
   const double line = static_cast<double>(p->heads_kv) * (p->tokens * group / rows + p->batch + 1) *
-                      (p->table_width * p->page_size / 32 + 2);
+                      (p->table_width * p->page_size / 32 + 2 + chia::kUnitCost);
   if (pl.grid * 4 > kTicketBytes || p->tokens * p->heads > kI32 || line > kI32)
     return CHIA_ERR_UNSUPPORTED;
   const int64_t slots = (2 + chia::kSplitWarps) * pl.grid * rows;

@@ -26,8 +26,10 @@
 // conversion a pair; int8 by a byte permutation and a subtraction); Q, brought
 // to [2^14, 2^15) by a power of two per row, is a half exactly down to 2^-29
 // of its row's largest value; so products lose nothing. P is rounded to a half
-// (11 bits) after it is multiplied by its page's value scale over the largest
-// such scale seen: it stays within [0, 1] whatever the scales are.
+// (11 bits) with its page's value scale in it: the softmax's running maximum is
+// that of s + log2(scale), so the largest P of a row is 1 whatever the scales
+// are, and its sum takes the scale out again. Sigmoid and ReLU divide by a
+// running power of two instead.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -65,7 +67,8 @@ struct PagedArgs {
 constexpr int kSplitMaxBatch = 1024;  // requests of one launch (prefix sums in shared memory)
 constexpr int kSplitWarps = 8;
 constexpr int kSplitThreads = 32 * kSplitWarps;
-constexpr int kUnitCost = 4;  // what a unit costs beside its tiles, in tiles
+constexpr int kUnitCost = 4;   // what a unit costs beside its tiles, in tiles
+constexpr int kWholeUnit = 64; // units of up to this cost are not cut between CTAs
 
 // Queries and keys of request b, checked: [t0, t0 + n) of q, keys [0, len).
 struct Request {
@@ -180,7 +183,7 @@ struct SplitConfig {
 // A unit: rows [row0, row0 + rows) of a request's queries with one K/V head.
 struct Unit {
   int t0, row0, rows, hk;  // first token of the request
-  long long cost;          // where it begins in the line, in cost
+  int cost;                // where it begins in the line, in cost
   int n;                   // its tiles
 };
 
@@ -192,6 +195,7 @@ __device__ __forceinline__ void split_store(const PagedArgs &a, const Unit &u, i
   float f = 1.f;
   if (SOFTMAX) f = L > 0.f ? 1.f / L : L;  // (a NaN stays)
   if (KIND == KIND_RELU) f = a.out_scale * ptx::ex2(M);
+  if (KIND == KIND_SIGMOID) f = ptx::ex2(M);
   const int hh = u.hk * a.group + (u.row0 + r) % a.group;
   const int64_t tok = u.t0 + (u.row0 + r) / a.group;
   uint16_t *dst = static_cast<uint16_t *>(a.o) + tok * a.o_st + hh * a.o_sh + c;
@@ -219,6 +223,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
   float *parts = reinterpret_cast<float *>(sm);  // [warps][ROWS][PITCH], in the spent ring
   __shared__ int tiles_pre[kSplitMaxBatch + 1], units_pre[kSplitMaxBatch + 1];
+  __shared__ Request req[kSplitMaxBatch];
   __shared__ int wsum[kSplitWarps][2];
   __shared__ __align__(8) uint64_t bars[kSplitWarps * NST];
   __shared__ float part_ml[kSplitWarps][ROWS][2];
@@ -233,13 +238,14 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   };
   __shared__ Group s_group[kSplitWarps + 1];
   __shared__ int s_groups, s_last[2];
+  __shared__ uint32_t s_ends;
 
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int gid = lane >> 2, tig = lane & 3;
   const uint32_t bar0 = ptx::smem_u32(bars) + warp * NST * 8;
   const uint32_t ring = ptx::smem_u32(sm) + warp * NST * C::STAGE;
-  float4 *scales = reinterpret_cast<float4 *>(sm + C::RING) + warp * C::SCALES;  // ks, vs of
-                                                                                 // keys 0-15, 16-31
+  float4 *scales = reinterpret_cast<float4 *>(sm + C::RING) + warp * C::SCALES;  // ks and the
+                                                             // value factor of keys 0-15, 16-31
   if (t < kSplitWarps * NST) ptx::mbar_init(ptx::smem_u32(bars) + 8 * t, 1);
   if (t == 0) {
     abort_flag = 0;
@@ -255,6 +261,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     bool bad = false;
     for (int b = b0; b < b1; ++b) {
       const Request r = request_of(a, b, bad);
+      req[b] = r;
       int n = 0, u = 0;
       if (r.n > 0) {
         u = (r.n * a.group + ROWS - 1) / ROWS * a.heads_kv;
@@ -284,19 +291,20 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     if (t == 0) tiles_pre[0] = units_pre[0] = 0;
     __syncthreads();
   }
-  auto cost_before = [&](int b) {
-    return tiles_pre[b] + static_cast<long long>(kUnitCost) * units_pre[b];
-  };
-  const long long total = cost_before(a.batch);
-  long long ctas = (total + kSplitWarps - 1) / kSplitWarps;
-  if (ctas > gridDim.x) ctas = gridDim.x;
+  auto cost_before = [&](int b) { return tiles_pre[b] + kUnitCost * units_pre[b]; };
+  const int total = cost_before(a.batch);
+  const int ctas = min(static_cast<int>(gridDim.x), (total + kSplitWarps - 1) / kSplitWarps);
   if (blockIdx.x >= ctas) return;
-  const long long workers = ctas * kSplitWarps;
-  // Worker w begins at cost total * w / workers. A border within the cost of a
-  // unit's own counts as its first tile.
-  auto tile_at = [&](long long w) {
-    const long long x = total * w / workers;
-    if (x >= total) return tiles_pre[a.batch];
+  // Border c of the CTAs' pieces: total * c / ctas in cost, moved to the nearer
+  // end of the unit that it cuts where the unit is short: a cut costs a round
+  // of the workspace (some 4 us), whole units wait for nobody.
+  const int step = total / ctas, rest = total % ctas;
+  auto even = [&](int c) { return step * c + rest * c / ctas; };
+  auto place = [&](int x, bool snap, int &tile) {  // cost x, as a cost and as a tile
+    if (x >= total) {
+      tile = tiles_pre[a.batch];
+      return total;
+    }
     int lo = 0, hi = a.batch;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -306,60 +314,82 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         hi = mid;
     }
     const int units = units_pre[lo + 1] - units_pre[lo];
-    const int n = (tiles_pre[lo + 1] - tiles_pre[lo]) / units;
-    const int in = static_cast<int>(x - cost_before(lo));
-    const int u = in / (n + kUnitCost);
-    return tiles_pre[lo] + u * n + max(0, in - u * (n + kUnitCost) - kUnitCost);
+    const int n = (tiles_pre[lo + 1] - tiles_pre[lo]) / units, cost = n + kUnitCost;
+    int in = x - cost_before(lo), u = in / cost;
+    in -= u * cost;
+    if (snap && cost <= kWholeUnit) {
+      u += 2 * in >= cost ? 1 : 0;
+      in = 0;
+    }
+    // (a border within the cost of a unit's own counts as its first tile)
+    tile = tiles_pre[lo] + u * n + max(0, in - kUnitCost);
+    return cost_before(lo) + u * cost + in;
   };
-  // the CTA that has tile k of a unit
+  // the CTA that has tile k of a unit that is cut: the last with a border not above it
   auto cta_of = [&](const Unit &u, int k) {
-    return static_cast<int>(((u.cost + kUnitCost + k + 1) * workers - 1) / total / kSplitWarps);
+    const int x = u.cost + kUnitCost + k;
+    int c = static_cast<int>(static_cast<float>(x) / static_cast<float>(total) * ctas);
+    c = max(0, min(ctas - 1, c));
+    while (c + 1 < ctas && even(c + 1) <= x) ++c;
+    while (even(c) > x) --c;
+    return c;
   };
   const int me = blockIdx.x * kSplitWarps + warp;
-  const int c0 = tile_at(me), c1 = tile_at(me + 1);
-  const int nk = c1 - c0;  // tiles of this worker
+  int c0, nk;  // first tile and number of tiles of this worker
+  {
+    int tile;  // lane 0: this border, lane 1: the next one
+    const int y = place(even(blockIdx.x + (lane & 1)), true, tile);
+    const int y0 = __shfl_sync(0xffffffffu, y, 0), y1 = __shfl_sync(0xffffffffu, y, 1);
+    place(y0 + static_cast<int>(static_cast<long long>(y1 - y0) * (warp + (lane & 1)) / kSplitWarps),
+          false, tile);
+    c0 = __shfl_sync(0xffffffffu, tile, 0);
+    nk = __shfl_sync(0xffffffffu, tile, 1) - c0;
+  }
   if (lane == 0) s_has_head[warp] = s_has_end[warp] = 0;
   auto head_o = [&](int w) { return a.part_o + (2ll * gridDim.x + w) * ROWS * D; };
   auto head_ml = [&](int w) { return a.part_ml + (2ll * gridDim.x + w) * ROWS * 2; };
   auto rings_spent = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
 
   // ---- loads
-  int row0 = -1, row1 = -1, tok = 0;  // of tile 32 * (issued / 32) + lane: rows of the tensor map
-  auto look_up = [&](int k) {         // (page * heads_kv + head), first token; the scales go to
-    row0 = row1 = -1;                 // shared memory
-    float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+  // Of tile 32 * (k / 32) + lane: rows of the tensor map (page * heads_kv + head), first token.
+  const int pshift = 31 - __clz(a.page);
+  int row0 = -1, row1 = -1, tok = 0;
+  auto look_up = [&](int k) {
+    row0 = row1 = -1;
     if (k + lane < nk) {
       const int g = c0 + k + lane;
       const int b = last_not_above(tiles_pre, a.batch, g);
-      bool bad = false;
-      const Request r = request_of(a, b, bad);
+      const Request r = req[b];
       const Tiles tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
       const int nrb = (r.n * a.group + ROWS - 1) / ROWS;
       const int in = g - tiles_pre[b], u = in / tl.n;
-      const int hk = u / nrb, key = tl.key_tile(in - u * tl.n) * TK;
-      const int32_t *table = a.block_table + b * a.table_stride;
-      tok = key % a.page;
-      if (key < r.len) {
-        const int pg = table[key / a.page];
-        if (pg < 0 || pg >= a.num_pages)
-          bad = true;
-        else
-          row0 = pg * a.heads_kv + hk;
-      }
-      if (a.page == 16 && key + 16 < r.len) {
-        const int pg = table[key / 16 + 1];
-        if (pg < 0 || pg >= a.num_pages)
-          bad = true;
-        else
-          row1 = pg * a.heads_kv + hk;
-      }
-      if (bad) report(a.status, kStatusBadIndex);
-      if (row0 >= 0) sc.x = a.k_scale[row0], sc.y = a.v_scale[row0];
-      if (a.page != 16)
-        sc.z = sc.x, sc.w = sc.y;
-      else if (row1 >= 0)
-        sc.z = a.k_scale[row1], sc.w = a.v_scale[row1];
+      const int hk = nrb == 1 ? u : u / nrb, key = tl.key_tile(in - u * tl.n) * TK;
+      const int32_t *table = a.block_table + b * a.table_stride + (key >> pshift);
+      tok = key & (a.page - 1);
+      const bool want0 = key < r.len, want1 = a.page == 16 && key + 16 < r.len;
+      const int pg0 = want0 ? table[0] : 0, pg1 = want1 ? table[1] : 0;
+      const bool ok0 = pg0 >= 0 && pg0 < a.num_pages, ok1 = pg1 >= 0 && pg1 < a.num_pages;
+      if (want0 && ok0) row0 = pg0 * a.heads_kv + hk;
+      if (want1 && ok1) row1 = pg1 * a.heads_kv + hk;
+      if (!ok0 || !ok1) report(a.status, kStatusBadIndex);
     }
+  };
+  // A value scale as it is used: for the softmax kinds its logarithm, exact for
+  // a power of two and at least -100 (a scale of zero).
+  auto v_factor = [](float v) {
+    if (!SOFTMAX) return v;
+    const uint32_t b = __float_as_uint(v);
+    if (v < 7.9e-31f) return -100.f;
+    return (b & 0x7fffffu) == 0 && b < 0x7f800000u ? static_cast<float>(static_cast<int>(b >> 23) - 127)
+                                                   : __log2f(v);
+  };
+  auto look_up_scales = [&](int k) {  // of the same tiles, to shared memory
+    float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row0 >= 0) sc.x = a.k_scale[row0], sc.y = v_factor(a.v_scale[row0]);
+    if (a.page != 16)
+      sc.z = sc.x, sc.w = sc.y;
+    else if (row1 >= 0)
+      sc.z = a.k_scale[row1], sc.w = v_factor(a.v_scale[row1]);
     scales[(k + lane) % C::SCALES] = sc;  // (those of 64 tiles ago are long used)
     __syncwarp();
   };
@@ -382,56 +412,77 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         tma_load_3d(dst + TK * D + 16 * D, &mv, bar, 0, 0, r1);
       }
     }
+    // (at the start the copies leave before the scales are asked for)
+    if (k % 32 == 0 && k > 0) look_up_scales(k);
   };
-  for (int k = 0; k < NST; ++k) issue(k);
 
-  // ---- units of the piece
+  // ---- units of the piece: the one that tile k belongs to, and its queries
+  Unit un;
+  Tiles tl;
+  int len = 0, p0 = 0, ut0 = 0, nt = 0;
+  uint4 raw[NT][H * 2];  // row 8 n + gid, channels 16 H tig .. + 16 H - 1
+  float hp[NT][2];       // of rows 8 n + 2 tig + e, as in the columns of S^T
+  auto begin_unit = [&](int k) {
+    const int g = c0 + k, b = last_not_above(tiles_pre, a.batch, g);
+    const Request rq = req[b];
+    len = rq.len;
+    p0 = len - rq.n;
+    tl = tiles_of<TK>(a, p0, len - 1, len);
+    const int nrows_all = rq.n * a.group, nrb = (nrows_all + ROWS - 1) / ROWS;
+    const int in = g - tiles_pre[b], u = in / tl.n;
+    ut0 = in - u * tl.n;
+    nt = min(tl.n - ut0, nk - k);
+    un.t0 = rq.t0;
+    un.hk = nrb == 1 ? u : u / nrb;
+    un.row0 = (u - un.hk * nrb) * ROWS;
+    un.rows = min(ROWS, nrows_all - un.row0);
+    un.cost = cost_before(b) + u * (tl.n + kUnitCost);
+    un.n = tl.n;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int rr = 8 * n + gid, row = un.row0 + rr;
+      if (rr < un.rows) {
+        const int qi = row / a.group;
+        const uint16_t *src = static_cast<const uint16_t *>(a.q) +
+                              static_cast<int64_t>(rq.t0 + qi) * a.q_st +
+                              (un.hk * a.group + row - qi * a.group) * a.q_sh + H * 16 * tig;
+#pragma unroll
+        for (int c = 0; c < H * 2; ++c) raw[n][c] = *reinterpret_cast<const uint4 *>(src + 8 * c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < H * 2; ++c) raw[n][c] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = min(8 * n + 2 * tig + x, un.rows - 1) + un.row0;
+        hp[n][x] = a.head_param != nullptr ? a.head_param[un.hk * a.group + r % a.group] : 1.f;
+      }
+    }
+  };
+  if (nk > 0) {
+    begin_unit(0);
+    for (int k = 0; k < NST; ++k) issue(k);
+    look_up_scales(0);
+  }
+
   bool aborted = false, has_end = false;
   for (int k = 0; k < nk;) {
-    const int g = c0 + k;
-    const int b = last_not_above(tiles_pre, a.batch, g);
-    bool bad = false;
-    const Request rq = request_of(a, b, bad);
-    const int p0 = rq.len - rq.n;
-    const Tiles tl = tiles_of<TK>(a, p0, rq.len - 1, rq.len);
-    const int nrows_all = rq.n * a.group, nrb = (nrows_all + ROWS - 1) / ROWS;
-    const int in = g - tiles_pre[b], u = in / tl.n, ut0 = in - u * tl.n;
-    const int nt = min(tl.n - ut0, nk - k);
-    Unit un;
-    un.t0 = rq.t0;
-    un.row0 = (u % nrb) * ROWS;
-    un.rows = min(ROWS, nrows_all - un.row0);
-    un.hk = u / nrb;
-    un.cost = cost_before(b) + static_cast<long long>(u) * (tl.n + kUnitCost);
-    un.n = tl.n;
     // all rows of the unit see keys [lo_max, hi_min]; none sees one outside [lo_min, hi_max]
     int lo_min, lo_max, hi_min, hi_max;
-    band32(a, p0 + un.row0 / a.group, rq.len, lo_min, hi_min);
-    band32(a, p0 + (un.row0 + un.rows - 1) / a.group, rq.len, lo_max, hi_max);
-    const int pf = min(a.prefix, rq.len);
+    band32(a, p0 + un.row0 / a.group, len, lo_min, hi_min);
+    band32(a, p0 + (un.row0 + un.rows - 1) / a.group, len, lo_max, hi_max);
+    const int pf = min(a.prefix, len);
 
-    // ---- Q: row 8 n + gid, channels 16 (H tig + h) + 4 s .. + 3 of step (h, s)
+    // Q as fragments: channels 16 (H tig + h) + 4 s .. + 3 of step (h, s)
     uint32_t qf[NT][H * 4][2];
-    float rowmul[NT][2], slope[NT][2];  // rows 8 n + 2 tig + e, as in the columns of S^T
+    float rowmul[NT][2], slope[NT][2];
     int posn[NT][2];
     uint32_t real = 0;  // bit 2 n + e: that row exists
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int rr = 8 * n + gid, row = un.row0 + rr;
-      uint4 raw[H * 2];
-      if (rr < un.rows) {
-        const uint16_t *src = static_cast<const uint16_t *>(a.q) +
-                              static_cast<int64_t>(rq.t0 + row / a.group) * a.q_st +
-                              (un.hk * a.group + row % a.group) * a.q_sh + H * 16 * tig;
-#pragma unroll
-        for (int c = 0; c < H * 2; ++c) raw[c] = *reinterpret_cast<const uint4 *>(src + 8 * c);
-      } else {
-#pragma unroll
-        for (int c = 0; c < H * 2; ++c) raw[c] = make_uint4(0, 0, 0, 0);
-      }
       float mx = 0.f;
       auto get = [&](int w, float2 &x) {  // 32-bit word w of the lane's channels
-        const uint4 &r4 = raw[w / 4];
+        const uint4 &r4 = raw[n][w / 4];
         const uint32_t v = w % 4 == 0 ? r4.x : w % 4 == 1 ? r4.y : w % 4 == 2 ? r4.z : r4.w;
         x = a.bf16 ? in16x2_to_float2<true>(v) : in16x2_to_float2<false>(v);
       };
@@ -457,24 +508,23 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       for (int x = 0; x < 2; ++x) {
         const float f = __shfl_sync(0xffffffffu, down, (2 * tig + x) * 4);
         const int r = min(8 * n + 2 * tig + x, un.rows - 1) + un.row0;
-        const float hp = a.head_param != nullptr ? a.head_param[un.hk * a.group + r % a.group] : 1.f;
         posn[n][x] = p0 + r / a.group;
         real |= (8 * n + 2 * tig + x < un.rows ? 1u : 0u) << (2 * n + x);
         float mul = a.score_scale * f;
         slope[n][x] = 0.f;
-        if (KIND == KIND_SOFTMAX) mul *= LOG2E * hp;
+        if (KIND == KIND_SOFTMAX) mul *= LOG2E * hp[n][x];
         if (KIND == KIND_SOFTCAP) mul *= 2.f * LOG2E / a.softcap;  // 2^(2 log2e s / cap) = e^(2s/cap)
-        if (KIND == KIND_ALIBI) mul *= LOG2E, slope[n][x] = hp * LOG2E;
+        if (KIND == KIND_ALIBI) mul *= LOG2E, slope[n][x] = hp[n][x] * LOG2E;
         if (KIND == KIND_SIGMOID) mul *= -LOG2E;
         rowmul[n][x] = mul;
       }
     }
-    float o[MT][NT][4], m_run[NT][2], l_run[NT][2], vref = 0.f, inv_vref = 0.f;
+    float o[MT][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int c = 0; c < MT; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
-      m_run[n][0] = m_run[n][1] = SOFTMAX ? -INFINITY : KIND == KIND_RELU ? -120.f : 0.f;
+      m_run[n][0] = m_run[n][1] = SOFTMAX ? -INFINITY : -120.f;
       l_run[n][0] = l_run[n][1] = 0.f;
     }
 
@@ -542,7 +592,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
-            const float f = rowmul[n][e] * (m ? sc.z : sc.x);
+            const float f = rowmul[n][e] * (m ? sc.z : sc.x), vf = m ? sc.w : sc.y;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               float &v = s[m][n][2 * x + e];
@@ -550,17 +600,17 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                 // cap tanh(y) = cap - 2 cap / (e^(2y) + 1), to 2^-22 cap: the
                 // approximate tanh instruction (2^-11) would show in P
                 const float z = ptx::ex2(v * f);
-                v = a.softcap * LOG2E * fmaf(-2.f, ptx::rcp_fast(z + 1.f), 1.f);
+                v = fmaf(a.softcap * LOG2E, fmaf(-2.f, ptx::rcp_fast(z + 1.f), 1.f), vf);
               } else if (KIND == KIND_ALIBI) {
-                v = fmaf(slope[n][e],
-                         static_cast<float>(j0 + 16 * m + 8 * x + gid - posn[n][e]), v * f);
+                v = fmaf(slope[n][e], static_cast<float>(j0 + 16 * m + 8 * x + gid - posn[n][e]),
+                         fmaf(v, f, vf));
               } else if (KIND == KIND_SIGMOID) {
-                v = ptx::rcp_fast(1.f + ptx::ex2(fmaf(v, f, -a.sig_bias * LOG2E)));
+                v = vf * ptx::rcp_fast(1.f + ptx::ex2(fmaf(v, f, -a.sig_bias * LOG2E)));
               } else if (KIND == KIND_RELU) {
                 v *= f;
-                v = v < 0.f ? 0.f : v;  // (a NaN stays)
+                v = v < 0.f ? 0.f : v * vf;  // (a NaN stays)
               } else {
-                v *= f;
+                v = fmaf(v, f, vf);
               }
             }
           }
@@ -571,7 +621,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           for (int e = 0; e < 2; ++e) {
             const int i_pos = posn[n][e];
             int lo, hi;
-            band32(a, i_pos, rq.len, lo, hi);
+            band32(a, i_pos, len, lo, hi);
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -584,7 +634,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               }
           }
       }
-      if (SOFTMAX || KIND == KIND_RELU) {
+      {
         float mx[NT][2];
         bool grow = false;
 #pragma unroll
@@ -592,7 +642,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             mx[n][e] = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
-            grow |= KIND == KIND_RELU ? mx[n][e] > ptx::ex2(m_run[n][e]) : mx[n][e] > m_run[n][e];
+            grow |= mx[n][e] > (SOFTMAX ? m_run[n][e] : ptx::ex2(m_run[n][e]));
           }
         if (__any_sync(0xffffffffu, grow)) {  // some row's maximum is exceeded
 #pragma unroll
@@ -602,7 +652,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               float v = mx[n][e];
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-              if (KIND == KIND_RELU)  // the power of two above it, as its logarithm
+              if (!SOFTMAX)  // the power of two above it, as its logarithm
                 v = static_cast<float>(static_cast<int>(__float_as_uint(v) >> 23) - 126);
               const float nm = fmaxf(m_run[n][e], v);
               const float al = ptx::ex2(m_run[n][e] - (nm == -INFINITY ? 0.f : nm));
@@ -616,44 +666,29 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             }
         }
       }
-      // the values' scales, relative to the largest power of two above one so far
-      {
-        const float vm = fmaxf(sc.y, sc.w);
-        if (vm > vref) {
-          const uint32_t bits = __float_as_uint(vm);
-          const float up = __uint_as_float(min((bits + 0x7fffffu) & 0xff800000u, 0x7f000000u));
-          const float al = vref * __frcp_rn(up);  // (exact: powers of two)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < MT; ++c)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) o[c][n][x] *= al;
-          vref = up;
-          inv_vref = __frcp_rn(up);
-        }
-      }
-      const float r0 = sc.y * inv_vref, r1 = sc.w * inv_vref;
+      const float il[2] = {SOFTMAX ? ptx::ex2(-sc.y) : 0.f, SOFTMAX ? ptx::ex2(-sc.w) : 0.f};
       uint32_t pb[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float mu = m_run[n][e] == -INFINITY ? 0.f : m_run[n][e];
-          const float down = KIND == KIND_RELU ? ptx::ex2(-mu) : 1.f;
-          float sum = 0.f;
+          const float down = SOFTMAX ? 0.f : ptx::ex2(-mu);
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < 2; ++m) {
+            float sum = 0.f;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               float &v = s[m][n][2 * x + e];
               if (SOFTMAX) {
                 v = ptx::ex2(v - mu);
                 sum += v;
+              } else {
+                v *= down;
               }
-              v *= (m ? r1 : r0) * down;
             }
-          l_run[n][e] += sum;
+            if (SOFTMAX) l_run[n][e] = fmaf(sum, il[m], l_run[n][e]);
+          }
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -701,7 +736,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             for (int e = 0; e < 2; ++e) {
               const int i_pos = posn[n][e];
               int lo, hi;
-              band32(a, i_pos, rq.len, lo, hi);
+              band32(a, i_pos, len, lo, hi);
               sees[n][e] = ((real >> (2 * n + e)) & 1u) &&
                            (j < pf || (j >= lo && j <= hi &&
                                        (a.dil == 1 || (i_pos - j) % a.dil == 0)));
@@ -746,7 +781,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
             // lanes of even and odd gid exchange, so that each has four channels of a row
-            const float x0 = o[c][n][e] * vref, x1 = o[c][n][2 + e] * vref;
+            const float x0 = o[c][n][e], x1 = o[c][n][2 + e];
             const float y0 = __shfl_xor_sync(0xffffffffu, x0, 4), y1 = __shfl_xor_sync(0xffffffffu, x1, 4);
             if (((gid ^ c) & 1) == 0 && r < un.rows) {
               if (gid & 1)
@@ -781,35 +816,42 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
           for (int c = 0; c < MT; ++c)
             *reinterpret_cast<float2 *>(po + r * pitch + 16 * c + 2 * gid) =
-                make_float2(o[c][n][e] * vref, o[c][n][2 + e] * vref);
+                make_float2(o[c][n][e], o[c][n][2 + e]);
           if (gid == 0) *reinterpret_cast<float2 *>(pm + 2 * r) = make_float2(m_run[n][e], l_run[n][e]);
         }
     }
+    if (k < nk) begin_unit(k);
   }
   if (!has_end) rings_spent();
   __syncthreads();
 
   // ================ the parts of this CTA's workers, in the order of the line
-  if (t == 0) {
-    int n = 0;
-    bool open = false;
-    Group gr;
-    for (int w = 0; w < kSplitWarps; ++w) {
-      if (s_has_head[w]) {  // closes the open group, or one begun in an earlier CTA
-        if (!open) gr.first = w, gr.before = true;
-        gr.last = w, gr.last_is_head = true, gr.after = false;
-        s_group[n++] = gr;
-        open = false;
+  if (t < 32) {
+    const uint32_t heads = __ballot_sync(0xffffffffu, lane < kSplitWarps && s_has_head[lane & 7] != 0);
+    const uint32_t ends = __ballot_sync(0xffffffffu, lane < kSplitWarps && s_has_end[lane & 7] != 0);
+    const uint32_t mid = __ballot_sync(0xffffffffu, lane < kSplitWarps && s_has_end[lane & 7] == 2);
+    if (lane == 0) {
+      int n = 0;
+      bool open = false;
+      Group gr;
+      for (int w = 0; w < kSplitWarps; ++w) {
+        if ((heads >> w) & 1) {  // closes the open group, or one begun in an earlier CTA
+          if (!open) gr.first = w, gr.before = true;
+          gr.last = w, gr.last_is_head = true, gr.after = false;
+          s_group[n++] = gr;
+          open = false;
+        }
+        if ((ends >> w) & 1) {
+          if (!open) gr.first = w, gr.before = (mid >> w) & 1;
+          open = true;
+          gr.last = w, gr.last_is_head = false, gr.after = true;
+        }
       }
-      if (s_has_end[w]) {
-        if (!open) gr.first = w, gr.before = s_has_end[w] == 2;
-        open = true;
-        gr.last = w, gr.last_is_head = false, gr.after = true;
-      }
+      if (open) s_group[n++] = gr;
+      s_groups = n;
+      s_ends = ends;
+      s_last[0] = s_last[1] = 0;
     }
-    if (open) s_group[n++] = gr;
-    s_groups = n;
-    s_last[0] = s_last[1] = 0;
   }
   __syncthreads();
   const int groups = s_groups;
@@ -829,25 +871,31 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     const Unit &un = unit_of(gr);
     const int r = e % ITEMS / (D / 4), c4 = e % (D / 4);
     if (r >= un.rows) continue;
-    auto ml = [&](int w) {
-      return w == gr.last && gr.last_is_head
-                 ? __ldcg(reinterpret_cast<const float2 *>(head_ml(blockIdx.x * kSplitWarps + w)) + r)
-                 : make_float2(part_ml[w][r][0], part_ml[w][r][1]);
-    };
-    auto has = [&](int w) { return s_has_end[w] || (w == gr.last && gr.last_is_head); };
-    float M = -INFINITY, L = 0.f;
-    for (int w = gr.first; w <= gr.last; ++w)
-      if (has(w)) M = fmaxf(M, ml(w).x);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = gr.first; w <= gr.last; ++w) {
-      if (!has(w)) continue;
-      const float2 x = ml(w);
-      const float4 v =
-          w == gr.last && gr.last_is_head
-              ? __ldcg(reinterpret_cast<const float4 *>(head_o(blockIdx.x * kSplitWarps + w) + r * D) + c4)
-              : *reinterpret_cast<const float4 *>(parts + (w * ROWS + r) * PITCH + 4 * c4);
-      add(acc, L, ptx::ex2(x.x - (M == -INFINITY ? 0.f : M)), v, x.y);
+    // the workers' parts in shared memory, then the one in the workspace; all loads at once
+    const uint32_t span = (2u << gr.last) - (1u << gr.first);
+    const uint32_t in_smem = span & s_ends & ~(gr.last_is_head ? 1u << gr.last : 0u);
+    float2 hml = make_float2(-INFINITY, 0.f);
+    float4 hv = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (gr.last_is_head) {
+      const int w = blockIdx.x * kSplitWarps + gr.last;
+      hml = __ldcg(reinterpret_cast<const float2 *>(head_ml(w)) + r);
+      hv = __ldcg(reinterpret_cast<const float4 *>(head_o(w) + r * D) + c4);
     }
+    float2 x[kSplitWarps];
+    float M = hml.x, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+      x[w] = (in_smem >> w) & 1 ? make_float2(part_ml[w][r][0], part_ml[w][r][1])
+                                : make_float2(-INFINITY, 0.f);
+      M = fmaxf(M, x[w].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w)
+      if ((in_smem >> w) & 1)
+        add(acc, L, ptx::ex2(x[w].x - (M == -INFINITY ? 0.f : M)),
+            *reinterpret_cast<const float4 *>(parts + (w * ROWS + r) * PITCH + 4 * c4), x[w].y);
+    if (gr.last_is_head) add(acc, L, ptx::ex2(hml.x - (M == -INFINITY ? 0.f : M)), hv, hml.y);
     if (!gr.before && !gr.after) {
       split_store<KIND>(a, un, r, 4 * c4, acc.x, acc.y, acc.z, acc.w, M, L);
     } else {
@@ -859,18 +907,18 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   if (groups == 0 || !(s_group[0].before || s_group[groups - 1].after)) return;
 
   // ================ the last CTA of a unit merges the CTAs' parts, in their order
-  __threadfence();
   __syncthreads();
   if (t < 2 && (t == 0 ? s_group[0].before : s_group[groups - 1].after && !s_group[groups - 1].before)) {
     const Unit &un = unit_of(s_group[t == 0 ? 0 : groups - 1]);
     const unsigned first = cta_of(un, 0), parts_less_1 = cta_of(un, un.n - 1) - first;
+    __threadfence();  // (the CTA's parts, seen through the barrier, before the ticket)
     // counts the unit's CTAs and wraps to zero
     s_last[t] = atomicInc(reinterpret_cast<unsigned *>(a.tickets) + first, parts_less_1) == parts_less_1;
+    __threadfence();
   }
   __syncthreads();
   for (int x = 0; x < 2; ++x) {
     if (!s_last[x]) continue;
-    __threadfence();
     const Unit &un = unit_of(s_group[x == 0 ? 0 : groups - 1]);
     const int first = cta_of(un, 0), last = cta_of(un, un.n - 1);
     for (int e = t; e < un.rows * (D / 4); e += kSplitThreads) {

@@ -41,6 +41,9 @@ _pack_tables = N.packer(N.TablesParams)
 _pack_append = N.packer(N.AppendParams)
 _pack_paged = N.packer(N.PagedParams)
 _workspaces: Dict[tuple, torch.Tensor] = {}
+_workspace_bytes: Dict[int, int] = {}
+_functions: Dict[str, object] = {}
+_stream = torch._C._cuda_getCurrentRawStream  # of a device index; current_stream() builds an object
 
 
 class PageStep(NamedTuple):
@@ -71,7 +74,9 @@ def _int32(name: str, t, shape: tuple, dev: torch.device) -> None:
 
 
 def _call(name: str, dev: torch.device, packed: bytes, stream: int, what) -> None:
-    fn = getattr(N.load(), name)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(N.load(), name)
     if torch.cuda.current_device() == dev.index:
         code = fn(packed, stream)
     else:
@@ -147,7 +152,7 @@ def _tables_call(name, seq_lens, lens, block_table, free_pages, free_state, page
     base = buf.data_ptr()
     o = (base, base + 4 * T, base + 8 * T, base + 8 * T + 4 * (B + 1),
          base + 8 * T + 4 * (2 * B + 1))
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    stream = _stream(dev.index)
     packed = _pack_tables(
         N.PAGED_ABI_VERSION, page_size, B, block_table.shape[1],
         max(block_table.stride(0), block_table.shape[1]), free_pages.shape[0], T,
@@ -220,21 +225,29 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
         v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
         _status_word(dev).data_ptr())
-    _call("chia_cache_append", dev, packed, torch.cuda.current_stream(dev).cuda_stream,
-          (k, k_cache))
+    _call("chia_cache_append", dev, packed, _stream(dev.index), (k, k_cache))
 
 
-def _workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """Workspace of ``paged_attention`` for one (device, stream). A call that
-    a CUDA graph captures gets one of its own, zero-filled within the graph:
-    the graph may be replayed beside calls on the stream that captured it."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+def _workspace(dev: torch.device, stream: int) -> torch.Tensor:
+    """Workspace of ``paged_attention`` for one (device, stream): as large as
+    any call needs. A call that a CUDA graph captures gets one of its own,
+    zero-filled within the graph: the graph may be replayed beside calls on the
+    stream that captured it."""
     key = (dev.index, stream)
     t = _workspaces.get(key)
-    if t is None or t.numel() < nbytes:
-        t = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-        _workspaces[key] = t
+    capturing = torch.cuda.is_current_stream_capturing()
+    if t is None or capturing:
+        n = _workspace_bytes.get(dev.index)
+        if n is None:
+            with torch.cuda.device(dev):  # the largest: head_dim 128, more than 8 rows a K/V head
+                n = N.load().chia_paged_attn_workspace_bytes(_pack_paged(
+                    N.PAGED_ABI_VERSION, 0, 0, 128, 0, 0, 1, 1, 16, 9, 1, 1, 1, 1, 1, *([256] * 2),
+                    *([0] * 4), *([256] * 6), 0, 0, 0, 1.0, 1.0, 0.0, 1.0, -1, -1, 0, 0, 1, 0, 0, 0,
+                    0))
+            _workspace_bytes[dev.index] = n
+        t = torch.zeros(n, dtype=torch.uint8, device=dev)
+        if not capturing:
+            _workspaces[key] = t
     return t
 
 
@@ -299,7 +312,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("max_q must be >= 1")
     q = _prep(q)
     if out is None:
-        o = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+        o = q.new_empty(q.shape)
     else:
         o = out
         if o.shape != q.shape or o.dtype is not q.dtype or o.device != dev:
@@ -312,22 +325,16 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
               else _param_tensor(head_param, H, dev))
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if T:
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        def pack(ws, nbytes):
-            return _pack_paged(
-                N.PAGED_ABI_VERSION, dt, ct, D, _NORMS[norm], _MODS[mod], H, shape[1], shape[2],
-                min(max_q, T), B, T, shape[0], W, max(block_table.stride(0), W), q.data_ptr(),
-                o.data_ptr(), q.stride(0), q.stride(1), o.stride(0), o.stride(1),
-                k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
-                0 if lse is None else lse.data_ptr(), 0 if hp is None else hp.data_ptr(),
-                1.0 / math.sqrt(D) if scale is None else scale, softcap, sig_bias, out_scale,
-                mask.left, mask.right, mask.block, mask.prefix, mask.dilation,
-                _status_word(dev).data_ptr(), ws, nbytes, wait_limit_ns)
-        nbytes = N.load().chia_paged_attn_workspace_bytes(pack(0, 0))
-        if nbytes < 0:
-            raise ValueError("invalid parameters")
-        ws = _workspace(dev, stream, nbytes)
-        _call("chia_paged_attn", dev, pack(ws.data_ptr(), ws.numel()), stream,
-              (q, k_cache, block_table))
+        stream = _stream(dev.index)
+        ws = _workspace(dev, stream)
+        packed = _pack_paged(
+            N.PAGED_ABI_VERSION, dt, ct, D, _NORMS[norm], _MODS[mod], H, shape[1], shape[2],
+            min(max_q, T), B, T, shape[0], W, max(block_table.stride(0), W), q.data_ptr(),
+            o.data_ptr(), *q.stride()[:2], *o.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            0 if cu_q is None else cu_q.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            0 if hp is None else hp.data_ptr(), 1.0 / math.sqrt(D) if scale is None else scale,
+            softcap, sig_bias, out_scale, mask.left, mask.right, mask.block, mask.prefix,
+            mask.dilation, _status_word(dev).data_ptr(), ws.data_ptr(), ws.numel(), wait_limit_ns)
+        _call("chia_paged_attn", dev, packed, stream, (q, k_cache, block_table))
     return (o, lse) if return_lse else o

@@ -445,9 +445,9 @@ def test_bad_pages_and_lengths_are_reported(cuda):
         with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
             cp.check_device_status(0)
     short = ints(table)[:, :3].contiguous()
-    for lens in ([2 ** 31 - 1, 33], [-4, 33]):
+    for lens, taken in (([2 ** 31 - 1, 33], [48, 33]), ([-4, 33], [0, 33])):
         got = cp.paged_attention(q, k, v, ks, vs, short, ints(lens), ints(cu))
-        assert torch.equal(got[1], good[1])
+        assert torch.equal(got, cp.paged_attention(q, k, v, ks, vs, short, ints(taken), ints(cu)))
         with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
             cp.check_device_status(0)
     for offs in ([0, 2 ** 30, 2], [0, -7, 2], [-3, 1, 2], [0, 1, 9]):
