@@ -184,7 +184,8 @@ int split_plan(const chia_paged_params_t *p, int sms, SplitPlan &pl) {
   const int64_t rows = 8 * pl.tiles;
   const double line = static_cast<double>(p->heads_kv) * (p->tokens * group / rows + p->batch + 1) *
                       (p->table_width * p->page_size / 32 + 2 + chia::kUnitCost);
-  if (pl.grid * 4 > kTicketBytes || p->tokens * p->heads > kI32 || line > kI32)
+  if (pl.grid * 4 > kTicketBytes || p->tokens * p->heads > kI32 ||
+      p->tokens * group * group > 2 * kI32 || line > kI32)
     return CHIA_ERR_UNSUPPORTED;
   const int64_t slots = (2 + chia::kSplitWarps) * pl.grid * rows;
   pl.off_ml = kTicketBytes + slots * p->head_dim * 4;
@@ -334,6 +335,7 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   a.heads = p->heads;
   a.heads_kv = p->heads_kv;
   a.group = p->heads / p->heads_kv;
+  a.group_magic = a.group == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + a.group - 1) / a.group);
   a.tokens = static_cast<int32_t>(p->tokens);
   a.page = p->page_size;
   a.width = static_cast<int32_t>(p->table_width);

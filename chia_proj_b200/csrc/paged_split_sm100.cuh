@@ -53,6 +53,7 @@ struct PagedArgs {
   int32_t left, right, block, prefix, dil;  // the mask, on positions (at most 2^30 each)
   float score_scale, softcap, sig_bias, out_scale;
   int32_t heads, heads_kv, group, batch, tokens, page, width;
+  uint32_t group_magic;  // ceil(2^32 / group); 0: a group of one
   int32_t num_pages;
   int32_t q_each;     // queries of a request where cu_q is null
   int32_t token0;     // first token of request 0 where cu_q is null
@@ -64,15 +65,23 @@ struct PagedArgs {
   uint64_t timeout_ns, drain_ns;
 };
 
-constexpr int kSplitMaxBatch = 1024;  // requests of one launch (prefix sums in shared memory)
+constexpr int kSplitMaxBatch = 512;  // requests of one launch (they are held in shared memory)
 constexpr int kSplitWarps = 8;
 constexpr int kSplitThreads = 32 * kSplitWarps;
 constexpr int kUnitCost = 4;   // what a unit costs beside its tiles, in tiles
 constexpr int kWholeUnit = 64; // units of up to this cost are not cut between CTAs
 
+// Tiles of TK keys that queries at positions [p0, p1] visit: `pre` tiles from
+// key 0 on, then those from `lo` on; `n` in all, at least one (a unit whose
+// rows see nothing still writes zeros).
+struct Tiles {
+  int pre, lo, n;
+  __device__ __forceinline__ int key_tile(int t) const { return t < pre ? t : lo + (t - pre); }
+};
 // Queries and keys of request b, checked: [t0, t0 + n) of q, keys [0, len).
 struct Request {
   int t0, n, len;
+  Tiles tl;
 };
 __device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &bad) {
   Request r;
@@ -98,6 +107,18 @@ __device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &b
   return r;
 }
 
+// The rare divisions stand in functions of their own: a call that needs none
+// of them fetches the less code, and its first pass over the code is most of
+// the time of a small call.
+static __device__ __noinline__ int block_start(int i, int block) {
+  return (i >= 0 ? i / block : -((-i + block - 1) / block)) * block;
+}
+static __device__ __noinline__ bool divides(int d, int x) { return x % d == 0; }
+// x / group for x * group < 2^32
+__device__ __forceinline__ int div_group(const PagedArgs &a, int x) {
+  return a.group_magic == 0 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), a.group_magic));
+}
+
 // The keys position i sees beside the prefix (position_band in 32 bits).
 __device__ __forceinline__ void band32(const PagedArgs &a, int i, int len, int &lo, int &hi) {
   lo = 0;
@@ -105,19 +126,12 @@ __device__ __forceinline__ void band32(const PagedArgs &a, int i, int len, int &
   if (a.left >= 0) lo = max(lo, i - a.left);
   if (a.right >= 0) hi = min(hi, i + a.right);
   if (a.block > 0) {
-    const int b0 = (i >= 0 ? i / a.block : -((-i + a.block - 1) / a.block)) * a.block;
+    const int b0 = block_start(i, a.block);
     lo = max(lo, b0);
     hi = min(hi, b0 + a.block - 1);
   }
 }
 
-// Tiles of TK keys that queries at positions [p0, p1] visit: `pre` tiles from
-// key 0 on, then those from `lo` on; `n` in all, at least one (a unit whose
-// rows see nothing still writes zeros).
-struct Tiles {
-  int pre, lo, n;
-  __device__ __forceinline__ int key_tile(int t) const { return t < pre ? t : lo + (t - pre); }
-};
 template <int TK>
 __device__ __forceinline__ Tiles tiles_of(const PagedArgs &a, int p0, int p1, int len) {
   Tiles r;
@@ -187,25 +201,28 @@ struct Unit {
   int n;                   // its tiles
 };
 
-// A row's four channels, normalised, to the output; the first also writes the log-sum-exp.
+// Where a row's output goes, and what it is multiplied by; `lse`: its log-sum-exp is written here too.
 template <int KIND>
-__device__ __forceinline__ void split_store(const PagedArgs &a, const Unit &u, int r, int c, float x0,
-                                            float x1, float x2, float x3, float M, float L) {
+__device__ __forceinline__ uint16_t *row_out(const PagedArgs &a, const Unit &u, int r, float M, float L,
+                                             bool lse, float &f) {
   constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
-  float f = 1.f;
+  f = 1.f;
   if (SOFTMAX) f = L > 0.f ? 1.f / L : L;  // (a NaN stays)
   if (KIND == KIND_RELU) f = a.out_scale * ptx::ex2(M);
   if (KIND == KIND_SIGMOID) f = ptx::ex2(M);
-  const int hh = u.hk * a.group + (u.row0 + r) % a.group;
-  const int64_t tok = u.t0 + (u.row0 + r) / a.group;
-  uint16_t *dst = static_cast<uint16_t *>(a.o) + tok * a.o_st + hh * a.o_sh + c;
+  const int qi = div_group(a, u.row0 + r), hh = u.hk * a.group + u.row0 + r - qi * a.group;
+  const int64_t tok = u.t0 + qi;
+  if (SOFTMAX && a.lse != nullptr && lse)
+    a.lse[tok * a.heads + hh] =
+        L > 0.f ? (M + __log2f(L)) * 0.6931471805599453f : L == 0.f ? -INFINITY : L;
+  return static_cast<uint16_t *>(a.o) + tok * a.o_st + hh * a.o_sh;
+}
+__device__ __forceinline__ void store4(const PagedArgs &a, uint16_t *dst, float f, float x0, float x1,
+                                       float x2, float x3) {
   x0 *= f, x1 *= f, x2 *= f, x3 *= f;
   *reinterpret_cast<uint2 *>(dst) =
       a.bf16 ? make_uint2(ptx::pack_bf16(x0, x1), ptx::pack_bf16(x2, x3))
              : make_uint2(ptx::pack_f16(x0, x1), ptx::pack_f16(x2, x3));
-  if (SOFTMAX && a.lse != nullptr && c == 0)
-    a.lse[tok * a.heads + hh] =
-        L > 0.f ? (M + __log2f(L)) * 0.6931471805599453f : L == 0.f ? -INFINITY : L;
 }
 
 // KIND: score modification and normaliser.
@@ -260,13 +277,14 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     int nt = 0, nu = 0;
     bool bad = false;
     for (int b = b0; b < b1; ++b) {
-      const Request r = request_of(a, b, bad);
-      req[b] = r;
+      Request r = request_of(a, b, bad);
       int n = 0, u = 0;
       if (r.n > 0) {
+        r.tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
         u = (r.n * a.group + ROWS - 1) / ROWS * a.heads_kv;
-        n = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len).n * u;
+        n = r.tl.n * u;
       }
+      req[b] = r;
       tiles_pre[b + 1] = n;
       units_pre[b + 1] = u;
       nt += n;
@@ -360,10 +378,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       const int g = c0 + k + lane;
       const int b = last_not_above(tiles_pre, a.batch, g);
       const Request r = req[b];
-      const Tiles tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
       const int nrb = (r.n * a.group + ROWS - 1) / ROWS;
-      const int in = g - tiles_pre[b], u = in / tl.n;
-      const int hk = nrb == 1 ? u : u / nrb, key = tl.key_tile(in - u * tl.n) * TK;
+      const int in = g - tiles_pre[b], u = in / r.tl.n;
+      const int hk = nrb == 1 ? u : u / nrb, key = r.tl.key_tile(in - u * r.tl.n) * TK;
       const int32_t *table = a.block_table + b * a.table_stride + (key >> pshift);
       tok = key & (a.page - 1);
       const bool want0 = key < r.len, want1 = a.page == 16 && key + 16 < r.len;
@@ -427,7 +444,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     const Request rq = req[b];
     len = rq.len;
     p0 = len - rq.n;
-    tl = tiles_of<TK>(a, p0, len - 1, len);
+    tl = rq.tl;
     const int nrows_all = rq.n * a.group, nrb = (nrows_all + ROWS - 1) / ROWS;
     const int in = g - tiles_pre[b], u = in / tl.n;
     ut0 = in - u * tl.n;
@@ -442,7 +459,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     for (int n = 0; n < NT; ++n) {
       const int rr = 8 * n + gid, row = un.row0 + rr;
       if (rr < un.rows) {
-        const int qi = row / a.group;
+        const int qi = div_group(a, row);
         const uint16_t *src = static_cast<const uint16_t *>(a.q) +
                               static_cast<int64_t>(rq.t0 + qi) * a.q_st +
                               (un.hk * a.group + row - qi * a.group) * a.q_sh + H * 16 * tig;
@@ -455,7 +472,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = min(8 * n + 2 * tig + x, un.rows - 1) + un.row0;
-        hp[n][x] = a.head_param != nullptr ? a.head_param[un.hk * a.group + r % a.group] : 1.f;
+        hp[n][x] = a.head_param != nullptr
+                       ? a.head_param[un.hk * a.group + r - div_group(a, r) * a.group]
+                       : 1.f;
       }
     }
   };
@@ -469,8 +488,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   for (int k = 0; k < nk;) {
     // all rows of the unit see keys [lo_max, hi_min]; none sees one outside [lo_min, hi_max]
     int lo_min, lo_max, hi_min, hi_max;
-    band32(a, p0 + un.row0 / a.group, len, lo_min, hi_min);
-    band32(a, p0 + (un.row0 + un.rows - 1) / a.group, len, lo_max, hi_max);
+    band32(a, p0 + div_group(a, un.row0), len, lo_min, hi_min);
+    band32(a, p0 + div_group(a, un.row0 + un.rows - 1), len, lo_max, hi_max);
     const int pf = min(a.prefix, len);
 
     // Q as fragments: channels 16 (H tig + h) + 4 s .. + 3 of step (h, s)
@@ -508,7 +527,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       for (int x = 0; x < 2; ++x) {
         const float f = __shfl_sync(0xffffffffu, down, (2 * tig + x) * 4);
         const int r = min(8 * n + 2 * tig + x, un.rows - 1) + un.row0;
-        posn[n][x] = p0 + r / a.group;
+        posn[n][x] = p0 + div_group(a, r);
         real |= (8 * n + 2 * tig + x < un.rows ? 1u : 0u) << (2 * n + x);
         float mul = a.score_scale * f;
         slope[n][x] = 0.f;
@@ -629,7 +648,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                 const int j = j0 + 16 * m + 8 * x + gid;
                 const bool vis = ((real >> (2 * n + e)) & 1u) &&
                                  (j < pf || (j >= lo && j <= hi &&
-                                             (a.dil == 1 || (i_pos - j) % a.dil == 0)));
+                                             (a.dil == 1 || divides(a.dil, i_pos - j))));
                 if (!vis) s[m][n][2 * x + e] = SOFTMAX ? -INFINITY : 0.f;
               }
           }
@@ -739,7 +758,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               band32(a, i_pos, len, lo, hi);
               sees[n][e] = ((real >> (2 * n + e)) & 1u) &&
                            (j < pf || (j >= lo && j <= hi &&
-                                       (a.dil == 1 || (i_pos - j) % a.dil == 0)));
+                                       (a.dil == 1 || divides(a.dil, i_pos - j))));
             }
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
@@ -778,17 +797,22 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = 8 * n + 2 * tig + e;
+          const bool odd = gid & 1;
+          float f;
+          uint16_t *dst = row_out<KIND>(a, un, min(r, un.rows - 1), m_run[n][e], l_run[n][e],
+                                        gid == 0 && r < un.rows, f) +
+                          2 * (gid & ~1);
 #pragma unroll
-          for (int c = 0; c < MT; ++c) {
-            // lanes of even and odd gid exchange, so that each has four channels of a row
-            const float x0 = o[c][n][e], x1 = o[c][n][2 + e];
-            const float y0 = __shfl_xor_sync(0xffffffffu, x0, 4), y1 = __shfl_xor_sync(0xffffffffu, x1, 4);
-            if (((gid ^ c) & 1) == 0 && r < un.rows) {
-              if (gid & 1)
-                split_store<KIND>(a, un, r, 16 * c + 2 * (gid - 1), y0, y1, x0, x1, m_run[n][e],
-                                  l_run[n][e]);
+          for (int c = 0; c < MT; c += 2) {
+            // neighbours in gid exchange, so that each has four channels of a row:
+            // the even one of channel tile c, the odd one of the next
+            const float x0 = __shfl_xor_sync(0xffffffffu, odd ? o[c][n][e] : o[c + 1][n][e], 4);
+            const float x1 = __shfl_xor_sync(0xffffffffu, odd ? o[c][n][2 + e] : o[c + 1][n][2 + e], 4);
+            if (r < un.rows) {
+              if (odd)
+                store4(a, dst + 16 * (c + 1), f, x0, x1, o[c + 1][n][e], o[c + 1][n][2 + e]);
               else
-                split_store<KIND>(a, un, r, 16 * c + 2 * gid, x0, x1, y0, y1, m_run[n][e], l_run[n][e]);
+                store4(a, dst + 16 * c, f, o[c][n][e], o[c][n][2 + e], x0, x1);
             }
           }
         }
@@ -897,7 +921,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             *reinterpret_cast<const float4 *>(parts + (w * ROWS + r) * PITCH + 4 * c4), x[w].y);
     if (gr.last_is_head) add(acc, L, ptx::ex2(hml.x - (M == -INFINITY ? 0.f : M)), hv, hml.y);
     if (!gr.before && !gr.after) {
-      split_store<KIND>(a, un, r, 4 * c4, acc.x, acc.y, acc.z, acc.w, M, L);
+      float f;
+      uint16_t *dst = row_out<KIND>(a, un, r, M, L, c4 == 0, f);
+      store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
     } else {
       const int64_t slot = 2ll * blockIdx.x + (gr.before ? 0 : 1);
       *reinterpret_cast<float4 *>(a.part_o + (slot * ROWS + r) * D + 4 * c4) = acc;
@@ -928,13 +954,15 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll 4
       for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(a.part_ml + part(c) * 2));
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 4
       for (int c = first; c <= last; ++c) {
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part(c) * 2));
         const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part(c) * D + 4 * c4));
         add(acc, L, ptx::ex2(ml.x - (M == -INFINITY ? 0.f : M)), v, ml.y);
       }
-      split_store<KIND>(a, un, r, 4 * c4, acc.x, acc.y, acc.z, acc.w, M, L);
+      float f;
+      uint16_t *dst = row_out<KIND>(a, un, r, M, L, c4 == 0, f);
+      store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
     }
   }
 }
