@@ -174,6 +174,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
+// D (16x8, fp32) += A (16x16, halves) * B (16x8). Not volatile: the compiler may
+// interleave products with the conversions of the next operands.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 // 8x8 16-bit matrix, one row a quad of lanes: transposed
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t r;
@@ -573,11 +581,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       }
       // ---------------- S^T = K Q^T
       float s[2][NT][4];
+      uint4 kr[2][2][H];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
-        uint4 kr[2][H];
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int row = 16 * m + 8 * x + gid;
@@ -585,24 +591,44 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
           for (int h = 0; h < H; ++h) {
             const uint32_t ad = kst + row * D + (((H * tig + h) ^ sw) << 4);
+            uint4 &k4 = kr[m][x][h];
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(kr[x][h].x), "=r"(kr[x][h].y), "=r"(kr[x][h].z), "=r"(kr[x][h].w)
+                         : "=r"(k4.x), "=r"(k4.y), "=r"(k4.z), "=r"(k4.w)
                          : "r"(ad));
           }
         }
 #pragma unroll
-        for (int h = 0; h < H; ++h)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int st = 0; st < 4; ++st) {
+        for (int n = 0; n < NT; ++n) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {  // (two chains of products side by side)
             auto word = [&](const uint4 &v) { return st == 0 ? v.x : st == 1 ? v.y : st == 2 ? v.z : v.w; };
             uint32_t ka[4];
-            cache4_to_f16<CT>(word(kr[0][h]), ka[0], ka[2]);
-            cache4_to_f16<CT>(word(kr[1][h]), ka[1], ka[3]);
+            cache4_to_f16<CT>(word(kr[m][0][h]), ka[0], ka[2]);
+            cache4_to_f16<CT>(word(kr[m][1][h]), ka[1], ka[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-              mma16816<false>(s[m][n], ka, qf[n][h * 4 + st][0], qf[n][h * 4 + st][1]);
+              mma_f16(s[m][n], ka, qf[n][h * 4 + st][0], qf[n][h * 4 + st][1]);
           }
-      }
+      // V: the loads of the first VP parts of 16 keys go ahead of the softmax
+      constexpr int VP = NT == 1 ? 2 : 1;
+      uint32_t vr[2][MT / 2][4];
+      auto load_v = [&](int m) {
+#pragma unroll
+        for (int c = 0; c < MT; c += 2) {
+          const int key = 16 * m + (lane & 7) + ((lane >> 3) & 1) * 8, ch = c + (lane >> 4);
+          const int sw = D == 128 ? key & 7 : (key >> 1) & 3;
+          ldsm_x4_t(vst + key * D + ((ch ^ sw) << 4), vr[m][c / 2][0], vr[m][c / 2][1], vr[m][c / 2][2],
+                    vr[m][c / 2][3]);
+        }
+      };
+#pragma unroll
+      for (int m = 0; m < VP; ++m) load_v(m);
       // ---------------- score modification, mask, normaliser
       // s[m][n][2 x + e]: key j0 + 16 m + 8 x + gid, row 8 n + 2 tig + e
 #pragma unroll
@@ -718,31 +744,28 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       // ---------------- O^T += V^T P^T
       bool nan_seen = false;
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < 2; ++m) {
+        if (m + VP < 2) load_v(m + VP);
+        if (CT == CACHE_E4M3 && !all) {  // NaN times a P of zero is not zero
 #pragma unroll
-        for (int c = 0; c < MT; c += 2) {
-          const int key = 16 * m + (lane & 7) + ((lane >> 3) & 1) * 8, ch = c + (lane >> 4);
-          const int sw = D == 128 ? key & 7 : (key >> 1) & 3;
-          uint32_t v[4];
-          ldsm_x4_t(vst + key * D + ((ch ^ sw) << 4), v[0], v[1], v[2], v[3]);
+          for (int c = 0; c < MT / 2; ++c)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            if (CT == CACHE_E4M3 && !all) {  // NaN times a P of zero is not zero
-              const uint32_t nan = (((v[w] & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
+            for (int w = 0; w < 4; ++w) {
+              uint32_t &v = vr[m][c][w];
+              const uint32_t nan = (((v & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
               nan_seen |= nan != 0;
-              v[w] &= ~(nan * 0xffu);
+              v &= ~(nan * 0xffu);
             }
-            v[w] = __byte_perm(v[w], 0, 0x3120);
-          }
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            uint32_t va[4];
-            cache4_to_f16<CT>(v[2 * y], va[0], va[1]);
-            cache4_to_f16<CT>(v[2 * y + 1], va[2], va[3]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816<false>(o[c + y][n], va, pb[m][n][0], pb[m][n][1]);
-          }
         }
+#pragma unroll
+        for (int c = 0; c < MT; ++c) {
+          uint32_t va[4];
+          cache4_to_f16<CT>(__byte_perm(vr[m][c / 2][2 * (c & 1)], 0, 0x3120), va[0], va[1]);
+          cache4_to_f16<CT>(__byte_perm(vr[m][c / 2][2 * (c & 1) + 1], 0, 0x3120), va[2], va[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(o[c][n], va, pb[m][n][0], pb[m][n][1]);
+        }
+      }
       if (CT == CACHE_E4M3 && !all && __any_sync(0xffffffffu, nan_seen)) {
         // The NaN values left out above go to the rows that do see their keys.
         for (int kk = 0; kk < TK; ++kk) {
