@@ -64,7 +64,7 @@ __device__ __forceinline__ Scan2 block_scan2(Scan2 v, Scan2 &tot, Scan2 *warp_su
 __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const TablesArgs a) {
   __shared__ Scan2 sums[32];
   __shared__ int32_t s_cu[kTablesThreads + 1], s_len[kTablesThreads], s_first[kTablesThreads];
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, shift = 31 - __clz(a.page);
   const bool first_cta = blockIdx.x == 0;
   int head = a.free_state[0], count = a.free_state[1];
   if (head < 0 || head >= a.ring || count < 0 || count > a.ring) {
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
     count = 0;
   }
   long long pages0 = 0, tokens0 = 0;
-  long long taken = 0;  // pages handed out (thread 0's sum over the chunks)
+  int taken = 0;  // pages handed out, as far as this thread's requests know
   int bad = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kTablesThreads) {
     const int b = b0 + t;
@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
         add = 0;
       }
     }
-    const int held = (len + a.page - 1) / a.page;
-    int need = static_cast<int>((static_cast<long long>(len) + add + a.page - 1) / a.page) - held;
+    const int held = static_cast<int>((static_cast<long long>(len) + a.page - 1) >> shift);
+    int need = static_cast<int>((static_cast<long long>(len) + add + a.page - 1) >> shift) - held;
     const bool fits = static_cast<long long>(held) + need <= a.width;
     if (!fits) need = 0;
     Scan2 tot;
@@ -108,35 +108,37 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
       a.cu_q[b] = static_cast<int32_t>(cu);
       a.new_seq_lens[b] = served ? len + add : len;
     }
-    // pages handed out: the served requests with a need come first
-    Scan2 got;
-    block_scan2(Scan2{served ? need : 0, 0}, got, sums);
-    taken += got.a;
-    // (s_* are visible: block_scan2 ends with a barrier)
+    if (served && need > 0) taken = static_cast<int>(upto);  // (those served come first)
+    __syncthreads();
     const int n = min(kTablesThreads, a.batch - b0);
     const int c0 = s_cu[0], c1 = s_cu[kTablesThreads];
-    for (int tile = c0 / kTablesThreads; tile * kTablesThreads < c1; ++tile) {
-      if (tile % static_cast<int>(gridDim.x) != static_cast<int>(blockIdx.x)) continue;
+    // this CTA's tiles of kTablesThreads tokens: blockIdx.x, blockIdx.x + gridDim.x, ...
+    const int g = static_cast<int>(gridDim.x);
+    int tile = c0 / kTablesThreads;
+    tile += (static_cast<int>(blockIdx.x) + g - tile % g) % g;
+    for (; static_cast<long long>(tile) * kTablesThreads < c1; tile += g) {
       const int x = tile * kTablesThreads + t;
       if (x < c0 || x >= c1) continue;
       const int r = last_not_above(s_cu, n, x);
-      const int row = b0 + r, l = s_len[r], first = s_first[r];
+      const int l = s_len[r], first = s_first[r];
       const int pos = l + (x - s_cu[r]);
-      const int pg = pos / a.page, off = pos % a.page, hp = (l + a.page - 1) / a.page;
+      const int pg = pos >> shift, off = pos & (a.page - 1), hp = (l + a.page - 1) >> shift;
       int slot = -1;
       if (first >= 0) {
-        int32_t *entry = a.block_table + row * a.table_stride + pg;
+        int32_t *entry = a.block_table + (b0 + r) * a.table_stride + pg;
         int page;
         if (pg < hp) {
           page = *entry;
         } else {
-          page = a.free_pages[(static_cast<long long>(head) + first + (pg - hp)) % a.ring];
+          unsigned at = static_cast<unsigned>(head) + first + (pg - hp);  // < 2 ring
+          if (at >= static_cast<unsigned>(a.ring)) at -= a.ring;
+          page = a.free_pages[at];
           if (off == 0) *entry = page;
         }
-        if (page < 0 || page > 0x7fffffff / a.page - 1)
+        if (page < 0 || page > (0x7fffffff >> shift) - 1)
           bad |= kStatusBadIndex;
         else
-          slot = page * a.page + off;
+          slot = (page << shift) + off;
       }
       a.slots[x] = slot;
       a.positions[x] = pos;
@@ -151,10 +153,18 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
     a.slots[x] = -1;
     a.positions[x] = 0;
   }
-  if (first_cta && t == 0) {
-    a.cu_q[a.batch] = static_cast<int32_t>(tokens0 < 0x7fffffff ? tokens0 : 0x7fffffff);
-    a.new_free_state[0] = static_cast<int32_t>((head + taken) % a.ring);
-    a.new_free_state[1] = static_cast<int32_t>(count - taken);
+  if (first_cta) {
+    taken = __reduce_max_sync(0xffffffffu, taken);
+    if ((t & 31) == 0) s_first[t >> 5] = taken;
+    __syncthreads();
+    if (t < 32) {
+      taken = __reduce_max_sync(0xffffffffu, s_first[t]);
+      if (t == 0) {
+        a.cu_q[a.batch] = static_cast<int32_t>(tokens0 < 0x7fffffff ? tokens0 : 0x7fffffff);
+        a.new_free_state[0] = static_cast<int32_t>((static_cast<long long>(head) + taken) % a.ring);
+        a.new_free_state[1] = count - taken;
+      }
+    }
   }
   if (bad && (first_cta || (bad & kStatusBadIndex))) report(a.status, bad);
 }
@@ -230,74 +240,125 @@ struct AppendArgs {
   int64_t num_pages;
 };
 
-// One CTA a token, K/V head and K or V (blockIdx.z); only the CTA of the first
-// token of a page's run works, on the whole run.
-template <int D, bool BF16, int CT>
-__global__ void __launch_bounds__(128) cache_append_kernel(const AppendArgs a) {
-  __shared__ float s_max[4];
-  const int t0 = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  const int slot0 = a.slots[t0];
-  if (slot0 < 0) return;
-  const int page = slot0 / a.page;
-  if (page >= a.num_pages) {
-    if (tid == 0 && h == 0 && blockIdx.z == 0) report(a.status, kStatusBadIndex);
-    return;
+// A page's tokens for one K/V head, K or V: 128 threads hold them in registers
+// (16 bytes a load, all loads in flight at once), so the input is read once:
+// the largest value decides the scale, then the values are rounded and stored.
+// Bound by HBM: 2 bytes in and 1 out for each value. A CTA looks at `window`
+// tokens and works on the runs of tokens of one page that begin there: a page's
+// worth for prompts, one for decode steps, so that their few runs spread out.
+template <int D, bool BF16, int CT, int IT>
+__global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(const AppendArgs a, int window) {
+  constexpr int LANES = D / 8;       // threads of a row: 16 bytes each
+  constexpr int STEP = 128 / LANES;  // rows of one load of the CTA
+  constexpr int PAGE = IT * STEP;    // page_size
+  constexpr int SHIFT = PAGE == 16 ? 4 : PAGE == 32 ? 5 : PAGE == 64 ? 6 : 7;
+  __shared__ float s_max[2][4];
+  __shared__ int s_slot[2 * PAGE + 1];  // from the token before the window on
+  __shared__ unsigned s_same[2][4], s_first[2][4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kinds = 2 * a.heads_kv;
+  const int which = blockIdx.x % kinds, h = which >> 1;
+  const bool is_v = which & 1;
+  const int w0 = static_cast<int>(blockIdx.x / kinds) * window;
+  const int w1 = min(w0 + window, a.tokens);
+  const uint16_t *src = static_cast<const uint16_t *>(is_v ? a.v : a.k) + h * (is_v ? a.v_sh : a.k_sh) +
+                        (tid % LANES) * 8;
+  const int64_t st = is_v ? a.v_st : a.k_st;
+  for (int e = tid; e < window + PAGE; e += 128) {  // (a run that begins in the window ends here)
+    const int x = w0 - 1 + e;
+    s_slot[e] = x >= 0 && x < a.tokens ? a.slots[x] : -1;
   }
-  if (t0 > 0) {
-    const int before = a.slots[t0 - 1];
-    if (before >= 0 && before / a.page == page) return;
-  }
-  const uint16_t *src = static_cast<const uint16_t *>(blockIdx.z ? a.v : a.k) +
-                        h * (blockIdx.z ? a.v_sh : a.k_sh);
-  const int64_t st = blockIdx.z ? a.v_st : a.k_st;
-  const int64_t ph = static_cast<int64_t>(page) * a.heads_kv + h;
-  uint8_t *dst = (blockIdx.z ? a.v_cache : a.k_cache) + ph * a.page * D;
-  float *scale = (blockIdx.z ? a.v_scale : a.k_scale) + ph;
-  int n = 0;
-  bool fresh = false;
-  while (n < a.page && t0 + n < a.tokens) {
-    const int s = a.slots[t0 + n];
-    if (s < 0 || s / a.page != page) break;
-    fresh |= s % a.page == 0;
-    ++n;
-  }
-  float mx = 0.f;
-  for (int e = tid; e < n * (D / 2); e += 128) {
-    const int r = e / (D / 2), c = e % (D / 2);
-    const float2 x = in16x2_to_float2<BF16>(
-        *reinterpret_cast<const uint32_t *>(src + (t0 + r) * st + 2 * c));
-    const float u = fabsf(x.x), w = fabsf(x.y);
-    if (u <= 3.4028235e38f) mx = fmaxf(mx, u);
-    if (w <= 3.4028235e38f) mx = fmaxf(mx, w);
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-  if ((tid & 31) == 0) s_max[tid >> 5] = mx;
-  const float old = *scale;
   __syncthreads();
-  mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  float sc = pow2f(scale_exp<CT>(mx));
-  if (!fresh) sc = fmaxf(sc, old);
-  const float inv = 1.f / sc;
-  if (!fresh && sc != old) {  // the page's values in the larger scale
-    const float ratio = old * inv;
-    for (int e = tid; e < a.page * D / 4; e += 128) {
-      uint32_t *p = reinterpret_cast<uint32_t *>(dst) + e;
-      uint32_t p01, p23;
-      cache4_to_f16<CT>(*p, p01, p23);
-      const float2 x = f16x2_to_float2(p01), y = f16x2_to_float2(p23);
-      *p = to_cache4<CT>(x.x * ratio, x.y * ratio, y.x * ratio, y.y * ratio);
+  int par = 0;
+  for (int t0 = w0; t0 < w1; par ^= 1) {
+    const int at = t0 - w0 + 1, slot0 = s_slot[at];
+    if (slot0 < 0) {  // skipped
+      ++t0;
+      continue;
     }
+    // the run: the following tokens in the same page
+    const int page = slot0 >> SHIFT;
+    const int mine = tid < PAGE && at + tid < window + PAGE ? s_slot[at + tid] : -1;
+    const bool in = mine >= 0 && (mine >> SHIFT) == page;
+    const unsigned same = __ballot_sync(0xffffffffu, in);
+    const unsigned first = __ballot_sync(0xffffffffu, in && (mine & (PAGE - 1)) == 0);
+    if (lane == 0) s_same[par][warp] = same, s_first[par][warp] = first;
     __syncthreads();
-  }
-  if (tid == 0) *scale = sc;
-  for (int e = tid; e < n * (D / 4); e += 128) {
-    const int r = e / (D / 4), c = e % (D / 4);
-    const uint2 raw = *reinterpret_cast<const uint2 *>(src + (t0 + r) * st + 4 * c);
-    const float2 x = in16x2_to_float2<BF16>(raw.x), y = in16x2_to_float2<BF16>(raw.y);
-    const int off = a.slots[t0 + r] % a.page;
-    *reinterpret_cast<uint32_t *>(dst + off * D + 4 * c) =
-        to_cache4<CT>(x.x * inv, x.y * inv, y.x * inv, y.y * inv);
+    int n = 0;
+    bool fresh = false;  // it holds the page's first slot
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (n == 32 * w) {
+        const unsigned gap = ~s_same[par][w];
+        const int here = gap == 0 ? 32 : __ffs(gap) - 1;
+        n += here;
+        fresh |= here > 0 && (s_first[par][w] << (32 - here)) != 0;
+      }
+    const int before = s_slot[at - 1];
+    const bool begun = before >= 0 && (before >> SHIFT) == page;  // in an earlier window
+    if (begun || page >= a.num_pages) {
+      if (!begun && tid == 0 && which == 0) report(a.status, kStatusBadIndex);
+      t0 += n;
+      continue;
+    }
+    const int64_t ph = static_cast<int64_t>(page) * a.heads_kv + h;
+    uint8_t *dst = (is_v ? a.v_cache : a.k_cache) + ph * PAGE * D;
+    float *scale = (is_v ? a.v_scale : a.k_scale) + ph;
+    uint4 x[IT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = i * STEP + tid / LANES;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (r < n) x[i] = *reinterpret_cast<const uint4 *>(src + (t0 + r) * st);
+    }
+    const float old = *scale;
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = in16x2_to_float2<BF16>(w[j]);
+        const float u = fabsf(f.x), v = fabsf(f.y);  // (infinities and NaN do not count)
+        mx = fmaxf(mx, fmaxf(u <= 3.4028235e38f ? u : 0.f, v <= 3.4028235e38f ? v : 0.f));
+      }
+    }
+    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));  // (not negative)
+    if (lane == 0) s_max[par][warp] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_max[par][0], s_max[par][1]), fmaxf(s_max[par][2], s_max[par][3]));
+    float sc = pow2f(scale_exp<CT>(mx));
+    if (!fresh) sc = fmaxf(sc, old);
+    const float inv = 1.f / sc;
+    if (!fresh && sc != old) {  // the page's values in the larger scale
+      const float ratio = old * inv;
+      for (int e = tid; e < PAGE * D / 16; e += 128) {
+        uint4 *p = reinterpret_cast<uint4 *>(dst) + e;
+        uint4 v = *p;
+        auto again = [&](uint32_t w) {
+          uint32_t p01, p23;
+          cache4_to_f16<CT>(w, p01, p23);
+          const float2 f = f16x2_to_float2(p01), g = f16x2_to_float2(p23);
+          return to_cache4<CT>(f.x * ratio, f.y * ratio, g.x * ratio, g.y * ratio);
+        };
+        v.x = again(v.x), v.y = again(v.y), v.z = again(v.z), v.w = again(v.w);
+        *p = v;
+      }
+      __syncthreads();
+    }
+    if (tid == 0 && (fresh || sc != old)) *scale = sc;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = i * STEP + tid / LANES;
+      if (r < n) {
+        const float2 f0 = in16x2_to_float2<BF16>(x[i].x), f1 = in16x2_to_float2<BF16>(x[i].y);
+        const float2 f2 = in16x2_to_float2<BF16>(x[i].z), f3 = in16x2_to_float2<BF16>(x[i].w);
+        *reinterpret_cast<uint2 *>(dst + (s_slot[at + r] & (PAGE - 1)) * D + (tid % LANES) * 8) =
+            make_uint2(to_cache4<CT>(f0.x * inv, f0.y * inv, f1.x * inv, f1.y * inv),
+                       to_cache4<CT>(f2.x * inv, f2.y * inv, f3.x * inv, f3.y * inv));
+      }
+    }
+    t0 += n;
   }
 }
 

@@ -111,10 +111,23 @@ int check_append(const chia_append_params_t *p) {
   return CHIA_OK;
 }
 
+// Tokens that a CTA of the append looks at: a page's, or as many fewer as give
+// every SM eight CTAs.
 template <int D, bool BF16, int CT>
-int launch_append(const chia::AppendArgs &a, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads_kv), 2);
-  chia::cache_append_kernel<D, BF16, CT><<<grid, 128, 0, s>>>(a);
+int launch_append(const chia::AppendArgs &a, int sms, cudaStream_t s) {
+  const int64_t kinds = 2ll * a.heads_kv;
+  int window = a.page;
+  while (window > 1 && (a.tokens + window - 1) / window * kinds < 8 * sms) window /= 2;
+  const int64_t grid = (a.tokens + window - 1) / window * kinds;
+  if (grid > kI32) return CHIA_ERR_UNSUPPORTED;
+  const unsigned g = static_cast<unsigned>(grid);
+  switch (a.page * D / 1024) {
+    case 1: chia::cache_append_kernel<64, BF16, CT, 1><<<g, 128, 0, s>>>(a, window); break;
+    case 2: chia::cache_append_kernel<D, BF16, CT, 2><<<g, 128, 0, s>>>(a, window); break;
+    case 4: chia::cache_append_kernel<D, BF16, CT, 4><<<g, 128, 0, s>>>(a, window); break;
+    case 8: chia::cache_append_kernel<D, BF16, CT, 8><<<g, 128, 0, s>>>(a, window); break;
+    default: chia::cache_append_kernel<128, BF16, CT, 16><<<g, 128, 0, s>>>(a, window); break;
+  }
   return launched();
 }
 
@@ -280,7 +293,7 @@ int chia_cache_append(const chia_append_params_t *p, void *stream) {
   a.heads_kv = p->heads_kv;
   a.page = p->page_size;
   a.num_pages = p->num_pages;
-  return CHIA_BY_TYPE(p, launch_append, a, static_cast<cudaStream_t>(stream));
+  return CHIA_BY_TYPE(p, launch_append, a, sms, static_cast<cudaStream_t>(stream));
 }
 
 int64_t chia_paged_attn_workspace_bytes(const chia_paged_params_t *p) {
