@@ -364,8 +364,8 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   a.drain_ns = kDefaultTimeoutNs;
   const int kind = kind_of(p);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  for (int64_t b = 0; b < p->batch; b += chia::kSplitMaxBatch) {
-    const int64_t n = p->batch - b < chia::kSplitMaxBatch ? p->batch - b : chia::kSplitMaxBatch;
+  for (int64_t b = 0; b < p->batch; b += chia::kLineBatch) {
+    const int64_t n = p->batch - b < chia::kLineBatch ? p->batch - b : chia::kLineBatch;
     a.batch = static_cast<int32_t>(n);
     a.seq_lens = p->seq_lens + b;
     a.cu_q = p->cu_q != nullptr ? p->cu_q + b : nullptr;

@@ -31,149 +31,16 @@
 // are, and its sum takes the scale out again. Sigmoid and ReLU divide by a
 // running power of two instead.
 #pragma once
-#include <cuda.h>
-#include <cuda_runtime.h>
-
-#include <atomic>
-
 #include "decode_sm100.cuh"
-#include "paged_common.cuh"
+#include "paged_line_sm100.cuh"
 
 namespace chia {
 
-struct PagedArgs {
-  const void *q;
-  void *o;
-  int64_t q_st, q_sh, o_st, o_sh;  // element strides: token, head
-  const float *k_scale, *v_scale;
-  const int32_t *block_table, *seq_lens, *cu_q;
-  int64_t table_stride;
-  float *lse;
-  const float *head_param;
-  int32_t left, right, block, prefix, dil;  // the mask, on positions (at most 2^30 each)
-  float score_scale, softcap, sig_bias, out_scale;
-  int32_t heads, heads_kv, group, batch, tokens, page, width;
-  uint32_t group_magic;  // ceil(2^32 / group); 0: a group of one
-  int32_t num_pages;
-  int32_t q_each;     // queries of a request where cu_q is null
-  int32_t token0;     // first token of request 0 where cu_q is null
-  int32_t bf16;       // type of q and o
-  int32_t *tickets;   // [gridDim.x], zero between launches
-  float *part_o;      // [10 gridDim.x][rows][D]: two parts a CTA, then one a worker
-  float *part_ml;     // [10 gridDim.x][rows][2]
-  int32_t *status;
-  uint64_t timeout_ns, drain_ns;
-};
-
-constexpr int kSplitMaxBatch = 512;  // requests of one launch (they are held in shared memory)
 constexpr int kSplitWarps = 8;
 constexpr int kSplitThreads = 32 * kSplitWarps;
-constexpr int kUnitCost = 4;   // what a unit costs beside its tiles, in tiles
-constexpr int kWholeUnit = 64; // units of up to this cost are not cut between CTAs
+constexpr int kUnitCost = 4;    // what a unit costs beside its tiles, in tiles
+constexpr int kWholeUnit = 64;  // units of up to this cost are not cut between CTAs
 
-// Tiles of TK keys that queries at positions [p0, p1] visit: `pre` tiles from
-// key 0 on, then those from `lo` on; `n` in all, at least one (a unit whose
-// rows see nothing still writes zeros).
-struct Tiles {
-  int pre, lo, n;
-  __device__ __forceinline__ int key_tile(int t) const { return t < pre ? t : lo + (t - pre); }
-};
-// Queries and keys of request b, checked: [t0, t0 + n) of q, keys [0, len).
-struct Request {
-  int t0, n, len;
-  Tiles tl;
-};
-__device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &bad) {
-  Request r;
-  if (a.cu_q != nullptr) {
-    r.t0 = a.cu_q[b];
-    const int t1 = a.cu_q[b + 1];
-    if (r.t0 < 0 || t1 < r.t0 || t1 > a.tokens) {
-      bad = true;
-      r.t0 = r.n = 0;
-    } else {
-      r.n = t1 - r.t0;
-    }
-  } else {
-    r.t0 = a.token0 + b * a.q_each;
-    r.n = a.q_each;
-  }
-  r.len = a.seq_lens[b];
-  const int most = a.width * a.page;
-  if (r.len < 0 || r.len > most) {
-    bad = true;
-    r.len = r.len < 0 ? 0 : most;
-  }
-  return r;
-}
-
-// The rare divisions stand in functions of their own: a call that needs none
-// of them fetches the less code, and its first pass over the code is most of
-// the time of a small call.
-static __device__ __noinline__ int block_start(int i, int block) {
-  return (i >= 0 ? i / block : -((-i + block - 1) / block)) * block;
-}
-static __device__ __noinline__ bool divides(int d, int x) { return x % d == 0; }
-// x / group for x * group < 2^32
-__device__ __forceinline__ int div_group(const PagedArgs &a, int x) {
-  return a.group_magic == 0 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), a.group_magic));
-}
-
-// The keys position i sees beside the prefix (position_band in 32 bits).
-__device__ __forceinline__ void band32(const PagedArgs &a, int i, int len, int &lo, int &hi) {
-  lo = 0;
-  hi = len - 1;
-  if (a.left >= 0) lo = max(lo, i - a.left);
-  if (a.right >= 0) hi = min(hi, i + a.right);
-  if (a.block > 0) {
-    const int b0 = block_start(i, a.block);
-    lo = max(lo, b0);
-    hi = min(hi, b0 + a.block - 1);
-  }
-}
-
-template <int TK>
-__device__ __forceinline__ Tiles tiles_of(const PagedArgs &a, int p0, int p1, int len) {
-  Tiles r;
-  int lo, hi, x;
-  band32(a, p0, len, lo, x);
-  band32(a, p1, len, x, hi);
-  const int pf = min(a.prefix, len);
-  r.pre = (pf + TK - 1) / TK;
-  r.lo = r.pre;
-  int n = r.pre;
-  if (lo <= hi) {
-    r.lo = max(lo / TK, r.pre);
-    n += max(0, hi / TK + 1 - r.lo);
-  }
-  r.n = max(n, 1);
-  return r;
-}
-
-// A wait of limited length. After one has run out (`abort`), all return at once.
-__device__ __forceinline__ bool split_wait(uint32_t bar, uint32_t parity, volatile int *abort,
-                                           const PagedArgs &a) {
-  if (ptx::mbar_test_wait(bar, parity)) return true;
-  const uint64_t t0 = ptx::globaltimer_ns();
-  while (!ptx::mbar_try_wait(bar, parity, 20000u)) {
-    if (*abort) return false;
-    if (ptx::globaltimer_ns() - t0 > a.timeout_ns) {
-      *abort = 1;
-      report(a.status, 5);  // CHIA_ERR_DEVICE_TIMEOUT
-      return false;
-    }
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar,
-                                            int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
 // D (16x8, fp32) += A (16x16, halves) * B (16x8). Not volatile: the compiler may
 // interleave products with the conversions of the next operands.
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -202,37 +69,6 @@ struct SplitConfig {
   static_assert(kSplitWarps * ROWS * PITCH * 4 <= RING, "the parts fit the spent ring");
 };
 
-// A unit: rows [row0, row0 + rows) of a request's queries with one K/V head.
-struct Unit {
-  int t0, row0, rows, hk;  // first token of the request
-  int cost;                // where it begins in the line, in cost
-  int n;                   // its tiles
-};
-
-// Where a row's output goes, and what it is multiplied by; `lse`: its log-sum-exp is written here too.
-template <int KIND>
-__device__ __forceinline__ uint16_t *row_out(const PagedArgs &a, const Unit &u, int r, float M, float L,
-                                             bool lse, float &f) {
-  constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
-  f = 1.f;
-  if (SOFTMAX) f = L > 0.f ? 1.f / L : L;  // (a NaN stays)
-  if (KIND == KIND_RELU) f = a.out_scale * ptx::ex2(M);
-  if (KIND == KIND_SIGMOID) f = ptx::ex2(M);
-  const int qi = div_group(a, u.row0 + r), hh = u.hk * a.group + u.row0 + r - qi * a.group;
-  const int64_t tok = u.t0 + qi;
-  if (SOFTMAX && a.lse != nullptr && lse)
-    a.lse[tok * a.heads + hh] =
-        L > 0.f ? (M + __log2f(L)) * 0.6931471805599453f : L == 0.f ? -INFINITY : L;
-  return static_cast<uint16_t *>(a.o) + tok * a.o_st + hh * a.o_sh;
-}
-__device__ __forceinline__ void store4(const PagedArgs &a, uint16_t *dst, float f, float x0, float x1,
-                                       float x2, float x3) {
-  x0 *= f, x1 *= f, x2 *= f, x3 *= f;
-  *reinterpret_cast<uint2 *>(dst) =
-      a.bf16 ? make_uint2(ptx::pack_bf16(x0, x1), ptx::pack_bf16(x2, x3))
-             : make_uint2(ptx::pack_f16(x0, x1), ptx::pack_f16(x2, x3));
-}
-
 // KIND: score modification and normaliser.
 template <int D, int CT, int NT, int KIND>
 __global__ void __launch_bounds__(kSplitThreads, 1)
@@ -247,9 +83,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   extern __shared__ uint8_t dyn[];
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
   float *parts = reinterpret_cast<float *>(sm);  // [warps][ROWS][PITCH], in the spent ring
-  __shared__ int tiles_pre[kSplitMaxBatch + 1], units_pre[kSplitMaxBatch + 1];
-  __shared__ Request req[kSplitMaxBatch];
-  __shared__ int wsum[kSplitWarps][2];
+  using L = Line<TK, ROWS, kSplitThreads, kUnitCost, kWholeUnit>;
+  __shared__ typename L::Shared line_sm;
   __shared__ __align__(8) uint64_t bars[kSplitWarps * NST];
   __shared__ float part_ml[kSplitWarps][ROWS][2];
   __shared__ Unit s_head[kSplitWarps], s_end[kSplitWarps];
@@ -278,95 +113,16 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     ptx::tma_prefetch_desc(&mv);
   }
 
-  // ---- the line: tiles and units before each request
-  {
-    const int per = (a.batch + kSplitThreads - 1) / kSplitThreads;
-    const int b0 = t * per, b1 = min(a.batch, b0 + per);
-    int nt = 0, nu = 0;
-    bool bad = false;
-    for (int b = b0; b < b1; ++b) {
-      Request r = request_of(a, b, bad);
-      int n = 0, u = 0;
-      if (r.n > 0) {
-        r.tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
-        u = (r.n * a.group + ROWS - 1) / ROWS * a.heads_kv;
-        n = r.tl.n * u;
-      }
-      req[b] = r;
-      tiles_pre[b + 1] = n;
-      units_pre[b + 1] = u;
-      nt += n;
-      nu += u;
-    }
-    if (bad && blockIdx.x == 0) report(a.status, kStatusBadIndex);
-    int it = nt, iu = nu;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, it, d), y = __shfl_up_sync(0xffffffffu, iu, d);
-      if (lane >= d) it += x, iu += y;
-    }
-    if (lane == 31) wsum[warp][0] = it, wsum[warp][1] = iu;
-    ptx::fence_barrier_init();
-    __syncthreads();
-    it -= nt, iu -= nu;
-    for (int w = 0; w < warp; ++w) it += wsum[w][0], iu += wsum[w][1];
-    for (int b = b0; b < b1; ++b) {
-      it += tiles_pre[b + 1], iu += units_pre[b + 1];
-      tiles_pre[b + 1] = it, units_pre[b + 1] = iu;
-    }
-    if (t == 0) tiles_pre[0] = units_pre[0] = 0;
-    __syncthreads();
-  }
-  auto cost_before = [&](int b) { return tiles_pre[b] + kUnitCost * units_pre[b]; };
-  const int total = cost_before(a.batch);
-  const int ctas = min(static_cast<int>(gridDim.x), (total + kSplitWarps - 1) / kSplitWarps);
-  if (blockIdx.x >= ctas) return;
-  // Border c of the CTAs' pieces: total * c / ctas in cost, moved to the nearer
-  // end of the unit that it cuts where the unit is short: a cut costs a round
-  // of the workspace (some 4 us), whole units wait for nobody.
-  const int step = total / ctas, rest = total % ctas;
-  auto even = [&](int c) { return step * c + rest * c / ctas; };
-  auto place = [&](int x, bool snap, int &tile) {  // cost x, as a cost and as a tile
-    if (x >= total) {
-      tile = tiles_pre[a.batch];
-      return total;
-    }
-    int lo = 0, hi = a.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cost_before(mid) <= x)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    const int units = units_pre[lo + 1] - units_pre[lo];
-    const int n = (tiles_pre[lo + 1] - tiles_pre[lo]) / units, cost = n + kUnitCost;
-    int in = x - cost_before(lo), u = in / cost;
-    in -= u * cost;
-    if (snap && cost <= kWholeUnit) {
-      u += 2 * in >= cost ? 1 : 0;
-      in = 0;
-    }
-    // (a border within the cost of a unit's own counts as its first tile)
-    tile = tiles_pre[lo] + u * n + max(0, in - kUnitCost);
-    return cost_before(lo) + u * cost + in;
-  };
-  // the CTA that has tile k of a unit that is cut: the last with a border not above it
-  auto cta_of = [&](const Unit &u, int k) {
-    const int x = u.cost + kUnitCost + k;
-    int c = static_cast<int>(static_cast<float>(x) / static_cast<float>(total) * ctas);
-    c = max(0, min(ctas - 1, c));
-    while (c + 1 < ctas && even(c + 1) <= x) ++c;
-    while (even(c) > x) --c;
-    return c;
-  };
+  ptx::fence_barrier_init();
+  const L line(line_sm, a, kSplitWarps);  // (its barriers also order the set-up above)
+  if (static_cast<int>(blockIdx.x) >= line.ctas) return;
   const int me = blockIdx.x * kSplitWarps + warp;
   int c0, nk;  // first tile and number of tiles of this worker
   {
     int tile;  // lane 0: this border, lane 1: the next one
-    const int y = place(even(blockIdx.x + (lane & 1)), true, tile);
+    const int y = line.place(line.even(blockIdx.x + (lane & 1)), true, tile);
     const int y0 = __shfl_sync(0xffffffffu, y, 0), y1 = __shfl_sync(0xffffffffu, y, 1);
-    place(y0 + static_cast<int>(static_cast<long long>(y1 - y0) * (warp + (lane & 1)) / kSplitWarps),
+    line.place(y0 + static_cast<int>(static_cast<long long>(y1 - y0) * (warp + (lane & 1)) / kSplitWarps),
           false, tile);
     c0 = __shfl_sync(0xffffffffu, tile, 0);
     nk = __shfl_sync(0xffffffffu, tile, 1) - c0;
@@ -384,11 +140,10 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     row0 = row1 = -1;
     if (k + lane < nk) {
       const int g = c0 + k + lane;
-      const int b = last_not_above(tiles_pre, a.batch, g);
-      const Request r = req[b];
-      const int nrb = (r.n * a.group + ROWS - 1) / ROWS;
-      const int in = g - tiles_pre[b], u = in / r.tl.n;
-      const int hk = nrb == 1 ? u : u / nrb, key = r.tl.key_tile(in - u * r.tl.n) * TK;
+      const int b = line.request_at(g);
+      const Request r = line_sm.req[b];
+      int ut;
+      const int hk = line.unit_at(g, b, r, ut).hk, key = r.tl.key_tile(ut) * TK;
       const int32_t *table = a.block_table + b * a.table_stride + (key >> pshift);
       tok = key & (a.page - 1);
       const bool want0 = key < r.len, want1 = a.page == 16 && key + 16 < r.len;
@@ -448,21 +203,13 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   uint4 raw[NT][H * 2];  // row 8 n + gid, channels 16 H tig .. + 16 H - 1
   float hp[NT][2];       // of rows 8 n + 2 tig + e, as in the columns of S^T
   auto begin_unit = [&](int k) {
-    const int g = c0 + k, b = last_not_above(tiles_pre, a.batch, g);
-    const Request rq = req[b];
+    const int g = c0 + k, b = line.request_at(g);
+    const Request rq = line_sm.req[b];
     len = rq.len;
     p0 = len - rq.n;
     tl = rq.tl;
-    const int nrows_all = rq.n * a.group, nrb = (nrows_all + ROWS - 1) / ROWS;
-    const int in = g - tiles_pre[b], u = in / tl.n;
-    ut0 = in - u * tl.n;
+    un = line.unit_at(g, b, rq, ut0);
     nt = min(tl.n - ut0, nk - k);
-    un.t0 = rq.t0;
-    un.hk = nrb == 1 ? u : u / nrb;
-    un.row0 = (u - un.hk * nrb) * ROWS;
-    un.rows = min(ROWS, nrows_all - un.row0);
-    un.cost = cost_before(b) + u * (tl.n + kUnitCost);
-    un.n = tl.n;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int rr = 8 * n + gid, row = un.row0 + rr;
@@ -557,13 +304,13 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 
     for (int i = 0; i < nt && !aborted; ++i) {
       const int kk = k + i, stage = kk % NST;
-      if (!split_wait(bar0 + 8 * stage, (kk / NST) & 1, &abort_flag, a)) {
+      if (!paged_wait(bar0 + 8 * stage, (kk / NST) & 1, &abort_flag, a)) {
         // leave no copy in flight: the ring's memory is used again, and the CTA may exit
         PagedArgs d = a;
         d.timeout_ns = a.drain_ns;
         int none = 0;
         for (int j = kk; j < min(nk, kk + NST); ++j)
-          split_wait(bar0 + 8 * (j % NST), (j / NST) & 1, &none, d);
+          paged_wait(bar0 + 8 * (j % NST), (j / NST) & 1, &none, d);
         aborted = true;
         break;
       }
@@ -959,7 +706,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   __syncthreads();
   if (t < 2 && (t == 0 ? s_group[0].before : s_group[groups - 1].after && !s_group[groups - 1].before)) {
     const Unit &un = unit_of(s_group[t == 0 ? 0 : groups - 1]);
-    const unsigned first = cta_of(un, 0), parts_less_1 = cta_of(un, un.n - 1) - first;
+    const unsigned first = line.cta_of(un, 0), parts_less_1 = line.cta_of(un, un.n - 1) - first;
     __threadfence();  // (the CTA's parts, seen through the barrier, before the ticket)
     // counts the unit's CTAs and wraps to zero
     s_last[t] = atomicInc(reinterpret_cast<unsigned *>(a.tickets) + first, parts_less_1) == parts_less_1;
@@ -969,7 +716,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   for (int x = 0; x < 2; ++x) {
     if (!s_last[x]) continue;
     const Unit &un = unit_of(s_group[x == 0 ? 0 : groups - 1]);
-    const int first = cta_of(un, 0), last = cta_of(un, un.n - 1);
+    const int first = line.cta_of(un, 0), last = line.cta_of(un, un.n - 1);
     for (int e = t; e < un.rows * (D / 4); e += kSplitThreads) {
       const int r = e / (D / 4), c4 = e % (D / 4);
       auto part = [&](int c) { return (2ll * c + (c == first ? 1 : 0)) * ROWS + r; };
@@ -994,16 +741,6 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 template <int D, int CT>
 cudaError_t launch_split(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a, int kind,
                          int tiles, int grid, int device, cudaStream_t s);
-
-// Once for each kernel and device.
-inline cudaError_t allow_smem(const void *kernel, int bytes, int device, std::atomic<uint64_t> &set) {
-  const uint64_t bit = 1ull << (device & 63);
-  if (device < 64 && (set.load(std::memory_order_acquire) & bit)) return cudaSuccess;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) set.fetch_or(bit, std::memory_order_release);
-  return e;
-}
 
 template <int D, int CT, int NT, int KIND>
 cudaError_t launch_split_one(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
