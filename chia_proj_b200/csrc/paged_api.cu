@@ -12,6 +12,7 @@
 #include "../../include/chia_paged.h"
 #include "cache_sm100.cuh"
 #include "paged_split_sm100.cuh"
+#include "paged_tiled_sm100.cuh"
 
 namespace {
 
@@ -182,27 +183,35 @@ int kind_of(const chia_paged_params_t *p) {
   }
 }
 
-// Workspace: the tickets, then the parts of two units a CTA and of one a worker.
+// Which kernel, and the workspace: the tickets, then the parts of two units a
+// CTA and (split kernel) of one a worker.
 constexpr int64_t kTicketBytes = 4096;
+// Rows of a K/V head from which the tiled kernel is the faster one.
+constexpr int64_t kTiledRows = 65;
 struct SplitPlan {
-  int tiles;  // rows of a unit: 8 (as many as most groups of heads have) or 16
+  bool tiled;
+  int tiles;  // split kernel: rows of a unit, 8 (as many as most groups of heads have) or 16
+  int rows;   // of a unit
   int grid;   // one CTA an SM
-  int64_t off_ml, bytes;
+  int64_t off_ml, off_cuts, bytes;
 };
 int split_plan(const chia_paged_params_t *p, int sms, SplitPlan &pl) {
   const int64_t group = p->heads / p->heads_kv;
+  pl.tiled = p->max_q * group >= kTiledRows;
   pl.tiles = p->max_q * group <= 8 ? 1 : 2;
+  pl.rows = pl.tiled ? chia::TiledConfig<128>::ROWS : 8 * pl.tiles;
   pl.grid = sms;
   // the line of tiles is counted in 32 bits
-  const int64_t rows = 8 * pl.tiles;
-  const double line = static_cast<double>(p->heads_kv) * (p->tokens * group / rows + p->batch + 1) *
-                      (p->table_width * p->page_size / 32 + 2 + chia::kUnitCost);
+  const int tk = pl.tiled ? 128 : 32;
+  const double line = static_cast<double>(p->heads_kv) * (p->tokens * group / pl.rows + p->batch + 1) *
+                      (p->table_width * p->page_size / tk + 2 + chia::kUnitCost);
   if (pl.grid * 4 > kTicketBytes || p->tokens * p->heads > kI32 ||
       p->tokens * group * group > 2 * kI32 || line > kI32)
     return CHIA_ERR_UNSUPPORTED;
-  const int64_t slots = (2 + chia::kSplitWarps) * pl.grid * rows;
+  const int64_t slots = (2 + (pl.tiled ? 0 : chia::kSplitWarps)) * static_cast<int64_t>(pl.grid) * pl.rows;
   pl.off_ml = kTicketBytes + slots * p->head_dim * 4;
-  pl.bytes = (pl.off_ml + slots * 8 + 255) / 256 * 256;
+  pl.off_cuts = (pl.off_ml + slots * 8 + 255) / 256 * 256;
+  pl.bytes = pl.off_cuts + (pl.tiled ? (pl.grid * sizeof(chia::CutUnit) + 255) / 256 * 256 : 0);
   return CHIA_OK;
 }
 
@@ -221,8 +230,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // A cache as (head_dim, page_size, pages * heads) bytes; a box is `rows` tokens
-// of one page and head, swizzled over their own width.
-bool encode_cache(CUtensorMap *map, const void *base, const chia_paged_params_t *p, int rows) {
+// of one page and head, swizzled over their own width or as they are.
+bool encode_cache(CUtensorMap *map, const void *base, const chia_paged_params_t *p, int rows,
+                  bool swizzle) {
   auto fn = encode_fn();
   if (fn == nullptr) return false;
   const cuuint64_t D = p->head_dim, P = p->page_size;
@@ -232,7 +242,8 @@ bool encode_cache(CUtensorMap *map, const void *base, const chia_paged_params_t 
   const cuuint32_t elem[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, elem,
             CU_TENSOR_MAP_INTERLEAVE_NONE,
-            D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE
+            : D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -320,8 +331,9 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   if (p->workspace_bytes < pl.bytes) return CHIA_ERR_INVALID_ARGUMENT;
   if (p->tokens == 0) return CHIA_OK;
   CUtensorMap mk, mv;
-  const int box = p->page_size < 32 ? p->page_size : 32;
-  if (!encode_cache(&mk, p->k_cache, p, box) || !encode_cache(&mv, p->v_cache, p, box))
+  const int most = pl.tiled ? 128 : 32, box = p->page_size < most ? p->page_size : most;
+  if (!encode_cache(&mk, p->k_cache, p, box, !pl.tiled) ||
+      !encode_cache(&mv, p->v_cache, p, box, !pl.tiled))
     return CHIA_ERR_LAUNCH;
   chia::PagedArgs a{};
   a.q = p->q;
@@ -371,14 +383,16 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
     a.cu_q = p->cu_q != nullptr ? p->cu_q + b : nullptr;
     a.token0 = static_cast<int32_t>(b * a.q_each);
     a.block_table = p->block_table + b * p->table_stride;
+    const uint8_t *v8 = static_cast<const uint8_t *>(p->v_cache);
+#define CHIA_LAUNCH(D, CT)                                                                   \
+  (pl.tiled ? chia::launch_tiled<D, CT>(mk, mv, a, v8, ws + pl.off_cuts, kind, pl.grid, dev, s)                \
+            : chia::launch_split<D, CT>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s))
+    const bool e4m3 = p->cache_dtype == CHIA_CACHE_E4M3;
     const cudaError_t e =
         p->head_dim == 128
-            ? (p->cache_dtype == CHIA_CACHE_E4M3
-                   ? chia::launch_split<128, chia::CACHE_E4M3>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s)
-                   : chia::launch_split<128, chia::CACHE_INT8>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s))
-            : (p->cache_dtype == CHIA_CACHE_E4M3
-                   ? chia::launch_split<64, chia::CACHE_E4M3>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s)
-                   : chia::launch_split<64, chia::CACHE_INT8>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s));
+            ? (e4m3 ? CHIA_LAUNCH(128, chia::CACHE_E4M3) : CHIA_LAUNCH(128, chia::CACHE_INT8))
+            : (e4m3 ? CHIA_LAUNCH(64, chia::CACHE_E4M3) : CHIA_LAUNCH(64, chia::CACHE_INT8));
+#undef CHIA_LAUNCH
     if (e != cudaSuccess) return CHIA_ERR_LAUNCH;
   }
   return CHIA_OK;

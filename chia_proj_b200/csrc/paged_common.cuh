@@ -6,7 +6,6 @@
 
 #include <cstdint>
 
-#include "mask_geom.cuh"
 #include "ptx.cuh"
 
 namespace chia {
@@ -92,19 +91,15 @@ __device__ __forceinline__ float2 in16x2_to_float2(uint32_t v) {
   return f16x2_to_float2(v);
 }
 
-// Band of the keys that the query at position i sees, beside the prefix:
-// row_band() for positions, which may be negative (a request with more
-// queries than keys); keys run from 0 to len - 1.
-CHIA_HD void position_band(const MaskGeom &g, int64_t i, int64_t len, int64_t &lo, int64_t &hi) {
-  lo = 0;
-  hi = len - 1;
-  if (g.left >= 0) lo = imax64(lo, i - g.left);
-  if (g.right >= 0) hi = imin64(hi, i + g.right);
-  if (g.block > 0) {
-    const int64_t b0 = (i >= 0 ? i / g.block : -((-i + g.block - 1) / g.block)) * g.block;
-    lo = imax64(lo, b0);
-    hi = imin64(hi, b0 + g.block - 1);
-  }
+// A value scale as the attention kernels use it: for the softmax kinds its
+// logarithm, exact for a power of two and at least -100 (a scale of zero).
+template <bool SOFTMAX>
+__device__ __forceinline__ float value_factor(float v) {
+  if (!SOFTMAX) return v;
+  const uint32_t b = __float_as_uint(v);
+  if (v < 7.9e-31f) return -100.f;
+  return (b & 0x7fffffu) == 0 && b < 0x7f800000u ? static_cast<float>(static_cast<int>(b >> 23) - 127)
+                                                 : __log2f(v);
 }
 
 // Largest r in [0, n) with off[r] <= x (off rises, off[0] <= x).

@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "fmha_sm100.cuh"
 #include "paged_common.cuh"
@@ -90,7 +91,8 @@ __device__ __forceinline__ int div_group(const PagedArgs &a, int x) {
   return a.group_magic == 0 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), a.group_magic));
 }
 
-// The keys position i sees beside the prefix (position_band in 32 bits).
+// The keys that the query at position i sees beside the prefix, of keys 0 to
+// len - 1; a position may be negative (a request with more queries than keys).
 __device__ __forceinline__ void band32(const PagedArgs &a, int i, int len, int &lo, int &hi) {
   lo = 0;
   hi = len - 1;

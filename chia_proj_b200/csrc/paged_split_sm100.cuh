@@ -27,7 +27,7 @@
 // to [2^14, 2^15) by a power of two per row, is a half exactly down to 2^-29
 // of its row's largest value; so products lose nothing. P is rounded to a half
 // (11 bits) with its page's value scale in it: the softmax's running maximum is
-// that of s + log2(scale), so the largest P of a row is 1 whatever the scales
+// that of s + log2(scale), so the largest P of a row is 2^15 whatever the scales
 // are, and its sum takes the scale out again. Sigmoid and ReLU divide by a
 // running power of two instead.
 #pragma once
@@ -38,6 +38,9 @@ namespace chia {
 
 constexpr int kSplitWarps = 8;
 constexpr int kSplitThreads = 32 * kSplitWarps;
+// The largest P is 2^kPTop: a half keeps 11 bits of a P down to 2^-14, so of one
+// that is 2^-29 of its row's largest.
+constexpr float kPTop = 15.f;
 constexpr int kUnitCost = 4;    // what a unit costs beside its tiles, in tiles
 constexpr int kWholeUnit = 64;  // units of up to this cost are not cut between CTAs
 
@@ -154,22 +157,13 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       if (!ok0 || !ok1) report(a.status, kStatusBadIndex);
     }
   };
-  // A value scale as it is used: for the softmax kinds its logarithm, exact for
-  // a power of two and at least -100 (a scale of zero).
-  auto v_factor = [](float v) {
-    if (!SOFTMAX) return v;
-    const uint32_t b = __float_as_uint(v);
-    if (v < 7.9e-31f) return -100.f;
-    return (b & 0x7fffffu) == 0 && b < 0x7f800000u ? static_cast<float>(static_cast<int>(b >> 23) - 127)
-                                                   : __log2f(v);
-  };
   auto look_up_scales = [&](int k) {  // of the same tiles, to shared memory
     float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row0 >= 0) sc.x = a.k_scale[row0], sc.y = v_factor(a.v_scale[row0]);
+    if (row0 >= 0) sc.x = a.k_scale[row0], sc.y = value_factor<SOFTMAX>(a.v_scale[row0]);
     if (a.page != 16)
       sc.z = sc.x, sc.w = sc.y;
     else if (row1 >= 0)
-      sc.z = a.k_scale[row1], sc.w = v_factor(a.v_scale[row1]);
+      sc.z = a.k_scale[row1], sc.w = value_factor<SOFTMAX>(a.v_scale[row1]);
     scales[(k + lane) % C::SCALES] = sc;  // (those of 64 tiles ago are long used)
     __syncwarp();
   };
@@ -298,7 +292,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int c = 0; c < MT; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
-      m_run[n][0] = m_run[n][1] = SOFTMAX ? -INFINITY : -120.f;
+      m_run[n][0] = m_run[n][1] = SOFTMAX ? -INFINITY : -100.f;
       l_run[n][0] = l_run[n][1] = 0.f;
     }
 
@@ -464,7 +458,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float mu = m_run[n][e] == -INFINITY ? 0.f : m_run[n][e];
+          const float mu = m_run[n][e] == -INFINITY ? 0.f : m_run[n][e] - kPTop;
           const float down = SOFTMAX ? 0.f : ptx::ex2(-mu);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
@@ -561,6 +555,10 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1)
           l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], d);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m_run[n][e] -= kPTop;  // what O and the sum are relative to
     if (begun && ended) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)

@@ -1,0 +1,712 @@
+// paged_tiled_sm100.cuh -- attention of many queries over the paged 8-bit K/V
+// cache: chunked prefill, on the 5th-generation tensor cores.
+//
+// A unit is up to 256 rows (queries x the heads of a group) of a request with
+// one K/V head, as two query tiles of 128 rows; keys come in tiles of 128. With
+// hundreds of rows to a key the work is bound by the tensor cores and the
+// exponentials, and the conversion of the cache to halves, done once for both
+// query tiles, hides behind them. One CTA an SM takes an equal piece of the
+// line of tiles; units that are cut leave parts in the workspace, which a small
+// kernel behind this one merges with the whole GPU.
+//
+//   warps 0-3, 4-7  softmax of query tile 0 and 1, a thread a row
+//   warp 8          issues the UMMAs, warp 9 looks up pages and loads by TMA
+//   warps 12-15     convert 8-bit tiles to halves
+//
+// Tensor memory: S0 S1 (128 columns each; P, in halves, takes the first 64 of
+// its S), O0 O1. Shared memory: Q0 Q1 | a ring of converted K and V tiles, all
+// in the 128-byte swizzle | a ring of 8-bit tiles as TMA brings them.
+//
+// The UMMAs of a CTA execute in the order of their issue, so S_w(t + 1) is
+// issued right behind PV_w(t), which reads P out of S_w's columns, and its
+// completion also says that O_w may be rescaled. The two query tiles take
+// turns: while one's products run, the other's exponentials do.
+//
+// Numbers as in the split kernel: Q times a power of two per row and the
+// cache's values are halves exactly; a key scale multiplies the scores of its
+// 16 columns, the logarithm of a value scale is part of the running maximum.
+#pragma once
+#include "paged_line_sm100.cuh"
+
+namespace chia {
+
+constexpr int kTiledThreads = 512;
+constexpr float kTiledPTop = 7.f;  // P is 2^7 at the running maximum, and at most 2^15 (a half's range)
+constexpr int kTiledCost = 1;   // what a unit costs beside its tiles of 128 keys
+constexpr int kTiledWhole = 6;  // units of up to this cost are not cut between CTAs
+constexpr int kTiledPiece = 6;  // the least cost of a piece: a part is 128 KB to write and to read
+
+template <int D>
+struct TiledConfig {
+  static constexpr int ROWS = 256;           // rows of a unit
+  static constexpr int TK = 128;             // keys of a tile
+  static constexpr int Q_TILE = 128 * D * 2;
+  static constexpr int CHUNK = 128 * 128;    // 64 channels of a tile's 128 rows
+  static constexpr int KV = TK * D * 2;      // a converted K or V tile
+  static constexpr int SLOTS = 3 * (128 / D);
+  static constexpr int STAGE = TK * D;       // an 8-bit one
+  static constexpr int STAGES = 2 * (128 / D);
+  static constexpr int SETS = 8;             // tiles whose scales are held
+  static constexpr int OFF_KV = 2 * Q_TILE;
+  static constexpr int OFF_ST = OFF_KV + SLOTS * KV;
+  static constexpr int OFF_SC = OFF_ST + STAGES * STAGE;
+  static constexpr int SMEM = 1024 + OFF_SC + SETS * 8 * 16;
+  // registers a thread: 512 threads begin with 128
+  static constexpr int REG_SOFTMAX = 184, REG_OTHER = 72;
+  static_assert(256 * REG_SOFTMAX + 256 * REG_OTHER == 65536, "register split");
+};
+
+// A unit that a CTA begins and later ones, up to `last`, go on with; rows 0: none.
+struct CutUnit {
+  Unit un;
+  int last;
+};
+
+// Merges the parts of the units that are cut: CTA (c, y) rows 16 y .. + 15 of the
+// unit that CTA c of the tiled kernel began, its parts in the order of the line.
+template <int D, int KIND>
+__global__ void __launch_bounds__(128) paged_merge_kernel(const PagedArgs a, const CutUnit *cuts) {
+  constexpr int ROWS = TiledConfig<D>::ROWS;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the tiled kernel is complete
+  const int first = blockIdx.x;
+  const CutUnit cu = cuts[first];
+  const int r1 = min(cu.un.rows, 16 * (static_cast<int>(blockIdx.y) + 1));
+  for (int e = 16 * blockIdx.y * (D / 4) + threadIdx.x; e < r1 * (D / 4); e += 128) {
+    const int r = e / (D / 4), c4 = e % (D / 4);
+    auto part = [&](int c) { return (2ll * c + (c == first ? 1 : 0)) * ROWS + r; };
+    float M = -INFINITY, L = 0.f;
+#pragma unroll 4
+    for (int c = first; c <= cu.last; ++c) M = fmaxf(M, __ldcg(a.part_ml + part(c) * 2));
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = first; c <= cu.last; ++c) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part(c) * 2));
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part(c) * D + 4 * c4));
+      const float wt = ptx::ex2(ml.x - (M == -INFINITY ? 0.f : M));
+      L = fmaf(wt, ml.y, L);
+      acc.x = fmaf(wt, v.x, acc.x);
+      acc.y = fmaf(wt, v.y, acc.y);
+      acc.z = fmaf(wt, v.z, acc.z);
+      acc.w = fmaf(wt, v.w, acc.w);
+    }
+    float f;
+    uint16_t *dst = row_out<KIND>(a, cu.un, r, M, L, c4 == 0, f);
+    store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
+  }
+}
+
+// Channels (bits) in which a visible key of tiles [t0, t1) of the unit holds
+// NaN, where the tile is not visible as a whole: the converters leave NaN out
+// of such tiles, since a P of zero would spread it to rows that do not see it.
+template <int D>
+__device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_cache, int b, int hk,
+                                          const Tiles &tl, int t0, int t1, int i, int len, int lo_max,
+                                          int hi_min, uint32_t *mask) {
+  int lo, hi;
+  band32(a, i, len, lo, hi);
+  const int pf = min(a.prefix, len);
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = tl.key_tile(t) * 128;
+    if ((a.dil == 1 && j0 >= lo_max && j0 + 127 <= hi_min) || j0 + 128 <= pf) continue;
+    for (int j = j0; j < min(j0 + 128, len); ++j) {
+      if (!(j < pf || (j >= lo && j <= hi && (a.dil == 1 || divides(a.dil, i - j))))) continue;
+      const int pg = a.block_table[b * a.table_stride + j / a.page];
+      if (pg < 0 || pg >= a.num_pages) continue;
+      const uint8_t *v = v_cache + ((static_cast<int64_t>(pg) * a.heads_kv + hk) * a.page + j % a.page) * D;
+      for (int c = 0; c < D; ++c)
+        if ((v[c] & 0x7f) == 0x7f) mask[c / 32] |= 1u << (c % 32);
+    }
+  }
+}
+
+template <int D, int CT, int KIND>
+__global__ void __launch_bounds__(kTiledThreads, 1)
+paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                   const PagedArgs a, const uint8_t *v_cache, CutUnit *cuts) {
+  using C = TiledConfig<D>;
+  constexpr int TK = C::TK, ROWS = C::ROWS, SLOTS = C::SLOTS, STAGES = C::STAGES, SETS = C::SETS;
+  constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
+  constexpr float LOG2E = 1.4426950408889634f;
+  using L = Line<TK, ROWS, kTiledThreads, kTiledCost, kTiledWhole>;
+  extern __shared__ uint8_t dyn[];
+  uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
+  const uint32_t sb = ptx::smem_u32(sm);
+  float4 *scales = reinterpret_cast<float4 *>(sm + C::OFF_SC);  // [SETS][8]: ks, value factor, its inverse
+  __shared__ typename L::Shared line_sm;
+  // st_full st_empty | kv_full kv_empty | q s p o o_empty (2 each) | scales | drain
+  enum { ST_FULL = 0, ST_EMPTY = ST_FULL + STAGES, KV_FULL = ST_EMPTY + STAGES, KV_EMPTY = KV_FULL + SLOTS,
+         Q_FULL = KV_EMPTY + SLOTS, S_FULL = Q_FULL + 2, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2,
+         O_EMPTY = O_FULL + 2, SC_FULL = O_EMPTY + 2, DRAIN = SC_FULL + SETS, BARS = DRAIN + 1 };
+  __shared__ __align__(8) uint64_t bars[BARS];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag, nan_flag;
+  __shared__ int tile_full[SETS];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  auto bar = [&](int i) { return ptx::smem_u32(bars) + 8 * i; };
+  if (t == 0) {
+    for (int i = 0; i < BARS; ++i) {
+      const bool four = (i >= ST_EMPTY && i < KV_EMPTY) || (i >= Q_FULL && i < S_FULL) ||
+                        (i >= P_FULL && i < O_FULL) || (i >= O_EMPTY && i < SC_FULL);
+      ptx::mbar_init(bar(i), four ? 4 : 1);
+    }
+    abort_flag = nan_flag = 0;
+    ptx::tma_prefetch_desc(&mk);
+    ptx::tma_prefetch_desc(&mv);
+  }
+  ptx::fence_barrier_init();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the merge waits for all of this)
+  const L line(line_sm, a, kTiledPiece);
+  if (static_cast<int>(blockIdx.x) >= line.ctas) {
+    if (t == 0) cuts[blockIdx.x].un.rows = 0;
+    return;
+  }
+  int c0, nk;  // this CTA's tiles
+  {
+    int tile;
+    line.place(line.even(blockIdx.x + (lane & 1)), true, tile);
+    c0 = __shfl_sync(0xffffffffu, tile, 0);
+    nk = __shfl_sync(0xffffffffu, tile, 1) - c0;
+  }
+  if (warp == 8) {
+    ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto wait = [&](int i, uint32_t parity) { return paged_wait(bar(i), parity, &abort_flag, a); };
+
+  // the unit of this CTA's tile k
+  struct Here {
+    Unit un;
+    Request rq;
+    int b, ut0, nt, p0, lo_max, hi_min;
+  };
+  auto unit_at = [&](int k) {
+    Here h;
+    h.b = line.request_at(c0 + k);
+    h.rq = line_sm.req[h.b];
+    h.un = line.unit_at(c0 + k, h.b, h.rq, h.ut0);
+    h.nt = min(h.un.n - h.ut0, nk - k);
+    h.p0 = h.rq.len - h.rq.n;
+    int x;
+    band32(a, h.p0 + div_group(a, h.un.row0), h.rq.len, x, h.hi_min);
+    band32(a, h.p0 + div_group(a, h.un.row0 + h.un.rows - 1), h.rq.len, h.lo_max, x);
+    return h;
+  };
+  auto sees_all = [&](const Here &h, int j0) {  // every row of the unit sees keys [j0, j0 + TK)
+    return (a.dil == 1 && j0 >= h.lo_max && j0 + TK - 1 <= h.hi_min) ||
+           j0 + TK <= min(a.prefix, h.rq.len);
+  };
+
+  if (warp >= 8) {
+    ptx::setmaxnreg_dec<C::REG_OTHER>();
+    if (warp == 9) {
+      // ==================================================== pages and TMA
+      const int pshift = 31 - __clz(a.page), rows = min(a.page, TK);
+      // Of the tile's keys 16 lane .. + 15 (lanes 0-7). What a tile needs from
+      // memory is asked for a tile or two ahead and looked at when its turn
+      // comes: the page of tile k + 2, the scales of tile k + 1.
+      struct Keys {
+        int key, pg;  // pg: -1 where there is nothing to load
+        int hk, all;
+      };
+      Here h;
+      int left = 0, lo_min = 0, hi_max = 0;  // tiles of the unit still to look up
+      auto page_of = [&](int k) {
+        Keys x{0, -1, 0, 0};
+        if (k >= nk) return x;
+        if (left == 0) {
+          h = unit_at(k), left = h.nt;
+          int y;
+          band32(a, h.p0 + div_group(a, h.un.row0), h.rq.len, lo_min, y);
+          band32(a, h.p0 + div_group(a, h.un.row0 + h.un.rows - 1), h.rq.len, y, hi_max);
+        }
+        const int j0 = h.rq.tl.key_tile(h.ut0 + h.nt - left) * TK;
+        --left;
+        x.key = j0 + 16 * lane;
+        x.hk = h.un.hk;
+        x.all = sees_all(h, j0);
+        // (the scales of 16 keys that no row sees may be anything)
+        if (!(x.key < min(a.prefix, h.rq.len) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
+        if (lane < 8 && x.key < h.rq.len) x.pg = a.block_table[h.b * a.table_stride + (x.key >> pshift)];
+        return x;
+      };
+      int issued = 0;
+      Keys k1 = page_of(0);
+      int row1 = -1, row = -1;
+      float ks1 = 0.f, vs1 = 0.f, ks = 0.f, vs = 0.f;
+      auto scales_of = [&](const Keys &x) {
+        row1 = -1;
+        if (x.pg >= 0 && x.pg < a.num_pages) {
+          row1 = x.pg * a.heads_kv + x.hk;
+          ks1 = a.k_scale[row1];
+          vs1 = a.v_scale[row1];
+        }
+      };
+      scales_of(k1);
+      Keys k2 = page_of(1);
+      for (int k = 0; k < nk; ++k) {
+        const Keys now = k1;
+        row = row1, ks = ks1, vs = vs1;
+        if (row < 0 && (now.pg != -1)) report(a.status, kStatusBadIndex);
+        if (lane < 8) {
+          float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (row >= 0 && !(now.all & 2)) {
+            sc.x = ks;
+            sc.y = value_factor<SOFTMAX>(vs);
+            sc.z = SOFTMAX ? ptx::ex2(-sc.y) : 0.f;
+          }
+          scales[(k % SETS) * 8 + lane] = sc;
+        }
+        if (lane == 0) tile_full[k % SETS] = now.all & 1;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(SC_FULL + k % SETS));
+        k1 = k2;
+        scales_of(k1);
+        k2 = page_of(k + 2);
+        const bool leads = lane < 8 && row >= 0 && (16 * lane) % rows == 0;
+        const int bytes = __popc(__ballot_sync(0xffffffffu, leads)) * rows * D;
+        bool ok = true;
+        for (int v = 0; v < 2 && ok; ++v) {
+          const int item = 2 * k + v, st = item % STAGES;
+          ok = __all_sync(0xffffffffu, wait(ST_EMPTY + st, ((item / STAGES) & 1) ^ 1));
+          if (!ok) break;
+          if (lane == 0) ptx::mbar_arrive_expect_tx(bar(ST_FULL + st), bytes);
+          __syncwarp();
+          if (leads)
+            tma_load_3d(sb + C::OFF_ST + st * C::STAGE + 16 * lane * D, v ? &mv : &mk, bar(ST_FULL + st), 0,
+                        now.key & (a.page - 1), row);
+          ++issued;
+        }
+        if (!ok) break;
+      }
+      // no copy is in flight when the CTA exits
+      PagedArgs d = a;
+      d.timeout_ns = a.drain_ns;
+      int none = 0;
+      for (int i = max(0, issued - STAGES); i < issued; ++i)
+        paged_wait(bar(ST_FULL + i % STAGES), (i / STAGES) & 1, &none, d);
+    } else if (warp == 8) {
+      // ==================================================== UMMA issue
+      constexpr uint32_t IDESC_QK = ptx::make_idesc_f16(128, 128, false, false, false);
+      constexpr uint32_t IDESC_PV = ptx::make_idesc_f16(128, D, false, false, true);
+      const uint64_t dq = ptx::make_sdesc_sw128(sb, 16, 1024);
+      const uint64_t dk = ptx::make_sdesc_sw128(sb + C::OFF_KV, 16, 1024);
+      const uint64_t dv = ptx::make_sdesc_sw128(sb + C::OFF_KV, C::CHUNK, 1024);
+      auto issue_s = [&](int w, int slot) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * C::CHUNK + (kk & 3) * 32) >> 4;
+          ptx::umma_ss_warp(tmem + w * 128, dq + ((w * C::Q_TILE) >> 4) + off,
+                            dk + ((slot * C::KV) >> 4) + off, IDESC_QK, kk > 0 ? 1u : 0u);
+        }
+        ptx::umma_commit_warp(bar(S_FULL + w));
+      };
+      auto issue_pv = [&](int w, int slot, bool first) {
+#pragma unroll
+        for (int kk = 0; kk < TK / 16; ++kk)
+          ptx::umma_ts_warp(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
+                            dv + ((slot * C::KV + kk * 2048) >> 4), IDESC_PV, first && kk == 0 ? 0u : 1u);
+      };
+      auto all_wait = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, wait(i, parity)); };
+      uint32_t tiles[2] = {0, 0}, units[2] = {0, 0};
+      bool ok = true;
+      for (int k = 0; k < nk && ok;) {
+        const Here h = unit_at(k);
+        const int act = h.un.rows > 128 ? 2 : 1;
+        for (int w = 0; w < act && ok; ++w) ok = all_wait(Q_FULL + w, units[w] & 1);
+        int item = 2 * k;
+        ok = ok && all_wait(KV_FULL + item % SLOTS, (item / SLOTS) & 1);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        for (int w = 0; w < act; ++w) issue_s(w, item % SLOTS);
+        ptx::umma_commit_warp(bar(KV_EMPTY + item % SLOTS));
+        for (int i = 0; i < h.nt && ok; ++i) {
+          const int vi = 2 * (k + i) + 1, ki = vi + 1;
+          ok = all_wait(KV_FULL + vi % SLOTS, (vi / SLOTS) & 1);
+          for (int w = 0; w < act && ok; ++w) {
+            ok = all_wait(P_FULL + w, tiles[w] & 1);
+            if (ok && i == 0 && units[w] > 0) ok = all_wait(O_EMPTY + w, (units[w] - 1) & 1);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            issue_pv(w, vi % SLOTS, i == 0);
+            ++tiles[w];
+            if (i == h.nt - 1) ptx::umma_commit_warp(bar(O_FULL + w));
+            if (w == act - 1) ptx::umma_commit_warp(bar(KV_EMPTY + vi % SLOTS));
+            if (i + 1 < h.nt) {
+              if (w == 0) {
+                ok = all_wait(KV_FULL + ki % SLOTS, (ki / SLOTS) & 1);
+                if (!ok) break;
+                ptx::tc_fence_after();
+              }
+              issue_s(w, ki % SLOTS);
+              if (w == act - 1) ptx::umma_commit_warp(bar(KV_EMPTY + ki % SLOTS));
+            }
+          }
+        }
+        for (int w = 0; w < act; ++w) ++units[w];
+        k += h.nt;
+      }
+      // all UMMAs are complete before tensor memory is freed
+      ptx::umma_commit_warp(bar(DRAIN));
+      PagedArgs d = a;
+      d.timeout_ns = a.drain_ns;
+      int none = 0;
+      paged_wait(bar(DRAIN), 0, &none, d);
+    } else if (warp >= 12) {
+      // ==================================================== conversion
+      const int c = t - 384;
+      for (int item = 0; item < 2 * nk; ++item) {
+        const int st = item % STAGES, sl = item % SLOTS;
+        if (!wait(ST_FULL + st, (item / STAGES) & 1)) break;
+        if (!wait(KV_EMPTY + sl, ((item / SLOTS) & 1) ^ 1)) break;
+        const bool sift = CT == CACHE_E4M3 && (item & 1) && !tile_full[(item / 2) % SETS];
+        bool nan_seen = false;
+        constexpr int PER = TK * D / 16 / 128;  // 16-byte pieces a thread
+        uint4 all[PER];
+#pragma unroll
+        for (int x = 0; x < PER; ++x)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(all[x].x), "=r"(all[x].y), "=r"(all[x].z), "=r"(all[x].w)
+                       : "r"(sb + C::OFF_ST + st * C::STAGE + (x * 128 + c) * 16));
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          const int piece = x * 128 + c, row = piece / (D / 16), v = piece % (D / 16);
+          uint4 q = all[x];
+          if (sift) {
+            auto clean = [&](uint32_t &w) {
+              const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
+              nan_seen |= nan != 0;
+              w &= ~(nan * 0xffu);
+            };
+            clean(q.x), clean(q.y), clean(q.z), clean(q.w);
+          }
+          uint32_t h[8];
+          cache4_to_f16<CT>(q.x, h[0], h[1]);
+          cache4_to_f16<CT>(q.y, h[2], h[3]);
+          cache4_to_f16<CT>(q.z, h[4], h[5]);
+          cache4_to_f16<CT>(q.w, h[6], h[7]);
+          // channels 16 v .. + 15: units 2 v, 2 v + 1 of the row, four pieces a
+          // chunk; lanes of different chunks store in opposite order, so that
+          // eight lanes' stores fall into different banks
+          const uint32_t base = sb + C::OFF_KV + sl * C::KV + (v / 4) * C::CHUNK + row * 128;
+          const int u = 2 * (v % 4), sw = row & 7, flip = D == 128 ? v / 4 : 0;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const bool hi = (y ^ flip) != 0;
+            ptx::st_shared_v4(base + (((u + (hi ? 1 : 0)) ^ sw) << 4), hi ? h[4] : h[0], hi ? h[5] : h[1],
+                              hi ? h[6] : h[2], hi ? h[7] : h[3]);
+          }
+        }
+        if (sift && nan_seen) nan_flag = 1;
+        ptx::fence_proxy_async_smem();  // the UMMAs read what was stored
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(bar(KV_FULL + sl));
+          ptx::mbar_arrive(bar(ST_EMPTY + st));
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    ptx::setmaxnreg_inc<C::REG_SOFTMAX>();
+    // ======================================================= softmax
+    const int w = warp >> 2, row = t & 127, rsw = row & 7;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_off + w * 128, tO = tmem + lane_off + 256 + w * 128;
+    uint32_t cnt = 0, units = 0;
+    bool ok = true;
+    if (t == 0) cuts[blockIdx.x].un.rows = 0;
+    for (int k = 0; k < nk && ok;) {
+      const Here h = unit_at(k);
+      const bool begun = h.ut0 == 0, ended = h.ut0 + h.nt == h.un.n, whole = begun && ended;
+      const int64_t slot = 2ll * blockIdx.x + (begun ? 1 : 0);
+      const int r = w * 128 + row;  // row of the unit
+      const bool real = r < h.un.rows;
+      if (h.un.rows > w * 128) {
+        const int rr = h.un.row0 + min(r, h.un.rows - 1);
+        const int qi = div_group(a, rr), head = h.un.hk * a.group + rr - qi * a.group;
+        const int pos = h.p0 + qi;
+        // ---- the row of Q, as halves
+        float rowmul;
+        {
+          const uint16_t *src = static_cast<const uint16_t *>(a.q) +
+                                static_cast<int64_t>(h.un.t0 + qi) * a.q_st + head * a.q_sh;
+          uint4 raw[D / 8];
+          float mx = 0.f;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            raw[c] = real ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+          auto two = [&](uint32_t v) {
+            return a.bf16 ? in16x2_to_float2<true>(v) : in16x2_to_float2<false>(v);
+          };
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float2 f = two(v[y]);
+              mx = ptx::max3(mx, fabsf(f.x), fabsf(f.y));
+            }
+          }
+          int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+          e = max(-100, min(127, e));
+          const float up = pow2f(14 - e);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float2 f = two(v[y]);
+              o[y] = ptx::pack_f16(f.x * up, f.y * up);
+            }
+            ptx::st_shared_v4(sb + w * C::Q_TILE + (c / 8) * C::CHUNK + row * 128 + (((c % 8) ^ rsw) << 4),
+                              o[0], o[1], o[2], o[3]);
+          }
+          rowmul = a.score_scale * pow2f(e - 14);
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(Q_FULL + w));
+        }
+        const float hp = a.head_param != nullptr ? a.head_param[head] : 1.f;
+        float slope = 0.f;
+        if (KIND == KIND_SOFTMAX) rowmul *= LOG2E * hp;
+        if (KIND == KIND_SOFTCAP) rowmul *= 2.f * LOG2E / a.softcap;
+        if (KIND == KIND_ALIBI) rowmul *= LOG2E, slope = hp * LOG2E;
+        if (KIND == KIND_SIGMOID) rowmul *= -LOG2E;
+        int lo, hi;
+        band32(a, pos, h.rq.len, lo, hi);
+        const int pf = min(a.prefix, h.rq.len);
+        const bool none = lo > hi;
+        float m_run = SOFTMAX ? -INFINITY : -100.f, l_run = 0.f;
+        for (int i = 0; i < h.nt; ++i, ++cnt) {
+          const int n = k + i;
+          if (!wait(SC_FULL + n % SETS, (n / SETS) & 1) || !wait(S_FULL + w, cnt & 1)) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          uint32_t sr[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ptx::tmem_ld32(tS + c * 32, sr[c]);
+          const int j0 = h.rq.tl.key_tile(h.ut0 + i) * TK;
+          const float4 *sc = scales + (n % SETS) * 8;
+          const bool all = sees_all(h, j0);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ptx::reg_fence(sr[c]);
+          RowMask rm;
+          rm.c_lo = none ? (1 << 30) : lo - j0;
+          rm.span = none ? 0u : static_cast<uint32_t>(hi - lo);
+          rm.c_pre = real ? pf - j0 : 0;
+          rm.i_rel = pos - j0;
+          rm.dil = a.dil;
+          const float rel = static_cast<float>(j0 - pos);
+          float mx = SOFTMAX ? -INFINITY : 0.f;
+          auto pass1 = [&](auto mode) {
+            constexpr int MODE = decltype(mode)::value;
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              const float4 s4 = sc[g];
+              const float f = rowmul * s4.x;
+              const uint64_t F2 = ptx::f2(f, f), V2 = ptx::f2(s4.y, s4.y);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const int col = 16 * g + e;
+                uint32_t &ra = sr[g / 2][(g & 1) * 16 + e], &rb = sr[g / 2][(g & 1) * 16 + e + 1];
+                uint64_t x2 = ptx::f2(__uint_as_float(ra), __uint_as_float(rb));
+                float x, y;
+                if (KIND == KIND_SOFTCAP) {
+                  ptx::f2_split(ptx::mul2(x2, F2), x, y);
+                  x = fmaf(a.softcap * LOG2E, fmaf(-2.f, ptx::rcp_fast(ptx::ex2(x) + 1.f), 1.f), s4.y);
+                  y = fmaf(a.softcap * LOG2E, fmaf(-2.f, ptx::rcp_fast(ptx::ex2(y) + 1.f), 1.f), s4.y);
+                } else if (KIND == KIND_SIGMOID) {
+                  const float bias = -a.sig_bias * LOG2E;
+                  ptx::f2_split(ptx::fma2(x2, F2, ptx::f2(bias, bias)), x, y);
+                  x = s4.y * ptx::rcp_fast(1.f + ptx::ex2(x));
+                  y = s4.y * ptx::rcp_fast(1.f + ptx::ex2(y));
+                } else if (KIND == KIND_RELU) {
+                  ptx::f2_split(ptx::mul2(x2, F2), x, y);
+                  x = x < 0.f ? 0.f : x * s4.y;
+                  y = y < 0.f ? 0.f : y * s4.y;
+                } else {
+                  x2 = ptx::fma2(x2, F2, V2);
+                  if (KIND == KIND_ALIBI) {
+                    const float c = static_cast<float>(col);
+                    x2 = ptx::fma2(ptx::f2(slope, slope), ptx::f2(rel + c, rel + c + 1.f), x2);
+                  }
+                  ptx::f2_split(x2, x, y);
+                }
+                if (MODE != 0) {
+                  if (!col_visible<MODE>(rm, col)) x = SOFTMAX ? -INFINITY : 0.f;
+                  if (!col_visible<MODE>(rm, col + 1)) y = SOFTMAX ? -INFINITY : 0.f;
+                }
+                mx = ptx::max3(mx, x, y);
+                ra = __float_as_uint(x), rb = __float_as_uint(y);
+              }
+            }
+          };
+          if (all)
+            pass1(std::integral_constant<int, 0>{});
+          else if (a.dil == 1)
+            pass1(std::integral_constant<int, 1>{});
+          else
+            pass1(std::integral_constant<int, 2>{});
+          if (!SOFTMAX) mx = static_cast<float>(static_cast<int>(__float_as_uint(mx) >> 23) - 126);
+          // the maximum moves only by more than 2^8: P stays below 2^(8 + kTiledPTop)
+          const float m_new = fmaxf(m_run, mx);
+          const bool need = m_new > m_run + 8.f;
+          float alpha = 1.f;
+          if (need) {
+            alpha = ptx::ex2(m_run - m_new);
+            l_run *= alpha;
+            m_run = m_new;
+          }
+          // (PV of the tile before is complete: S of this one came after it)
+          if (i > 0 && __any_sync(0xffffffffu, need)) {
+            rescale_rows<D>(tO, alpha);
+            ptx::tmem_wait_st();
+          }
+          const float mu = m_run == -INFINITY ? 0.f : m_run - kTiledPTop;
+          const uint64_t NM2 = ptx::f2(-mu, -mu);
+          const float down = SOFTMAX ? 0.f : ptx::ex2(-mu);
+          const uint64_t DN2 = ptx::f2(down, down);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int g = 4 * q; g < 4 * q + 4; ++g) {
+              uint64_t sum = ptx::f2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                uint64_t x2 = ptx::f2(__uint_as_float(sr[g / 2][(g & 1) * 16 + e]),
+                                      __uint_as_float(sr[g / 2][(g & 1) * 16 + e + 1]));
+                float x, y;
+                if (SOFTMAX) {
+                  ptx::f2_split(ptx::add2(x2, NM2), x, y);
+                  x = ptx::ex2(x), y = ptx::ex2(y);
+                  sum = ptx::add2(sum, ptx::f2(x, y));
+                } else {
+                  ptx::f2_split(ptx::mul2(x2, DN2), x, y);
+                }
+                pk[(g - 4 * q) * 8 + e / 2] = ptx::pack_f16(x, y);
+              }
+              if (SOFTMAX) {
+                float x, y;
+                ptx::f2_split(sum, x, y);
+                l_run = fmaf(x + y, sc[g].z, l_run);
+              }
+            }
+            ptx::tmem_st32(tS + q * 32, pk);
+          }
+          ptx::tmem_wait_st();
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(P_FULL + w));
+        }
+        if (!ok) break;
+        // ---- O
+        if (!wait(O_FULL + w, units & 1)) {
+          ok = false;
+          break;
+        }
+        ++units;
+        ptx::tc_fence_after();
+        m_run -= kTiledPTop;  // what O and the sum are relative to
+        uint32_t nan[D / 32] = {};
+        if (CT == CACHE_E4M3 && nan_flag && real)
+          nan_channels<D>(a, v_cache, h.b, h.un.hk, h.rq.tl, h.ut0, h.ut0 + h.nt, pos, h.rq.len, h.lo_max,
+                          h.hi_min, nan);
+        float f = 1.f;
+        uint16_t *dst = row_out<KIND>(a, h.un, min(r, h.un.rows - 1), m_run, l_run, whole && real, f);
+        float *part = a.part_o + (slot * ROWS + r) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          ptx::tmem_ld32(tO + c * 32, o);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence(o);
+          if (CT == CACHE_E4M3 && nan[c] != 0)
+            for (int e = 0; e < 32; ++e) o[e] |= (nan[c] >> e) & 1 ? 0x7fffffffu : 0u;
+          if (!real) continue;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              store4(a, dst + c * 32 + e, f, __uint_as_float(o[e]), __uint_as_float(o[e + 1]),
+                     __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              ptx::st_global_v4(part + c * 32 + e, o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (!whole && real)
+          *reinterpret_cast<float2 *>(a.part_ml + (slot * ROWS + r) * 2) = make_float2(m_run, l_run);
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(O_EMPTY + w));
+      }
+      k += h.nt;
+      // a unit that begins here and goes on in later CTAs
+      if (t == 0 && begun && !ended)
+        cuts[blockIdx.x] = CutUnit{h.un, line.cta_of(h.un, h.un.n - 1)};
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Launches of one head size and cache type; each has a source file of its own.
+template <int D, int CT>
+cudaError_t launch_tiled(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
+                         const uint8_t *v_cache, void *cuts, int kind, int grid, int device, cudaStream_t s);
+
+template <int D, int CT, int KIND>
+cudaError_t launch_tiled_one(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
+                             const uint8_t *v_cache, void *cuts, int grid, int device, cudaStream_t s) {
+  static std::atomic<uint64_t> set{0};
+  constexpr int bytes = TiledConfig<D>::SMEM;
+  cudaError_t e = allow_smem(reinterpret_cast<const void *>(&paged_tiled_kernel<D, CT, KIND>), bytes,
+                             device, set);
+  if (e != cudaSuccess) return e;
+  paged_tiled_kernel<D, CT, KIND>
+      <<<grid, kTiledThreads, bytes, s>>>(mk, mv, a, v_cache, static_cast<CutUnit *>(cuts));
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  // the merge may be set up while the last of the tiled CTAs run; it waits for them
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, TiledConfig<D>::ROWS / 16);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, KIND>, a, static_cast<const CutUnit *>(cuts));
+}
+
+#define CHIA_TILED_CASE(D, CT, KIND) \
+  case KIND: return launch_tiled_one<D, CT, KIND>(mk, mv, a, v_cache, cuts, grid, device, s);
+#define CHIA_INSTANTIATE_TILED(D, CT)                                                         \
+  template <>                                                                                 \
+  cudaError_t chia::launch_tiled<D, CT>(const CUtensorMap &mk, const CUtensorMap &mv,         \
+                                        const PagedArgs &a, const uint8_t *v_cache,           \
+                                        void *cuts, int kind, int grid, int device,           \
+                                        cudaStream_t s) {                                     \
+    switch (kind) {                                                                           \
+      CHIA_TILED_CASE(D, CT, KIND_SOFTCAP)                                                    \
+      CHIA_TILED_CASE(D, CT, KIND_ALIBI)                                                      \
+      CHIA_TILED_CASE(D, CT, KIND_SIGMOID)                                                    \
+      CHIA_TILED_CASE(D, CT, KIND_RELU)                                                       \
+      default: return launch_tiled_one<D, CT, KIND_SOFTMAX>(mk, mv, a, v_cache, cuts, grid, device, s); \
+    }                                                                                         \
+  }
+
+}  // namespace chia

@@ -239,11 +239,11 @@ def _workspace(dev: torch.device, stream: int) -> torch.Tensor:
     if t is None or capturing:
         n = _workspace_bytes.get(dev.index)
         if n is None:
-            with torch.cuda.device(dev):  # the largest: head_dim 128, more than 8 rows a K/V head
-                n = N.load().chia_paged_attn_workspace_bytes(_pack_paged(
-                    N.PAGED_ABI_VERSION, 0, 0, 128, 0, 0, 1, 1, 16, 9, 1, 1, 1, 1, 1, *([256] * 2),
+            with torch.cuda.device(dev):  # head_dim 128, few and many rows a K/V head
+                n = max(N.load().chia_paged_attn_workspace_bytes(_pack_paged(
+                    N.PAGED_ABI_VERSION, 0, 0, 128, 0, 0, 1, 1, 16, q, 1, 1, 1, 1, 1, *([256] * 2),
                     *([0] * 4), *([256] * 6), 0, 0, 0, 1.0, 1.0, 0.0, 1.0, -1, -1, 0, 0, 1, 0, 0, 0,
-                    0))
+                    0)) for q in (16, 1024))
             _workspace_bytes[dev.index] = n
         t = torch.zeros(n, dtype=torch.uint8, device=dev)
         if not capturing:
