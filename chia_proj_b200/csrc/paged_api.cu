@@ -202,7 +202,7 @@ int split_plan(const chia_paged_params_t *p, int sms, SplitPlan &pl) {
   pl.rows = pl.tiled ? chia::TiledConfig<128>::ROWS : 8 * pl.tiles;
   pl.grid = sms;
   // the line of tiles is counted in 32 bits
-  const int tk = pl.tiled ? 128 : 32;
+  const int tk = pl.tiled ? 64 : 32;
   const double line = static_cast<double>(p->heads_kv) * (p->tokens * group / pl.rows + p->batch + 1) *
                       (p->table_width * p->page_size / tk + 2 + chia::kUnitCost);
   if (pl.grid * 4 > kTicketBytes || p->tokens * p->heads > kI32 ||
@@ -331,7 +331,7 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   if (p->workspace_bytes < pl.bytes) return CHIA_ERR_INVALID_ARGUMENT;
   if (p->tokens == 0) return CHIA_OK;
   CUtensorMap mk, mv;
-  const int most = pl.tiled ? 128 : 32, box = p->page_size < most ? p->page_size : most;
+  const int most = pl.tiled ? 64 : 32, box = p->page_size < most ? p->page_size : most;
   if (!encode_cache(&mk, p->k_cache, p, box, !pl.tiled) ||
       !encode_cache(&mv, p->v_cache, p, box, !pl.tiled))
     return CHIA_ERR_LAUNCH;

@@ -2,7 +2,7 @@
 // cache: chunked prefill, on the 5th-generation tensor cores.
 //
 // A unit is up to 256 rows (queries x the heads of a group) of a request with
-// one K/V head, as two query tiles of 128 rows; keys come in tiles of 128. With
+// one K/V head, as two query tiles of 128 rows; keys come in tiles of 64. With
 // hundreds of rows to a key the work is bound by the tensor cores and the
 // exponentials, and the conversion of the cache to halves, done once for both
 // query tiles, hides behind them. One CTA an SM takes an equal piece of the
@@ -10,17 +10,20 @@
 // kernel behind this one merges with the whole GPU.
 //
 //   warps 0-3, 4-7  softmax of query tile 0 and 1, a thread a row
-//   warp 8          issues the UMMAs, warp 9 looks up pages and loads by TMA
+//   warps 8, 10     issue the UMMAs of query tile 0 and 1, warp 9 looks up pages
+//                   and loads by TMA
 //   warps 12-15     convert 8-bit tiles to halves
 //
-// Tensor memory: S0 S1 (128 columns each; P, in halves, takes the first 64 of
-// its S), O0 O1. Shared memory: Q0 Q1 | a ring of converted K and V tiles, all
-// in the 128-byte swizzle | a ring of 8-bit tiles as TMA brings them.
+// Tensor memory: two S buffers of 64 columns for each query tile (P, in halves,
+// takes the first 32 of its S), O0 O1. Shared memory: Q0 Q1 | a ring of
+// converted K and V tiles, all in the 128-byte swizzle | a ring of 8-bit tiles
+// as TMA brings them.
 //
-// The UMMAs of a CTA execute in the order of their issue, so S_w(t + 1) is
-// issued right behind PV_w(t), which reads P out of S_w's columns, and its
-// completion also says that O_w may be rescaled. The two query tiles take
-// turns: while one's products run, the other's exponentials do.
+// The UMMAs of a CTA execute in the order of their issue, so S_w(t + 2) is
+// issued right behind PV_w(t), which reads P_w(t) out of its columns, while the
+// softmax works on S_w(t + 1): it finds the next S ready. (With tiles of 128
+// keys one S buffer a query tile is all that fits beside O, and each softmax
+// waited some 2000 of 5200 cycles for PV and the next S.)
 //
 // Numbers as in the split kernel: Q times a power of two per row and the
 // cache's values are halves exactly; a key scale multiplies the scores of its
@@ -32,27 +35,29 @@ namespace chia {
 
 constexpr int kTiledThreads = 512;
 constexpr float kTiledPTop = 7.f;  // P is 2^7 at the running maximum, and at most 2^15 (a half's range)
-constexpr int kTiledCost = 1;   // what a unit costs beside its tiles of 128 keys
-constexpr int kTiledWhole = 6;  // units of up to this cost are not cut between CTAs
-constexpr int kTiledPiece = 6;  // the least cost of a piece: a part is 128 KB to write and to read
+constexpr int kTiledCost = 2;    // what a unit costs beside its tiles of 64 keys
+constexpr int kTiledWhole = 12;  // units of up to this cost are not cut between CTAs
+constexpr int kTiledPiece = 12;  // the least cost of a piece: a part is 128 KB to write and to read
 
 template <int D>
 struct TiledConfig {
-  static constexpr int ROWS = 256;           // rows of a unit
-  static constexpr int TK = 128;             // keys of a tile
+  static constexpr int ROWS = 256;             // rows of a unit
+  static constexpr int TK = 64;                // keys of a tile
+  static constexpr int GROUPS = TK / 16;       // of keys that share their scales
   static constexpr int Q_TILE = 128 * D * 2;
-  static constexpr int CHUNK = 128 * 128;    // 64 channels of a tile's 128 rows
-  static constexpr int KV = TK * D * 2;      // a converted K or V tile
-  static constexpr int SLOTS = 3 * (128 / D);
-  static constexpr int STAGE = TK * D;       // an 8-bit one
-  static constexpr int STAGES = 2 * (128 / D);
+  static constexpr int Q_CHUNK = 128 * 128;    // 64 channels of a query tile
+  static constexpr int CHUNK = TK * 128;       // 64 channels of a key tile
+  static constexpr int KV = TK * D * 2;        // a converted K or V tile
+  static constexpr int SLOTS = 6;
+  static constexpr int STAGE = TK * D;         // an 8-bit one
+  static constexpr int STAGES = 4;
   static constexpr int SETS = 8;             // tiles whose scales are held
   static constexpr int OFF_KV = 2 * Q_TILE;
   static constexpr int OFF_ST = OFF_KV + SLOTS * KV;
   static constexpr int OFF_SC = OFF_ST + STAGES * STAGE;
-  static constexpr int SMEM = 1024 + OFF_SC + SETS * 8 * 16;
+  static constexpr int SMEM = 1024 + OFF_SC + SETS * GROUPS * 16;
   // registers a thread: 512 threads begin with 128
-  static constexpr int REG_SOFTMAX = 184, REG_OTHER = 72;
+  static constexpr int REG_SOFTMAX = 160, REG_OTHER = 96;
   static_assert(256 * REG_SOFTMAX + 256 * REG_OTHER == 65536, "register split");
 };
 
@@ -106,9 +111,10 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
   band32(a, i, len, lo, hi);
   const int pf = min(a.prefix, len);
   for (int t = t0; t < t1; ++t) {
-    const int j0 = tl.key_tile(t) * 128;
-    if ((a.dil == 1 && j0 >= lo_max && j0 + 127 <= hi_min) || j0 + 128 <= pf) continue;
-    for (int j = j0; j < min(j0 + 128, len); ++j) {
+    constexpr int TK = TiledConfig<D>::TK;
+    const int j0 = tl.key_tile(t) * TK;
+    if ((a.dil == 1 && j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf) continue;
+    for (int j = j0; j < min(j0 + TK, len); ++j) {
       if (!(j < pf || (j >= lo && j <= hi && (a.dil == 1 || divides(a.dil, i - j))))) continue;
       const int pg = a.block_table[b * a.table_stride + j / a.page];
       if (pg < 0 || pg >= a.num_pages) continue;
@@ -124,30 +130,32 @@ __global__ void __launch_bounds__(kTiledThreads, 1)
 paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const PagedArgs a, const uint8_t *v_cache, CutUnit *cuts) {
   using C = TiledConfig<D>;
-  constexpr int TK = C::TK, ROWS = C::ROWS, SLOTS = C::SLOTS, STAGES = C::STAGES, SETS = C::SETS;
+  constexpr int TK = C::TK, ROWS = C::ROWS, SLOTS = C::SLOTS, STAGES = C::STAGES, SETS = C::SETS,
+                GROUPS = C::GROUPS;
   constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
   constexpr float LOG2E = 1.4426950408889634f;
   using L = Line<TK, ROWS, kTiledThreads, kTiledCost, kTiledWhole>;
   extern __shared__ uint8_t dyn[];
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
   const uint32_t sb = ptx::smem_u32(sm);
-  float4 *scales = reinterpret_cast<float4 *>(sm + C::OFF_SC);  // [SETS][8]: ks, value factor, its inverse
+  float4 *scales = reinterpret_cast<float4 *>(sm + C::OFF_SC);  // [SETS][GROUPS]: ks, value factor, its inverse
   __shared__ typename L::Shared line_sm;
-  // st_full st_empty | kv_full kv_empty | q s p o o_empty (2 each) | scales | drain
+  // st_full st_empty | kv_full kv_empty | q (2) | s p (2 buffers x 2) | pv o o_empty (2 each) | scales | drain
   enum { ST_FULL = 0, ST_EMPTY = ST_FULL + STAGES, KV_FULL = ST_EMPTY + STAGES, KV_EMPTY = KV_FULL + SLOTS,
-         Q_FULL = KV_EMPTY + SLOTS, S_FULL = Q_FULL + 2, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2,
-         O_EMPTY = O_FULL + 2, SC_FULL = O_EMPTY + 2, DRAIN = SC_FULL + SETS, BARS = DRAIN + 1 };
+         Q_FULL = KV_EMPTY + SLOTS, S_FULL = Q_FULL + 2, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4,
+         O_FULL = PV_DONE + 2, O_EMPTY = O_FULL + 2, SC_FULL = O_EMPTY + 2, DRAIN = SC_FULL + SETS,
+         BARS = DRAIN + 2 };
   __shared__ __align__(8) uint64_t bars[BARS];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, nan_flag;
-  __shared__ int tile_full[SETS];
+  __shared__ int tile_full[SETS], tile_live[SETS];  // all rows see the whole tile; keys there are
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   auto bar = [&](int i) { return ptx::smem_u32(bars) + 8 * i; };
   if (t == 0) {
     for (int i = 0; i < BARS; ++i) {
       const bool four = (i >= ST_EMPTY && i < KV_EMPTY) || (i >= Q_FULL && i < S_FULL) ||
-                        (i >= P_FULL && i < O_FULL) || (i >= O_EMPTY && i < SC_FULL);
-      ptx::mbar_init(bar(i), four ? 4 : 1);
+                        (i >= P_FULL && i < PV_DONE) || (i >= O_EMPTY && i < SC_FULL);
+      ptx::mbar_init(bar(i), i >= KV_EMPTY && i < Q_FULL ? 2 : four ? 4 : 1);
     }
     abort_flag = nan_flag = 0;
     ptx::tma_prefetch_desc(&mk);
@@ -205,17 +213,17 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     if (warp == 9) {
       // ==================================================== pages and TMA
       const int pshift = 31 - __clz(a.page), rows = min(a.page, TK);
-      // Of the tile's keys 16 lane .. + 15 (lanes 0-7). What a tile needs from
+      // Of the tile's keys 16 lane .. + 15 (lanes 0-3). What a tile needs from
       // memory is asked for a tile or two ahead and looked at when its turn
       // comes: the page of tile k + 2, the scales of tile k + 1.
       struct Keys {
         int key, pg;  // pg: -1 where there is nothing to load
-        int hk, all;
+        int hk, all, live;
       };
       Here h;
       int left = 0, lo_min = 0, hi_max = 0;  // tiles of the unit still to look up
       auto page_of = [&](int k) {
-        Keys x{0, -1, 0, 0};
+        Keys x{0, -1, 0, 0, 0};
         if (k >= nk) return x;
         if (left == 0) {
           h = unit_at(k), left = h.nt;
@@ -228,9 +236,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         x.key = j0 + 16 * lane;
         x.hk = h.un.hk;
         x.all = sees_all(h, j0);
+        x.live = h.rq.len - j0;
         // (the scales of 16 keys that no row sees may be anything)
         if (!(x.key < min(a.prefix, h.rq.len) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
-        if (lane < 8 && x.key < h.rq.len) x.pg = a.block_table[h.b * a.table_stride + (x.key >> pshift)];
+        if (lane < GROUPS && x.key < h.rq.len) x.pg = a.block_table[h.b * a.table_stride + (x.key >> pshift)];
         return x;
       };
       int issued = 0;
@@ -251,22 +260,22 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         const Keys now = k1;
         row = row1, ks = ks1, vs = vs1;
         if (row < 0 && (now.pg != -1)) report(a.status, kStatusBadIndex);
-        if (lane < 8) {
+        if (lane < GROUPS) {
           float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
           if (row >= 0 && !(now.all & 2)) {
             sc.x = ks;
             sc.y = value_factor<SOFTMAX>(vs);
             sc.z = SOFTMAX ? ptx::ex2(-sc.y) : 0.f;
           }
-          scales[(k % SETS) * 8 + lane] = sc;
+          scales[(k % SETS) * GROUPS + lane] = sc;
         }
-        if (lane == 0) tile_full[k % SETS] = now.all & 1;
+        if (lane == 0) tile_full[k % SETS] = now.all & 1, tile_live[k % SETS] = now.live;
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(SC_FULL + k % SETS));
         k1 = k2;
         scales_of(k1);
         k2 = page_of(k + 2);
-        const bool leads = lane < 8 && row >= 0 && (16 * lane) % rows == 0;
+        const bool leads = lane < GROUPS && row >= 0 && (16 * lane) % rows == 0;
         const int bytes = __popc(__ballot_sync(0xffffffffu, leads)) * rows * D;
         bool ok = true;
         for (int v = 0; v < 2 && ok; ++v) {
@@ -288,73 +297,80 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       int none = 0;
       for (int i = max(0, issued - STAGES); i < issued; ++i)
         paged_wait(bar(ST_FULL + i % STAGES), (i / STAGES) & 1, &none, d);
-    } else if (warp == 8) {
+    } else if (warp == 8 || warp == 10) {
       // ==================================================== UMMA issue
-      constexpr uint32_t IDESC_QK = ptx::make_idesc_f16(128, 128, false, false, false);
+      // A warp a query tile: one warp's issue (some 40 cycles a UMMA) would be
+      // the limit, since a UMMA of 64 keys runs for 32.
+      const int w = warp == 10;
+      constexpr uint32_t IDESC_QK = ptx::make_idesc_f16(128, TK, false, false, false);
       constexpr uint32_t IDESC_PV = ptx::make_idesc_f16(128, D, false, false, true);
-      const uint64_t dq = ptx::make_sdesc_sw128(sb, 16, 1024);
+      const uint64_t dq = ptx::make_sdesc_sw128(sb + w * C::Q_TILE, 16, 1024);
       const uint64_t dk = ptx::make_sdesc_sw128(sb + C::OFF_KV, 16, 1024);
       const uint64_t dv = ptx::make_sdesc_sw128(sb + C::OFF_KV, C::CHUNK, 1024);
-      auto issue_s = [&](int w, int slot) {
+      const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
+      auto issue_s = [&](int buf, int slot) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * C::CHUNK + (kk & 3) * 32) >> 4;
-          ptx::umma_ss_warp(tmem + w * 128, dq + ((w * C::Q_TILE) >> 4) + off,
-                            dk + ((slot * C::KV) >> 4) + off, IDESC_QK, kk > 0 ? 1u : 0u);
+        for (int c = 0; c < D / 64; ++c) {
+          const uint64_t q0 = dq + ((c * C::Q_CHUNK) >> 4), k0 = dk + ((slot * C::KV + c * C::CHUNK) >> 4);
+          const uint64_t qa[4] = {q0, q0 + 2, q0 + 4, q0 + 6}, kb[4] = {k0, k0 + 2, k0 + 4, k0 + 6};
+          ptx::umma_ss_x4_warp(tS + buf * 64, qa, kb, IDESC_QK, c > 0 ? 1u : 0u);
         }
-        ptx::umma_commit_warp(bar(S_FULL + w));
+        ptx::umma_commit_warp(bar(S_FULL + 2 * w + buf));
+        ptx::umma_commit_warp(bar(KV_EMPTY + slot));
       };
-      auto issue_pv = [&](int w, int slot, bool first) {
-#pragma unroll
-        for (int kk = 0; kk < TK / 16; ++kk)
-          ptx::umma_ts_warp(tmem + 256 + w * 128, tmem + w * 128 + kk * 8,
-                            dv + ((slot * C::KV + kk * 2048) >> 4), IDESC_PV, first && kk == 0 ? 0u : 1u);
+      auto issue_pv = [&](int buf, int slot, bool first, bool last) {
+        static_assert(TK == 64, "four steps of 16 keys");
+        const uint32_t p0 = tS + buf * 64, pa[4] = {p0, p0 + 8, p0 + 16, p0 + 24};
+        const uint64_t v0 = dv + ((slot * C::KV) >> 4), vb[4] = {v0, v0 + 128, v0 + 256, v0 + 384};
+        ptx::umma_ts_x4_warp(tO, pa, vb, IDESC_PV, first ? 0u : 1u);
+        ptx::umma_commit_warp(bar(PV_DONE + w));
+        ptx::umma_commit_warp(bar(KV_EMPTY + slot));
+        if (last) ptx::umma_commit_warp(bar(O_FULL + w));
       };
       auto all_wait = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, wait(i, parity)); };
-      uint32_t tiles[2] = {0, 0}, units[2] = {0, 0};
+      uint32_t tiles = 0, units = 0;
       bool ok = true;
       for (int k = 0; k < nk && ok;) {
         const Here h = unit_at(k);
-        const int act = h.un.rows > 128 ? 2 : 1;
-        for (int w = 0; w < act && ok; ++w) ok = all_wait(Q_FULL + w, units[w] & 1);
-        int item = 2 * k;
-        ok = ok && all_wait(KV_FULL + item % SLOTS, (item / SLOTS) & 1);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        for (int w = 0; w < act; ++w) issue_s(w, item % SLOTS);
-        ptx::umma_commit_warp(bar(KV_EMPTY + item % SLOTS));
-        for (int i = 0; i < h.nt && ok; ++i) {
-          const int vi = 2 * (k + i) + 1, ki = vi + 1;
-          ok = all_wait(KV_FULL + vi % SLOTS, (vi / SLOTS) & 1);
-          for (int w = 0; w < act && ok; ++w) {
-            ok = all_wait(P_FULL + w, tiles[w] & 1);
-            if (ok && i == 0 && units[w] > 0) ok = all_wait(O_EMPTY + w, (units[w] - 1) & 1);
-            if (!ok) break;
-            ptx::tc_fence_after();
-            issue_pv(w, vi % SLOTS, i == 0);
-            ++tiles[w];
-            if (i == h.nt - 1) ptx::umma_commit_warp(bar(O_FULL + w));
-            if (w == act - 1) ptx::umma_commit_warp(bar(KV_EMPTY + vi % SLOTS));
-            if (i + 1 < h.nt) {
-              if (w == 0) {
-                ok = all_wait(KV_FULL + ki % SLOTS, (ki / SLOTS) & 1);
-                if (!ok) break;
-                ptx::tc_fence_after();
-              }
-              issue_s(w, ki % SLOTS);
-              if (w == act - 1) ptx::umma_commit_warp(bar(KV_EMPTY + ki % SLOTS));
-            }
+        if (h.un.rows <= 128 * w) {  // no second query tile: the slots are let go as they come
+          for (int i = 2 * k; i < 2 * (k + h.nt) && ok; ++i) {
+            ok = all_wait(KV_FULL + i % SLOTS, (i / SLOTS) & 1);
+            if (ok && lane == 0) ptx::mbar_arrive(bar(KV_EMPTY + i % SLOTS));
           }
+          k += h.nt;
+          continue;
         }
-        for (int w = 0; w < act; ++w) ++units[w];
+        ok = all_wait(Q_FULL + w, units & 1);
+        // S of the unit's first two tiles, then behind each PV the S two tiles on
+        auto next_s = [&](int i) {
+          const int ki = 2 * (k + i);
+          if (!all_wait(KV_FULL + ki % SLOTS, (ki / SLOTS) & 1)) return false;
+          ptx::tc_fence_after();
+          issue_s((tiles + i) & 1, ki % SLOTS);
+          return true;
+        };
+        for (int i = 0; i < min(2, h.nt) && ok; ++i) ok = next_s(i);
+        for (int i = 0; i < h.nt && ok; ++i) {
+          const int vi = 2 * (k + i) + 1;
+          const uint32_t n = tiles + i;
+          ok = all_wait(KV_FULL + vi % SLOTS, (vi / SLOTS) & 1) &&
+               all_wait(P_FULL + 2 * w + (n & 1), (n >> 1) & 1) &&
+               (i > 0 || units == 0 || all_wait(O_EMPTY + w, (units - 1) & 1));
+          if (!ok) break;
+          ptx::tc_fence_after();
+          issue_pv(n & 1, vi % SLOTS, i == 0, i == h.nt - 1);
+          if (i + 2 < h.nt) ok = next_s(i + 2);
+        }
+        tiles += h.nt;
+        ++units;
         k += h.nt;
       }
       // all UMMAs are complete before tensor memory is freed
-      ptx::umma_commit_warp(bar(DRAIN));
+      ptx::umma_commit_warp(bar(DRAIN + w));
       PagedArgs d = a;
       d.timeout_ns = a.drain_ns;
       int none = 0;
-      paged_wait(bar(DRAIN), 0, &none, d);
+      paged_wait(bar(DRAIN + w), 0, &none, d);
     } else if (warp >= 12) {
       // ==================================================== conversion
       const int c = t - 384;
@@ -362,43 +378,44 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         const int st = item % STAGES, sl = item % SLOTS;
         if (!wait(ST_FULL + st, (item / STAGES) & 1)) break;
         if (!wait(KV_EMPTY + sl, ((item / SLOTS) & 1) ^ 1)) break;
-        const bool sift = CT == CACHE_E4M3 && (item & 1) && !tile_full[(item / 2) % SETS];
+        const int set = (item / 2) % SETS;
+        const bool sift = CT == CACHE_E4M3 && (item & 1) && !tile_full[set];
         bool nan_seen = false;
+        // Eight lanes read 128 bytes of two neighbouring rows, 64 of each, that
+        // fall into different banks, and store to units of the two rows' swizzled
+        // lines that do so too: the rows' swizzles differ in the lowest bit.
         constexpr int PER = TK * D / 16 / 128;  // 16-byte pieces a thread
-        uint4 all[PER];
+        const int half = (lane >> 2) & 1, r0 = (c >> 5) * (TK / 4) + 2 * (lane >> 3) + half;
+        auto row_of = [&](int x) { return r0 + 8 * (D == 128 ? x >> 1 : x); };
+        auto piece_of = [&](int x) { return (lane & 3) + (D == 128 ? 4 * (half ^ (x & 1)) : 0); };
+        uint4 q[PER];
 #pragma unroll
         for (int x = 0; x < PER; ++x)
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(all[x].x), "=r"(all[x].y), "=r"(all[x].z), "=r"(all[x].w)
-                       : "r"(sb + C::OFF_ST + st * C::STAGE + (x * 128 + c) * 16));
+                       : "=r"(q[x].x), "=r"(q[x].y), "=r"(q[x].z), "=r"(q[x].w)
+                       : "r"(sb + C::OFF_ST + st * C::STAGE + row_of(x) * D + piece_of(x) * 16));
 #pragma unroll
         for (int x = 0; x < PER; ++x) {
-          const int piece = x * 128 + c, row = piece / (D / 16), v = piece % (D / 16);
-          uint4 q = all[x];
+          const int row = row_of(x), v = piece_of(x);
           if (sift) {
+            const bool live = row < tile_live[set];
             auto clean = [&](uint32_t &w) {
               const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
-              nan_seen |= nan != 0;
+              nan_seen |= live && nan != 0;
               w &= ~(nan * 0xffu);
             };
-            clean(q.x), clean(q.y), clean(q.z), clean(q.w);
+            clean(q[x].x), clean(q[x].y), clean(q[x].z), clean(q[x].w);
           }
           uint32_t h[8];
-          cache4_to_f16<CT>(q.x, h[0], h[1]);
-          cache4_to_f16<CT>(q.y, h[2], h[3]);
-          cache4_to_f16<CT>(q.z, h[4], h[5]);
-          cache4_to_f16<CT>(q.w, h[6], h[7]);
-          // channels 16 v .. + 15: units 2 v, 2 v + 1 of the row, four pieces a
-          // chunk; lanes of different chunks store in opposite order, so that
-          // eight lanes' stores fall into different banks
+          cache4_to_f16<CT>(q[x].x, h[0], h[1]);
+          cache4_to_f16<CT>(q[x].y, h[2], h[3]);
+          cache4_to_f16<CT>(q[x].z, h[4], h[5]);
+          cache4_to_f16<CT>(q[x].w, h[6], h[7]);
+          // channels 16 v .. + 15: units 2 v, 2 v + 1 of the row, four pieces a chunk
           const uint32_t base = sb + C::OFF_KV + sl * C::KV + (v / 4) * C::CHUNK + row * 128;
-          const int u = 2 * (v % 4), sw = row & 7, flip = D == 128 ? v / 4 : 0;
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const bool hi = (y ^ flip) != 0;
-            ptx::st_shared_v4(base + (((u + (hi ? 1 : 0)) ^ sw) << 4), hi ? h[4] : h[0], hi ? h[5] : h[1],
-                              hi ? h[6] : h[2], hi ? h[7] : h[3]);
-          }
+          const int u = 2 * (v % 4), sw = row & 7;
+          ptx::st_shared_v4(base + ((u ^ sw) << 4), h[0], h[1], h[2], h[3]);
+          ptx::st_shared_v4(base + (((u + 1) ^ sw) << 4), h[4], h[5], h[6], h[7]);
         }
         if (sift && nan_seen) nan_flag = 1;
         ptx::fence_proxy_async_smem();  // the UMMAs read what was stored
@@ -413,9 +430,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   } else {
     ptx::setmaxnreg_inc<C::REG_SOFTMAX>();
     // ======================================================= softmax
-    const int w = warp >> 2, row = t & 127, rsw = row & 7;
+    const int w = warp >> 2, row = t & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lane_off + w * 128, tO = tmem + lane_off + 256 + w * 128;
+    const uint32_t tS0 = tmem + lane_off + w * 128, tO = tmem + lane_off + 256 + w * 128;
     uint32_t cnt = 0, units = 0;
     bool ok = true;
     if (t == 0) cuts[blockIdx.x].un.rows = 0;
@@ -430,43 +447,48 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         const int qi = div_group(a, rr), head = h.un.hk * a.group + rr - qi * a.group;
         const int pos = h.p0 + qi;
         // ---- the row of Q, as halves
-        float rowmul;
+        // (16 bytes a lane, neighbouring lanes along a row)
+        float rowmul = 0.f;
         {
-          const uint16_t *src = static_cast<const uint16_t *>(a.q) +
-                                static_cast<int64_t>(h.un.t0 + qi) * a.q_st + head * a.q_sh;
-          uint4 raw[D / 8];
-          float mx = 0.f;
+          constexpr int UPR = D / 8, RPI = 32 / UPR, IT = 32 / RPI;  // units a row, rows a load, loads
+          const int u = lane % UPR, sub = lane / UPR, base = (warp & 3) * 32;
+          uint4 raw[IT];
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            raw[c] = real ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+          for (int x = 0; x < IT; ++x) {
+            const int q = w * 128 + base + x * RPI + sub, qr = h.un.row0 + q;
+            const int qt = div_group(a, qr), qh = h.un.hk * a.group + qr - qt * a.group;
+            raw[x] = q < h.un.rows ? *reinterpret_cast<const uint4 *>(
+                                         static_cast<const uint16_t *>(a.q) +
+                                         static_cast<int64_t>(h.un.t0 + qt) * a.q_st + qh * a.q_sh + 8 * u)
+                                   : make_uint4(0, 0, 0, 0);
+          }
           auto two = [&](uint32_t v) {
             return a.bf16 ? in16x2_to_float2<true>(v) : in16x2_to_float2<false>(v);
           };
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+          for (int x = 0; x < IT; ++x) {
+            const uint32_t v[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+            float2 f[4];
+            float mx = 0.f;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const float2 f = two(v[y]);
-              mx = ptx::max3(mx, fabsf(f.x), fabsf(f.y));
+              f[y] = two(v[y]);
+              mx = ptx::max3(mx, fabsf(f[y].x), fabsf(f[y].y));
             }
-          }
-          int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
-          e = max(-100, min(127, e));
-          const float up = pow2f(14 - e);
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint32_t v[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-            uint32_t o[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const float2 f = two(v[y]);
-              o[y] = ptx::pack_f16(f.x * up, f.y * up);
-            }
-            ptx::st_shared_v4(sb + w * C::Q_TILE + (c / 8) * C::CHUNK + row * 128 + (((c % 8) ^ rsw) << 4),
-                              o[0], o[1], o[2], o[3]);
+            for (int d = 1; d < UPR; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+            e = max(-100, min(127, e));
+            const float up = pow2f(14 - e);
+            const int qrow = base + x * RPI + sub;
+            ptx::st_shared_v4(sb + w * C::Q_TILE + (u / 8) * C::Q_CHUNK + qrow * 128 +
+                                  (((u % 8) ^ (qrow & 7)) << 4),
+                              ptx::pack_f16(f[0].x * up, f[0].y * up), ptx::pack_f16(f[1].x * up, f[1].y * up),
+                              ptx::pack_f16(f[2].x * up, f[2].y * up), ptx::pack_f16(f[3].x * up, f[3].y * up));
+            // the power of two of each row goes to its thread
+            const float down = __shfl_sync(0xffffffffu, pow2f(e - 14), (lane % RPI) * UPR);
+            if (lane / RPI == x) rowmul = a.score_scale * down;
           }
-          rowmul = a.score_scale * pow2f(e - 14);
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(bar(Q_FULL + w));
@@ -480,36 +502,47 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         int lo, hi;
         band32(a, pos, h.rq.len, lo, hi);
         const int pf = min(a.prefix, h.rq.len);
-        const bool none = lo > hi;
         float m_run = SOFTMAX ? -INFINITY : -100.f, l_run = 0.f;
         for (int i = 0; i < h.nt; ++i, ++cnt) {
           const int n = k + i;
-          if (!wait(SC_FULL + n % SETS, (n / SETS) & 1) || !wait(S_FULL + w, cnt & 1)) {
+          if (!wait(SC_FULL + n % SETS, (n / SETS) & 1) ||
+              !wait(S_FULL + 2 * w + (cnt & 1), (cnt >> 1) & 1)) {
             ok = false;
             break;
           }
           ptx::tc_fence_after();
-          uint32_t sr[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) ptx::tmem_ld32(tS + c * 32, sr[c]);
+          const uint32_t tS = tS0 + (cnt & 1) * 64;
+          uint32_t sr[2][32];
+          ptx::tmem_ld32(tS, sr[0]);
+          ptx::tmem_ld32(tS + 32, sr[1]);
           const int j0 = h.rq.tl.key_tile(h.ut0 + i) * TK;
-          const float4 *sc = scales + (n % SETS) * 8;
+          const float4 *sc = scales + (n % SETS) * GROUPS;
           const bool all = sees_all(h, j0);
-          ptx::tmem_wait_ld();
+          uint32_t vis[2] = {~0u, ~0u};  // the keys of the tile that this row sees
+          if (!all) {
+            auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; };
 #pragma unroll
-          for (int c = 0; c < 4; ++c) ptx::reg_fence(sr[c]);
-          RowMask rm;
-          rm.c_lo = none ? (1 << 30) : lo - j0;
-          rm.span = none ? 0u : static_cast<uint32_t>(hi - lo);
-          rm.c_pre = real ? pf - j0 : 0;
-          rm.i_rel = pos - j0;
-          rm.dil = a.dil;
+            for (int c = 0; c < 2; ++c) {
+              const int k0 = j0 + 32 * c;
+              uint32_t m = lo > hi ? 0u : below(hi + 1 - k0) & ~below(lo - k0);
+              if (a.dil != 1) {
+                uint32_t every = 0;
+                int first = (pos - k0) % a.dil;
+                for (int e = first < 0 ? first + a.dil : first; e < 32; e += a.dil) every |= 1u << e;
+                m &= every;
+              }
+              vis[c] = real ? m | below(pf - k0) : 0u;
+            }
+          }
+          ptx::tmem_wait_ld();
+          ptx::reg_fence(sr[0]);
+          ptx::reg_fence(sr[1]);
           const float rel = static_cast<float>(j0 - pos);
           float mx = SOFTMAX ? -INFINITY : 0.f;
-          auto pass1 = [&](auto mode) {
-            constexpr int MODE = decltype(mode)::value;
+          auto pass1 = [&](auto masked) {
+            constexpr bool MASKED = decltype(masked)::value;
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
+            for (int g = 0; g < GROUPS; ++g) {
               const float4 s4 = sc[g];
               const float f = rowmul * s4.x;
               const uint64_t F2 = ptx::f2(f, f), V2 = ptx::f2(s4.y, s4.y);
@@ -540,9 +573,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                   }
                   ptx::f2_split(x2, x, y);
                 }
-                if (MODE != 0) {
-                  if (!col_visible<MODE>(rm, col)) x = SOFTMAX ? -INFINITY : 0.f;
-                  if (!col_visible<MODE>(rm, col + 1)) y = SOFTMAX ? -INFINITY : 0.f;
+                if (MASKED) {
+                  if (!((vis[g / 2] >> ((g & 1) * 16 + e)) & 1)) x = SOFTMAX ? -INFINITY : 0.f;
+                  if (!((vis[g / 2] >> ((g & 1) * 16 + e + 1)) & 1)) y = SOFTMAX ? -INFINITY : 0.f;
                 }
                 mx = ptx::max3(mx, x, y);
                 ra = __float_as_uint(x), rb = __float_as_uint(y);
@@ -550,11 +583,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             }
           };
           if (all)
-            pass1(std::integral_constant<int, 0>{});
-          else if (a.dil == 1)
-            pass1(std::integral_constant<int, 1>{});
+            pass1(std::false_type{});
           else
-            pass1(std::integral_constant<int, 2>{});
+            pass1(std::true_type{});
           if (!SOFTMAX) mx = static_cast<float>(static_cast<int>(__float_as_uint(mx) >> 23) - 126);
           // the maximum moves only by more than 2^8: P stays below 2^(8 + kTiledPTop)
           const float m_new = fmaxf(m_run, mx);
@@ -565,47 +596,47 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             l_run *= alpha;
             m_run = m_new;
           }
-          // (PV of the tile before is complete: S of this one came after it)
-          if (i > 0 && __any_sync(0xffffffffu, need)) {
+          if (i > 0 && __any_sync(0xffffffffu, need)) {  // O is rescaled once the tile before is in it
+            if (!__all_sync(0xffffffffu, wait(PV_DONE + w, (cnt - 1) & 1))) {
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
             rescale_rows<D>(tO, alpha);
-            ptx::tmem_wait_st();
           }
           const float mu = m_run == -INFINITY ? 0.f : m_run - kTiledPTop;
           const uint64_t NM2 = ptx::f2(-mu, -mu);
           const float down = SOFTMAX ? 0.f : ptx::ex2(-mu);
           const uint64_t DN2 = ptx::f2(down, down);
+          uint32_t pk[32];
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t pk[32];
+          for (int g = 0; g < GROUPS; ++g) {
+            uint64_t sum = ptx::f2(0.f, 0.f);
 #pragma unroll
-            for (int g = 4 * q; g < 4 * q + 4; ++g) {
-              uint64_t sum = ptx::f2(0.f, 0.f);
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                uint64_t x2 = ptx::f2(__uint_as_float(sr[g / 2][(g & 1) * 16 + e]),
-                                      __uint_as_float(sr[g / 2][(g & 1) * 16 + e + 1]));
-                float x, y;
-                if (SOFTMAX) {
-                  ptx::f2_split(ptx::add2(x2, NM2), x, y);
-                  x = ptx::ex2(x), y = ptx::ex2(y);
-                  sum = ptx::add2(sum, ptx::f2(x, y));
-                } else {
-                  ptx::f2_split(ptx::mul2(x2, DN2), x, y);
-                }
-                pk[(g - 4 * q) * 8 + e / 2] = ptx::pack_f16(x, y);
-              }
+            for (int e = 0; e < 16; e += 2) {
+              uint64_t x2 = ptx::f2(__uint_as_float(sr[g / 2][(g & 1) * 16 + e]),
+                                    __uint_as_float(sr[g / 2][(g & 1) * 16 + e + 1]));
+              float x, y;
               if (SOFTMAX) {
-                float x, y;
-                ptx::f2_split(sum, x, y);
-                l_run = fmaf(x + y, sc[g].z, l_run);
+                ptx::f2_split(ptx::add2(x2, NM2), x, y);
+                x = ptx::ex2(x), y = ptx::ex2(y);
+                sum = ptx::add2(sum, ptx::f2(x, y));
+              } else {
+                ptx::f2_split(ptx::mul2(x2, DN2), x, y);
               }
+              pk[g * 8 + e / 2] = ptx::pack_f16(x, y);
             }
-            ptx::tmem_st32(tS + q * 32, pk);
+            if (SOFTMAX) {
+              float x, y;
+              ptx::f2_split(sum, x, y);
+              l_run = fmaf(x + y, sc[g].z, l_run);
+            }
           }
+          ptx::tmem_st32(tS, pk);
           ptx::tmem_wait_st();
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(P_FULL + w));
+          if (lane == 0) ptx::mbar_arrive(bar(P_FULL + 2 * w + (cnt & 1)));
         }
         if (!ok) break;
         // ---- O
@@ -621,26 +652,69 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           nan_channels<D>(a, v_cache, h.b, h.un.hk, h.rq.tl, h.ut0, h.ut0 + h.nt, pos, h.rq.len, h.lo_max,
                           h.hi_min, nan);
         float f = 1.f;
-        uint16_t *dst = row_out<KIND>(a, h.un, min(r, h.un.rows - 1), m_run, l_run, whole && real, f);
-        float *part = a.part_o + (slot * ROWS + r) * D;
+        row_out<KIND>(a, h.un, min(r, h.un.rows - 1), m_run, l_run, whole && real, f);
+        // Through this warp's rows of Q's memory (free: the unit's UMMAs are
+        // complete), so that neighbouring lanes write along a row: 16-byte units,
+        // as halves of 32 rows x 64 or 128 channels, or fp32 of 64 channels.
+        {
+          const int base = (warp & 3) * 32;
+          auto unit16 = [&](int lr, int u) {  // 16 bytes of row lr: where this warp's row of Q was
+            return sb + w * C::Q_TILE + (u >> 3) * C::Q_CHUNK + (base + lr) * 128 + (((u ^ lr) & 7) << 4);
+          };
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          ptx::tmem_ld32(tO + c * 32, o);
-          ptx::tmem_wait_ld();
-          ptx::reg_fence(o);
-          if (CT == CACHE_E4M3 && nan[c] != 0)
-            for (int e = 0; e < 32; ++e) o[e] |= (nan[c] >> e) & 1 ? 0x7fffffffu : 0u;
-          if (!real) continue;
-          if (whole) {
+          for (int c0 = 0; c0 < D; c0 += (D == 128 && whole) ? 128 : 64) {
+            const int cols = (D == 128 && whole) ? 128 : 64;
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 32) {
+              uint32_t o[32];
+              ptx::tmem_ld32(tO + c0 + c, o);
+              ptx::tmem_wait_ld();
+              ptx::reg_fence(o);
+              const uint32_t nn = nan[(c0 + c) / 32];
+              if (CT == CACHE_E4M3 && nn != 0)
+                for (int e = 0; e < 32; ++e) o[e] |= (nn >> e) & 1 ? 0x7fffffffu : 0u;
+              if (whole) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              store4(a, dst + c * 32 + e, f, __uint_as_float(o[e]), __uint_as_float(o[e + 1]),
-                     __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-          } else {
+                for (int e = 0; e < 32; e += 8) {
+                  uint32_t x[4];
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              ptx::st_global_v4(part + c * 32 + e, o[e], o[e + 1], o[e + 2], o[e + 3]);
+                  for (int y = 0; y < 4; ++y) {
+                    const float p = __uint_as_float(o[e + 2 * y]) * f, q = __uint_as_float(o[e + 2 * y + 1]) * f;
+                    x[y] = a.bf16 ? ptx::pack_bf16(p, q) : ptx::pack_f16(p, q);
+                  }
+                  ptx::st_shared_v4(unit16(lane, (c + e) / 8), x[0], x[1], x[2], x[3]);
+                }
+              } else if (D == 128) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                  ptx::st_shared_v4(unit16(lane, (c + e) / 4), o[e], o[e + 1], o[e + 2], o[e + 3]);
+              } else if (real) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                  ptx::st_global_v4(a.part_o + (slot * ROWS + r) * D + c + e, o[e], o[e + 1], o[e + 2], o[e + 3]);
+              }
+            }
+            if (D == 64 && !whole) break;
+            __syncwarp();
+            const int upr = whole ? cols / 8 : 16, rpi = 32 / upr;
+            for (int x = 0; x < 32; x += rpi) {
+              const int lr = x + lane / upr, u = lane % upr, q = w * 128 + base + lr;
+              uint4 v;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                           : "r"(unit16(lr, u)));
+              if (q < h.un.rows) {
+                if (whole) {
+                  const int qr = h.un.row0 + q, qt = div_group(a, qr), qh = h.un.hk * a.group + qr - qt * a.group;
+                  uint16_t *dst = static_cast<uint16_t *>(a.o) + static_cast<int64_t>(h.un.t0 + qt) * a.o_st +
+                                  qh * a.o_sh;
+                  *reinterpret_cast<uint4 *>(dst + 8 * u) = v;
+                } else {
+                  *reinterpret_cast<uint4 *>(a.part_o + (slot * ROWS + q) * D + c0 + 4 * u) = v;
+                }
+              }
+            }
+            __syncwarp();
           }
         }
         if (!whole && real)
