@@ -53,10 +53,13 @@ struct Tiles {
 // Queries and keys of request b, checked: [t0, t0 + n) of q, keys [0, len).
 struct Request {
   int t0, n, len;
-  Tiles tl;
+  int b;           // its row of the block table
+  int row0, row1;  // an entry of the line: these rows (queries x heads of a group) of the request
+  Tiles tl;        // the tiles that they visit
 };
 __device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &bad) {
   Request r;
+  r.b = b;
   if (a.cu_q != nullptr) {
     r.t0 = a.cu_q[b];
     const int t1 = a.cu_q[b + 1];
@@ -76,6 +79,8 @@ __device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &b
     bad = true;
     r.len = r.len < 0 ? 0 : most;
   }
+  r.row0 = 0;
+  r.row1 = r.n * a.group;
   return r;
 }
 
@@ -178,58 +183,101 @@ __device__ __forceinline__ void store4(const PagedArgs &a, uint16_t *dst, float 
              : make_uint2(ptx::pack_f16(x0, x1), ptx::pack_f16(x2, x3));
 }
 
-// The line of units of ROWS rows and tiles of TK keys, in shared memory.
-// WHOLE: units of up to this cost are not cut between CTAs.
-template <int TK, int ROWS, int THREADS, int COST, int WHOLE>
+// The line of units of ROWS rows and tiles of TK keys, in shared memory: its
+// entries in their order. An entry is a request, or with BLOCKS a block of ROWS
+// rows of one (several, where there are more blocks than entries fit): blocks
+// of a long run of queries see different keys. An entry's units visit the same
+// tiles. WHOLE: units of up to this cost are not cut between CTAs.
+template <int TK, int ROWS, int THREADS, int COST, int WHOLE, bool BLOCKS>
 struct Line {
   struct Shared {
-    int tiles_pre[kLineBatch + 1], units_pre[kLineBatch + 1];  // before each request
+    int tiles_pre[kLineBatch + 1], units_pre[kLineBatch + 1];  // before each entry
     Request req[kLineBatch];
     int wsum[THREADS / 32][2];
+    int starts[BLOCKS ? kLineBatch + 1 : 1];  // first entry of each request
   };
   Shared &s;
   const PagedArgs &a;
-  int total, ctas, step, rest;
+  int entries, total, ctas, step, rest;
+
+  // Sums over the block of x and y before this thread's; the totals in tx, ty.
+  __device__ __forceinline__ void scan(int &x, int &y, int &tx, int &ty) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int x0 = x, y0 = y;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
+      if (lane >= d) x += u, y += v;
+    }
+    if (lane == 31) s.wsum[warp][0] = x, s.wsum[warp][1] = y;
+    __syncthreads();
+    x -= x0, y -= y0;
+    tx = ty = 0;
+#pragma unroll 4
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) x += s.wsum[w][0], y += s.wsum[w][1];
+      tx += s.wsum[w][0], ty += s.wsum[w][1];
+    }
+    __syncthreads();
+  }
 
   // All threads of the CTA; per_cta: the least cost of a CTA's piece.
   __device__ __forceinline__ Line(Shared &sh, const PagedArgs &args, int per_cta) : s(sh), a(args) {
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int per = (a.batch + THREADS - 1) / THREADS;
-    const int b0 = t * per, b1 = min(a.batch, b0 + per);
-    int nt = 0, nu = 0;
+    const int t = threadIdx.x;
     bool bad = false;
-    for (int b = b0; b < b1; ++b) {
-      Request r = request_of(a, b, bad);
-      int n = 0, u = 0;
-      if (r.n > 0) {
-        r.tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
-        u = (r.n * a.group + ROWS - 1) / ROWS * a.heads_kv;
-        n = r.tl.n * u;
+    entries = a.batch;
+    if (BLOCKS) {
+      // (a launch has fewer requests than entries) the blocks of each request,
+      // `each` to an entry so that all fit
+      static_assert(!BLOCKS || kLineBatch <= THREADS, "an entry a thread");
+      int blocks = 0, none = 0, all = 0, x;
+      if (t < a.batch) blocks = (request_of(a, t, bad).row1 + ROWS - 1) / ROWS;
+      int before = blocks;
+      scan(before, none, all, x);
+      const int each = max(1, (all + kLineBatch - a.batch - 1) / max(1, kLineBatch - a.batch));
+      int at = (blocks + each - 1) / each;
+      scan(at, none, entries, x);
+      if (t < a.batch) s.starts[t] = at;
+      if (t == 0) s.starts[a.batch] = entries;
+      __syncthreads();
+      if (t < entries) {
+        const int b = last_not_above(s.starts, a.batch, t);
+        Request r = request_of(a, b, bad);
+        r.row0 = (t - s.starts[b]) * each * ROWS;
+        r.row1 = min(r.row1, r.row0 + each * ROWS);
+        r.tl = tiles_of<TK>(a, r.len - r.n + div_group(a, r.row0), r.len - r.n + div_group(a, r.row1 - 1), r.len);
+        s.req[t] = r;
       }
-      s.req[b] = r;
-      s.tiles_pre[b + 1] = n;
-      s.units_pre[b + 1] = u;
-      nt += n;
-      nu += u;
+    } else {
+      for (int b = t; b < entries; b += THREADS) {
+        Request r = request_of(a, b, bad);
+        if (r.n > 0) r.tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
+        s.req[b] = r;
+      }
     }
     if (bad && blockIdx.x == 0) report(a.status, kStatusBadIndex);
-    int it = nt, iu = nu;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, it, d), y = __shfl_up_sync(0xffffffffu, iu, d);
-      if (lane >= d) it += x, iu += y;
-    }
-    if (lane == 31) s.wsum[warp][0] = it, s.wsum[warp][1] = iu;
     __syncthreads();
-    it -= nt, iu -= nu;
-    for (int w = 0; w < warp; ++w) it += s.wsum[w][0], iu += s.wsum[w][1];
+    const int per = (entries + THREADS - 1) / THREADS;
+    const int b0 = t * per, b1 = min(entries, b0 + per);
+    auto units_of = [&](const Request &r) {
+      return r.row1 > r.row0 ? (r.row1 - r.row0 + ROWS - 1) / ROWS * a.heads_kv : 0;
+    };
+    int it = 0, iu = 0, x, y;
     for (int b = b0; b < b1; ++b) {
-      it += s.tiles_pre[b + 1], iu += s.units_pre[b + 1];
-      s.tiles_pre[b + 1] = it, s.units_pre[b + 1] = iu;
+      const int u = units_of(s.req[b]);
+      iu += u;
+      if (u > 0) it += s.req[b].tl.n * u;
     }
-    if (t == 0) s.tiles_pre[0] = s.units_pre[0] = 0;
+    scan(it, iu, x, y);
+    for (int b = b0; b < b1; ++b) {
+      const int u = units_of(s.req[b]);
+      s.tiles_pre[b] = it, s.units_pre[b] = iu;
+      iu += u;
+      if (u > 0) it += s.req[b].tl.n * u;
+    }
+    if (t == 0) s.tiles_pre[entries] = x, s.units_pre[entries] = y;
     __syncthreads();
-    total = cost_before(a.batch);
+    total = cost_before(entries);
     ctas = min(static_cast<int>(gridDim.x), (total + per_cta - 1) / per_cta);
     step = ctas > 0 ? total / ctas : 0;
     rest = ctas > 0 ? total % ctas : 0;
@@ -242,10 +290,10 @@ struct Line {
   // workspace (some 4 us), whole units wait for nobody.
   __device__ __forceinline__ int place(int x, bool snap, int &tile) const {
     if (x >= total) {
-      tile = s.tiles_pre[a.batch];
+      tile = s.tiles_pre[entries];
       return total;
     }
-    int lo = 0, hi = a.batch;
+    int lo = 0, hi = entries;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (cost_before(mid) <= x)
@@ -274,19 +322,17 @@ struct Line {
     while (even(c) > x) --c;
     return c;
   }
-  // The request of tile g of the line, and the unit: its tiles from ut0 on follow.
-  __device__ __forceinline__ int request_at(int g) const {
-    return last_not_above(s.tiles_pre, a.batch, g);
-  }
+  // The entry of tile g of the line, and the unit: its tiles from ut0 on follow.
+  __device__ __forceinline__ int entry_at(int g) const { return last_not_above(s.tiles_pre, entries, g); }
   __device__ __forceinline__ Unit unit_at(int g, int b, const Request &r, int &ut0) const {
-    const int rows = r.n * a.group, blocks = (rows + ROWS - 1) / ROWS;
+    const int blocks = (r.row1 - r.row0 + ROWS - 1) / ROWS;
     const int in = g - s.tiles_pre[b], u = in / r.tl.n;
     ut0 = in - u * r.tl.n;
     Unit un;
     un.t0 = r.t0;
     un.hk = blocks == 1 ? u : u / blocks;
-    un.row0 = (u - un.hk * blocks) * ROWS;
-    un.rows = min(ROWS, rows - un.row0);
+    un.row0 = r.row0 + (u - un.hk * blocks) * ROWS;
+    un.rows = min(ROWS, r.row1 - un.row0);
     un.cost = cost_before(b) + u * (r.tl.n + COST);
     un.n = r.tl.n;
     return un;

@@ -86,7 +86,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   extern __shared__ uint8_t dyn[];
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
   float *parts = reinterpret_cast<float *>(sm);  // [warps][ROWS][PITCH], in the spent ring
-  using L = Line<TK, ROWS, kSplitThreads, kUnitCost, kWholeUnit>;
+  using L = Line<TK, ROWS, kSplitThreads, kUnitCost, kWholeUnit, false>;
   __shared__ typename L::Shared line_sm;
   __shared__ __align__(8) uint64_t bars[kSplitWarps * NST];
   __shared__ float part_ml[kSplitWarps][ROWS][2];
@@ -143,7 +143,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     row0 = row1 = -1;
     if (k + lane < nk) {
       const int g = c0 + k + lane;
-      const int b = line.request_at(g);
+      const int b = line.entry_at(g);
       const Request r = line_sm.req[b];
       int ut;
       const int hk = line.unit_at(g, b, r, ut).hk, key = r.tl.key_tile(ut) * TK;
@@ -197,7 +197,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   uint4 raw[NT][H * 2];  // row 8 n + gid, channels 16 H tig .. + 16 H - 1
   float hp[NT][2];       // of rows 8 n + 2 tig + e, as in the columns of S^T
   auto begin_unit = [&](int k) {
-    const int g = c0 + k, b = line.request_at(g);
+    const int g = c0 + k, b = line.entry_at(g);
     const Request rq = line_sm.req[b];
     len = rq.len;
     p0 = len - rq.n;

@@ -134,7 +134,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                 GROUPS = C::GROUPS;
   constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
   constexpr float LOG2E = 1.4426950408889634f;
-  using L = Line<TK, ROWS, kTiledThreads, kTiledCost, kTiledWhole>;
+  using L = Line<TK, ROWS, kTiledThreads, kTiledCost, kTiledWhole, true>;
   extern __shared__ uint8_t dyn[];
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
   const uint32_t sb = ptx::smem_u32(sm);
@@ -189,13 +189,13 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   struct Here {
     Unit un;
     Request rq;
-    int b, ut0, nt, p0, lo_max, hi_min;
+    int ut0, nt, p0, lo_max, hi_min;
   };
   auto unit_at = [&](int k) {
     Here h;
-    h.b = line.request_at(c0 + k);
-    h.rq = line_sm.req[h.b];
-    h.un = line.unit_at(c0 + k, h.b, h.rq, h.ut0);
+    const int e = line.entry_at(c0 + k);
+    h.rq = line_sm.req[e];
+    h.un = line.unit_at(c0 + k, e, h.rq, h.ut0);
     h.nt = min(h.un.n - h.ut0, nk - k);
     h.p0 = h.rq.len - h.rq.n;
     int x;
@@ -239,7 +239,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         x.live = h.rq.len - j0;
         // (the scales of 16 keys that no row sees may be anything)
         if (!(x.key < min(a.prefix, h.rq.len) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
-        if (lane < GROUPS && x.key < h.rq.len) x.pg = a.block_table[h.b * a.table_stride + (x.key >> pshift)];
+        if (lane < GROUPS && x.key < h.rq.len) x.pg = a.block_table[h.rq.b * a.table_stride + (x.key >> pshift)];
         return x;
       };
       int issued = 0;
@@ -649,7 +649,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         m_run -= kTiledPTop;  // what O and the sum are relative to
         uint32_t nan[D / 32] = {};
         if (CT == CACHE_E4M3 && nan_flag && real)
-          nan_channels<D>(a, v_cache, h.b, h.un.hk, h.rq.tl, h.ut0, h.ut0 + h.nt, pos, h.rq.len, h.lo_max,
+          nan_channels<D>(a, v_cache, h.rq.b, h.un.hk, h.rq.tl, h.ut0, h.ut0 + h.nt, pos, h.rq.len, h.lo_max,
                           h.hi_min, nan);
         float f = 1.f;
         row_out<KIND>(a, h.un, min(r, h.un.rows - 1), m_run, l_run, whole && real, f);
@@ -697,6 +697,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             if (D == 64 && !whole) break;
             __syncwarp();
             const int upr = whole ? cols / 8 : 16, rpi = 32 / upr;
+#pragma unroll 4
             for (int x = 0; x < 32; x += rpi) {
               const int lr = x + lane / upr, u = lane % upr, q = w * 128 + base + lr;
               uint4 v;
