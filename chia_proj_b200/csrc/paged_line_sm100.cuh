@@ -230,13 +230,15 @@ struct Line {
       // (a launch has fewer requests than entries) the blocks of each request,
       // `each` to an entry so that all fit
       static_assert(!BLOCKS || kLineBatch <= THREADS, "an entry a thread");
-      int blocks = 0, none = 0, all = 0, x;
+      int blocks = 0, none = 0, x, each = 1;
       if (t < a.batch) blocks = (request_of(a, t, bad).row1 + ROWS - 1) / ROWS;
-      int before = blocks;
-      scan(before, none, all, x);
-      const int each = max(1, (all + kLineBatch - a.batch - 1) / max(1, kLineBatch - a.batch));
-      int at = (blocks + each - 1) / each;
+      int at = blocks;
       scan(at, none, entries, x);
+      if (entries > kLineBatch) {
+        each = (entries + kLineBatch - a.batch - 1) / max(1, kLineBatch - a.batch);
+        at = (blocks + each - 1) / each;
+        scan(at, none, entries, x);
+      }
       if (t < a.batch) s.starts[t] = at;
       if (t == 0) s.starts[a.batch] = entries;
       __syncthreads();

@@ -67,32 +67,49 @@ struct CutUnit {
   int last;
 };
 
-// Merges the parts of the units that are cut: CTA (c, y) rows 16 y .. + 15 of the
-// unit that CTA c of the tiled kernel began, its parts in the order of the line.
+// Merges the parts of the units that are cut: CTA (c, y) some rows of the unit that
+// CTA c of the tiled kernel began, its parts in the order of the line, eight of
+// them in flight at once.
+constexpr int kMergeThreads = 256, kMergeSlices = 16;
 template <int D, int KIND>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const PagedArgs a, const CutUnit *cuts) {
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedArgs a, const CutUnit *cuts) {
   constexpr int ROWS = TiledConfig<D>::ROWS;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the tiled kernel is complete
   const int first = blockIdx.x;
   const CutUnit cu = cuts[first];
-  const int r1 = min(cu.un.rows, 16 * (static_cast<int>(blockIdx.y) + 1));
-  for (int e = 16 * blockIdx.y * (D / 4) + threadIdx.x; e < r1 * (D / 4); e += 128) {
+  for (int e = blockIdx.y * kMergeThreads + threadIdx.x; e < cu.un.rows * (D / 4);
+       e += kMergeSlices * kMergeThreads) {
     const int r = e / (D / 4), c4 = e % (D / 4);
-    auto part = [&](int c) { return (2ll * c + (c == first ? 1 : 0)) * ROWS + r; };
     float M = -INFINITY, L = 0.f;
-#pragma unroll 4
-    for (int c = first; c <= cu.last; ++c) M = fmaxf(M, __ldcg(a.part_ml + part(c) * 2));
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = first; c <= cu.last; ++c) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part(c) * 2));
-      const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part(c) * D + 4 * c4));
-      const float wt = ptx::ex2(ml.x - (M == -INFINITY ? 0.f : M));
-      L = fmaf(wt, ml.y, L);
-      acc.x = fmaf(wt, v.x, acc.x);
-      acc.y = fmaf(wt, v.y, acc.y);
-      acc.z = fmaf(wt, v.z, acc.z);
-      acc.w = fmaf(wt, v.w, acc.w);
+    for (int c0 = first; c0 <= cu.last; c0 += 8) {
+      float2 ml[8];
+      float4 v[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        ml[x] = make_float2(-INFINITY, 0.f);
+        v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c0 + x <= cu.last) {
+          const int64_t part = (2ll * (c0 + x) + (c0 + x == first ? 1 : 0)) * ROWS + r;
+          ml[x] = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part * 2));
+          v[x] = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part * D + 4 * c4));
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) top = fmaxf(top, ml[x].x);
+      const float base = top == -INFINITY ? 0.f : top, old = ptx::ex2(M - base);
+      L *= old, acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+      M = top;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float wt = ptx::ex2(ml[x].x - base);
+        L = fmaf(wt, ml[x].y, L);
+        acc.x = fmaf(wt, v[x].x, acc.x);
+        acc.y = fmaf(wt, v[x].y, acc.y);
+        acc.z = fmaf(wt, v[x].z, acc.z);
+        acc.w = fmaf(wt, v[x].w, acc.w);
+      }
     }
     float f;
     uint16_t *dst = row_out<KIND>(a, cu.un, r, M, L, c4 == 0, f);
@@ -756,8 +773,8 @@ cudaError_t launch_tiled_one(const CUtensorMap &mk, const CUtensorMap &mv, const
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   // the merge may be set up while the last of the tiled CTAs run; it waits for them
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, TiledConfig<D>::ROWS / 16);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(grid, kMergeSlices);
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

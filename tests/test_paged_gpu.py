@@ -362,6 +362,29 @@ def test_many_requests(cuda):
     check_attention([5000, 3, 0, 900] * 3, [1, 2, 1, 4] * 3, 4, 2, 128, 64, E4M3, BF16, max_q=1)
 
 
+def near(a, b, dtype):
+    """Two schedules of the same call: each within the tolerance of the exact result, which both lie beside."""
+    a, b = a.double(), b.double()
+    return ((a - b).abs() <= 2.0 ** (-7 if dtype == BF16 else -10) * torch.maximum(a.abs(), b.abs())
+            + 2.0 ** -9 * b.abs().amax(-1, keepdim=True)).all()
+
+
+def test_long_runs_of_queries(cuda):
+    """More blocks of rows than a CTA keeps entries for, and more requests than one launch takes, in the tiled schedule
+    against the split one."""
+    g = torch.Generator().manual_seed(8)
+    for lens, counts, H in (([20000, 50], [20000, 3], 8), ([70 + i % 50 for i in range(1100)], [1 + i % 40 for i in range(1100)], 4)):
+        page, D, B = 64, 64, len(lens)
+        W = max(po.pages_for(n, page) for n in lens)
+        k, v, ks, vs = make_cache(200, 1, page, D, E4M3, g)
+        table = torch.randint(0, 200, (B, W), generator=g, dtype=torch.int32).cuda()
+        q = torch.randn(sum(counts), H, D, generator=g).to(BF16).cuda()
+        cu = ints([0] + torch.tensor(counts).cumsum(0).tolist())
+        for mask in (cp.CAUSAL, cp.Mask(left=300, right=0)):
+            a, b = (cp.paged_attention(q, k, v, ks, vs, table, ints(lens), cu, max_q=m, mask=mask) for m in (1, 20000))
+            assert near(a, b, BF16)
+
+
 def test_large_and_small_scales(cuda):
     """Scales far from one another in one request; P and V stay within the range of their 16-bit forms."""
     for ct in (E4M3, I8):
