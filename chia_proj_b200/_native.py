@@ -9,8 +9,10 @@ fails to load, importing the operators raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.metadata
+import importlib.util
 import os
-import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -219,18 +221,25 @@ class PagedParams(ctypes.Structure):
     ]
 
 
-def packer(struct_type):
-    """``struct.Struct(...).pack`` for a ctypes structure of this file: all
-    fields in one call, which is several times quicker than setting them one by
-    one. Arrays take one value an element."""
-    codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_uint64: "Q", ctypes.c_float: "f",
-             ctypes.c_void_p: "Q"}
-    fmt = ""
-    for _, t in struct_type._fields_:
-        fmt += codes[t._type_] * t._length_ if hasattr(t, "_length_") else codes[t]
-    s = struct.Struct("@" + fmt)
-    assert s.size == ctypes.sizeof(struct_type), struct_type
-    return s.pack
+_binding_module = None
+
+
+def binding():
+    """The compiled argument checks of ``paged.py`` (``csrc/binding.cpp``),
+    given the entry points of the library. Raises if it has not been built."""
+    global _binding_module
+    if _binding_module is not None:
+        return _binding_module
+    lib = load()
+    path = os.path.join(_HERE, "_lib", f"_binding-{importlib.metadata.version('torch')}.so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python -m chia_proj_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_binding", path)
+    m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+    loader.exec_module(m)
+    m.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in PAGED_SYMBOLS))
+    _binding_module = m
+    return m
 
 
 class ChiaError(RuntimeError):

@@ -5,18 +5,23 @@
 The library is a plain shared object with C linkage (``include/chia_attn.h``,
 ``include/chia_paged.h``);
 it links the CUDA runtime statically and fetches ``cuTensorMapEncodeTiled``
-from the driver at run time, so it needs no libcuda at link time.
+from the driver at run time, so it needs no libcuda at link time. Beside it
+stands a small CPython module (``csrc/binding.cpp``) that checks the tensors of
+the paged cache's operators.
 """
 
 from __future__ import annotations
 
 import argparse
 import glob
+import importlib.metadata
+import importlib.util
 import os
 import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -24,6 +29,9 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "_lib", "libchia_attn.so")
 OBJ = os.path.join(HERE, "_lib", "_build")
+# the binding is compiled against one torch version and named after it
+BINDING_SRC = os.path.join(CSRC, "binding.cpp")
+BINDING = os.path.join(HERE, "_lib", f"_binding-{importlib.metadata.version('torch')}.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -50,10 +58,31 @@ def _deps():
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not _binding_up_to_date():
         return False
     t = os.path.getmtime(OUT)
     return all(os.path.getmtime(d) <= t for d in _deps())
+
+
+def _binding_up_to_date() -> bool:
+    newest = max(os.path.getmtime(p) for p in (BINDING_SRC, *_headers(BINDING_SRC)))
+    return os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest
+
+
+def _build_binding(force: bool) -> None:
+    """The CPython module over torch's C++ tensors (g++; no device code)."""
+    if not force and _binding_up_to_date():
+        return
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    inc, lib = os.path.join(torch, "include"), os.path.join(torch, "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1", "-o", BINDING + ".tmp", BINDING_SRC,
+           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-isystem", cuda, "-I", sysconfig.get_paths()["include"], "-L", lib, "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    subprocess.run(cmd, check=True)
+    os.replace(BINDING + ".tmp", BINDING)
 
 
 def _headers(src: str, seen=None):
@@ -92,8 +121,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
         os.replace(obj + ".tmp", obj)
         return obj
 
-    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+    with ThreadPoolExecutor((os.cpu_count() or 1) + 1) as pool:
+        binding = pool.submit(_build_binding, force)
         objects = list(pool.map(compile_one, sources()))
+        binding.result()
     tmp = OUT + ".tmp"
     subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", tmp, *objects], check=True)
     os.replace(tmp, OUT)

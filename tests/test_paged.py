@@ -109,14 +109,6 @@ def test_paged_refusals(lib, change, code):
     assert lib.chia_paged_attn_workspace_bytes(packed(N.PagedParams, **PAGED)) > 0
 
 
-def test_packer_matches_the_struct():
-    pack = N.packer(N.PagedParams)
-    n = sum(getattr(t, "_length_", 1) for _, t in N.PagedParams._fields_)
-    s = N.PagedParams.from_buffer_copy(pack(*range(1, n + 1)))
-    assert (s.abi_version, s.max_q, s.batch, s.wait_limit_ns) == (1, 10, 11, n)
-    assert (list(s.q_stride), list(s.o_stride), s.scale) == ([18, 19], [20, 21], 31.0)
-
-
 def test_no_cpu_fallback(lib):
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
