@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -154,10 +155,21 @@ PyObject *guarded(F f) {
   return nullptr;
 }
 
+// Elements [at, at + n) of a 1-D tensor, sharing its storage (narrow() takes ten
+// times as long to set up).
+Tensor piece(const Tensor &buf, int64_t at, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()),
+                                                      buf.key_set(), buf.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 // --------------------------------------------------------------------- tables
 // seq_lens, lens, block_table, free_pages, free_state, page_size, max_tokens (-1: release), status
 PyObject *tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;  // outputs carry no gradients
     const Args a(args, nargs, 8);
     const Tensor &lens = a.tensor(0, "seq_lens", 1);
     const at::Device dev = lens.device();
@@ -203,7 +215,7 @@ PyObject *tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const int64_t at[5] = {0, T, 2 * T, 2 * T + B + 1, 2 * T + 2 * B + 1}, n[5] = {T, T, B + 1, B, 2};
     PyObject *out = PyTuple_New(release ? 2 : 5);
     for (int i = release ? 3 : 0, j = 0; i < 5; ++i, ++j)
-      PyTuple_SET_ITEM(out, j, THPVariable_Wrap(buf.narrow(0, at[i], n[i])));
+      PyTuple_SET_ITEM(out, j, THPVariable_Wrap(piece(buf, at[i], n[i])));
     return out;
   });
 }
@@ -212,6 +224,7 @@ PyObject *tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 // k, v, slots, k_cache, v_cache, k_scale, v_scale, status
 PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;  // outputs carry no gradients
     const Args a(args, nargs, 8);
     const Cache c(a, 3);
     const Tensor *k = &a.tensor(0, "k", 3), *v = &a.tensor(1, "v", 3);
@@ -293,6 +306,7 @@ Tensor workspace(const at::Device &dev, void *stream) {
 // of 5), scale (None: 1 / sqrt(D)), softcap, head_param, sig_bias, out_scale, out, return_lse, wait_limit_ns, status
 PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;
     const Args a(args, nargs, 21);
     const Cache c(a, 1);
     const Tensor *q = &a.tensor(0, "q", 3);

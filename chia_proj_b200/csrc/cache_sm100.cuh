@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
   __shared__ int32_t s_cu[kTablesThreads + 1], s_len[kTablesThreads], s_first[kTablesThreads];
   const int t = threadIdx.x, shift = 31 - __clz(a.page);
   const bool first_cta = blockIdx.x == 0;
+  follow();
   int head = a.free_state[0], count = a.free_state[1];
   if (head < 0 || head >= a.ring || count < 0 || count > a.ring) {
     if (t == 0 && first_cta) report(a.status, kStatusBadIndex);
@@ -176,6 +177,7 @@ __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const Tab
   __shared__ int32_t s_at[kTablesThreads + 1];
   const int t = threadIdx.x;
   const bool first_cta = blockIdx.x == 0;
+  follow();
   int head = a.free_state[0], count = a.free_state[1];
   if (head < 0 || head >= a.ring || count < 0 || count > a.ring) {
     if (t == 0 && first_cta) report(a.status, kStatusBadIndex);
@@ -264,6 +266,7 @@ __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(con
   const uint16_t *src = static_cast<const uint16_t *>(is_v ? a.v : a.k) + h * (is_v ? a.v_sh : a.k_sh) +
                         (tid % LANES) * 8;
   const int64_t st = is_v ? a.v_st : a.k_st;
+  follow();
   for (int e = tid; e < window + PAGE; e += 128) {  // (a run that begins in the window ends here)
     const int x = w0 - 1 + e;
     s_slot[e] = x >= 0 && x < a.tokens ? a.slots[x] : -1;

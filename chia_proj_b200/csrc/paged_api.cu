@@ -34,7 +34,7 @@ int device_sms(int &sms) {
   return CHIA_OK;
 }
 
-int launched() { return cudaGetLastError() == cudaSuccess ? CHIA_OK : CHIA_ERR_LAUNCH; }
+int launched(cudaError_t e) { return e == cudaSuccess ? CHIA_OK : CHIA_ERR_LAUNCH; }
 
 // ---------------------------------------------------------------------- tables
 int tables_args(const chia_tables_params_t *p, bool release, chia::TablesArgs &a) {
@@ -122,14 +122,16 @@ int launch_append(const chia::AppendArgs &a, int sms, cudaStream_t s) {
   const int64_t grid = (a.tokens + window - 1) / window * kinds;
   if (grid > kI32) return CHIA_ERR_UNSUPPORTED;
   const unsigned g = static_cast<unsigned>(grid);
+  auto run = [&](void (*kernel)(chia::AppendArgs, int)) {
+    return launched(chia::launch_after(kernel, dim3(g), 128, 0, s, a, window));
+  };
   switch (a.page * D / 1024) {
-    case 1: chia::cache_append_kernel<64, BF16, CT, 1><<<g, 128, 0, s>>>(a, window); break;
-    case 2: chia::cache_append_kernel<D, BF16, CT, 2><<<g, 128, 0, s>>>(a, window); break;
-    case 4: chia::cache_append_kernel<D, BF16, CT, 4><<<g, 128, 0, s>>>(a, window); break;
-    case 8: chia::cache_append_kernel<D, BF16, CT, 8><<<g, 128, 0, s>>>(a, window); break;
-    default: chia::cache_append_kernel<128, BF16, CT, 16><<<g, 128, 0, s>>>(a, window); break;
+    case 1: return run(chia::cache_append_kernel<64, BF16, CT, 1>);
+    case 2: return run(chia::cache_append_kernel<D, BF16, CT, 2>);
+    case 4: return run(chia::cache_append_kernel<D, BF16, CT, 4>);
+    case 8: return run(chia::cache_append_kernel<D, BF16, CT, 8>);
+    default: return run(chia::cache_append_kernel<128, BF16, CT, 16>);
   }
-  return launched();
 }
 
 // ------------------------------------------------------------------- attention
@@ -271,18 +273,16 @@ int chia_page_tables(const chia_tables_params_t *p, void *stream) {
   chia::TablesArgs a{};
   int rc = tables_args(p, false, a), sms = 0;
   if (rc != CHIA_OK || (rc = device_sms(sms)) != CHIA_OK) return rc;
-  chia::page_tables_kernel<<<tables_grid(p->max_tokens, sms), chia::kTablesThreads, 0,
-                             static_cast<cudaStream_t>(stream)>>>(a);
-  return launched();
+  return launched(chia::launch_after(chia::page_tables_kernel, dim3(tables_grid(p->max_tokens, sms)), chia::kTablesThreads, 0,
+                                     static_cast<cudaStream_t>(stream), a));
 }
 
 int chia_release_pages(const chia_tables_params_t *p, void *stream) {
   chia::TablesArgs a{};
   int rc = tables_args(p, true, a), sms = 0;
   if (rc != CHIA_OK || (rc = device_sms(sms)) != CHIA_OK) return rc;
-  chia::release_pages_kernel<<<tables_grid(p->ring_size, sms), chia::kTablesThreads, 0,
-                               static_cast<cudaStream_t>(stream)>>>(a);
-  return launched();
+  return launched(chia::launch_after(chia::release_pages_kernel, dim3(tables_grid(p->ring_size, sms)), chia::kTablesThreads, 0,
+                                     static_cast<cudaStream_t>(stream), a));
 }
 
 int chia_cache_append(const chia_append_params_t *p, void *stream) {

@@ -3,6 +3,7 @@
 // cannot see (lengths, pages, offsets).
 #pragma once
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
 
 #include <cstdint>
 
@@ -18,6 +19,31 @@ constexpr int kMinScaleExp = -64;    // the smallest scale is 2^-64
 
 __device__ __forceinline__ void report(int32_t *status, int bits) {
   if (status != nullptr) atomicOr(status, bits);
+}
+
+// The kernels of a serving step follow one another on a stream and take some
+// microseconds each, so each is launched while the one before still runs
+// (programmatic stream serialisation) and waits for its completion, memory
+// included, before it touches any: follow() is the first thing a kernel does.
+// It lets the next one be set up in turn, whose own wait is for all of this.
+__device__ __forceinline__ void follow() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <class... P, class... A>
+inline cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s,
+                                A &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 // 2^e for -126 <= e <= 127

@@ -117,6 +117,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   }
 
   ptx::fence_barrier_init();
+  follow();
   const L line(line_sm, a, kSplitWarps);  // (its barriers also order the set-up above)
   if (static_cast<int>(blockIdx.x) >= line.ctas) return;
   const int me = blockIdx.x * kSplitWarps + warp;
@@ -748,8 +749,7 @@ cudaError_t launch_split_one(const CUtensorMap &mk, const CUtensorMap &mv, const
   const cudaError_t e = allow_smem(
       reinterpret_cast<const void *>(&paged_split_kernel<D, CT, NT, KIND>), bytes, device, set);
   if (e != cudaSuccess) return e;
-  paged_split_kernel<D, CT, NT, KIND><<<grid, kSplitThreads, bytes, s>>>(mk, mv, a);
-  return cudaGetLastError();
+  return launch_after(paged_split_kernel<D, CT, NT, KIND>, dim3(grid), kSplitThreads, bytes, s, mk, mv, a);
 }
 
 template <int D, int CT, int NT>

@@ -74,7 +74,7 @@ constexpr int kMergeThreads = 256, kMergeSlices = 16;
 template <int D, int KIND>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedArgs a, const CutUnit *cuts) {
   constexpr int ROWS = TiledConfig<D>::ROWS;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the tiled kernel is complete
+  follow();
   const int first = blockIdx.x;
   const CutUnit cu = cuts[first];
   for (int e = blockIdx.y * kMergeThreads + threadIdx.x; e < cu.un.rows * (D / 4);
@@ -179,7 +179,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     ptx::tma_prefetch_desc(&mv);
   }
   ptx::fence_barrier_init();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the merge waits for all of this)
+  follow();
   const L line(line_sm, a, kTiledPiece);
   if (static_cast<int>(blockIdx.x) >= line.ctas) {
     if (t == 0) cuts[blockIdx.x].un.rows = 0;
@@ -768,20 +768,11 @@ cudaError_t launch_tiled_one(const CUtensorMap &mk, const CUtensorMap &mv, const
   cudaError_t e = allow_smem(reinterpret_cast<const void *>(&paged_tiled_kernel<D, CT, KIND>), bytes,
                              device, set);
   if (e != cudaSuccess) return e;
-  paged_tiled_kernel<D, CT, KIND>
-      <<<grid, kTiledThreads, bytes, s>>>(mk, mv, a, v_cache, static_cast<CutUnit *>(cuts));
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  // the merge may be set up while the last of the tiled CTAs run; it waits for them
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, kMergeSlices);
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, KIND>, a, static_cast<const CutUnit *>(cuts));
+  e = launch_after(paged_tiled_kernel<D, CT, KIND>, dim3(grid), kTiledThreads, bytes, s, mk, mv, a, v_cache,
+                   static_cast<CutUnit *>(cuts));
+  if (e != cudaSuccess) return e;
+  return launch_after(paged_merge_kernel<D, KIND>, dim3(grid, kMergeSlices), kMergeThreads, 0, s, a,
+                      static_cast<const CutUnit *>(cuts));
 }
 
 #define CHIA_TILED_CASE(D, CT, KIND) \
