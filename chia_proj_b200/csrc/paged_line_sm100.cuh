@@ -183,6 +183,42 @@ __device__ __forceinline__ void store4(const PagedArgs &a, uint16_t *dst, float 
              : make_uint2(ptx::pack_f16(x0, x1), ptx::pack_f16(x2, x3));
 }
 
+// Channels 4 c4 .. + 3 of row r from the parts that CTAs first..last left of a
+// unit (the first one's is its later part), eight in flight at once.
+template <int ROWS, int D>
+__device__ __forceinline__ void merge_parts(const PagedArgs &a, int first, int last, int r, int c4, float &M,
+                                            float &L, float4 &acc) {
+  for (int c0 = first; c0 <= last; c0 += 8) {
+    float2 ml[8];
+    float4 v[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      ml[x] = make_float2(-INFINITY, 0.f);
+      v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c0 + x <= last) {
+        const int64_t part = (2ll * (c0 + x) + (c0 + x == first ? 1 : 0)) * ROWS + r;
+        ml[x] = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part * 2));
+        v[x] = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part * D + 4 * c4));
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) top = fmaxf(top, ml[x].x);
+    const float base = top == -INFINITY ? 0.f : top, old = ptx::ex2(M - base);
+    L *= old, acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+    M = top;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float wt = ptx::ex2(ml[x].x - base);
+      L = fmaf(wt, ml[x].y, L);
+      acc.x = fmaf(wt, v[x].x, acc.x);
+      acc.y = fmaf(wt, v[x].y, acc.y);
+      acc.z = fmaf(wt, v[x].z, acc.z);
+      acc.w = fmaf(wt, v[x].w, acc.w);
+    }
+  }
+}
+
 // The line of units of ROWS rows and tiles of TK keys, in shared memory: its
 // entries in their order. An entry is a request, or with BLOCKS a block of ROWS
 // rows of one (several, where there are more blocks than entries fit): blocks

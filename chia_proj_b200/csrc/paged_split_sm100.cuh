@@ -138,42 +138,59 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 
   // ---- loads
   // Of tile 32 * (k / 32) + lane: rows of the tensor map (page * heads_kv + head), first token.
+  // The next 32 tiles' pages are asked for while the first of these 32 are
+  // computed, their scales a while later, and both are looked at when they are
+  // needed: with HBM busy a load takes longer than the ring lasts.
   const int pshift = 31 - __clz(a.page);
   int row0 = -1, row1 = -1, tok = 0;
-  auto look_up = [&](int k) {
-    row0 = row1 = -1;
+  int next_pg0 = -1, next_pg1 = -1, next_hk = 0, next_tok = 0;  // pages
+  int wanted = 0;                                                // bits: that there are such keys
+  float next_ks0 = 0.f, next_vs0 = 0.f, next_ks1 = 0.f, next_vs1 = 0.f;
+  auto ask_pages = [&](int k) {
+    next_pg0 = next_pg1 = -1, wanted = 0;
     if (k + lane < nk) {
       const int g = c0 + k + lane;
       const int b = line.entry_at(g);
       const Request r = line_sm.req[b];
       int ut;
-      const int hk = line.unit_at(g, b, r, ut).hk, key = r.tl.key_tile(ut) * TK;
+      next_hk = line.unit_at(g, b, r, ut).hk;
+      const int key = r.tl.key_tile(ut) * TK;
       const int32_t *table = a.block_table + b * a.table_stride + (key >> pshift);
-      tok = key & (a.page - 1);
-      const bool want0 = key < r.len, want1 = a.page == 16 && key + 16 < r.len;
-      const int pg0 = want0 ? table[0] : 0, pg1 = want1 ? table[1] : 0;
-      const bool ok0 = pg0 >= 0 && pg0 < a.num_pages, ok1 = pg1 >= 0 && pg1 < a.num_pages;
-      if (want0 && ok0) row0 = pg0 * a.heads_kv + hk;
-      if (want1 && ok1) row1 = pg1 * a.heads_kv + hk;
-      if (!ok0 || !ok1) report(a.status, kStatusBadIndex);
+      next_tok = key & (a.page - 1);
+      if (key < r.len) next_pg0 = table[0], wanted = 1;
+      if (a.page == 16 && key + 16 < r.len) next_pg1 = table[1], wanted = 3;
     }
   };
-  auto look_up_scales = [&](int k) {  // of the same tiles, to shared memory
+  auto row_at = [&](int pg) { return pg >= 0 && pg < a.num_pages ? pg * a.heads_kv + next_hk : -1; };
+  auto ask_scales = [&] {
+    const int r0 = row_at(next_pg0), r1 = row_at(next_pg1);
+    if (r0 >= 0) next_ks0 = a.k_scale[r0], next_vs0 = a.v_scale[r0];
+    if (r1 >= 0) next_ks1 = a.k_scale[r1], next_vs1 = a.v_scale[r1];
+  };
+  auto take_rows = [&] {
+    row0 = row_at(next_pg0), row1 = row_at(next_pg1), tok = next_tok;
+    if ((row0 < 0 && (wanted & 1)) || (row1 < 0 && (wanted & 2))) report(a.status, kStatusBadIndex);
+  };
+  auto take_scales = [&](int k) {  // to shared memory
     float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row0 >= 0) sc.x = a.k_scale[row0], sc.y = value_factor<SOFTMAX>(a.v_scale[row0]);
+    if (row0 >= 0) sc.x = next_ks0, sc.y = value_factor<SOFTMAX>(next_vs0);
     if (a.page != 16)
       sc.z = sc.x, sc.w = sc.y;
     else if (row1 >= 0)
-      sc.z = a.k_scale[row1], sc.w = value_factor<SOFTMAX>(a.v_scale[row1]);
+      sc.z = next_ks1, sc.w = value_factor<SOFTMAX>(next_vs1);
     scales[(k + lane) % C::SCALES] = sc;  // (those of 64 tiles ago are long used)
     __syncwarp();
   };
   auto issue = [&](int k) {  // start the copies of tile k, whose stage is free
     if (k >= nk) return;
-    if (k % 32 == 0) look_up(k);
-    const int r0 = __shfl_sync(0xffffffffu, row0, k % 32);
-    const int r1 = __shfl_sync(0xffffffffu, row1, k % 32);
-    const int tk = __shfl_sync(0xffffffffu, tok, k % 32);
+    const int in = k % 32;
+    if (in == 0 && k > 0) {
+      take_rows();
+      take_scales(k);
+    }
+    const int r0 = __shfl_sync(0xffffffffu, row0, in);
+    const int r1 = __shfl_sync(0xffffffffu, row1, in);
+    const int tk = __shfl_sync(0xffffffffu, tok, in);
     if (lane == 0) {
       const uint32_t dst = ring + (k % NST) * C::STAGE, bar = bar0 + 8 * (k % NST);
       const int rows = a.page == 16 ? 16 : TK;
@@ -187,8 +204,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         tma_load_3d(dst + TK * D + 16 * D, &mv, bar, 0, 0, r1);
       }
     }
-    // (at the start the copies leave before the scales are asked for)
-    if (k % 32 == 0 && k > 0) look_up_scales(k);
+    if (in == 12 && k + 20 < nk) ask_pages(k + 20);
+    if (in == 22 && k + 10 < nk) ask_scales();
   };
 
   // ---- units of the piece: the one that tile k belongs to, and its queries
@@ -229,9 +246,12 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     }
   };
   if (nk > 0) {
+    ask_pages(0);
     begin_unit(0);
+    take_rows();
     for (int k = 0; k < NST; ++k) issue(k);
-    look_up_scales(0);
+    ask_scales();
+    take_scales(0);
   }
 
   bool aborted = false, has_end = false;
@@ -489,13 +509,20 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       for (int m = 0; m < 2; ++m) {
         if (m + VP < 2) load_v(m + VP);
         if (CT == CACHE_E4M3 && !all) {  // NaN times a P of zero is not zero
+          uint32_t some[2];  // bytes of keys 16 m + 8 x + 2 tig, + 1 that some row sees
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int j = j0 + 16 * m + 8 * x + 2 * tig;
+            some[x] = (j < pf || (j >= lo_min && j <= hi_max) ? 0x0101u : 0u) |
+                      (j + 1 < pf || (j + 1 >= lo_min && j + 1 <= hi_max) ? 0x01010000u : 0u);
+          }
 #pragma unroll
           for (int c = 0; c < MT / 2; ++c)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               uint32_t &v = vr[m][c][w];
               const uint32_t nan = (((v & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
-              nan_seen |= nan != 0;
+              nan_seen |= (nan & some[w & 1]) != 0;
               v &= ~(nan * 0xffu);
             }
         }
@@ -718,17 +745,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     const int first = line.cta_of(un, 0), last = line.cta_of(un, un.n - 1);
     for (int e = t; e < un.rows * (D / 4); e += kSplitThreads) {
       const int r = e / (D / 4), c4 = e % (D / 4);
-      auto part = [&](int c) { return (2ll * c + (c == first ? 1 : 0)) * ROWS + r; };
       float M = -INFINITY, L = 0.f;
-#pragma unroll 4
-      for (int c = first; c <= last; ++c) M = fmaxf(M, __ldcg(a.part_ml + part(c) * 2));
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int c = first; c <= last; ++c) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part(c) * 2));
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part(c) * D + 4 * c4));
-        add(acc, L, ptx::ex2(ml.x - (M == -INFINITY ? 0.f : M)), v, ml.y);
-      }
+      merge_parts<ROWS, D>(a, first, last, r, c4, M, L, acc);
       float f;
       uint16_t *dst = row_out<KIND>(a, un, r, M, L, c4 == 0, f);
       store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);

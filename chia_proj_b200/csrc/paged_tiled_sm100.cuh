@@ -82,35 +82,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedA
     const int r = e / (D / 4), c4 = e % (D / 4);
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c0 = first; c0 <= cu.last; c0 += 8) {
-      float2 ml[8];
-      float4 v[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        ml[x] = make_float2(-INFINITY, 0.f);
-        v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c0 + x <= cu.last) {
-          const int64_t part = (2ll * (c0 + x) + (c0 + x == first ? 1 : 0)) * ROWS + r;
-          ml[x] = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + part * 2));
-          v[x] = __ldcg(reinterpret_cast<const float4 *>(a.part_o + part * D + 4 * c4));
-        }
-      }
-      float top = M;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) top = fmaxf(top, ml[x].x);
-      const float base = top == -INFINITY ? 0.f : top, old = ptx::ex2(M - base);
-      L *= old, acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
-      M = top;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const float wt = ptx::ex2(ml[x].x - base);
-        L = fmaf(wt, ml[x].y, L);
-        acc.x = fmaf(wt, v[x].x, acc.x);
-        acc.y = fmaf(wt, v[x].y, acc.y);
-        acc.z = fmaf(wt, v[x].z, acc.z);
-        acc.w = fmaf(wt, v[x].w, acc.w);
-      }
-    }
+    merge_parts<ROWS, D>(a, first, cu.last, r, c4, M, L, acc);
     float f;
     uint16_t *dst = row_out<KIND>(a, cu.un, r, M, L, c4 == 0, f);
     store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
@@ -234,8 +206,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       // memory is asked for a tile or two ahead and looked at when its turn
       // comes: the page of tile k + 2, the scales of tile k + 1.
       struct Keys {
-        int key, pg;  // pg: -1 where there is nothing to load
-        int hk, all, live;
+        int key, pg;
+        int hk, all, live;  // all: bit 0 every row sees the tile, 1 no row these keys, 2 there are such keys
       };
       Here h;
       int left = 0, lo_min = 0, hi_max = 0;  // tiles of the unit still to look up
@@ -256,7 +228,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         x.live = h.rq.len - j0;
         // (the scales of 16 keys that no row sees may be anything)
         if (!(x.key < min(a.prefix, h.rq.len) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
-        if (lane < GROUPS && x.key < h.rq.len) x.pg = a.block_table[h.rq.b * a.table_stride + (x.key >> pshift)];
+        if (lane < GROUPS && x.key < h.rq.len) 
+          x.pg = a.block_table[h.rq.b * a.table_stride + (x.key >> pshift)], x.all |= 4;
         return x;
       };
       int issued = 0;
@@ -276,7 +249,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       for (int k = 0; k < nk; ++k) {
         const Keys now = k1;
         row = row1, ks = ks1, vs = vs1;
-        if (row < 0 && (now.pg != -1)) report(a.status, kStatusBadIndex);
+        if (row < 0 && (now.all & 4)) report(a.status, kStatusBadIndex);
         if (lane < GROUPS) {
           float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
           if (row >= 0 && !(now.all & 2)) {

@@ -481,6 +481,16 @@ def test_bad_pages_and_lengths_are_reported(cuda):
     assert torch.equal(cp.paged_attention(q, k, v, ks, vs, ints(table), ints([70, 33]), ints(cu)), good)
 
 
+@pytest.mark.parametrize("page", [-1, -2 ** 31, 2 ** 31 - 1])
+@pytest.mark.parametrize("counts", [[1, 1], [100, 90]])
+def test_every_bad_page_is_reported(cuda, page, counts):
+    q, k, v, ks, vs, table, cu = setup([300, 133], counts, 8, 2, 64, 64, I8, F16)
+    table[1][1] = page
+    cp.paged_attention(q, k, v, ks, vs, ints(table), ints([300, 133]), ints(cu))
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+
+
 def test_other_streams_and_a_graph(cuda):
     q, k, v, ks, vs, table, cu = setup([5000, 100], [1, 1], 8, 2, 128, 64, E4M3, BF16)
     args = (q, k, v, ks, vs, ints(table), ints([5000, 100]), ints(cu))
