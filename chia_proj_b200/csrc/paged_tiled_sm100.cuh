@@ -137,6 +137,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   __shared__ __align__(8) uint64_t bars[BARS];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, nan_flag;
+  __shared__ float q_scale[256];  // of the rows of Q, undone in the scores
   __shared__ int tile_full[SETS], tile_live[SETS];  // all rows see the whole tile; keys there are
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   auto bar = [&](int i) { return ptx::smem_u32(bars) + 8 * i; };
@@ -437,51 +438,54 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         const int qi = div_group(a, rr), head = h.un.hk * a.group + rr - qi * a.group;
         const int pos = h.p0 + qi;
         // ---- the row of Q, as halves
-        // (16 bytes a lane, neighbouring lanes along a row)
-        float rowmul = 0.f;
+        // (16 bytes a lane, neighbouring lanes along a row, four loads on their way
+        // while four are converted: unrolled further, fetching the code takes longer)
+        float rowmul = a.score_scale;
         {
-          constexpr int UPR = D / 8, RPI = 32 / UPR, IT = 32 / RPI;  // units a row, rows a load, loads
-          const int u = lane % UPR, sub = lane / UPR, base = (warp & 3) * 32;
-          uint4 raw[IT];
-#pragma unroll
-          for (int x = 0; x < IT; ++x) {
-            const int q = w * 128 + base + x * RPI + sub, qr = h.un.row0 + q;
+          constexpr int UPR = D / 8, RPI = 32 / UPR, IT = 32 / RPI, AHEAD = 4;
+          const int u = lane % UPR, q0 = w * 128 + (warp & 3) * 32 + lane / UPR;  // row of the first load
+          uint4 raw[AHEAD];
+          auto load = [&](int x) {
+            const int q = q0 + x * RPI, qr = h.un.row0 + q;
             const int qt = div_group(a, qr), qh = h.un.hk * a.group + qr - qt * a.group;
-            raw[x] = q < h.un.rows ? *reinterpret_cast<const uint4 *>(
-                                         static_cast<const uint16_t *>(a.q) +
-                                         static_cast<int64_t>(h.un.t0 + qt) * a.q_st + qh * a.q_sh + 8 * u)
-                                   : make_uint4(0, 0, 0, 0);
-          }
-          auto two = [&](uint32_t v) {
-            return a.bf16 ? in16x2_to_float2<true>(v) : in16x2_to_float2<false>(v);
+            return q < h.un.rows
+                       ? *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) +
+                                                          static_cast<int64_t>(h.un.t0 + qt) * a.q_st +
+                                                          qh * a.q_sh + 8 * u)
+                       : make_uint4(0, 0, 0, 0);
           };
 #pragma unroll
-          for (int x = 0; x < IT; ++x) {
-            const uint32_t v[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
-            float2 f[4];
-            float mx = 0.f;
+          for (int x = 0; x < AHEAD; ++x) raw[x] = load(x);
+#pragma unroll 1
+          for (int x0 = 0; x0 < IT; x0 += AHEAD) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              f[y] = two(v[y]);
-              mx = ptx::max3(mx, fabsf(f[y].x), fabsf(f[y].y));
+            for (int x = 0; x < AHEAD; ++x) {
+              const uint32_t v[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+              if (x0 + AHEAD < IT) raw[x] = load(x0 + AHEAD + x);
+              float2 f[4];
+              float mx = 0.f;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                f[y] = a.bf16 ? in16x2_to_float2<true>(v[y]) : in16x2_to_float2<false>(v[y]);
+                mx = ptx::max3(mx, fabsf(f[y].x), fabsf(f[y].y));
+              }
+#pragma unroll
+              for (int d = 1; d < UPR; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+              int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+              e = max(-100, min(127, e));
+              const float up = pow2f(14 - e);
+              const int q = q0 + (x0 + x) * RPI;
+              ptx::st_shared_v4(sb + w * C::Q_TILE + (u / 8) * C::Q_CHUNK + (q & 127) * 128 +
+                                    (((u % 8) ^ (q & 7)) << 4),
+                                ptx::pack_f16(f[0].x * up, f[0].y * up), ptx::pack_f16(f[1].x * up, f[1].y * up),
+                                ptx::pack_f16(f[2].x * up, f[2].y * up), ptx::pack_f16(f[3].x * up, f[3].y * up));
+              if (u == 0) q_scale[q] = pow2f(e - 14);
             }
-#pragma unroll
-            for (int d = 1; d < UPR; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
-            e = max(-100, min(127, e));
-            const float up = pow2f(14 - e);
-            const int qrow = base + x * RPI + sub;
-            ptx::st_shared_v4(sb + w * C::Q_TILE + (u / 8) * C::Q_CHUNK + qrow * 128 +
-                                  (((u % 8) ^ (qrow & 7)) << 4),
-                              ptx::pack_f16(f[0].x * up, f[0].y * up), ptx::pack_f16(f[1].x * up, f[1].y * up),
-                              ptx::pack_f16(f[2].x * up, f[2].y * up), ptx::pack_f16(f[3].x * up, f[3].y * up));
-            // the power of two of each row goes to its thread
-            const float down = __shfl_sync(0xffffffffu, pow2f(e - 14), (lane % RPI) * UPR);
-            if (lane / RPI == x) rowmul = a.score_scale * down;
           }
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(bar(Q_FULL + w));
+          rowmul *= q_scale[r];
         }
         const float hp = a.head_param != nullptr ? a.head_param[head] : 1.f;
         float slope = 0.f;
@@ -644,64 +648,57 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         float f = 1.f;
         row_out<KIND>(a, h.un, min(r, h.un.rows - 1), m_run, l_run, whole && real, f);
         // Through this warp's rows of Q's memory (free: the unit's UMMAs are
-        // complete), so that neighbouring lanes write along a row: 16-byte units,
-        // as halves of 32 rows x 64 or 128 channels, or fp32 of 64 channels.
+        // complete), so that neighbouring lanes write along a row: a pass is 128
+        // bytes of each of 32 rows, 64 channels as halves or 32 as fp32.
         {
-          const int base = (warp & 3) * 32;
-          auto unit16 = [&](int lr, int u) {  // 16 bytes of row lr: where this warp's row of Q was
-            return sb + w * C::Q_TILE + (u >> 3) * C::Q_CHUNK + (base + lr) * 128 + (((u ^ lr) & 7) << 4);
+          const int base = (warp & 3) * 32, cols = whole ? 64 : 32;
+          auto unit16 = [&](int lr, int u) {
+            return sb + w * C::Q_TILE + (base + lr) * 128 + (((u ^ lr) & 7) << 4);
           };
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += (D == 128 && whole) ? 128 : 64) {
-            const int cols = (D == 128 && whole) ? 128 : 64;
+          for (int c0 = 0; c0 < D; c0 += cols) {
 #pragma unroll 1
-            for (int c = 0; c < cols; c += 32) {
-              uint32_t o[32];
-              ptx::tmem_ld32(tO + c0 + c, o);
+            for (int c = 0; c < cols; c += 16) {
+              uint32_t o[16];
+              ptx::tmem_ld16(tO + c0 + c, o);
               ptx::tmem_wait_ld();
-              ptx::reg_fence(o);
-              const uint32_t nn = nan[(c0 + c) / 32];
-              if (CT == CACHE_E4M3 && nn != 0)
-                for (int e = 0; e < 32; ++e) o[e] |= (nn >> e) & 1 ? 0x7fffffffu : 0u;
+              ptx::reg_fence16(o);
+              if (CT == CACHE_E4M3 && nan_flag) {
+                const uint32_t nn = nan[(c0 + c) / 32] >> ((c0 + c) % 32);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] |= (nn >> e) & 1 ? 0x7fffffffu : 0u;
+              }
               if (whole) {
+                uint32_t x[8];
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                  uint32_t x[4];
-#pragma unroll
-                  for (int y = 0; y < 4; ++y) {
-                    const float p = __uint_as_float(o[e + 2 * y]) * f, q = __uint_as_float(o[e + 2 * y + 1]) * f;
-                    x[y] = a.bf16 ? ptx::pack_bf16(p, q) : ptx::pack_f16(p, q);
-                  }
-                  ptx::st_shared_v4(unit16(lane, (c + e) / 8), x[0], x[1], x[2], x[3]);
+                for (int y = 0; y < 8; ++y) {
+                  const float p = __uint_as_float(o[2 * y]) * f, q = __uint_as_float(o[2 * y + 1]) * f;
+                  x[y] = a.bf16 ? ptx::pack_bf16(p, q) : ptx::pack_f16(p, q);
                 }
-              } else if (D == 128) {
+                ptx::st_shared_v4(unit16(lane, c / 8), x[0], x[1], x[2], x[3]);
+                ptx::st_shared_v4(unit16(lane, c / 8 + 1), x[4], x[5], x[6], x[7]);
+              } else {
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
+                for (int e = 0; e < 16; e += 4)
                   ptx::st_shared_v4(unit16(lane, (c + e) / 4), o[e], o[e + 1], o[e + 2], o[e + 3]);
-              } else if (real) {
-#pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                  ptx::st_global_v4(a.part_o + (slot * ROWS + r) * D + c + e, o[e], o[e + 1], o[e + 2], o[e + 3]);
               }
             }
-            if (D == 64 && !whole) break;
             __syncwarp();
-            const int upr = whole ? cols / 8 : 16, rpi = 32 / upr;
 #pragma unroll 4
-            for (int x = 0; x < 32; x += rpi) {
-              const int lr = x + lane / upr, u = lane % upr, q = w * 128 + base + lr;
+            for (int x = 0; x < 32; x += 4) {
+              const int lr = x + lane / 8, u = lane % 8, q = w * 128 + base + lr;
               uint4 v;
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                            : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                            : "r"(unit16(lr, u)));
+              const int ch = c0 + u * (whole ? 8 : 4);
               if (q < h.un.rows) {
                 if (whole) {
                   const int qr = h.un.row0 + q, qt = div_group(a, qr), qh = h.un.hk * a.group + qr - qt * a.group;
-                  uint16_t *dst = static_cast<uint16_t *>(a.o) + static_cast<int64_t>(h.un.t0 + qt) * a.o_st +
-                                  qh * a.o_sh;
-                  *reinterpret_cast<uint4 *>(dst + 8 * u) = v;
+                  *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.o) +
+                                             static_cast<int64_t>(h.un.t0 + qt) * a.o_st + qh * a.o_sh + ch) = v;
                 } else {
-                  *reinterpret_cast<uint4 *>(a.part_o + (slot * ROWS + q) * D + c0 + 4 * u) = v;
+                  *reinterpret_cast<uint4 *>(a.part_o + (slot * ROWS + q) * D + ch) = v;
                 }
               }
             }
