@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(con
   constexpr int STEP = 128 / LANES;  // rows of one load of the CTA
   constexpr int PAGE = IT * STEP;    // page_size
   constexpr int SHIFT = PAGE == 16 ? 4 : PAGE == 32 ? 5 : PAGE == 64 ? 6 : 7;
-  __shared__ float s_max[2][4];
+  __shared__ uint32_t s_max[2][4];
   __shared__ int s_slot[2 * PAGE + 1];  // from the token before the window on
   __shared__ unsigned s_same[2][4], s_first[2][4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -315,21 +315,33 @@ __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(con
       if (r < n) x[i] = *reinterpret_cast<const uint4 *>(src + (t0 + r) * st);
     }
     const float old = *scale;
-    float mx = 0.f;
+    // the largest value: 16-bit patterns without their signs order as the values do
+    constexpr uint32_t INF = BF16 ? 0x7f80u : 0x7c00u;
+    uint32_t m2 = 0;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = in16x2_to_float2<BF16>(w[j]);
-        const float u = fabsf(f.x), v = fabsf(f.y);  // (infinities and NaN do not count)
-        mx = fmaxf(mx, fmaxf(u <= 3.4028235e38f ? u : 0.f, v <= 3.4028235e38f ? v : 0.f));
+      for (int j = 0; j < 4; ++j) m2 = __vmaxu2(m2, w[j] & 0x7fff7fffu);
+    }
+    m2 = max(m2 & 0xffffu, m2 >> 16);
+    if (m2 >= INF) {  // infinities and NaN do not count
+      m2 = 0;
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t u = w[j] & 0x7fffu, v = (w[j] >> 16) & 0x7fffu;
+          m2 = max(m2, max(u < INF ? u : 0u, v < INF ? v : 0u));
+        }
       }
     }
-    mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));  // (not negative)
-    if (lane == 0) s_max[par][warp] = mx;
+    m2 = __reduce_max_sync(0xffffffffu, m2);
+    if (lane == 0) s_max[par][warp] = m2;
     __syncthreads();
-    mx = fmaxf(fmaxf(s_max[par][0], s_max[par][1]), fmaxf(s_max[par][2], s_max[par][3]));
+    m2 = max(max(s_max[par][0], s_max[par][1]), max(s_max[par][2], s_max[par][3]));
+    const float mx = in16x2_to_float2<BF16>(m2).x;
     float sc = pow2f(scale_exp<CT>(mx));
     if (!fresh) sc = fmaxf(sc, old);
     const float inv = 1.f / sc;
