@@ -129,11 +129,15 @@ __device__ __forceinline__ Tiles tiles_of(const PagedArgs &a, int p0, int p1, in
 }
 
 // A wait of limited length. After one has run out (`abort`), all return at once.
+// The answer is a lane's own: where lanes go on together the caller takes the
+// warp's (warp_all), since lanes that gave up alone would leave the others waiting
+// for them.
 __device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volatile int *abort,
                                            const PagedArgs &a) {
   if (ptx::mbar_test_wait(bar, parity)) return true;
   const uint64_t t0 = ptx::globaltimer_ns();
-  while (!ptx::mbar_try_wait(bar, parity, 20000u)) {
+  const uint32_t nap = a.timeout_ns < 20000 ? static_cast<uint32_t>(a.timeout_ns) : 20000u;
+  while (!ptx::mbar_try_wait(bar, parity, nap)) {
     if (*abort) return false;
     if (ptx::globaltimer_ns() - t0 > a.timeout_ns) {
       *abort = 1;
@@ -143,6 +147,7 @@ __device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volati
   }
   return true;
 }
+__device__ __forceinline__ bool warp_all(bool x) { return __all_sync(0xffffffffu, x); }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar,
                                             int c0, int c1, int c2) {

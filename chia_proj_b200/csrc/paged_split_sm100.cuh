@@ -319,7 +319,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 
     for (int i = 0; i < nt && !aborted; ++i) {
       const int kk = k + i, stage = kk % NST;
-      if (!paged_wait(bar0 + 8 * stage, (kk / NST) & 1, &abort_flag, a)) {
+      if (!warp_all(paged_wait(bar0 + 8 * stage, (kk / NST) & 1, &abort_flag, a))) {
         // leave no copy in flight: the ring's memory is used again, and the CTA may exit
         PagedArgs d = a;
         d.timeout_ns = a.drain_ns;
@@ -329,7 +329,6 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         aborted = true;
         break;
       }
-      __syncwarp();
       const int j0 = tl.key_tile(ut0 + i) * TK;
       float4 sc = scales[kk % C::SCALES];
       const uint32_t kst = ring + stage * C::STAGE, vst = kst + TK * D;

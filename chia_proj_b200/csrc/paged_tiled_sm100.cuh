@@ -271,7 +271,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         bool ok = true;
         for (int v = 0; v < 2 && ok; ++v) {
           const int item = 2 * k + v, st = item % STAGES;
-          ok = __all_sync(0xffffffffu, wait(ST_EMPTY + st, ((item / STAGES) & 1) ^ 1));
+          ok = warp_all(wait(ST_EMPTY + st, ((item / STAGES) & 1) ^ 1));
           if (!ok) break;
           if (lane == 0) ptx::mbar_arrive_expect_tx(bar(ST_FULL + st), bytes);
           __syncwarp();
@@ -318,24 +318,23 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         ptx::umma_commit_warp(bar(KV_EMPTY + slot));
         if (last) ptx::umma_commit_warp(bar(O_FULL + w));
       };
-      auto all_wait = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, wait(i, parity)); };
       uint32_t tiles = 0, units = 0;
       bool ok = true;
       for (int k = 0; k < nk && ok;) {
         const Here h = unit_at(k);
         if (h.un.rows <= 128 * w) {  // no second query tile: the slots are let go as they come
           for (int i = 2 * k; i < 2 * (k + h.nt) && ok; ++i) {
-            ok = all_wait(KV_FULL + i % SLOTS, (i / SLOTS) & 1);
+            ok = warp_all(wait(KV_FULL + i % SLOTS, (i / SLOTS) & 1));
             if (ok && lane == 0) ptx::mbar_arrive(bar(KV_EMPTY + i % SLOTS));
           }
           k += h.nt;
           continue;
         }
-        ok = all_wait(Q_FULL + w, units & 1);
+        ok = warp_all(wait(Q_FULL + w, units & 1));
         // S of the unit's first two tiles, then behind each PV the S two tiles on
         auto next_s = [&](int i) {
           const int ki = 2 * (k + i);
-          if (!all_wait(KV_FULL + ki % SLOTS, (ki / SLOTS) & 1)) return false;
+          if (!warp_all(wait(KV_FULL + ki % SLOTS, (ki / SLOTS) & 1))) return false;
           ptx::tc_fence_after();
           issue_s((tiles + i) & 1, ki % SLOTS);
           return true;
@@ -344,9 +343,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         for (int i = 0; i < h.nt && ok; ++i) {
           const int vi = 2 * (k + i) + 1;
           const uint32_t n = tiles + i;
-          ok = all_wait(KV_FULL + vi % SLOTS, (vi / SLOTS) & 1) &&
-               all_wait(P_FULL + 2 * w + (n & 1), (n >> 1) & 1) &&
-               (i > 0 || units == 0 || all_wait(O_EMPTY + w, (units - 1) & 1));
+          ok = warp_all(wait(KV_FULL + vi % SLOTS, (vi / SLOTS) & 1) &&
+                        wait(P_FULL + 2 * w + (n & 1), (n >> 1) & 1) &&
+                        (i > 0 || units == 0 || wait(O_EMPTY + w, (units - 1) & 1)));
           if (!ok) break;
           ptx::tc_fence_after();
           issue_pv(n & 1, vi % SLOTS, i == 0, i == h.nt - 1);
@@ -367,8 +366,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       const int c = t - 384;
       for (int item = 0; item < 2 * nk; ++item) {
         const int st = item % STAGES, sl = item % SLOTS;
-        if (!wait(ST_FULL + st, (item / STAGES) & 1)) break;
-        if (!wait(KV_EMPTY + sl, ((item / SLOTS) & 1) ^ 1)) break;
+        // (after a wait that ran out what is read and stored is anything; the vote below ends the work)
+        const bool got = wait(ST_FULL + st, (item / STAGES) & 1) && wait(KV_EMPTY + sl, ((item / SLOTS) & 1) ^ 1);
         const int set = (item / 2) % SETS;
         const bool sift = CT == CACHE_E4M3 && (item & 1) && !tile_full[set];
         bool nan_seen = false;
@@ -411,6 +410,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         if (sift && nan_seen) nan_flag = 1;
         ptx::fence_proxy_async_smem();  // the UMMAs read what was stored
         __syncwarp();
+        if (!warp_all(got)) break;
         if (lane == 0) {
           ptx::mbar_arrive(bar(KV_FULL + sl));
           ptx::mbar_arrive(bar(ST_EMPTY + st));
@@ -499,11 +499,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         float m_run = SOFTMAX ? -INFINITY : -100.f, l_run = 0.f;
         for (int i = 0; i < h.nt; ++i, ++cnt) {
           const int n = k + i;
-          if (!wait(SC_FULL + n % SETS, (n / SETS) & 1) ||
-              !wait(S_FULL + 2 * w + (cnt & 1), (cnt >> 1) & 1)) {
-            ok = false;
-            break;
-          }
+          // (after a wait that ran out S is anything; the vote below ends the work before P is stored)
+          const bool got = wait(SC_FULL + n % SETS, (n / SETS) & 1) &&
+                           wait(S_FULL + 2 * w + (cnt & 1), (cnt >> 1) & 1);
           ptx::tc_fence_after();
           const uint32_t tS = tS0 + (cnt & 1) * 64;
           uint32_t sr[2][32];
@@ -590,8 +588,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             l_run *= alpha;
             m_run = m_new;
           }
-          if (i > 0 && __any_sync(0xffffffffu, need)) {  // O is rescaled once the tile before is in it
-            if (!__all_sync(0xffffffffu, wait(PV_DONE + w, (cnt - 1) & 1))) {
+          if (__any_sync(0xffffffffu, !got || (need && i > 0))) {
+            // O is rescaled once the tile before is in it
+            if (!warp_all(got && (i == 0 || wait(PV_DONE + w, (cnt - 1) & 1)))) {
               ok = false;
               break;
             }
@@ -634,7 +633,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         }
         if (!ok) break;
         // ---- O
-        if (!wait(O_FULL + w, units & 1)) {
+        if (!warp_all(wait(O_FULL + w, units & 1))) {
           ok = false;
           break;
         }
@@ -710,6 +709,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(O_EMPTY + w));
+      } else {  // no rows for this query tile: it keeps step, so that no phase of the scales is passed by
+        for (int n = k; n < k + h.nt && ok; ++n) ok = warp_all(wait(SC_FULL + n % SETS, (n / SETS) & 1));
+        if (!ok) break;
       }
       k += h.nt;
       // a unit that begins here and goes on in later CTAs

@@ -569,3 +569,29 @@ def test_a_step_end_to_end(cuda):
                 assert rel < 0.06, rel  # e4m3: 2^-4 relative at most, about 2.6% rms in K and in V
             at += n
     assert lens.tolist() == [78, 4, 135] and state.tolist()[1] == 16 - (2 + 1 + 3)
+
+
+@pytest.mark.parametrize("lens,counts,D,waits", [([9000, 700], [1, 1], 64, False), ([9000, 700], [1, 1], 128, False),
+                                                 ([600000, 700], [1, 1], 128, True), ([9000, 700], [200, 130], 64, True),
+                                                 ([9000, 700], [200, 130], 128, True)])
+def test_wait_that_runs_out_is_reported(cuda, lens, counts, D, waits):
+    """A wait that is not met at once runs out under a limit of a nanosecond: the kernel reports it, drains its copies and
+    MMAs and returns; the next call on the same device and workspace is right. (Single tokens whose keys are in L2 find
+    their tiles there when they ask for them: no wait runs out, and the result is right.)"""
+    q, k, v, ks, vs, table, cu = setup(lens, counts, 8, 2, D, 64, E4M3, BF16)
+    args = (q, k, v, ks, vs, ints(table), ints(lens), ints(cu))
+    want = cp.paged_attention(*args)
+    cp.check_device_status(0)
+    code = 0
+    for _ in range(3):  # waits that all happen to be met at once would not run out
+        got = cp.paged_attention(*args, wait_limit_ns=1)
+        torch.cuda.synchronize()
+        try:
+            cp.check_device_status(0)
+        except cp.ChiaError as e:
+            code = e.code
+            break
+        assert torch.equal(got, want)
+    assert code == 5 or (code == 0 and not waits), "no wait ran out"
+    for _ in range(2):
+        assert torch.equal(cp.paged_attention(*args), want)
