@@ -175,6 +175,12 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   const uint32_t tmem = tmem_slot;
   auto wait = [&](int i, uint32_t parity) { return paged_wait(bar(i), parity, &abort_flag, a); };
 
+  // both of two: asked for together, since an answer takes some 100 cycles
+  auto wait2 = [&](int i, uint32_t pi, int j, uint32_t pj) {
+    const bool x = ptx::mbar_test_wait(bar(i), pi), y = ptx::mbar_test_wait(bar(j), pj);
+    return (x && y) || (wait(i, pi) && wait(j, pj));
+  };
+
   // the unit of this CTA's tile k
   struct Here {
     Unit un;
@@ -367,7 +373,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       for (int item = 0; item < 2 * nk; ++item) {
         const int st = item % STAGES, sl = item % SLOTS;
         // (after a wait that ran out what is read and stored is anything; the vote below ends the work)
-        const bool got = wait(ST_FULL + st, (item / STAGES) & 1) && wait(KV_EMPTY + sl, ((item / SLOTS) & 1) ^ 1);
+        const bool got = wait2(ST_FULL + st, (item / STAGES) & 1, KV_EMPTY + sl, ((item / SLOTS) & 1) ^ 1);
         const int set = (item / 2) % SETS;
         const bool sift = CT == CACHE_E4M3 && (item & 1) && !tile_full[set];
         bool nan_seen = false;
@@ -500,8 +506,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         for (int i = 0; i < h.nt; ++i, ++cnt) {
           const int n = k + i;
           // (after a wait that ran out S is anything; the vote below ends the work before P is stored)
-          const bool got = wait(SC_FULL + n % SETS, (n / SETS) & 1) &&
-                           wait(S_FULL + 2 * w + (cnt & 1), (cnt >> 1) & 1);
+          const bool got =
+              wait2(SC_FULL + n % SETS, (n / SETS) & 1, S_FULL + 2 * w + (cnt & 1), (cnt >> 1) & 1);
           ptx::tc_fence_after();
           const uint32_t tS = tS0 + (cnt & 1) * 64;
           uint32_t sr[2][32];
