@@ -180,12 +180,14 @@ __device__ __forceinline__ uint16_t *row_out(const PagedArgs &a, const Unit &u, 
         L > 0.f ? (M + __log2f(L)) * 0.6931471805599453f : L == 0.f ? -INFINITY : L;
   return static_cast<uint16_t *>(a.o) + tok * a.o_st + hh * a.o_sh;
 }
+
+template <bool BF16>
 __device__ __forceinline__ void store4(const PagedArgs &a, uint16_t *dst, float f, float x0, float x1,
                                        float x2, float x3) {
   x0 *= f, x1 *= f, x2 *= f, x3 *= f;
   *reinterpret_cast<uint2 *>(dst) =
-      a.bf16 ? make_uint2(ptx::pack_bf16(x0, x1), ptx::pack_bf16(x2, x3))
-             : make_uint2(ptx::pack_f16(x0, x1), ptx::pack_f16(x2, x3));
+      BF16 ? make_uint2(ptx::pack_bf16(x0, x1), ptx::pack_bf16(x2, x3))
+           : make_uint2(ptx::pack_f16(x0, x1), ptx::pack_f16(x2, x3));
 }
 
 // Channels 4 c4 .. + 3 of row r from the parts that CTAs first..last left of a

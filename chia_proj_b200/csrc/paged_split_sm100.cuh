@@ -73,7 +73,7 @@ struct SplitConfig {
 };
 
 // KIND: score modification and normaliser.
-template <int D, int CT, int NT, int KIND>
+template <int D, int CT, int NT, int KIND, bool BF16>
 __global__ void __launch_bounds__(kSplitThreads, 1)
 paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const PagedArgs a) {
@@ -273,7 +273,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       auto get = [&](int w, float2 &x) {  // 32-bit word w of the lane's channels
         const uint4 &r4 = raw[n][w / 4];
         const uint32_t v = w % 4 == 0 ? r4.x : w % 4 == 1 ? r4.y : w % 4 == 2 ? r4.z : r4.w;
-        x = a.bf16 ? in16x2_to_float2<true>(v) : in16x2_to_float2<false>(v);
+        x = in16x2_to_float2<BF16>(v);
       };
 #pragma unroll
       for (int w = 0; w < H * 8; ++w) {
@@ -473,7 +473,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         }
       }
       const float il[2] = {SOFTMAX ? ptx::ex2(-sc.y) : 0.f, SOFTMAX ? ptx::ex2(-sc.w) : 0.f};
-      uint32_t pb[2][NT][2];
+      // P as halves. Beside outputs of 8 bits (bf16) that rounding, 2^-12, is nothing;
+      // outputs of 11 bits get what it left as halves too.
+      uint32_t pb[2][NT][2], rest[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -502,6 +504,18 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           for (int x = 0; x < 2; ++x)
             pb[m][n][x] = movmatrix(ptx::pack_f16(s[m][n][2 * x], s[m][n][2 * x + 1]));
       }
+      if (!BF16) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float p = s[m][n][2 * x], q = s[m][n][2 * x + 1];
+              const float2 f = f16x2_to_float2(ptx::pack_f16(p, q));
+              rest[m][n][x] = movmatrix(ptx::pack_f16(p - f.x, q - f.y));
+            }
+      }
       // ---------------- O^T += V^T P^T
       bool nan_seen = false;
 #pragma unroll
@@ -525,14 +539,18 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               v &= ~(nan * 0xffu);
             }
         }
+        auto add_pv = [&](const uint32_t(&p)[NT][2]) {
 #pragma unroll
-        for (int c = 0; c < MT; ++c) {
-          uint32_t va[4];
-          cache4_to_f16<CT>(__byte_perm(vr[m][c / 2][2 * (c & 1)], 0, 0x3120), va[0], va[1]);
-          cache4_to_f16<CT>(__byte_perm(vr[m][c / 2][2 * (c & 1) + 1], 0, 0x3120), va[2], va[3]);
+          for (int c = 0; c < MT; ++c) {
+            uint32_t va[4];
+            cache4_to_f16<CT>(__byte_perm(vr[m][c / 2][2 * (c & 1)], 0, 0x3120), va[0], va[1]);
+            cache4_to_f16<CT>(__byte_perm(vr[m][c / 2][2 * (c & 1) + 1], 0, 0x3120), va[2], va[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(o[c][n], va, pb[m][n][0], pb[m][n][1]);
-        }
+            for (int n = 0; n < NT; ++n) mma_f16(o[c][n], va, p[n][0], p[n][1]);
+          }
+        };
+        add_pv(pb[m]);
+        if (!BF16) add_pv(rest[m]);
       }
       if (CT == CACHE_E4M3 && !all && __any_sync(0xffffffffu, nan_seen)) {
         // The NaN values left out above go to the rows that do see their keys.
@@ -605,9 +623,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             const float x1 = __shfl_xor_sync(0xffffffffu, odd ? o[c][n][2 + e] : o[c + 1][n][2 + e], 4);
             if (r < un.rows) {
               if (odd)
-                store4(a, dst + 16 * (c + 1), f, x0, x1, o[c + 1][n][e], o[c + 1][n][2 + e]);
+                store4<BF16>(a, dst + 16 * (c + 1), f, x0, x1, o[c + 1][n][e], o[c + 1][n][2 + e]);
               else
-                store4(a, dst + 16 * c, f, o[c][n][e], o[c][n][2 + e], x0, x1);
+                store4<BF16>(a, dst + 16 * c, f, o[c][n][e], o[c][n][2 + e], x0, x1);
             }
           }
         }
@@ -718,7 +736,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     if (!gr.before && !gr.after) {
       float f;
       uint16_t *dst = row_out<KIND>(a, un, r, M, L, c4 == 0, f);
-      store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
+      store4<BF16>(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
     } else {
       const int64_t slot = 2ll * blockIdx.x + (gr.before ? 0 : 1);
       *reinterpret_cast<float4 *>(a.part_o + (slot * ROWS + r) * D + 4 * c4) = acc;
@@ -749,7 +767,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       merge_parts<ROWS, D>(a, first, last, r, c4, M, L, acc);
       float f;
       uint16_t *dst = row_out<KIND>(a, un, r, M, L, c4 == 0, f);
-      store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
+      store4<BF16>(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
     }
   }
 }
@@ -759,26 +777,26 @@ template <int D, int CT>
 cudaError_t launch_split(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a, int kind,
                          int tiles, int grid, int device, cudaStream_t s);
 
-template <int D, int CT, int NT, int KIND>
+template <int D, int CT, int NT, int KIND, bool BF16>
 cudaError_t launch_split_one(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                              int grid, int device, cudaStream_t s) {
   static std::atomic<uint64_t> set{0};
   constexpr int bytes = SplitConfig<D, NT>::SMEM;
   const cudaError_t e = allow_smem(
-      reinterpret_cast<const void *>(&paged_split_kernel<D, CT, NT, KIND>), bytes, device, set);
+      reinterpret_cast<const void *>(&paged_split_kernel<D, CT, NT, KIND, BF16>), bytes, device, set);
   if (e != cudaSuccess) return e;
-  return launch_after(paged_split_kernel<D, CT, NT, KIND>, dim3(grid), kSplitThreads, bytes, s, mk, mv, a);
+  return launch_after(paged_split_kernel<D, CT, NT, KIND, BF16>, dim3(grid), kSplitThreads, bytes, s, mk, mv, a);
 }
 
-template <int D, int CT, int NT>
+template <int D, int CT, int NT, bool BF16>
 cudaError_t launch_split_kind(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                               int kind, int grid, int device, cudaStream_t s) {
   switch (kind) {
-    case KIND_SOFTCAP: return launch_split_one<D, CT, NT, KIND_SOFTCAP>(mk, mv, a, grid, device, s);
-    case KIND_ALIBI: return launch_split_one<D, CT, NT, KIND_ALIBI>(mk, mv, a, grid, device, s);
-    case KIND_SIGMOID: return launch_split_one<D, CT, NT, KIND_SIGMOID>(mk, mv, a, grid, device, s);
-    case KIND_RELU: return launch_split_one<D, CT, NT, KIND_RELU>(mk, mv, a, grid, device, s);
-    default: return launch_split_one<D, CT, NT, KIND_SOFTMAX>(mk, mv, a, grid, device, s);
+    case KIND_SOFTCAP: return launch_split_one<D, CT, NT, KIND_SOFTCAP, BF16>(mk, mv, a, grid, device, s);
+    case KIND_ALIBI: return launch_split_one<D, CT, NT, KIND_ALIBI, BF16>(mk, mv, a, grid, device, s);
+    case KIND_SIGMOID: return launch_split_one<D, CT, NT, KIND_SIGMOID, BF16>(mk, mv, a, grid, device, s);
+    case KIND_RELU: return launch_split_one<D, CT, NT, KIND_RELU, BF16>(mk, mv, a, grid, device, s);
+    default: return launch_split_one<D, CT, NT, KIND_SOFTMAX, BF16>(mk, mv, a, grid, device, s);
   }
 }
 
@@ -787,8 +805,11 @@ cudaError_t launch_split_kind(const CUtensorMap &mk, const CUtensorMap &mv, cons
   cudaError_t chia::launch_split<D, CT>(const CUtensorMap &mk, const CUtensorMap &mv,           \
                                         const PagedArgs &a, int kind, int tiles, int grid,      \
                                         int device, cudaStream_t s) {                           \
-    return tiles == 1 ? launch_split_kind<D, CT, 1>(mk, mv, a, kind, grid, device, s)           \
-                      : launch_split_kind<D, CT, 2>(mk, mv, a, kind, grid, device, s);          \
+    if (a.bf16)                                                                                 \
+      return tiles == 1 ? launch_split_kind<D, CT, 1, true>(mk, mv, a, kind, grid, device, s)   \
+                        : launch_split_kind<D, CT, 2, true>(mk, mv, a, kind, grid, device, s);  \
+    return tiles == 1 ? launch_split_kind<D, CT, 1, false>(mk, mv, a, kind, grid, device, s)    \
+                      : launch_split_kind<D, CT, 2, false>(mk, mv, a, kind, grid, device, s);   \
   }
 
 }  // namespace chia

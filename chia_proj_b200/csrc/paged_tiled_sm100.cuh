@@ -15,7 +15,7 @@
 //   warps 12-15     convert 8-bit tiles to halves
 //
 // Tensor memory: two S buffers of 64 columns for each query tile (P, in halves,
-// takes the first 32 of its S), O0 O1. Shared memory: Q0 Q1 | a ring of
+// takes the first 32 of its S, the rest of its rounding the others), O0 O1. Shared memory: Q0 Q1 | a ring of
 // converted K and V tiles, all in the 128-byte swizzle | a ring of 8-bit tiles
 // as TMA brings them.
 //
@@ -71,7 +71,7 @@ struct CutUnit {
 // CTA c of the tiled kernel began, its parts in the order of the line, eight of
 // them in flight at once.
 constexpr int kMergeThreads = 256, kMergeSlices = 16;
-template <int D, int KIND>
+template <int D, int KIND, bool BF16>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedArgs a, const CutUnit *cuts) {
   constexpr int ROWS = TiledConfig<D>::ROWS;
   follow();
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedA
     merge_parts<ROWS, D>(a, first, cu.last, r, c4, M, L, acc);
     float f;
     uint16_t *dst = row_out<KIND>(a, cu.un, r, M, L, c4 == 0, f);
-    store4(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
+    store4<BF16>(a, dst + 4 * c4, f, acc.x, acc.y, acc.z, acc.w);
   }
 }
 
@@ -114,7 +114,7 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
   }
 }
 
-template <int D, int CT, int KIND>
+template <int D, int CT, int KIND, bool BF16>
 __global__ void __launch_bounds__(kTiledThreads, 1)
 paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const PagedArgs a, const uint8_t *v_cache, CutUnit *cuts) {
@@ -320,6 +320,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         const uint32_t p0 = tS + buf * 64, pa[4] = {p0, p0 + 8, p0 + 16, p0 + 24};
         const uint64_t v0 = dv + ((slot * C::KV) >> 4), vb[4] = {v0, v0 + 128, v0 + 256, v0 + 384};
         ptx::umma_ts_x4_warp(tO, pa, vb, IDESC_PV, first ? 0u : 1u);
+        if (!BF16) {  // what P's rounding left
+          const uint32_t pb[4] = {p0 + 32, p0 + 40, p0 + 48, p0 + 56};
+          ptx::umma_ts_x4_warp(tO, pb, vb, IDESC_PV, 1u);
+        }
         ptx::umma_commit_warp(bar(PV_DONE + w));
         ptx::umma_commit_warp(bar(KV_EMPTY + slot));
         if (last) ptx::umma_commit_warp(bar(O_FULL + w));
@@ -472,7 +476,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               float mx = 0.f;
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                f[y] = a.bf16 ? in16x2_to_float2<true>(v[y]) : in16x2_to_float2<false>(v[y]);
+                f[y] = in16x2_to_float2<BF16>(v[y]);
                 mx = ptx::max3(mx, fabsf(f[y].x), fabsf(f[y].y));
               }
 #pragma unroll
@@ -607,31 +611,50 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           const uint64_t NM2 = ptx::f2(-mu, -mu);
           const float down = SOFTMAX ? 0.f : ptx::ex2(-mu);
           const uint64_t DN2 = ptx::f2(down, down);
-          uint32_t pk[32];
+          // P as halves. Beside outputs of 8 bits (bf16) that rounding, 2^-12, is nothing;
+          // outputs of 11 bits get what it left as halves too, in the other columns of S.
+          {
+            constexpr bool BOTH = !BF16;
+            constexpr int AT = BOTH ? 16 : 32;  // columns of P that are stored at once
 #pragma unroll
-          for (int g = 0; g < GROUPS; ++g) {
-            uint64_t sum = ptx::f2(0.f, 0.f);
+            for (int part = 0; part < 32 / AT; ++part) {
+              uint32_t pk[AT], rest[AT];
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              uint64_t x2 = ptx::f2(__uint_as_float(sr[g / 2][(g & 1) * 16 + e]),
-                                    __uint_as_float(sr[g / 2][(g & 1) * 16 + e + 1]));
-              float x, y;
-              if (SOFTMAX) {
-                ptx::f2_split(ptx::add2(x2, NM2), x, y);
-                x = ptx::ex2(x), y = ptx::ex2(y);
-                sum = ptx::add2(sum, ptx::f2(x, y));
-              } else {
-                ptx::f2_split(ptx::mul2(x2, DN2), x, y);
+              for (int g = part * AT / 8; g < (part + 1) * AT / 8; ++g) {
+                uint64_t sum = ptx::f2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                  uint64_t x2 = ptx::f2(__uint_as_float(sr[g / 2][(g & 1) * 16 + e]),
+                                        __uint_as_float(sr[g / 2][(g & 1) * 16 + e + 1]));
+                  float x, y;
+                  if (SOFTMAX) {
+                    ptx::f2_split(ptx::add2(x2, NM2), x, y);
+                    x = ptx::ex2(x), y = ptx::ex2(y);
+                    sum = ptx::add2(sum, ptx::f2(x, y));
+                  } else {
+                    ptx::f2_split(ptx::mul2(x2, DN2), x, y);
+                  }
+                  uint32_t &h = pk[(g * 8 + e / 2) % AT];
+                  h = ptx::pack_f16(x, y);
+                  if (BOTH) {
+                    const float2 f = f16x2_to_float2(h);
+                    rest[(g * 8 + e / 2) % AT] = ptx::pack_f16(x - f.x, y - f.y);
+                  }
+                }
+                if (SOFTMAX) {
+                  float x, y;
+                  ptx::f2_split(sum, x, y);
+                  l_run = fmaf(x + y, sc[g].z, l_run);
+                }
               }
-              pk[g * 8 + e / 2] = ptx::pack_f16(x, y);
-            }
-            if (SOFTMAX) {
-              float x, y;
-              ptx::f2_split(sum, x, y);
-              l_run = fmaf(x + y, sc[g].z, l_run);
+              if constexpr (BOTH) {
+                ptx::tmem_st16(tS + AT * part, pk);
+                ptx::tmem_st16(tS + 32 + AT * part, rest);
+              } else {
+                ptx::tmem_st32(tS, pk);
+              }
             }
           }
-          ptx::tmem_st32(tS, pk);
           ptx::tmem_wait_st();
           ptx::tc_fence_before();
           __syncwarp();
@@ -678,7 +701,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
                 for (int y = 0; y < 8; ++y) {
                   const float p = __uint_as_float(o[2 * y]) * f, q = __uint_as_float(o[2 * y + 1]) * f;
-                  x[y] = a.bf16 ? ptx::pack_bf16(p, q) : ptx::pack_f16(p, q);
+                  x[y] = BF16 ? ptx::pack_bf16(p, q) : ptx::pack_f16(p, q);
                 }
                 ptx::st_shared_v4(unit16(lane, c / 8), x[0], x[1], x[2], x[3]);
                 ptx::st_shared_v4(unit16(lane, c / 8 + 1), x[4], x[5], x[6], x[7]);
@@ -738,36 +761,41 @@ template <int D, int CT>
 cudaError_t launch_tiled(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                          const uint8_t *v_cache, void *cuts, int kind, int grid, int device, cudaStream_t s);
 
-template <int D, int CT, int KIND>
+template <int D, int CT, int KIND, bool BF16>
 cudaError_t launch_tiled_one(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                              const uint8_t *v_cache, void *cuts, int grid, int device, cudaStream_t s) {
   static std::atomic<uint64_t> set{0};
   constexpr int bytes = TiledConfig<D>::SMEM;
-  cudaError_t e = allow_smem(reinterpret_cast<const void *>(&paged_tiled_kernel<D, CT, KIND>), bytes,
+  cudaError_t e = allow_smem(reinterpret_cast<const void *>(&paged_tiled_kernel<D, CT, KIND, BF16>), bytes,
                              device, set);
   if (e != cudaSuccess) return e;
-  e = launch_after(paged_tiled_kernel<D, CT, KIND>, dim3(grid), kTiledThreads, bytes, s, mk, mv, a, v_cache,
+  e = launch_after(paged_tiled_kernel<D, CT, KIND, BF16>, dim3(grid), kTiledThreads, bytes, s, mk, mv, a, v_cache,
                    static_cast<CutUnit *>(cuts));
   if (e != cudaSuccess) return e;
-  return launch_after(paged_merge_kernel<D, KIND>, dim3(grid, kMergeSlices), kMergeThreads, 0, s, a,
+  return launch_after(paged_merge_kernel<D, KIND, BF16>, dim3(grid, kMergeSlices), kMergeThreads, 0, s, a,
                       static_cast<const CutUnit *>(cuts));
 }
 
-#define CHIA_TILED_CASE(D, CT, KIND) \
-  case KIND: return launch_tiled_one<D, CT, KIND>(mk, mv, a, v_cache, cuts, grid, device, s);
-#define CHIA_INSTANTIATE_TILED(D, CT)                                                         \
-  template <>                                                                                 \
-  cudaError_t chia::launch_tiled<D, CT>(const CUtensorMap &mk, const CUtensorMap &mv,         \
-                                        const PagedArgs &a, const uint8_t *v_cache,           \
-                                        void *cuts, int kind, int grid, int device,           \
-                                        cudaStream_t s) {                                     \
-    switch (kind) {                                                                           \
-      CHIA_TILED_CASE(D, CT, KIND_SOFTCAP)                                                    \
-      CHIA_TILED_CASE(D, CT, KIND_ALIBI)                                                      \
-      CHIA_TILED_CASE(D, CT, KIND_SIGMOID)                                                    \
-      CHIA_TILED_CASE(D, CT, KIND_RELU)                                                       \
-      default: return launch_tiled_one<D, CT, KIND_SOFTMAX>(mk, mv, a, v_cache, cuts, grid, device, s); \
-    }                                                                                         \
+template <int D, int CT, bool BF16>
+cudaError_t launch_tiled_kind(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
+                              const uint8_t *v_cache, void *cuts, int kind, int grid, int device, cudaStream_t s) {
+  switch (kind) {
+    case KIND_SOFTCAP: return launch_tiled_one<D, CT, KIND_SOFTCAP, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
+    case KIND_ALIBI: return launch_tiled_one<D, CT, KIND_ALIBI, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
+    case KIND_SIGMOID: return launch_tiled_one<D, CT, KIND_SIGMOID, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
+    case KIND_RELU: return launch_tiled_one<D, CT, KIND_RELU, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
+    default: return launch_tiled_one<D, CT, KIND_SOFTMAX, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
+  }
+}
+
+#define CHIA_INSTANTIATE_TILED(D, CT)                                                          \
+  template <>                                                                                  \
+  cudaError_t chia::launch_tiled<D, CT>(const CUtensorMap &mk, const CUtensorMap &mv,          \
+                                        const PagedArgs &a, const uint8_t *v_cache,            \
+                                        void *cuts, int kind, int grid, int device,            \
+                                        cudaStream_t s) {                                      \
+    return a.bf16 ? launch_tiled_kind<D, CT, true>(mk, mv, a, v_cache, cuts, kind, grid, device, s)   \
+                  : launch_tiled_kind<D, CT, false>(mk, mv, a, v_cache, cuts, kind, grid, device, s); \
   }
 
 }  // namespace chia

@@ -341,6 +341,19 @@ def test_masks(cuda, name, counts):
                     head_param=cp.alibi_slopes_geometric(8))
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("counts", [[1, 3], [100, 37]])
+def test_fp16_outputs_are_rounded_once(cuda, kind, counts):
+    """P's rounding is made up for where outputs have 11 bits: 2^-12 |o| and 2^-14 of a term are left; twice their sum."""
+    lens, H, D, page = [700, 333], 8, 128, 32
+    kw = kind_args(kind, H)
+    q, k, v, ks, vs, table, cu = setup(lens, counts, H, 2, D, page, E4M3, F16, 6)
+    got = cp.paged_attention(q, k, v, ks, vs, ints(table), ints(lens), ints(cu), **kw)
+    out, _, mass = po.attention(q.cpu(), k.cpu(), v.cpu(), ks.cpu(), vs.cpu(), table, lens, cu, mask=cp.CAUSAL, **kw)
+    err = (got.double().cpu() - out).abs()
+    assert (err <= 2.0 ** -11 * out.abs() + 2.0 ** -13 * mass + 2.0 ** -23).all(), float((err / out.abs()).max())
+
+
 def test_rows_without_keys(cuda):
     """More queries than keys, no keys, no queries, a window before the first key."""
     got = check_attention([3, 0, 5, 0], [6, 2, 0, 1], 4, 2, 128, 16, E4M3, BF16)
