@@ -333,9 +333,11 @@ struct Line {
   // Cost x, as a cost and as a tile. `snap`: moved to the nearer end of the
   // unit that it cuts where the unit is short: a cut costs a round of the
   // workspace (some 4 us), whole units wait for nobody.
-  __device__ __forceinline__ int place(int x, bool snap, int &tile) const {
+  // `entry`: the one that the tile is in.
+  __device__ __forceinline__ int place(int x, bool snap, int &tile, int &entry) const {
     if (x >= total) {
       tile = s.tiles_pre[entries];
+      entry = entries;
       return total;
     }
     int lo = 0, hi = entries;
@@ -356,6 +358,8 @@ struct Line {
     }
     // (a border within the cost of a unit's own counts as its first tile)
     tile = s.tiles_pre[lo] + u * n + max(0, in - COST);
+    entry = u < units ? lo : entries;
+    if (u == units && tile < s.tiles_pre[entries]) entry = entry_at(tile);
     return cost_before(lo) + u * cost + in;
   }
   // The CTA that has tile k of a unit that is cut: the last with a border not above it.

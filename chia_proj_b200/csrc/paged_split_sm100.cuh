@@ -100,7 +100,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     bool before, after, last_is_head;
   };
   __shared__ Group s_group[kSplitWarps + 1];
-  __shared__ int s_groups, s_last[2];
+  __shared__ int s_groups, s_last[2], s_first_cta[2], s_last_cta[2];
   __shared__ uint32_t s_ends;
 
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -121,13 +121,14 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   const L line(line_sm, a, kSplitWarps);  // (its barriers also order the set-up above)
   if (static_cast<int>(blockIdx.x) >= line.ctas) return;
   const int me = blockIdx.x * kSplitWarps + warp;
-  int c0, nk;  // first tile and number of tiles of this worker
+  int c0, nk, e0;  // first tile and number of tiles of this worker, the first one's entry
   {
     int tile;  // lane 0: this border, lane 1: the next one
-    const int y = line.place(line.even(blockIdx.x + (lane & 1)), true, tile);
+    const int y = line.place(line.even(blockIdx.x + (lane & 1)), true, tile, e0);
     const int y0 = __shfl_sync(0xffffffffu, y, 0), y1 = __shfl_sync(0xffffffffu, y, 1);
     line.place(y0 + static_cast<int>(static_cast<long long>(y1 - y0) * (warp + (lane & 1)) / kSplitWarps),
-          false, tile);
+          false, tile, e0);
+    e0 = __shfl_sync(0xffffffffu, e0, 0);
     c0 = __shfl_sync(0xffffffffu, tile, 0);
     nk = __shfl_sync(0xffffffffu, tile, 1) - c0;
   }
@@ -146,11 +147,11 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   int next_pg0 = -1, next_pg1 = -1, next_hk = 0, next_tok = 0;  // pages
   int wanted = 0;                                                // bits: that there are such keys
   float next_ks0 = 0.f, next_vs0 = 0.f, next_ks1 = 0.f, next_vs1 = 0.f;
-  auto ask_pages = [&](int k) {
+  auto ask_pages = [&](int k, bool one_entry) {  // one_entry: the 32 tiles are all of entry e0
     next_pg0 = next_pg1 = -1, wanted = 0;
     if (k + lane < nk) {
       const int g = c0 + k + lane;
-      const int b = line.entry_at(g);
+      const int b = one_entry ? e0 : line.entry_at(g);
       const Request r = line_sm.req[b];
       int ut;
       next_hk = line.unit_at(g, b, r, ut).hk;
@@ -204,7 +205,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         tma_load_3d(dst + TK * D + 16 * D, &mv, bar, 0, 0, r1);
       }
     }
-    if (in == 12 && k + 20 < nk) ask_pages(k + 20);
+    if (in == 12 && k + 20 < nk) ask_pages(k + 20, false);
     if (in == 22 && k + 10 < nk) ask_scales();
   };
 
@@ -214,8 +215,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   int len = 0, p0 = 0, ut0 = 0, nt = 0;
   uint4 raw[NT][H * 2];  // row 8 n + gid, channels 16 H tig .. + 16 H - 1
   float hp[NT][2];       // of rows 8 n + 2 tig + e, as in the columns of S^T
-  auto begin_unit = [&](int k) {
-    const int g = c0 + k, b = line.entry_at(g);
+  auto begin_unit = [&](int k, int b) {  // b: the entry
+    const int g = c0 + k;
     const Request rq = line_sm.req[b];
     len = rq.len;
     p0 = len - rq.n;
@@ -246,11 +247,11 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     }
   };
   if (nk > 0) {
-    ask_pages(0);
-    begin_unit(0);
+    ask_pages(0, line_sm.tiles_pre[e0 + 1] >= c0 + min(nk, 32));
+    begin_unit(0, e0);
     take_rows();
-    for (int k = 0; k < NST; ++k) issue(k);
     ask_scales();
+    for (int k = 0; k < NST; ++k) issue(k);
     take_scales(0);
   }
 
@@ -657,7 +658,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           if (gid == 0) *reinterpret_cast<float2 *>(pm + 2 * r) = make_float2(m_run[n][e], l_run[n][e]);
         }
     }
-    if (k < nk) begin_unit(k);
+    if (k < nk) begin_unit(k, line.entry_at(c0 + k));
   }
   if (!has_end) rings_spent();
   __syncthreads();
@@ -749,7 +750,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   __syncthreads();
   if (t < 2 && (t == 0 ? s_group[0].before : s_group[groups - 1].after && !s_group[groups - 1].before)) {
     const Unit &un = unit_of(s_group[t == 0 ? 0 : groups - 1]);
-    const unsigned first = line.cta_of(un, 0), parts_less_1 = line.cta_of(un, un.n - 1) - first;
+    const int first = line.cta_of(un, 0), last = line.cta_of(un, un.n - 1);
+    const unsigned parts_less_1 = last - first;
+    s_first_cta[t] = first, s_last_cta[t] = last;
     __threadfence();  // (the CTA's parts, seen through the barrier, before the ticket)
     // counts the unit's CTAs and wraps to zero
     s_last[t] = atomicInc(reinterpret_cast<unsigned *>(a.tickets) + first, parts_less_1) == parts_less_1;
@@ -759,7 +762,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   for (int x = 0; x < 2; ++x) {
     if (!s_last[x]) continue;
     const Unit &un = unit_of(s_group[x == 0 ? 0 : groups - 1]);
-    const int first = line.cta_of(un, 0), last = line.cta_of(un, un.n - 1);
+    const int first = s_first_cta[x], last = s_last_cta[x];
     for (int e = t; e < un.rows * (D / 4); e += kSplitThreads) {
       const int r = e / (D / 4), c4 = e % (D / 4);
       float M = -INFINITY, L = 0.f;

@@ -160,8 +160,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   }
   int c0, nk;  // this CTA's tiles
   {
-    int tile;
-    line.place(line.even(blockIdx.x + (lane & 1)), true, tile);
+    int tile, entry;
+    line.place(line.even(blockIdx.x + (lane & 1)), true, tile, entry);
     c0 = __shfl_sync(0xffffffffu, tile, 0);
     nk = __shfl_sync(0xffffffffu, tile, 1) - c0;
   }
