@@ -131,13 +131,13 @@ __device__ __forceinline__ Tiles tiles_of(const PagedArgs &a, int p0, int p1, in
 // A wait of limited length. After one has run out (`abort`), all return at once.
 // The answer is a lane's own: where lanes go on together the caller takes the
 // warp's (warp_all), since lanes that gave up alone would leave the others waiting
-// for them.
+// for them. Under a limit below a microsecond, what the clock and a suspended lane
+// cannot tell apart, a wait that is not met at once runs out.
 __device__ __forceinline__ bool paged_wait(uint32_t bar, uint32_t parity, volatile int *abort,
                                            const PagedArgs &a) {
   if (ptx::mbar_test_wait(bar, parity)) return true;
   const uint64_t t0 = ptx::globaltimer_ns();
-  const uint32_t nap = a.timeout_ns < 20000 ? static_cast<uint32_t>(a.timeout_ns) : 20000u;
-  while (!ptx::mbar_try_wait(bar, parity, nap)) {
+  while (a.timeout_ns < 1000 || !ptx::mbar_try_wait(bar, parity, 20000u)) {
     if (*abort) return false;
     if (ptx::globaltimer_ns() - t0 > a.timeout_ns) {
       *abort = 1;
@@ -349,7 +349,7 @@ struct Line {
         hi = mid;
     }
     const int units = s.units_pre[lo + 1] - s.units_pre[lo];
-    const int n = (s.tiles_pre[lo + 1] - s.tiles_pre[lo]) / units, cost = n + COST;
+    const int n = s.req[lo].tl.n, cost = n + COST;
     int in = x - cost_before(lo), u = in / cost;
     in -= u * cost;
     if (snap && cost <= WHOLE) {

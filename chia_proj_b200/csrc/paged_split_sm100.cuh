@@ -124,10 +124,13 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   int c0, nk, e0;  // first tile and number of tiles of this worker, the first one's entry
   {
     int tile;  // lane 0: this border, lane 1: the next one
-    const int y = line.place(line.even(blockIdx.x + (lane & 1)), true, tile, e0);
-    const int y0 = __shfl_sync(0xffffffffu, y, 0), y1 = __shfl_sync(0xffffffffu, y, 1);
-    line.place(y0 + static_cast<int>(static_cast<long long>(y1 - y0) * (warp + (lane & 1)) / kSplitWarps),
-          false, tile, e0);
+    int x = line.even(blockIdx.x + (lane & 1));
+#pragma unroll 1  // (one copy of the code: fetching it is most of the time)
+    for (int own = 0; own < 2; ++own) {  // the CTA's borders, then the worker's within them
+      const int y = line.place(x, own == 0, tile, e0);
+      const int y0 = __shfl_sync(0xffffffffu, y, 0), y1 = __shfl_sync(0xffffffffu, y, 1);
+      x = y0 + static_cast<int>(static_cast<long long>(y1 - y0) * (warp + (lane & 1)) / kSplitWarps);
+    }
     e0 = __shfl_sync(0xffffffffu, e0, 0);
     c0 = __shfl_sync(0xffffffffu, tile, 0);
     nk = __shfl_sync(0xffffffffu, tile, 1) - c0;

@@ -178,7 +178,11 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   // both of two: asked for together, since an answer takes some 100 cycles
   auto wait2 = [&](int i, uint32_t pi, int j, uint32_t pj) {
     const bool x = ptx::mbar_test_wait(bar(i), pi), y = ptx::mbar_test_wait(bar(j), pj);
-    return (x && y) || (wait(i, pi) && wait(j, pj));
+    if (x && y) return true;
+#pragma unroll 1  // (one copy of the code)
+    for (int second = 0; second < 2; ++second)
+      if (!wait(second ? j : i, second ? pj : pi)) return false;
+    return true;
   };
 
   // the unit of this CTA's tile k
