@@ -113,7 +113,8 @@ int check_append(const chia_append_params_t *p) {
 }
 
 // Tokens that a CTA of the append looks at: a page's, or as many fewer as give
-// every SM eight CTAs.
+// every SM eight CTAs. 16 prompts of some 4,100 tokens: 42 us by pages, 590 by single
+// tokens (every CTA then reads its neighbours' slots); 64 single tokens: 62 and 3.7.
 template <int D, bool BF16, int CT>
 int launch_append(const chia::AppendArgs &a, int sms, cudaStream_t s) {
   const int64_t kinds = 2ll * a.heads_kv;
@@ -188,11 +189,15 @@ int kind_of(const chia_paged_params_t *p) {
 // Which kernel, and the workspace: the tickets, then the parts of two units a
 // CTA and (split kernel) of one a worker.
 constexpr int64_t kTicketBytes = 4096;
-// Rows of a K/V head from which the tiled kernel is the faster one.
-constexpr int64_t kTiledRows = 65;
+// Rows of a K/V head (queries x heads of a group) from which the tiled kernel is the
+// faster one. Split and tiled, us, D 128, 8 K/V heads: 8 requests x 4096 keys, 48 rows 53, 57,
+// 64 rows 65, 58, 256 rows 206, 69; 32 x 1024, 48 rows 63, 63, 64 rows 71, 63.
+constexpr int64_t kTiledRows = 56;
 struct SplitPlan {
   bool tiled;
-  int tiles;  // split kernel: rows of a unit, 8 (as many as most groups of heads have) or 16
+  // split kernel: eights of rows of a unit. Two from 9 rows on: 64 requests x 8192 keys, 16
+  // rows 208 us, and 363 in units of 8, which read the keys twice (24 x 1500, 20 rows: 35 and 27).
+  int tiles;
   int rows;   // of a unit
   int grid;   // one CTA an SM
   int64_t off_ml, off_cuts, bytes;

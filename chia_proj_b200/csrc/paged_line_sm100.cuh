@@ -230,7 +230,8 @@ __device__ __forceinline__ void merge_parts(const PagedArgs &a, int first, int l
 // entries in their order. An entry is a request, or with BLOCKS a block of ROWS
 // rows of one (several, where there are more blocks than entries fit): blocks
 // of a long run of queries see different keys. An entry's units visit the same
-// tiles. WHOLE: units of up to this cost are not cut between CTAs.
+// tiles. WHOLE: units of up to this cost (with BLOCKS: and of no more than a CTA's
+// share) are not cut between CTAs.
 template <int TK, int ROWS, int THREADS, int COST, int WHOLE, bool BLOCKS>
 struct Line {
   struct Shared {
@@ -352,7 +353,7 @@ struct Line {
     const int n = s.req[lo].tl.n, cost = n + COST;
     int in = x - cost_before(lo), u = in / cost;
     in -= u * cost;
-    if (snap && cost <= WHOLE) {
+    if (snap && cost <= WHOLE && (!BLOCKS || cost <= step)) {
       u += 2 * in >= cost ? 1 : 0;
       in = 0;
     }

@@ -25,6 +25,14 @@
 // keys one S buffer a query tile is all that fits beside O, and each softmax
 // waited some 2000 of 5200 cycles for PV and the next S.)
 //
+// Measured (D 128, e4m3, bf16, 32 query and 8 K/V heads): 4 requests x 1024
+// queries over 8192 keys 600 us, 0.86 PFLOP/s, 52% of the rate of a plain matrix
+// product; up to that many each, ragged, 262 us, 39%. Bound by the softmax warps: of a tile's 2,550 cycles the UMMAs take 1,024; 500 go to scores and
+// maximum, 1,150 to exponentials, sums and packing (64 a thread, two warps a
+// scheduler: issue and latency), 700 to barriers and tensor memory. fp16: 696 us.
+// Tried: two threads a row on 16 warps 282 us ragged where this had 273; the two
+// query tiles' exponentials in turns 290.
+//
 // Numbers as in the split kernel: Q times a power of two per row and the
 // cache's values are halves exactly; a key scale multiplies the scores of its
 // 16 columns, the logarithm of a value scale is part of the running maximum.
@@ -35,9 +43,18 @@ namespace chia {
 
 constexpr int kTiledThreads = 512;
 constexpr float kTiledPTop = 7.f;  // P is 2^7 at the running maximum, and at most 2^15 (a half's range)
-constexpr int kTiledCost = 2;    // what a unit costs beside its tiles of 64 keys
-constexpr int kTiledWhole = 12;  // units of up to this cost are not cut between CTAs
-constexpr int kTiledPiece = 12;  // the least cost of a piece: a part is 128 KB to write and to read
+// The pieces (32 query heads, 8 K/V heads, D 128 unless said; us, requests x queries / keys).
+// What a unit costs beside its tiles of 64 keys: 6 against 2: 1 x 4000 / 4000 230, 370;
+// 3 x 128 / 20000 93, 97; 4 x 1024 / 8192 601, 603.
+constexpr int kTiledCost = 6;
+// Units of up to this cost, and of no more than a CTA's share, are not cut: a cut is a part of
+// 128 KB to write and to read and another start. 48 against 12: 16 x 100 / 900 67, 85. Without
+// the share 1 x 2000 / 2000 (8 query heads to one K/V head) takes 58, with it 38; never whole,
+// 64 x 32 / 400 takes 103 in place of 82.
+constexpr int kTiledWhole = 48;
+// The least cost of a piece: 1, 4, 12 and 40 on 1 x 64 / 700: 24, 25, 41, 83; on
+// 30 x 256 / 2000 119.2, 118.7 (1 and 4).
+constexpr int kTiledPiece = 4;
 
 template <int D>
 struct TiledConfig {
