@@ -146,11 +146,11 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   const uint32_t sb = ptx::smem_u32(sm);
   float4 *scales = reinterpret_cast<float4 *>(sm + C::OFF_SC);  // [SETS][GROUPS]: ks, value factor, its inverse
   __shared__ typename L::Shared line_sm;
-  // st_full st_empty | kv_full kv_empty | q (2) | s p (2 buffers x 2) | pv o o_empty (2 each) | scales | drain
+  // st_full st_empty | kv_full kv_empty | q (2) | s p (2 buffers x 2) | pv o o_empty (2 each) | scales full empty | drain
   enum { ST_FULL = 0, ST_EMPTY = ST_FULL + STAGES, KV_FULL = ST_EMPTY + STAGES, KV_EMPTY = KV_FULL + SLOTS,
          Q_FULL = KV_EMPTY + SLOTS, S_FULL = Q_FULL + 2, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4,
-         O_FULL = PV_DONE + 2, O_EMPTY = O_FULL + 2, SC_FULL = O_EMPTY + 2, DRAIN = SC_FULL + SETS,
-         BARS = DRAIN + 2 };
+         O_FULL = PV_DONE + 2, O_EMPTY = O_FULL + 2, SC_FULL = O_EMPTY + 2, SC_EMPTY = SC_FULL + SETS,
+         DRAIN = SC_EMPTY + SETS, BARS = DRAIN + 2 };
   __shared__ __align__(8) uint64_t bars[BARS];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, nan_flag;
@@ -162,7 +162,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     for (int i = 0; i < BARS; ++i) {
       const bool four = (i >= ST_EMPTY && i < KV_EMPTY) || (i >= Q_FULL && i < S_FULL) ||
                         (i >= P_FULL && i < PV_DONE) || (i >= O_EMPTY && i < SC_FULL);
-      ptx::mbar_init(bar(i), i >= KV_EMPTY && i < Q_FULL ? 2 : four ? 4 : 1);
+      ptx::mbar_init(bar(i), i >= KV_EMPTY && i < Q_FULL ? 2 : four ? 4 : i >= SC_EMPTY && i < DRAIN ? 8 : 1);
     }
     abort_flag = nan_flag = 0;
     ptx::tma_prefetch_desc(&mk);
@@ -275,6 +275,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       scales_of(k1);
       Keys k2 = page_of(1);
       for (int k = 0; k < nk; ++k) {
+        // A softmax warp may be far behind: a query tile without rows takes part in no other wait
+        // for these tiles, and its warps may still be writing the unit before.
+        if (!warp_all(wait(SC_EMPTY + k % SETS, ((k / SETS) & 1) ^ 1))) break;
         const Keys now = k1;
         row = row1, ks = ks1, vs = vs1;
         if (row < 0 && (now.all & 4)) report(a.status, kStatusBadIndex);
@@ -679,7 +682,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           ptx::tmem_wait_st();
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(P_FULL + 2 * w + (cnt & 1)));
+          if (lane == 0) {
+            ptx::mbar_arrive(bar(P_FULL + 2 * w + (cnt & 1)));
+            ptx::mbar_arrive(bar(SC_EMPTY + n % SETS));
+          }
         }
         if (!ok) break;
         // ---- O
@@ -760,7 +766,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(O_EMPTY + w));
       } else {  // no rows for this query tile: it keeps step, so that no phase of the scales is passed by
-        for (int n = k; n < k + h.nt && ok; ++n) ok = warp_all(wait(SC_FULL + n % SETS, (n / SETS) & 1));
+        for (int n = k; n < k + h.nt && ok; ++n) {
+          ok = warp_all(wait(SC_FULL + n % SETS, (n / SETS) & 1));
+          if (ok && lane == 0) ptx::mbar_arrive(bar(SC_EMPTY + n % SETS));
+        }
         if (!ok) break;
       }
       k += h.nt;
