@@ -276,14 +276,17 @@ __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(con
     s_slot[e] = x >= 0 && x < a.tokens ? a.slots[x] : -1;
   }
   __syncthreads();
-  int par = 0;
-  for (int t0 = w0; t0 < w1; par ^= 1) {
+  // Two sets of s_same, s_first and s_max by turns, one a run: a run has a barrier at
+  // least, so a set is written again only behind the barrier of the run between.
+  int par = 1;
+  for (int t0 = w0; t0 < w1;) {
     const int at = t0 - w0 + 1, slot0 = s_slot[at];
     if (slot0 < 0) {  // skipped
       ++t0;
       continue;
     }
     // the run: the following tokens in the same page
+    par ^= 1;
     const int page = slot0 >> SHIFT;
     const int mine = tid < PAGE && at + tid < window + PAGE ? s_slot[at + tid] : -1;
     const bool in = mine >= 0 && (mine >> SHIFT) == page;

@@ -1,0 +1,45 @@
+"""The write into the paged 8-bit K/V cache and its tables where calls are ragged: many runs of tokens in the rows that
+one CTA looks at, skipped tokens, pages out of range. Contents are compared exactly with ``paged_oracle.py``."""
+
+import pytest
+import torch
+
+import chia_proj_b200 as cp
+import paged_oracle as po
+from test_paged_gpu import BF16, E4M3, F16, I8, check_append, ints, make_cache  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda):
+    yield
+    cp.check_device_status(0)
+
+
+@pytest.mark.parametrize("page,hkv,D,ct,dtype,T", [(16, 8, 64, E4M3, BF16, 2500), (64, 16, 64, I8, F16, 4000),
+                                                   (128, 16, 64, E4M3, F16, 9000), (32, 8, 128, I8, BF16, 3200)])
+@pytest.mark.parametrize("seed", range(4))
+def test_runs_between_skipped_tokens(cuda, page, hkv, D, ct, dtype, T, seed):
+    """So many tokens that a CTA looks at a whole page's worth of them: runs that begin in the rows of one CTA and end
+    in the next one's, skipped tokens of every number behind them, pages that are not in the cache, short runs."""
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda n: int(torch.randint(0, n, (1,), generator=g))  # noqa: E731
+    slots, pages, bad = [], 0, False
+    while len(slots) < T:
+        off = rnd(page) if rnd(3) else 0
+        n = 1 + rnd(page - off) if rnd(3) else page - off
+        if rnd(8) == 0:
+            p, bad = 100000 + pages, True
+        else:
+            p, pages = pages, pages + 1
+        slots += [p * page + off + i for i in range(n)]
+        slots += [-1] * (rnd(6) if rnd(2) else 0)
+    kinds = 2 * hkv
+    assert len(slots) // page * kinds >= 8 * 148  # the rule by which a CTA looks at a page's worth
+    cache = make_cache(pages, hkv, page, D, ct, g)
+    x = torch.randn(len(slots), kinds, D, generator=g).to(dtype).cuda()
+    check_append(x[:, :hkv], x[:, hkv:], slots, cache)
+    if bad:
+        with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+            cp.check_device_status(0)
