@@ -198,25 +198,27 @@ __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const Tab
         len = 0;
       }
     }
-    int pages = done ? (len + a.page - 1) / a.page : 0;
-    if (pages > a.width) {
+    long long pages = done ? (static_cast<long long>(len) + a.page - 1) / a.page : 0;
+    if (pages > a.width) {  // which pages it holds is not known: it is not released
       bad |= kStatusBadIndex;
-      pages = a.width;
+      pages = done = 0;
     }
     Scan2 tot;
     const Scan2 sc = block_scan2(Scan2{pages, 0}, tot, sums);
-    s_at[t] = static_cast<int32_t>(sc.a - pages);
-    if (t == 0) s_at[kTablesThreads] = static_cast<int32_t>(tot.a);
+    // (of lengths that make no sense: pages past the 2^31st are in no ring)
+    constexpr long long kMost = 0x7fffffff;
+    s_at[t] = static_cast<int32_t>(min(sc.a - pages, kMost));
+    if (t == 0) s_at[kTablesThreads] = static_cast<int32_t>(min(tot.a, kMost));
     __syncthreads();
     if (first_cta && b < a.batch) a.new_seq_lens[b] = done ? 0 : len;
     const int n = min(kTablesThreads, a.batch - b0);
     const int end = s_at[kTablesThreads];
-    for (int x = blockIdx.x * kTablesThreads + t; x < end; x += gridDim.x * kTablesThreads) {
-      const int r = last_not_above(s_at, n, x);
+    for (long long y = blockIdx.x * kTablesThreads + t; y < end; y += gridDim.x * kTablesThreads) {
+      const int x = static_cast<int>(y), r = last_not_above(s_at, n, x);
       const int page = a.block_table[(b0 + r) * a.table_stride + (x - s_at[r])];
       const long long at = pages0 + x;  // among all released pages
       if (count + at < a.ring)
-        a.free_pages[(head + count + at) % a.ring] = page;
+        a.free_pages[(static_cast<long long>(head) + count + at) % a.ring] = page;
       else
         bad |= kStatusBadIndex;  // more pages than the ring holds: given back twice
     }

@@ -83,8 +83,9 @@ typedef struct chia_tables_params {
 CHIA_API int chia_page_tables(const chia_tables_params_t *params, void *stream);
 
 /* The pages of finished requests (new_lens[b] != 0) go to the ring's tail, in
- * order; their lengths become 0 in new_seq_lens. The outputs slots, positions
- * and cu_q are not used. */
+ * order; their lengths become 0 in new_seq_lens. A request whose length is more
+ * than its row holds is reported and keeps length and pages. The outputs slots,
+ * positions and cu_q are not used. */
 CHIA_API int chia_release_pages(const chia_tables_params_t *params, void *stream);
 
 /* ------------------------------------------------------------------ append */

@@ -43,3 +43,23 @@ def test_runs_between_skipped_tokens(cuda, page, hkv, D, ct, dtype, T, seed):
     if bad:
         with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
             cp.check_device_status(0)
+
+
+@pytest.mark.parametrize("B", [3, 1024, 2300])
+def test_release_of_bad_lengths(cuda, B):
+    """Lengths that no row holds, near 2^31 and below zero, give nothing back; the others' pages come back in order."""
+    page, width = 16, 5
+    bad = {0: 2 ** 31 - 1, 1: -1, B // 2: 2 ** 31 - 9, B - 1: width * page + 1, 2 * B // 3: -2 ** 31}
+    lens = [bad.get(b, (7 * b) % (width * page + 1)) for b in range(B)]
+    table = [[width * b + p for p in range(width)] for b in range(B)]
+    back = [p for b in range(B) if b not in bad for p in table[b][:po.pages_for(lens[b], page)]]
+    ring = ints([-5] * (B * width))
+    lens2, state = cp.release_pages(ints([1] * B), ints(lens), ints(table), ring, ints([4, 2]), page_size=page)
+    assert state.tolist() == [4, 2 + len(back)]
+    got = ring.tolist()
+    at = [(6 + i) % (B * width) for i in range(len(back))]
+    assert [got[i] for i in at] == back
+    assert all(got[i] == -5 for i in set(range(B * width)) - set(at))
+    assert lens2.tolist() == [max(bad[b], 0) if b in bad else 0 for b in range(B)]
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
