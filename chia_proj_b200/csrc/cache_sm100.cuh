@@ -180,10 +180,12 @@ __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const Tab
   const bool first_cta = blockIdx.x == 0;
   follow();
   int head = a.free_state[0], count = a.free_state[1];
-  if (head < 0 || head >= a.ring || count < 0 || count > a.ring) {
+  // In a ring that makes no sense there is no place for a page: nobody is released,
+  // and the ring that goes on is empty, as page_tables leaves it then.
+  const bool ring_ok = head >= 0 && head < a.ring && count >= 0 && count <= a.ring;
+  if (!ring_ok) {
     if (t == 0 && first_cta) report(a.status, kStatusBadIndex);
-    head = 0;
-    count = a.ring;  // nothing more is taken
+    head = count = 0;
   }
   long long pages0 = 0;
   int bad = 0;
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const Tab
     int len = 0, done = 0;
     if (b < a.batch) {
       len = a.seq_lens[b];
-      done = a.new_lens[b] != 0;
+      done = a.new_lens[b] != 0 && ring_ok;
       if (len < 0) {
         bad |= kStatusBadIndex;
         len = 0;

@@ -77,14 +77,16 @@ typedef struct chia_tables_params {
  * order. A request that would not fit its row of the table, or that needs pages
  * when the ring has not enough left for it and those before it, is not served:
  * its slots are -1, its length stays, and CHIA_ERR_NO_PAGES is reported (cu_q
- * counts its tokens all the same). Entries of slots and positions past the
+ * counts its tokens all the same). A free_state out of range is reported and
+ * taken as an empty ring. Entries of slots and positions past the
  * step's tokens are -1 and 0. seq_lens and free_state are not changed (the new
  * ones are outputs), so a step may be run again. */
 CHIA_API int chia_page_tables(const chia_tables_params_t *params, void *stream);
 
 /* The pages of finished requests (new_lens[b] != 0) go to the ring's tail, in
  * order; their lengths become 0 in new_seq_lens. A request whose length is more
- * than its row holds is reported and keeps length and pages. The outputs slots,
+ * than its row holds is reported and keeps length and pages; where free_state is
+ * out of range all do, and new_free_state is an empty ring. The outputs slots,
  * positions and cu_q are not used. */
 CHIA_API int chia_release_pages(const chia_tables_params_t *params, void *stream);
 

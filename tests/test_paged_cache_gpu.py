@@ -63,3 +63,18 @@ def test_release_of_bad_lengths(cuda, B):
     assert lens2.tolist() == [max(bad[b], 0) if b in bad else 0 for b in range(B)]
     with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
         cp.check_device_status(0)
+
+
+@pytest.mark.parametrize("state", [[-1, 2], [5, 0], [2 ** 31 - 1, 1], [0, 6], [0, -1], [3, 2 ** 31 - 1]])
+def test_release_into_a_bad_ring(cuda, state):
+    """Nobody is released, and the ring that is returned hands out nothing."""
+    ring = ints([9, 8, 7, 6, 5])
+    table = ints([[1, 2], [3, 4]])
+    lens, got = cp.release_pages(ints([1, 0]), ints([20, 30]), table, ring, ints(state), page_size=16)
+    assert lens.tolist() == [20, 30] and got.tolist() == [0, 0] and ring.tolist() == [9, 8, 7, 6, 5]
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+    step = cp.page_tables(lens, ints([1, 3]), table, ring, got, page_size=16, max_tokens=4)
+    assert step.slots.tolist() == [36, -1, -1, -1] and step.seq_lens.tolist() == [21, 30]
+    with pytest.raises(cp.ChiaError, match="NO_PAGES"):
+        cp.check_device_status(0)
