@@ -57,17 +57,29 @@ struct Request {
   int row0, row1;  // an entry of the line: these rows (queries x heads of a group) of the request
   Tiles tl;        // the tiles that they visit
 };
-__device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &bad) {
+__device__ __forceinline__ bool offsets_ok(const PagedArgs &a, int t0, int t1) {
+  return t0 >= 0 && t1 >= t0 && t1 <= a.tokens;
+}
+// The requests before the first whose offsets are out of range or fall. Those behind it
+// are not served: they could own rows that others own, and the line, whose length the
+// host bounds by the number of rows, could pass 32 bits.
+static __device__ __noinline__ int requests_in_order(const PagedArgs &a) {
+  int b = 0;
+  while (b < a.batch && offsets_ok(a, a.cu_q[b], a.cu_q[b + 1])) ++b;
+  return b;
+}
+// bad: what the status word is told; gap: the offsets are bad
+__device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &bad, bool &gap) {
   Request r;
   r.b = b;
   if (a.cu_q != nullptr) {
     r.t0 = a.cu_q[b];
     const int t1 = a.cu_q[b + 1];
-    if (r.t0 < 0 || t1 < r.t0 || t1 > a.tokens) {
-      bad = true;
-      r.t0 = r.n = 0;
-    } else {
+    if (offsets_ok(a, r.t0, t1)) {
       r.n = t1 - r.t0;
+    } else {
+      bad = gap = true;
+      r.t0 = r.n = 0;
     }
   } else {
     r.t0 = a.token0 + b * a.q_each;
@@ -244,8 +256,9 @@ struct Line {
   const PagedArgs &a;
   int entries, total, ctas, step, rest;
 
-  // Sums over the block of x and y before this thread's; the totals in tx, ty.
-  __device__ __forceinline__ void scan(int &x, int &y, int &tx, int &ty) {
+  // Sums over the block of x and y before this thread's; the totals in tx, ty. Whether any
+  // thread's `flag` is set.
+  __device__ __forceinline__ bool scan(int &x, int &y, int &tx, int &ty, bool flag = false) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int x0 = x, y0 = y;
 #pragma unroll
@@ -254,7 +267,7 @@ struct Line {
       if (lane >= d) x += u, y += v;
     }
     if (lane == 31) s.wsum[warp][0] = x, s.wsum[warp][1] = y;
-    __syncthreads();
+    const bool any = __syncthreads_or(flag);
     x -= x0, y -= y0;
     tx = ty = 0;
 #pragma unroll 4
@@ -263,21 +276,26 @@ struct Line {
       tx += s.wsum[w][0], ty += s.wsum[w][1];
     }
     __syncthreads();
+    return any;
   }
 
   // All threads of the CTA; per_cta: the least cost of a CTA's piece.
   __device__ __forceinline__ Line(Shared &sh, const PagedArgs &args, int per_cta) : s(sh), a(args) {
     const int t = threadIdx.x;
-    bool bad = false;
+    bool bad = false, gap = false;
     entries = a.batch;
     if (BLOCKS) {
       // (a launch has fewer requests than entries) the blocks of each request,
       // `each` to an entry so that all fit
       static_assert(!BLOCKS || kLineBatch <= THREADS, "an entry a thread");
       int blocks = 0, none = 0, x, each = 1;
-      if (t < a.batch) blocks = (request_of(a, t, bad).row1 + ROWS - 1) / ROWS;
+      if (t < a.batch) blocks = (request_of(a, t, bad, gap).row1 + ROWS - 1) / ROWS;
       int at = blocks;
-      scan(at, none, entries, x);
+      if (scan(at, none, entries, x, gap)) {
+        if (t >= requests_in_order(a)) blocks = 0;
+        at = blocks;
+        scan(at, none, entries, x);
+      }
       if (entries > kLineBatch) {
         each = (entries + kLineBatch - a.batch - 1) / max(1, kLineBatch - a.batch);
         at = (blocks + each - 1) / each;
@@ -288,7 +306,7 @@ struct Line {
       __syncthreads();
       if (t < entries) {
         const int b = last_not_above(s.starts, a.batch, t);
-        Request r = request_of(a, b, bad);
+        Request r = request_of(a, b, bad, gap);
         r.row0 = (t - s.starts[b]) * each * ROWS;
         r.row1 = min(r.row1, r.row0 + each * ROWS);
         r.tl = tiles_of<TK>(a, r.len - r.n + div_group(a, r.row0), r.len - r.n + div_group(a, r.row1 - 1), r.len);
@@ -296,13 +314,20 @@ struct Line {
       }
     } else {
       for (int b = t; b < entries; b += THREADS) {
-        Request r = request_of(a, b, bad);
+        Request r = request_of(a, b, bad, gap);
         if (r.n > 0) r.tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
         s.req[b] = r;
       }
     }
     if (bad && blockIdx.x == 0) report(a.status, kStatusBadIndex);
-    __syncthreads();
+    if (BLOCKS) {
+      __syncthreads();
+    } else if (__syncthreads_or(gap)) {
+      const int ordered = requests_in_order(a);
+      for (int b = t; b < entries; b += THREADS)
+        if (b >= ordered) s.req[b].row1 = 0;
+      __syncthreads();
+    }
     const int per = (entries + THREADS - 1) / THREADS;
     const int b0 = t * per, b1 = min(entries, b0 + per);
     auto units_of = [&](const Request &r) {

@@ -150,7 +150,9 @@ typedef struct chia_paged_params {
   const int32_t *block_table;
   const int32_t *seq_lens; /* [batch] keys of each request, its queries' own
                               tokens among them                              */
-  const int32_t *cu_q; /* [batch + 1], or NULL: tokens / batch queries each  */
+  const int32_t *cu_q; /* [batch + 1], not falling, or NULL: tokens / batch
+                          queries each. Where an offset falls or is out of range
+                          the requests from there on may not be served          */
   float *lse;          /* optional fp32 [tokens, heads], softmax only        */
   const float *head_param; /* as in chia_attn.h                              */
   float scale;
