@@ -57,15 +57,14 @@ struct Request {
   int row0, row1;  // an entry of the line: these rows (queries x heads of a group) of the request
   Tiles tl;        // the tiles that they visit
 };
-__device__ __forceinline__ bool offsets_ok(const PagedArgs &a, int t0, int t1) {
-  return t0 >= 0 && t1 >= t0 && t1 <= a.tokens;
-}
+__device__ __forceinline__ bool offsets_ok(int t0, int t1, int tokens) { return t0 >= 0 && t1 >= t0 && t1 <= tokens; }
 // The requests before the first whose offsets are out of range or fall. Those behind it
 // are not served: they could own rows that others own, and the line, whose length the
-// host bounds by the number of rows, could pass 32 bits.
-static __device__ __noinline__ int requests_in_order(const PagedArgs &a) {
+// host bounds by the number of rows, could pass 32 bits. (It takes no PagedArgs: a
+// reference would have every call put a copy of them on the stack.)
+static __device__ __noinline__ int requests_in_order(const int32_t *cu_q, int batch, int tokens) {
   int b = 0;
-  while (b < a.batch && offsets_ok(a, a.cu_q[b], a.cu_q[b + 1])) ++b;
+  while (b < batch && offsets_ok(cu_q[b], cu_q[b + 1], tokens)) ++b;
   return b;
 }
 // bad: what the status word is told; gap: the offsets are bad
@@ -75,7 +74,7 @@ __device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &b
   if (a.cu_q != nullptr) {
     r.t0 = a.cu_q[b];
     const int t1 = a.cu_q[b + 1];
-    if (offsets_ok(a, r.t0, t1)) {
+    if (offsets_ok(r.t0, t1, a.tokens)) {
       r.n = t1 - r.t0;
     } else {
       bad = gap = true;
@@ -292,7 +291,7 @@ struct Line {
       if (t < a.batch) blocks = (request_of(a, t, bad, gap).row1 + ROWS - 1) / ROWS;
       int at = blocks;
       if (scan(at, none, entries, x, gap)) {
-        if (t >= requests_in_order(a)) blocks = 0;
+        if (t >= requests_in_order(a.cu_q, a.batch, a.tokens)) blocks = 0;
         at = blocks;
         scan(at, none, entries, x);
       }
@@ -323,7 +322,7 @@ struct Line {
     if (BLOCKS) {
       __syncthreads();
     } else if (__syncthreads_or(gap)) {
-      const int ordered = requests_in_order(a);
+      const int ordered = requests_in_order(a.cu_q, a.batch, a.tokens);
       for (int b = t; b < entries; b += THREADS)
         if (b >= ordered) s.req[b].row1 = 0;
       __syncthreads();
