@@ -102,6 +102,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   __shared__ typename L::Shared line_sm;
   __shared__ __align__(8) uint64_t bars[kSplitWarps * NST];
   __shared__ float part_ml[kSplitWarps][ROWS][2];
+  __shared__ uint8_t s_lost[kSplitWarps][C::SCALES];  // beside the scales: see `lost`
   __shared__ Unit s_head[kSplitWarps], s_end[kSplitWarps];
   __shared__ int s_has_head[kSplitWarps], s_has_end[kSplitWarps];  // end: 1 begun here, 2 before
   __shared__ volatile int abort_flag;
@@ -159,6 +160,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   // needed: with HBM busy a load takes longer than the ring lasts.
   const int pshift = 31 - __clz(a.page);
   int row0 = -1, row1 = -1, tok = 0;
+  int lost = 0;           // bits: keys 0-15, 16-31 have a page out of range: nothing is loaded, no row sees them
+  bool any_lost = false;  // so far
   int next_pg0 = -1, next_pg1 = -1, next_hk = 0, next_tok = 0;  // pages
   int wanted = 0;                                                // bits: that there are such keys
   float next_ks0 = 0.f, next_vs0 = 0.f, next_ks1 = 0.f, next_vs1 = 0.f;
@@ -185,7 +188,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   };
   auto take_rows = [&] {
     row0 = row_at(next_pg0), row1 = row_at(next_pg1), tok = next_tok;
-    if ((row0 < 0 && (wanted & 1)) || (row1 < 0 && (wanted & 2))) report(a.status, kStatusBadIndex);
+    lost = row0 < 0 && (wanted & 1) ? (a.page == 16 ? 1 : 3) : 0;
+    if (row1 < 0 && (wanted & 2)) lost |= 2;
+    if (lost) report(a.status, kStatusBadIndex);
   };
   auto take_scales = [&](int k) {  // to shared memory
     float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -195,6 +200,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     else if (row1 >= 0)
       sc.z = next_ks1, sc.w = value_factor<SOFTMAX>(next_vs1);
     scales[(k + lane) % C::SCALES] = sc;  // (those of 64 tiles ago are long used)
+    s_lost[warp][(k + lane) % C::SCALES] = static_cast<uint8_t>(lost);
+    any_lost |= __any_sync(0xffffffffu, lost != 0);
     __syncwarp();
   };
   auto issue = [&](int k) {  // start the copies of tile k, whose stage is free
@@ -348,8 +355,9 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       const int j0 = tl.key_tile(ut0 + i) * TK;
       float4 sc = scales[kk % C::SCALES];
       const uint32_t kst = ring + stage * C::STAGE, vst = kst + TK * D;
-      const bool all = a.dil == 1 ? (j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf
-                                  : j0 + TK <= pf;
+      const int gone = any_lost ? s_lost[warp][kk % C::SCALES] : 0;  // keys that are not there
+      const bool all = gone == 0 && (a.dil == 1 ? (j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf
+                                                : j0 + TK <= pf);
       if (!all) {  // the scales of 16 keys that nobody sees may be anything
         const bool s0 = j0 < pf || (j0 <= hi_max && j0 + 15 >= lo_min);
         const bool s1 = j0 + 16 < pf || (j0 + 16 <= hi_max && j0 + 31 >= lo_min);
@@ -449,7 +457,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
                 const int j = j0 + 16 * m + 8 * x + gid;
-                const bool vis = ((real >> (2 * n + e)) & 1u) &&
+                const bool vis = ((real >> (2 * n + e)) & 1u) && !((gone >> m) & 1) &&
                                  (j < pf || (j >= lo && j <= hi &&
                                              (a.dil == 1 || divides(a.dil, i_pos - j))));
                 if (!vis) s[m][n][2 * x + e] = SOFTMAX ? -INFINITY : 0.f;
@@ -544,6 +552,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             const int j = j0 + 16 * m + 8 * x + 2 * tig;
             some[x] = (j < pf || (j >= lo_min && j <= hi_max) ? 0x0101u : 0u) |
                       (j + 1 < pf || (j + 1 >= lo_min && j + 1 <= hi_max) ? 0x01010000u : 0u);
+            if ((gone >> m) & 1) some[x] = 0;
           }
 #pragma unroll
           for (int c = 0; c < MT / 2; ++c)
@@ -571,6 +580,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       if (CT == CACHE_E4M3 && !all && __any_sync(0xffffffffu, nan_seen)) {
         // The NaN values left out above go to the rows that do see their keys.
         for (int kk = 0; kk < TK; ++kk) {
+          if ((gone >> (kk / 16)) & 1) continue;
           const int j = j0 + kk;
           const int sw = D == 128 ? kk & 7 : (kk >> 1) & 3;
           bool sees[NT][2];

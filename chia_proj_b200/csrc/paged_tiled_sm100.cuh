@@ -107,8 +107,9 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedA
 }
 
 // Channels (bits) in which a visible key of tiles [t0, t1) of the unit holds
-// NaN, where the tile is not visible as a whole: the converters leave NaN out
-// of such tiles, since a P of zero would spread it to rows that do not see it.
+// NaN, where the tile is not visible as a whole (pages out of range are not): the
+// converters leave NaN out of such tiles, since a P of zero would spread it to rows
+// that do not see it.
 template <int D>
 __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_cache, int b, int hk,
                                           const Tiles &tl, int t0, int t1, int i, int len, int lo_max,
@@ -119,7 +120,12 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
   for (int t = t0; t < t1; ++t) {
     constexpr int TK = TiledConfig<D>::TK;
     const int j0 = tl.key_tile(t) * TK;
-    if ((a.dil == 1 && j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf) continue;
+    bool whole = (a.dil == 1 && j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf;
+    for (int j = j0; j < j0 + TK && whole; j += 16) {
+      const int pg = a.block_table[b * a.table_stride + j / a.page];
+      whole = pg >= 0 && pg < a.num_pages;
+    }
+    if (whole) continue;
     for (int j = j0; j < min(j0 + TK, len); ++j) {
       if (!(j < pf || (j >= lo && j <= hi && (a.dil == 1 || divides(a.dil, i - j))))) continue;
       const int pg = a.block_table[b * a.table_stride + j / a.page];
@@ -155,7 +161,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, nan_flag;
   __shared__ float q_scale[256];  // of the rows of Q, undone in the scores
-  __shared__ int tile_full[SETS], tile_live[SETS];  // all rows see the whole tile; keys there are
+  // of a tile: all rows see the whole of it; keys there are; bits, 16 keys each: their page
+  // is out of range, so that nothing is loaded and no row sees them
+  __shared__ int tile_full[SETS], tile_live[SETS], tile_lost[SETS];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   auto bar = [&](int i) { return ptx::smem_u32(bars) + 8 * i; };
   if (t == 0) {
@@ -280,7 +288,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         if (!warp_all(wait(SC_EMPTY + k % SETS, ((k / SETS) & 1) ^ 1))) break;
         const Keys now = k1;
         row = row1, ks = ks1, vs = vs1;
-        if (row < 0 && (now.all & 4)) report(a.status, kStatusBadIndex);
+        const bool bad = row < 0 && (now.all & 4);
+        const int lost = static_cast<int>(__ballot_sync(0xffffffffu, bad));
+        if (bad) report(a.status, kStatusBadIndex);
         if (lane < GROUPS) {
           float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
           if (row >= 0 && !(now.all & 2)) {
@@ -290,7 +300,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           }
           scales[(k % SETS) * GROUPS + lane] = sc;
         }
-        if (lane == 0) tile_full[k % SETS] = now.all & 1, tile_live[k % SETS] = now.live;
+        if (lane == 0)
+          tile_full[k % SETS] = lost == 0 && (now.all & 1), tile_live[k % SETS] = now.live, tile_lost[k % SETS] = lost;
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar(SC_FULL + k % SETS));
         k1 = k2;
@@ -543,7 +554,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           ptx::tmem_ld32(tS + 32, sr[1]);
           const int j0 = h.rq.tl.key_tile(h.ut0 + i) * TK;
           const float4 *sc = scales + (n % SETS) * GROUPS;
-          const bool all = sees_all(h, j0);
+          const bool all = tile_full[n % SETS];
           uint32_t vis[2] = {~0u, ~0u};  // the keys of the tile that this row sees
           if (!all) {
             auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; };
@@ -558,6 +569,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                 m &= every;
               }
               vis[c] = real ? m | below(pf - k0) : 0u;
+              const int lost = tile_lost[n % SETS] >> (2 * c);
+              vis[c] &= (lost & 1 ? 0u : 0xffffu) | (lost & 2 ? 0u : 0xffff0000u);
             }
           }
           ptx::tmem_wait_ld();

@@ -173,7 +173,8 @@ typedef struct chia_paged_params {
   uint64_t wait_limit_ns; /* as in chia_attn.h                               */
 } chia_paged_params_t;
 
-/* A row that sees no key gets zeros (log-sum-exp -inf). Rows of q that no
+/* Keys whose page is out of range are reported and left out, as if the mask hid
+ * them. A row that sees no key gets zeros (log-sum-exp -inf). Rows of q that no
  * request owns are not written. */
 CHIA_API int chia_paged_attn(const chia_paged_params_t *params, void *stream);
 
