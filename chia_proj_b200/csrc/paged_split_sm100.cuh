@@ -190,7 +190,6 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     row0 = row_at(next_pg0), row1 = row_at(next_pg1), tok = next_tok;
     lost = row0 < 0 && (wanted & 1) ? (a.page == 16 ? 1 : 3) : 0;
     if (row1 < 0 && (wanted & 2)) lost |= 2;
-    if (lost) report(a.status, kStatusBadIndex);
   };
   auto take_scales = [&](int k) {  // to shared memory
     float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -363,6 +362,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         const bool s1 = j0 + 16 < pf || (j0 + 16 <= hi_max && j0 + 31 >= lo_min);
         if (!s0) sc.x = sc.y = 0.f;
         if (!s1) sc.z = sc.w = 0.f;
+        // (so may their page, a window's left behind for one)
+        if (lane == 0 && ((s0 && (gone & 1)) || (s1 && (gone & 2)))) report(a.status, kStatusBadIndex);
       }
       // ---------------- S^T = K Q^T
       float s[2][NT][4];

@@ -288,7 +288,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         if (!warp_all(wait(SC_EMPTY + k % SETS, ((k / SETS) & 1) ^ 1))) break;
         const Keys now = k1;
         row = row1, ks = ks1, vs = vs1;
-        const bool bad = row < 0 && (now.all & 4);
+        const bool bad = row < 0 && (now.all & 6) == 4;
         const int lost = static_cast<int>(__ballot_sync(0xffffffffu, bad));
         if (bad) report(a.status, kStatusBadIndex);
         if (lane < GROUPS) {

@@ -174,7 +174,7 @@ typedef struct chia_paged_params {
 } chia_paged_params_t;
 
 /* Keys whose page is out of range are reported and left out, as if the mask hid
- * them. A row that sees no key gets zeros (log-sum-exp -inf). Rows of q that no
+ * them; entries of pages that no query sees may be anything. A row that sees no key gets zeros (log-sum-exp -inf). Rows of q that no
  * request owns are not written. */
 CHIA_API int chia_paged_attn(const chia_paged_params_t *params, void *stream);
 

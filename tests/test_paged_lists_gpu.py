@@ -150,3 +150,18 @@ def test_nan_beside_a_page_out_of_range(cuda, counts):
     reported()
     want[:cu[1], 2:, 77] = float("nan")
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("counts", [[1, 3], [120, 100]])
+def test_pages_that_no_query_sees_may_be_anything(cuda, counts, page):
+    """A window has moved on and its old pages are given back: their entries are no pages any more. Nothing is reported,
+    and no bit changes."""
+    lens, mask = [1037, 796], cp.Mask(left=37, right=0, prefix=1)  # first keys of the windows amid a tile
+    q, k, v, ks, vs, table, cu = setup(lens, counts, 8, 2, 64, page, E4M3, BF16, 7)
+    run = lambda: cp.paged_attention(q, k, v, ks, vs, ints(table), ints(lens), ints(cu), mask=mask)  # noqa: E731
+    want = run()
+    for b, n in enumerate(lens):
+        for p in range(1, (n - counts[b] - 37) // page):
+            table[b][p] = (-1, 2 ** 31 - 1, k.shape[0])[p % 3]
+    assert torch.equal(run(), want)
