@@ -99,15 +99,17 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
     const bool served = fits && (need == 0 || upto <= count);
     if (b < a.batch && !served) bad |= kStatusNoPages;
     const long long cu = tokens0 + sc.b - add;
-    s_cu[t] = static_cast<int32_t>(cu < a.max_tokens ? cu : a.max_tokens);
+    // (tokens past max_tokens have no slot to be told, but their pages are entered all the same)
+    constexpr long long kMost = 0x7fffffff;
+    s_cu[t] = static_cast<int32_t>(min(cu, kMost));
     s_len[t] = len;
     s_first[t] = served ? static_cast<int32_t>(upto - need) : -1;
     if (t == kTablesThreads - 1) {
       const long long end = tokens0 + tot.b;
-      s_cu[kTablesThreads] = static_cast<int32_t>(end < a.max_tokens ? end : a.max_tokens);
+      s_cu[kTablesThreads] = static_cast<int32_t>(min(end, kMost));
     }
     if (first_cta && b < a.batch) {
-      a.cu_q[b] = static_cast<int32_t>(cu);
+      a.cu_q[b] = static_cast<int32_t>(min(cu, kMost));
       a.new_seq_lens[b] = served ? len + add : len;
     }
     if (served && need > 0) taken = static_cast<int>(upto);  // (those served come first)
@@ -142,8 +144,10 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
         else
           slot = (page << shift) + off;
       }
-      a.slots[x] = slot;
-      a.positions[x] = pos;
+      if (x < a.max_tokens) {
+        a.slots[x] = slot;
+        a.positions[x] = pos;
+      }
     }
     pages0 += tot.a;
     tokens0 += tot.b;

@@ -78,7 +78,8 @@ typedef struct chia_tables_params {
  * when the ring has not enough left for it and those before it, is not served:
  * its slots are -1, its length stays, and CHIA_ERR_NO_PAGES is reported (cu_q
  * counts its tokens all the same). A free_state out of range is reported and
- * taken as an empty ring. Entries of slots and positions past the
+ * taken as an empty ring. Tokens past max_tokens are reported; they have pages
+ * and count in the lengths, but no slots. Entries of slots and positions past the
  * step's tokens are -1 and 0. seq_lens and free_state are not changed (the new
  * ones are outputs), so a step may be run again. */
 CHIA_API int chia_page_tables(const chia_tables_params_t *params, void *stream);

@@ -78,3 +78,24 @@ def test_release_into_a_bad_ring(cuda, state):
     assert step.slots.tolist() == [36, -1, -1, -1] and step.seq_lens.tolist() == [21, 30]
     with pytest.raises(cp.ChiaError, match="NO_PAGES"):
         cp.check_device_status(0)
+
+
+@pytest.mark.parametrize("most", [0, 1, 40, 1500, 2999])
+def test_no_page_is_lost_past_max_tokens(cuda, most):
+    """A step with more tokens than max_tokens is reported; the pages that it took stand in the table all the same, so that
+    they can be given back."""
+    page, width = 16, 80
+    lens, new = [5, 0, 33], [1000, 1200, 800]
+    table = torch.full((3, width), -9, dtype=torch.int32)
+    table[0, 0], table[2, :3] = 500, torch.tensor([501, 502, 503])
+    ring = list(range(300))
+    want = po.tables(lens, new, table.tolist(), ring, [290, 250], page, 3000)
+    dev, dring = table.cuda(), ints(ring)
+    got = cp.page_tables(ints(lens), ints(new), dev, dring, ints([290, 250]), page_size=page, max_tokens=most)
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+    assert got.slots.tolist() == want[0][:most] and got.positions.tolist() == want[1][:most]
+    assert got.cu_q.tolist() == want[2] and got.seq_lens.tolist() == want[3] and got.free_state.tolist() == want[4]
+    assert dev.tolist() == want[5]
+    _, state = cp.release_pages(ints([1, 1, 1]), got.seq_lens, dev, dring, got.free_state, page_size=page)
+    assert state.tolist()[1] == 250 + 4
