@@ -256,9 +256,14 @@ struct AppendArgs {
 // the largest value decides the scale, then the values are rounded and stored.
 // Bound by HBM: 2 bytes in and 1 out for each value. A CTA looks at `window`
 // tokens and works on the runs of tokens of one page that begin there: a page's
-// worth for prompts, one for decode steps, so that their few runs spread out.
+// worth for prompts, one for decode steps, so that their few runs spread out. A run is
+// what follows a page's first token within a page's number of rows, up to a token of
+// another page; skipped tokens may lie between. The tokens before tell whether the run
+// began earlier. A page that comes again behind another one, or goes on for more rows,
+// would be rewritten by two CTAs at a time: that is seen a page's number of rows back,
+// reported, and the later tokens are left out.
 // Measured (8 K/V heads, D 128, bf16 to e4m3, pages of 64): 16 prompts of up to 4,099
-// tokens 42 us, 5.2 TB/s, 79% of the copy rate; 64 single tokens 3.7 us, the launch and
+// tokens 43 us, 5.1 TB/s, 78% of the copy rate; 64 single tokens 3.9 us, the launch and
 // three dependent loads (slots, input, scale).
 template <int D, bool BF16, int CT, int IT>
 __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(const AppendArgs a, int window) {
@@ -267,8 +272,15 @@ __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(con
   constexpr int PAGE = IT * STEP;    // page_size
   constexpr int SHIFT = PAGE == 16 ? 4 : PAGE == 32 ? 5 : PAGE == 64 ? 6 : 7;
   __shared__ uint32_t s_max[2][4];
-  __shared__ int s_slot[2 * PAGE + 1];  // from the token before the window on
-  __shared__ unsigned s_same[2][4], s_first[2][4];
+  __shared__ int s_slot[4 * PAGE];  // of the window, one page's number of rows before it and two behind it
+  // Ballots of a run, one set for each of the warps whose lanes stand for a page's rows:
+  // rows from its first token on that continue it; tokens of the page among them, of the
+  // page's first slot; tokens in the rows before it, nearest first, of the page among them.
+  struct __align__(16) Ballots {
+    unsigned same, in, first, prev, prev_in;
+  };
+  constexpr int WORDS = (PAGE + 31) / 32;
+  __shared__ Ballots s_run[2][WORDS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kinds = 2 * a.heads_kv;
   const int which = blockIdx.x % kinds, h = which >> 1;
@@ -279,55 +291,80 @@ __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(con
                         (tid % LANES) * 8;
   const int64_t st = is_v ? a.v_st : a.k_st;
   follow();
-  for (int e = tid; e < window + PAGE; e += 128) {  // (a run that begins in the window ends here)
-    const int x = w0 - 1 + e;
-    s_slot[e] = x >= 0 && x < a.tokens ? a.slots[x] : -1;
+#pragma unroll
+  for (int e = tid; e < 4 * PAGE; e += 128) {  // (all loads at once)
+    const int x = w0 - PAGE + e;
+    s_slot[e] = e < window + 3 * PAGE && x >= 0 && x < a.tokens ? a.slots[x] : -1;
   }
   __syncthreads();
-  // Two sets of s_same, s_first and s_max by turns, one a run: a run has a barrier at
-  // least, so a set is written again only behind the barrier of the run between.
+  // Two sets of s_run and s_max by turns, one a run: a run has a barrier at least, so a set
+  // is written again only behind the barrier of the run between.
   int par = 1;
   for (int t0 = w0; t0 < w1;) {
-    const int at = t0 - w0 + 1, slot0 = s_slot[at];
+    const int at = t0 - w0 + PAGE, slot0 = s_slot[at];
     if (slot0 < 0) {  // skipped
       ++t0;
       continue;
     }
-    // the run: the following tokens in the same page
+    // the run: the following tokens in the same page, and skipped ones between them
     par ^= 1;
     const int page = slot0 >> SHIFT;
-    const int mine = tid < PAGE && at + tid < window + PAGE ? s_slot[at + tid] : -1;
-    const bool in = mine >= 0 && (mine >> SHIFT) == page;
-    const unsigned same = __ballot_sync(0xffffffffu, in);
-    const unsigned first = __ballot_sync(0xffffffffu, in && (mine & (PAGE - 1)) == 0);
-    if (lane == 0) s_same[par][warp] = same, s_first[par][warp] = first;
+    if (warp < WORDS) {
+      const bool row = PAGE >= 32 || lane < PAGE;
+      const int next = row ? s_slot[at + tid] : -1, last = row ? s_slot[at - 1 - tid] : -1;
+      const int later = row ? s_slot[at + PAGE + tid] : -1;
+      const bool in = (next >> SHIFT) == page;  // (that of a skipped one is negative)
+      Ballots b;
+      b.in = __ballot_sync(0xffffffffu, in);
+      b.same = b.in | __ballot_sync(0xffffffffu, row && next < 0);
+      b.first = __ballot_sync(0xffffffffu, in && (next & (PAGE - 1)) == 0);
+      b.prev = __ballot_sync(0xffffffffu, last >= 0);
+      b.prev_in = __ballot_sync(0xffffffffu, (last >> SHIFT) == page);
+      if (lane == 0) s_run[par][warp] = b;
+      if ((later >> SHIFT) == page && which == 0) report(a.status, kStatusBadIndex);  // more rows than a page's
+    }
     __syncthreads();
     int n = 0;
     bool fresh = false;  // it holds the page's first slot
+    bool begun = false;  // the token before is of this page, or one before that
+    bool adjacent = false;
+    bool holes = false;  // skipped tokens in the run
+    unsigned before = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-      if (n == 32 * w) {
-        const unsigned gap = ~s_same[par][w];
-        const int here = gap == 0 ? 32 : __ffs(gap) - 1;
-        n += here;
-        fresh |= here > 0 && (s_first[par][w] << (32 - here)) != 0;
+    for (int w = 0; w < WORDS; ++w) {
+      const Ballots b = s_run[par][w];
+      if (before == 0) {
+        before = b.prev & -b.prev;
+        adjacent = (b.prev_in & before) != 0;
       }
-    const int before = s_slot[at - 1];
-    const bool begun = before >= 0 && (before >> SHIFT) == page;  // in an earlier window
+      begun |= b.prev_in != 0;
+      if (n == 32 * w) {
+        const int here = b.same == ~0u ? 32 : __ffs(~b.same) - 1;
+        const unsigned rows = here == 32 ? ~0u : (1u << here) - 1;
+        n += here;
+        fresh |= (b.first & rows) != 0;
+        holes |= (~b.in & rows) != 0;
+      }
+    }
     if (begun || page >= a.num_pages) {
-      if (!begun && tid == 0 && which == 0) report(a.status, kStatusBadIndex);
+      if (!adjacent && tid == 0 && which == 0) report(a.status, kStatusBadIndex);
       t0 += n;
       continue;
     }
     const int64_t ph = static_cast<int64_t>(page) * a.heads_kv + h;
     uint8_t *dst = (is_v ? a.v_cache : a.k_cache) + ph * PAGE * D;
     float *scale = (is_v ? a.v_scale : a.k_scale) + ph;
+    unsigned skipped = 0;  // bits: this thread's rows
+    if (holes) {
+#pragma unroll 1
+      for (int i = 0; i < IT; ++i) skipped |= (s_slot[at + i * STEP + tid / LANES] < 0 ? 1u : 0u) << i;
+    }
     uint4 x[IT];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int r = i * STEP + tid / LANES;
       x[i] = make_uint4(0, 0, 0, 0);
-      if (r < n) x[i] = *reinterpret_cast<const uint4 *>(src + (t0 + r) * st);
+      if (r < n && !((skipped >> i) & 1)) x[i] = *reinterpret_cast<const uint4 *>(src + (t0 + r) * st);
     }
     const float old = *scale;
     // the largest value: 16-bit patterns without their signs order as the values do
@@ -380,7 +417,7 @@ __global__ void __launch_bounds__(128, IT == 16 ? 4 : 8) cache_append_kernel(con
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int r = i * STEP + tid / LANES;
-      if (r < n) {
+      if (r < n && !((skipped >> i) & 1)) {
         const float2 f0 = in16x2_to_float2<BF16>(x[i].x), f1 = in16x2_to_float2<BF16>(x[i].y);
         const float2 f2 = in16x2_to_float2<BF16>(x[i].z), f3 = in16x2_to_float2<BF16>(x[i].w);
         *reinterpret_cast<uint2 *>(dst + (s_slot[at + r] & (PAGE - 1)) * D + (tid % LANES) * 8) =

@@ -107,7 +107,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache:
     """Write the tokens ``k, v`` ``[T, H_kv, D]`` (bf16 or fp16) to ``slots``
     ``[T]`` (int32; -1: skipped) of the cache, in place.
 
-    The tokens of one page are adjacent rows, as ``page_tables`` lays them out.
+    The tokens of one page are adjacent rows, as ``page_tables`` lays them out;
+    skipped ones may lie between them.
     Scales are powers of two, the smallest that hold the page's largest finite
     value. Tokens that hold a page's first slot begin the page anew; others
     keep its scale or, where they need a larger one, have the values that the

@@ -114,7 +114,10 @@ typedef struct chia_append_params {
 } chia_append_params_t;
 
 /* The tokens of one page in one call are adjacent rows of k and v (as
- * chia_page_tables lays them out). Where they hold the page's first slot the
+ * chia_page_tables lays them out), skipped ones between them or not, page_size
+ * rows at most. A page that comes again within so many rows is reported, and those
+ * tokens are left out; further apart it is not seen, and what the page then holds
+ * is not defined. Where they hold the page's first slot the
  * page begins anew: its scale comes from them alone. Otherwise the page keeps
  * its scale if that is large enough for them, or takes theirs, and then every
  * value the page holds is expressed in the new scale. Values are rounded to

@@ -45,6 +45,71 @@ def test_runs_between_skipped_tokens(cuda, page, hkv, D, ct, dtype, T, seed):
             cp.check_device_status(0)
 
 
+def compact(slots, x):
+    """The tokens that are not skipped: what one page gets in one call is written together."""
+    keep = [t for t, s in enumerate(slots) if s >= 0]
+    return [slots[t] for t in keep], x[keep]
+
+
+def check_contents(x, slots, before, cache, hkv):
+    """The cache after the call, against the oracle's write of these tokens into what was there before."""
+    for i in range(2):
+        w, s = (before[i].double(), cache[i].dtype), before[2 + i].double()
+        po.append(x[:, i * hkv:(i + 1) * hkv], slots, w, s)
+        assert torch.equal(cache[2 + i].double().cpu(), s)
+        assert torch.equal(cache[i].double().cpu(), w[0])
+
+
+@pytest.mark.parametrize("page,hkv,D,ct,T", [(16, 8, 64, E4M3, 2500), (64, 16, 64, I8, 4000), (128, 16, 64, E4M3, 9000),
+                                             (16, 2, 128, I8, 300), (128, 1, 128, E4M3, 400)])
+@pytest.mark.parametrize("seed", range(3))
+def test_skipped_tokens_within_a_page(cuda, page, hkv, D, ct, T, seed):
+    """Tokens of runs of every kind skipped at random, also a page's first and all but its last: as if the others alone
+    were there, with one scale for them all."""
+    g = torch.Generator().manual_seed(100 + seed)
+    rnd = lambda n: int(torch.randint(0, n, (1,), generator=g))  # noqa: E731
+    slots, pages = [], 0
+    while len(slots) < T:
+        off = rnd(page) if rnd(3) else 0
+        n = 1 + rnd(page - off) if rnd(3) else page - off
+        run = [pages * page + off + i for i in range(n)]
+        pages += 1
+        often = rnd(4)
+        slots += [-1 if rnd(4) < often else s for s in run]
+    cache = make_cache(pages, hkv, page, D, ct, g)
+    before = [c.clone().cpu() for c in cache]
+    x = (torch.randn(len(slots), 2 * hkv, D, generator=g) * 30).to(BF16)
+    dev = x.cuda()
+    cp.cache_append(dev[:, :hkv], dev[:, hkv:], ints(slots), *cache)
+    kept, xs = compact(slots, x)
+    check_contents(xs, kept, before, cache, hkv)
+
+
+@pytest.mark.parametrize("page,hkv,lead", [(16, 2, 0), (32, 1, 0), (64, 2, 0), (128, 2, 0), (16, 8, 75), (64, 16, 40), (128, 16, 40)])
+def test_a_page_that_comes_again_is_reported(cuda, page, hkv, lead):
+    """Two requests' tokens by turns, a page behind another one, more rows than a page has: what came first is written.
+    Alone, where a CTA looks at one token, and behind so many pages (lead) that it looks at a page's worth."""
+    D = 64
+    g = torch.Generator().manual_seed(page)
+    a, b, c = ([(lead + p) * page + i for i in range(page)] for p in (2, 0, 3))
+    ahead = [p * page + i for p in range(lead) for i in range(page)][:lead * page - 5]
+    n = len(ahead)
+    assert not lead or n // page * 2 * hkv >= 8 * 148
+    for slots, first in (([a[1], b[1], a[2], b[2]], [0, 1]), (a[3:6] + b[:2] + a[6:8] + c[1:2], [0, 1, 2, 3, 4, 7]),
+                         (a + [a[0]], range(page)), (a + a[:3] + b[4:6], [*range(page), page + 3, page + 4]),
+                         (a + [-1, -1, a[5]] + b[4:6], [*range(page), page + 3, page + 4])):
+        cache = make_cache(lead + 4, hkv, page, D, E4M3, g)
+        before = [t.clone().cpu() for t in cache]
+        slots = ahead + slots
+        x = torch.randn(len(slots), 2 * hkv, D, generator=g).to(BF16)
+        dev = x.cuda()
+        cp.cache_append(dev[:, :hkv], dev[:, hkv:], ints(slots), *cache)
+        with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+            cp.check_device_status(0)
+        kept = [*range(n), *(n + t for t in first)]
+        check_contents(x[kept], [slots[t] for t in kept], before, cache, hkv)
+
+
 @pytest.mark.parametrize("B", [3, 1024, 2300])
 def test_release_of_bad_lengths(cuda, B):
     """Lengths that no row holds, near 2^31 and below zero, give nothing back; the others' pages come back in order."""
