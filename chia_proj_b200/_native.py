@@ -120,6 +120,7 @@ PAGED_SYMBOLS = (
     "chia_cache_append",
     "chia_paged_attn",
     "chia_paged_attn_workspace_bytes",
+    "chia_trim_pages",
 )
 
 
@@ -292,7 +293,7 @@ def load() -> ctypes.CDLL:
             lib.chia_attn_status_string.restype = ctypes.c_char_p
             lib.chia_attn_abi_version.argtypes = []
             lib.chia_attn_abi_version.restype = ctypes.c_int
-            for name in PAGED_SYMBOLS[:4]:  # the parameters as the bytes of their struct
+            for name in PAGED_SYMBOLS[:4] + PAGED_SYMBOLS[5:]:  # the parameters as the bytes of their struct
                 getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
                 getattr(lib, name).restype = ctypes.c_int
             lib.chia_paged_attn_workspace_bytes.argtypes = [ctypes.c_char_p]

@@ -31,7 +31,7 @@ namespace {
 
 using at::Tensor;
 
-decltype(&chia_page_tables) g_tables, g_release;
+decltype(&chia_page_tables) g_tables, g_release, g_trim;
 decltype(&chia_cache_append) g_append;
 decltype(&chia_paged_attn) g_attn;
 decltype(&chia_paged_attn_workspace_bytes) g_bytes;
@@ -166,7 +166,7 @@ Tensor piece(const Tensor &buf, int64_t at, int64_t n) {
 }
 
 // --------------------------------------------------------------------- tables
-// seq_lens, lens, block_table, free_pages, free_state, page_size, max_tokens (-1: release), status
+// seq_lens, lens, block_table, free_pages, free_state, page_size, max_tokens (-1: release, -2: trim), status
 PyObject *tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
     const at::AutoDispatchBelowADInplaceOrView plain;  // outputs carry no gradients
@@ -180,7 +180,7 @@ PyObject *tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (B < 1 || table.size(1) < 1 || ring.size(0) < 1)
       throw ValueError("empty seq_lens, block_table or free_pages");
     a.ints(0, "seq_lens", {B}, dev);
-    const Tensor &what = a.ints(1, release ? "done" : "new_lens", {B}, dev);
+    const Tensor &what = a.ints(1, most == -1 ? "done" : release ? "keep_lens" : "new_lens", {B}, dev);
     a.ints(2, "block_table", {B, table.size(1)}, dev);
     a.ints(3, "free_pages", {ring.size(0)}, dev);
     const Tensor &state = a.ints(4, "free_state", {2}, dev);
@@ -210,7 +210,7 @@ PyObject *tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     p.new_free_state = o + 2 * T + 2 * B + 1;
     p.status = reinterpret_cast<int32_t *>(a.integer(7));
     void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-    const int code = release ? g_release(&p, stream) : g_tables(&p, stream);
+    const int code = (most == -1 ? g_release : release ? g_trim : g_tables)(&p, stream);
     if (code != CHIA_OK) return PyLong_FromLong(code);
     const int64_t at[5] = {0, T, 2 * T, 2 * T + B + 1, 2 * T + 2 * B + 1}, n[5] = {T, T, B + 1, B, 2};
     PyObject *out = PyTuple_New(release ? 2 : 5);
@@ -414,11 +414,11 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 // Addresses of libchia_attn.so's entry points, in the order below.
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
-    const Args a(args, nargs, 5);
+    const Args a(args, nargs, 6);
     auto set = [&](auto &f, int i) {
       f = reinterpret_cast<std::decay_t<decltype(f)>>(static_cast<uintptr_t>(a.integer(i)));
     };
-    set(g_tables, 0), set(g_release, 1), set(g_append, 2), set(g_attn, 3), set(g_bytes, 4);
+    set(g_tables, 0), set(g_release, 1), set(g_append, 2), set(g_attn, 3), set(g_bytes, 4), set(g_trim, 5);
     Py_RETURN_NONE;
   });
 }

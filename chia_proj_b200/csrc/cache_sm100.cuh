@@ -175,11 +175,12 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
   if (bad && (first_cta || (bad & kStatusBadIndex))) report(a.status, bad);
 }
 
-// Pages of finished requests to the ring's tail: the same sums, the pages of a
-// chunk in the place of its tokens.
+// Pages of finished requests (TRIM: those past the tokens that a request keeps) to the
+// ring's tail: the same sums, the pages of a chunk in the place of its tokens.
+template <bool TRIM>
 __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const TablesArgs a) {
   __shared__ Scan2 sums[32];
-  __shared__ int32_t s_at[kTablesThreads + 1];
+  __shared__ int32_t s_at[kTablesThreads + 1], s_kept[kTablesThreads];  // s_kept: pages
   const int t = threadIdx.x;
   const bool first_cta = blockIdx.x == 0;
   follow();
@@ -195,20 +196,27 @@ __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const Tab
   int bad = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kTablesThreads) {
     const int b = b0 + t;
-    int len = 0, done = 0;
+    int len = 0, keep = 0;
     if (b < a.batch) {
       len = a.seq_lens[b];
-      done = a.new_lens[b] != 0 && ring_ok;
       if (len < 0) {
         bad |= kStatusBadIndex;
         len = 0;
       }
+      keep = TRIM ? a.new_lens[b] : a.new_lens[b] != 0 ? 0 : len;
+      if (keep < 0 || keep > len) {
+        bad |= kStatusBadIndex;
+        keep = len;
+      }
+      if (!ring_ok) keep = len;
     }
-    long long pages = done ? (static_cast<long long>(len) + a.page - 1) / a.page : 0;
-    if (pages > a.width) {  // which pages it holds is not known: it is not released
+    auto pages_of = [&](int n) { return (static_cast<long long>(n) + a.page - 1) / a.page; };
+    if (keep < len && pages_of(len) > a.width) {  // which pages it holds is not known: it keeps them
       bad |= kStatusBadIndex;
-      pages = done = 0;
+      keep = len;
     }
+    const long long kept = pages_of(keep), pages = pages_of(len) - kept;
+    s_kept[t] = static_cast<int32_t>(kept);
     Scan2 tot;
     const Scan2 sc = block_scan2(Scan2{pages, 0}, tot, sums);
     // (of lengths that make no sense: pages past the 2^31st are in no ring)
@@ -216,12 +224,12 @@ __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const Tab
     s_at[t] = static_cast<int32_t>(min(sc.a - pages, kMost));
     if (t == 0) s_at[kTablesThreads] = static_cast<int32_t>(min(tot.a, kMost));
     __syncthreads();
-    if (first_cta && b < a.batch) a.new_seq_lens[b] = done ? 0 : len;
+    if (first_cta && b < a.batch) a.new_seq_lens[b] = keep;
     const int n = min(kTablesThreads, a.batch - b0);
     const int end = s_at[kTablesThreads];
     for (long long y = blockIdx.x * kTablesThreads + t; y < end; y += gridDim.x * kTablesThreads) {
       const int x = static_cast<int>(y), r = last_not_above(s_at, n, x);
-      const int page = a.block_table[(b0 + r) * a.table_stride + (x - s_at[r])];
+      const int page = a.block_table[(b0 + r) * a.table_stride + s_kept[r] + (x - s_at[r])];
       const long long at = pages0 + x;  // among all released pages
       if (count + at < a.ring)
         a.free_pages[(static_cast<long long>(head) + count + at) % a.ring] = page;

@@ -87,6 +87,15 @@ int tables_grid(int64_t items, int sms) {
   return static_cast<int>(n < 1 ? 1 : n > sms ? sms : n);
 }
 
+template <bool TRIM>
+int give_back(const chia_tables_params_t *p, void *stream) {
+  chia::TablesArgs a{};
+  int rc = tables_args(p, true, a), sms = 0;
+  if (rc != CHIA_OK || (rc = device_sms(sms)) != CHIA_OK) return rc;
+  return launched(chia::launch_after(chia::release_pages_kernel<TRIM>, dim3(tables_grid(p->ring_size, sms)),
+                                     chia::kTablesThreads, 0, static_cast<cudaStream_t>(stream), a));
+}
+
 // ---------------------------------------------------------------------- append
 int check_append(const chia_append_params_t *p) {
   if (p == nullptr || p->abi_version != CHIA_PAGED_ABI_VERSION) return CHIA_ERR_INVALID_ARGUMENT;
@@ -282,13 +291,9 @@ int chia_page_tables(const chia_tables_params_t *p, void *stream) {
                                      static_cast<cudaStream_t>(stream), a));
 }
 
-int chia_release_pages(const chia_tables_params_t *p, void *stream) {
-  chia::TablesArgs a{};
-  int rc = tables_args(p, true, a), sms = 0;
-  if (rc != CHIA_OK || (rc = device_sms(sms)) != CHIA_OK) return rc;
-  return launched(chia::launch_after(chia::release_pages_kernel, dim3(tables_grid(p->ring_size, sms)), chia::kTablesThreads, 0,
-                                     static_cast<cudaStream_t>(stream), a));
-}
+int chia_release_pages(const chia_tables_params_t *p, void *stream) { return give_back<false>(p, stream); }
+
+int chia_trim_pages(const chia_tables_params_t *p, void *stream) { return give_back<true>(p, stream); }
 
 int chia_cache_append(const chia_append_params_t *p, void *stream) {
   int rc = check_append(p), sms = 0;

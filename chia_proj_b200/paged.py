@@ -89,16 +89,25 @@ def page_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: tor
     return PageStep(*r)
 
 
-def release_pages(done: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor,
-                  free_pages: torch.Tensor, free_state: torch.Tensor, *,
-                  page_size: int) -> Tuple[torch.Tensor, torch.Tensor]:
+def release_pages(done: Optional[torch.Tensor], seq_lens: torch.Tensor, block_table: torch.Tensor,
+                  free_pages: torch.Tensor, free_state: torch.Tensor, *, page_size: int,
+                  keep_lens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Give the pages of the requests with ``done[b] != 0`` (int32) back: they
     are written to the ring's tail. Returns the new ``seq_lens`` (0 for those
-    requests) and ``free_state``."""
-    r = N.binding().tables(seq_lens, done, block_table, free_pages, free_state, page_size, -1,
+    requests) and ``free_state``.
+
+    ``keep_lens`` (int32, with ``done=None``): each request keeps its first
+    ``keep_lens[b]`` tokens, and the pages past them are given back. This is how
+    rejected tokens are taken out: a length that is lowered by hand leaves their
+    pages in no request and not in the ring.
+    """
+    if (done is None) == (keep_lens is None):
+        raise ValueError("release_pages takes either done or keep_lens")
+    what, mode = (done, -1) if keep_lens is None else (keep_lens, -2)
+    r = N.binding().tables(seq_lens, what, block_table, free_pages, free_state, page_size, mode,
                            _status(seq_lens))
     if type(r) is int:
-        N.check(r, "chia_release_pages")
+        N.check(r, "chia_release_pages" if mode == -1 else "chia_trim_pages")
     return r
 
 

@@ -5,7 +5,8 @@
  *
  *   chia_page_tables   the step's new pages, slots, positions and offsets from
  *                      the requests' lengths (chia_release_pages gives the
- *                      pages of finished requests back)
+ *                      pages of finished requests back, chia_trim_pages those
+ *                      of rejected tokens)
  *   chia_cache_append  the new tokens' keys and values into the cache, in 8
  *                      bits with one scale for each (page, K/V head)
  *   chia_paged_attn    the step's queries over the cache: every operator of
@@ -60,7 +61,8 @@ typedef struct chia_tables_params {
   int64_t max_tokens;  /* entries of slots and positions                     */
   const int32_t *seq_lens; /* [batch] tokens in the cache before the step    */
   const int32_t *new_lens; /* [batch] tokens the step adds (tables); non-zero:
-                              the request is finished (release)              */
+                              the request is finished (release); tokens that
+                              it keeps (trim)                                */
   int32_t *block_table;    /* [batch, table_width]; new pages are entered    */
   int32_t *free_pages;     /* ring of free pages; release writes its tail    */
   const int32_t *free_state; /* [2]: first entry of the ring, number of pages */
@@ -90,6 +92,13 @@ CHIA_API int chia_page_tables(const chia_tables_params_t *params, void *stream);
  * out of range all do, and new_free_state is an empty ring. The outputs slots,
  * positions and cu_q are not used. */
 CHIA_API int chia_release_pages(const chia_tables_params_t *params, void *stream);
+
+/* The same for the tail of a request, after drafted tokens were rejected: it keeps
+ * its first new_lens[b] tokens (0 to seq_lens[b]; anything else is reported and
+ * keeps all), and the pages past them go to the ring. A length that is lowered
+ * without this call takes the pages past it out of use: chia_page_tables enters
+ * new ones over them. */
+CHIA_API int chia_trim_pages(const chia_tables_params_t *params, void *stream);
 
 /* ------------------------------------------------------------------ append */
 typedef struct chia_append_params {
