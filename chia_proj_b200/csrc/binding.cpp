@@ -105,6 +105,16 @@ bool fits(const Tensor &t) {
          t.stride(1) >= 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// The kernels write below autograd; this tells it (a tensor that a graph has saved
+// must not change unseen).
+void written(const Tensor &t) {
+  if (!t.unsafeGetTensorImpl()->is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void no_tangent(const Tensor &t, const char *name) {
+  if (t._fw_grad(0).defined())
+    throw ValueError(std::string(name) + " has a forward-mode tangent: there is no derivative");
+}
+
 struct Cache {
   const Tensor &k, &v, &ks, &vs;
   int type;
@@ -132,11 +142,6 @@ struct Cache {
                          std::to_string(pages) + ", " + std::to_string(heads) + ") on " + dev.str());
   }
 };
-
-PyObject *code_or_none(int code) {
-  if (code != CHIA_OK) return PyLong_FromLong(code);
-  Py_RETURN_NONE;
-}
 
 // Any C++ exception ends here as a Python one.
 template <class F>
@@ -212,6 +217,7 @@ PyObject *tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     void *stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     const int code = (most == -1 ? g_release : release ? g_trim : g_tables)(&p, stream);
     if (code != CHIA_OK) return PyLong_FromLong(code);
+    written(release ? ring : table);
     const int64_t at[5] = {0, T, 2 * T, 2 * T + B + 1, 2 * T + 2 * B + 1}, n[5] = {T, T, B + 1, B, 2};
     PyObject *out = PyTuple_New(release ? 2 : 5);
     for (int i = release ? 3 : 0, j = 0; i < 5; ++i, ++j)
@@ -238,6 +244,7 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       throw ValueError("k, v must be " + str({shape, 3}) + " on " + c.dev.str() + ", got " + str(k->sizes()) + ", " +
                        str(v->sizes()));
     const Tensor &slots = a.ints(2, "slots", {T}, c.dev);
+    no_tangent(*k, "k"), no_tangent(*v, "v");
     if (T == 0) Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(c.dev);
     Tensor kc, vc;
@@ -262,7 +269,10 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     p.k_scale = ptr<float>(c.ks);
     p.v_scale = ptr<float>(c.vs);
     p.status = reinterpret_cast<int32_t *>(a.integer(7));
-    return code_or_none(g_append(&p, c10::cuda::getCurrentCUDAStream(c.dev.index()).stream()));
+    const int code = g_append(&p, c10::cuda::getCurrentCUDAStream(c.dev.index()).stream());
+    if (code != CHIA_OK) return PyLong_FromLong(code);
+    for (const Tensor *t : {&c.k, &c.v, &c.ks, &c.vs}) written(*t);
+    Py_RETURN_NONE;
   });
 }
 
@@ -318,6 +328,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
                        str(c.k.sizes()) + " on " + c.dev.str());
     if (q->requires_grad() && c10::GradMode::is_enabled())
       throw ValueError("paged_attention has no backward pass");
+    no_tangent(*q, "q");
     const Tensor &table = a.tensor(5, "block_table", 2);
     const int64_t B = table.size(0), W = table.size(1);
     if (B < 1 || W < 1) throw ValueError("empty block_table");
@@ -404,6 +415,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       p.wait_limit_ns = static_cast<uint64_t>(a.integer(19));
       const int code = g_attn(&p, stream);
       if (code != CHIA_OK) return PyLong_FromLong(code);
+      if (!a.none(17)) written(out);
     }
     PyObject *o = a.none(17) ? THPVariable_Wrap(out) : Py_NewRef(a.v[17]);
     if (!lse.defined()) return o;

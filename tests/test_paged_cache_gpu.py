@@ -233,3 +233,35 @@ def test_attention_after_a_rollback(cuda):
     plain = play([(list(range(n)), n)])
     drafts = play([(list(range(60)), 60), (list(range(80, 109)), 63), (list(range(70, 73)), 60), (list(range(60, n)), n)])
     assert (plain - drafts).norm() / plain.norm() < 0.06  # e4m3: 2.6% rms in K and in V, either way
+
+
+def test_writes_are_known_to_autograd(cuda):
+    """What is written in place has a new version, so that a graph that saved it refuses its backward pass; inference
+    tensors have none. A forward-mode tangent, which would be dropped, is refused."""
+    def play():
+        cache = cp.new_cache(4, 2, 64, page_size=16)
+        x = torch.randn(3, 2, 64, dtype=BF16, device="cuda")
+        table, ring, out = ints([[0, 0]]), ints([2, 1, 0]), torch.zeros_like(x)
+        kept = [*cache, table, ring, out]
+        before = None if x.is_inference() else [t._version for t in kept]
+        step = cp.page_tables(ints([0]), ints([3]), table, ring, ints([0, 3]), page_size=16, max_tokens=3)
+        cp.cache_append(x, x, step.slots, *cache)
+        cp.paged_attention(x, *cache, table, step.seq_lens, step.cu_q, out=out)
+        cp.release_pages(ints([1]), step.seq_lens, table, ring, step.free_state, page_size=16)
+        return kept, before, x
+    kept, before, x = play()
+    assert all(t._version > v for t, v in zip(kept, before))
+    with torch.inference_mode():
+        play()
+    w = torch.ones(4, 2, device="cuda", requires_grad=True)
+    loss = (w * kept[2]).sum()  # saves k_scale
+    cp.cache_append(x, x, ints([5, 6, 7]), *kept[:4])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for k, v in ((dual, x), (x, dual)):
+            with pytest.raises(ValueError, match="tangent"):
+                cp.cache_append(k, v, ints([5, 6, 7]), *kept[:4])
+        with pytest.raises(ValueError, match="tangent"):
+            cp.paged_attention(dual, *kept[:4], kept[4], ints([3]))
