@@ -243,12 +243,22 @@ def binding():
     return m
 
 
+def status_name(code: int) -> str:
+    """Its name; of a status word, where kernels OR their errors, the names of all of them."""
+    if code in STATUS:
+        return STATUS[code]
+    parts = [b for b in (code & 7, code & 8, code & 16) if b]
+    if sum(parts) != code or any(p not in STATUS for p in parts):
+        return f"status {code}"
+    return " | ".join(STATUS[p] for p in parts)
+
+
 class ChiaError(RuntimeError):
     """A non-zero ``chia_status`` returned by the library."""
 
     def __init__(self, code: int, what: str = ""):
         self.code = code
-        name = STATUS.get(code, f"status {code}")
+        name = status_name(code)
         super().__init__(f"{name}{': ' + what if what else ''}")
 
 
