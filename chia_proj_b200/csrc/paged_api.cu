@@ -263,7 +263,8 @@ bool encode_cache(CUtensorMap *map, const void *base, const chia_paged_params_t 
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int32_t clamp30(int64_t v) { return static_cast<int32_t>(v > (1 << 30) ? (1 << 30) : v); }
+// (no position is that large)
+int32_t clamp32(int64_t v) { return static_cast<int32_t>(v > kI32 ? kI32 : v); }
 
 // FN<D, BF16, CT>(...) for the call's types.
 #define CHIA_BY_TYPE(p, FN, ...)                                                          \
@@ -358,11 +359,11 @@ int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
   a.table_stride = p->table_stride;
   a.lse = p->norm == CHIA_NORM_SOFTMAX ? p->lse : nullptr;
   a.head_param = (p->mod == CHIA_MOD_ALIBI || p->mod == CHIA_MOD_TEMP) ? p->head_param : nullptr;
-  a.left = clamp30(p->win_left);
-  a.right = clamp30(p->win_right);
-  a.block = clamp30(p->block);
-  a.prefix = clamp30(p->prefix);
-  a.dil = clamp30(p->dilation);
+  a.left = clamp32(p->win_left);
+  a.right = clamp32(p->win_right);
+  a.block = clamp32(p->block);
+  a.prefix = clamp32(p->prefix);
+  a.dil = clamp32(p->dilation);
   a.score_scale = p->scale;
   a.softcap = p->softcap;
   a.sig_bias = p->sig_bias;

@@ -26,7 +26,7 @@ struct PagedArgs {
   int64_t table_stride;
   float *lse;
   const float *head_param;
-  int32_t left, right, block, prefix, dil;  // the mask, on positions (at most 2^30 each)
+  int32_t left, right, block, prefix, dil;  // the mask, on positions
   float score_scale, softcap, sig_bias, out_scale;
   int32_t heads, heads_kv, group, batch, tokens, page, width;
   uint32_t group_magic;  // ceil(2^32 / group); 0: a group of one
@@ -99,7 +99,7 @@ __device__ __forceinline__ Request request_of(const PagedArgs &a, int b, bool &b
 // of them fetches the less code, and its first pass over the code is most of
 // the time of a small call.
 static __device__ __noinline__ int block_start(int i, int block) {
-  return (i >= 0 ? i / block : -((-i + block - 1) / block)) * block;
+  return (i >= 0 ? i / block : -(-(i + 1) / block + 1)) * block;
 }
 static __device__ __noinline__ bool divides(int d, int x) { return x % d == 0; }
 // x / group for x * group < 2^32
@@ -109,15 +109,16 @@ __device__ __forceinline__ int div_group(const PagedArgs &a, int x) {
 
 // The keys that the query at position i sees beside the prefix, of keys 0 to
 // len - 1; a position may be negative (a request with more queries than keys).
+// Position and width may each be near 2^31, so sums of them are not formed.
 __device__ __forceinline__ void band32(const PagedArgs &a, int i, int len, int &lo, int &hi) {
   lo = 0;
   hi = len - 1;
-  if (a.left >= 0) lo = max(lo, i - a.left);
-  if (a.right >= 0) hi = min(hi, i + a.right);
+  if (a.left >= 0 && a.left < i) lo = i - a.left;
+  if (a.right >= 0 && a.right < hi - i) hi = i + a.right;
   if (a.block > 0) {
-    const int b0 = block_start(i, a.block);
+    const int b0 = block_start(i, a.block), more = a.block - 1;
     lo = max(lo, b0);
-    hi = min(hi, b0 + a.block - 1);
+    if (b0 <= 0x7fffffff - more) hi = min(hi, b0 + more);
   }
 }
 
@@ -128,7 +129,7 @@ __device__ __forceinline__ Tiles tiles_of(const PagedArgs &a, int p0, int p1, in
   band32(a, p0, len, lo, x);
   band32(a, p1, len, x, hi);
   const int pf = min(a.prefix, len);
-  r.pre = (pf + TK - 1) / TK;
+  r.pre = pf / TK + (pf % TK != 0);
   r.lo = r.pre;
   int n = r.pre;
   if (lo <= hi) {

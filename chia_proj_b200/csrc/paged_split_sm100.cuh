@@ -355,8 +355,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       float4 sc = scales[kk % C::SCALES];
       const uint32_t kst = ring + stage * C::STAGE, vst = kst + TK * D;
       const int gone = any_lost ? s_lost[warp][kk % C::SCALES] : 0;  // keys that are not there
-      const bool all = gone == 0 && (a.dil == 1 ? (j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf
-                                                : j0 + TK <= pf);
+      const bool all = gone == 0 && (a.dil == 1 ? (j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 <= pf - TK
+                                                : j0 <= pf - TK);
       if (!all) {  // the scales of 16 keys that nobody sees may be anything
         const bool s0 = j0 < pf || (j0 <= hi_max && j0 + 15 >= lo_min);
         const bool s1 = j0 + 16 < pf || (j0 + 16 <= hi_max && j0 + 31 >= lo_min);

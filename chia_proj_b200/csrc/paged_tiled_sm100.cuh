@@ -120,13 +120,13 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
   for (int t = t0; t < t1; ++t) {
     constexpr int TK = TiledConfig<D>::TK;
     const int j0 = tl.key_tile(t) * TK;
-    bool whole = (a.dil == 1 && j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 + TK <= pf;
-    for (int j = j0; j < j0 + TK && whole; j += 16) {
-      const int pg = a.block_table[b * a.table_stride + j / a.page];
+    bool whole = (a.dil == 1 && j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 <= pf - TK;
+    for (int x = 0; x < TK && whole; x += 16) {
+      const int pg = a.block_table[b * a.table_stride + (j0 + x) / a.page];
       whole = pg >= 0 && pg < a.num_pages;
     }
     if (whole) continue;
-    for (int j = j0; j < min(j0 + TK, len); ++j) {
+    for (int j = j0; j - j0 < TK && j < len; ++j) {
       if (!(j < pf || (j >= lo && j <= hi && (a.dil == 1 || divides(a.dil, i - j))))) continue;
       const int pg = a.block_table[b * a.table_stride + j / a.page];
       if (pg < 0 || pg >= a.num_pages) continue;
@@ -230,7 +230,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   };
   auto sees_all = [&](const Here &h, int j0) {  // every row of the unit sees keys [j0, j0 + TK)
     return (a.dil == 1 && j0 >= h.lo_max && j0 + TK - 1 <= h.hi_min) ||
-           j0 + TK <= min(a.prefix, h.rq.len);
+           j0 <= min(a.prefix, h.rq.len) - TK;
   };
 
   if (warp >= 8) {
