@@ -111,8 +111,6 @@ class AttnGrads(ctypes.Structure):
 
 # ---- the paged 8-bit K/V cache (include/chia_paged.h)
 PAGED_ABI_VERSION = 1
-CACHE_E4M3, CACHE_INT8 = 0, 1
-BAD_INDEX, NO_PAGES = 8, 16
 
 PAGED_SYMBOLS = (
     "chia_page_tables",
