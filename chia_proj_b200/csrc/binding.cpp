@@ -105,6 +105,15 @@ bool fits(const Tensor &t) {
          t.stride(1) >= 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// No two elements of [rows, heads, channels] share memory.
+bool apart(const Tensor &t) {
+  if (t.numel() == 0) return true;
+  const int near = t.stride(0) < t.stride(1) ? 0 : 1;  // the dimension of the smaller stride
+  const int64_t one = t.size(near) > 1 ? t.stride(near) : t.size(2);
+  const int64_t all = (t.size(near) - 1) * one + t.size(2);
+  return one >= t.size(2) && (t.size(1 - near) == 1 || t.stride(1 - near) >= all);
+}
+
 // The kernels write below autograd; this tells it (a tensor that a graph has saved
 // must not change unseen).
 void written(const Tensor &t) {
@@ -355,6 +364,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       if (out.sizes() != q->sizes() || out.scalar_type() != q->scalar_type() || out.device() != c.dev)
         throw ValueError("out must match q in shape, dtype and device");
       if (!fits(out)) throw ValueError("out must have unit last stride and 16-byte aligned rows");
+      if (!apart(out)) throw ValueError("out must not overlap itself");
     }
     if (!a.none(14)) {
       if (!THPVariable_Check(a.v[14])) throw ValueError("head_param must be a tensor");

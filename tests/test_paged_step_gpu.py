@@ -78,3 +78,19 @@ def test_a_graph_of_a_step_while_requests_grow(cuda, ct, window):
     assert again[1].tolist() == [n + steps for n in start]
     for a, b in zip((*eager[0], *eager[1:]), (*again[0], *again[1:])):
         assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+
+
+def test_out_that_overlaps_itself_is_refused(cuda):
+    """Rows that share memory would be written by many CTAs at a time. What does not overlap is taken in any order."""
+    q, k, v, ks, vs, table, cu = setup([70, 33], [2, 1], 4, 2, 64, 16, E4M3, BF16)
+    args = (q, k, v, ks, vs, ints(table), ints([70, 33]), ints(cu))
+    want = cp.paged_attention(*args)
+    buf = torch.zeros(4096, dtype=BF16, device="cuda")
+    for strides in ((0, 64, 1), (256, 0, 1), (64, 64, 1), (248, 64, 1), (64, 128, 1), (256, 56, 1), (0, 0, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            cp.paged_attention(*args, out=buf.as_strided((3, 4, 64), strides))
+    for strides in ((256, 64, 1), (64, 192, 1), (264, 64, 1), (1024, 72, 1), (72, 256, 1)):
+        out = buf.as_strided((3, 4, 64), strides)
+        assert torch.equal(cp.paged_attention(*args, out=out), want)
+    one = buf.as_strided((1, 4, 64), (0, 64, 1))
+    assert torch.equal(cp.paged_attention(q[2:], k, v, ks, vs, ints(table[1:]), ints([33]), out=one), want[2:])
