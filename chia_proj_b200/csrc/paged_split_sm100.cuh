@@ -102,7 +102,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   __shared__ typename L::Shared line_sm;
   __shared__ __align__(8) uint64_t bars[kSplitWarps * NST];
   __shared__ float part_ml[kSplitWarps][ROWS][2];
-  __shared__ uint8_t s_lost[kSplitWarps][C::SCALES];  // beside the scales: see `lost`
+  __shared__ __align__(2) uint8_t s_lost[kSplitWarps][C::SCALES];  // beside the scales: see `lost`
   __shared__ Unit s_head[kSplitWarps], s_end[kSplitWarps];
   __shared__ int s_has_head[kSplitWarps], s_has_end[kSplitWarps];  // end: 1 begun here, 2 before
   __shared__ volatile int abort_flag;
@@ -123,6 +123,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   float4 *scales = reinterpret_cast<float4 *>(sm + C::RING) + warp * C::SCALES;  // ks and the
                                                              // value factor of keys 0-15, 16-31
   if (t < kSplitWarps * NST) ptx::mbar_init(ptx::smem_u32(bars) + 8 * t, 1);
+  static_assert(kSplitWarps * C::SCALES == 2 * kSplitThreads, "two a thread");
+  reinterpret_cast<uint16_t *>(s_lost)[t] = 0;
   if (t == 0) {
     abort_flag = 0;
     ptx::tma_prefetch_desc(&mk);
@@ -161,7 +163,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   const int pshift = 31 - __clz(a.page);
   int row0 = -1, row1 = -1, tok = 0;
   int lost = 0;           // bits: keys 0-15, 16-31 have a page out of range: nothing is loaded, no row sees them
-  bool any_lost = false;  // so far
+  bool any_lost = false;  // so far: from then on no tile counts as one that all rows see
   int next_pg0 = -1, next_pg1 = -1, next_hk = 0, next_tok = 0;  // pages
   int wanted = 0;                                                // bits: that there are such keys
   float next_ks0 = 0.f, next_vs0 = 0.f, next_ks1 = 0.f, next_vs1 = 0.f;
@@ -191,6 +193,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     lost = row0 < 0 && (wanted & 1) ? (a.page == 16 ? 1 : 3) : 0;
     if (row1 < 0 && (wanted & 2)) lost |= 2;
   };
+  // all rows of the unit see keys [lo_max, hi_min] and tiles that begin up to pf_all
+  int lo_max = 0, hi_min = 0, pf_all = 0;
   auto take_scales = [&](int k) {  // to shared memory
     float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row0 >= 0) sc.x = next_ks0, sc.y = value_factor<SOFTMAX>(next_vs0);
@@ -199,8 +203,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     else if (row1 >= 0)
       sc.z = next_ks1, sc.w = value_factor<SOFTMAX>(next_vs1);
     scales[(k + lane) % C::SCALES] = sc;  // (those of 64 tiles ago are long used)
-    s_lost[warp][(k + lane) % C::SCALES] = static_cast<uint8_t>(lost);
-    any_lost |= __any_sync(0xffffffffu, lost != 0);
+    if (__any_sync(0xffffffffu, lost != 0)) any_lost = true, hi_min = pf_all = -1;
+    if (any_lost) s_lost[warp][(k + lane) % C::SCALES] = static_cast<uint8_t>(lost);
     __syncwarp();
   };
   auto issue = [&](int k) {  // start the copies of tile k, whose stage is free
@@ -278,11 +282,12 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 
   bool aborted = false, has_end = false;
   for (int k = 0; k < nk;) {
-    // all rows of the unit see keys [lo_max, hi_min]; none sees one outside [lo_min, hi_max]
-    int lo_min, lo_max, hi_min, hi_max;
+    int lo_min, hi_max;  // no row sees a key outside of them and the prefix
     band32(a, p0 + div_group(a, un.row0), len, lo_min, hi_min);
     band32(a, p0 + div_group(a, un.row0 + un.rows - 1), len, lo_max, hi_max);
     const int pf = min(a.prefix, len);
+    pf_all = pf - TK;
+    if (any_lost) hi_min = pf_all = -1;
 
     // Q as fragments: channels 16 (H tig + h) + 4 s .. + 3 of step (h, s)
     uint32_t qf[NT][H * 4][2];
@@ -354,15 +359,16 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       const int j0 = tl.key_tile(ut0 + i) * TK;
       float4 sc = scales[kk % C::SCALES];
       const uint32_t kst = ring + stage * C::STAGE, vst = kst + TK * D;
-      const int gone = any_lost ? s_lost[warp][kk % C::SCALES] : 0;  // keys that are not there
-      const bool all = gone == 0 && (a.dil == 1 ? (j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 <= pf - TK
-                                                : j0 <= pf - TK);
+      const bool all =
+          a.dil == 1 ? (j0 >= lo_max && j0 + TK - 1 <= hi_min) || j0 <= pf_all : j0 <= pf_all;
+      int gone = 0;  // keys that are not there
       if (!all) {  // the scales of 16 keys that nobody sees may be anything
         const bool s0 = j0 < pf || (j0 <= hi_max && j0 + 15 >= lo_min);
         const bool s1 = j0 + 16 < pf || (j0 + 16 <= hi_max && j0 + 31 >= lo_min);
         if (!s0) sc.x = sc.y = 0.f;
         if (!s1) sc.z = sc.w = 0.f;
         // (so may their page, a window's left behind for one)
+        if (any_lost) gone = s_lost[warp][kk % C::SCALES];
         if (lane == 0 && ((s0 && (gone & 1)) || (s1 && (gone & 2)))) report(a.status, kStatusBadIndex);
       }
       // ---------------- S^T = K Q^T
