@@ -61,7 +61,7 @@ __device__ __forceinline__ Scan2 block_scan2(Scan2 v, Scan2 &tot, Scan2 *warp_su
 // time (a few KB from L2), and then fills its share of each chunk's tokens:
 // one launch, and no CTA waits for another. The token at a page's first slot
 // enters the page in the block table. A few KB, so the time is latency: 64 decode
-// steps 3.6 us, 512 prompts of up to 300 tokens 4.2 us, on the device.
+// steps 3.6 us, 512 prompts of up to 300 tokens 4.0 us, on the device.
 __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const TablesArgs a) {
   __shared__ Scan2 sums[32];
   __shared__ int32_t s_cu[kTablesThreads + 1], s_len[kTablesThreads], s_first[kTablesThreads];
@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(kTablesThreads) page_tables_kernel(const Table
 }
 
 // Pages of finished requests (TRIM: those past the tokens that a request keeps) to the
-// ring's tail: the same sums, the pages of a chunk in the place of its tokens.
+// ring's tail: the same sums, the pages of a chunk in the place of its tokens. 64
+// requests 3.5 us, 2048 of up to 128 pages 6.8, on the device.
 template <bool TRIM>
 __global__ void __launch_bounds__(kTablesThreads) release_pages_kernel(const TablesArgs a) {
   __shared__ Scan2 sums[32];

@@ -122,8 +122,8 @@ int check_append(const chia_append_params_t *p) {
 }
 
 // Tokens that a CTA of the append looks at: a page's, or as many fewer as give
-// every SM eight CTAs. 16 prompts of some 4,100 tokens: 42 us by pages, 590 by single
-// tokens (every CTA then reads its neighbours' slots); 64 single tokens: 62 and 3.7.
+// every SM eight CTAs. 16 prompts of some 4,100 tokens: 43 us by pages, 590 by single
+// tokens (every CTA then reads its neighbours' slots); 64 single tokens: 62 and 3.9.
 template <int D, bool BF16, int CT>
 int launch_append(const chia::AppendArgs &a, int sms, cudaStream_t s) {
   const int64_t kinds = 2ll * a.heads_kv;

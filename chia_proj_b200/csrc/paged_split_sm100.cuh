@@ -33,9 +33,9 @@
 // left through a second product.
 //
 // Measured (D 128, e4m3, bf16 unless said): 64 requests x 32,768 keys, 64 query
-// and 8 K/V heads 662 us, 6.5 TB/s, the copy rate; 96 x up to 16,384, pages of
-// 16, 64 us, 5.0 TB/s; 8 x 8192, 4 K/V heads, capped, 23.4 us, 2.9 TB/s; one of
-// 601 keys 9.8 us. What is beside HBM there is a chain of some 6 us before the
+// and 8 K/V heads 640 to 705 us from GPU to GPU, 6.7 to 6.1 TB/s (a plain copy
+// has 6.5, reading alone 6.9); 96 x up to 16,384, pages of 16, 65 us, 4.9 TB/s;
+// 8 x 8192, 4 K/V heads, capped, 23.5 us, 2.9 TB/s; one of 601 keys 10.0 us. What is beside HBM there is a chain of some 6 us before the
 // first tile (lengths, the line, page, scales; half of it the fetch of the code,
 // run once a call) and 2 us of joining parts.
 #pragma once
@@ -53,7 +53,8 @@ constexpr float kPTop = 15.f;
 // 75, 68, 67, 69 us, on 48 with a window of 1024 keys 17.0, 18.0, 17.8, 18.6.
 constexpr int kUnitCost = 4;
 // Units of up to this cost are not cut between CTAs: 0, 64, 160 on one request of 601 keys 12.8,
-// 10.1, 10.1 us, on 24 with five queries each over up to 4,100 keys 22.4, 22.6, 39.
+// 10.1, 10.1 us, on 24 with five queries each over up to 4,100 keys 22.4, 22.6, 39. It does
+// not ask for a CTA's share: of those 24 the fullest CTA has 50 tiles where the mean is 17.
 constexpr int kWholeUnit = 64;
 
 // D (16x8, fp32) += A (16x16, halves) * B (16x8). Not volatile: the compiler may

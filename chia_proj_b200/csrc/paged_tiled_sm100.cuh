@@ -26,10 +26,11 @@
 // waited some 2000 of 5200 cycles for PV and the next S.)
 //
 // Measured (D 128, e4m3, bf16, 32 query and 8 K/V heads): 4 requests x 1024
-// queries over 8192 keys 600 us, 0.86 PFLOP/s, 52% of the rate of a plain matrix
-// product; up to that many each, ragged, 262 us, 39%. Bound by the softmax warps: of a tile's 2,550 cycles the UMMAs take 1,024; 500 go to scores and
+// queries over 8192 keys 602 us, 0.86 PFLOP/s, 52% of the rate of a plain matrix
+// product; up to that many each, ragged, 265 us, 39% (the fullest CTA has 185 tiles where the mean is 150).
+// Bound by the softmax warps: of a tile's 2,550 cycles the UMMAs take 1,024; 500 go to scores and
 // maximum, 1,150 to exponentials, sums and packing (64 a thread, two warps a
-// scheduler: issue and latency), 700 to barriers and tensor memory. fp16: 696 us.
+// scheduler: issue and latency), 700 to barriers and tensor memory. fp16: 700 us.
 // Tried: two threads a row on 16 warps 282 us ragged where this had 273; the two
 // query tiles' exponentials in turns 290.
 //

@@ -147,8 +147,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``scale``, ``softcap``, ``head_param``, ``sig_bias``, ``out_scale``,
     ``wait_limit_ns`` as in ``attention``; ``H % H_kv == 0``. ``max_q``: the
     most queries of any request, as far as the host knows (``None``: ``T -
-    B + 1``, or ``T / B`` without ``cu_q``); it chooses the schedule, never the result. A
-    row that sees no key is zero. ``return_lse``: also the natural log-sum-exp,
+    B + 1``, or ``T / B`` without ``cu_q``); it chooses the schedule, never the result.
+    Keys whose page is out of range are left out and reported, and so are requests
+    from an offset on that falls. A row that sees no key is zero. ``return_lse``: also the natural log-sum-exp,
     fp32 ``[T, H]`` (softmax only). Forward only.
     """
     if norm not in _NORMS or mod not in _MODS:

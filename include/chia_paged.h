@@ -13,7 +13,7 @@
  *                      chia_attn.h (score modification, mask, normaliser)
  *
  * The cache. k_cache and v_cache are [num_pages, heads_kv, page_size, head_dim]
- * bytes (e4m3 or int8), contiguous; k_scale and v_scale are fp32
+ * bytes (e4m3 or int8), contiguous; k_scale and v_scale are fp32, not negative,
  * [num_pages, heads_kv]. A stored value q stands for q * scale. chia_cache_append
  * writes scales that are powers of two: the smallest 2^e, e >= -64, with
  * max|x| <= 448 * 2^e (e4m3) or 127 * 2^e (int8), the maximum taken over the
