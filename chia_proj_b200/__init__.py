@@ -40,5 +40,17 @@ from .paged import (  # noqa: F401
     paged_attention,
     release_pages,
 )
+from .draft import (  # noqa: F401
+    TreeStep,
+    Verified,
+    cache_compact,
+    tree_tables,
+    verify_drafts,
+)
+from .rope import (  # noqa: F401
+    qk_norm_rope,
+    qk_norm_rope_backward,
+    rope_frequencies,
+)
 from ._native import ChiaError  # noqa: F401
 from . import flex  # noqa: F401,E402

@@ -1,5 +1,5 @@
-"""ctypes binding of ``libchia_attn.so`` (declared in ``include/chia_attn.h``
-and ``include/chia_paged.h``).
+"""ctypes binding of ``libchia_attn.so`` (declared in ``include/chia_attn.h``,
+``chia_paged.h``, ``chia_draft.h`` and ``chia_rope.h``).
 
 The library is built in-tree by ``chia_proj_b200.build`` and loaded from
 ``chia_proj_b200/_lib/``. There is no fallback: if the library is missing or
@@ -122,6 +122,24 @@ PAGED_SYMBOLS = (
 )
 
 
+# ---- trees of drafted tokens (include/chia_draft.h), norm and rotation (include/chia_rope.h)
+DRAFT_ABI_VERSION = 1
+ROPE_ABI_VERSION = 1
+TREE_NODES = 64
+
+DRAFT_SYMBOLS = (
+    "chia_tree_tables",
+    "chia_tree_attn",
+    "chia_verify_drafts",
+    "chia_cache_compact",
+)
+ROPE_SYMBOLS = (
+    "chia_qk_norm_rope",
+    "chia_qk_norm_rope_bwd",
+    "chia_qk_norm_rope_bwd_workspace_bytes",
+)
+
+
 class TablesParams(ctypes.Structure):
     """Mirror of ``chia_tables_params_t`` (include/chia_paged.h)."""
 
@@ -220,11 +238,129 @@ class PagedParams(ctypes.Structure):
     ]
 
 
+class TreeParams(ctypes.Structure):
+    """Mirror of ``chia_tree_params_t`` (include/chia_draft.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("pad", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("parents", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("ancestors", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class VerifyParams(ctypes.Structure):
+    """Mirror of ``chia_verify_params_t`` (include/chia_draft.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("max_tokens", ctypes.c_int64),
+        ("target_probs", ctypes.c_void_p),
+        ("draft_probs", ctypes.c_void_p),
+        ("target_stride", ctypes.c_int64),
+        ("draft_stride", ctypes.c_int64),
+        ("node_tokens", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p),
+        ("uniforms", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("out_tokens", ctypes.c_void_p),
+        ("path", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class CompactParams(ctypes.Structure):
+    """Mirror of ``chia_compact_params_t`` (include/chia_draft.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("pad", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("max_tokens", ctypes.c_int64),
+        ("num_pages", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("path", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("keep_lens", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class RopeParams(ctypes.Structure):
+    """Mirror of ``chia_rope_params_t`` (include/chia_rope.h)."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("heads_kv", ctypes.c_int32),
+        ("rot", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("seqlen", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("q_out_stride", ctypes.c_int64 * 3),
+        ("k_out_stride", ctypes.c_int64 * 3),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("freqs", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("weight_offset", ctypes.c_float),
+    ]
+
+
+class RopeGrads(ctypes.Structure):
+    """Mirror of ``chia_rope_grads_t`` (include/chia_rope.h)."""
+
+    _fields_ = [
+        ("dq_out", ctypes.c_void_p),
+        ("dk_out", ctypes.c_void_p),
+        ("dq_out_stride", ctypes.c_int64 * 3),
+        ("dk_out_stride", ctypes.c_int64 * 3),
+        ("dq", ctypes.c_void_p),
+        ("dk", ctypes.c_void_p),
+        ("dq_weight", ctypes.c_void_p),
+        ("dk_weight", ctypes.c_void_p),
+    ]
+
+
 _binding_module = None
 
 
 def binding():
-    """The compiled argument checks of ``paged.py`` (``csrc/binding.cpp``),
+    """The compiled argument checks of ``paged.py``, ``draft.py`` and ``rope.py`` (``csrc/binding.cpp``),
     given the entry points of the library. Raises if it has not been built."""
     global _binding_module
     if _binding_module is not None:
@@ -236,7 +372,7 @@ def binding():
     loader = importlib.machinery.ExtensionFileLoader("_binding", path)
     m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
     loader.exec_module(m)
-    m.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in PAGED_SYMBOLS))
+    m.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in PAGED_SYMBOLS + DRAFT_SYMBOLS + ROPE_SYMBOLS))
     _binding_module = m
     return m
 
@@ -306,6 +442,16 @@ def load() -> ctypes.CDLL:
                 getattr(lib, name).restype = ctypes.c_int
             lib.chia_paged_attn_workspace_bytes.argtypes = [ctypes.c_char_p]
             lib.chia_paged_attn_workspace_bytes.restype = ctypes.c_int64
+            for name in ("chia_tree_tables", "chia_verify_drafts", "chia_cache_compact", "chia_qk_norm_rope"):
+                getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+                getattr(lib, name).restype = ctypes.c_int
+            lib.chia_tree_attn.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+            lib.chia_tree_attn.restype = ctypes.c_int
+            lib.chia_qk_norm_rope_bwd.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p,
+                                                  ctypes.c_int64, ctypes.c_void_p]
+            lib.chia_qk_norm_rope_bwd.restype = ctypes.c_int
+            lib.chia_qk_norm_rope_bwd_workspace_bytes.argtypes = [ctypes.c_char_p]
+            lib.chia_qk_norm_rope_bwd_workspace_bytes.restype = ctypes.c_int64
             if lib.chia_attn_abi_version() != ABI_VERSION:
                 raise ImportError(f"{LIB_PATH}: ABI version mismatch")
             _lib = lib

@@ -3,7 +3,7 @@
     python -m chia_proj_b200.build [--force] [--verbose]
 
 The library is a plain shared object with C linkage (``include/chia_attn.h``,
-``include/chia_paged.h``);
+``chia_paged.h``, ``chia_draft.h``, ``chia_rope.h``);
 it links the CUDA runtime statically and fetches ``cuTensorMapEncodeTiled``
 from the driver at run time, so it needs no libcuda at link time. Beside it
 stands a small CPython module (``csrc/binding.cpp``) that checks the tensors of

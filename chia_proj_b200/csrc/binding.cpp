@@ -1,183 +1,22 @@
 // binding.cpp -- the Python side of include/chia_paged.h: argument checks, output
-// tensors and workspaces of the paged 8-bit K/V cache's operators.
+// tensors and workspaces of the paged 8-bit K/V cache's operators. (Those of drafted
+// tokens, and of the norm and rotation of queries and keys, are in binding_draft.h.)
 //
 // A decode step calls these once a layer, and on an idle GPU a call is a dozen
 // microseconds, so the checks are made here, on the tensors themselves: the
 // same checks in Python took 9 to 15 us a call. The functions take positional
 // arguments only; the public signatures and their documentation are in
-// chia_proj_b200/paged.py, the computation in libchia_attn.so, whose entry
+// chia_proj_b200/paged.py, draft.py and rope.py, the computation in libchia_attn.so, whose entry
 // points bind() is given. A status other than CHIA_OK is returned as an int.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <ATen/core/LegacyTypeDispatch.h>
-#include <c10/core/GradMode.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <cmath>
-#include <cstring>
-#include <map>
-#include <stdexcept>
-#include <string>
-#include <utility>
-
-#include "../../include/chia_paged.h"
+#include "binding_args.h"
+#include "binding_draft.h"
 
 namespace {
-
-using at::Tensor;
 
 decltype(&chia_page_tables) g_tables, g_release, g_trim;
 decltype(&chia_cache_append) g_append;
 decltype(&chia_paged_attn) g_attn;
 decltype(&chia_paged_attn_workspace_bytes) g_bytes;
-
-struct ValueError : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
-
-std::string str(at::IntArrayRef s) {
-  std::string r = "(";
-  for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
-  return r + ")";
-}
-
-// ------------------------------------------------------------------ arguments
-struct Args {
-  PyObject *const *v;
-  Py_ssize_t n;
-  Args(PyObject *const *args, Py_ssize_t nargs, Py_ssize_t want) : v(args), n(nargs) {
-    if (nargs != want) throw ValueError("wrong number of arguments");
-  }
-  int64_t integer(int i) const {
-    const long long x = PyLong_AsLongLong(v[i]);
-    if (x == -1 && PyErr_Occurred()) throw 0;
-    return x;
-  }
-  double number(int i) const {
-    const double x = PyFloat_AsDouble(v[i]);
-    if (x == -1.0 && PyErr_Occurred()) throw 0;
-    return x;
-  }
-  bool none(int i) const { return v[i] == Py_None; }
-  // A tensor of `dim` dimensions on a GPU.
-  const Tensor &tensor(int i, const char *name, int64_t dim) const {
-    if (!THPVariable_Check(v[i])) throw ValueError(std::string(name) + " must be a " + std::to_string(dim) + "-D tensor");
-    const Tensor &t = THPVariable_Unpack(v[i]);
-    if (t.dim() != dim) throw ValueError(std::string(name) + " must be a " + std::to_string(dim) + "-D tensor");
-    if (!t.is_cuda())
-      throw std::runtime_error(std::string(name) + " is on " + t.device().str() +
-                               ": the library runs on CUDA only (no CPU fallback)");
-    return t;
-  }
-  // int32 of this shape and device, unit stride in the last dimension.
-  const Tensor &ints(int i, const char *name, at::IntArrayRef shape, const at::Device &dev) const {
-    const Tensor &t = tensor(i, name, static_cast<int64_t>(shape.size()));
-    if (t.scalar_type() != at::kInt || t.sizes() != shape || t.device() != dev)
-      throw ValueError(std::string(name) + " must be int32 " + str(shape) + " on " + dev.str() + ", got " +
-                       c10::toString(t.scalar_type()) + " " + str(t.sizes()) + " on " + t.device().str());
-    if (t.size(-1) > 1 && t.stride(-1) != 1) throw ValueError(std::string(name) + " must have unit stride");
-    return t;
-  }
-};
-
-template <class T>
-T *ptr(const Tensor &t) {
-  return static_cast<T *>(t.data_ptr());
-}
-
-bool page_ok(int64_t p) { return p == 16 || p == 32 || p == 64 || p == 128; }
-void check_page(int64_t p) {
-  if (!page_ok(p)) throw ValueError("page_size " + std::to_string(p) + " unsupported (16, 32, 64 or 128)");
-}
-
-int value_type(const Tensor &t) {
-  return t.scalar_type() == at::kBFloat16 ? CHIA_DTYPE_BF16 : t.scalar_type() == at::kHalf ? CHIA_DTYPE_F16 : -1;
-}
-
-// Unit stride on the channels, 16-byte aligned rows; a copy where it is not so.
-bool fits(const Tensor &t) {
-  return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) >= 0 &&
-         t.stride(1) >= 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-}
-
-// No two elements of [rows, heads, channels] share memory.
-bool apart(const Tensor &t) {
-  if (t.numel() == 0) return true;
-  const int near = t.stride(0) < t.stride(1) ? 0 : 1;  // the dimension of the smaller stride
-  const int64_t one = t.size(near) > 1 ? t.stride(near) : t.size(2);
-  const int64_t all = (t.size(near) - 1) * one + t.size(2);
-  return one >= t.size(2) && (t.size(1 - near) == 1 || t.stride(1 - near) >= all);
-}
-
-// The kernels write below autograd; this tells it (a tensor that a graph has saved
-// must not change unseen).
-void written(const Tensor &t) {
-  if (!t.unsafeGetTensorImpl()->is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-void no_tangent(const Tensor &t, const char *name) {
-  if (t._fw_grad(0).defined())
-    throw ValueError(std::string(name) + " has a forward-mode tangent: there is no derivative");
-}
-
-struct Cache {
-  const Tensor &k, &v, &ks, &vs;
-  int type;
-  at::Device dev;
-  int64_t pages, heads, page, dim;
-  Cache(const Args &a, int i)
-      : k(a.tensor(i, "k_cache", 4)), v(a.tensor(i + 1, "v_cache", 4)), ks(a.tensor(i + 2, "k_scale", 2)),
-        vs(a.tensor(i + 3, "v_scale", 2)), dev(k.device()) {
-    const auto ty = k.scalar_type();
-    type = ty == at::kFloat8_e4m3fn ? CHIA_CACHE_E4M3 : ty == at::kChar ? CHIA_CACHE_INT8 : -1;
-    if (type < 0 || v.scalar_type() != ty)
-      throw ValueError(std::string("k_cache, v_cache must share a type, float8_e4m3fn or int8; got ") +
-                       c10::toString(ty) + ", " + c10::toString(v.scalar_type()));
-    if (v.sizes() != k.sizes() || v.device() != dev)
-      throw ValueError("k_cache, v_cache must match in shape and device");
-    if (!k.is_contiguous() || !v.is_contiguous()) throw ValueError("k_cache, v_cache must be contiguous");
-    pages = k.size(0), heads = k.size(1), page = k.size(2), dim = k.size(3);
-    check_page(page);
-    if (dim != 64 && dim != 128) throw ValueError("head_dim " + std::to_string(dim) + " unsupported (64 or 128)");
-    if (pages < 1 || heads < 1) throw ValueError("empty cache");
-    for (const Tensor *s : {&ks, &vs})
-      if (s->scalar_type() != at::kFloat || s->size(0) != pages || s->size(1) != heads || s->device() != dev ||
-          !s->is_contiguous())
-        throw ValueError(std::string(s == &ks ? "k_scale" : "v_scale") + " must be contiguous fp32 (" +
-                         std::to_string(pages) + ", " + std::to_string(heads) + ") on " + dev.str());
-  }
-};
-
-// Any C++ exception ends here as a Python one.
-template <class F>
-PyObject *guarded(F f) {
-  try {
-    return f();
-  } catch (int) {
-    return nullptr;  // the Python error is set
-  } catch (const ValueError &e) {
-    PyErr_SetString(PyExc_ValueError, e.what());
-  } catch (const c10::Error &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-  }
-  return nullptr;
-}
-
-// Elements [at, at + n) of a 1-D tensor, sharing its storage (narrow() takes ten
-// times as long to set up).
-Tensor piece(const Tensor &buf, int64_t at, int64_t n) {
-  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()),
-                                                      buf.key_set(), buf.dtype());
-  t.unsafeGetTensorImpl()->set_storage_offset(at);
-  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
-  return t;
-}
 
 // --------------------------------------------------------------------- tables
 // seq_lens, lens, block_table, free_pages, free_state, page_size, max_tokens (-1: release, -2: trim), status
@@ -322,11 +161,12 @@ Tensor workspace(const at::Device &dev, void *stream) {
 }
 
 // q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_q, max_q (0: not known), norm, mod, mask (tuple
-// of 5), scale (None: 1 / sqrt(D)), softcap, head_param, sig_bias, out_scale, out, return_lse, wait_limit_ns, status
+// of 5), scale (None: 1 / sqrt(D)), softcap, head_param, sig_bias, out_scale, out, return_lse, wait_limit_ns, status,
+// tree (None, or a tuple: positions, ancestors)
 PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
     const at::AutoDispatchBelowADInplaceOrView plain;
-    const Args a(args, nargs, 21);
+    const Args a(args, nargs, 22);
     const Cache c(a, 1);
     const Tensor *q = &a.tensor(0, "q", 3);
     const int64_t T = q->size(0), H = q->size(1), D = q->size(2);
@@ -349,6 +189,18 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       cu = &a.ints(7, "cu_q", {B + 1}, c.dev);
     else if (T % B != 0)
       throw ValueError(std::to_string(T) + " queries for " + std::to_string(B) + " requests need cu_q");
+    const int32_t *tree_pos = nullptr;
+    const uint64_t *tree_word = nullptr;
+    if (!a.none(21)) {
+      if (!PyTuple_Check(a.v[21]) || PyTuple_GET_SIZE(a.v[21]) != 2)
+        throw ValueError("tree must be what tree_tables returns");
+      const Args tree(&PyTuple_GET_ITEM(a.v[21], 0), 2, 2);
+      tree_pos = ptr<int32_t>(tree.ints(0, "tree.positions", {T}, c.dev));
+      const Tensor &w = tree.tensor(1, "tree.ancestors", 1);
+      if (w.scalar_type() != at::kLong || w.size(0) != T || w.device() != c.dev || !w.is_contiguous())
+        throw ValueError("tree.ancestors must be contiguous int64 (" + std::to_string(T) + ",) on " + c.dev.str());
+      tree_word = ptr<uint64_t>(w);
+    }
     int64_t max_q = a.none(8) ? (cu == nullptr ? T / B : T - B + 1) : a.integer(8);
     if (!a.none(8) && max_q < 1) throw ValueError("max_q must be >= 1");
     max_q = std::max<int64_t>(1, std::min(max_q, T));
@@ -423,7 +275,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
       p.workspace = ws.data_ptr();
       p.workspace_bytes = ws.numel();
       p.wait_limit_ns = static_cast<uint64_t>(a.integer(19));
-      const int code = g_attn(&p, stream);
+      const int code = tree_pos != nullptr ? g_tree_attn(&p, tree_pos, tree_word, stream) : g_attn(&p, stream);
       if (code != CHIA_OK) return PyLong_FromLong(code);
       if (!a.none(17)) written(out);
     }
@@ -436,11 +288,13 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 // Addresses of libchia_attn.so's entry points, in the order below.
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
-    const Args a(args, nargs, 6);
+    const Args a(args, nargs, 13);
     auto set = [&](auto &f, int i) {
       f = reinterpret_cast<std::decay_t<decltype(f)>>(static_cast<uintptr_t>(a.integer(i)));
     };
     set(g_tables, 0), set(g_release, 1), set(g_append, 2), set(g_attn, 3), set(g_bytes, 4), set(g_trim, 5);
+    set(g_tree_tables, 6), set(g_tree_attn, 7), set(g_verify, 8), set(g_compact, 9);
+    set(g_rope, 10), set(g_rope_bwd, 11), set(g_rope_bytes, 12);
     Py_RETURN_NONE;
   });
 }
@@ -452,6 +306,11 @@ PyMethodDef kMethods[] = {{"bind", fast(bind), METH_FASTCALL, nullptr},
                           {"tables", fast(tables), METH_FASTCALL, nullptr},
                           {"append", fast(append), METH_FASTCALL, nullptr},
                           {"attention", fast(attention), METH_FASTCALL, nullptr},
+                          {"tree_tables", fast(tree_tables), METH_FASTCALL, nullptr},
+                          {"verify", fast(verify), METH_FASTCALL, nullptr},
+                          {"compact", fast(compact), METH_FASTCALL, nullptr},
+                          {"qk_norm_rope", fast(qk_norm_rope), METH_FASTCALL, nullptr},
+                          {"qk_norm_rope_bwd", fast(qk_norm_rope_bwd), METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods};
 

@@ -1,0 +1,334 @@
+// binding_draft.h -- the Python side of include/chia_draft.h and chia_rope.h.
+#pragma once
+#include "binding_args.h"
+
+namespace {
+
+decltype(&chia_tree_tables) g_tree_tables;
+decltype(&chia_tree_attn) g_tree_attn;
+decltype(&chia_verify_drafts) g_verify;
+decltype(&chia_cache_compact) g_compact;
+decltype(&chia_qk_norm_rope) g_rope;
+decltype(&chia_qk_norm_rope_bwd) g_rope_bwd;
+decltype(&chia_qk_norm_rope_bwd_workspace_bytes) g_rope_bytes;
+
+int any_type(const Tensor &t) { return t.scalar_type() == at::kFloat ? CHIA_DTYPE_F32 : value_type(t); }
+
+// The offsets of requests: int32 [B + 1], B > 0.
+const Tensor &offsets(const Args &a, int i, const at::Device &dev) {
+  const Tensor &cu = a.tensor(i, "cu_q", 1);
+  if (cu.size(0) < 2) throw ValueError("cu_q must have an entry more than there are requests, two at least");
+  return a.ints(i, "cu_q", {cu.size(0)}, dev);
+}
+
+// ---------------------------------------------------------------------- tables
+// parents, cu_q, seq_lens, status
+PyObject *tree_tables(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    const Args a(args, nargs, 4);
+    const Tensor &parents = a.tensor(0, "parents", 1);
+    const at::Device dev = parents.device();
+    const int64_t T = parents.size(0);
+    a.ints(0, "parents", {T}, dev);
+    const Tensor &cu = offsets(a, 1, dev), &lens = a.ints(2, "seq_lens", {cu.size(0) - 1}, dev);
+    const c10::cuda::CUDAGuard guard(dev);
+    Tensor words = at::empty({T}, parents.options().dtype(at::kLong)), positions = at::empty({T}, parents.options());
+    chia_tree_params_t p{};
+    p.abi_version = CHIA_DRAFT_ABI_VERSION;
+    p.batch = cu.size(0) - 1;
+    p.tokens = T;
+    p.parents = ptr<int32_t>(parents);
+    p.cu_q = ptr<int32_t>(cu);
+    p.seq_lens = ptr<int32_t>(lens);
+    p.positions = ptr<int32_t>(positions);
+    p.ancestors = ptr<uint64_t>(words);
+    p.status = reinterpret_cast<int32_t *>(a.integer(3));
+    const int code = g_tree_tables(&p, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    if (code != CHIA_OK) return PyLong_FromLong(code);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(positions), THPVariable_Wrap(words));
+  });
+}
+
+// ---------------------------------------------------------------- verification
+// target_probs, tokens, parents, cu_q, uniforms, draft_probs, max_tokens, status
+PyObject *verify(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    const Args a(args, nargs, 8);
+    const Tensor &probs = a.tensor(0, "target_probs", 2);
+    const at::Device dev = probs.device();
+    const int64_t T = probs.size(0), V = probs.size(1), most = a.integer(6);
+    const int dt = any_type(probs);
+    if (dt < 0) throw ValueError(std::string("dtype ") + c10::toString(probs.scalar_type()) + " unsupported (fp32, bf16 or fp16)");
+    if (V < 1) throw ValueError("target_probs of an empty vocabulary");
+    if (most < 1) throw ValueError("max_tokens must be >= 1");
+    const Tensor &tokens = a.ints(1, "tokens", {T}, dev), &parents = a.ints(2, "parents", {T}, dev);
+    const Tensor &cu = offsets(a, 3, dev);
+    const Tensor &u = a.tensor(4, "uniforms", 1);
+    if (u.scalar_type() != at::kFloat || u.size(0) != T || u.device() != dev || !u.is_contiguous())
+      throw ValueError("uniforms must be contiguous fp32 (" + std::to_string(T) + ",) on " + dev.str());
+    auto rows = [&](const Tensor &t) {  // rows that do not overlap, or that are all one
+      return t.stride(1) == 1 || V == 1 ? t.stride(0) >= V || T == 1 : false;
+    };
+    Tensor p2 = rows(probs) ? probs : probs.contiguous(), q2;
+    no_tangent(probs, "target_probs");
+    if (!a.none(5)) {
+      const Tensor &q = a.tensor(5, "draft_probs", 2);
+      if (q.sizes() != probs.sizes() || q.scalar_type() != probs.scalar_type() || q.device() != dev)
+        throw ValueError("draft_probs must match target_probs in shape, dtype and device");
+      no_tangent(q, "draft_probs");
+      q2 = rows(q) ? q : q.contiguous();
+    }
+    const c10::cuda::CUDAGuard guard(dev);
+    const int64_t B = cu.size(0) - 1;
+    // one allocation for all outputs
+    Tensor buf = at::empty({B + 2 * B * most}, cu.options());
+    int32_t *o = ptr<int32_t>(buf);
+    chia_verify_params_t p{};
+    p.abi_version = CHIA_DRAFT_ABI_VERSION;
+    p.dtype = dt;
+    p.batch = B;
+    p.tokens = T;
+    p.vocab = V;
+    p.max_tokens = most;
+    p.target_probs = p2.data_ptr();
+    p.target_stride = T > 1 ? p2.stride(0) : V;
+    if (q2.defined()) {
+      p.draft_probs = q2.data_ptr();
+      p.draft_stride = T > 1 ? q2.stride(0) : V;
+    }
+    p.node_tokens = ptr<int32_t>(tokens);
+    p.parents = ptr<int32_t>(parents);
+    p.cu_q = ptr<int32_t>(cu);
+    p.uniforms = ptr<float>(u);
+    p.counts = o;
+    p.out_tokens = o + B;
+    p.path = o + B + B * most;
+    p.status = reinterpret_cast<int32_t *>(a.integer(7));
+    const int code = g_verify(&p, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+    if (code != CHIA_OK) return PyLong_FromLong(code);
+    auto table = [&](int64_t at) {
+      Tensor t = piece(buf, at, B * most);
+      t.unsafeGetTensorImpl()->set_sizes_contiguous({B, most});
+      return THPVariable_Wrap(t);
+    };
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(piece(buf, 0, B)), table(B), table(B + B * most));
+  });
+}
+
+// ------------------------------------------------------------------ compaction
+// path, counts, cu_q, seq_lens, block_table, k_cache, v_cache, k_scale, v_scale, status
+PyObject *compact(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    const Args a(args, nargs, 10);
+    const Cache c(a, 5);
+    const Tensor &path = a.tensor(0, "path", 2), &table = a.tensor(4, "block_table", 2);
+    const int64_t B = table.size(0), W = table.size(1), most = path.size(1);
+    if (B < 1 || W < 1 || most < 1) throw ValueError("empty path or block_table");
+    a.ints(0, "path", {B, most}, c.dev);
+    if (!path.is_contiguous()) throw ValueError("path must be contiguous");
+    a.ints(4, "block_table", {B, W}, c.dev);
+    if (B > 1 && table.stride(0) < W) throw ValueError("the rows of block_table must not overlap");
+    const Tensor &counts = a.ints(1, "counts", {B}, c.dev), &cu = a.ints(2, "cu_q", {B + 1}, c.dev);
+    const Tensor &lens = a.ints(3, "seq_lens", {B}, c.dev);
+    const c10::cuda::CUDAGuard guard(c.dev);
+    Tensor keep = at::empty({B}, lens.options());
+    chia_compact_params_t p{};
+    p.abi_version = CHIA_DRAFT_ABI_VERSION;
+    p.cache_dtype = c.type;
+    p.head_dim = static_cast<int32_t>(c.dim);
+    p.heads_kv = static_cast<int32_t>(c.heads);
+    p.page_size = static_cast<int32_t>(c.page);
+    p.batch = B;
+    p.max_tokens = most;
+    p.num_pages = c.pages;
+    p.table_width = W;
+    p.table_stride = table.stride(0) > W ? table.stride(0) : W;
+    p.path = ptr<int32_t>(path);
+    p.counts = ptr<int32_t>(counts);
+    p.cu_q = ptr<int32_t>(cu);
+    p.seq_lens = ptr<int32_t>(lens);
+    p.block_table = ptr<int32_t>(table);
+    p.k_cache = c.k.data_ptr();
+    p.v_cache = c.v.data_ptr();
+    p.k_scale = ptr<float>(c.ks);
+    p.v_scale = ptr<float>(c.vs);
+    p.keep_lens = ptr<int32_t>(keep);
+    p.status = reinterpret_cast<int32_t *>(a.integer(9));
+    const int code = g_compact(&p, c10::cuda::getCurrentCUDAStream(c.dev.index()).stream());
+    if (code != CHIA_OK) return PyLong_FromLong(code);
+    for (const Tensor *t : {&c.k, &c.v, &c.ks, &c.vs}) written(*t);
+    return THPVariable_Wrap(keep);
+  });
+}
+
+// -------------------------------------------------------------- norm, rotation
+// Queries and keys as [batch, heads, tokens, channels]: from [T, H, D], or as they are.
+struct Rows {
+  Tensor t;
+  int64_t b, h, s, d;
+  int64_t st[3];  // batch, head, token
+};
+bool rows_fit(const Tensor &t) {
+  const int64_t n = t.dim();
+  if (t.stride(n - 1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+  for (int64_t i = 0; i + 1 < n; ++i)
+    if (t.stride(i) % 8 != 0 || t.stride(i) < 0) return false;
+  return true;
+}
+Rows rows_of(const Tensor &t) {
+  Rows r{t, 1, 0, 0, 0, {0, 0, 0}};
+  if (t.dim() == 3) {
+    r.s = t.size(0), r.h = t.size(1), r.d = t.size(2);
+    r.st[1] = t.stride(1), r.st[2] = t.stride(0);
+  } else {
+    r.b = t.size(0), r.h = t.size(1), r.s = t.size(2), r.d = t.size(3);
+    r.st[0] = t.stride(0), r.st[1] = t.stride(1), r.st[2] = t.stride(2);
+  }
+  return r;
+}
+// An input: a copy where its rows are not 16-byte aligned with unit stride.
+Rows rows_in(const Tensor &t) { return rows_of(rows_fit(t) ? t : t.detach().contiguous()); }
+// A new tensor like an input, in its order of dimensions.
+Rows rows_out(const Tensor &like) {
+  Tensor o = at::empty_like(like, like.options().requires_grad(false));
+  if (!rows_fit(o)) o = at::empty(like.sizes(), like.options().requires_grad(false));
+  return rows_of(o);
+}
+
+struct Rope {
+  Rows q, k;
+  Tensor qw, kw, pos;
+  chia_rope_params_t p{};
+  // q, k, q_weight, k_weight, freqs, positions, eps, interleaved, weight_offset
+  explicit Rope(const Args &a, int i)
+      : q(rows_in(input(a, i, "q"))), k(rows_in(input(a, i + 1, "k"))) {
+    const Tensor &qt = q.t, &kt = k.t;
+    const at::Device dev = qt.device();
+    const int dt = any_type(qt);
+    if (dt < 0) throw ValueError(std::string("dtype ") + c10::toString(qt.scalar_type()) + " unsupported (bf16, fp16 or fp32)");
+    if (kt.scalar_type() != qt.scalar_type() || kt.device() != dev || kt.dim() != qt.dim() || k.b != q.b || k.s != q.s || k.d != q.d)
+      throw ValueError("q " + str(qt.sizes()) + ", k " + str(kt.sizes()) + " must match in all but the heads, in dtype and in device");
+    if (q.d != 64 && q.d != 128) throw ValueError("head_dim " + std::to_string(q.d) + " unsupported (64 or 128)");
+    if (q.h < 1 || k.h < 1 || q.b < 1) throw ValueError("empty q or k");
+    weight(a, i + 2, "q_weight", dev, qw);
+    weight(a, i + 3, "k_weight", dev, kw);
+    if (qw.defined() && kw.defined() && qw.scalar_type() != kw.scalar_type())
+      throw ValueError("q_weight, k_weight must share a dtype");
+    const Tensor &freqs = a.tensor(i + 4, "freqs", 1);
+    if (freqs.scalar_type() != at::kLong || freqs.device() != dev || !freqs.is_contiguous())
+      throw ValueError("freqs must be contiguous int64 on " + dev.str() + " (rope_frequencies makes them)");
+    const int64_t rot = 2 * freqs.size(0);
+    if (rot > q.d || rot % 8 != 0)
+      throw ValueError("freqs for " + std::to_string(rot) + " channels: a multiple of 8 up to " + std::to_string(q.d));
+    if (!a.none(i + 5)) {
+      if (!THPVariable_Check(a.v[i + 5])) throw ValueError("positions must be a tensor");
+      const int64_t dim = THPVariable_Unpack(a.v[i + 5]).dim();
+      const bool each = qt.dim() == 4 && dim == 2;  // of each batch entry
+      const int64_t shape[2] = {q.b, q.s};
+      pos = a.ints(i + 5, "positions", each ? at::IntArrayRef(shape, 2) : at::IntArrayRef(shape + 1, 1), dev);
+      p.positions = ptr<int32_t>(pos);
+      if (each) p.position_stride = pos.stride(0);
+    }
+    p.abi_version = CHIA_ROPE_ABI_VERSION;
+    p.dtype = dt;
+    p.weight_dtype = qw.defined() ? any_type(qw) : kw.defined() ? any_type(kw) : CHIA_DTYPE_F32;
+    p.head_dim = static_cast<int32_t>(q.d);
+    p.heads = static_cast<int32_t>(q.h);
+    p.heads_kv = static_cast<int32_t>(k.h);
+    p.rot = static_cast<int32_t>(rot);
+    p.batch = q.b;
+    p.seqlen = q.s;
+    p.q = qt.data_ptr();
+    p.k = kt.data_ptr();
+    for (int x = 0; x < 3; ++x) p.q_stride[x] = q.st[x], p.k_stride[x] = k.st[x];
+    if (qw.defined()) p.q_weight = qw.data_ptr();
+    if (kw.defined()) p.k_weight = kw.data_ptr();
+    p.freqs = ptr<uint64_t>(freqs);
+    p.eps = static_cast<float>(a.number(i + 6));
+    const int inter = PyObject_IsTrue(a.v[i + 7]);
+    if (inter < 0) throw 0;
+    p.interleaved = inter;
+    p.weight_offset = static_cast<float>(a.number(i + 8));
+    if (!(p.eps >= 0.f) || !std::isfinite(p.eps) || !std::isfinite(p.weight_offset))
+      throw ValueError("eps must be >= 0, eps and weight_offset finite");
+  }
+  static const Tensor &input(const Args &a, int i, const char *name) {
+    if (!THPVariable_Check(a.v[i]) || (THPVariable_Unpack(a.v[i]).dim() != 3 && THPVariable_Unpack(a.v[i]).dim() != 4))
+      throw ValueError(std::string(name) + " must be a 3-D or 4-D tensor");
+    const Tensor &t = a.tensor(i, name, THPVariable_Unpack(a.v[i]).dim());
+    no_tangent(t, name);
+    return t;
+  }
+  void weight(const Args &a, int i, const char *name, const at::Device &dev, Tensor &to) {
+    if (a.none(i)) return;
+    const Tensor &w = a.tensor(i, name, 1);
+    if (w.size(0) != q.d || any_type(w) < 0 || w.device() != dev)
+      throw ValueError(std::string(name) + " must be bf16, fp16 or fp32 (" + std::to_string(q.d) + ",) on " + dev.str() + ", got " +
+                       c10::toString(w.scalar_type()) + " " + str(w.sizes()) + " on " + w.device().str());
+    no_tangent(w, name);
+    to = w.is_contiguous() ? w : w.detach().contiguous();
+  }
+};
+
+// the nine arguments of Rope
+PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    const Args a(args, nargs, 9);
+    Rope r(a, 0);
+    const c10::cuda::CUDAGuard guard(r.q.t.device());
+    const Rows qo = rows_out(r.q.t), ko = rows_out(r.k.t);
+    r.p.q_out = qo.t.data_ptr(), r.p.k_out = ko.t.data_ptr();
+    for (int x = 0; x < 3; ++x) r.p.q_out_stride[x] = qo.st[x], r.p.k_out_stride[x] = ko.st[x];
+    const int code = g_rope(&r.p, c10::cuda::getCurrentCUDAStream(r.q.t.device().index()).stream());
+    if (code != CHIA_OK) return PyLong_FromLong(code);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(qo.t), THPVariable_Wrap(ko.t));
+  });
+}
+
+// dq_out, dk_out, then the nine arguments of Rope, want_q_weight, want_k_weight
+PyObject *qk_norm_rope_bwd(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject * {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    const Args a(args, nargs, 13);
+    Rope r(a, 2);
+    const Tensor *dy[2] = {&Rope::input(a, 0, "dq_out"), &Rope::input(a, 1, "dk_out")};
+    const Rows *x[2] = {&r.q, &r.k};
+    Rows g[2];
+    for (int i = 0; i < 2; ++i) {
+      if (dy[i]->sizes() != x[i]->t.sizes() || dy[i]->scalar_type() != x[i]->t.scalar_type() ||
+          dy[i]->device() != r.q.t.device())
+        throw ValueError(std::string(i ? "dk_out" : "dq_out") + " must match " + (i ? "k" : "q") + " in shape, dtype and device");
+      g[i] = rows_in(*dy[i]);
+    }
+    const c10::cuda::CUDAGuard guard(r.q.t.device());
+    const Rows dq = rows_out(r.q.t), dk = rows_out(r.k.t);
+    for (int i = 0; i < 3; ++i) r.p.q_out_stride[i] = dq.st[i], r.p.k_out_stride[i] = dk.st[i];
+    chia_rope_grads_t gr{};
+    gr.dq_out = g[0].t.data_ptr(), gr.dk_out = g[1].t.data_ptr();
+    for (int i = 0; i < 3; ++i) gr.dq_out_stride[i] = g[0].st[i], gr.dk_out_stride[i] = g[1].st[i];
+    gr.dq = dq.t.data_ptr(), gr.dk = dk.t.data_ptr();
+    Tensor dw[2], ws;
+    const Tensor *w[2] = {&r.qw, &r.kw};
+    for (int i = 0; i < 2; ++i)
+      if (w[i]->defined() && PyObject_IsTrue(a.v[11 + i])) dw[i] = at::empty({r.q.d}, w[i]->options().requires_grad(false));
+    if (dw[0].defined()) gr.dq_weight = dw[0].data_ptr();
+    if (dw[1].defined()) gr.dk_weight = dw[1].data_ptr();
+    int64_t bytes = 0;
+    if (r.qw.defined() || r.kw.defined()) {
+      bytes = g_rope_bytes(&r.p);
+      if (bytes < 0) throw ValueError("invalid backward parameters");
+      ws = at::empty({bytes}, r.q.t.options().dtype(at::kByte).requires_grad(false));
+    }
+    const int code = g_rope_bwd(&r.p, &gr, ws.defined() ? ws.data_ptr() : nullptr, bytes,
+                                c10::cuda::getCurrentCUDAStream(r.q.t.device().index()).stream());
+    if (code != CHIA_OK) return PyLong_FromLong(code);
+    auto wrap = [](const Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); };
+    return Py_BuildValue("(NNNN)", THPVariable_Wrap(dq.t), THPVariable_Wrap(dk.t), wrap(dw[0]), wrap(dw[1]));
+  });
+}
+
+}  // namespace

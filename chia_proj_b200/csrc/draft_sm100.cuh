@@ -1,0 +1,428 @@
+// draft_sm100.cuh -- trees of drafted tokens over the paged 8-bit K/V cache: their
+// tables, their verification, and the compaction of what was accepted.
+#pragma once
+#include "paged_common.cuh"
+
+namespace chia {
+
+// A request's rows [t0, t0 + n), n < 0 where its offsets are out of range or fall.
+struct TreeRows {
+  int t0, n;
+};
+__device__ __forceinline__ TreeRows tree_rows(const int32_t *cu_q, int b, int tokens) {
+  const int t0 = cu_q[b], t1 = cu_q[b + 1];
+  if (t0 < 0 || t1 < t0 || t1 > tokens) return {0, -1};
+  return {t0, t1 - t0};
+}
+
+// ---------------------------------------------------------------------- tables
+struct TreeArgs {
+  const int32_t *parents, *cu_q, *seq_lens;
+  int32_t *positions;
+  unsigned long long *ancestors;
+  int32_t *status;
+  int32_t batch, tokens;
+};
+
+constexpr int kTreeThreads = 256;
+
+// A warp a request, two nodes a lane. Words are completed by doubling: a node's word
+// takes up that of the node 2^i above it, and then looks twice as far up; six rounds
+// reach the root of any tree. The depth is the number of ancestors. Requests from an
+// offset on that falls are not served, as everywhere; rows that nobody owns get zeros.
+// A few KB: the time is latency.
+static __global__ void __launch_bounds__(kTreeThreads) tree_tables_kernel(const TreeArgs a) {
+  __shared__ int s_ordered;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) s_ordered = a.batch;
+  follow();
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.batch; b += kTreeThreads)
+    if (tree_rows(a.cu_q, b, a.tokens).n < 0) atomicMin(&s_ordered, b);
+  __syncthreads();
+  const int ordered = s_ordered;
+  bool bad = ordered < a.batch;
+  for (int b = blockIdx.x * (kTreeThreads / 32) + warp; b < ordered; b += gridDim.x * (kTreeThreads / 32)) {
+    const TreeRows r = tree_rows(a.cu_q, b, a.tokens);
+    const int base = a.seq_lens[b] - r.n;
+    if (r.n > kTreeNodes) {
+      for (int i = lane; i < r.n; i += 32) a.positions[r.t0 + i] = base + i, a.ancestors[r.t0 + i] = 0;
+      continue;
+    }
+    unsigned long long word[2];
+    int up[2];  // the node that is looked at next, itself where there is none
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int i = lane + 32 * x;
+      word[x] = 1ull << i, up[x] = i;
+      if (i < r.n) {
+        const int p = a.parents[r.t0 + i];
+        if (p >= 0 && p < i)
+          up[x] = p;
+        else if (p != -1)
+          bad = true;
+      }
+    }
+#pragma unroll
+    for (int round = 0; round < 6; ++round) {
+      unsigned long long w[2];
+      int u[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const unsigned long long w0 = __shfl_sync(0xffffffffu, word[0], up[x] & 31),
+                                 w1 = __shfl_sync(0xffffffffu, word[1], up[x] & 31);
+        const int u0 = __shfl_sync(0xffffffffu, up[0], up[x] & 31), u1 = __shfl_sync(0xffffffffu, up[1], up[x] & 31);
+        w[x] = up[x] < 32 ? w0 : w1, u[x] = up[x] < 32 ? u0 : u1;
+      }
+      word[0] |= w[0], word[1] |= w[1], up[0] = u[0], up[1] = u[1];
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int i = lane + 32 * x;
+      if (i < r.n) {
+        a.positions[r.t0 + i] = base + __popcll(word[x]) - 1;
+        a.ancestors[r.t0 + i] = word[x];
+      }
+    }
+  }
+  // rows before the first and behind the last request that is served
+  const int first = ordered > 0 ? a.cu_q[0] : a.tokens, last = ordered > 0 ? a.cu_q[ordered] : 0;
+  for (int t = blockIdx.x * kTreeThreads + threadIdx.x; t < a.tokens; t += gridDim.x * kTreeThreads)
+    if (t < first || t >= last) a.positions[t] = 0, a.ancestors[t] = 0;
+  if (bad) report(a.status, kStatusBadIndex);
+}
+
+// ---------------------------------------------------------------- verification
+struct VerifyArgs {
+  const void *p, *q;
+  int64_t p_st, q_st;
+  const int32_t *tokens, *parents, *cu_q;
+  const float *u;
+  int32_t *counts, *out, *path, *status;
+  int32_t batch, rows, vocab, most, chunks;  // chunks: of kVerifyChunk entries, in all
+};
+
+constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyCtas = 8;  // of a request: a cluster
+constexpr int kVerifyChunk = 512;  // entries that a warp sums at a time
+constexpr int kVerifyMostChunks = 1024;  // of a CTA
+
+// an entry; one that is no positive finite number is 0
+__device__ __forceinline__ float verify_clean(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+template <int T>
+__device__ __forceinline__ float verify_one(const void *p, int64_t e) {
+  if (T == 2) return verify_clean(static_cast<const float *>(p)[e]);
+  const uint32_t v = static_cast<const uint16_t *>(p)[e];
+  return verify_clean(T == 0 ? in16x2_to_float2<true>(v).x : in16x2_to_float2<false>(v).x);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+// to the same place in the shared memory of CTA `rank` of the cluster
+__device__ __forceinline__ void cluster_store(double *at, int rank, double v) {
+  uint32_t to;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(ptx::smem_u32(at)), "r"(rank));
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(v) : "memory");
+}
+__device__ __forceinline__ double shfl_up(double x, int d) { return __shfl_up_sync(0xffffffffu, x, d); }
+
+// A request's walk down its tree, by a cluster. What decides at a child is four numbers
+// (u, p, q at its token, and the residual's mass), so the probabilities of all nodes'
+// tokens are gathered at the start and the walk itself takes no memory. The rows are
+// read only for a mass: the residual behind rejected children is
+//   r = max(p - F q, 0),  F = sum of their Z / (1 - s)
+// (max(max(x - a, 0) - b, 0) = max(x - a - b, 0) for a, b >= 0), a function of the two
+// rows alone, so a pass keeps nothing but its sums: one for each chunk of 512 entries,
+// in the order of the vocabulary, so the drawn token is found from the last pass's sums
+// and one chunk that is read again. Without draft rows the mass is 1 minus what was
+// rejected, and the only pass is the last. All CTAs walk alike.
+template <int T, bool DRAFTS>
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
+  __shared__ double s_sum[kVerifyMostChunks];  // of this CTA's chunks
+  __shared__ double s_total[2][kVerifyCtas];   // of each CTA, two passes by turns
+  __shared__ float s_p[kTreeNodes], s_q[kTreeNodes], s_u[kTreeNodes];
+  __shared__ int s_parent[kTreeNodes], s_token[kTreeNodes];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = cluster_rank(), b = blockIdx.x / kVerifyCtas;
+  follow();
+  TreeRows r = tree_rows(a.cu_q, b, a.rows);
+  bool bad = r.n < 0 || r.n > kTreeNodes;
+  int32_t *out = a.out + static_cast<int64_t>(b) * a.most, *path = a.path + static_cast<int64_t>(b) * a.most;
+  if (r.n == 0 || bad) {
+    if (rank == 0) {
+      for (int i = t; i < a.most; i += kVerifyThreads) out[i] = path[i] = -1;
+      if (t == 0) a.counts[b] = 0;
+      if (t == 0 && bad) report(a.status, kStatusBadIndex);
+    }
+    return;  // (all CTAs of the cluster do)
+  }
+  if (t < r.n) {
+    const int x = a.tokens[r.t0 + t];
+    int p = a.parents[r.t0 + t];
+    s_u[t] = a.u[r.t0 + t];
+    if (t == 0) {
+      bad = p != -1;
+      p = -1;
+    } else if (p < -1 || p >= t || x < 0 || x >= a.vocab) {
+      bad = true;
+      p = -1;
+    }
+    s_parent[t] = p, s_token[t] = x;
+    if (p >= 0) {
+      s_p[t] = verify_one<T>(a.p, (r.t0 + p) * a.p_st + x);
+      if (DRAFTS) s_q[t] = verify_one<T>(a.q, (r.t0 + p) * a.q_st + x);
+    }
+    if (bad && rank == 0) report(a.status, kStatusBadIndex);
+  }
+  __syncthreads();
+
+  // Sums of the residual at `node`; returns the mass, the same in all CTAs.
+  int turn = 0;
+  const int per = (a.chunks + kVerifyCtas - 1) / kVerifyCtas, c0 = rank * per, mine = max(0, min(per, a.chunks - c0));
+  unsigned long long dropped = 0;  // (without draft rows) rejected children of the node
+  auto entry = [&](int node, double F, int v) {
+    if (v >= a.vocab) return 0.0;
+    double x = verify_one<T>(a.p, (r.t0 + node) * a.p_st + v);
+    if (DRAFTS && F != 0.0) x = fmax(fma(-F, static_cast<double>(verify_one<T>(a.q, (r.t0 + node) * a.q_st + v)), x), 0.0);
+    if (!DRAFTS)
+      for (unsigned long long m = dropped; m != 0; m &= m - 1)
+        if (s_token[__ffsll(m) - 1] == v) x = 0.0;
+    return x;
+  };
+  auto mass = [&](int node, double F) {
+    for (int c = warp; c < mine; c += kVerifyWarps) {
+      double sum = 0.0;
+#pragma unroll 4
+      for (int i = 0; i < kVerifyChunk / 32; ++i) sum += entry(node, F, (c0 + c) * kVerifyChunk + 32 * i + lane);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) s_sum[c] = sum;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      double sum = 0.0;
+      for (int c = lane; c < mine; c += 32) sum += s_sum[c];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane < kVerifyCtas) cluster_store(&s_total[turn][rank], lane, sum);
+    }
+    cluster_sync();
+    double z = 0.0;
+#pragma unroll
+    for (int x = 0; x < kVerifyCtas; ++x) z += s_total[turn][x];
+    turn ^= 1;
+    return z;
+  };
+
+  int node = 0, count = 1;
+  double Z = 1.0, F = 0.0, sib = 0.0;
+  bool known = true;  // Z is that of the residual
+  if (rank == 0 && t == 0) path[0] = 0;
+  for (int i = 1; i < r.n && count < a.most; ++i) {
+    if (s_parent[i] != node) continue;
+    const double u = s_u[i], p = s_p[i];
+    bool yes;
+    if (DRAFTS) {
+      const double q = s_q[i];
+      if (!known) Z = mass(node, F), known = true;
+      double here = fmax(fma(-F, q, p), 0.0), qx = q;
+      // (a token that an earlier sibling had is in neither)
+      for (int j = node + 1; j < i; ++j)
+        if (s_parent[j] == node && s_token[j] == s_token[i]) qx = 0.0;
+      const double d = 1.0 - sib;
+      yes = u * Z * qx < here * d;
+      if (!yes) {
+        if (d > 0.0) F += Z / d, known = false;
+        sib += qx;
+      }
+    } else {
+      double here = p;
+      for (unsigned long long m = dropped; m != 0; m &= m - 1)
+        if (s_token[__ffsll(m) - 1] == s_token[i]) here = 0.0;
+      yes = u * Z < here;
+      if (!yes) Z -= here, dropped |= 1ull << i;
+    }
+    if (yes) {
+      if (rank == 0 && t == 0) path[count] = i, out[count - 1] = s_token[i];
+      node = i, ++count, Z = 1.0, F = 0.0, sib = 0.0, known = true, dropped = 0;
+    }
+  }
+
+  // the token behind the last accepted node
+  Z = mass(node, F);
+  if (!(Z > 0.0)) F = 0.0, dropped = 0, Z = mass(node, F);
+  const double *total = s_total[turn ^ 1];
+  const double target = static_cast<double>(s_u[0]) * Z;
+  // the CTA whose chunks hold the place, or the last that holds anything
+  int owner = -1;
+  double before = 0.0, sum = 0.0;
+#pragma unroll
+  for (int x = 0; x < kVerifyCtas; ++x) {
+    if (total[x] > 0.0 && (owner < 0 || !(sum > target))) owner = x, before = sum;
+    sum += total[x];
+  }
+  if (rank == 0) {
+    for (int i = count + t; i < a.most; i += kVerifyThreads) out[i] = path[i] = -1;
+    if (t == 0) {
+      a.counts[b] = count;
+      if (owner < 0) out[count - 1] = -1;
+    }
+  }
+  if (owner == rank && warp == 0) {
+    // the chunk likewise, 32 at a time
+    int chunk = -1;
+    double base = before, in = before;  // the sum before the chunk
+    for (int x0 = 0; x0 < mine; x0 += 32) {
+      const double own = x0 + lane < mine ? s_sum[x0 + lane] : 0.0;
+      double inc = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double y = shfl_up(inc, d);
+        if (lane >= d) inc += y;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, own > 0.0 && base + inc > target);
+      const unsigned some = __ballot_sync(0xffffffffu, own > 0.0);
+      const int pick = over != 0 ? __ffs(over) - 1 : some != 0 ? 31 - __clz(some) : -1;
+      if (pick >= 0) {
+        chunk = x0 + pick;
+        in = base + __shfl_sync(0xffffffffu, inc - own, pick);
+      }
+      if (over != 0) break;
+      base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    // the entry likewise
+    int found = -1;
+    base = in;
+    for (int i = 0; i < kVerifyChunk / 32 && chunk >= 0; ++i) {
+      const int v = (c0 + chunk) * kVerifyChunk + 32 * i + lane;
+      const double own = entry(node, F, v);
+      double inc = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double y = shfl_up(inc, d);
+        if (lane >= d) inc += y;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, own > 0.0 && base + inc > target);
+      const unsigned some = __ballot_sync(0xffffffffu, own > 0.0);
+      const int pick = over != 0 ? __ffs(over) - 1 : some != 0 ? 31 - __clz(some) : -1;
+      if (pick >= 0) found = v - lane + pick;
+      if (over != 0) break;
+      base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) out[count - 1] = found;
+  }
+}
+
+// ------------------------------------------------------------------ compaction
+struct CompactArgs {
+  const int32_t *path, *counts, *cu_q, *seq_lens, *block_table;
+  uint8_t *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  int32_t *keep_lens, *status;
+  int64_t table_stride, num_pages;
+  int32_t batch, most, heads_kv, page, width;
+};
+
+constexpr int kCompactThreads = 128;
+
+// A CTA a request, K/V head, K or V. The path's nodes rise, so a token moves to a place
+// before its own; all of them are read (and their pages' scales) before anything is
+// written. Then page by page: the scale, where it grows what the page holds, and the
+// tokens.
+template <int D, int CT>
+__global__ void __launch_bounds__(kCompactThreads) cache_compact_kernel(const CompactArgs a) {
+  constexpr int PIECES = D / 16;  // 16-byte pieces of a token
+  __shared__ uint4 s_code[kTreeNodes * PIECES];
+  __shared__ float s_scale[kTreeNodes];                 // of the page that token k comes from
+  __shared__ float s_old[kTreeNodes];                   // of the one that it goes to
+  __shared__ int s_from[kTreeNodes], s_to[kTreeNodes];  // slots; -1: it stays
+  const int t = threadIdx.x, kinds = 2 * a.heads_kv;
+  const int b = blockIdx.x / kinds, which = blockIdx.x % kinds, h = which >> 1;
+  uint8_t *cache = which & 1 ? a.v_cache : a.k_cache;
+  float *scale = which & 1 ? a.v_scale : a.k_scale;
+  const int shift = 31 - __clz(a.page);
+  follow();
+  const int len = a.seq_lens[b], count = a.counts[b], t0 = a.cu_q[b], n = a.cu_q[b + 1] - t0;
+  const int base = len - n;
+  if (n > kTreeNodes && t0 >= 0) {  // a chunk: nothing of it was drafted
+    if (which == 0 && t == 0) a.keep_lens[b] = len;
+    return;
+  }
+  bool bad = t0 < 0 || n < 0 || len < n || count < 0 || count > n || count > a.most ||
+             len > static_cast<int64_t>(a.width) * a.page;
+  bool moves = false;
+  if (!bad && t < count) {
+    const int x = a.path[static_cast<int64_t>(b) * a.most + t];
+    const int last = t > 0 ? a.path[static_cast<int64_t>(b) * a.most + t - 1] : -1;
+    int from = -1, to = -1;
+    if (x <= last || x >= n) {
+      bad = true;
+    } else if (x != t) {
+      const int32_t *table = a.block_table + b * a.table_stride;
+      const int fp = table[(base + x) >> shift], tp = table[(base + t) >> shift];
+      if (fp < 0 || fp >= a.num_pages || tp < 0 || tp >= a.num_pages) {
+        bad = true;
+      } else {
+        from = (fp << shift) + ((base + x) & (a.page - 1)), to = (tp << shift) + ((base + t) & (a.page - 1));
+        moves = true;
+      }
+    }
+    s_from[t] = from, s_to[t] = to;
+  }
+  bad = __syncthreads_or(bad);
+  if (which == 0 && t == 0) {
+    a.keep_lens[b] = bad ? len : base + count;
+    if (bad) report(a.status, kStatusBadIndex);
+  }
+  const int moved = __syncthreads_count(moves && !bad);  // the last `moved` ones
+  if (moved == 0) return;
+  const int k0 = count - moved;
+  auto token = [&](int slot) {  // a token's bytes
+    return cache + ((static_cast<int64_t>(slot >> shift) * a.heads_kv + h) * a.page + (slot & (a.page - 1))) * D;
+  };
+  for (int e = t; e < moved * PIECES; e += kCompactThreads)
+    s_code[e] = reinterpret_cast<const uint4 *>(token(s_from[k0 + e / PIECES]))[e % PIECES];
+  if (t >= k0 && t < count) {
+    s_scale[t] = scale[static_cast<int64_t>(s_from[t] >> shift) * a.heads_kv + h];
+    s_old[t] = scale[static_cast<int64_t>(s_to[t] >> shift) * a.heads_kv + h];
+  }
+  __syncthreads();
+  auto again = [&](uint4 v, float ratio) {
+    auto one = [&](uint32_t w) {
+      uint32_t p01, p23;
+      cache4_to_f16<CT>(w, p01, p23);
+      const float2 f = f16x2_to_float2(p01), g = f16x2_to_float2(p23);
+      return to_cache4<CT>(f.x * ratio, f.y * ratio, g.x * ratio, g.y * ratio);
+    };
+    return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+  };
+  for (int k = k0; k < count;) {
+    const int page = s_to[k] >> shift;
+    int end = k;
+    float top = 0.f;
+    for (; end < count && s_to[end] >> shift == page; ++end) top = fmaxf(top, s_scale[end]);
+    const int64_t ph = static_cast<int64_t>(page) * a.heads_kv + h;
+    // (read once, by one thread: a barrier stands in a branch on it)
+    const float old = s_old[k], now = fmaxf(old, top);
+    if (now > old) {
+      if (t == 0) scale[ph] = now;
+      uint4 *p = reinterpret_cast<uint4 *>(cache + ph * a.page * D);
+      for (int e = t; e < a.page * PIECES; e += kCompactThreads) p[e] = again(p[e], old / now);
+      __syncthreads();  // the tokens below go on top
+    }
+    for (int e = t; e < (end - k) * PIECES; e += kCompactThreads) {
+      const int x = k + e / PIECES;
+      const uint4 v = s_code[(x - k0) * PIECES + e % PIECES];
+      const float own = s_scale[x];
+      reinterpret_cast<uint4 *>(token(s_to[x]))[e % PIECES] = own == now ? v : again(v, own / now);
+    }
+    k = end;
+  }
+}
+
+}  // namespace chia

@@ -1,5 +1,5 @@
 // paged_api.cu -- extern "C" entry points of the paged 8-bit K/V cache
-// (include/chia_paged.h): argument checks, choice of the kernel, launch. No
+// (include/chia_paged.h, and chia_tree_attn of chia_draft.h): argument checks, choice of the kernel, launch. No
 // allocation, no synchronisation.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -9,7 +9,7 @@
 #include <cstdint>
 #include <mutex>
 
-#include "../../include/chia_paged.h"
+#include "../../include/chia_draft.h"
 #include "cache_sm100.cuh"
 #include "paged_split_sm100.cuh"
 #include "paged_tiled_sm100.cuh"
@@ -211,10 +211,10 @@ struct SplitPlan {
   int grid;   // one CTA an SM
   int64_t off_ml, off_cuts, bytes;
 };
-int split_plan(const chia_paged_params_t *p, int sms, SplitPlan &pl) {
+int split_plan(const chia_paged_params_t *p, bool tree, int sms, SplitPlan &pl) {
   const int64_t group = p->heads / p->heads_kv;
   pl.tiled = p->max_q * group >= kTiledRows;
-  pl.tiles = p->max_q * group <= 8 ? 1 : 2;
+  pl.tiles = p->max_q * group <= 8 && !tree ? 1 : 2;  // (trees have units of 16 rows only)
   pl.rows = pl.tiled ? chia::TiledConfig<128>::ROWS : 8 * pl.tiles;
   pl.grid = sms;
   // the line of tiles is counted in 32 bits
@@ -280,6 +280,93 @@ int32_t clamp32(int64_t v) { return static_cast<int32_t>(v > kI32 ? kI32 : v); }
               : ((p)->cache_dtype == CHIA_CACHE_E4M3 ? FN<64, false, 0>(__VA_ARGS__)      \
                                                      : FN<64, false, 1>(__VA_ARGS__))))
 
+// positions, ancestors: of trees of drafted tokens; null: there are none.
+int attend(const chia_paged_params_t *p, const int32_t *positions, const uint64_t *ancestors, void *stream) {
+  const bool tree = positions != nullptr;
+  int rc = check_paged(p), sms = 0, dev = 0;
+  if (rc != CHIA_OK) return rc;
+  if (p->workspace == nullptr) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!aligned(p->workspace, 256)) return CHIA_ERR_MISALIGNED;
+  // (a workspace for no device is too small for any)
+  if (p->workspace_bytes <= kTicketBytes) return CHIA_ERR_INVALID_ARGUMENT;
+  if ((rc = device_sms(sms)) != CHIA_OK) return rc;
+  if (cudaGetDevice(&dev) != cudaSuccess) return CHIA_ERR_NO_DEVICE;
+  SplitPlan pl;
+  if ((rc = split_plan(p, tree, sms, pl)) != CHIA_OK) return rc;
+  if (p->workspace_bytes < pl.bytes) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p->tokens == 0) return CHIA_OK;
+  CUtensorMap mk, mv;
+  const int most = pl.tiled ? 64 : 32, box = p->page_size < most ? p->page_size : most;
+  if (!encode_cache(&mk, p->k_cache, p, box, !pl.tiled) ||
+      !encode_cache(&mv, p->v_cache, p, box, !pl.tiled))
+    return CHIA_ERR_LAUNCH;
+  chia::PagedArgs a{};
+  a.q = p->q;
+  a.o = p->o;
+  a.q_st = p->q_stride[0], a.q_sh = p->q_stride[1];
+  a.o_st = p->o_stride[0], a.o_sh = p->o_stride[1];
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.block_table = p->block_table;
+  a.seq_lens = p->seq_lens;
+  a.cu_q = p->cu_q;
+  a.table_stride = p->table_stride;
+  a.lse = p->norm == CHIA_NORM_SOFTMAX ? p->lse : nullptr;
+  a.head_param = (p->mod == CHIA_MOD_ALIBI || p->mod == CHIA_MOD_TEMP) ? p->head_param : nullptr;
+  a.left = clamp32(p->win_left);
+  a.right = clamp32(p->win_right);
+  a.block = clamp32(p->block);
+  a.prefix = clamp32(p->prefix);
+  a.dil = clamp32(p->dilation);
+  a.score_scale = p->scale;
+  a.softcap = p->softcap;
+  a.sig_bias = p->sig_bias;
+  a.out_scale = p->out_scale;
+  a.heads = p->heads;
+  a.heads_kv = p->heads_kv;
+  a.group = p->heads / p->heads_kv;
+  a.group_magic = a.group == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + a.group - 1) / a.group);
+  a.tokens = static_cast<int32_t>(p->tokens);
+  a.page = p->page_size;
+  a.width = static_cast<int32_t>(p->table_width);
+  a.num_pages = static_cast<int32_t>(p->num_pages);
+  a.q_each = static_cast<int32_t>(p->tokens / p->batch);
+  a.bf16 = p->dtype == CHIA_DTYPE_BF16;
+  a.status = p->status;
+  a.tree_pos = positions;
+  a.tree_word = reinterpret_cast<const unsigned long long *>(ancestors);
+  uint8_t *ws = static_cast<uint8_t *>(p->workspace);
+  a.tickets = reinterpret_cast<int32_t *>(ws);
+  a.part_o = reinterpret_cast<float *>(ws + kTicketBytes);
+  a.part_ml = reinterpret_cast<float *>(ws + pl.off_ml);
+  a.timeout_ns = p->wait_limit_ns > 0 ? p->wait_limit_ns : kDefaultTimeoutNs;
+  a.drain_ns = kDefaultTimeoutNs;
+  const int kind = kind_of(p);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int64_t b = 0; b < p->batch; b += chia::kLineBatch) {
+    const int64_t n = p->batch - b < chia::kLineBatch ? p->batch - b : chia::kLineBatch;
+    a.batch = static_cast<int32_t>(n);
+    a.seq_lens = p->seq_lens + b;
+    a.cu_q = p->cu_q != nullptr ? p->cu_q + b : nullptr;
+    a.token0 = static_cast<int32_t>(b * a.q_each);
+    a.block_table = p->block_table + b * p->table_stride;
+    const uint8_t *v8 = static_cast<const uint8_t *>(p->v_cache);
+#define CHIA_LAUNCH(D, CT)                                                                   \
+  (tree ? pl.tiled ? chia::launch_tiled_tree<D, CT>(mk, mv, a, v8, ws + pl.off_cuts, kind, pl.grid, dev, s)    \
+                   : chia::launch_split_tree<D, CT>(mk, mv, a, kind, pl.grid, dev, s)                         \
+   : pl.tiled ? chia::launch_tiled<D, CT>(mk, mv, a, v8, ws + pl.off_cuts, kind, pl.grid, dev, s)              \
+              : chia::launch_split<D, CT>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s))
+    const bool e4m3 = p->cache_dtype == CHIA_CACHE_E4M3;
+    const cudaError_t e =
+        p->head_dim == 128
+            ? (e4m3 ? CHIA_LAUNCH(128, chia::CACHE_E4M3) : CHIA_LAUNCH(128, chia::CACHE_INT8))
+            : (e4m3 ? CHIA_LAUNCH(64, chia::CACHE_E4M3) : CHIA_LAUNCH(64, chia::CACHE_INT8));
+#undef CHIA_LAUNCH
+    if (e != cudaSuccess) return CHIA_ERR_LAUNCH;
+  }
+  return CHIA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -324,89 +411,17 @@ int64_t chia_paged_attn_workspace_bytes(const chia_paged_params_t *p) {
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1)
     sms = 148;  // host-only callers (no GPU): size for a B200
-  SplitPlan pl;
-  return split_plan(p, sms, pl) == CHIA_OK ? pl.bytes : -1;
+  SplitPlan pl, tree;  // (for chia_tree_attn too)
+  if (split_plan(p, false, sms, pl) != CHIA_OK || split_plan(p, true, sms, tree) != CHIA_OK) return -1;
+  return pl.bytes > tree.bytes ? pl.bytes : tree.bytes;
 }
 
-int chia_paged_attn(const chia_paged_params_t *p, void *stream) {
-  int rc = check_paged(p), sms = 0, dev = 0;
-  if (rc != CHIA_OK) return rc;
-  if (p->workspace == nullptr) return CHIA_ERR_INVALID_ARGUMENT;
-  if (!aligned(p->workspace, 256)) return CHIA_ERR_MISALIGNED;
-  // (a workspace for no device is too small for any)
-  if (p->workspace_bytes <= kTicketBytes) return CHIA_ERR_INVALID_ARGUMENT;
-  if ((rc = device_sms(sms)) != CHIA_OK) return rc;
-  if (cudaGetDevice(&dev) != cudaSuccess) return CHIA_ERR_NO_DEVICE;
-  SplitPlan pl;
-  if ((rc = split_plan(p, sms, pl)) != CHIA_OK) return rc;
-  if (p->workspace_bytes < pl.bytes) return CHIA_ERR_INVALID_ARGUMENT;
-  if (p->tokens == 0) return CHIA_OK;
-  CUtensorMap mk, mv;
-  const int most = pl.tiled ? 64 : 32, box = p->page_size < most ? p->page_size : most;
-  if (!encode_cache(&mk, p->k_cache, p, box, !pl.tiled) ||
-      !encode_cache(&mv, p->v_cache, p, box, !pl.tiled))
-    return CHIA_ERR_LAUNCH;
-  chia::PagedArgs a{};
-  a.q = p->q;
-  a.o = p->o;
-  a.q_st = p->q_stride[0], a.q_sh = p->q_stride[1];
-  a.o_st = p->o_stride[0], a.o_sh = p->o_stride[1];
-  a.k_scale = p->k_scale;
-  a.v_scale = p->v_scale;
-  a.block_table = p->block_table;
-  a.seq_lens = p->seq_lens;
-  a.cu_q = p->cu_q;
-  a.table_stride = p->table_stride;
-  a.lse = p->norm == CHIA_NORM_SOFTMAX ? p->lse : nullptr;
-  a.head_param = (p->mod == CHIA_MOD_ALIBI || p->mod == CHIA_MOD_TEMP) ? p->head_param : nullptr;
-  a.left = clamp32(p->win_left);
-  a.right = clamp32(p->win_right);
-  a.block = clamp32(p->block);
-  a.prefix = clamp32(p->prefix);
-  a.dil = clamp32(p->dilation);
-  a.score_scale = p->scale;
-  a.softcap = p->softcap;
-  a.sig_bias = p->sig_bias;
-  a.out_scale = p->out_scale;
-  a.heads = p->heads;
-  a.heads_kv = p->heads_kv;
-  a.group = p->heads / p->heads_kv;
-  a.group_magic = a.group == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + a.group - 1) / a.group);
-  a.tokens = static_cast<int32_t>(p->tokens);
-  a.page = p->page_size;
-  a.width = static_cast<int32_t>(p->table_width);
-  a.num_pages = static_cast<int32_t>(p->num_pages);
-  a.q_each = static_cast<int32_t>(p->tokens / p->batch);
-  a.bf16 = p->dtype == CHIA_DTYPE_BF16;
-  a.status = p->status;
-  uint8_t *ws = static_cast<uint8_t *>(p->workspace);
-  a.tickets = reinterpret_cast<int32_t *>(ws);
-  a.part_o = reinterpret_cast<float *>(ws + kTicketBytes);
-  a.part_ml = reinterpret_cast<float *>(ws + pl.off_ml);
-  a.timeout_ns = p->wait_limit_ns > 0 ? p->wait_limit_ns : kDefaultTimeoutNs;
-  a.drain_ns = kDefaultTimeoutNs;
-  const int kind = kind_of(p);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  for (int64_t b = 0; b < p->batch; b += chia::kLineBatch) {
-    const int64_t n = p->batch - b < chia::kLineBatch ? p->batch - b : chia::kLineBatch;
-    a.batch = static_cast<int32_t>(n);
-    a.seq_lens = p->seq_lens + b;
-    a.cu_q = p->cu_q != nullptr ? p->cu_q + b : nullptr;
-    a.token0 = static_cast<int32_t>(b * a.q_each);
-    a.block_table = p->block_table + b * p->table_stride;
-    const uint8_t *v8 = static_cast<const uint8_t *>(p->v_cache);
-#define CHIA_LAUNCH(D, CT)                                                                   \
-  (pl.tiled ? chia::launch_tiled<D, CT>(mk, mv, a, v8, ws + pl.off_cuts, kind, pl.grid, dev, s)                \
-            : chia::launch_split<D, CT>(mk, mv, a, kind, pl.tiles, pl.grid, dev, s))
-    const bool e4m3 = p->cache_dtype == CHIA_CACHE_E4M3;
-    const cudaError_t e =
-        p->head_dim == 128
-            ? (e4m3 ? CHIA_LAUNCH(128, chia::CACHE_E4M3) : CHIA_LAUNCH(128, chia::CACHE_INT8))
-            : (e4m3 ? CHIA_LAUNCH(64, chia::CACHE_E4M3) : CHIA_LAUNCH(64, chia::CACHE_INT8));
-#undef CHIA_LAUNCH
-    if (e != cudaSuccess) return CHIA_ERR_LAUNCH;
-  }
-  return CHIA_OK;
+int chia_paged_attn(const chia_paged_params_t *p, void *stream) { return attend(p, nullptr, nullptr, stream); }
+
+int chia_tree_attn(const chia_paged_params_t *p, const int32_t *positions, const uint64_t *ancestors, void *stream) {
+  if (positions == nullptr || ancestors == nullptr) return CHIA_ERR_INVALID_ARGUMENT;
+  if (!aligned(positions, 4) || !aligned(ancestors, 8)) return CHIA_ERR_MISALIGNED;
+  return attend(p, positions, ancestors, stream);
 }
 
 }  // extern "C"

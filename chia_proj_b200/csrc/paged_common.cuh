@@ -16,6 +16,7 @@ enum CacheType : int { CACHE_E4M3 = 0, CACHE_INT8 = 1 };
 constexpr int kStatusBadIndex = 8;   // CHIA_ERR_BAD_INDEX
 constexpr int kStatusNoPages = 16;   // CHIA_ERR_NO_PAGES
 constexpr int kMinScaleExp = -64;    // the smallest scale is 2^-64
+constexpr int kTreeNodes = 64;       // CHIA_TREE_NODES: the bits of a word of ancestors
 
 __device__ __forceinline__ void report(int32_t *status, int bits) {
   if (status != nullptr) atomicOr(status, bits);

@@ -39,6 +39,8 @@ struct PagedArgs {
   float *part_ml;     // [parts][rows][2]
   int32_t *status;
   uint64_t timeout_ns, drain_ns;
+  const int32_t *tree_pos;              // trees of drafted tokens: of each row of q its position,
+  const unsigned long long *tree_word;  // the nodes of its tree that it sees
 };
 
 constexpr int kLineBatch = 512;  // requests of one launch (they are held in shared memory)
@@ -120,6 +122,31 @@ __device__ __forceinline__ void band32(const PagedArgs &a, int i, int len, int &
     lo = max(lo, b0);
     if (b0 <= 0x7fffffff - more) hi = min(hi, b0 + more);
   }
+}
+
+// Position of node i of the tree whose first token is row t0 of q: of its request's own ones.
+__device__ __forceinline__ int tree_position(const PagedArgs &a, int t0, int i, int p0, int len) {
+  return max(p0, min(len - 1, a.tree_pos[t0 + i]));
+}
+// Bits: the nodes of its tree (n of them) that node i, at position `pos`, sees: those of its
+// word that the mask does not put too far back. A word holds a path, so few are looked at.
+__device__ __forceinline__ unsigned long long tree_word_of(const PagedArgs &a, int t0, int i, int n, int pos, int len) {
+  unsigned long long word = a.tree_word[t0 + i];
+  if (n < 64) word &= (1ull << n) - 1;
+  if (a.left < 0 && a.block == 0 && a.dil == 1) return word;
+  int lo, hi;
+  band32(a, pos, len, lo, hi);
+#pragma unroll 1
+  for (unsigned long long m = word; m != 0; m &= m - 1) {
+    const int x = __ffsll(m) - 1, j = tree_position(a, t0, x, len - n, len);
+    if (j >= a.prefix && (j < lo || (a.dil != 1 && !divides(a.dil, pos - j)))) word &= ~(1ull << x);
+  }
+  return word;
+}
+// Of 32 keys from k0 on, where the tree's begin at `first`: the bits of `word`.
+__device__ __forceinline__ uint32_t tree_bits(unsigned long long word, int k0, int first) {
+  const int by = k0 - first;
+  return by >= 64 || by <= -32 ? 0u : by >= 0 ? static_cast<uint32_t>(word >> by) : static_cast<uint32_t>(word << -by);
 }
 
 template <int TK>
@@ -243,8 +270,8 @@ __device__ __forceinline__ void merge_parts(const PagedArgs &a, int first, int l
 // rows of one (several, where there are more blocks than entries fit): blocks
 // of a long run of queries see different keys. An entry's units visit the same
 // tiles. WHOLE: units of up to this cost (with BLOCKS: and of no more than a CTA's
-// share) are not cut between CTAs.
-template <int TK, int ROWS, int THREADS, int COST, int WHOLE, bool BLOCKS>
+// share) are not cut between CTAs. TREE: requests of up to kTreeNodes queries are trees.
+template <int TK, int ROWS, int THREADS, int COST, int WHOLE, bool BLOCKS, bool TREE = false>
 struct Line {
   struct Shared {
     int tiles_pre[kLineBatch + 1], units_pre[kLineBatch + 1];  // before each entry
@@ -309,7 +336,10 @@ struct Line {
         Request r = request_of(a, b, bad, gap);
         r.row0 = (t - s.starts[b]) * each * ROWS;
         r.row1 = min(r.row1, r.row0 + each * ROWS);
-        r.tl = tiles_of<TK>(a, r.len - r.n + div_group(a, r.row0), r.len - r.n + div_group(a, r.row1 - 1), r.len);
+        if (TREE && r.n <= kTreeNodes)  // (rows do not stand in the order of their positions)
+          r.tl = tiles_of<TK>(a, r.len - r.n, r.len - 1, r.len);
+        else
+          r.tl = tiles_of<TK>(a, r.len - r.n + div_group(a, r.row0), r.len - r.n + div_group(a, r.row1 - 1), r.len);
         s.req[t] = r;
       }
     } else {

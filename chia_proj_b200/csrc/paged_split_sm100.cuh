@@ -85,8 +85,11 @@ struct SplitConfig {
   static_assert(kSplitWarps * ROWS * PITCH * 4 <= RING, "the parts fit the spent ring");
 };
 
-// KIND: score modification and normaliser.
-template <int D, int CT, int NT, int KIND, bool BF16>
+// KIND: score modification and normaliser. TREE: requests of up to kTreeNodes queries are
+// trees of drafted tokens. A row then has a position and a word of its tree's nodes that it
+// sees; of keys from the tree's first one on the word decides, and none of their tiles
+// counts as one that all rows see.
+template <int D, int CT, int NT, int KIND, bool BF16, bool TREE>
 __global__ void __launch_bounds__(kSplitThreads, 1)
 paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const PagedArgs a) {
@@ -99,7 +102,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   extern __shared__ uint8_t dyn[];
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
   float *parts = reinterpret_cast<float *>(sm);  // [warps][ROWS][PITCH], in the spent ring
-  using L = Line<TK, ROWS, kSplitThreads, kUnitCost, kWholeUnit, false>;
+  using L = Line<TK, ROWS, kSplitThreads, kUnitCost, kWholeUnit, false, TREE>;
   __shared__ typename L::Shared line_sm;
   __shared__ __align__(8) uint64_t bars[kSplitWarps * NST];
   __shared__ float part_ml[kSplitWarps][ROWS][2];
@@ -241,11 +244,15 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   int len = 0, p0 = 0, ut0 = 0, nt = 0;
   uint4 raw[NT][H * 2];  // row 8 n + gid, channels 16 H tig .. + 16 H - 1
   float hp[NT][2];       // of rows 8 n + 2 tig + e, as in the columns of S^T
+  // TREE: of those rows; the tree's first key (none: the largest number) and row of q
+  unsigned long long word[TREE ? NT : 1][2];
+  int tpos[TREE ? NT : 1][2], first = 0x7fffffff, tree_t0 = 0;
   auto begin_unit = [&](int k, int b) {  // b: the entry
     const int g = c0 + k;
     const Request rq = line_sm.req[b];
     len = rq.len;
     p0 = len - rq.n;
+    if (TREE) first = rq.n <= kTreeNodes ? p0 : 0x7fffffff, tree_t0 = rq.t0;
     tl = rq.tl;
     un = line.unit_at(g, b, rq, ut0);
     nt = min(tl.n - ut0, nk - k);
@@ -269,6 +276,14 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         hp[n][x] = a.head_param != nullptr
                        ? a.head_param[un.hk * a.group + r - div_group(a, r) * a.group]
                        : 1.f;
+        if (TREE) {
+          const int qi = div_group(a, r);
+          word[n][x] = 0, tpos[n][x] = p0 + qi;
+          if (rq.n <= kTreeNodes) {
+            tpos[n][x] = tree_position(a, rq.t0, qi, p0, len);
+            word[n][x] = tree_word_of(a, rq.t0, qi, rq.n, tpos[n][x], len);
+          }
+        }
       }
     }
   };
@@ -286,7 +301,13 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     int lo_min, hi_max;  // no row sees a key outside of them and the prefix
     band32(a, p0 + div_group(a, un.row0), len, lo_min, hi_min);
     band32(a, p0 + div_group(a, un.row0 + un.rows - 1), len, lo_max, hi_max);
-    const int pf = min(a.prefix, len);
+    int pf = min(a.prefix, len);
+    if (TREE && first != 0x7fffffff) {
+      band32(a, p0, len, lo_min, hi_min);
+      band32(a, len - 1, len, lo_max, hi_max);
+      hi_min = min(hi_min, first - 1);
+      pf = max(0, min(pf, first));
+    }
     pf_all = pf - TK;
     if (any_lost) hi_min = pf_all = -1;
 
@@ -325,7 +346,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       for (int x = 0; x < 2; ++x) {
         const float f = __shfl_sync(0xffffffffu, down, (2 * tig + x) * 4);
         const int r = min(8 * n + 2 * tig + x, un.rows - 1) + un.row0;
-        posn[n][x] = p0 + div_group(a, r);
+        posn[n][x] = TREE ? tpos[n][x] : p0 + div_group(a, r);
         real |= (8 * n + 2 * tig + x < un.rows ? 1u : 0u) << (2 * n + x);
         float mul = a.score_scale * f;
         slope[n][x] = 0.f;
@@ -336,6 +357,11 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         rowmul[n][x] = mul;
       }
     }
+    // whether row 8 n + 2 tig + e sees key j, [lo, hi] being its band
+    auto sees_key = [&](int n, int e, int j, int lo, int hi) {
+      if (TREE && j >= first) return j - first < 64 && ((word[n][e] >> (j - first)) & 1) != 0;
+      return j < pf || (j >= lo && j <= hi && (a.dil == 1 || divides(a.dil, posn[n][e] - j)));
+    };
     float o[MT][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -422,6 +448,18 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       };
 #pragma unroll
       for (int m = 0; m < VP; ++m) load_v(m);
+      // positions of this lane's keys (ALiBi); of a tree's nodes their own
+      int key_pos[2][2];
+      if (TREE && KIND == KIND_ALIBI) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int j = j0 + 16 * m + 8 * x + gid;
+            key_pos[m][x] = j;
+            if (j >= first && j < len) key_pos[m][x] = tree_position(a, tree_t0, j - first, p0, len);
+          }
+      }
       // ---------------- score modification, mask, normaliser
       // s[m][n][2 x + e]: key j0 + 16 m + 8 x + gid, row 8 n + 2 tig + e
 #pragma unroll
@@ -440,7 +478,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                 const float z = ptx::ex2(v * f);
                 v = fmaf(a.softcap * LOG2E, fmaf(-2.f, ptx::rcp_fast(z + 1.f), 1.f), vf);
               } else if (KIND == KIND_ALIBI) {
-                v = fmaf(slope[n][e], static_cast<float>(j0 + 16 * m + 8 * x + gid - posn[n][e]),
+                const int j = TREE ? key_pos[m][x] : j0 + 16 * m + 8 * x + gid;
+                v = fmaf(slope[n][e], static_cast<float>(j - posn[n][e]),
                          fmaf(v, f, vf));
               } else if (KIND == KIND_SIGMOID) {
                 v = vf * ptx::rcp_fast(1.f + ptx::ex2(fmaf(v, f, -a.sig_bias * LOG2E)));
@@ -465,9 +504,8 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
                 const int j = j0 + 16 * m + 8 * x + gid;
-                const bool vis = ((real >> (2 * n + e)) & 1u) && !((gone >> m) & 1) &&
-                                 (j < pf || (j >= lo && j <= hi &&
-                                             (a.dil == 1 || divides(a.dil, i_pos - j))));
+                const bool vis =
+                    ((real >> (2 * n + e)) & 1u) && !((gone >> m) & 1) && sees_key(n, e, j, lo, hi);
                 if (!vis) s[m][n][2 * x + e] = SOFTMAX ? -INFINITY : 0.f;
               }
           }
@@ -599,9 +637,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               const int i_pos = posn[n][e];
               int lo, hi;
               band32(a, i_pos, len, lo, hi);
-              sees[n][e] = ((real >> (2 * n + e)) & 1u) &&
-                           (j < pf || (j >= lo && j <= hi &&
-                                       (a.dil == 1 || divides(a.dil, i_pos - j))));
+              sees[n][e] = ((real >> (2 * n + e)) & 1u) && sees_key(n, e, j, lo, hi);
             }
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
@@ -808,31 +844,36 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   }
 }
 
-// Launches of one head size and cache type; each has a source file of its own.
+// Launches of one head size and cache type; each has a source file of its own, and so have
+// those of trees (units of 16 rows).
 template <int D, int CT>
 cudaError_t launch_split(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a, int kind,
                          int tiles, int grid, int device, cudaStream_t s);
 
-template <int D, int CT, int NT, int KIND, bool BF16>
+template <int D, int CT>
+cudaError_t launch_split_tree(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a, int kind,
+                              int grid, int device, cudaStream_t s);
+
+template <int D, int CT, int NT, int KIND, bool BF16, bool TREE>
 cudaError_t launch_split_one(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                              int grid, int device, cudaStream_t s) {
   static std::atomic<uint64_t> set{0};
   constexpr int bytes = SplitConfig<D, NT>::SMEM;
   const cudaError_t e = allow_smem(
-      reinterpret_cast<const void *>(&paged_split_kernel<D, CT, NT, KIND, BF16>), bytes, device, set);
+      reinterpret_cast<const void *>(&paged_split_kernel<D, CT, NT, KIND, BF16, TREE>), bytes, device, set);
   if (e != cudaSuccess) return e;
-  return launch_after(paged_split_kernel<D, CT, NT, KIND, BF16>, dim3(grid), kSplitThreads, bytes, s, mk, mv, a);
+  return launch_after(paged_split_kernel<D, CT, NT, KIND, BF16, TREE>, dim3(grid), kSplitThreads, bytes, s, mk, mv, a);
 }
 
-template <int D, int CT, int NT, bool BF16>
+template <int D, int CT, int NT, bool BF16, bool TREE = false>
 cudaError_t launch_split_kind(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                               int kind, int grid, int device, cudaStream_t s) {
   switch (kind) {
-    case KIND_SOFTCAP: return launch_split_one<D, CT, NT, KIND_SOFTCAP, BF16>(mk, mv, a, grid, device, s);
-    case KIND_ALIBI: return launch_split_one<D, CT, NT, KIND_ALIBI, BF16>(mk, mv, a, grid, device, s);
-    case KIND_SIGMOID: return launch_split_one<D, CT, NT, KIND_SIGMOID, BF16>(mk, mv, a, grid, device, s);
-    case KIND_RELU: return launch_split_one<D, CT, NT, KIND_RELU, BF16>(mk, mv, a, grid, device, s);
-    default: return launch_split_one<D, CT, NT, KIND_SOFTMAX, BF16>(mk, mv, a, grid, device, s);
+    case KIND_SOFTCAP: return launch_split_one<D, CT, NT, KIND_SOFTCAP, BF16, TREE>(mk, mv, a, grid, device, s);
+    case KIND_ALIBI: return launch_split_one<D, CT, NT, KIND_ALIBI, BF16, TREE>(mk, mv, a, grid, device, s);
+    case KIND_SIGMOID: return launch_split_one<D, CT, NT, KIND_SIGMOID, BF16, TREE>(mk, mv, a, grid, device, s);
+    case KIND_RELU: return launch_split_one<D, CT, NT, KIND_RELU, BF16, TREE>(mk, mv, a, grid, device, s);
+    default: return launch_split_one<D, CT, NT, KIND_SOFTMAX, BF16, TREE>(mk, mv, a, grid, device, s);
   }
 }
 
@@ -846,6 +887,14 @@ cudaError_t launch_split_kind(const CUtensorMap &mk, const CUtensorMap &mv, cons
                         : launch_split_kind<D, CT, 2, true>(mk, mv, a, kind, grid, device, s);  \
     return tiles == 1 ? launch_split_kind<D, CT, 1, false>(mk, mv, a, kind, grid, device, s)    \
                       : launch_split_kind<D, CT, 2, false>(mk, mv, a, kind, grid, device, s);   \
+  }
+#define CHIA_INSTANTIATE_SPLIT_TREE(D, CT)                                                      \
+  template <>                                                                                   \
+  cudaError_t chia::launch_split_tree<D, CT>(const CUtensorMap &mk, const CUtensorMap &mv,      \
+                                             const PagedArgs &a, int kind, int grid,            \
+                                             int device, cudaStream_t s) {                      \
+    return a.bf16 ? launch_split_kind<D, CT, 2, true, true>(mk, mv, a, kind, grid, device, s)   \
+                  : launch_split_kind<D, CT, 2, false, true>(mk, mv, a, kind, grid, device, s); \
   }
 
 }  // namespace chia

@@ -110,14 +110,22 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const PagedA
 // Channels (bits) in which a visible key of tiles [t0, t1) of the unit holds
 // NaN, where the tile is not visible as a whole (pages out of range are not): the
 // converters leave NaN out of such tiles, since a P of zero would spread it to rows
-// that do not see it.
-template <int D>
+// that do not see it. Tree: the first key of the row's tree, and the row's word.
+template <int D, class... Tree>
 __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_cache, int b, int hk,
                                           const Tiles &tl, int t0, int t1, int i, int len, int lo_max,
-                                          int hi_min, uint32_t *mask) {
+                                          int hi_min, uint32_t *mask, Tree... tree) {
   int lo, hi;
   band32(a, i, len, lo, hi);
-  const int pf = min(a.prefix, len);
+  int pf = min(a.prefix, len);
+  auto sees = [&](int j) { return j < pf || (j >= lo && j <= hi && (a.dil == 1 || divides(a.dil, i - j))); };
+  auto sees_node = [&](int j, int first, unsigned long long word) {
+    return j < first ? sees(j) : j - first < 64 && ((word >> (j - first)) & 1) != 0;
+  };
+  if constexpr (sizeof...(Tree) > 0) {
+    const auto clip = [&](int first, unsigned long long) { pf = max(0, min(pf, first)); };
+    clip(tree...);
+  }
   for (int t = t0; t < t1; ++t) {
     constexpr int TK = TiledConfig<D>::TK;
     const int j0 = tl.key_tile(t) * TK;
@@ -128,7 +136,11 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
     }
     if (whole) continue;
     for (int j = j0; j - j0 < TK && j < len; ++j) {
-      if (!(j < pf || (j >= lo && j <= hi && (a.dil == 1 || divides(a.dil, i - j))))) continue;
+      if constexpr (sizeof...(Tree) > 0) {
+        if (!sees_node(j, tree...)) continue;
+      } else if (!sees(j)) {
+        continue;
+      }
       const int pg = a.block_table[b * a.table_stride + j / a.page];
       if (pg < 0 || pg >= a.num_pages) continue;
       const uint8_t *v = v_cache + ((static_cast<int64_t>(pg) * a.heads_kv + hk) * a.page + j % a.page) * D;
@@ -138,7 +150,8 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
   }
 }
 
-template <int D, int CT, int KIND, bool BF16>
+// TREE: requests of up to kTreeNodes queries are trees of drafted tokens, as in the split kernel.
+template <int D, int CT, int KIND, bool BF16, bool TREE>
 __global__ void __launch_bounds__(kTiledThreads, 1)
 paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                    const PagedArgs a, const uint8_t *v_cache, CutUnit *cuts) {
@@ -147,7 +160,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                 GROUPS = C::GROUPS;
   constexpr bool SOFTMAX = KIND <= KIND_ALIBI;
   constexpr float LOG2E = 1.4426950408889634f;
-  using L = Line<TK, ROWS, kTiledThreads, kTiledCost, kTiledWhole, true>;
+  using L = Line<TK, ROWS, kTiledThreads, kTiledCost, kTiledWhole, true, TREE>;
   extern __shared__ uint8_t dyn[];
   uint8_t *sm = dyn + ((1024u - (ptx::smem_u32(dyn) & 1023u)) & 1023u);
   const uint32_t sb = ptx::smem_u32(sm);
@@ -217,6 +230,8 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     Request rq;
     int ut0, nt, p0, lo_max, hi_min;
   };
+  // the first key of a request's tree (none: the largest number)
+  auto tree_first = [](const Request &r) { return TREE && r.n <= kTreeNodes ? r.len - r.n : 0x7fffffff; };
   auto unit_at = [&](int k) {
     Here h;
     const int e = line.entry_at(c0 + k);
@@ -227,11 +242,20 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     int x;
     band32(a, h.p0 + div_group(a, h.un.row0), h.rq.len, x, h.hi_min);
     band32(a, h.p0 + div_group(a, h.un.row0 + h.un.rows - 1), h.rq.len, h.lo_max, x);
+    if (TREE && h.rq.n <= kTreeNodes) {
+      band32(a, h.p0, h.rq.len, x, h.hi_min);
+      band32(a, h.rq.len - 1, h.rq.len, h.lo_max, x);
+      h.hi_min = min(h.hi_min, h.p0 - 1);
+    }
     return h;
+  };
+  auto prefix_of = [&](const Here &h) {  // keys that every row sees
+    const int pf = min(a.prefix, h.rq.len);
+    return TREE ? max(0, min(pf, tree_first(h.rq))) : pf;
   };
   auto sees_all = [&](const Here &h, int j0) {  // every row of the unit sees keys [j0, j0 + TK)
     return (a.dil == 1 && j0 >= h.lo_max && j0 + TK - 1 <= h.hi_min) ||
-           j0 <= min(a.prefix, h.rq.len) - TK;
+           j0 <= prefix_of(h) - TK;
   };
 
   if (warp >= 8) {
@@ -256,6 +280,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           int y;
           band32(a, h.p0 + div_group(a, h.un.row0), h.rq.len, lo_min, y);
           band32(a, h.p0 + div_group(a, h.un.row0 + h.un.rows - 1), h.rq.len, y, hi_max);
+          if (TREE && h.rq.n <= kTreeNodes) {
+            band32(a, h.p0, h.rq.len, lo_min, y);
+            band32(a, h.rq.len - 1, h.rq.len, y, hi_max);
+          }
         }
         const int j0 = h.rq.tl.key_tile(h.ut0 + h.nt - left) * TK;
         --left;
@@ -264,7 +292,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         x.all = sees_all(h, j0);
         x.live = h.rq.len - j0;
         // (the scales of 16 keys that no row sees may be anything)
-        if (!(x.key < min(a.prefix, h.rq.len) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
+        if (!(x.key < prefix_of(h) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
         if (lane < GROUPS && x.key < h.rq.len) 
           x.pg = a.block_table[h.rq.b * a.table_stride + (x.key >> pshift)], x.all |= 4;
         return x;
@@ -482,7 +510,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       if (h.un.rows > w * 128) {
         const int rr = h.un.row0 + min(r, h.un.rows - 1);
         const int qi = div_group(a, rr), head = h.un.hk * a.group + rr - qi * a.group;
-        const int pos = h.p0 + qi;
+        const int first = tree_first(h.rq);
+        const int pos = TREE && first != 0x7fffffff ? tree_position(a, h.rq.t0, qi, h.p0, h.rq.len) : h.p0 + qi;
+        unsigned long long word = 0;  // TREE: the nodes that this row sees
+        if (TREE && first != 0x7fffffff) word = tree_word_of(a, h.rq.t0, qi, h.rq.n, pos, h.rq.len);
         // ---- the row of Q, as halves
         // (16 bytes a lane, neighbouring lanes along a row, four loads on their way
         // while four are converted: unrolled further, fetching the code takes longer)
@@ -541,7 +572,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         if (KIND == KIND_SIGMOID) rowmul *= -LOG2E;
         int lo, hi;
         band32(a, pos, h.rq.len, lo, hi);
-        const int pf = min(a.prefix, h.rq.len);
+        const int pf = prefix_of(h);
         float m_run = SOFTMAX ? -INFINITY : -100.f, l_run = 0.f;
         for (int i = 0; i < h.nt; ++i, ++cnt) {
           const int n = k + i;
@@ -569,7 +600,10 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                 for (int e = first < 0 ? first + a.dil : first; e < 32; e += a.dil) every |= 1u << e;
                 m &= every;
               }
-              vis[c] = real ? m | below(pf - k0) : 0u;
+              m |= below(pf - k0);
+              // (differences from the largest number do not fit: no tree's keys are near)
+              if (TREE && first - 32 < k0) m = (m & below(first - k0)) | tree_bits(word, k0, first);
+              vis[c] = real ? m : 0u;
               const int lost = tile_lost[n % SETS] >> (2 * c);
               vis[c] &= (lost & 1 ? 0u : 0xffffu) | (lost & 2 ? 0u : 0xffff0000u);
             }
@@ -578,6 +612,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           ptx::reg_fence(sr[0]);
           ptx::reg_fence(sr[1]);
           const float rel = static_cast<float>(j0 - pos);
+          const bool at_tree = TREE && KIND == KIND_ALIBI && first < j0 + TK;
           float mx = SOFTMAX ? -INFINITY : 0.f;
           auto pass1 = [&](auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
@@ -609,7 +644,15 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                   x2 = ptx::fma2(x2, F2, V2);
                   if (KIND == KIND_ALIBI) {
                     const float c = static_cast<float>(col);
-                    x2 = ptx::fma2(ptx::f2(slope, slope), ptx::f2(rel + c, rel + c + 1.f), x2);
+                    float d0 = rel + c, d1 = rel + c + 1.f;
+                    if (MASKED && at_tree) {  // a tree's nodes have positions of their own
+                      const int j = j0 + col;
+                      if (j >= first && j < h.rq.len)
+                        d0 = static_cast<float>(tree_position(a, h.rq.t0, j - first, h.p0, h.rq.len) - pos);
+                      if (j + 1 >= first && j + 1 < h.rq.len)
+                        d1 = static_cast<float>(tree_position(a, h.rq.t0, j + 1 - first, h.p0, h.rq.len) - pos);
+                    }
+                    x2 = ptx::fma2(ptx::f2(slope, slope), ptx::f2(d0, d1), x2);
                   }
                   ptx::f2_split(x2, x, y);
                 }
@@ -711,9 +754,16 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         ptx::tc_fence_after();
         m_run -= kTiledPTop;  // what O and the sum are relative to
         uint32_t nan[D / 32] = {};
-        if (CT == CACHE_E4M3 && nan_flag && real)
-          nan_channels<D>(a, v_cache, h.rq.b, h.un.hk, h.rq.tl, h.ut0, h.ut0 + h.nt, pos, h.rq.len, h.lo_max,
-                          h.hi_min, nan);
+        if (CT == CACHE_E4M3 && nan_flag && real) {
+          auto find = [&](auto... tree) {
+            nan_channels<D>(a, v_cache, h.rq.b, h.un.hk, h.rq.tl, h.ut0, h.ut0 + h.nt, pos, h.rq.len, h.lo_max,
+                            h.hi_min, nan, tree...);
+          };
+          if constexpr (TREE)
+            find(first, word);
+          else
+            find();
+        }
         float f = 1.f;
         row_out<KIND>(a, h.un, min(r, h.un.rows - 1), m_run, l_run, whole && real, f);
         // Through this warp's rows of Q's memory (free: the unit's UMMAs are
@@ -800,35 +850,39 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   }
 }
 
-// Launches of one head size and cache type; each has a source file of its own.
+// Launches of one head size and cache type; each has a source file of its own, and so have
+// those of trees.
 template <int D, int CT>
 cudaError_t launch_tiled(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                          const uint8_t *v_cache, void *cuts, int kind, int grid, int device, cudaStream_t s);
+template <int D, int CT>
+cudaError_t launch_tiled_tree(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
+                              const uint8_t *v_cache, void *cuts, int kind, int grid, int device, cudaStream_t s);
 
-template <int D, int CT, int KIND, bool BF16>
+template <int D, int CT, int KIND, bool BF16, bool TREE>
 cudaError_t launch_tiled_one(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                              const uint8_t *v_cache, void *cuts, int grid, int device, cudaStream_t s) {
   static std::atomic<uint64_t> set{0};
   constexpr int bytes = TiledConfig<D>::SMEM;
-  cudaError_t e = allow_smem(reinterpret_cast<const void *>(&paged_tiled_kernel<D, CT, KIND, BF16>), bytes,
+  cudaError_t e = allow_smem(reinterpret_cast<const void *>(&paged_tiled_kernel<D, CT, KIND, BF16, TREE>), bytes,
                              device, set);
   if (e != cudaSuccess) return e;
-  e = launch_after(paged_tiled_kernel<D, CT, KIND, BF16>, dim3(grid), kTiledThreads, bytes, s, mk, mv, a, v_cache,
+  e = launch_after(paged_tiled_kernel<D, CT, KIND, BF16, TREE>, dim3(grid), kTiledThreads, bytes, s, mk, mv, a, v_cache,
                    static_cast<CutUnit *>(cuts));
   if (e != cudaSuccess) return e;
   return launch_after(paged_merge_kernel<D, KIND, BF16>, dim3(grid, kMergeSlices), kMergeThreads, 0, s, a,
                       static_cast<const CutUnit *>(cuts));
 }
 
-template <int D, int CT, bool BF16>
+template <int D, int CT, bool BF16, bool TREE = false>
 cudaError_t launch_tiled_kind(const CUtensorMap &mk, const CUtensorMap &mv, const PagedArgs &a,
                               const uint8_t *v_cache, void *cuts, int kind, int grid, int device, cudaStream_t s) {
   switch (kind) {
-    case KIND_SOFTCAP: return launch_tiled_one<D, CT, KIND_SOFTCAP, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
-    case KIND_ALIBI: return launch_tiled_one<D, CT, KIND_ALIBI, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
-    case KIND_SIGMOID: return launch_tiled_one<D, CT, KIND_SIGMOID, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
-    case KIND_RELU: return launch_tiled_one<D, CT, KIND_RELU, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
-    default: return launch_tiled_one<D, CT, KIND_SOFTMAX, BF16>(mk, mv, a, v_cache, cuts, grid, device, s);
+    case KIND_SOFTCAP: return launch_tiled_one<D, CT, KIND_SOFTCAP, BF16, TREE>(mk, mv, a, v_cache, cuts, grid, device, s);
+    case KIND_ALIBI: return launch_tiled_one<D, CT, KIND_ALIBI, BF16, TREE>(mk, mv, a, v_cache, cuts, grid, device, s);
+    case KIND_SIGMOID: return launch_tiled_one<D, CT, KIND_SIGMOID, BF16, TREE>(mk, mv, a, v_cache, cuts, grid, device, s);
+    case KIND_RELU: return launch_tiled_one<D, CT, KIND_RELU, BF16, TREE>(mk, mv, a, v_cache, cuts, grid, device, s);
+    default: return launch_tiled_one<D, CT, KIND_SOFTMAX, BF16, TREE>(mk, mv, a, v_cache, cuts, grid, device, s);
   }
 }
 
@@ -840,6 +894,15 @@ cudaError_t launch_tiled_kind(const CUtensorMap &mk, const CUtensorMap &mv, cons
                                         cudaStream_t s) {                                      \
     return a.bf16 ? launch_tiled_kind<D, CT, true>(mk, mv, a, v_cache, cuts, kind, grid, device, s)   \
                   : launch_tiled_kind<D, CT, false>(mk, mv, a, v_cache, cuts, kind, grid, device, s); \
+  }
+#define CHIA_INSTANTIATE_TILED_TREE(D, CT)                                                          \
+  template <>                                                                                  \
+  cudaError_t chia::launch_tiled_tree<D, CT>(const CUtensorMap &mk, const CUtensorMap &mv,          \
+                                        const PagedArgs &a, const uint8_t *v_cache,            \
+                                        void *cuts, int kind, int grid, int device,            \
+                                        cudaStream_t s) {                                      \
+    return a.bf16 ? launch_tiled_kind<D, CT, true, true>(mk, mv, a, v_cache, cuts, kind, grid, device, s)   \
+                  : launch_tiled_kind<D, CT, false, true>(mk, mv, a, v_cache, cuts, kind, grid, device, s); \
   }
 
 }  // namespace chia

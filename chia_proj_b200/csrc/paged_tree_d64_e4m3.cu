@@ -1,0 +1,6 @@
+// The kernels for trees of drafted tokens of head size 64 over an e4m3 cache.
+#include "paged_split_sm100.cuh"
+#include "paged_tiled_sm100.cuh"
+
+CHIA_INSTANTIATE_SPLIT_TREE(64, chia::CACHE_E4M3)
+CHIA_INSTANTIATE_TILED_TREE(64, chia::CACHE_E4M3)

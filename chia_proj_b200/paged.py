@@ -136,7 +136,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     head_param: Optional[Union[torch.Tensor, Sequence[float]]] = None,
                     sig_bias: float = 0.0, out_scale: float = 1.0,
                     out: Optional[torch.Tensor] = None, return_lse: bool = False,
-                    wait_limit_ns: int = 0):
+                    wait_limit_ns: int = 0, tree: Optional["TreeStep"] = None):
     """``attention`` of a step's queries over the paged cache.
 
     ``q`` ``[T, H, D]`` (bf16 or fp16), request ``b``'s queries in rows
@@ -151,6 +151,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Keys whose page is out of range are left out and reported, and so are requests
     from an offset on that falls. A row that sees no key is zero. ``return_lse``: also the natural log-sum-exp,
     fp32 ``[T, H]`` (softmax only). Forward only.
+
+    ``tree`` (what ``tree_tables`` returns): a request's queries are a tree of
+    drafted tokens. Each sees the keys before the tree that ``mask`` shows to its
+    position, and of the tree's itself and its ancestors, as far as the mask does not
+    put them too far back. Requests of more than 64 queries are chunks, as without.
     """
     if norm not in _NORMS or mod not in _MODS:
         raise ValueError(f"unknown norm/mod {norm!r}/{mod!r}")
@@ -172,8 +177,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     r = N.binding().attention(
         q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_q, max_q, _NORMS[norm],
         _MODS[mod], (mask.left, mask.right, mask.block, mask.prefix, mask.dilation), scale, softcap,
-        hp, sig_bias, out_scale, out, return_lse, wait_limit_ns, _status(k_cache))
+        hp, sig_bias, out_scale, out, return_lse, wait_limit_ns, _status(k_cache), tree)
     if type(r) is int:  # the message is formatted only on failure
-        N.check(r, f"chia_paged_attn(norm={norm}, mod={mod}, mask={mask}, q={tuple(q.shape)}, "
+        N.check(r, f"chia_{'paged' if tree is None else 'tree'}_attn(norm={norm}, mod={mod}, mask={mask}, q={tuple(q.shape)}, "
                    f"cache={tuple(k_cache.shape)})")
     return r

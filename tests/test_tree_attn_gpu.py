@@ -1,0 +1,330 @@
+"""paged_attention(tree=...) (chia_tree_attn of include/chia_draft.h) on the GPU against the plain 64-bit restatement
+(``draft_oracle.py``), and a whole step of speculative decoding.
+
+Tolerances, element by element, as of the attention without trees: the output is rounded once (2^-8 relative for bf16,
+2^-11 for fp16); P may be rounded to 11 significant bits before P V (2^-12 of each term, the sum of whose sizes is the
+oracle's ``mass``); exponentials, hyperbolic tangents, reciprocals and sums in fp32 stay under 2^-14 of a term for the
+scores used here (|s| < 64). 2^-8 |o| (2^-11) + 2^-10 mass + 2^-24 is allowed; a log-sum-exp is off by 2^-11 at most.
+"""
+
+import math
+
+import pytest
+import torch
+
+import chia_proj_b200 as cp
+import draft_oracle as do
+import paged_oracle as po
+
+pytestmark = pytest.mark.gpu
+E4M3, I8 = torch.float8_e4m3fn, torch.int8
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda):
+    yield
+    cp.check_device_status(0)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def make(sizes, bases, *, H=8, hkv=2, D=128, page=64, ct=E4M3, dtype=BF16, seed=0, shape="tree", q_size=1.0):
+    """Requests of sizes[b] nodes behind bases[b] keys (negative: fewer keys than nodes)."""
+    g = torch.Generator().manual_seed(seed)
+    lens = [b + n for b, n in zip(bases, sizes)]
+    cu = [sum(sizes[:i]) for i in range(len(sizes) + 1)]
+    parents = [p for i, n in enumerate(sizes) for p in do.tree(n, seed + i, shape == "chain", shape == "wide")]
+    need = [po.pages_for(n, page) for n in lens]
+    pages = sum(need) + 2
+    perm = torch.randperm(pages, generator=g).tolist()
+    width = max(max(need), 1) + 1
+    table = [perm[sum(need[:i]):sum(need[:i + 1])] + [-7] * (width - need[i]) for i in range(len(need))]
+
+    def cache():
+        x = torch.randn(pages, hkv, page, D, generator=g) * (150 if ct == E4M3 else 40)
+        x = x.clamp(-448, 448).to(ct) if ct == E4M3 else x.round().clamp(-127, 127).to(ct)
+        return x, 2.0 ** torch.randint(-9, -6, (pages, hkv), generator=g).float()
+
+    (k, ks), (v, vs) = cache(), cache()
+    q = (torch.randn(cu[-1], H, D, generator=g) * q_size).to(dtype)
+    return dict(q=q, k=k, v=v, ks=ks, vs=vs, table=table, lens=lens, cu=cu, parents=parents)
+
+
+def run(c, tree=None, **kw):
+    d = [c[n].cuda() for n in ("k", "v", "ks", "vs")]
+    lens, cu = ints(c["lens"]), ints(c["cu"])
+    if tree is None:
+        tree = cp.tree_tables(ints(c["parents"]), cu, lens)
+    return cp.paged_attention(c["q"].cuda(), *d, ints(c["table"]), lens, cu, tree=tree, **kw)
+
+
+def check(c, got, lse=None, rows=None, **kw):
+    mask = kw.pop("mask", cp.CAUSAL)
+    out, want_lse, mass = do.attention(c["q"], c["k"], c["v"], c["ks"], c["vs"], c["table"], c["lens"], c["cu"], c["parents"],
+                                       mask=mask, **kw)
+    rel = 2.0 ** -8 if c["q"].dtype == BF16 else 2.0 ** -11
+    ok = (got.double().cpu() - out).abs() <= rel * out.abs() + 2.0 ** -10 * mass + 2.0 ** -24
+    assert ok[rows].all() if rows is not None else ok.all()
+    if lse is not None:
+        l = lse.double().cpu()
+        assert torch.equal(l == -math.inf, want_lse == -math.inf)
+        assert ((l - want_lse).abs()[want_lse > -math.inf] <= 2.0 ** -11).all()
+
+
+SIZES = [13, 1, 0, 5, 30, 2]
+BASES = [100, 0, 0, 31, 257, 64]
+KINDS = [dict(), dict(mod="softcap", softcap=20.0), dict(mod="alibi"), dict(mod="temp"), dict(norm="sigmoid", sig_bias=-2.0),
+         dict(norm="relu", out_scale=0.01)]
+MASKS = [cp.CAUSAL, cp.Mask(left=6, right=0), cp.Mask(left=70, right=0), cp.Mask(right=0, block=24),
+         cp.Mask(right=0, dilation=3), cp.Mask(left=10, right=0, prefix=20), cp.FULL]
+
+
+def with_params(kw, H):
+    if kw.get("mod") in ("alibi", "temp"):
+        return {**kw, "head_param": [0.25 + 0.1 * h for h in range(H)]}
+    return kw
+
+
+# max_q 64 takes the tensor-memory kernel (rows of a K/V head from 56 on), 1 the one for few queries; both serve any tree
+@pytest.mark.parametrize("max_q", [1, 64])
+@pytest.mark.parametrize("kind", range(len(KINDS)))
+@pytest.mark.parametrize("ct,dtype,D,page", [(E4M3, BF16, 128, 64), (I8, F16, 64, 16), (E4M3, F16, 64, 32), (I8, BF16, 128, 128)])
+def test_kinds(cuda, max_q, kind, ct, dtype, D, page):
+    kw = with_params(KINDS[kind], 8)
+    c = make(SIZES, BASES, D=D, page=page, ct=ct, dtype=dtype, seed=kind)
+    check(c, run(c, max_q=max_q, **kw), **kw)
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+@pytest.mark.parametrize("mask", range(len(MASKS)))
+@pytest.mark.parametrize("kind", [0, 2])
+@pytest.mark.parametrize("page", [16, 64])
+def test_masks(cuda, max_q, mask, kind, page):
+    kw = with_params(KINDS[kind], 8)
+    c = make([13, 64, 3, 40], [50, 20, 5, 130], page=page, seed=mask)
+    if kind == 0:
+        got, lse = run(c, max_q=max_q, mask=MASKS[mask], return_lse=True, **kw)
+    else:
+        got, lse = run(c, max_q=max_q, mask=MASKS[mask], **kw), None
+    check(c, got, lse, mask=MASKS[mask], **kw)
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+@pytest.mark.parametrize("shape", ["tree", "chain", "wide"])
+@pytest.mark.parametrize("H,hkv", [(4, 4), (8, 1), (14, 2), (6, 2)])
+def test_shapes(cuda, max_q, shape, H, hkv):
+    c = make([64, 33, 1, 32, 63], [0, 31, 700, 33, 15], H=H, hkv=hkv, page=32, shape=shape, seed=H)
+    got = run(c, max_q=max_q)
+    check(c, got)
+    if shape == "chain":  # in a row they are what drafted tokens are without a tree
+        d = [c[n].cuda() for n in ("k", "v", "ks", "vs")]
+        plain = cp.paged_attention(c["q"].cuda(), *d, ints(c["table"]), ints(c["lens"]), ints(c["cu"]), max_q=max_q)
+        check(c, plain)
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_long_contexts_are_split(cuda, max_q):
+    """Units that several CTAs share, trees at the end of the last one's piece, and in pages that end inside a tile."""
+    c = make([64, 7, 25], [9000, 4099, 1], H=8, hkv=2, page=16, seed=3)
+    got, lse = run(c, max_q=max_q, return_lse=True)
+    check(c, got, lse)
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_chunks_beside_trees(cuda, max_q):
+    """A request of more than 64 queries is a chunk of a prompt."""
+    c = make([5, 65, 20, 130], [40, 10, 0, 77], seed=9)
+    check(c, run(c, max_q=max_q, mask=cp.Mask(left=50, right=0)), mask=cp.Mask(left=50, right=0))
+    check(c, run(c, max_q=max_q))
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_more_nodes_than_keys(cuda, max_q):
+    """Lengths that do not hold the tree: the first nodes have no place in the cache, and none for a first node's row."""
+    c = make([10, 6, 3], [-4, -6, 20], seed=2, shape="chain")
+    got, lse = run(c, max_q=max_q, return_lse=True)
+    check(c, got, lse)
+    assert not got[10:16].float().any()
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+@pytest.mark.parametrize("B", [513, 1100])
+def test_many_requests(cuda, max_q, B):
+    c = make([1 + i % 4 for i in range(B)], [(7 * i) % 40 for i in range(B)], H=2, hkv=1, D=64, page=16, seed=B)
+    check(c, run(c, max_q=max_q))
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+@pytest.mark.parametrize("kind", [0, 4])
+def test_nan_of_nodes_that_are_not_seen(cuda, max_q, kind):
+    """NaN values (e4m3) in a node's place reach those that see it, and nobody else; scales of places that no row sees
+    may be anything."""
+    kw = KINDS[kind]
+    c = make([20, 9], [45, 3], page=16, seed=6)
+    base, page = 45, 16
+    seen = do.paths(c["parents"][:20])
+    node = 11
+    p, o = c["table"][0][(base + node) // page], (base + node) % page
+    clean = run(c, max_q=max_q, **kw)
+    c["v"].view(torch.uint8)[p, 0, o, 3] = 0x7f
+    got = run(c, max_q=max_q, **kw)
+    hit = torch.tensor([node in s for s in seen] + [False] * 9)
+    assert hit.any() and not hit.all()
+    assert got.cpu()[hit][:, :4, 3].isnan().all()
+    keep = torch.ones_like(got, dtype=torch.bool).cpu()
+    keep[hit.nonzero().flatten(), :4, 3] = False
+    assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_bad_pages_and_offsets(cuda, max_q):
+    c = make([13, 4], [50, 30], page=16, seed=4)
+    clean = run(c, max_q=max_q)
+    c["table"][1][1] = 10 ** 6  # keys 16 .. 31 of the second request are left out
+    got = run(c, max_q=max_q)
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+    assert torch.equal(got[:13], clean[:13]) and got.isfinite().all()
+    c["table"][1][1] = 0
+    tree = cp.tree_tables(ints(c["parents"]), ints(c["cu"]), ints(c["lens"]))
+    c["cu"] = [0, 13, 12]
+    out = torch.full((17, 8, 128), 5.0, dtype=BF16, device="cuda")
+    got = run(c, tree=tree, max_q=max_q, out=out)
+    with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
+        cp.check_device_status(0)
+    check(dict(c, cu=[0, 13, 17]), got, rows=slice(0, 13))  # (fewer requests are cut into other pieces: not bit by bit)
+    assert (got[13:] == 5).all()  # rows that nobody owns stay
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_words_of_any_kind(cuda, max_q):
+    """Positions out of range and words with any bits: the result may be anything, but memory is not left, and what the
+    bits beyond the tree say is not looked at."""
+    c = make([9, 64], [20, 100], seed=12)
+    tree = cp.tree_tables(ints(c["parents"]), ints(c["cu"]), ints(c["lens"]))
+    want = run(c, tree=tree, max_q=max_q)
+    more = tree._replace(ancestors=tree.ancestors.clone())
+    more.ancestors[:9] |= -1 << 9
+    assert torch.equal(run(c, tree=more, max_q=max_q), want)
+    wild = tree._replace(positions=torch.where(tree.positions % 2 == 0, -2 ** 31, 2 ** 31 - 1).int(),
+                         ancestors=torch.full_like(tree.ancestors, -1))
+    for kw in (dict(), dict(mod="alibi"), dict(mask=cp.Mask(left=3, right=0, dilation=2))):
+        assert run(c, tree=wild, max_q=max_q, **kw).shape == want.shape
+    only = torch.arange(9).tolist() + torch.arange(64).tolist()  # nodes that see themselves and the context alone
+    alone = tree._replace(ancestors=torch.tensor([1 << i if i < 63 else -2 ** 63 for i in only], device="cuda"),
+                          positions=ints([20] * 9 + [100] * 64))
+    check(dict(c, parents=[-1] * 73), run(c, tree=alone, max_q=max_q))
+
+
+def test_refusals(cuda):
+    c = make([4, 3], [10, 20], seed=1)
+    tree = cp.tree_tables(ints(c["parents"]), ints(c["cu"]), ints(c["lens"]))
+    for bad in (tree.positions, (tree.positions,), tree._replace(positions=tree.positions[:5]),
+                tree._replace(positions=tree.ancestors), tree._replace(ancestors=tree.positions),
+                tree._replace(ancestors=tree.ancestors[:-1]), tree._replace(ancestors=tree.ancestors.repeat(2)[::2]),
+                tree._replace(ancestors=tree.ancestors.cpu())):
+        with pytest.raises((ValueError, RuntimeError)):
+            run(c, tree=bad)
+
+
+def test_streams_and_graphs(cuda):
+    """Two streams at once, and a captured step that is replayed on new trees."""
+    c = make([13, 40, 2], [300, 20, 0], seed=8)
+    d = [c[n].cuda() for n in ("k", "v", "ks", "vs")]
+    q, table, lens, cu, parents = c["q"].cuda(), ints(c["table"]), ints(c["lens"]), ints(c["cu"]), ints(c["parents"])
+
+    def step():
+        tree = cp.tree_tables(parents, cu, lens)
+        return [cp.paged_attention(q, *d, table, lens, cu, max_q=m, tree=tree) for m in (1, 64)]
+
+    want = step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append([step() for _ in range(3)])
+    torch.cuda.synchronize()
+    for runs in got:
+        for r in runs:
+            assert torch.equal(r[0], want[0]) and torch.equal(r[1], want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    other = [p for i, n in enumerate([13, 40, 2]) for p in do.tree(n, 77 + i)]
+    parents.copy_(ints(other))
+    lens.copy_(ints([250, 60, 2]))
+    graph.replay()
+    again = step()
+    assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
+    check(dict(c, parents=other, lens=[250, 60, 2]), out[0])
+
+
+@pytest.mark.parametrize("ct,page,dtype", [(E4M3, 16, BF16), (I8, 64, F16)])
+def test_steps_of_speculative_decoding(cuda, ct, page, dtype):
+    """Three steps of all operators together. After each, the pages that requests hold and the free ones are all there
+    is; the cache holds what appending the accepted tokens alone would have left, to the cache's precision."""
+    H, hkv, D, V, B, pages = 4, 2, 64, 300, 5, 60
+    g = torch.Generator().manual_seed(page)
+    cache = cp.new_cache(pages, hkv, D, page_size=page, dtype=ct)
+    table, ring = ints([[0] * 12] * B), torch.arange(pages, dtype=torch.int32, device="cuda")
+    state, lens = ints([0, pages]), ints([0] * B)
+    freqs = cp.rope_frequencies(D)
+    qw, kw = (torch.ones(D, dtype=dtype, device="cuda") for _ in range(2))
+    known = [[] for _ in range(B)]  # K and V of each request's tokens, normed and turned, in 16 bits
+    for it, sizes in enumerate([[64, 1, 20, 0, 33], [13, 25, 7, 9, 1], [30, 30, 30, 30, 30]]):
+        T = sum(sizes)
+        cu = [sum(sizes[:i]) for i in range(B + 1)]
+        parents = [p for i, n in enumerate(sizes) for p in do.tree(n, 10 * it + i)]
+        qkv = torch.randn(T, H + 2 * hkv, D, generator=g).to(dtype).cuda()
+        q, k, v = qkv.split([H, hkv, hkv], 1)
+        st = cp.page_tables(lens, ints(sizes), table, ring, state, page_size=page, max_tokens=T)
+        tree = cp.tree_tables(ints(parents), st.cu_q, st.seq_lens)
+        q, k = cp.qk_norm_rope(q, k, qw, kw, freqs, tree.positions)
+        cp.cache_append(k, v, st.slots, *cache)
+        got = cp.paged_attention(q, *cache, table, st.seq_lens, st.cu_q, max_q=max(sizes), tree=tree)
+        c = dict(q=q.cpu(), k=cache[0].cpu(), v=cache[1].cpu(), ks=cache[2].cpu(), vs=cache[3].cpu(), table=table.tolist(),
+                 lens=st.seq_lens.tolist(), cu=cu, parents=parents)
+        assert st.cu_q.tolist() == cu
+        check(c, got)
+        p = torch.softmax(2 * torch.randn(T, V, generator=g), 1)
+        d = torch.softmax(p.log() + 0.3 * torch.randn(T, V, generator=g), 1)
+        tokens, u = [0] * T, torch.rand(T, generator=g)
+        for b in range(B):
+            left = {}
+            for i in range(sizes[b]):
+                up = parents[cu[b] + i]
+                if up >= 0:
+                    row = left.setdefault(up, d[cu[b] + up].clone())
+                    tokens[cu[b] + i] = int(torch.multinomial(row, 1, generator=g))
+                    row[tokens[cu[b] + i]] = 0
+        done = cp.verify_drafts(p.cuda(), ints(tokens), ints(parents), st.cu_q, u.cuda(), draft_probs=d.cuda(), max_tokens=9)
+        counts, toks, path = do.verify(p, tokens, parents, cu, u, d, 9)
+        assert done.counts.tolist() == counts and done.tokens.tolist() == toks and done.path.tolist() == path
+        keep = cp.cache_compact(done.path, done.counts, st.cu_q, st.seq_lens, table, *cache)
+        before = lens.tolist()
+        assert keep.tolist() == [n + m for n, m in zip(before, counts)]
+        lens, state = cp.release_pages(None, st.seq_lens, table, ring, st.free_state, page_size=page, keep_lens=keep)
+        assert lens.tolist() == keep.tolist()
+        held = [x for b in range(B) for x in table[b, :po.pages_for(int(lens[b]), page)].tolist()]
+        first, count = state.tolist()
+        free = [int(ring[(first + i) % pages]) for i in range(count)]
+        assert sorted(held + free) == list(range(pages))
+        for b in range(B):
+            rows = [cu[b] + x for x in path[b][:counts[b]]]
+            known[b] += [(k[r].double().cpu(), v[r].double().cpu()) for r in rows]
+            if not known[b]:
+                continue
+            at = torch.arange(len(known[b]))
+            pg = table[b].cpu()[at // page].long()
+            for x, (codes, scale) in enumerate(((cache[0], cache[2]), (cache[1], cache[3]))):
+                s = scale.double().cpu()[pg][:, :, None]  # [n, heads, 1]
+                have = codes.double().cpu()[pg, :, at % page] * s
+                want = torch.stack([kv[x] for kv in known[b]])
+                # each of up to four roundings (appended, expressed in a larger scale, moved, expressed again) is off by
+                # half a step: int8 0.5 of the scale; e4m3 2^-4 of the value, or 2^-10 of the scale where it is subnormal
+                step = 0.5 * s if ct == I8 else torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10)
+                assert ((have - want).abs() <= 4.6 * step).all()
