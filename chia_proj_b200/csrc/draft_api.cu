@@ -26,11 +26,19 @@ int device_sms(int &sms) {
 
 int launched(cudaError_t e) { return e == cudaSuccess ? CHIA_OK : CHIA_ERR_LAUNCH; }
 
+// vec: rows are aligned so that four entries are one load
 template <int T>
-int launch_verify(const chia::VerifyArgs &a, cudaStream_t s) {
+int launch_verify(const chia::VerifyArgs &a, bool vec, int sms, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * chia::kVerifyCtas);
-  cfg.blockDim = dim3(chia::kVerifyThreads);
+  // A warp for each chunk of a CTA, but no more threads than the GPU holds at once (1024 an SM):
+  // a request alone waits for one round of loads, a full batch runs side by side.
+  int threads = 128;
+  const int chunks = (a.chunks + chia::kVerifyCtas - 1) / chia::kVerifyCtas;
+  while (threads < chia::kVerifyMostThreads && threads < 32 * chunks &&
+         2ll * threads * chia::kVerifyCtas * a.batch <= 1024ll * sms)
+    threads *= 2;
+  cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -39,8 +47,9 @@ int launch_verify(const chia::VerifyArgs &a, cudaStream_t s) {
   at[1].val.clusterDim.x = chia::kVerifyCtas, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return launched(a.q != nullptr ? cudaLaunchKernelEx(&cfg, chia::verify_kernel<T, true>, a)
-                                 : cudaLaunchKernelEx(&cfg, chia::verify_kernel<T, false>, a));
+  auto run = [&](void (*kernel)(chia::VerifyArgs)) { return launched(cudaLaunchKernelEx(&cfg, kernel, a)); };
+  if (a.q != nullptr) return vec ? run(chia::verify_kernel<T, true, true>) : run(chia::verify_kernel<T, true, false>);
+  return vec ? run(chia::verify_kernel<T, false, true>) : run(chia::verify_kernel<T, false, false>);
 }
 
 }  // namespace
@@ -112,9 +121,12 @@ int chia_verify_drafts(const chia_verify_params_t *p, void *stream) {
   a.vocab = static_cast<int32_t>(p->vocab);
   a.most = static_cast<int32_t>(p->max_tokens);
   a.chunks = static_cast<int32_t>((p->vocab + chia::kVerifyChunk - 1) / chia::kVerifyChunk);
+  const bool vec = aligned(p->target_probs, 4 * size) && p->target_stride % 4 == 0 &&
+                   (!p->draft_probs || (aligned(p->draft_probs, 4 * size) && p->draft_stride % 4 == 0));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return p->dtype == CHIA_DTYPE_BF16 ? launch_verify<0>(a, s) : p->dtype == CHIA_DTYPE_F16 ? launch_verify<1>(a, s)
-                                                                                          : launch_verify<2>(a, s);
+  return p->dtype == CHIA_DTYPE_BF16  ? launch_verify<0>(a, vec, sms, s)
+         : p->dtype == CHIA_DTYPE_F16 ? launch_verify<1>(a, vec, sms, s)
+                                      : launch_verify<2>(a, vec, sms, s);
 }
 
 int chia_cache_compact(const chia_compact_params_t *p, void *stream) {

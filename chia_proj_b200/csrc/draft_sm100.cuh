@@ -102,18 +102,52 @@ struct VerifyArgs {
   int32_t batch, rows, vocab, most, chunks;  // chunks: of kVerifyChunk entries, in all
 };
 
-constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyMostThreads = 1024;
 constexpr int kVerifyCtas = 8;  // of a request: a cluster
 constexpr int kVerifyChunk = 512;  // entries that a warp sums at a time
 constexpr int kVerifyMostChunks = 1024;  // of a CTA
 
-// an entry; one that is no positive finite number is 0
-__device__ __forceinline__ float verify_clean(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+// An entry; one that is no positive finite number is 0 (its bits are none of those up to infinity's).
+__device__ __forceinline__ float verify_clean(float x) {
+  return __float_as_uint(x) < 0x7f800000u ? x : 0.f;
+}
 template <int T>
 __device__ __forceinline__ float verify_one(const void *p, int64_t e) {
   if (T == 2) return verify_clean(static_cast<const float *>(p)[e]);
   const uint32_t v = static_cast<const uint16_t *>(p)[e];
   return verify_clean(T == 0 ? in16x2_to_float2<true>(v).x : in16x2_to_float2<false>(v).x);
+}
+
+// Four entries from v on, of a row whose first one is e (VEC: rows are aligned for it); behind the
+// row's end there are zeros.
+template <int T, bool VEC>
+__device__ __forceinline__ void verify_four(const void *p, int64_t e, int v, int vocab, float (&x)[4]) {
+  if (VEC && v + 4 <= vocab) {
+    if (T == 2) {
+      const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + e + v);
+      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + e + v);
+      const float2 a = in16x2_to_float2<T == 0>(w.x), b = in16x2_to_float2<T == 0>(w.y);
+      x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = 0.f;
+      if (v + i < vocab) {
+        if (T == 2)
+          x[i] = static_cast<const float *>(p)[e + v + i];
+        else
+          x[i] = in16x2_to_float2<T == 0>(static_cast<const uint16_t *>(p)[e + v + i]).x;
+      }
+    }
+  }
+}
+
+template <int T>
+__device__ __forceinline__ void verify_prefetch(const void *p, int64_t e) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t *>(p) + e * (T == 2 ? 4 : 2)));
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -142,25 +176,28 @@ __device__ __forceinline__ double shfl_up(double x, int d) { return __shfl_up_sy
 // in the order of the vocabulary, so the drawn token is found from the last pass's sums
 // and one chunk that is read again. Without draft rows the mass is 1 minus what was
 // rejected, and the only pass is the last. All CTAs walk alike.
-template <int T, bool DRAFTS>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
+template <int T, bool DRAFTS, bool VEC>
+__global__ void __launch_bounds__(kVerifyMostThreads, 1) verify_kernel(const VerifyArgs a) {
   __shared__ double s_sum[kVerifyMostChunks];  // of this CTA's chunks
   __shared__ double s_total[2][kVerifyCtas];   // of each CTA, two passes by turns
   __shared__ float s_p[kTreeNodes], s_q[kTreeNodes], s_u[kTreeNodes];
   __shared__ int s_parent[kTreeNodes], s_token[kTreeNodes];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = cluster_rank(), b = blockIdx.x / kVerifyCtas;
+  __shared__ double s_warp[kVerifyMostThreads / 32];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x / 32;
+  const int rank = cluster_rank(), b = blockIdx.x / kVerifyCtas;
   follow();
   TreeRows r = tree_rows(a.cu_q, b, a.rows);
   bool bad = r.n < 0 || r.n > kTreeNodes;
   int32_t *out = a.out + static_cast<int64_t>(b) * a.most, *path = a.path + static_cast<int64_t>(b) * a.most;
   if (r.n == 0 || bad) {
     if (rank == 0) {
-      for (int i = t; i < a.most; i += kVerifyThreads) out[i] = path[i] = -1;
+      for (int i = t; i < a.most; i += blockDim.x) out[i] = path[i] = -1;
       if (t == 0) a.counts[b] = 0;
       if (t == 0 && bad) report(a.status, kStatusBadIndex);
     }
     return;  // (all CTAs of the cluster do)
   }
+  const int per = (a.chunks + kVerifyCtas - 1) / kVerifyCtas;  // chunks of a CTA
   if (t < r.n) {
     const int x = a.tokens[r.t0 + t];
     int p = a.parents[r.t0 + t];
@@ -173,6 +210,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       p = -1;
     }
     s_parent[t] = p, s_token[t] = x;
+    // (the rows are far apart: their first access waits for an address translation too)
+    const int64_t slice = min(static_cast<int64_t>(a.vocab) - 1, static_cast<int64_t>(rank) * per * kVerifyChunk);
+    verify_prefetch<T>(a.p, (r.t0 + t) * a.p_st + slice);
+    if (DRAFTS) verify_prefetch<T>(a.q, (r.t0 + t) * a.q_st + slice);
     if (p >= 0) {
       s_p[t] = verify_one<T>(a.p, (r.t0 + p) * a.p_st + x);
       if (DRAFTS) s_q[t] = verify_one<T>(a.q, (r.t0 + p) * a.q_st + x);
@@ -183,32 +224,89 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
 
   // Sums of the residual at `node`; returns the mass, the same in all CTAs.
   int turn = 0;
-  const int per = (a.chunks + kVerifyCtas - 1) / kVerifyCtas, c0 = rank * per, mine = max(0, min(per, a.chunks - c0));
+  const int c0 = rank * per, mine = max(0, min(per, a.chunks - c0));
   unsigned long long dropped = 0;  // (without draft rows) rejected children of the node
-  auto entry = [&](int node, double F, int v) {
-    if (v >= a.vocab) return 0.0;
-    double x = verify_one<T>(a.p, (r.t0 + node) * a.p_st + v);
-    if (DRAFTS && F != 0.0) x = fmax(fma(-F, static_cast<double>(verify_one<T>(a.q, (r.t0 + node) * a.q_st + v)), x), 0.0);
+  // four entries of the residual, from the rows'
+  auto residual = [&](double F, const float (&p)[4], const float (&q)[4], double (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = verify_clean(p[i]);
+      if (DRAFTS) {
+        x[i] = fma(-F, static_cast<double>(verify_clean(q[i])), x[i]);
+        if (__double2hiint(x[i]) < 0) x[i] = 0.0;
+      }
+    }
+  };
+  // without draft rows: rejected tokens among the chunk's (few chunks have any)
+  auto drop = [&](int c, int v, double (&x)[4]) {
+    for (unsigned long long m = dropped; m != 0; m &= m - 1) {
+      const int at = s_token[__ffsll(m) - 1];
+      if (at / kVerifyChunk != c) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v + i == at) x[i] = 0.0;
+    }
+  };
+  auto has_dropped = [&](int c) {
+    bool any = false;
     if (!DRAFTS)
-      for (unsigned long long m = dropped; m != 0; m &= m - 1)
-        if (s_token[__ffsll(m) - 1] == v) x = 0.0;
+      for (unsigned long long m = dropped; m != 0; m &= m - 1) any |= s_token[__ffsll(m) - 1] / kVerifyChunk == c;
+    return any;
+  };
+  auto chunk_sum = [&](int64_t pe, int64_t qe, double F, int c) {  // this lane's part of it
+    constexpr int N = kVerifyChunk / 128;
+    float p[N][4], q[N][4];
+    const int v0 = (c0 + c) * kVerifyChunk + 4 * lane;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) verify_four<T, VEC>(a.p, pe, v0 + 128 * i, a.vocab, p[i]);  // (all loads at once)
+    if (DRAFTS && F != 0.0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) verify_four<T, VEC>(a.q, qe, v0 + 128 * i, a.vocab, q[i]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        double x[4];
+        residual(F, p[i], q[i], x);
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
+      }
+    } else {  // nothing was rejected, or there is no draft row
+      const bool dropping = has_dropped(c0 + c);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        double x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = verify_clean(p[i][e]);
+        if (dropping) drop(c0 + c, v0 + 128 * i, x);
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
+      }
+    }
+    return sum;
+  };
+  auto warp_sum = [&](double x) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
     return x;
   };
-  auto mass = [&](int node, double F) {
-    for (int c = warp; c < mine; c += kVerifyWarps) {
-      double sum = 0.0;
-#pragma unroll 4
-      for (int i = 0; i < kVerifyChunk / 32; ++i) sum += entry(node, F, (c0 + c) * kVerifyChunk + 32 * i + lane);
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == 0) s_sum[c] = sum;
+  // `last`: the sums of chunks are kept (a mass that a sibling waits for is never the last)
+  auto mass = [&](int node, double F, bool last) {
+    const int64_t pe = (r.t0 + node) * a.p_st, qe = (r.t0 + node) * a.q_st;
+    double sum = 0.0;
+#pragma unroll 1
+    for (int c = warp; c < mine; c += warps) {
+      const double x = chunk_sum(pe, qe, F, c);
+      if (last) {
+        const double all = warp_sum(x);
+        if (lane == 0) s_sum[c] = all;
+        sum += all;
+      } else {
+        sum += x;
+      }
     }
+    if (!last) sum = warp_sum(sum);
+    if (lane == 0) s_warp[warp] = sum;
     __syncthreads();
     if (warp == 0) {
-      double sum = 0.0;
-      for (int c = lane; c < mine; c += 32) sum += s_sum[c];
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      sum = warp_sum(lane < warps ? s_warp[lane] : 0.0);
       if (lane < kVerifyCtas) cluster_store(&s_total[turn][rank], lane, sum);
     }
     cluster_sync();
@@ -229,7 +327,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     bool yes;
     if (DRAFTS) {
       const double q = s_q[i];
-      if (!known) Z = mass(node, F), known = true;
+      if (!known) Z = mass(node, F, false), known = true;
       double here = fmax(fma(-F, q, p), 0.0), qx = q;
       // (a token that an earlier sibling had is in neither)
       for (int j = node + 1; j < i; ++j)
@@ -254,8 +352,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   }
 
   // the token behind the last accepted node
-  Z = mass(node, F);
-  if (!(Z > 0.0)) F = 0.0, dropped = 0, Z = mass(node, F);
+  Z = mass(node, F, true);
+  if (!(Z > 0.0)) F = 0.0, dropped = 0, Z = mass(node, F, true);
   const double *total = s_total[turn ^ 1];
   const double target = static_cast<double>(s_u[0]) * Z;
   // the CTA whose chunks hold the place, or the last that holds anything
@@ -267,7 +365,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     sum += total[x];
   }
   if (rank == 0) {
-    for (int i = count + t; i < a.most; i += kVerifyThreads) out[i] = path[i] = -1;
+    for (int i = count + t; i < a.most; i += blockDim.x) out[i] = path[i] = -1;
     if (t == 0) {
       a.counts[b] = count;
       if (owner < 0) out[count - 1] = -1;
@@ -295,26 +393,49 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
       if (over != 0) break;
       base += __shfl_sync(0xffffffffu, inc, 31);
     }
-    // the entry likewise
-    int found = -1;
-    base = in;
-    for (int i = 0; i < kVerifyChunk / 32 && chunk >= 0; ++i) {
-      const int v = (c0 + chunk) * kVerifyChunk + 32 * i + lane;
-      const double own = entry(node, F, v);
+    // the lane likewise, 16 entries each, and the entry
+    if (chunk >= 0) {
+      constexpr int N = kVerifyChunk / 128;
+      const int64_t pe = (r.t0 + node) * a.p_st, qe = (r.t0 + node) * a.q_st;
+      const int v0 = (c0 + chunk) * kVerifyChunk + 4 * N * lane;
+      double x[N][4], own = 0.0;
+      {
+        float p[N][4], q[N][4];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          verify_four<T, VEC>(a.p, pe, v0 + 4 * i, a.vocab, p[i]);
+          if (DRAFTS) verify_four<T, VEC>(a.q, qe, v0 + 4 * i, a.vocab, q[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          residual(F, p[i], q[i], x[i]);
+          if (!DRAFTS) drop(c0 + chunk, v0 + 4 * i, x[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) own += x[i][e];
+        }
+      }
       double inc = own;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const double y = shfl_up(inc, d);
         if (lane >= d) inc += y;
       }
-      const unsigned over = __ballot_sync(0xffffffffu, own > 0.0 && base + inc > target);
+      const unsigned over = __ballot_sync(0xffffffffu, own > 0.0 && in + inc > target);
       const unsigned some = __ballot_sync(0xffffffffu, own > 0.0);
-      const int pick = over != 0 ? __ffs(over) - 1 : some != 0 ? 31 - __clz(some) : -1;
-      if (pick >= 0) found = v - lane + pick;
-      if (over != 0) break;
-      base += __shfl_sync(0xffffffffu, inc, 31);
+      if (lane == (over != 0 ? __ffs(over) - 1 : 31 - __clz(some))) {
+        int found = -1;
+        double sum = in + (inc - own);
+        bool done = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sum += x[i][e];
+            if (!done && x[i][e] > 0.0) found = v0 + 4 * i + e, done = sum > target;
+          }
+        out[count - 1] = found;
+      }
     }
-    if (lane == 0) out[count - 1] = found;
   }
 }
 
