@@ -269,7 +269,9 @@ struct Rope {
       throw ValueError(std::string(name) + " must be bf16, fp16 or fp32 (" + std::to_string(q.d) + ",) on " + dev.str() + ", got " +
                        c10::toString(w.scalar_type()) + " " + str(w.sizes()) + " on " + w.device().str());
     no_tangent(w, name);
-    to = w.is_contiguous() ? w : w.detach().contiguous();
+    to = w.is_contiguous() && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0
+             ? w
+             : w.detach().clone(at::MemoryFormat::Contiguous);
   }
 };
 

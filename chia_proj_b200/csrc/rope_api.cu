@@ -47,9 +47,8 @@ int check(const chia_rope_params_t *p, bool outputs) {
   if (!std::isfinite(p->eps) || p->eps < 0.f || !std::isfinite(p->weight_offset)) return CHIA_ERR_INVALID_ARGUMENT;
   if (p->rot > 0 && p->freqs == nullptr) return CHIA_ERR_INVALID_ARGUMENT;
   if (p->seqlen > 0 && (!p->q || !p->k || (outputs && (!p->q_out || !p->k_out)))) return CHIA_ERR_INVALID_ARGUMENT;
-  const unsigned w = p->weight_dtype == CHIA_DTYPE_F32 ? 4 : 2;
   if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->q_out, 16) || !aligned(p->k_out, 16) ||
-      !aligned(p->q_weight, w) || !aligned(p->k_weight, w) || !aligned(p->freqs, 8) || !aligned(p->positions, 4))
+      !aligned(p->q_weight, 16) || !aligned(p->k_weight, 16) || !aligned(p->freqs, 8) || !aligned(p->positions, 4))
     return CHIA_ERR_MISALIGNED;
   for (const int64_t *s : {p->q_stride, p->k_stride, p->q_out_stride, p->k_out_stride}) {
     const int rc = check_strides(s);
@@ -60,7 +59,6 @@ int check(const chia_rope_params_t *p, bool outputs) {
 
 void set_side(chia::RopeSide &d, const void *x, void *y, const void *w, int heads, const int64_t *xs, const int64_t *ys) {
   d.x = x, d.y = y, d.w = w, d.heads = heads;
-  d.magic = heads == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads);
   for (int i = 0; i < 3; ++i) d.x_st[i] = xs[i], d.y_st[i] = ys[i];
 }
 
@@ -78,35 +76,36 @@ void set_args(const chia_rope_params_t *p, chia::RopeArgs &a) {
   a.w_offset = p->weight_offset;
 }
 
-// Tokens of a CTA: as many fewer than kRopeTokens as give every SM four CTAs.
-int tokens_per_cta(int64_t tokens, int sms) {
-  int n = chia::kRopeTokens;
-  while (n > 1 && (tokens + n - 1) / n < 4 * sms) n /= 2;
-  return n;
+// Groups that share a token: as many as make kTasks pieces of work for the GPU, a head at least
+// to each.
+constexpr int64_t kTasks = 32768;
+// CTAs of the backward kernel, an SM: its groups go on from token to token and leave one sum of
+// the weights' gradients a CTA.
+constexpr int kBwdCtas = 4;
+int set_grid(chia::RopeArgs &a, int dim, bool back, int sms) {
+  const int heads = a.side[0].heads > a.side[1].heads ? a.side[0].heads : a.side[1].heads;
+  a.part_bits = 0;
+  while ((2 << a.part_bits) <= heads && (static_cast<int64_t>(a.tokens) << a.part_bits) < kTasks) ++a.part_bits;
+  const int groups = chia::kRopeThreads / (dim / 8);
+  const int64_t ctas = ((static_cast<int64_t>(a.tokens) << a.part_bits) + groups - 1) / groups;
+  const int64_t most = back ? static_cast<int64_t>(kBwdCtas) * sms : kI32;
+  return static_cast<int>(ctas < most ? ctas : most);
 }
 
-// CTAs of the backward kernel: each goes on over blocks of tokens and leaves its sums of
-// the weights' gradients.
-constexpr int kBwdCtas = 4;  // an SM
-int bwd_grid(int64_t tokens, int per_cta, int sms) {
-  const int64_t n = (tokens + per_cta - 1) / per_cta;
-  return static_cast<int>(n < kBwdCtas * sms ? n : kBwdCtas * sms);
-}
-
-template <int T, int D>
-int launch_fwd(const chia::RopeArgs &a, bool inter, cudaStream_t s) {
-  const dim3 grid((a.tokens + a.per_cta - 1) / a.per_cta);
+template <int T, int D, bool BACK>
+int launch(const chia::RopeArgs &a, bool inter, int grid, cudaStream_t s) {
   const cudaError_t e =
-      inter ? chia::launch_after(chia::qk_norm_rope_kernel<T, D, true>, grid, chia::kRopeThreads, 0, s, a)
-            : chia::launch_after(chia::qk_norm_rope_kernel<T, D, false>, grid, chia::kRopeThreads, 0, s, a);
+      inter ? chia::launch_after(chia::qk_norm_rope_kernel<T, D, true, BACK>, dim3(grid), chia::kRopeThreads, 0, s, a)
+            : chia::launch_after(chia::qk_norm_rope_kernel<T, D, false, BACK>, dim3(grid), chia::kRopeThreads, 0, s, a);
   return e == cudaSuccess ? CHIA_OK : CHIA_ERR_LAUNCH;
+}
+template <int T, int D>
+int launch_fwd(const chia::RopeArgs &a, bool inter, int grid, cudaStream_t s) {
+  return launch<T, D, false>(a, inter, grid, s);
 }
 template <int T, int D>
 int launch_bwd(const chia::RopeArgs &a, bool inter, int grid, cudaStream_t s) {
-  const cudaError_t e =
-      inter ? chia::launch_after(chia::qk_norm_rope_bwd_kernel<T, D, true>, dim3(grid), chia::kRopeThreads, 0, s, a)
-            : chia::launch_after(chia::qk_norm_rope_bwd_kernel<T, D, false>, dim3(grid), chia::kRopeThreads, 0, s, a);
-  return e == cudaSuccess ? CHIA_OK : CHIA_ERR_LAUNCH;
+  return launch<T, D, true>(a, inter, grid, s);
 }
 #define CHIA_ROPE_BY_TYPE(p, FN, ...)                                                             \
   ((p)->head_dim == 128 ? ((p)->dtype == CHIA_DTYPE_BF16  ? FN<chia::ROPE_BF16, 128>(__VA_ARGS__) \
@@ -126,8 +125,8 @@ int chia_qk_norm_rope(const chia_rope_params_t *p, void *stream) {
   if (p->seqlen == 0) return CHIA_OK;
   chia::RopeArgs a{};
   set_args(p, a);
-  a.per_cta = tokens_per_cta(a.tokens, sms);
-  return CHIA_ROPE_BY_TYPE(p, launch_fwd, a, p->interleaved != 0, static_cast<cudaStream_t>(stream));
+  const int grid = set_grid(a, p->head_dim, false, sms);
+  return CHIA_ROPE_BY_TYPE(p, launch_fwd, a, p->interleaved != 0, grid, static_cast<cudaStream_t>(stream));
 }
 
 int64_t chia_qk_norm_rope_bwd_workspace_bytes(const chia_rope_params_t *p) {
@@ -163,8 +162,7 @@ int chia_qk_norm_rope_bwd(const chia_rope_params_t *p, const chia_rope_grads_t *
   a.side[0].dy = g->dq_out, a.side[1].dy = g->dk_out;
   for (int i = 0; i < 3; ++i) a.side[0].dy_st[i] = g->dq_out_stride[i], a.side[1].dy_st[i] = g->dk_out_stride[i];
   a.partial = static_cast<float *>(workspace);
-  a.per_cta = tokens_per_cta(a.tokens, sms);
-  const int grid = bwd_grid(a.tokens, a.per_cta, sms);
+  const int grid = set_grid(a, p->head_dim, true, sms);
   if (grid > 0) {
     rc = CHIA_ROPE_BY_TYPE(p, launch_bwd, a, p->interleaved != 0, grid, s);
     if (rc != CHIA_OK) return rc;

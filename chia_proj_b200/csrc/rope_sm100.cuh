@@ -5,13 +5,16 @@
 // eight channels a lane as four pairs that turn together: channels 4 l .. + 3 and
 // those rot / 2 on, or (interleaved, and the channels that do not turn) 8 l .. + 7.
 // So the rotation needs no exchange, and a lane's angles are pairs 4 l .. + 3 in
-// either layout. A CTA takes a few tokens with all their heads: their angles' sines
-// and cosines are computed once.
+// either layout. A group stays with a token and goes over its heads (or each `parts`-th
+// of them): its angles and their products with the weights are computed once, in
+// registers, and the next row is a stride away. Groups have nothing in common, so there
+// is no barrier.
 //
 // An angle is pos * freq, in turns a product of whole numbers modulo 2^64, so the
-// reduction is exact for any position; its upper 32 bits go to sincospi.
+// reduction is exact for any position; of its upper 32 bits sine and cosine are computed.
 //
-// Sums are in 32 bits; the output is rounded once. Bound by HBM.
+// Sums are in 32 bits; the output is rounded once. Bound by HBM, and next to it by the
+// number of instructions.
 #pragma once
 #include "paged_common.cuh"
 
@@ -25,21 +28,19 @@ struct RopeSide {  // queries or keys
   const void *w;
   int64_t x_st[3], y_st[3], dy_st[3];  // element strides: batch, head, token
   int32_t heads;
-  uint32_t magic;  // ceil(2^32 / heads); 0: one head
 };
 struct RopeArgs {
   RopeSide side[2];
   const uint64_t *freqs;
   const int32_t *positions;
   int64_t pos_stride;
-  int32_t tokens, seqlen, rot, per_cta;  // tokens: of all batch entries
+  int32_t tokens, seqlen, rot, part_bits;  // tokens: of all batch entries; 2^part_bits groups share a token
   int32_t w_type;
   float eps, w_offset;
   float *partial;  // backward: [CTAs][2][D] sums of the weights' gradients
 };
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeTokens = 8;  // most tokens of a CTA at a time
+constexpr int kRopeThreads = 128;
 
 template <int T>
 struct RopeRaw {  // four channels
@@ -54,87 +55,105 @@ __device__ __forceinline__ const typename RopeRaw<T>::type *rope_at(const void *
   return reinterpret_cast<const typename RopeRaw<T>::type *>(static_cast<const uint8_t *>(p) +
                                                              e * (T == ROPE_F32 ? 4 : 2));
 }
-template <int T>
-__device__ __forceinline__ float4 rope_values(const typename RopeRaw<T>::type &r) {
-  if constexpr (T == ROPE_F32) {
-    return make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w));
-  } else {
-    const float2 a = in16x2_to_float2<T == ROPE_BF16>(r.x), b = in16x2_to_float2<T == ROPE_BF16>(r.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-  }
-}
-template <int T>
-__device__ __forceinline__ void rope_store(void *p, int64_t e, const float *v) {
-  auto *dst = const_cast<typename RopeRaw<T>::type *>(rope_at<T>(p, e));
-  if constexpr (T == ROPE_F32)
-    *dst = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  else if constexpr (T == ROPE_BF16)
-    *dst = make_uint2(ptx::pack_bf16(v[0], v[1]), ptx::pack_bf16(v[2], v[3]));
-  else
-    *dst = make_uint2(ptx::pack_f16(v[0], v[1]), ptx::pack_f16(v[2], v[3]));
-}
-__device__ __forceinline__ float rope_weight(const void *w, int type, int c) {
-  if (type == ROPE_F32) return static_cast<const float *>(w)[c];
-  const uint32_t v = static_cast<const uint16_t *>(w)[c];
-  return type == ROPE_BF16 ? in16x2_to_float2<true>(v).x : in16x2_to_float2<false>(v).x;
-}
-
-// What both directions begin with: the angles of tokens [t0, t0 + n), where their rows are.
-template <int D>
-struct RopeShared {
-  float cos[kRopeTokens][D / 2], sin[kRopeTokens][D / 2];
-  int64_t x_at[2][kRopeTokens], y_at[2][kRopeTokens], dy_at[2][kRopeTokens];
+// A lane's eight channels as four pairs (a_i, b_i), two to a register pair: packed
+// arithmetic takes half the instructions, which are what bounds these kernels next to HBM.
+struct RopeVals {
+  uint64_t a[2], b[2];
 };
-template <int D, bool BACK>
-__device__ __forceinline__ void rope_tokens(const RopeArgs &a, RopeShared<D> &s, int t0, int n) {
-  for (int e = threadIdx.x; e < n * (D / 2); e += kRopeThreads) {
-    const int j = e / (D / 2), i = e % (D / 2), t = t0 + j;
-    float c = 1.f, sn = 0.f;
-    if (i < a.rot / 2) {
-      const int b = t / a.seqlen, at = t - b * a.seqlen;
-      const int pos = a.positions != nullptr ? a.positions[b * a.pos_stride + at] : at;
-      const uint64_t turn = static_cast<uint64_t>(static_cast<int64_t>(pos)) * a.freqs[i];
-      // the upper 32 bits as -1/2 .. 1/2 of a turn, in half turns
-      sincospif(static_cast<float>(static_cast<int32_t>(turn >> 32)) * 0x1p-31f, &sn, &c);
+// INTER: the channels are a0 b0 a1 b1 .., otherwise the first four and the second four
+template <bool INTER>
+__device__ __forceinline__ RopeVals rope_pairs(const float (&x)[8]) {
+  if (INTER) return {{ptx::f2(x[0], x[2]), ptx::f2(x[4], x[6])}, {ptx::f2(x[1], x[3]), ptx::f2(x[5], x[7])}};
+  return {{ptx::f2(x[0], x[1]), ptx::f2(x[2], x[3])}, {ptx::f2(x[4], x[5]), ptx::f2(x[6], x[7])}};
+}
+template <int T, bool INTER>
+__device__ __forceinline__ RopeVals rope_values(const typename RopeRaw<T>::type (&r)[2]) {
+  float x[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (T == ROPE_F32) {
+      x[4 * h] = __uint_as_float(r[h].x), x[4 * h + 1] = __uint_as_float(r[h].y);
+      x[4 * h + 2] = __uint_as_float(r[h].z), x[4 * h + 3] = __uint_as_float(r[h].w);
+    } else {
+      const float2 f = in16x2_to_float2<T == ROPE_BF16>(r[h].x), g = in16x2_to_float2<T == ROPE_BF16>(r[h].y);
+      x[4 * h] = f.x, x[4 * h + 1] = f.y, x[4 * h + 2] = g.x, x[4 * h + 3] = g.y;
     }
-    s.cos[j][i] = c, s.sin[j][i] = sn;
   }
-  if (threadIdx.x < 2 * n) {
-    const int j = threadIdx.x >> 1, t = t0 + j;
-    const int64_t b = t / a.seqlen, at = t - b * a.seqlen;
-    const int k = threadIdx.x & 1;
-    const RopeSide &d = a.side[k];
-    s.x_at[k][j] = b * d.x_st[0] + at * d.x_st[2];
-    s.y_at[k][j] = b * d.y_st[0] + at * d.y_st[2];
-    if (BACK) s.dy_at[k][j] = b * d.dy_st[0] + at * d.dy_st[2];
+  return rope_pairs<INTER>(x);
+}
+// the channels in their order again
+template <bool INTER>
+__device__ __forceinline__ void rope_channels(const RopeVals &v, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float a0, a1, b0, b1;
+    ptx::f2_split(v.a[h], a0, a1);
+    ptx::f2_split(v.b[h], b0, b1);
+    if (INTER)
+      x[4 * h] = a0, x[4 * h + 1] = b0, x[4 * h + 2] = a1, x[4 * h + 3] = b1;
+    else
+      x[2 * h] = a0, x[2 * h + 1] = a1, x[4 + 2 * h] = b0, x[4 + 2 * h + 1] = b1;
   }
 }
-
+template <int T, bool INTER>
+__device__ __forceinline__ void rope_store(uint8_t *p, int ab, const RopeVals &v) {  // ab: bytes between the fours
+  float x[8];
+  rope_channels<INTER>(v, x);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    auto *dst = reinterpret_cast<typename RopeRaw<T>::type *>(p + (h ? ab : 0));
+    const float *y = x + 4 * h;
+    if constexpr (T == ROPE_F32)
+      *dst = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+    else if constexpr (T == ROPE_BF16)
+      *dst = make_uint2(ptx::pack_bf16(y[0], y[1]), ptx::pack_bf16(y[2], y[3]));
+    else
+      *dst = make_uint2(ptx::pack_f16(y[0], y[1]), ptx::pack_f16(y[2], y[3]));
+  }
+}
+__device__ __forceinline__ RopeVals rope_mul(const RopeVals &x, const RopeVals &y) {
+  return {{ptx::mul2(x.a[0], y.a[0]), ptx::mul2(x.a[1], y.a[1])}, {ptx::mul2(x.b[0], y.b[0]), ptx::mul2(x.b[1], y.b[1])}};
+}
+__device__ __forceinline__ RopeVals rope_fma(const RopeVals &x, const RopeVals &y, const RopeVals &z) {
+  return {{ptx::fma2(x.a[0], y.a[0], z.a[0]), ptx::fma2(x.a[1], y.a[1], z.a[1])},
+          {ptx::fma2(x.b[0], y.b[0], z.b[0]), ptx::fma2(x.b[1], y.b[1], z.b[1])}};
+}
+__device__ __forceinline__ RopeVals rope_all(float f) {
+  const uint64_t x = ptx::f2(f, f);
+  return {{x, x}, {x, x}};
+}
+// sum of a lane's products
+__device__ __forceinline__ float rope_dot(const RopeVals &x, const RopeVals &y) {
+  const uint64_t s = ptx::fma2(x.b[1], y.b[1], ptx::fma2(x.b[0], y.b[0], ptx::fma2(x.a[1], y.a[1], ptx::mul2(x.a[0], y.a[0]))));
+  float lo, hi;
+  ptx::f2_split(s, lo, hi);
+  return lo + hi;
+}
 // A lane's channels, of a row and of its angles.
 struct RopeLane {
   int a, b;    // first channels of its two fours
   int pair;    // first pair
   bool turns;
-  bool split;  // its pairs are (i, i + 4) of the eight, otherwise neighbours
 };
 template <int D, bool INTER>
 __device__ __forceinline__ RopeLane rope_lane(int rot) {
   const int l = threadIdx.x % (D / 8);
   const bool turns = l < rot / 8, half = !INTER && turns;
-  return {half ? 4 * l : 8 * l, half ? rot / 2 + 4 * l : 8 * l + 4, 4 * l, turns, half};
+  return {half ? 4 * l : 8 * l, half ? rot / 2 + 4 * l : 8 * l + 4, 4 * l, turns};
 }
-// (a, b) -> (a c - b s, b c + a s) of a lane's pairs
-__device__ __forceinline__ void rope_turn(float (&v)[8], bool split, const float4 &c, const float4 &s) {
-  const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+// (a, b) -> (a ca - b sb, b cb + a sa) of a lane's pairs; lanes that do not turn have no sines
+struct RopeTurn {
+  uint64_t ca[2], cb[2], sa[2], sb[2];  // sb: negative
+};
+__device__ __forceinline__ RopeVals rope_turn(const RopeVals &v, const RopeTurn &c, bool turns) {
+  RopeVals r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = split ? v[i] : v[2 * i], b = split ? v[i + 4] : v[2 * i + 1];
-    const float x = a * cc[i] - b * ss[i], y = b * cc[i] + a * ss[i];
-    if (split)
-      v[i] = x, v[i + 4] = y;
-    else
-      v[2 * i] = x, v[2 * i + 1] = y;
+  for (int h = 0; h < 2; ++h) r.a[h] = ptx::mul2(v.a[h], c.ca[h]), r.b[h] = ptx::mul2(v.b[h], c.cb[h]);
+  if (turns) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) r.a[h] = ptx::fma2(v.b[h], c.sb[h], r.a[h]), r.b[h] = ptx::fma2(v.a[h], c.sa[h], r.b[h]);
   }
+  return r;
 }
 template <int LANES>
 __device__ __forceinline__ float rope_sum(float x) {
@@ -142,165 +161,189 @@ __device__ __forceinline__ float rope_sum(float x) {
   for (int d = 1; d < LANES; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
   return x;
 }
-__device__ __forceinline__ int rope_div(uint32_t magic, int x) {
-  return magic == 0 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), magic));
+// a lane's eight weights (ones where there are none)
+template <bool INTER>
+__device__ __forceinline__ RopeVals rope_weights(const RopeArgs &a, const void *w, const RopeLane &me) {
+  if (w == nullptr) return rope_all(1.f);
+  RopeVals v;
+  if (a.w_type == ROPE_F32) {
+    const uint4 r[2] = {*rope_at<ROPE_F32>(w, me.a), *rope_at<ROPE_F32>(w, me.b)};
+    v = rope_values<ROPE_F32, INTER>(r);
+  } else {
+    const uint2 r[2] = {*rope_at<ROPE_BF16>(w, me.a), *rope_at<ROPE_BF16>(w, me.b)};
+    v = a.w_type == ROPE_BF16 ? rope_values<ROPE_BF16, INTER>(r) : rope_values<ROPE_F16, INTER>(r);
+  }
+  const RopeVals o = rope_all(a.w_offset);
+  return {{ptx::add2(v.a[0], o.a[0]), ptx::add2(v.a[1], o.a[0])}, {ptx::add2(v.b[0], o.a[0]), ptx::add2(v.b[1], o.a[0])}};
 }
-
-template <int T, int D, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int LANES = D / 8, GROUPS = kRopeThreads / LANES, U = 4;  // rows of a group at a time
-  using Raw = typename RopeRaw<T>::type;
-  __shared__ RopeShared<D> s;
-  const RopeLane me = rope_lane<D, INTER>(a.rot);
-  const int g = threadIdx.x / LANES;
-  follow();
-  const int t0 = blockIdx.x * a.per_cta, n = min(a.per_cta, a.tokens - t0);
-  rope_tokens<D, false>(a, s, t0, n);
-  __syncthreads();
-#pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    const RopeSide &d = a.side[k];
-    float w[8];
+// Cosines and sines of four angles, turns in units of 2^-64. The nearest quarter turn goes to a
+// choice of signs and sides; what is left, |x| <= pi / 4, to the Taylor polynomials
+//   sin x = x - x^3/3! + .. + x^9/9!,  cos x = 1 - x^2/2! + .. + x^10/10!
+// whose next terms are 2^-29 and 2^-30.
+__device__ __forceinline__ void rope_angles(const uint64_t (&turn)[4], uint64_t (&cos)[2], uint64_t (&sin)[2]) {
+  float c[4], s[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      w[i] = d.w != nullptr ? rope_weight(d.w, a.w_type, (i < 4 ? me.a : me.b - 4) + i) + a.w_offset : 1.f;
-    const int rows = n * d.heads;
-#pragma unroll 1
-    for (int r0 = g; r0 - g < rows; r0 += U * GROUPS) {
-      Raw raw[U][2];
-      int tok[U], head[U];
+  for (int h = 0; h < 2; ++h) {
+    float x[2];
+    uint32_t quarter[2];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * GROUPS;
-        tok[u] = rope_div(d.magic, r), head[u] = r - tok[u] * d.heads;
-        if (r < rows) {
-          const int64_t at = s.x_at[k][tok[u]] + head[u] * d.x_st[1];
-          raw[u][0] = *rope_at<T>(d.x, at + me.a);
-          raw[u][1] = *rope_at<T>(d.x, at + me.b);
-        } else {
-          raw[u][0] = raw[u][1] = Raw{};
-        }
-      }
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t t = static_cast<uint32_t>(turn[2 * h + i] >> 32);
+      quarter[i] = (t + 0x20000000u) >> 30;
+      x[i] = static_cast<float>(static_cast<int32_t>(t - (quarter[i] << 30))) * 1.4629180792671596e-9f;  // pi / 2^31
+    }
+    auto all = [](float f) { return ptx::f2(f, f); };
+    const uint64_t X = ptx::f2(x[0], x[1]), X2 = ptx::mul2(X, X);
+    uint64_t S = ptx::fma2(X2, all(1.f / 362880.f), all(-1.f / 5040.f));
+    S = ptx::fma2(X2, S, all(1.f / 120.f));
+    S = ptx::fma2(X2, S, all(-1.f / 6.f));
+    S = ptx::fma2(ptx::mul2(X, X2), S, X);
+    uint64_t C = ptx::fma2(X2, all(-1.f / 3628800.f), all(1.f / 40320.f));
+    C = ptx::fma2(X2, C, all(-1.f / 720.f));
+    C = ptx::fma2(X2, C, all(1.f / 24.f));
+    C = ptx::fma2(X2, C, all(-0.5f));
+    C = ptx::fma2(X2, C, all(1.f));
+    float sv[2], cv[2];
+    ptx::f2_split(S, sv[0], sv[1]);
+    ptx::f2_split(C, cv[0], cv[1]);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float4 x0 = rope_values<T>(raw[u][0]), x1 = rope_values<T>(raw[u][1]);
-        float v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
-        const float rstd = rsqrtf(rope_sum<LANES>(sum) * (1.f / D) + a.eps);
-        if (r0 + u * GROUPS < rows) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= rstd * w[i];
-          if (me.turns)
-            rope_turn(v, me.split, *reinterpret_cast<const float4 *>(&s.cos[tok[u]][me.pair]),
-                      *reinterpret_cast<const float4 *>(&s.sin[tok[u]][me.pair]));
-          const int64_t at = s.y_at[k][tok[u]] + head[u] * d.y_st[1];
-          rope_store<T>(d.y, at + me.a, v);
-          rope_store<T>(d.y, at + me.b, v + 4);
-        }
-      }
+    for (int i = 0; i < 2; ++i) {  // by q quarter turns: (c, s), (-s, c), (-c, -s), (s, -c)
+      const uint32_t q = quarter[i];
+      const float a = q & 1 ? sv[i] : cv[i], b = q & 1 ? cv[i] : sv[i];
+      c[2 * h + i] = __uint_as_float(__float_as_uint(a) ^ (((q + 1) & 2) << 30));
+      s[2 * h + i] = __uint_as_float(__float_as_uint(b) ^ ((q & 2) << 30));
     }
   }
+  cos[0] = ptx::f2(c[0], c[1]), cos[1] = ptx::f2(c[2], c[3]);
+  sin[0] = ptx::f2(s[0], s[1]), sin[1] = ptx::f2(s[2], s[3]);
 }
 
-// Backward: with g the output's gradient turned back, xhat = x rstd,
-//   dw = sum of g xhat,   dx = rstd (g w - xhat mean(g w xhat)).
-// x and the gradient are read once, so the row's rstd is computed again. A CTA goes
-// on over blocks of tokens and keeps its sums of dw in registers; they are added up
-// by group, by CTA and in the kernel below in an order that is always the same.
-template <int T, int D, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_bwd_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int LANES = D / 8, GROUPS = kRopeThreads / LANES, U = 2;
+// Forward: y = turn(x rstd w). Backward (BACK): with g the output's gradient turned back
+// and xhat = x rstd,
+//   dw = sum of g xhat,   dx = rstd (g w - xhat mean(g w xhat));
+// x and the gradient are read once, so the row's rstd is computed again. Sums of dw stay in
+// registers while a group goes on from token to token; they are added up by group, by CTA
+// and in the kernel below in an order that is always the same.
+template <int T, int D, bool INTER, bool BACK>
+__global__ void __launch_bounds__(kRopeThreads, BACK ? 4 : 8) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int LANES = D / 8, GROUPS = kRopeThreads / LANES, SIZE = T == ROPE_F32 ? 4 : 2;
+  constexpr int U = (BACK ? 2 : 4) / (T == ROPE_F32 ? 2 : 1);  // rows on their way at a time
   using Raw = typename RopeRaw<T>::type;
-  __shared__ RopeShared<D> s;
-  __shared__ float s_dw[GROUPS][D];
+  __shared__ float s_dw[BACK ? GROUPS : 1][D];
   const RopeLane me = rope_lane<D, INTER>(a.rot);
-  const int g = threadIdx.x / LANES;
-  float dw[2][8] = {};
+  const int ab = (me.b - me.a) * SIZE;  // bytes
+  const int g = threadIdx.x / LANES, parts = 1 << a.part_bits;
+  const int64_t tasks = static_cast<int64_t>(a.tokens) << a.part_bits;
+  RopeVals dw[BACK ? 2 : 1] = {};
   follow();
-  for (int t0 = blockIdx.x * a.per_cta; t0 < a.tokens; t0 += gridDim.x * a.per_cta) {
-    const int n = min(a.per_cta, a.tokens - t0);
-    rope_tokens<D, true>(a, s, t0, n);
-    __syncthreads();
+  // (a warp's groups go on together, as its shuffles want)
+  const int64_t warp0 = static_cast<int64_t>(blockIdx.x) * GROUPS + g / (32 / LANES) * (32 / LANES);
+#pragma unroll 1
+  for (int64_t task0 = warp0; task0 < tasks; task0 += static_cast<int64_t>(gridDim.x) * GROUPS) {
+    const int64_t task = task0 + g % (32 / LANES);
+    const bool there = task < tasks;
+    const int token = there ? static_cast<int>(task >> a.part_bits) : 0, part = static_cast<int>(task) & (parts - 1);
+    int b = 0, at = token;
+    if (a.seqlen != a.tokens) b = token / a.seqlen, at = token - b * a.seqlen;
+    uint64_t cos[2], sin[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const RopeSide &d = a.side[k];
-      float w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        w[i] = d.w != nullptr ? rope_weight(d.w, a.w_type, (i < 4 ? me.a : me.b - 4) + i) + a.w_offset : 1.f;
-      const int rows = n * d.heads;
-#pragma unroll 1
-      for (int r0 = g; r0 - g < rows; r0 += U * GROUPS) {
-        Raw raw[U][2], grad[U][2];
-        int tok[U], head[U];
+      auto row = [&](const void *p, const int64_t(&st)[3]) {
+        return static_cast<const uint8_t *>(p) + (b * st[0] + at * st[2] + part * st[1] + me.a) * SIZE;
+      };
+      const uint8_t *xp = row(d.x, d.x_st), *dp = BACK ? row(d.dy, d.dy_st) : nullptr;
+      uint8_t *yp = const_cast<uint8_t *>(row(d.y, d.y_st));
+      const int64_t xs = (d.x_st[1] << a.part_bits) * SIZE, ys = (d.y_st[1] << a.part_bits) * SIZE,
+                    ds = BACK ? (d.dy_st[1] << a.part_bits) * SIZE : 0;
+      const int trips = (d.heads + parts - 1) >> a.part_bits;
+      const int have = there ? (d.heads - part + parts - 1) >> a.part_bits : 0;  // rows of this group
+      Raw raw[U][2], grad[BACK ? U : 1][2];
+      auto get = [](const uint8_t *p) { return *reinterpret_cast<const Raw *>(p); };
+      auto load = [&](int left) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int r = r0 + u * GROUPS;
-          tok[u] = rope_div(d.magic, r), head[u] = r - tok[u] * d.heads;
-          if (r < rows) {
-            const int64_t at = s.x_at[k][tok[u]] + head[u] * d.x_st[1];
-            const int64_t dat = s.dy_at[k][tok[u]] + head[u] * d.dy_st[1];
-            raw[u][0] = *rope_at<T>(d.x, at + me.a);
-            raw[u][1] = *rope_at<T>(d.x, at + me.b);
-            grad[u][0] = *rope_at<T>(d.dy, dat + me.a);
-            grad[u][1] = *rope_at<T>(d.dy, dat + me.b);
-          } else {
-            raw[u][0] = raw[u][1] = grad[u][0] = grad[u][1] = Raw{};
+          if (u < left) {
+            raw[u][0] = get(xp), raw[u][1] = get(xp + ab);
+            if (BACK) grad[u][0] = get(dp), grad[u][1] = get(dp + ab);
           }
+          xp += xs, dp += ds;
         }
+      };
+      load(have);  // (the angles and weights are computed while the first rows are on their way)
+      if (k == 0) {
+        const int pos = a.positions != nullptr ? a.positions[b * a.pos_stride + at] : at;
+        uint64_t turn[4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const bool real = r0 + u * GROUPS < rows;
-          const float4 x0 = rope_values<T>(raw[u][0]), x1 = rope_values<T>(raw[u][1]);
-          const float4 g0 = rope_values<T>(grad[u][0]), g1 = rope_values<T>(grad[u][1]);
-          float v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-          float q[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
-          const int j = real ? tok[u] : 0;
-          const float4 sn = *reinterpret_cast<const float4 *>(&s.sin[j][me.pair]);
-          if (me.turns)
-            rope_turn(q, me.split, *reinterpret_cast<const float4 *>(&s.cos[j][me.pair]),
-                      make_float4(-sn.x, -sn.y, -sn.z, -sn.w));
-          float sum = 0.f, dot = 0.f;
+        for (int i = 0; i < 4; ++i)
+          turn[i] = me.turns ? static_cast<uint64_t>(static_cast<int64_t>(pos)) * a.freqs[me.pair + i] : 0;
+        rope_angles(turn, cos, sin);
+      }
+      const RopeVals w = rope_weights<INTER>(a, d.w, me);
+      RopeTurn c;
+      const uint64_t neg = ptx::f2(-1.f, -1.f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum), dot = fmaf(q[i] * w[i], v[i], dot);
-          const float rstd = rsqrtf(rope_sum<LANES>(sum) * (1.f / D) + a.eps);
-          dot = rope_sum<LANES>(dot) * (1.f / D) * rstd;  // mean(g w xhat)
-          float o[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float xhat = v[i] * rstd;
-            dw[k][i] = fmaf(q[i], xhat, dw[k][i]);
-            o[i] = rstd * (q[i] * w[i] - xhat * dot);
-          }
-          if (real) {
-            const int64_t at = s.y_at[k][tok[u]] + head[u] * d.y_st[1];
-            rope_store<T>(d.y, at + me.a, o);
-            rope_store<T>(d.y, at + me.b, o + 4);
-          }
+      for (int h = 0; h < 2; ++h) {
+        if (BACK) {
+          c.ca[h] = c.cb[h] = cos[h], c.sb[h] = sin[h], c.sa[h] = ptx::mul2(sin[h], neg);
+        } else {
+          c.ca[h] = ptx::mul2(w.a[h], cos[h]), c.cb[h] = ptx::mul2(w.b[h], cos[h]);
+          c.sa[h] = ptx::mul2(w.a[h], sin[h]), c.sb[h] = ptx::mul2(ptx::mul2(w.b[h], sin[h]), neg);
         }
       }
+      int left = have;
+#pragma unroll 1
+      for (int j = 0; j < trips; j += U, left -= U) {
+        Raw x[U][2], dy[BACK ? U : 1][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          x[u][0] = raw[u][0], x[u][1] = raw[u][1];
+          if (BACK) dy[u][0] = grad[u][0], dy[u][1] = grad[u][1];
+        }
+        if (BACK && j + U < trips) load(left - U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const RopeVals v = rope_values<T, INTER>(x[u]);
+          const float rstd = rsqrtf(rope_sum<LANES>(rope_dot(v, v)) * (1.f / D) + a.eps);
+          if constexpr (BACK) {
+            const RopeVals q = rope_turn(rope_values<T, INTER>(dy[u]), c, me.turns);
+            const RopeVals gw = rope_mul(q, w);
+            const float dot = rope_sum<LANES>(rope_dot(gw, v)) * (1.f / D) * rstd;  // mean(g w xhat)
+            if (u < left) {
+              const RopeVals xhat = rope_mul(v, rope_all(rstd));
+              dw[k] = rope_fma(q, xhat, dw[k]);
+              rope_store<T, INTER>(yp, ab, rope_mul(rope_fma(xhat, rope_all(-dot), gw), rope_all(rstd)));
+            }
+          } else {
+            if (u < left) rope_store<T, INTER>(yp, ab, rope_turn(rope_mul(v, rope_all(rstd)), c, me.turns));
+          }
+          yp += ys;
+        }
+        if (!BACK && j + U < trips) load(left - U);
+      }
     }
-    __syncthreads();
   }
+  if constexpr (BACK) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (a.side[k].w == nullptr) continue;
+    for (int k = 0; k < 2; ++k) {
+      if (a.side[k].w == nullptr) continue;
+      __syncthreads();
+      float x[8];
+      rope_channels<INTER>(dw[k], x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s_dw[g][(i < 4 ? me.a : me.b - 4) + i] = dw[k][i];
-    __syncthreads();
-    if (threadIdx.x < D) {
-      float sum = 0.f;
-      for (int x = 0; x < GROUPS; ++x) sum += s_dw[x][threadIdx.x];
-      a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + k) * D + threadIdx.x] = sum;
+      for (int i = 0; i < 8; ++i) s_dw[g][(i < 4 ? me.a : me.b - 4) + i] = x[i];
+      __syncthreads();
+      if (threadIdx.x < D) {
+        float sum = 0.f;
+        for (int x = 0; x < GROUPS; ++x) sum += s_dw[x][threadIdx.x];
+        a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + k) * D + threadIdx.x] = sum;
+      }
     }
-    __syncthreads();
   }
 }
 
-// The CTAs' sums of the weights' gradients, [parts][2][D], to dw[k][D]: a CTA 32
-// channels, its 32 warps every 32nd part.
+// The CTAs' sums of the weights' gradients, [parts][2][D], to dw[k][D]: a CTA 32 channels,
+// its 32 warps every 32nd part.
 struct RopeSumArgs {
   const float *partial;
   void *dw[2];
@@ -309,19 +352,19 @@ struct RopeSumArgs {
 static __global__ void __launch_bounds__(1024) rope_weight_sum_kernel(const RopeSumArgs a) {
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane, k = c / a.dim;
+  const int c = blockIdx.x * 32 + lane, k = c / a.dim, e = c - k * a.dim;
   follow();
+  void *dw = k == 0 ? a.dw[0] : a.dw[1];
+  if (dw == nullptr) return;
   float sum = 0.f;
 #pragma unroll 4
   for (int p = warp; p < a.parts; p += 32) sum += a.partial[static_cast<int64_t>(p) * 2 * a.dim + c];
   s[warp][lane] = sum;
   __syncthreads();
-  void *dw = k == 0 ? a.dw[0] : a.dw[1];
-  if (warp == 0 && dw != nullptr) {
+  if (warp == 0) {
     sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 32; ++x) sum += s[x][lane];
-    const int e = c - k * a.dim;
     if (a.w_type == ROPE_F32)
       static_cast<float *>(dw)[e] = sum;
     else

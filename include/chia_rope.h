@@ -49,7 +49,8 @@ typedef struct chia_rope_params {
   int64_t k_stride[3];
   int64_t q_out_stride[3];
   int64_t k_out_stride[3];
-  const void *q_weight; /* [head_dim], or NULL: none for this input           */
+  const void *q_weight; /* [head_dim], 16-byte aligned, or NULL: none for this
+                           input                                             */
   const void *k_weight;
   const uint64_t *freqs;    /* [rot / 2]                                     */
   const int32_t *positions; /* NULL: 0, 1, 2, ... in each batch entry        */
