@@ -128,10 +128,10 @@ __device__ __forceinline__ void band32(const PagedArgs &a, int i, int len, int &
 __device__ __forceinline__ int tree_position(const PagedArgs &a, int t0, int i, int p0, int len) {
   return max(p0, min(len - 1, a.tree_pos[t0 + i]));
 }
-// Bits: the nodes of its tree (n of them) that node i, at position `pos`, sees: those of its
+// Bits: the nodes of its tree (n of them) that a node at position `pos` sees: those of its
 // word that the mask does not put too far back. A word holds a path, so few are looked at.
-__device__ __forceinline__ unsigned long long tree_word_of(const PagedArgs &a, int t0, int i, int n, int pos, int len) {
-  unsigned long long word = a.tree_word[t0 + i];
+__device__ __forceinline__ unsigned long long tree_word_of(const PagedArgs &a, unsigned long long word, int t0, int n,
+                                                           int pos, int len) {
   if (n < 64) word &= (1ull << n) - 1;
   if (a.left < 0 && a.block == 0 && a.dil == 1) return word;
   int lo, hi;

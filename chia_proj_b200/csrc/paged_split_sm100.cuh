@@ -281,7 +281,7 @@ paged_split_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           word[n][x] = 0, tpos[n][x] = p0 + qi;
           if (rq.n <= kTreeNodes) {
             tpos[n][x] = tree_position(a, rq.t0, qi, p0, len);
-            word[n][x] = tree_word_of(a, rq.t0, qi, rq.n, tpos[n][x], len);
+            word[n][x] = tree_word_of(a, a.tree_word[rq.t0 + qi], rq.t0, rq.n, tpos[n][x], len);
           }
         }
       }

@@ -151,9 +151,11 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
 }
 
 // TREE: requests of up to kTreeNodes queries are trees of drafted tokens, as in the split kernel.
-// Their units are often of 128 rows or fewer. Such a unit is a pair: both halves of the
-// softmax warps hold the same rows, each takes every second key tile into a sum of its own, and
-// the first half joins the two at the end. And warps without rows do no arithmetic.
+// Their units often have few rows: warps without any do no arithmetic. (Tried: for units of up to
+// 128 rows both halves of the softmax warps with the same rows, a key tile each by turns, joined at
+// the end: 291 us where this has 300 on 16 x 25 nodes over 16,000 keys, 207 and 212 on 32 x 16 over
+// 4,096, 337 and 330 on capped trees over up to 16,384. The conversion, four warps at 1,200 cycles a
+// tile beside the others, and the copies' way round are next to the softmax then.)
 template <int D, int CT, int KIND, bool BF16, bool TREE>
 __global__ void __launch_bounds__(kTiledThreads, 1)
 paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -173,12 +175,11 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   enum { ST_FULL = 0, ST_EMPTY = ST_FULL + STAGES, KV_FULL = ST_EMPTY + STAGES, KV_EMPTY = KV_FULL + SLOTS,
          Q_FULL = KV_EMPTY + SLOTS, S_FULL = Q_FULL + 2, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4,
          O_FULL = PV_DONE + 2, O_EMPTY = O_FULL + 2, SC_FULL = O_EMPTY + 2, SC_EMPTY = SC_FULL + SETS,
-         DRAIN = SC_EMPTY + SETS, PAIR = DRAIN + 2, BARS = PAIR + (TREE ? 1 : 0) };
+         DRAIN = SC_EMPTY + SETS, BARS = DRAIN + 2 };
   __shared__ __align__(8) uint64_t bars[BARS];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag, nan_flag;
   __shared__ float q_scale[256];  // of the rows of Q, undone in the scores
-  __shared__ float2 s_pair[TREE ? 128 : 1];               // a pair's second half: maximum and sum of each row
   __shared__ unsigned long long s_word[TREE ? 256 : 1];  // the nodes that each row sees
   // of a tile: all rows see the whole of it; keys there are; bits, 16 keys each: their page
   // is out of range, so that nothing is loaded and no row sees them
@@ -188,7 +189,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
   if (t == 0) {
     for (int i = 0; i < BARS; ++i) {
       const bool four = (i >= ST_EMPTY && i < KV_EMPTY) || (i >= Q_FULL && i < S_FULL) ||
-                        (i >= P_FULL && i < PV_DONE) || (i >= O_EMPTY && i < SC_FULL) || i == PAIR;
+                        (i >= P_FULL && i < PV_DONE) || (i >= O_EMPTY && i < SC_FULL);
       ptx::mbar_init(bar(i), i >= KV_EMPTY && i < Q_FULL ? 2 : four ? 4 : i >= SC_EMPTY && i < DRAIN ? 8 : 1);
     }
     abort_flag = nan_flag = 0;
@@ -258,9 +259,6 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     const int pf = min(a.prefix, h.rq.len);
     return TREE ? max(0, min(pf, tree_first(h.rq))) : pf;
   };
-  auto is_pair = [&](const Here &h) { return TREE && h.un.rows <= 128; };
-  // key tiles of a pair that half w takes: w, w + 2, ..
-  auto tiles_of_half = [](int nt, int w) { return (nt + 1 - w) >> 1; };
   auto sees_all = [&](const Here &h, int j0) {  // every row of the unit sees keys [j0, j0 + TK)
     return (a.dil == 1 && j0 >= h.lo_max && j0 + TK - 1 <= h.hi_min) ||
            j0 <= prefix_of(h) - TK;
@@ -401,46 +399,11 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
       bool ok = true;
       for (int k = 0; k < nk && ok;) {
         const Here h = unit_at(k);
-        auto let_go = [&](int from, int to) {  // tiles that this half has no part in
-          for (int i = 2 * (k + from); i < 2 * (k + to) && ok; ++i) {
+        if (h.un.rows <= 128 * w) {  // no second query tile: the slots are let go as they come
+          for (int i = 2 * k; i < 2 * (k + h.nt) && ok; ++i) {
             ok = warp_all(wait(KV_FULL + i % SLOTS, (i / SLOTS) & 1));
             if (ok && lane == 0) ptx::mbar_arrive(bar(KV_EMPTY + i % SLOTS));
           }
-        };
-        const bool pair = is_pair(h);
-        if (pair ? tiles_of_half(h.nt, w) == 0 : h.un.rows <= 128 * w) {  // the slots are let go as they come
-          let_go(0, h.nt);
-          k += h.nt;
-          continue;
-        }
-        if (TREE && pair) {
-          // As below, with every second tile; those between are let go in their turn, so that no wait
-          // is for an item whose place in the ring waits for this warp.
-          const int own = tiles_of_half(h.nt, w);
-          ok = warp_all(wait(Q_FULL + w, units & 1));
-          auto pair_s = [&](int m) {
-            const int i = 2 * m + w, ki = 2 * (k + i);
-            let_go(i > 0 ? i - 1 : 0, i);
-            if (!ok || !warp_all(wait(KV_FULL + ki % SLOTS, (ki / SLOTS) & 1))) return false;
-            ptx::tc_fence_after();
-            issue_s((tiles + m) & 1, ki % SLOTS);
-            return true;
-          };
-          for (int m = 0; m < min(2, own) && ok; ++m) ok = pair_s(m);
-          for (int m = 0; m < own && ok; ++m) {
-            const int vi = 2 * (k + 2 * m + w) + 1;
-            const uint32_t n = tiles + m;
-            ok = warp_all(wait(KV_FULL + vi % SLOTS, (vi / SLOTS) & 1) &&
-                          wait(P_FULL + 2 * w + (n & 1), (n >> 1) & 1) &&
-                          (m > 0 || units == 0 || wait(O_EMPTY + w, (units - 1) & 1)));
-            if (!ok) break;
-            ptx::tc_fence_after();
-            issue_pv(n & 1, vi % SLOTS, m == 0, m == own - 1);
-            if (m + 2 < own) ok = pair_s(m + 2);
-          }
-          if (ok) let_go(2 * own + w - 1, h.nt);
-          tiles += own;
-          ++units;
           k += h.nt;
           continue;
         }
@@ -539,32 +502,29 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS0 = tmem + lane_off + w * 128, tO = tmem + lane_off + 256 + w * 128;
     uint32_t cnt = 0, units = 0;
-    uint32_t units1 = 0, pairs = 0;  // units that the second half has had a part in; as the half of a pair
     bool ok = true;
     if (t == 0) cuts[blockIdx.x].un.rows = 0;
     for (int k = 0; k < nk && ok;) {
       const Here h = unit_at(k);
       const bool begun = h.ut0 == 0, ended = h.ut0 + h.nt == h.un.n, whole = begun && ended;
       const int64_t slot = 2ll * blockIdx.x + (begun ? 1 : 0);
-      const bool pair = is_pair(h);
-      const int half0 = pair ? 0 : w * 128;  // first row of this half
-      const int r = half0 + row;             // row of the unit
+      const int r = w * 128 + row;  // row of the unit
       const bool real = r < h.un.rows;
-      const bool both = pair && h.nt > 1;  // its two halves have tiles
-      if (TREE && (pair ? both : h.un.rows > 128)) ++units1;
-      if (pair ? tiles_of_half(h.nt, w) > 0 : h.un.rows > w * 128) {
+      if (h.un.rows > w * 128) {
         const int rr = h.un.row0 + min(r, h.un.rows - 1);
         const int qi = div_group(a, rr), head = h.un.hk * a.group + rr - qi * a.group;
         const int first = tree_first(h.rq);
-        const int pos = TREE && first != 0x7fffffff ? tree_position(a, h.rq.t0, qi, h.p0, h.rq.len) : h.p0 + qi;
-        if (TREE) s_word[t] = first != 0x7fffffff ? tree_word_of(a, h.rq.t0, qi, h.rq.n, pos, h.rq.len) : 0;
+        // (asked for here, looked at behind Q)
+        int pos = h.p0 + qi;
+        unsigned long long word = 0;
+        if (TREE && first != 0x7fffffff) pos = a.tree_pos[h.rq.t0 + qi], word = a.tree_word[h.rq.t0 + qi];
         // ---- the row of Q, as halves
         // (16 bytes a lane, neighbouring lanes along a row, four loads on their way
         // while four are converted: unrolled further, fetching the code takes longer)
         float rowmul = a.score_scale;
         {
           constexpr int UPR = D / 8, RPI = 32 / UPR, IT = 32 / RPI, AHEAD = 4;
-          const int u = lane % UPR, q0 = half0 + (warp & 3) * 32 + lane / UPR;  // row of the first load
+          const int u = lane % UPR, q0 = w * 128 + (warp & 3) * 32 + lane / UPR;  // row of the first load
           uint4 raw[AHEAD];
           auto load = [&](int x) {
             const int q = q0 + x * RPI, qr = h.un.row0 + q;
@@ -600,13 +560,13 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
                                     (((u % 8) ^ (q & 7)) << 4),
                                 ptx::pack_f16(f[0].x * up, f[0].y * up), ptx::pack_f16(f[1].x * up, f[1].y * up),
                                 ptx::pack_f16(f[2].x * up, f[2].y * up), ptx::pack_f16(f[3].x * up, f[3].y * up));
-              if (u == 0) q_scale[w * 128 + (q & 127)] = pow2f(e - 14);
+              if (u == 0) q_scale[q] = pow2f(e - 14);
             }
           }
           ptx::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(bar(Q_FULL + w));
-          rowmul *= q_scale[w * 128 + row];
+          rowmul *= q_scale[r];
         }
         const float hp = a.head_param != nullptr ? a.head_param[head] : 1.f;
         float slope = 0.f;
@@ -614,22 +574,17 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         if (KIND == KIND_SOFTCAP) rowmul *= 2.f * LOG2E / a.softcap;
         if (KIND == KIND_ALIBI) rowmul *= LOG2E, slope = hp * LOG2E;
         if (KIND == KIND_SIGMOID) rowmul *= -LOG2E;
+        if (TREE && first != 0x7fffffff) {
+          pos = max(h.p0, min(h.rq.len - 1, pos));
+          s_word[t] = tree_word_of(a, word, h.rq.t0, h.rq.n, pos, h.rq.len);
+        }
         int lo, hi;
         band32(a, pos, h.rq.len, lo, hi);
         const int pf = prefix_of(h);
         float m_run = SOFTMAX ? -INFINITY : -100.f, l_run = 0.f;
-        const bool idle = TREE && half0 + (warp & 3) * 32 >= h.un.rows;  // a warp without rows
-        int done = 0;  // tiles of this half
-        for (int i = 0; i < h.nt; ++i) {
+        const bool idle = TREE && w * 128 + (warp & 3) * 32 >= h.un.rows;  // a warp without rows
+        for (int i = 0; i < h.nt; ++i, ++cnt) {
           const int n = k + i;
-          if (TREE && pair && (i & 1) != w) {  // the other half's
-            if (!warp_all(wait(SC_FULL + n % SETS, (n / SETS) & 1))) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) ptx::mbar_arrive(bar(SC_EMPTY + n % SETS));
-            continue;
-          }
           // (after a wait that ran out S is anything; the vote below ends the work before P is stored)
           const bool got =
               wait2(SC_FULL + n % SETS, (n / SETS) & 1, S_FULL + 2 * w + (cnt & 1), (cnt >> 1) & 1);
@@ -642,7 +597,6 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               ptx::mbar_arrive(bar(P_FULL + 2 * w + (cnt & 1)));
               ptx::mbar_arrive(bar(SC_EMPTY + n % SETS));
             }
-            ++cnt, ++done;
             continue;
           }
           ptx::tc_fence_after();
@@ -745,9 +699,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             l_run *= alpha;
             m_run = m_new;
           }
-          if (__any_sync(0xffffffffu, !got || (need && done > 0))) {
+          if (__any_sync(0xffffffffu, !got || (need && i > 0))) {
             // O is rescaled once the tile before is in it
-            if (!warp_all(got && (done == 0 || wait(PV_DONE + w, (cnt - 1) & 1)))) {
+            if (!warp_all(got && (i == 0 || wait(PV_DONE + w, (cnt - 1) & 1)))) {
               ok = false;
               break;
             }
@@ -809,7 +763,6 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
             ptx::mbar_arrive(bar(P_FULL + 2 * w + (cnt & 1)));
             ptx::mbar_arrive(bar(SC_EMPTY + n % SETS));
           }
-          ++cnt, ++done;
         }
         if (!ok) break;
         // ---- O
@@ -820,26 +773,6 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         ++units;
         ptx::tc_fence_after();
         m_run -= kTiledPTop;  // what O and the sum are relative to
-        float e0 = 1.f, e1 = 0.f;  // a pair's two sums, relative to the larger maximum
-        if (TREE && both) {
-          if (w == 1) {  // the first half has the rest
-            s_pair[row] = make_float2(m_run, l_run);
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(bar(PAIR));
-            k += h.nt;
-            continue;
-          }
-          if (!warp_all(wait(PAIR, pairs & 1) && wait(O_FULL + 1, (units1 - 1) & 1))) {
-            ok = false;
-            break;
-          }
-          ++pairs;
-          ptx::tc_fence_after();
-          const float2 o = s_pair[row];
-          const float top = fmaxf(m_run, o.x), base = top == -INFINITY ? 0.f : top;
-          e0 = ptx::ex2(m_run - base), e1 = ptx::ex2(o.x - base);
-          m_run = top, l_run = l_run * e0 + o.y * e1;
-        }
         uint32_t nan[D / 32] = {};
         if (CT == CACHE_E4M3 && nan_flag && real) {
           auto find = [&](auto... tree) {
@@ -869,15 +802,6 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               ptx::tmem_ld16(tO + c0 + c, o);
               ptx::tmem_wait_ld();
               ptx::reg_fence16(o);
-              if (TREE && both) {
-                uint32_t o1[16];
-                ptx::tmem_ld16(tO + 128 + c0 + c, o1);
-                ptx::tmem_wait_ld();
-                ptx::reg_fence16(o1);
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), e1, __uint_as_float(o[e]) * e0));
-              }
               if (CT == CACHE_E4M3 && nan_flag) {
                 const uint32_t nn = nan[(c0 + c) / 32] >> ((c0 + c) % 32);
 #pragma unroll
@@ -924,10 +848,7 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
           *reinterpret_cast<float2 *>(a.part_ml + (slot * ROWS + r) * 2) = make_float2(m_run, l_run);
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          ptx::mbar_arrive(bar(O_EMPTY + w));
-          if (TREE && both) ptx::mbar_arrive(bar(O_EMPTY + 1));
-        }
+        if (lane == 0) ptx::mbar_arrive(bar(O_EMPTY + w));
       } else {  // no rows for this query tile: it keeps step, so that no phase of the scales is passed by
         for (int n = k; n < k + h.nt && ok; ++n) {
           ok = warp_all(wait(SC_FULL + n % SETS, (n / SETS) & 1));
