@@ -202,6 +202,12 @@ constexpr int64_t kTicketBytes = 4096;
 // faster one. Split and tiled, us, D 128, 8 K/V heads: 8 requests x 4096 keys, 48 rows 53, 57,
 // 64 rows 65, 58, 256 rows 206, 69; 32 x 1024, 48 rows 63, 63, 64 rows 71, 63.
 constexpr int64_t kTiledRows = 56;
+// Trees: from so many rows on in the mean, since their sizes differ, and the split kernel's time
+// goes by the rows that there are, the tiled kernel's by the requests. Split and tiled, us, D 128,
+// 8 K/V heads, all requests alike: 8 x 4096 keys, 64 rows 64, 68, 72 rows 76, 69; 32 x 2048, 64 rows
+// 120, 114, 80 rows 145, 114. Sizes spread from one node up to 80 rows (30 in the mean) 32, 53, to
+// 96 rows 45, 53.
+constexpr int64_t kTreeRows = 65;
 struct SplitPlan {
   bool tiled;
   // split kernel: eights of rows of a unit. Two from 9 rows on: 64 requests x 8192 keys, 16
@@ -213,7 +219,7 @@ struct SplitPlan {
 };
 int split_plan(const chia_paged_params_t *p, bool tree, int sms, SplitPlan &pl) {
   const int64_t group = p->heads / p->heads_kv;
-  pl.tiled = p->max_q * group >= kTiledRows;
+  pl.tiled = p->max_q * group >= kTiledRows && (!tree || p->tokens * group >= kTreeRows * p->batch);
   pl.tiles = p->max_q * group <= 8 && !tree ? 1 : 2;  // (trees have units of 16 rows only)
   pl.rows = pl.tiled ? chia::TiledConfig<128>::ROWS : 8 * pl.tiles;
   pl.grid = sms;

@@ -75,24 +75,25 @@ def attention(q, k, v, ks, vs, table, lens, cu, parents, *, norm="softmax", mod=
                 continue
             idx = torch.tensor([x for x, _ in keep])
             away = torch.tensor([j - at for _, j in keep], dtype=torch.float64)
-            for h in range(H):
-                g = h // (H // hkv)
-                x = kk[g, idx] @ q[t0 + i, h].double() * scale
-                if mod == "softcap":
-                    x = softcap * torch.tanh(x / softcap)
-                elif mod == "alibi":
-                    x = x + float(head_param[h]) * away
-                elif mod == "temp":
-                    x = x * float(head_param[h])
-                if norm == "sigmoid":
-                    p = torch.sigmoid(x + sig_bias)
-                elif norm == "relu":
-                    p = x.clamp(min=0) * out_scale
-                else:
-                    lse[t0 + i, h] = torch.logsumexp(x, 0)
-                    p = torch.softmax(x, 0)
-                out[t0 + i, h] = p @ vv[g, idx]
-                mass[t0 + i, h] = p.abs() @ vv[g, idx].abs()
+            qh = q[t0 + i].double().view(hkv, H // hkv, D)
+            x = torch.einsum("gkd,ghd->ghk", kk[:, idx], qh).reshape(H, -1) * scale
+            hp = None if head_param is None else torch.as_tensor(head_param).double()[:, None]
+            if mod == "softcap":
+                x = softcap * torch.tanh(x / softcap)
+            elif mod == "alibi":
+                x = x + hp * away
+            elif mod == "temp":
+                x = x * hp
+            if norm == "sigmoid":
+                p = torch.sigmoid(x + sig_bias)
+            elif norm == "relu":
+                p = x.clamp(min=0) * out_scale
+            else:
+                lse[t0 + i] = torch.logsumexp(x, 1)
+                p = torch.softmax(x, 1)
+            p = p.view(hkv, H // hkv, -1)
+            out[t0 + i] = (p @ vv[:, idx]).reshape(H, D)
+            mass[t0 + i] = (p.abs() @ vv[:, idx].abs()).reshape(H, D)
     return out, lse, mass
 
 

@@ -88,13 +88,19 @@ def with_params(kw, H):
     return kw
 
 
-# max_q 64 takes the tensor-memory kernel (rows of a K/V head from 56 on), 1 the one for few queries; both serve any tree
+# Trees of more than 64 rows (nodes x heads of a group) in the mean take the kernel of many queries: with 16 heads to each
+# K/V head and a max_q that allows it. Both kernels serve any tree.
+def heads(max_q, hkv=2):
+    return hkv * (4 if max_q == 1 else 16)
+
+
 @pytest.mark.parametrize("max_q", [1, 64])
 @pytest.mark.parametrize("kind", range(len(KINDS)))
 @pytest.mark.parametrize("ct,dtype,D,page", [(E4M3, BF16, 128, 64), (I8, F16, 64, 16), (E4M3, F16, 64, 32), (I8, BF16, 128, 128)])
 def test_kinds(cuda, max_q, kind, ct, dtype, D, page):
-    kw = with_params(KINDS[kind], 8)
-    c = make(SIZES, BASES, D=D, page=page, ct=ct, dtype=dtype, seed=kind)
+    H = heads(max_q)
+    kw = with_params(KINDS[kind], H)
+    c = make(SIZES, BASES, H=H, D=D, page=page, ct=ct, dtype=dtype, seed=kind)
     check(c, run(c, max_q=max_q, **kw), **kw)
 
 
@@ -103,8 +109,9 @@ def test_kinds(cuda, max_q, kind, ct, dtype, D, page):
 @pytest.mark.parametrize("kind", [0, 2])
 @pytest.mark.parametrize("page", [16, 64])
 def test_masks(cuda, max_q, mask, kind, page):
-    kw = with_params(KINDS[kind], 8)
-    c = make([13, 64, 3, 40], [50, 20, 5, 130], page=page, seed=mask)
+    H = heads(max_q)
+    kw = with_params(KINDS[kind], H)
+    c = make([13, 64, 3, 40], [50, 20, 5, 130], H=H, page=page, seed=mask)
     if kind == 0:
         got, lse = run(c, max_q=max_q, mask=MASKS[mask], return_lse=True, **kw)
     else:
@@ -128,7 +135,7 @@ def test_shapes(cuda, max_q, shape, H, hkv):
 @pytest.mark.parametrize("max_q", [1, 64])
 def test_long_contexts_are_split(cuda, max_q):
     """Units that several CTAs share, trees at the end of the last one's piece, and in pages that end inside a tile."""
-    c = make([64, 7, 25], [9000, 4099, 1], H=8, hkv=2, page=16, seed=3)
+    c = make([64, 7, 25], [9000, 4099, 1], H=heads(max_q), hkv=2, page=16, seed=3)
     got, lse = run(c, max_q=max_q, return_lse=True)
     check(c, got, lse)
 
@@ -136,7 +143,7 @@ def test_long_contexts_are_split(cuda, max_q):
 @pytest.mark.parametrize("max_q", [1, 64])
 def test_chunks_beside_trees(cuda, max_q):
     """A request of more than 64 queries is a chunk of a prompt."""
-    c = make([5, 65, 20, 130], [40, 10, 0, 77], seed=9)
+    c = make([5, 65, 20, 130], [40, 10, 0, 77], H=heads(max_q), seed=9)
     check(c, run(c, max_q=max_q, mask=cp.Mask(left=50, right=0)), mask=cp.Mask(left=50, right=0))
     check(c, run(c, max_q=max_q))
 
@@ -144,7 +151,7 @@ def test_chunks_beside_trees(cuda, max_q):
 @pytest.mark.parametrize("max_q", [1, 64])
 def test_more_nodes_than_keys(cuda, max_q):
     """Lengths that do not hold the tree: the first nodes have no place in the cache, and none for a first node's row."""
-    c = make([10, 6, 3], [-4, -6, 20], seed=2, shape="chain")
+    c = make([10, 6, 3], [-4, -6, 20], H=heads(max_q), seed=2, shape="chain")
     got, lse = run(c, max_q=max_q, return_lse=True)
     check(c, got, lse)
     assert not got[10:16].float().any()
@@ -153,7 +160,8 @@ def test_more_nodes_than_keys(cuda, max_q):
 @pytest.mark.parametrize("max_q", [1, 64])
 @pytest.mark.parametrize("B", [513, 1100])
 def test_many_requests(cuda, max_q, B):
-    c = make([1 + i % 4 for i in range(B)], [(7 * i) % 40 for i in range(B)], H=2, hkv=1, D=64, page=16, seed=B)
+    H = 2 if max_q == 1 else 32
+    c = make([1 + i % 4 for i in range(B)], [(7 * i) % 40 for i in range(B)], H=H, hkv=1, D=64, page=16, seed=B)
     check(c, run(c, max_q=max_q))
 
 
@@ -163,7 +171,8 @@ def test_nan_of_nodes_that_are_not_seen(cuda, max_q, kind):
     """NaN values (e4m3) in a node's place reach those that see it, and nobody else; scales of places that no row sees
     may be anything."""
     kw = KINDS[kind]
-    c = make([20, 9], [45, 3], page=16, seed=6)
+    H = heads(max_q)
+    c = make([20, 9], [45, 3], H=H, page=16, seed=6)
     base, page = 45, 16
     seen = do.paths(c["parents"][:20])
     node = 11
@@ -173,15 +182,16 @@ def test_nan_of_nodes_that_are_not_seen(cuda, max_q, kind):
     got = run(c, max_q=max_q, **kw)
     hit = torch.tensor([node in s for s in seen] + [False] * 9)
     assert hit.any() and not hit.all()
-    assert got.cpu()[hit][:, :4, 3].isnan().all()
+    assert got.cpu()[hit][:, :H // 2, 3].isnan().all()
     keep = torch.ones_like(got, dtype=torch.bool).cpu()
-    keep[hit.nonzero().flatten(), :4, 3] = False
+    keep[hit.nonzero().flatten(), :H // 2, 3] = False
     assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
 
 
 @pytest.mark.parametrize("max_q", [1, 64])
 def test_bad_pages_and_offsets(cuda, max_q):
-    c = make([13, 4], [50, 30], page=16, seed=4)
+    H = heads(max_q)
+    c = make([13, 4], [50, 30], H=H, page=16, seed=4)
     clean = run(c, max_q=max_q)
     c["table"][1][1] = 10 ** 6  # keys 16 .. 31 of the second request are left out
     got = run(c, max_q=max_q)
@@ -191,7 +201,7 @@ def test_bad_pages_and_offsets(cuda, max_q):
     c["table"][1][1] = 0
     tree = cp.tree_tables(ints(c["parents"]), ints(c["cu"]), ints(c["lens"]))
     c["cu"] = [0, 13, 12]
-    out = torch.full((17, 8, 128), 5.0, dtype=BF16, device="cuda")
+    out = torch.full((17, H, 128), 5.0, dtype=BF16, device="cuda")
     got = run(c, tree=tree, max_q=max_q, out=out)
     with pytest.raises(cp.ChiaError, match="BAD_INDEX"):
         cp.check_device_status(0)
@@ -203,7 +213,7 @@ def test_bad_pages_and_offsets(cuda, max_q):
 def test_words_of_any_kind(cuda, max_q):
     """Positions out of range and words with any bits: the result may be anything, but memory is not left, and what the
     bits beyond the tree say is not looked at."""
-    c = make([9, 64], [20, 100], seed=12)
+    c = make([9, 64], [20, 100], H=heads(max_q), seed=12)
     tree = cp.tree_tables(ints(c["parents"]), ints(c["cu"]), ints(c["lens"]))
     want = run(c, tree=tree, max_q=max_q)
     more = tree._replace(ancestors=tree.ancestors.clone())
@@ -211,7 +221,7 @@ def test_words_of_any_kind(cuda, max_q):
     assert torch.equal(run(c, tree=more, max_q=max_q), want)
     wild = tree._replace(positions=torch.where(tree.positions % 2 == 0, -2 ** 31, 2 ** 31 - 1).int(),
                          ancestors=torch.full_like(tree.ancestors, -1))
-    for kw in (dict(), dict(mod="alibi"), dict(mask=cp.Mask(left=3, right=0, dilation=2))):
+    for kw in (dict(), dict(mod="alibi", head_param=[0.5] * c["q"].shape[1]), dict(mask=cp.Mask(left=3, right=0, dilation=2))):
         assert run(c, tree=wild, max_q=max_q, **kw).shape == want.shape
     only = torch.arange(9).tolist() + torch.arange(64).tolist()  # nodes that see themselves and the context alone
     alone = tree._replace(ancestors=torch.tensor([1 << i if i < 63 else -2 ** 63 for i in only], device="cuda"),
@@ -232,7 +242,7 @@ def test_refusals(cuda):
 
 def test_streams_and_graphs(cuda):
     """Two streams at once, and a captured step that is replayed on new trees."""
-    c = make([13, 40, 2], [300, 20, 0], seed=8)
+    c = make([13, 40, 2], [300, 20, 0], H=32, seed=8)
     d = [c[n].cuda() for n in ("k", "v", "ks", "vs")]
     q, table, lens, cu, parents = c["q"].cuda(), ints(c["table"]), ints(c["lens"]), ints(c["cu"]), ints(c["parents"])
 
@@ -267,7 +277,7 @@ def test_streams_and_graphs(cuda):
 def test_steps_of_speculative_decoding(cuda, ct, page, dtype):
     """Three steps of all operators together. After each, the pages that requests hold and the free ones are all there
     is; the cache holds what appending the accepted tokens alone would have left, to the cache's precision."""
-    H, hkv, D, V, B, pages = 4, 2, 64, 300, 5, 60
+    H, hkv, D, V, B, pages = 16, 2, 64, 300, 5, 60  # (the kernel of few queries in the second step)
     g = torch.Generator().manual_seed(page)
     cache = cp.new_cache(pages, hkv, D, page_size=page, dtype=ct)
     table, ring = ints([[0] * 12] * B), torch.arange(pages, dtype=torch.int32, device="cuda")
