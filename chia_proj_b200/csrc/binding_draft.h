@@ -2,6 +2,9 @@
 #pragma once
 #include "binding_args.h"
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 namespace {
 
 decltype(&chia_tree_tables) g_tree_tables;
@@ -198,39 +201,64 @@ Rows rows_out(const Tensor &like) {
   return rows_of(o);
 }
 
+// The arguments of qk_norm_rope; weights and positions may be undefined.
+struct RopeIn {
+  Tensor q, k, qw, kw, freqs, pos;
+  double eps, offset;
+  bool inter;
+  RopeIn() = default;
+  // q, k, q_weight, k_weight, freqs, positions, eps, interleaved, weight_offset
+  RopeIn(const Args &a, int i) {
+    q = input(a, i, "q"), k = input(a, i + 1, "k");
+    if (!a.none(i + 2)) qw = a.tensor(i + 2, "q_weight", 1);
+    if (!a.none(i + 3)) kw = a.tensor(i + 3, "k_weight", 1);
+    freqs = a.tensor(i + 4, "freqs", 1);
+    if (!a.none(i + 5)) {
+      if (!THPVariable_Check(a.v[i + 5])) throw ValueError("positions must be a tensor");
+      const int64_t dim = THPVariable_Unpack(a.v[i + 5]).dim();
+      const bool each = q.dim() == 4 && dim == 2;  // of each batch entry
+      const int64_t shape[2] = {q.size(0), q.size(q.dim() == 3 ? 0 : 2)};
+      pos = a.ints(i + 5, "positions", each ? at::IntArrayRef(shape, 2) : at::IntArrayRef(shape + 1, 1), q.device());
+    }
+    eps = a.number(i + 6);
+    const int x = PyObject_IsTrue(a.v[i + 7]);
+    if (x < 0) throw 0;
+    inter = x;
+    offset = a.number(i + 8);
+  }
+  static const Tensor &input(const Args &a, int i, const char *name) {
+    if (!THPVariable_Check(a.v[i]) || (THPVariable_Unpack(a.v[i]).dim() != 3 && THPVariable_Unpack(a.v[i]).dim() != 4))
+      throw ValueError(std::string(name) + " must be a 3-D or 4-D tensor");
+    return a.tensor(i, name, THPVariable_Unpack(a.v[i]).dim());
+  }
+};
+
+// The same checked, as the library takes it.
 struct Rope {
   Rows q, k;
-  Tensor qw, kw, pos;
+  Tensor qw, kw;
   chia_rope_params_t p{};
-  // q, k, q_weight, k_weight, freqs, positions, eps, interleaved, weight_offset
-  explicit Rope(const Args &a, int i)
-      : q(rows_in(input(a, i, "q"))), k(rows_in(input(a, i + 1, "k"))) {
+  explicit Rope(const RopeIn &in) : q(rows_in(in.q)), k(rows_in(in.k)) {
     const Tensor &qt = q.t, &kt = k.t;
     const at::Device dev = qt.device();
     const int dt = any_type(qt);
+    no_tangent(in.q, "q"), no_tangent(in.k, "k");
     if (dt < 0) throw ValueError(std::string("dtype ") + c10::toString(qt.scalar_type()) + " unsupported (bf16, fp16 or fp32)");
     if (kt.scalar_type() != qt.scalar_type() || kt.device() != dev || kt.dim() != qt.dim() || k.b != q.b || k.s != q.s || k.d != q.d)
       throw ValueError("q " + str(qt.sizes()) + ", k " + str(kt.sizes()) + " must match in all but the heads, in dtype and in device");
     if (q.d != 64 && q.d != 128) throw ValueError("head_dim " + std::to_string(q.d) + " unsupported (64 or 128)");
     if (q.h < 1 || k.h < 1 || q.b < 1) throw ValueError("empty q or k");
-    weight(a, i + 2, "q_weight", dev, qw);
-    weight(a, i + 3, "k_weight", dev, kw);
+    qw = weight(in.qw, "q_weight"), kw = weight(in.kw, "k_weight");
     if (qw.defined() && kw.defined() && qw.scalar_type() != kw.scalar_type())
       throw ValueError("q_weight, k_weight must share a dtype");
-    const Tensor &freqs = a.tensor(i + 4, "freqs", 1);
-    if (freqs.scalar_type() != at::kLong || freqs.device() != dev || !freqs.is_contiguous())
+    if (in.freqs.scalar_type() != at::kLong || in.freqs.device() != dev || !in.freqs.is_contiguous())
       throw ValueError("freqs must be contiguous int64 on " + dev.str() + " (rope_frequencies makes them)");
-    const int64_t rot = 2 * freqs.size(0);
+    const int64_t rot = 2 * in.freqs.size(0);
     if (rot > q.d || rot % 8 != 0)
       throw ValueError("freqs for " + std::to_string(rot) + " channels: a multiple of 8 up to " + std::to_string(q.d));
-    if (!a.none(i + 5)) {
-      if (!THPVariable_Check(a.v[i + 5])) throw ValueError("positions must be a tensor");
-      const int64_t dim = THPVariable_Unpack(a.v[i + 5]).dim();
-      const bool each = qt.dim() == 4 && dim == 2;  // of each batch entry
-      const int64_t shape[2] = {q.b, q.s};
-      pos = a.ints(i + 5, "positions", each ? at::IntArrayRef(shape, 2) : at::IntArrayRef(shape + 1, 1), dev);
-      p.positions = ptr<int32_t>(pos);
-      if (each) p.position_stride = pos.stride(0);
+    if (in.pos.defined()) {
+      p.positions = ptr<int32_t>(in.pos);
+      if (in.pos.dim() == 2) p.position_stride = in.pos.stride(0);
     }
     p.abi_version = CHIA_ROPE_ABI_VERSION;
     p.dtype = dt;
@@ -246,90 +274,150 @@ struct Rope {
     for (int x = 0; x < 3; ++x) p.q_stride[x] = q.st[x], p.k_stride[x] = k.st[x];
     if (qw.defined()) p.q_weight = qw.data_ptr();
     if (kw.defined()) p.k_weight = kw.data_ptr();
-    p.freqs = ptr<uint64_t>(freqs);
-    p.eps = static_cast<float>(a.number(i + 6));
-    const int inter = PyObject_IsTrue(a.v[i + 7]);
-    if (inter < 0) throw 0;
-    p.interleaved = inter;
-    p.weight_offset = static_cast<float>(a.number(i + 8));
+    p.freqs = ptr<uint64_t>(in.freqs);
+    p.eps = static_cast<float>(in.eps);
+    p.interleaved = in.inter;
+    p.weight_offset = static_cast<float>(in.offset);
     if (!(p.eps >= 0.f) || !std::isfinite(p.eps) || !std::isfinite(p.weight_offset))
       throw ValueError("eps must be >= 0, eps and weight_offset finite");
   }
-  static const Tensor &input(const Args &a, int i, const char *name) {
-    if (!THPVariable_Check(a.v[i]) || (THPVariable_Unpack(a.v[i]).dim() != 3 && THPVariable_Unpack(a.v[i]).dim() != 4))
-      throw ValueError(std::string(name) + " must be a 3-D or 4-D tensor");
-    const Tensor &t = a.tensor(i, name, THPVariable_Unpack(a.v[i]).dim());
-    no_tangent(t, name);
-    return t;
-  }
-  void weight(const Args &a, int i, const char *name, const at::Device &dev, Tensor &to) {
-    if (a.none(i)) return;
-    const Tensor &w = a.tensor(i, name, 1);
-    if (w.size(0) != q.d || any_type(w) < 0 || w.device() != dev)
-      throw ValueError(std::string(name) + " must be bf16, fp16 or fp32 (" + std::to_string(q.d) + ",) on " + dev.str() + ", got " +
-                       c10::toString(w.scalar_type()) + " " + str(w.sizes()) + " on " + w.device().str());
+  Tensor weight(const Tensor &w, const char *name) const {
+    if (!w.defined()) return w;
+    if (w.size(0) != q.d || any_type(w) < 0 || w.device() != q.t.device())
+      throw ValueError(std::string(name) + " must be bf16, fp16 or fp32 (" + std::to_string(q.d) + ",) on " + q.t.device().str() +
+                       ", got " + c10::toString(w.scalar_type()) + " " + str(w.sizes()) + " on " + w.device().str());
     no_tangent(w, name);
-    to = w.is_contiguous() && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0
-             ? w
-             : w.detach().clone(at::MemoryFormat::Contiguous);
+    return w.is_contiguous() && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0
+               ? w
+               : w.detach().clone(at::MemoryFormat::Contiguous);
+  }
+  void *stream() const { return c10::cuda::getCurrentCUDAStream(q.t.device().index()).stream(); }
+};
+
+// Outputs in out; a status.
+int rope_forward(const RopeIn &in, Tensor (&out)[2]) {
+  Rope r(in);
+  const c10::cuda::CUDAGuard guard(r.q.t.device());
+  const Rows qo = rows_out(r.q.t), ko = rows_out(r.k.t);
+  r.p.q_out = qo.t.data_ptr(), r.p.k_out = ko.t.data_ptr();
+  for (int x = 0; x < 3; ++x) r.p.q_out_stride[x] = qo.st[x], r.p.k_out_stride[x] = ko.st[x];
+  out[0] = qo.t, out[1] = ko.t;
+  return g_rope(&r.p, r.stream());
+}
+
+// dq, dk, dq_weight, dk_weight (undefined where it is not wanted) in out; a status.
+int rope_backward(const RopeIn &in, const Tensor &dq_out, const Tensor &dk_out, bool want_qw, bool want_kw, Tensor (&out)[4]) {
+  Rope r(in);
+  const Tensor *dy[2] = {&dq_out, &dk_out};
+  const Rows *x[2] = {&r.q, &r.k};
+  Rows g[2];
+  for (int i = 0; i < 2; ++i) {
+    no_tangent(*dy[i], i ? "dk_out" : "dq_out");
+    if (dy[i]->sizes() != x[i]->t.sizes() || dy[i]->scalar_type() != x[i]->t.scalar_type() ||
+        dy[i]->device() != r.q.t.device())
+      throw ValueError(std::string(i ? "dk_out" : "dq_out") + " must match " + (i ? "k" : "q") + " in shape, dtype and device");
+    g[i] = rows_in(*dy[i]);
+  }
+  const c10::cuda::CUDAGuard guard(r.q.t.device());
+  const Rows dq = rows_out(r.q.t), dk = rows_out(r.k.t);
+  for (int i = 0; i < 3; ++i) r.p.q_out_stride[i] = dq.st[i], r.p.k_out_stride[i] = dk.st[i];
+  chia_rope_grads_t gr{};
+  gr.dq_out = g[0].t.data_ptr(), gr.dk_out = g[1].t.data_ptr();
+  for (int i = 0; i < 3; ++i) gr.dq_out_stride[i] = g[0].st[i], gr.dk_out_stride[i] = g[1].st[i];
+  gr.dq = dq.t.data_ptr(), gr.dk = dk.t.data_ptr();
+  out[0] = dq.t, out[1] = dk.t;
+  if (r.qw.defined() && want_qw) out[2] = at::empty({r.q.d}, r.qw.options().requires_grad(false)), gr.dq_weight = out[2].data_ptr();
+  if (r.kw.defined() && want_kw) out[3] = at::empty({r.q.d}, r.kw.options().requires_grad(false)), gr.dk_weight = out[3].data_ptr();
+  Tensor ws;
+  int64_t bytes = 0;
+  if (r.qw.defined() || r.kw.defined()) {
+    bytes = g_rope_bytes(&r.p);
+    if (bytes < 0) throw ValueError("invalid backward parameters");
+    ws = at::empty({bytes}, r.q.t.options().dtype(at::kByte).requires_grad(false));
+  }
+  return g_rope_bwd(&r.p, &gr, ws.defined() ? ws.data_ptr() : nullptr, bytes, r.stream());
+}
+
+PyObject *wrap(const Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
+
+// The graph's node of a call: its inputs are kept, the backward kernel computes the norms again. (As a
+// Python function of autograd's a step took 40 us of the host's time more.)
+struct RopeNode : torch::autograd::Function<RopeNode> {
+  using List = torch::autograd::variable_list;
+  using Context = torch::autograd::AutogradContext;
+  using Maybe = std::optional<Tensor>;  // (a weight that is not there has no edge)
+  static List forward(Context *ctx, const Tensor &q, const Tensor &k, const Maybe &, const Maybe &, const RopeIn *in) {
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    Tensor out[2];
+    const int code = rope_forward(*in, out);
+    if (code != CHIA_OK) throw std::runtime_error("chia_qk_norm_rope: status " + std::to_string(code));
+    ctx->save_for_backward({q, k, in->qw, in->kw, in->freqs, in->pos});
+    ctx->saved_data["eps"] = in->eps;
+    ctx->saved_data["offset"] = in->offset;
+    ctx->saved_data["inter"] = in->inter;
+    return {out[0], out[1]};
+  }
+  static List backward(Context *ctx, List grads) {
+    const List saved = ctx->get_saved_variables();
+    RopeIn in;
+    in.q = saved[0], in.k = saved[1], in.qw = saved[2], in.kw = saved[3], in.freqs = saved[4], in.pos = saved[5];
+    in.eps = ctx->saved_data["eps"].toDouble(), in.offset = ctx->saved_data["offset"].toDouble();
+    in.inter = ctx->saved_data["inter"].toBool();
+    Tensor out[4];
+    {
+      const at::AutoDispatchBelowADInplaceOrView plain;
+      const Tensor dq = grads[0].defined() ? grads[0] : at::zeros_like(in.q);
+      const Tensor dk = grads[1].defined() ? grads[1] : at::zeros_like(in.k);
+      size_t edge = 2;
+      const bool want_qw = in.qw.defined() && ctx->needs_input_grad(edge++);
+      const bool want_kw = in.kw.defined() && ctx->needs_input_grad(edge);
+      const int code = rope_backward(in, dq, dk, want_qw, want_kw, out);
+      if (code != CHIA_OK) throw std::runtime_error("chia_qk_norm_rope_bwd: status " + std::to_string(code));
+    }
+    List result = {out[0], out[1], out[2], out[3], Tensor()};
+    if (c10::GradMode::is_enabled()) {  // the gradients' own gradients are refused when they are asked for
+      List some;
+      for (const Tensor &t : out)
+        if (t.defined()) some.push_back(t.detach().set_requires_grad(true));  // (so that the results have a graph)
+      some = torch::autograd::DelayedError("qk_norm_rope has no second derivative", static_cast<int>(some.size())).apply(std::move(some));
+      for (int i = 0, j = 0; i < 4; ++i)
+        if (out[i].defined()) result[i] = some[j++];
+    }
+    return result;
   }
 };
 
-// the nine arguments of Rope
+// the nine arguments of RopeIn
 PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
-    const at::AutoDispatchBelowADInplaceOrView plain;
     const Args a(args, nargs, 9);
-    Rope r(a, 0);
-    const c10::cuda::CUDAGuard guard(r.q.t.device());
-    const Rows qo = rows_out(r.q.t), ko = rows_out(r.k.t);
-    r.p.q_out = qo.t.data_ptr(), r.p.k_out = ko.t.data_ptr();
-    for (int x = 0; x < 3; ++x) r.p.q_out_stride[x] = qo.st[x], r.p.k_out_stride[x] = ko.st[x];
-    const int code = g_rope(&r.p, c10::cuda::getCurrentCUDAStream(r.q.t.device().index()).stream());
-    if (code != CHIA_OK) return PyLong_FromLong(code);
-    return Py_BuildValue("(NN)", THPVariable_Wrap(qo.t), THPVariable_Wrap(ko.t));
+    const RopeIn in(a, 0);
+    Tensor out[2];
+    auto learns = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
+    if (c10::GradMode::is_enabled() && (learns(in.q) || learns(in.k) || learns(in.qw) || learns(in.kw))) {
+      auto maybe = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+      const auto r = RopeNode::apply(in.q, in.k, maybe(in.qw), maybe(in.kw), &in);
+      out[0] = r[0], out[1] = r[1];
+    } else {
+      const at::AutoDispatchBelowADInplaceOrView plain;
+      const int code = rope_forward(in, out);
+      if (code != CHIA_OK) return PyLong_FromLong(code);
+    }
+    return Py_BuildValue("(NN)", wrap(out[0]), wrap(out[1]));
   });
 }
 
-// dq_out, dk_out, then the nine arguments of Rope, want_q_weight, want_k_weight
+// dq_out, dk_out, then the nine arguments of RopeIn, want_q_weight, want_k_weight
 PyObject *qk_norm_rope_bwd(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
     const at::AutoDispatchBelowADInplaceOrView plain;
     const Args a(args, nargs, 13);
-    Rope r(a, 2);
-    const Tensor *dy[2] = {&Rope::input(a, 0, "dq_out"), &Rope::input(a, 1, "dk_out")};
-    const Rows *x[2] = {&r.q, &r.k};
-    Rows g[2];
-    for (int i = 0; i < 2; ++i) {
-      if (dy[i]->sizes() != x[i]->t.sizes() || dy[i]->scalar_type() != x[i]->t.scalar_type() ||
-          dy[i]->device() != r.q.t.device())
-        throw ValueError(std::string(i ? "dk_out" : "dq_out") + " must match " + (i ? "k" : "q") + " in shape, dtype and device");
-      g[i] = rows_in(*dy[i]);
-    }
-    const c10::cuda::CUDAGuard guard(r.q.t.device());
-    const Rows dq = rows_out(r.q.t), dk = rows_out(r.k.t);
-    for (int i = 0; i < 3; ++i) r.p.q_out_stride[i] = dq.st[i], r.p.k_out_stride[i] = dk.st[i];
-    chia_rope_grads_t gr{};
-    gr.dq_out = g[0].t.data_ptr(), gr.dk_out = g[1].t.data_ptr();
-    for (int i = 0; i < 3; ++i) gr.dq_out_stride[i] = g[0].st[i], gr.dk_out_stride[i] = g[1].st[i];
-    gr.dq = dq.t.data_ptr(), gr.dk = dk.t.data_ptr();
-    Tensor dw[2], ws;
-    const Tensor *w[2] = {&r.qw, &r.kw};
-    for (int i = 0; i < 2; ++i)
-      if (w[i]->defined() && PyObject_IsTrue(a.v[11 + i])) dw[i] = at::empty({r.q.d}, w[i]->options().requires_grad(false));
-    if (dw[0].defined()) gr.dq_weight = dw[0].data_ptr();
-    if (dw[1].defined()) gr.dk_weight = dw[1].data_ptr();
-    int64_t bytes = 0;
-    if (r.qw.defined() || r.kw.defined()) {
-      bytes = g_rope_bytes(&r.p);
-      if (bytes < 0) throw ValueError("invalid backward parameters");
-      ws = at::empty({bytes}, r.q.t.options().dtype(at::kByte).requires_grad(false));
-    }
-    const int code = g_rope_bwd(&r.p, &gr, ws.defined() ? ws.data_ptr() : nullptr, bytes,
-                                c10::cuda::getCurrentCUDAStream(r.q.t.device().index()).stream());
+    const Tensor &dq = RopeIn::input(a, 0, "dq_out"), &dk = RopeIn::input(a, 1, "dk_out");
+    const RopeIn in(a, 2);
+    Tensor out[4];
+    const int code = rope_backward(in, dq, dk, PyObject_IsTrue(a.v[11]), PyObject_IsTrue(a.v[12]), out);
     if (code != CHIA_OK) return PyLong_FromLong(code);
-    auto wrap = [](const Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); };
-    return Py_BuildValue("(NNNN)", THPVariable_Wrap(dq.t), THPVariable_Wrap(dk.t), wrap(dw[0]), wrap(dw[1]));
+    return Py_BuildValue("(NNNN)", wrap(out[0]), wrap(out[1]), wrap(out[2]), wrap(out[3]));
   });
 }
 

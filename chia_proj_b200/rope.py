@@ -53,11 +53,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     are taken as they are (strides that are multiples of 8 elements, unit last stride); outputs have their order of
     dimensions. ``q_weight``, ``k_weight`` ``[D]`` (bf16, fp16 or fp32; ``None``: ones, without the offset). Pair ``i`` is
     channels ``i`` and ``i + rot / 2``, or neighbours with ``interleaved``. ``freqs``: ``rope_frequencies``; an empty one
-    turns nothing. Computed in 32 bits and rounded once. Differentiable in ``q``, ``k`` and the weights.
+    turns nothing. Computed in 32 bits and rounded once. Differentiable in ``q``, ``k`` and the weights, once; only the inputs are kept for the backward pass.
     """
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                       for t in (q, k, q_weight, k_weight)):
-        return _QKNormRopeFn.apply(q, k, q_weight, k_weight, freqs, positions, eps, interleaved, weight_offset)
     r = N.binding().qk_norm_rope(q, k, q_weight, k_weight, freqs, positions, eps, interleaved, weight_offset)
     if type(r) is int:
         N.check(r, f"chia_qk_norm_rope(q={tuple(q.shape)}, k={tuple(k.shape)})")
@@ -76,24 +73,3 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     if type(r) is int:
         N.check(r, f"chia_qk_norm_rope_bwd(q={tuple(q.shape)}, k={tuple(k.shape)})")
     return r
-
-
-class _QKNormRopeFn(torch.autograd.Function):
-    """Autograd for ``qk_norm_rope``: only its inputs are kept, the backward kernel computes the norms again."""
-
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, freqs, positions, eps, interleaved, weight_offset):
-        with torch.no_grad():
-            out = qk_norm_rope(q, k, q_weight, k_weight, freqs, positions, eps=eps, interleaved=interleaved,
-                               weight_offset=weight_offset)
-        ctx.save_for_backward(q, k, q_weight, k_weight, freqs, positions)
-        ctx.kw = dict(eps=eps, interleaved=interleaved, weight_offset=weight_offset)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq_out, dk_out):
-        q, k, q_weight, k_weight, freqs, positions = ctx.saved_tensors
-        dq, dk, dqw, dkw = qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, freqs, positions,
-                                                 weight_grads=ctx.needs_input_grad[2:4], **ctx.kw)
-        return dq, dk, dqw, dkw, None, None, None, None, None

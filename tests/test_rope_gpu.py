@@ -185,9 +185,43 @@ def test_only_what_is_wanted(cuda):
     assert torch.equal(torch.autograd.grad(out, kw, [q, k])[0], full[3])
     some = cp.qk_norm_rope_backward(q, k, q, k, qw, kw, freqs, weight_grads=(True, False))
     assert some[3] is None and torch.equal(some[2], full[2]) and torch.equal(some[0], full[0])
+    qw.requires_grad_()
+    only_k = torch.autograd.grad(cp.qk_norm_rope(q, k, None, kw, freqs), kw, [q, k])[0]  # no weight before it
+    assert torch.equal(only_k, full[3])
+    assert torch.equal(torch.autograd.grad(cp.qk_norm_rope(q, k, qw, None, freqs), qw, [q, k])[0], full[2])
     none = cp.qk_norm_rope_backward(q, k, q, k, qw, None, freqs)
     assert none[3] is None and torch.equal(none[0], full[0])
-    assert not cp.qk_norm_rope(q.detach(), k.detach(), qw, kw.detach(), freqs)[0].requires_grad
+    assert not cp.qk_norm_rope(q, k, qw.detach(), kw.detach(), freqs)[0].requires_grad
+
+
+def test_one_output_and_second_derivatives(cuda):
+    q, k, qw, kw = make(1, 9, 2, 1, 64, F32, F32, seed=13, fused=False)
+    freqs = cp.rope_frequencies(64)
+    leaves = [t.requires_grad_() for t in (q, k, qw, kw)]
+    a, b = cp.qk_norm_rope(*leaves, freqs)
+    c = torch.randn(a.shape, device="cuda")
+    got = torch.autograd.grad((a * c).sum(), leaves, retain_graph=True)
+    want = cp.qk_norm_rope_backward(c, torch.zeros_like(k), q, k, qw, kw, freqs)
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and not got[1].any() and not got[3].any()
+    both = torch.autograd.grad((a, b), leaves, [c, torch.ones_like(k)])  # the same graph again
+    assert torch.equal(both[0], want[0]) and both[1].any()
+    a, _ = cp.qk_norm_rope(*leaves, freqs)
+    (g,) = torch.autograd.grad(a.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):  # (not a part of the graph)
+        torch.autograd.grad(g.sum(), q, retain_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.sum().backward()
+    a, _ = cp.qk_norm_rope(*leaves, freqs)
+    with torch.no_grad():
+        q.add_(1.0)  # what is kept must not change
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        a.sum().backward()
+    import threading
+    seen = []
+    x = q.detach().requires_grad_()
+    th = threading.Thread(target=lambda: seen.append(torch.autograd.grad(cp.qk_norm_rope(x, k, qw, kw, freqs)[0].sum(), x)[0]))
+    th.start(), th.join()
+    assert torch.equal(seen[0], torch.autograd.grad(cp.qk_norm_rope(x, k, qw, kw, freqs)[0].sum(), x)[0])
 
 
 def test_views_streams_and_empty_inputs(cuda):
