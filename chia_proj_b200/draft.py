@@ -28,16 +28,9 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as N
-from .paged import _status
+from .paged import TreeStep, _status
 
 __all__ = ["TreeStep", "Verified", "tree_tables", "verify_drafts", "cache_compact"]
-
-
-class TreeStep(NamedTuple):
-    """What ``tree_tables`` returns, for each token."""
-
-    positions: torch.Tensor  # [T] int32: the tokens before the tree, and the node's depth
-    ancestors: torch.Tensor  # [T] int64: bit i: node i is an ancestor, or the node itself
 
 
 class Verified(NamedTuple):

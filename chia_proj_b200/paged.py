@@ -27,7 +27,7 @@ import torch
 from . import _native as N
 from .ops import CAUSAL, Mask, _MODS, _NORMS, _cached_default, _param_tensor, _status_word
 
-__all__ = ["PAGE_SIZES", "PageStep", "new_cache", "page_tables", "release_pages", "cache_append",
+__all__ = ["PAGE_SIZES", "PageStep", "TreeStep", "new_cache", "page_tables", "release_pages", "cache_append",
            "paged_attention"]
 
 PAGE_SIZES = (16, 32, 64, 128)
@@ -40,6 +40,13 @@ class PageStep(NamedTuple):
     cu_q: torch.Tensor        # [B + 1] offsets of the requests' tokens
     seq_lens: torch.Tensor    # [B] lengths after the step
     free_state: torch.Tensor  # [2] the ring of free pages after the step
+
+
+class TreeStep(NamedTuple):
+    """What ``tree_tables`` (``draft.py``) returns, for each token of the trees of drafted tokens."""
+
+    positions: torch.Tensor  # [T] int32: the tokens before the tree, and the node's depth
+    ancestors: torch.Tensor  # [T] int64: bit i: node i is an ancestor, or the node itself
 
 
 def _status(t) -> int:
@@ -136,7 +143,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     head_param: Optional[Union[torch.Tensor, Sequence[float]]] = None,
                     sig_bias: float = 0.0, out_scale: float = 1.0,
                     out: Optional[torch.Tensor] = None, return_lse: bool = False,
-                    wait_limit_ns: int = 0, tree: Optional["TreeStep"] = None):
+                    wait_limit_ns: int = 0, tree: Optional[TreeStep] = None):
     """``attention`` of a step's queries over the paged cache.
 
     ``q`` ``[T, H, D]`` (bf16 or fp16), request ``b``'s queries in rows

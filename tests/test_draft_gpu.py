@@ -290,6 +290,64 @@ def test_compact_bad_values_are_reported(cuda):
     assert keep.tolist() == [100, 2] and all(torch.equal(a, b) for a, b in zip(big, was))
 
 
+# ------------------------------------------------------------ streams and graphs
+def test_streams_and_graphs(cuda):
+    """Two streams at once; captured calls replayed on new values."""
+    g = torch.Generator().manual_seed(21)
+    sizes = [9, 30, 1, 64]
+    cu = [sum(sizes[:i]) for i in range(5)]
+    parents = [p for i, n in enumerate(sizes) for p in do.tree(n, i)]
+    n, V = cu[-1], 5000
+    p, q, u = rows(n, V, g, torch.float32), rows(n, V, g, torch.float32), torch.rand(n, generator=g)
+    tokens = [t for b in range(4) for t in drawn(parents[cu[b]:cu[b + 1]], q[cu[b]:cu[b + 1]], g)]
+    dp, dq, du, dt, dpar, dcu = p.cuda(), q.cuda(), u.cuda(), ints(tokens), ints(parents), ints(cu)
+    lens, table = ints([s + 20 for s in sizes]), ints([[6 * b + i for i in range(6)] for b in range(4)])
+    cache = [t.cuda() for t in cache_of(24, 2, 16, 64, E4M3, g)]
+
+    def step(cache):
+        done = cp.verify_drafts(dp, dt, dpar, dcu, du, draft_probs=dq, max_tokens=8)
+        return [*done, cp.cache_compact(done.path, done.counts, dcu, lens, table, *cache), *cp.tree_tables(dpar, dcu, lens)]
+
+    first = [t.clone() for t in cache]
+    want = step(first)
+    assert want[0].tolist() == do.verify(p, tokens, parents, cu, u, q, 8)[0]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append([(c, step(c)) for c in [[t.clone() for t in cache] for _ in range(3)]])
+    torch.cuda.synchronize()
+    for runs in got:
+        for c, r in runs:
+            assert all(torch.equal(a, b) for a, b in zip(r, want))
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(c, first))
+    mine = [t.clone() for t in cache]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(mine)
+    u2 = torch.rand(n, generator=g)
+    du.copy_(u2)
+    for a, b in zip(mine, cache):
+        a.copy_(b)
+    graph.replay()
+    other = [t.clone() for t in cache]
+    again = step(other)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(mine, other))
+    assert out[0].tolist() == do.verify(p, tokens, parents, cu, u2, q, 8)[0]
+
+
+def test_autograd_sees_what_is_written(cuda):
+    """The cache's tensors have new versions; probabilities that learn are taken without a graph."""
+    cache = [t.cuda() for t in cache_of(4, 1, 16, 64, E4M3, torch.Generator().manual_seed(1))]
+    was = [t._version for t in cache]
+    cp.cache_compact(ints([[0, 3]]), ints([2]), ints([0, 5]), ints([9]), ints([[0, 1]]), *cache)
+    assert all(t._version > v for t, v in zip(cache, was))
+    p = torch.rand(3, 40, device="cuda", requires_grad=True)
+    r = cp.verify_drafts(p, ints([0, 1, 2]), ints([-1, 0, 1]), ints([0, 3]), torch.rand(3, device="cuda"), max_tokens=3)
+    assert not any(t.requires_grad for t in r)
+
+
 # -------------------------------------------------------------------- refusals
 def test_refusals(cuda):
     p, u, i = torch.rand(4, 9, device="cuda"), torch.rand(4, device="cuda"), ints([0, 0, 0, 0])

@@ -229,6 +229,18 @@ def test_words_of_any_kind(cuda, max_q):
     check(dict(c, parents=[-1] * 73), run(c, tree=alone, max_q=max_q))
 
 
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_trees_of_one_size_without_offsets(cuda, max_q):
+    c = make([12] * 5, [7, 0, 300, 64, 31], H=heads(max_q), seed=15)
+    d = [c[n].cuda() for n in ("k", "v", "ks", "vs")]
+    tree = cp.tree_tables(ints(c["parents"]), ints(c["cu"]), ints(c["lens"]))
+    q = c["q"].cuda().repeat_interleave(2, 0)[::2]  # (rows with a stride)
+    out = torch.zeros(60, 2 * q.shape[1], 128, dtype=BF16, device="cuda")[:, ::2]
+    got = cp.paged_attention(q, *d, ints(c["table"]), ints(c["lens"]), tree=tree, out=out, max_q=max(max_q, 12))
+    assert got.data_ptr() == out.data_ptr()
+    check(c, got)
+
+
 def test_refusals(cuda):
     c = make([4, 3], [10, 20], seed=1)
     tree = cp.tree_tables(ints(c["parents"]), ints(c["cu"]), ints(c["lens"]))
