@@ -151,11 +151,12 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
 }
 
 // TREE: requests of up to kTreeNodes queries are trees of drafted tokens, as in the split kernel.
-// Their units often have few rows: warps without any do no arithmetic. (Tried: for units of up to
-// 128 rows both halves of the softmax warps with the same rows, a key tile each by turns, joined at
-// the end: 291 us where this has 300 on 16 x 25 nodes over 16,000 keys, 207 and 212 on 32 x 16 over
-// 4,096, 337 and 330 on capped trees over up to 16,384. The conversion, four warps at 1,200 cycles a
-// tile beside the others, and the copies' way round are next to the softmax then.)
+// Measured (D 128, e4m3, bf16, 8 K/V heads): 8 x 64 nodes of 64 heads over 4,096 keys 119 us, 16 x 25
+// of 32 over 16,000 323, 32 x 1 to 64 of 64 over up to 16,384 keys, capped, 314. A tile takes 2,400
+// to 3,500 cycles whatever its rows: 1,140 of the conversion, 700 of waits for copies, 1,700 to 2,150
+// of the softmax. Tried for units of up to 128 rows: both halves of the softmax warps with the same
+// rows, a key tile each by turns, joined at the end: 291 and 300 us on 16 x 25 nodes, 337 and 330
+// capped; warps without rows that do no arithmetic: 325 and 314 capped.
 template <int D, int CT, int KIND, bool BF16, bool TREE>
 __global__ void __launch_bounds__(kTiledThreads, 1)
 paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -582,23 +583,11 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
         band32(a, pos, h.rq.len, lo, hi);
         const int pf = prefix_of(h);
         float m_run = SOFTMAX ? -INFINITY : -100.f, l_run = 0.f;
-        const bool idle = TREE && w * 128 + (warp & 3) * 32 >= h.un.rows;  // a warp without rows
         for (int i = 0; i < h.nt; ++i, ++cnt) {
           const int n = k + i;
           // (after a wait that ran out S is anything; the vote below ends the work before P is stored)
           const bool got =
               wait2(SC_FULL + n % SETS, (n / SETS) & 1, S_FULL + 2 * w + (cnt & 1), (cnt >> 1) & 1);
-          if (TREE && idle) {  // (in step with the others; what P holds for its rows is nobody's)
-            if (!warp_all(got)) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) {
-              ptx::mbar_arrive(bar(P_FULL + 2 * w + (cnt & 1)));
-              ptx::mbar_arrive(bar(SC_EMPTY + n % SETS));
-            }
-            continue;
-          }
           ptx::tc_fence_after();
           const uint32_t tS = tS0 + (cnt & 1) * 64;
           uint32_t sr[2][32];
