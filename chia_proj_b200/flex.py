@@ -31,8 +31,9 @@ flex requires.
 from __future__ import annotations
 
 import math
+import weakref
 from dataclasses import dataclass
-from typing import Callable, Dict, Optional, Tuple
+from typing import Callable, Optional, Tuple
 
 import torch
 
@@ -230,7 +231,22 @@ def identify_score_mod(score_mod: Optional[Callable], H: int, device) -> ScoreMo
                          "an ALiBi slope or a tanh softcap")
 
 
-_score_cache: Dict[tuple, ScoreMod] = {}
+# What a callable was identified as, as long as it lives. (Its address alone names nothing: another
+# callable may have it next.)
+_score_cache: "weakref.WeakKeyDictionary" = weakref.WeakKeyDictionary()
+
+
+def _score_of(score_mod: Optional[Callable], H: int, device) -> ScoreMod:
+    if score_mod is None:
+        return ScoreMod("none")
+    try:
+        known = _score_cache.setdefault(score_mod, {})
+    except TypeError:  # neither hashed nor referred to weakly
+        return identify_score_mod(score_mod, H, device)
+    key = (H, str(device))
+    if key not in known:
+        known[key] = identify_score_mod(score_mod, H, device)
+    return known[key]
 
 
 def flex_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -252,11 +268,7 @@ def flex_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
             raise ValueError(f"block_mask was made for {block_mask.shape}, "
                              f"inputs are {(Sq, Skv)}")
         mask = block_mask.mask
-    key_ = (id(score_mod), H, str(query.device))
-    sm = _score_cache.get(key_) if score_mod is not None else ScoreMod("none")
-    if sm is None:
-        sm = identify_score_mod(score_mod, H, query.device)
-        _score_cache[key_] = sm
+    sm = _score_of(score_mod, H, query.device)
     kw = {}
     if sm.mod == "softcap":
         kw["softcap"] = sm.softcap
