@@ -150,8 +150,11 @@ __device__ __forceinline__ void verify_prefetch(const void *p, int64_t e) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t *>(p) + e * (T == 2 ? 4 : 2)));
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 __device__ __forceinline__ int cluster_rank() {
   uint32_t r;
@@ -185,8 +188,10 @@ __global__ void __launch_bounds__(kVerifyMostThreads, 1) verify_kernel(const Ver
   __shared__ double s_warp[kVerifyMostThreads / 32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x / 32;
   const int rank = cluster_rank(), b = blockIdx.x / kVerifyCtas;
+  cluster_arrive();
   follow();
-  TreeRows r = tree_rows(a.cu_q, b, a.rows);
+  cluster_wait();  // all CTAs of the cluster run: their shared memory may be written
+  const TreeRows r = tree_rows(a.cu_q, b, a.rows);
   bool bad = r.n < 0 || r.n > kTreeNodes;
   int32_t *out = a.out + static_cast<int64_t>(b) * a.most, *path = a.path + static_cast<int64_t>(b) * a.most;
   if (r.n == 0 || bad) {

@@ -270,91 +270,173 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
     if (warp == 9) {
       // ==================================================== pages and TMA
       const int pshift = 31 - __clz(a.page), rows = min(a.page, TK);
-      // A lane looks up 16 keys of a tile, four lanes a tile, so eight tiles at a time: the pages of
-      // the next eight are asked for while the first of these are loaded, their scales four tiles
-      // later. (Looked up one tile ahead, a tile of few rows took 2,900 cycles, 2,100 of them this
-      // warp's waits for its loads.)
-      static_assert(GROUPS == 4, "four lanes a tile");
       struct Keys {
         int key, pg;
         int hk, all, live;  // all: bit 0 every row sees the tile, 1 no row these keys, 2 there are such keys
       };
-      const int grp = lane & 3;
-      auto page_of = [&](int k) {
-        Keys x{0, -1, 0, 0, 0};
-        if (k >= nk) return x;
-        const Here h = unit_at(k);
-        int y, lo_min, hi_max;
-        band32(a, h.p0 + div_group(a, h.un.row0), h.rq.len, lo_min, y);
-        band32(a, h.p0 + div_group(a, h.un.row0 + h.un.rows - 1), h.rq.len, y, hi_max);
-        if (TREE && h.rq.n <= kTreeNodes) {
-          band32(a, h.p0, h.rq.len, lo_min, y);
-          band32(a, h.rq.len - 1, h.rq.len, y, hi_max);
-        }
-        const int j0 = h.rq.tl.key_tile(h.ut0) * TK;
-        x.key = j0 + 16 * grp;
-        x.hk = h.un.hk;
-        x.all = sees_all(h, j0);
-        x.live = h.rq.len - j0;
-        // (the scales of 16 keys that no row sees may be anything)
-        if (!(x.key < prefix_of(h) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
-        if (x.key < h.rq.len) x.pg = a.block_table[h.rq.b * a.table_stride + (x.key >> pshift)], x.all |= 4;
-        return x;
-      };
       int issued = 0;
-      Keys now, next = page_of(lane >> 2);
-      int row = -1, next_row = -1;
-      float ks = 0.f, vs = 0.f, next_ks = 0.f, next_vs = 0.f;
-      auto ask_scales = [&] {
-        next_row = -1;
-        if (next.pg >= 0 && next.pg < a.num_pages) {
-          next_row = next.pg * a.heads_kv + next.hk;
-          next_ks = a.k_scale[next_row];
-          next_vs = a.v_scale[next_row];
-        }
-      };
-      ask_scales();
-      for (int k = 0; k < nk; ++k) {
-        const int in = k & 7;
-        if (in == 0) now = next, row = next_row, ks = next_ks, vs = next_vs;
-        // A softmax warp may be far behind: a query tile without rows takes part in no other wait
-        // for these tiles, and its warps may still be writing the unit before.
-        if (!warp_all(wait(SC_EMPTY + k % SETS, ((k / SETS) & 1) ^ 1))) break;
-        const bool me = (lane >> 2) == in;  // this lane's keys are of the tile
-        const bool bad = me && row < 0 && (now.all & 6) == 4;
-        const int lost = static_cast<int>(__ballot_sync(0xffffffffu, bad)) >> (4 * in) & 15;
-        if (bad) report(a.status, kStatusBadIndex);
-        if (me && grp == 0)
-          tile_full[k % SETS] = lost == 0 && (now.all & 1), tile_live[k % SETS] = now.live, tile_lost[k % SETS] = lost;
-        __syncwarp();
-        const bool leads = me && row >= 0 && (16 * grp) % rows == 0;
-        const int bytes = __popc(__ballot_sync(0xffffffffu, leads)) * rows * D;
-        bool ok = true;
-        for (int v = 0; v < 2 && ok; ++v) {
-          const int item = 2 * k + v, st = item % STAGES;
-          ok = warp_all(wait(ST_EMPTY + st, ((item / STAGES) & 1) ^ 1));
-          if (!ok) break;
-          if (lane == 0) ptx::mbar_arrive_expect_tx(bar(ST_FULL + st), bytes);
-          __syncwarp();
-          if (leads)
-            tma_load_3d(sb + C::OFF_ST + st * C::STAGE + 16 * grp * D, v ? &mv : &mk, bar(ST_FULL + st), 0,
-                        now.key & (a.page - 1), row);
-          ++issued;
-        }
-        if (!ok) break;
-        if (me) {
-          float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (row >= 0 && !(now.all & 2)) {
-            sc.x = ks;
-            sc.y = value_factor<SOFTMAX>(vs);
-            sc.z = SOFTMAX ? ptx::ex2(-sc.y) : 0.f;
+      if constexpr (TREE) {
+        // Trees: a lane looks up 16 keys of a tile, four lanes a tile, so eight tiles at a time: the pages
+        // of the next eight are asked for while the first of these are loaded, their scales four tiles
+        // later. (16 x 25 nodes over 16,000 keys 326 us, with the way below 348; without trees 302 and 296.)
+        static_assert(GROUPS == 4, "four lanes a tile");
+        const int grp = lane & 3;
+        auto page_of = [&](int k) {
+          Keys x{0, -1, 0, 0, 0};
+          if (k >= nk) return x;
+          const Here h = unit_at(k);
+          int y, lo_min, hi_max;
+          band32(a, h.p0 + div_group(a, h.un.row0), h.rq.len, lo_min, y);
+          band32(a, h.p0 + div_group(a, h.un.row0 + h.un.rows - 1), h.rq.len, y, hi_max);
+          if (h.rq.n <= kTreeNodes) {
+            band32(a, h.p0, h.rq.len, lo_min, y);
+            band32(a, h.rq.len - 1, h.rq.len, y, hi_max);
           }
-          scales[(k % SETS) * GROUPS + grp] = sc;
+          const int j0 = h.rq.tl.key_tile(h.ut0) * TK;
+          x.key = j0 + 16 * grp;
+          x.hk = h.un.hk;
+          x.all = sees_all(h, j0);
+          x.live = h.rq.len - j0;
+          // (the scales of 16 keys that no row sees may be anything)
+          if (!(x.key < prefix_of(h) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
+          if (x.key < h.rq.len) x.pg = a.block_table[h.rq.b * a.table_stride + (x.key >> pshift)], x.all |= 4;
+          return x;
+        };
+        Keys now, next = page_of(lane >> 2);
+        int row = -1, next_row = -1;
+        float ks = 0.f, vs = 0.f, next_ks = 0.f, next_vs = 0.f;
+        auto ask_scales = [&] {
+          next_row = -1;
+          if (next.pg >= 0 && next.pg < a.num_pages) {
+            next_row = next.pg * a.heads_kv + next.hk;
+            next_ks = a.k_scale[next_row];
+            next_vs = a.v_scale[next_row];
+          }
+        };
+        ask_scales();
+        for (int k = 0; k < nk; ++k) {
+          const int in = k & 7;
+          if (in == 0) now = next, row = next_row, ks = next_ks, vs = next_vs;
+          // A softmax warp may be far behind: a query tile without rows takes part in no other wait
+          // for these tiles, and its warps may still be writing the unit before.
+          if (!warp_all(wait(SC_EMPTY + k % SETS, ((k / SETS) & 1) ^ 1))) break;
+          const bool me = (lane >> 2) == in;  // this lane's keys are of the tile
+          const bool bad = me && row < 0 && (now.all & 6) == 4;
+          const int lost = static_cast<int>(__ballot_sync(0xffffffffu, bad)) >> (4 * in) & 15;
+          if (bad) report(a.status, kStatusBadIndex);
+          if (me && grp == 0)
+            tile_full[k % SETS] = lost == 0 && (now.all & 1), tile_live[k % SETS] = now.live, tile_lost[k % SETS] = lost;
+          __syncwarp();
+          const bool leads = me && row >= 0 && (16 * grp) % rows == 0;
+          const int bytes = __popc(__ballot_sync(0xffffffffu, leads)) * rows * D;
+          bool ok = true;
+          for (int v = 0; v < 2 && ok; ++v) {
+            const int item = 2 * k + v, st = item % STAGES;
+            ok = warp_all(wait(ST_EMPTY + st, ((item / STAGES) & 1) ^ 1));
+            if (!ok) break;
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(ST_FULL + st), bytes);
+            __syncwarp();
+            if (leads)
+              tma_load_3d(sb + C::OFF_ST + st * C::STAGE + 16 * grp * D, v ? &mv : &mk, bar(ST_FULL + st), 0,
+                          now.key & (a.page - 1), row);
+            ++issued;
+          }
+          if (!ok) break;
+          if (me) {
+            float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row >= 0 && !(now.all & 2)) {
+              sc.x = ks;
+              sc.y = value_factor<SOFTMAX>(vs);
+              sc.z = SOFTMAX ? ptx::ex2(-sc.y) : 0.f;
+            }
+            scales[(k % SETS) * GROUPS + grp] = sc;
+          }
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(SC_FULL + k % SETS));
+          if (in == 1) next = page_of(k - 1 + 8 + (lane >> 2));
+          if (in == 5) ask_scales();
         }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(SC_FULL + k % SETS));
-        if (in == 1) next = page_of(k - 1 + 8 + (lane >> 2));
-        if (in == 5) ask_scales();
+      } else {
+        // Of the tile's keys 16 lane .. + 15 (lanes 0-3). What a tile needs from
+        // memory is asked for a tile or two ahead and looked at when its turn
+        // comes: the page of tile k + 2, the scales of tile k + 1.
+        Here h;
+        int left = 0, lo_min = 0, hi_max = 0;  // tiles of the unit still to look up
+        auto page_of = [&](int k) {
+          Keys x{0, -1, 0, 0, 0};
+          if (k >= nk) return x;
+          if (left == 0) {
+            h = unit_at(k), left = h.nt;
+            int y;
+            band32(a, h.p0 + div_group(a, h.un.row0), h.rq.len, lo_min, y);
+            band32(a, h.p0 + div_group(a, h.un.row0 + h.un.rows - 1), h.rq.len, y, hi_max);
+          }
+          const int j0 = h.rq.tl.key_tile(h.ut0 + h.nt - left) * TK;
+          --left;
+          x.key = j0 + 16 * lane;
+          x.hk = h.un.hk;
+          x.all = sees_all(h, j0);
+          x.live = h.rq.len - j0;
+          // (the scales of 16 keys that no row sees may be anything)
+          if (!(x.key < min(a.prefix, h.rq.len) || (x.key <= hi_max && x.key + 15 >= lo_min))) x.all |= 2;
+          if (lane < GROUPS && x.key < h.rq.len) 
+            x.pg = a.block_table[h.rq.b * a.table_stride + (x.key >> pshift)], x.all |= 4;
+          return x;
+        };
+        Keys k1 = page_of(0);
+        int row1 = -1, row = -1;
+        float ks1 = 0.f, vs1 = 0.f, ks = 0.f, vs = 0.f;
+        auto scales_of = [&](const Keys &x) {
+          row1 = -1;
+          if (x.pg >= 0 && x.pg < a.num_pages) {
+            row1 = x.pg * a.heads_kv + x.hk;
+            ks1 = a.k_scale[row1];
+            vs1 = a.v_scale[row1];
+          }
+        };
+        scales_of(k1);
+        Keys k2 = page_of(1);
+        for (int k = 0; k < nk; ++k) {
+          // A softmax warp may be far behind: a query tile without rows takes part in no other wait
+          // for these tiles, and its warps may still be writing the unit before.
+          if (!warp_all(wait(SC_EMPTY + k % SETS, ((k / SETS) & 1) ^ 1))) break;
+          const Keys now = k1;
+          row = row1, ks = ks1, vs = vs1;
+          const bool bad = row < 0 && (now.all & 6) == 4;
+          const int lost = static_cast<int>(__ballot_sync(0xffffffffu, bad));
+          if (bad) report(a.status, kStatusBadIndex);
+          if (lane < GROUPS) {
+            float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row >= 0 && !(now.all & 2)) {
+              sc.x = ks;
+              sc.y = value_factor<SOFTMAX>(vs);
+              sc.z = SOFTMAX ? ptx::ex2(-sc.y) : 0.f;
+            }
+            scales[(k % SETS) * GROUPS + lane] = sc;
+          }
+          if (lane == 0)
+            tile_full[k % SETS] = lost == 0 && (now.all & 1), tile_live[k % SETS] = now.live, tile_lost[k % SETS] = lost;
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(SC_FULL + k % SETS));
+          k1 = k2;
+          scales_of(k1);
+          k2 = page_of(k + 2);
+          const bool leads = lane < GROUPS && row >= 0 && (16 * lane) % rows == 0;
+          const int bytes = __popc(__ballot_sync(0xffffffffu, leads)) * rows * D;
+          bool ok = true;
+          for (int v = 0; v < 2 && ok; ++v) {
+            const int item = 2 * k + v, st = item % STAGES;
+            ok = warp_all(wait(ST_EMPTY + st, ((item / STAGES) & 1) ^ 1));
+            if (!ok) break;
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(ST_FULL + st), bytes);
+            __syncwarp();
+            if (leads)
+              tma_load_3d(sb + C::OFF_ST + st * C::STAGE + 16 * lane * D, v ? &mv : &mk, bar(ST_FULL + st), 0,
+                          now.key & (a.page - 1), row);
+            ++issued;
+          }
+          if (!ok) break;
+        }
       }
       // no copy is in flight when the CTA exits
       PagedArgs d = a;
