@@ -14,7 +14,11 @@
 // reduction is exact for any position; of its upper 32 bits sine and cosine are computed.
 //
 // Sums are in 32 bits; the output is rounded once. Bound by HBM, and next to it by the
-// number of instructions.
+// number of instructions. Measured, bf16, D 128: 4 x 4,096 tokens of 16 + 16 heads forward 46.9 us
+// (5.7 TB/s, 89% of the rate of a copy), backward 79.7 (5.1 TB/s); 16,421 tokens of 32 + 8 heads out
+// of one projection, half of the channels turned, 60.1 (5.6 TB/s); one token 2.9. Tried: a block of
+// tokens a CTA with the angles in shared memory, forward 53.2 and backward 114; rows through
+// rings of asynchronous copies, 74.6 and 114 (240 instructions a warp and pair of rows where this has 124).
 #pragma once
 #include "paged_common.cuh"
 
@@ -223,7 +227,9 @@ __device__ __forceinline__ void rope_angles(const uint64_t (&turn)[4], uint64_t 
 //   dw = sum of g xhat,   dx = rstd (g w - xhat mean(g w xhat));
 // x and the gradient are read once, so the row's rstd is computed again. Sums of dw stay in
 // registers while a group goes on from token to token; they are added up by group, by CTA
-// and in the kernel below in an order that is always the same.
+// and in the kernel below in an order that is always the same. The backward kernel asks for the
+// next rows before it computes these: 108 us without, and 80 at 128 registers a thread; forward,
+// eight CTAs an SM of 64 registers do as much.
 template <int T, int D, bool INTER, bool BACK>
 __global__ void __launch_bounds__(kRopeThreads, BACK ? 4 : 8) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int LANES = D / 8, GROUPS = kRopeThreads / LANES, SIZE = T == ROPE_F32 ? 4 : 2;

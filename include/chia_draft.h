@@ -57,7 +57,8 @@ CHIA_API int chia_tree_tables(const chia_tree_params_t *params, void *stream);
 /* chia_paged_attn for trees: a node sees the keys before its tree that the mask
  * shows to its position, and of the tree's keys those in its word that the mask does
  * not put too far back (win_left, the begin of a block, the dilation, of positions;
- * score modifications likewise). The workspace is that of chia_paged_attn. positions and ancestors are those of chia_tree_tables; a position outside of its
+ * score modifications likewise). The workspace is that of chia_paged_attn.
+ * positions and ancestors are those of chia_tree_tables; a position outside of its
  * request's tokens counts as the nearest inside. The words may hold any nodes of
  * the request. Requests of more than CHIA_TREE_NODES queries are served as by
  * chia_paged_attn. */

@@ -302,6 +302,24 @@ def test_in_a_graph(cuda):
     del alive
 
 
+@pytest.mark.parametrize("dtype,code", [(BF16, 0), (F32, 2)])
+def test_in_place_through_the_c_abi(lib, cuda, dtype, code):
+    import ctypes
+
+    from chia_proj_b200 import _native as N
+    q, k, qw, kw = make(2, 37, 6, 2, 128, dtype, dtype, seed=17, fused=False)
+    freqs = cp.rope_frequencies(64)
+    want = cp.qk_norm_rope(q, k, qw, kw, freqs)
+    p = N.RopeParams(abi_version=N.ROPE_ABI_VERSION, dtype=code, weight_dtype=code, head_dim=128, heads=6, heads_kv=2,
+                     rot=64, batch=2, seqlen=37, q=q.data_ptr(), k=k.data_ptr(), q_out=q.data_ptr(), k_out=k.data_ptr(),
+                     q_weight=qw.data_ptr(), k_weight=kw.data_ptr(), freqs=freqs.data_ptr(), eps=EPS)
+    for f, t in (("q_stride", q), ("q_out_stride", q), ("k_stride", k), ("k_out_stride", k)):
+        getattr(p, f)[:] = t.stride()[:3]
+    stream = ctypes.c_void_p(torch.cuda.current_stream(cuda).cuda_stream)
+    assert lib.chia_qk_norm_rope(bytes(p), stream) == 0
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
 def test_refusals(cuda):
     q, k, qw, kw = make(1, 4, 4, 2, 64, BF16, BF16, seed=1, fused=False)
     f, pos = cp.rope_frequencies(64), torch.arange(4, dtype=torch.int32, device="cuda")
