@@ -44,7 +44,8 @@ def tables(parents, cu, lens, rows):
 def attention(q, k, v, ks, vs, table, lens, cu, parents, *, norm="softmax", mod="none", mask=None, scale=None,
               softcap=30.0, head_param=None, sig_bias=0.0, out_scale=1.0):
     """64-bit (out, lse, mass) as ``paged_oracle.attention``: each row attends to a cache of its own, the keys before the
-    tree and its ancestors' in a row, where it is the last token."""
+    tree and its ancestors' in a row, where it is the last token. More than 64 queries are a chunk, which attends as
+    without trees."""
     T, H, D = q.shape
     hkv, page = k.shape[1], k.shape[2]
     out, mass = torch.zeros(T, H, D, dtype=torch.float64), torch.zeros(T, H, D, dtype=torch.float64)
@@ -58,11 +59,15 @@ def attention(q, k, v, ks, vs, table, lens, cu, parents, *, norm="softmax", mod=
         pg = torch.as_tensor(table[b][:po.pages_for(n, page)])
         kk = (k[pg].double() * ks[pg].double()[:, :, None, None]).transpose(0, 1).reshape(hkv, -1, D)[:, :n]
         vv = (v[pg].double() * vs[pg].double()[:, :, None, None]).transpose(0, 1).reshape(hkv, -1, D)[:, :n]
-        seen = paths(parents[t0:t1]) if m <= 64 else [list(range(i + 1)) for i in range(m)]
+        seen = paths(parents[t0:t1]) if m <= 64 else [None] * m
         for i, path in enumerate(seen):
-            keys = list(range(max(0, n - m))) + [n - m + x for x in path if n - m + x >= 0]
-            pos = [j for j in range(max(0, n - m))] + [n - m + d for d, x in enumerate(path) if n - m + x >= 0]
-            at = n - m + len(path) - 1
+            if path is None:  # a chunk: as without trees, the mask alone says what a query sees
+                keys = pos = list(range(n))
+                at = n - m + i
+            else:
+                keys = list(range(max(0, n - m))) + [n - m + x for x in path if n - m + x >= 0]
+                pos = [j for j in range(max(0, n - m))] + [n - m + d for d, x in enumerate(path) if n - m + x >= 0]
+                at = n - m + len(path) - 1
             keep = []
             for key, j in zip(keys, pos):
                 ok = mask.left < 0 or at - j <= mask.left

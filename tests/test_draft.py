@@ -13,6 +13,7 @@ import torch
 
 import chia_proj_b200 as cp
 import draft_oracle as do
+import paged_oracle as po
 from chia_proj_b200 import _native as N
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -199,3 +200,22 @@ def test_verification_draws_from_the_target():
         first[out[0][0]] += 1
     for x in range(4):
         assert abs(first[x] / n - float(p[0, x])) < 0.0142
+
+
+@pytest.mark.parametrize("mask", [cp.CAUSAL, cp.FULL, cp.Mask(right=0, prefix=38), cp.Mask(left=5, right=9),
+                                  cp.Mask(left=10, right=0, prefix=60, dilation=2), cp.Mask(right=0, block=24)])
+@pytest.mark.parametrize("base", [0, 1, 40, -5])
+def test_chunks_attend_as_without_trees(mask, base):
+    """The restatement's own: more than 64 queries are no tree, whatever the mask and the parents."""
+    g, n, H, hkv, D, page = torch.Generator().manual_seed(3), 70, 4, 2, 8, 16
+    length = n + base
+    pages = po.pages_for(length, page)
+    q = torch.randn(n, H, D, generator=g)
+    k, v = torch.randn(pages, hkv, page, D, generator=g), torch.randn(pages, hkv, page, D, generator=g)
+    ks, vs = torch.ones(pages, hkv), torch.ones(pages, hkv)
+    a = (q, k, v, ks, vs, [list(range(pages))], [length], [0, n])
+    want, got = po.attention(*a, mask=mask), do.attention(*a, [-1] * n, mask=mask)
+    for x, y in zip(got, want):
+        fin = torch.isfinite(y)
+        assert torch.equal(fin, torch.isfinite(x))
+        assert (x - y)[fin].abs().max() < 1e-12

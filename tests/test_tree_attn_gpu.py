@@ -149,6 +149,18 @@ def test_chunks_beside_trees(cuda, max_q):
 
 
 @pytest.mark.parametrize("max_q", [1, 64])
+@pytest.mark.parametrize("mask", [cp.Mask(right=0, prefix=38), cp.Mask(left=12, right=0, prefix=38, dilation=3),
+                                  cp.Mask(left=10, right=0, prefix=60), cp.Mask(left=5, right=9), cp.FULL])
+@pytest.mark.parametrize("sizes,bases", [([90, 5], [1, 40]), ([5, 65, 20, 130], [40, 10, 0, 0])])
+def test_chunks_beside_trees_see_what_follows(cuda, max_q, mask, sizes, bases):
+    """A chunk that begins inside the prefix sees all of it, with a mask that shows later keys also those: what the call
+    without trees gives it."""
+    c = make(sizes, bases, H=heads(max_q), page=32, seed=5)
+    got, lse = run(c, max_q=max_q, mask=mask, return_lse=True)
+    check(c, got, lse, mask=mask)
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
 def test_more_nodes_than_keys(cuda, max_q):
     """Lengths that do not hold the tree: the first nodes have no place in the cache, and none for a first node's row."""
     c = make([10, 6, 3], [-4, -6, 20], H=heads(max_q), seed=2, shape="chain")
