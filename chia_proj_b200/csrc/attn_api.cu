@@ -42,6 +42,11 @@ struct Derived {
   int vdil;       // 1, or d for the dilated fast path
 };
 
+// Numbers of a mask that lie beyond any position (S <= 2^30) say the same at 2^30. Clipped, their sums
+// with positions stay in 64 bits, and a dilation in the kernels' 32, where one of 2^31 or 2^32 would be
+// negative or zero: a step that no loop over a tile's columns gets past its end with.
+int64_t clip(int64_t x, int bits = 30) { return x < (int64_t(1) << bits) ? x : int64_t(1) << bits; }
+
 int derive(const chia_attn_params_t *p, Derived &out) {
   if (p->win_left < -1 || p->win_right < -1 || p->block < 0 || p->prefix < 0 ||
       p->dilation < 1)
@@ -49,11 +54,11 @@ int derive(const chia_attn_params_t *p, Derived &out) {
   MaskGeom g{};
   g.sq = p->seqlen_q;
   g.skv = p->seqlen_kv;
-  g.left = p->win_left;
-  g.right = p->win_right;
-  g.block = p->block;
+  g.left = clip(p->win_left);
+  g.right = clip(p->win_right);
+  g.block = clip(p->block);
   g.prefix = p->prefix < p->seqlen_kv ? p->prefix : p->seqlen_kv;
-  g.dil = p->dilation;
+  g.dil = clip(p->dilation);
   g.seg = p->seq_offsets;
   g.nseg = p->num_seqs;
   out.vdil = 1;
@@ -77,9 +82,9 @@ MaskGeom real_geom(const chia_attn_params_t *p) {
   MaskGeom g{};
   g.sq = p->seqlen_q;
   g.skv = p->seqlen_kv;
-  g.left = p->win_left;
-  g.right = p->win_right;
-  g.block = p->block;
+  g.left = clip(p->win_left, 62);
+  g.right = clip(p->win_right, 62);
+  g.block = clip(p->block, 62);
   g.prefix = p->prefix < p->seqlen_kv ? p->prefix : p->seqlen_kv;
   g.dil = p->dilation;
   return g;
