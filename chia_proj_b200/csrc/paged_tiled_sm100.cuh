@@ -687,8 +687,9 @@ paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant
               uint32_t m = lo > hi ? 0u : below(hi + 1 - k0) & ~below(lo - k0);
               if (a.dil != 1) {
                 uint32_t every = 0;
-                int first = (pos - k0) % a.dil;
-                for (int e = first < 0 ? first + a.dil : first; e < 32; e += a.dil) every |= 1u << e;
+                const int first = (pos - k0) % a.dil;
+                const int by = min(a.dil, 32);  // (a step of up to 2^31 - 1 would wrap around and come back)
+                for (int e = first < 0 ? first + a.dil : first; e < 32; e += by) every |= 1u << e;
                 m &= every;
               }
               m |= below(pf - k0);

@@ -10,6 +10,8 @@ import pytest
 import torch
 
 import chia_proj_b200 as cp
+import paged_oracle as po
+import test_tree_attn_gpu as ta
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -62,3 +64,19 @@ def test_windows_and_blocks(cuda, far):
         x, y = (cp.attention(a, k, v, mask=m).float() for m in (mask, want))
         assert ((x - y).abs() <= 2.0 ** -6 * y.abs() + 2.0 ** -9).all()
     assert cp.visible_pairs(cp.Mask(left=far, right=far, block=far), 300) == 300 * 300
+
+
+@pytest.mark.parametrize("max_q", [1, 128])  # the kernel for few rows, and that for many
+@pytest.mark.parametrize("dilation", [33, 2 ** 31 - 31, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 31, 2 ** 40])
+@pytest.mark.parametrize("prefix", [0, 21])
+def test_dilations_over_the_paged_cache(cuda, max_q, dilation, prefix):
+    """With trees and without; tolerances as in ``test_tree_attn_gpu.py``."""
+    mask = cp.Mask(left=-1, right=0, prefix=prefix, dilation=dilation)
+    c = ta.make([13, 64, 90, 1], [50, 20, 5, 130], H=ta.heads(max_q), seed=6)  # (90: a chunk)
+    got, lse = ta.run(c, max_q=max_q, mask=mask, return_lse=True)
+    ta.check(c, got, lse, mask=mask)
+    d = [c[n].cuda() for n in ("k", "v", "ks", "vs")]
+    table, lens, cu = (ta.ints(c[n]) for n in ("table", "lens", "cu"))
+    got = cp.paged_attention(c["q"].cuda(), *d, table, lens, cu, max_q=max_q, mask=mask)
+    out, _, mass = po.attention(c["q"], c["k"], c["v"], c["ks"], c["vs"], c["table"], c["lens"], c["cu"], mask=mask)
+    assert ((got.double().cpu() - out).abs() <= 2.0 ** -8 * out.abs() + 2.0 ** -10 * mass + 2.0 ** -24).all()
