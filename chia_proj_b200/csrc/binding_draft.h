@@ -375,13 +375,15 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
       if (code != CHIA_OK) throw std::runtime_error("chia_qk_norm_rope_bwd: status " + std::to_string(code));
     }
     List result = {out[0], out[1], out[2], out[3], Tensor()};
-    if (c10::GradMode::is_enabled()) {  // the gradients' own gradients are refused when they are asked for
-      List some;
-      for (const Tensor &t : out)
-        if (t.defined()) some.push_back(t.detach().set_requires_grad(true));  // (so that the results have a graph)
-      some = torch::autograd::DelayedError("qk_norm_rope has no second derivative", static_cast<int>(some.size())).apply(std::move(some));
-      for (int i = 0, j = 0; i < 4; ++i)
-        if (out[i].defined()) result[i] = some[j++];
+    if (c10::GradMode::is_enabled()) {
+      // The gradients' own gradients are refused when they are asked for: each gets a node that throws, with
+      // edges to all that the gradients depend on, so that whatever leads to one of them leads through it.
+      List all;
+      for (int i = 0; i < 4; ++i) all.push_back(out[i].defined() ? out[i].detach() : Tensor());
+      for (const Tensor &t : {in.q, in.k, in.qw, in.kw, grads[0], grads[1]}) all.push_back(t);
+      all = torch::autograd::DelayedError("qk_norm_rope has no second derivative", static_cast<int>(all.size())).apply(std::move(all));
+      for (int i = 0; i < 4; ++i)
+        if (out[i].defined()) result[i] = all[i];
     }
     return result;
   }
