@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -141,13 +142,18 @@ struct Cache {
   }
 };
 
-// Any C++ exception ends here as a Python one.
+// Any C++ exception ends here as a Python one; one that Python threw below (a hook of saved tensors: a
+// checkpoint stops its second run by one) goes on as it is.
 template <class F>
 PyObject *guarded(F f) {
   try {
     return f();
   } catch (int) {
     return nullptr;  // the Python error is set
+  } catch (python_error &e) {
+    e.restore();
+  } catch (py::error_already_set &e) {
+    e.restore();
   } catch (const ValueError &e) {
     PyErr_SetString(PyExc_ValueError, e.what());
   } catch (const c10::Error &e) {

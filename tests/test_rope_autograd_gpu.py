@@ -1,8 +1,9 @@
 """The graph's node of qk_norm_rope among PyTorch's other tools: second derivatives are refused by whatever way they are asked
-for, tensors that are saved elsewhere come back, transforms are refused."""
+for, tensors that are saved elsewhere come back, a checkpoint computes again, transforms are refused."""
 
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 import chia_proj_b200 as cp
 from test_rope_gpu import BF16, F32, make
@@ -90,6 +91,41 @@ def test_saved_elsewhere(cuda):
     with torch.autograd.graph.save_on_cpu():
         a, _ = cp.qk_norm_rope(odd, *x[1:], freqs, pos)
     assert torch.equal(torch.autograd.grad(a.float().square().sum(), odd)[0], want[0])
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpoint(cuda, reentrant):
+    x, freqs = leaves(seed=15), cp.rope_frequencies(64)
+
+    def part(q, k):
+        a, b = cp.qk_norm_rope(q, k, x[2], x[3], freqs)
+        return a * 2, b * 3
+    want = part(x[0], x[1])
+    want = torch.autograd.grad(want[0].sum() + want[1].square().sum(), x)
+    a, b = checkpoint(part, x[0], x[1], use_reentrant=reentrant)
+    if reentrant:
+        (a.sum() + b.square().sum()).backward()
+        got = [t.grad for t in x]
+    else:
+        got = torch.autograd.grad(a.sum() + b.square().sum(), x)
+    assert all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+def test_errors_of_hooks_come_through(cuda):
+    class Stop(Exception):
+        pass
+
+    def refuse(t):
+        raise Stop("no room")
+    x, freqs = leaves(), cp.rope_frequencies(64)
+    with torch.autograd.graph.saved_tensors_hooks(refuse, lambda t: t):
+        with pytest.raises(Stop, match="no room"):
+            cp.qk_norm_rope(*x, freqs)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, refuse):
+        a, _ = cp.qk_norm_rope(*x, freqs)
+    with pytest.raises(Stop, match="no room"):
+        a.sum().backward()
+    torch.autograd.grad(cp.qk_norm_rope(*x, freqs)[0].sum(), x)
 
 
 def test_transforms_are_refused(cuda):
