@@ -96,8 +96,8 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (T == 0) Py_RETURN_NONE;
     const c10::cuda::CUDAGuard guard(c.dev);
     Tensor kc, vc;
-    if (!fits(*k)) kc = k->detach().contiguous(), k = &kc;
-    if (!fits(*v)) vc = v->detach().contiguous(), v = &vc;
+    if (!fits(*k)) kc = fitting(*k), k = &kc;
+    if (!fits(*v)) vc = fitting(*v), v = &vc;
     chia_append_params_t p{};
     p.abi_version = CHIA_PAGED_ABI_VERSION;
     p.dtype = dt;
@@ -206,7 +206,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     max_q = std::max<int64_t>(1, std::min(max_q, T));
     const c10::cuda::CUDAGuard guard(c.dev);
     Tensor qc;
-    if (!fits(*q)) qc = q->detach().contiguous(), q = &qc;
+    if (!fits(*q)) qc = fitting(*q), q = &qc;
     chia_paged_params_t p{};
     Tensor out, hp, lse;
     if (a.none(17)) {

@@ -89,6 +89,9 @@ int value_type(const Tensor &t) {
   return t.scalar_type() == at::kBFloat16 ? CHIA_DTYPE_BF16 : t.scalar_type() == at::kHalf ? CHIA_DTYPE_F16 : -1;
 }
 
+// A dense copy at an address of its own (contiguous() gives back a dense tensor as it is, wherever it begins).
+Tensor fitting(const Tensor &t) { return t.detach().clone(at::MemoryFormat::Contiguous); }
+
 // Unit stride on the channels, 16-byte aligned rows; a copy where it is not so.
 bool fits(const Tensor &t) {
   return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) >= 0 &&

@@ -193,7 +193,7 @@ Rows rows_of(const Tensor &t) {
   return r;
 }
 // An input: a copy where its rows are not 16-byte aligned with unit stride.
-Rows rows_in(const Tensor &t) { return rows_of(rows_fit(t) ? t : t.detach().contiguous()); }
+Rows rows_in(const Tensor &t) { return rows_of(rows_fit(t) ? t : fitting(t)); }
 // A new tensor like an input, in its order of dimensions.
 Rows rows_out(const Tensor &like) {
   Tensor o = at::empty_like(like, like.options().requires_grad(false));

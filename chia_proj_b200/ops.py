@@ -175,7 +175,8 @@ def _cached_default(kind: str, H: int, device: torch.device) -> torch.Tensor:
 def _prep(x: torch.Tensor) -> torch.Tensor:
     """Make a tensor TMA-compatible: unit last stride, 16-byte aligned rows."""
     if x.stride(-1) != 1 or any(s % 8 for s in x.stride()[:-1]) or x.data_ptr() % 16:
-        x = x.contiguous()
+        # (contiguous() gives back a dense tensor as it is, wherever it begins)
+        x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
