@@ -340,6 +340,10 @@ int rope_backward(const RopeIn &in, const Tensor &dq_out, const Tensor &dk_out, 
 
 PyObject *wrap(const Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
 
+struct Status {  // other than CHIA_OK, on its way to the function that returns it
+  int code;
+};
+
 // The graph's node of a call: its inputs are kept, the backward kernel computes the norms again. (As a
 // Python function of autograd's a step took 40 us of the host's time more.)
 struct RopeNode : torch::autograd::Function<RopeNode> {
@@ -350,7 +354,7 @@ struct RopeNode : torch::autograd::Function<RopeNode> {
     const at::AutoDispatchBelowADInplaceOrView plain;
     Tensor out[2];
     const int code = rope_forward(*in, out);
-    if (code != CHIA_OK) throw std::runtime_error("chia_qk_norm_rope: status " + std::to_string(code));
+    if (code != CHIA_OK) throw Status{code};
     ctx->save_for_backward({q, k, in->qw, in->kw, in->freqs, in->pos});
     ctx->saved_data["eps"] = in->eps;
     ctx->saved_data["offset"] = in->offset;
@@ -398,8 +402,12 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     auto learns = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
     if (c10::GradMode::is_enabled() && (learns(in.q) || learns(in.k) || learns(in.qw) || learns(in.kw))) {
       auto maybe = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-      const auto r = RopeNode::apply(in.q, in.k, maybe(in.qw), maybe(in.kw), &in);
-      out[0] = r[0], out[1] = r[1];
+      try {
+        const auto r = RopeNode::apply(in.q, in.k, maybe(in.qw), maybe(in.kw), &in);
+        out[0] = r[0], out[1] = r[1];
+      } catch (const Status &s) {
+        return PyLong_FromLong(s.code);
+      }
     } else {
       const at::AutoDispatchBelowADInplaceOrView plain;
       const int code = rope_forward(in, out);

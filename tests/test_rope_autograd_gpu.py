@@ -128,6 +128,16 @@ def test_errors_of_hooks_come_through(cuda):
     torch.autograd.grad(cp.qk_norm_rope(*x, freqs)[0].sum(), x)
 
 
+@pytest.mark.parametrize("learns", [False, True])
+def test_errors_of_the_library(cuda, learns):
+    """The same error with gradients and without."""
+    q, k = torch.zeros(1, 20000, 64, device="cuda", requires_grad=learns), torch.zeros(1, 1, 64, device="cuda")
+    with pytest.raises(cp.ChiaError, match="INVALID_ARGUMENT"):
+        cp.qk_norm_rope(q, k, None, None, cp.rope_frequencies(64))
+    with pytest.raises(ValueError):
+        cp.qk_norm_rope(q[:, :0], k, None, None, cp.rope_frequencies(64))
+
+
 def test_transforms_are_refused(cuda):
     q, k, qw, kw = (t.detach() for t in leaves())
     freqs = cp.rope_frequencies(64)
