@@ -475,7 +475,14 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout, dlse):
         q, k, v, o, lse = ctx.saved_tensors
-        dq, dk, dv = attention_backward(dout.to(o.dtype), q, k, v, o, lse, **ctx.kw)
+        with torch.no_grad():
+            grads = attention_backward(dout.to(o.dtype), q, k, v, o, lse, **ctx.kw)
+        if torch.is_grad_enabled():
+            # The gradients' own gradients are refused when they are asked for: each gets a node that throws, with
+            # edges to all that the gradients depend on, so that whatever leads to one of them leads through it.
+            refuse = torch._C._functions.DelayedError("attention has no second derivative", 7)
+            grads = refuse(*(g.detach() for g in grads), q, k, v, dout)[:3]
+        dq, dk, dv = grads
         return dq, dk, dv, None, None, None, None, None, None, None, None
 
 
