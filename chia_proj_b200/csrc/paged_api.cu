@@ -217,9 +217,9 @@ struct SplitPlan {
   int grid;   // one CTA an SM
   int64_t off_ml, off_cuts, bytes;
 };
-int split_plan(const chia_paged_params_t *p, bool tree, int sms, SplitPlan &pl) {
+int plan_of(const chia_paged_params_t *p, bool tree, bool tiled, int sms, SplitPlan &pl) {
   const int64_t group = p->heads / p->heads_kv;
-  pl.tiled = p->max_q * group >= kTiledRows && (!tree || p->tokens * group >= kTreeRows * p->batch);
+  pl.tiled = tiled;
   pl.tiles = p->max_q * group <= 8 && !tree ? 1 : 2;  // (trees have units of 16 rows only)
   pl.rows = pl.tiled ? chia::TiledConfig<128>::ROWS : 8 * pl.tiles;
   pl.grid = sms;
@@ -235,6 +235,14 @@ int split_plan(const chia_paged_params_t *p, bool tree, int sms, SplitPlan &pl) 
   pl.off_cuts = (pl.off_ml + slots * 8 + 255) / 256 * 256;
   pl.bytes = pl.off_cuts + (pl.tiled ? (pl.grid * sizeof(chia::CutUnit) + 255) / 256 * 256 : 0);
   return CHIA_OK;
+}
+
+int split_plan(const chia_paged_params_t *p, bool tree, int sms, SplitPlan &pl) {
+  const int64_t group = p->heads / p->heads_kv;
+  const bool tiled = p->max_q * group >= kTiledRows && (!tree || p->tokens * group >= kTreeRows * p->batch);
+  const int rc = plan_of(p, tree, tiled, sms, pl);
+  // (many trees over wide tables: the line in units of 16 rows may be too long where that of 256 is not)
+  return rc != CHIA_OK && tree && !tiled ? plan_of(p, tree, true, sms, pl) : rc;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -417,9 +425,12 @@ int64_t chia_paged_attn_workspace_bytes(const chia_paged_params_t *p) {
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1)
     sms = 148;  // host-only callers (no GPU): size for a B200
-  SplitPlan pl, tree;  // (for chia_tree_attn too)
-  if (split_plan(p, false, sms, pl) != CHIA_OK || split_plan(p, true, sms, tree) != CHIA_OK) return -1;
-  return pl.bytes > tree.bytes ? pl.bytes : tree.bytes;
+  int64_t most = -1;  // (for chia_tree_attn too: each may serve a call that the other does not)
+  for (const bool tree : {false, true}) {
+    SplitPlan pl;
+    if (split_plan(p, tree, sms, pl) == CHIA_OK && pl.bytes > most) most = pl.bytes;
+  }
+  return most;
 }
 
 int chia_paged_attn(const chia_paged_params_t *p, void *stream) { return attend(p, nullptr, nullptr, stream); }

@@ -219,3 +219,22 @@ def test_chunks_attend_as_without_trees(mask, base):
         fin = torch.isfinite(y)
         assert torch.equal(fin, torch.isfinite(x))
         assert (x - y)[fin].abs().max() < 1e-12
+
+
+# 4096 requests of 8 queries each, 64 query and 8 K/V heads, tables of a million tokens: in units of 16 rows the line of
+# key tiles does not fit 32 bits, in units of 256 it does.
+WIDE = dict(PAGED, head_dim=128, heads=64, heads_kv=8, max_q=64, batch=4096, tokens=4096 * 8, num_pages=16384,
+            table_width=16384, table_stride=16384, cu_q=A, q_stride=(8192, 128), o_stride=(8192, 128))
+
+
+@pytest.mark.parametrize("change,served", [
+    (dict(), True),  # (both: in units of 256)
+    (dict(table_width=1000), True),
+    (dict(tokens=4096 * 64), True),
+    (dict(max_q=6), True),  # without trees refused; with them served
+    (dict(table_width=1 << 24, table_stride=1 << 24, num_pages=1 << 24), False),
+    (dict(max_q=6, table_width=1 << 24, table_stride=1 << 24, num_pages=1 << 24), False)])
+def test_workspace_of_wide_tables(lib, change, served):
+    """A size for each call that chia_paged_attn or chia_tree_attn serves."""
+    n = lib.chia_paged_attn_workspace_bytes(packed(N.PagedParams, **{**WIDE, **change}))
+    assert n > 0 if served else n == -1

@@ -362,3 +362,33 @@ def test_steps_of_speculative_decoding(cuda, ct, page, dtype):
                 # half a step: int8 0.5 of the scale; e4m3 2^-4 of the value, or 2^-10 of the scale where it is subnormal
                 step = 0.5 * s if ct == I8 else torch.maximum(want.abs() * 2.0 ** -4, s * 2.0 ** -10)
                 assert ((have - want).abs() <= 4.6 * step).all()
+
+
+def test_wide_tables(cuda):
+    """Tables of a million tokens for 4096 requests, whose line of key tiles fits 32 bits in units of 256 rows only. The
+    lengths are short, so the answer is that with the tables' first columns, from the other kernel; both within the
+    tolerance above, that is within twice of it of one another (mass: at most the largest value, since the weights' sum is
+    1)."""
+    g = torch.Generator().manual_seed(5)
+    B, n, H, hkv, D, page = 4096, 8, 64, 8, 64, 64
+    sizes = [(64 if b % 97 == 0 else 1 + b % 8) for b in range(B)]
+    cu = [0]
+    for m in sizes:
+        cu.append(cu[-1] + m)
+    T = max(cu[-1], B * n)  # (rows behind the last request)
+    lens = [m + b % 50 for b, m in enumerate(sizes)]
+    parents = [i - 1 if i < 2 else i - 2 for m in sizes for i in range(m)]
+    table = torch.full((B, 16384), -1, dtype=torch.int32, device="cuda")
+    table[:, :2] = torch.randint(0, 40, (B, 2), generator=g).to(torch.int32).cuda()
+    q = torch.randn(T, H, D, generator=g).to(BF16).cuda()
+    cache = [torch.randn(40, hkv, page, D, generator=g).mul(100).clamp(-448, 448).to(E4M3).cuda() for _ in range(2)]
+    scale = torch.full((40, hkv), 2.0 ** -7, device="cuda")
+    lens, cu = ints(lens), ints(cu)
+    tree = cp.tree_tables(torch.nn.functional.pad(ints(parents), (0, T - len(parents))), cu, lens)
+    with torch.no_grad():
+        wide = cp.paged_attention(q, *cache, scale, scale, table, lens, cu, max_q=64, tree=tree)
+        near = cp.paged_attention(q, *cache, scale, scale, table[:, :2].contiguous(), lens, cu, max_q=64, tree=tree)
+    rows = int(cu[-1])
+    top = 448 * 2.0 ** -7
+    err = (wide[:rows].float() - near[:rows].float()).abs()
+    assert (err <= 2.0 ** -7 * near[:rows].float().abs() + 2.0 ** -9 * top).all()
