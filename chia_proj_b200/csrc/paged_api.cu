@@ -226,7 +226,7 @@ int plan_of(const chia_paged_params_t *p, bool tree, bool tiled, int sms, SplitP
   // the line of tiles is counted in 32 bits
   const int tk = pl.tiled ? 64 : 32;
   const double line = static_cast<double>(p->heads_kv) * (p->tokens * group / pl.rows + p->batch + 1) *
-                      (p->table_width * p->page_size / tk + 2 + chia::kUnitCost);
+                      (p->table_width * p->page_size / tk + 2 + (pl.tiled ? chia::kTiledCost : chia::kUnitCost));
   if (pl.grid * 4 > kTicketBytes || p->tokens * p->heads > kI32 ||
       p->tokens * group * group > 2 * kI32 || line > kI32)
     return CHIA_ERR_UNSUPPORTED;

@@ -170,3 +170,12 @@ def test_python_refusals(cuda):
         with pytest.raises(ValueError):
             cp.page_tables(*args, page_size=16, max_tokens=2)
     cp.check_device_status(0)
+
+
+def test_the_line_of_tiles_fits_32_bits(lib):
+    """2^20 K/V heads of 338 requests of up to 48 keys: units of one tile each, which count as 7 with what a unit costs in the
+    kernel for many rows."""
+    p = dict(PAGED, heads=1 << 20, heads_kv=1 << 20, page_size=16, table_width=3, table_stride=3, max_q=56, num_pages=1000)
+    assert 338 * 2 ** 20 * 7 > 2 ** 31 > 200 * 2 ** 20 * 8 * 257 / 256
+    assert lib.chia_paged_attn_workspace_bytes(packed(N.PagedParams, **{**p, "batch": 338, "tokens": 338})) == -1
+    assert lib.chia_paged_attn_workspace_bytes(packed(N.PagedParams, **{**p, "batch": 200, "tokens": 200})) > 0
