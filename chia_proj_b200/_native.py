@@ -124,6 +124,7 @@ PAGED_SYMBOLS = (
 
 # ---- trees of drafted tokens (include/chia_draft.h), norm and rotation (include/chia_rope.h)
 DRAFT_ABI_VERSION = 1
+COMPACT_ABI_VERSION = 2
 ROPE_ABI_VERSION = 1
 TREE_NODES = 64
 
@@ -306,6 +307,8 @@ class CompactParams(ctypes.Structure):
         ("v_scale", ctypes.c_void_p),
         ("keep_lens", ctypes.c_void_p),
         ("status", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
     ]
 
 

@@ -121,11 +121,11 @@ PyObject *verify(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 }
 
 // ------------------------------------------------------------------ compaction
-// path, counts, cu_q, seq_lens, block_table, k_cache, v_cache, k_scale, v_scale, status
+// path, counts, cu_q, seq_lens, block_table, k_cache, v_cache, k_scale, v_scale, status, slots
 PyObject *compact(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject * {
     const at::AutoDispatchBelowADInplaceOrView plain;
-    const Args a(args, nargs, 10);
+    const Args a(args, nargs, 11);
     const Cache c(a, 5);
     const Tensor &path = a.tensor(0, "path", 2), &table = a.tensor(4, "block_table", 2);
     const int64_t B = table.size(0), W = table.size(1), most = path.size(1);
@@ -139,7 +139,7 @@ PyObject *compact(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const c10::cuda::CUDAGuard guard(c.dev);
     Tensor keep = at::empty({B}, lens.options());
     chia_compact_params_t p{};
-    p.abi_version = CHIA_DRAFT_ABI_VERSION;
+    p.abi_version = CHIA_COMPACT_ABI_VERSION;
     p.cache_dtype = c.type;
     p.head_dim = static_cast<int32_t>(c.dim);
     p.heads_kv = static_cast<int32_t>(c.heads);
@@ -160,6 +160,10 @@ PyObject *compact(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     p.v_scale = ptr<float>(c.vs);
     p.keep_lens = ptr<int32_t>(keep);
     p.status = reinterpret_cast<int32_t *>(a.integer(9));
+    if (!a.none(10)) {
+      p.tokens = a.tensor(10, "slots", 1).size(0);
+      p.slots = ptr<int32_t>(a.ints(10, "slots", {p.tokens}, c.dev));
+    }
     const int code = g_compact(&p, c10::cuda::getCurrentCUDAStream(c.dev.index()).stream());
     if (code != CHIA_OK) return PyLong_FromLong(code);
     for (const Tensor *t : {&c.k, &c.v, &c.ks, &c.vs}) written(*t);

@@ -130,7 +130,9 @@ int chia_verify_drafts(const chia_verify_params_t *p, void *stream) {
 }
 
 int chia_cache_compact(const chia_compact_params_t *p, void *stream) {
-  if (p == nullptr || p->abi_version != CHIA_DRAFT_ABI_VERSION) return CHIA_ERR_INVALID_ARGUMENT;
+  if (p == nullptr || p->abi_version < 1 || p->abi_version > CHIA_COMPACT_ABI_VERSION) return CHIA_ERR_INVALID_ARGUMENT;
+  const int32_t *slots = p->abi_version > 1 ? p->slots : nullptr;  // (the field is not there before)
+  if (slots != nullptr && p->tokens < 0) return CHIA_ERR_INVALID_ARGUMENT;
   if (p->cache_dtype != CHIA_CACHE_E4M3 && p->cache_dtype != CHIA_CACHE_INT8) return CHIA_ERR_UNSUPPORTED;
   if ((p->head_dim != 64 && p->head_dim != 128) ||
       (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128))
@@ -144,7 +146,7 @@ int chia_cache_compact(const chia_compact_params_t *p, void *stream) {
     return CHIA_ERR_INVALID_ARGUMENT;
   if (!aligned(p->k_cache, 16) || !aligned(p->v_cache, 16) || !aligned(p->k_scale, 4) || !aligned(p->v_scale, 4) ||
       !aligned(p->path, 4) || !aligned(p->counts, 4) || !aligned(p->cu_q, 4) || !aligned(p->seq_lens, 4) ||
-      !aligned(p->block_table, 4) || !aligned(p->keep_lens, 4) || !aligned(p->status, 4))
+      !aligned(p->block_table, 4) || !aligned(p->keep_lens, 4) || !aligned(p->status, 4) || !aligned(slots, 4))
     return CHIA_ERR_MISALIGNED;
   const int64_t grid = p->batch * 2 * p->heads_kv;
   if (grid > kI32) return CHIA_ERR_UNSUPPORTED;
@@ -163,6 +165,8 @@ int chia_cache_compact(const chia_compact_params_t *p, void *stream) {
   a.v_scale = p->v_scale;
   a.keep_lens = p->keep_lens;
   a.status = p->status;
+  a.slots = slots;
+  a.tokens = slots != nullptr ? p->tokens : 0;
   a.table_stride = p->table_stride;
   a.num_pages = p->num_pages;
   a.batch = static_cast<int32_t>(p->batch);

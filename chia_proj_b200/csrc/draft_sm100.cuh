@@ -447,7 +447,8 @@ struct CompactArgs {
   uint8_t *k_cache, *v_cache;
   float *k_scale, *v_scale;
   int32_t *keep_lens, *status;
-  int64_t table_stride, num_pages;
+  const int32_t *slots;  // [tokens] or null
+  int64_t table_stride, num_pages, tokens;
   int32_t batch, most, heads_kv, page, width;
 };
 
@@ -476,6 +477,13 @@ __global__ void __launch_bounds__(kCompactThreads) cache_compact_kernel(const Co
   if (n > kTreeNodes && t0 >= 0) {  // a chunk: nothing of it was drafted
     if (which == 0 && t == 0) a.keep_lens[b] = len;
     return;
+  }
+  if (a.slots != nullptr) {  // a request without a place for its tokens: len has no tree in it
+    const bool missing = t0 >= 0 && t < n && (static_cast<int64_t>(t0) + t >= a.tokens || a.slots[t0 + t] < 0);
+    if (__syncthreads_or(missing)) {
+      if (which == 0 && t == 0) a.keep_lens[b] = len;
+      return;
+    }
   }
   bool bad = t0 < 0 || n < 0 || len < n || count < 0 || count > n || count > a.most ||
              len > static_cast<int64_t>(a.width) * a.page;

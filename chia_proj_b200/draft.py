@@ -13,7 +13,7 @@ root. A row of single drafts is the tree with ``parents = -1, 0, 1, ...``. On on
     # then
     done = verify_drafts(target_probs, tokens, parents, step.cu_q, uniforms, draft_probs=..., max_tokens=...)
     # in each layer
-    keep = cache_compact(done.path, done.counts, step.cu_q, step.seq_lens, block_table, *cache)
+    keep = cache_compact(done.path, done.counts, step.cu_q, step.seq_lens, block_table, *cache, step.slots)
     seq_lens, free_state = release_pages(None, step.seq_lens, block_table, free_pages, step.free_state,
                                          page_size=64, keep_lens=keep)
 
@@ -82,16 +82,20 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, parents: tor
 
 def cache_compact(path: torch.Tensor, counts: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
                   block_table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
-                  v_scale: torch.Tensor) -> torch.Tensor:
+                  v_scale: torch.Tensor, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Move the keys and values of an accepted path together, in place: node ``path[b, i]``'s go to the place of node
     ``i``, for ``i < counts[b]``. Returns the lengths that the requests keep, ``[B]`` int32, for ``release_pages``.
 
     A page keeps its scale or, where a page that its new tokens come from has a larger one, takes that and has its values
     expressed in it, as in ``cache_append``. A path rises. One that does not, or whose pages are out of range, is
     reported, and its request left as it is; requests of more than 64 tokens (chunks) are left as they are.
+
+    ``slots`` (``[T]`` int32, what ``page_tables`` returned): a request that it did not serve, whose tokens have no slot,
+    is left as it is with its length, so that the step may be run again. Without ``slots`` the last tokens of such a request,
+    which are none of the tree's, would be taken for it.
     """
     r = N.binding().compact(path, counts, cu_q, seq_lens, block_table, k_cache, v_cache, k_scale, v_scale,
-                            _status(k_cache))
+                            _status(k_cache), slots)
     if type(r) is int:
         N.check(r, f"chia_cache_compact(path={tuple(path.shape)}, cache={tuple(k_cache.shape)})")
     return r

@@ -31,6 +31,7 @@ extern "C" {
 #endif
 
 #define CHIA_DRAFT_ABI_VERSION 1
+#define CHIA_COMPACT_ABI_VERSION 2
 #define CHIA_TREE_NODES 64
 
 /* ------------------------------------------------------------------ tables */
@@ -112,7 +113,7 @@ CHIA_API int chia_verify_drafts(const chia_verify_params_t *params, void *stream
 
 /* -------------------------------------------------------------- compaction */
 typedef struct chia_compact_params {
-  int32_t abi_version;
+  int32_t abi_version; /* CHIA_COMPACT_ABI_VERSION, or 1: without the last two */
   int32_t cache_dtype; /* enum chia_cache_dtype                              */
   int32_t head_dim;    /* 64 or 128                                          */
   int32_t heads_kv;
@@ -135,6 +136,9 @@ typedef struct chia_compact_params {
   int32_t *keep_lens; /* out [batch]: seq_lens[b] - n + counts[b], what
                          chia_trim_pages takes                               */
   int32_t *status;    /* optional                                            */
+  const int32_t *slots; /* [tokens], those of chia_page_tables, or NULL: every
+                           request's tokens are in the cache                 */
+  int64_t tokens;
 } chia_compact_params_t;
 
 /* Keys and values of node path[b][i] go to the place of node i, for i < counts[b].
@@ -142,6 +146,8 @@ typedef struct chia_compact_params {
  * that is larger than its own, and what it holds is then expressed in it, as
  * chia_cache_append does. A request whose path does not rise, has nodes that are not
  * its own or pages out of range is reported and left as it is, with its seq_lens[b].
+ * So, without a report, is one that chia_page_tables did not serve (a slot of its
+ * tokens is -1): its seq_lens[b] has no tree in it, and the step may be run again.
  * No two requests share a page that is written. */
 CHIA_API int chia_cache_compact(const chia_compact_params_t *params, void *stream);
 

@@ -238,3 +238,13 @@ def test_workspace_of_wide_tables(lib, change, served):
     """A size for each call that chia_paged_attn or chia_tree_attn serves."""
     n = lib.chia_paged_attn_workspace_bytes(packed(N.PagedParams, **{**WIDE, **change}))
     assert n > 0 if served else n == -1
+
+
+@pytest.mark.parametrize("change,code", [(dict(abi_version=3), 1), (dict(abi_version=2, slots=A + 2), 3),
+                                         (dict(abi_version=2, slots=A, tokens=-1), 1), (dict(abi_version=1, slots=A + 2), 6),
+                                         (dict(abi_version=2), 6), (dict(abi_version=2, slots=A, tokens=8), 6)])
+def test_compact_refusals_with_slots(lib, change, code):
+    """(6: no GPU here, the arguments were taken. Version 1 has no slots.)"""
+    if code == 6 and torch.cuda.is_available():
+        pytest.skip("would launch")
+    assert lib.chia_cache_compact(packed(N.CompactParams, **{**COMPACT, **change}), None) == code

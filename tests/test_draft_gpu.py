@@ -372,3 +372,63 @@ def test_refusals(cuda):
                 dict(k_cache=cache[0].view(torch.int8)), dict(v_scale=cache[3][:1])):
         with pytest.raises(ValueError):
             cp.cache_compact(**{**good, **bad})
+
+
+@pytest.mark.parametrize("ct,page", [(E4M3, 16), (I8, 64)])
+def test_a_step_that_was_not_served_can_be_run_again(cuda, ct, page):
+    """The second of three requests finds no page. Its cache and its length stay as they were, the others go on as alone;
+    with pages the same step serves it."""
+    g = torch.Generator().manual_seed(page)
+    B, hkv, D, n = 3, 2, 64, 12
+    start = [page - 3, 2 * page - 2, 5]  # the first and the second need a page for 12 more (the third, in small pages)
+    cache = cp.new_cache(12, hkv, D, page_size=page, dtype=ct)
+    table, ring = ints([[0] * 4] * B), torch.arange(12, dtype=torch.int32, device="cuda")
+    first = cp.page_tables(ints([0] * B), ints(start), table, ring, ints([0, 12]), page_size=page, max_tokens=sum(start))
+    kv = torch.randn(sum(start), 2, hkv, D, generator=g).to(torch.bfloat16).cuda()
+    cp.cache_append(kv[:, 0], kv[:, 1], first.slots, *cache)
+    parents = [-1, 0, 0, 1, 1, 2, 2, 5, 6, 7, 8, 9]
+    kv = torch.randn(B * n, 2, hkv, D, generator=g).to(torch.bfloat16).cuda()
+    path, counts = ints([[0, 2, 6, 8]] * B), ints([4] * B)
+
+    def step(cache, table, free):
+        st = cp.page_tables(first.seq_lens, ints([n] * B), table, ring, free, page_size=page, max_tokens=B * n)
+        cp.tree_tables(ints(parents * B), st.cu_q, st.seq_lens)
+        cp.cache_append(kv[:, 0], kv[:, 1], st.slots, *cache)
+        return st, cp.cache_compact(path, counts, st.cu_q, st.seq_lens, table, *cache, st.slots)
+
+    copy = lambda: ([t.clone() for t in cache], table.clone())
+    (few, few_table), (all_, all_table) = copy(), copy()
+    head = int(first.free_state[0])
+    st, keep = step(few, few_table, ints([head, 1]))  # a page for the first alone
+    with pytest.raises(cp.ChiaError, match="NO_PAGES"):
+        cp.check_device_status(0)
+    served = [bool((st.slots[b * n:(b + 1) * n] >= 0).all()) for b in range(B)]
+    assert served[0] and not served[1]
+    assert keep.tolist() == [s + 4 if ok else s for s, ok in zip(start, served)]
+    st2, keep2 = step(all_, all_table, ints([head, 12 - head]))
+    assert keep2.tolist() == [s + 4 for s in start]
+    used = lambda tab, b, m: tab[b, :po.pages_for(m, page)].long()
+    for b in range(B):
+        for a, c, was in zip(*([t.view(torch.uint8) for t in ts] for ts in (few, all_, cache))):
+            if served[b]:  # as with pages enough (a page of another number may hold it)
+                x, y = a[used(few_table, b, start[b] + n)], c[used(all_table, b, start[b] + n)]
+            else:
+                x, y = a[used(few_table, b, start[b])], was[used(table, b, start[b])]
+            assert torch.equal(x, y)
+    # without the slots the last tokens of the request would be moved
+    lost = [t.clone() for t in cache]
+    bad = cp.cache_compact(path[1:2], counts[1:2], ints([0, n]), st.seq_lens[1:2], few_table[1:2], *lost)
+    assert bad.tolist() == [start[1] - n + 4]
+
+
+def test_compact_refuses_other_slots(cuda):
+    cache = [t.cuda() for t in cache_of(2, 1, 16, 64, E4M3, torch.Generator().manual_seed(1))]
+    args = (ints([[0, 1]]), ints([2]), ints([0, 2]), ints([2]), ints([[0]]), *cache)
+    assert cp.cache_compact(*args, ints([0, 1])).tolist() == [2]
+    assert cp.cache_compact(*args, ints([0])).tolist() == [2] and cp.cache_compact(*args, ints([0, -1])).tolist() == [2]
+    assert cp.cache_compact(*args, torch.empty(0, dtype=torch.int32, device="cuda")).tolist() == [2]
+    for bad in (torch.tensor([0, 1], device="cuda"), ints([[0, 1]]), ints([0, 9, 1, 9])[::2]):
+        with pytest.raises(ValueError):
+            cp.cache_compact(*args, bad)
+    with pytest.raises(RuntimeError):
+        cp.cache_compact(*args, torch.zeros(2, dtype=torch.int32))
