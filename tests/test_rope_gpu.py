@@ -338,3 +338,26 @@ def test_refusals(cuda):
         cp.qk_norm_rope_backward(q, k[:, :, :3], **good)
     with pytest.raises(RuntimeError):
         cp.qk_norm_rope(**{**good, "freqs": f.cpu()})
+
+
+@pytest.mark.parametrize("dtype,T,H,Hk,D,one_sign", [(BF16, 60001, 8, 1, 64, False), (BF16, 60001, 8, 1, 64, True),
+                                                     (F32, 4 * 4096, 16, 16, 128, True)])
+def test_long_sums_of_the_weights_gradients(cuda, dtype, T, H, Hk, D, one_sign):
+    """Sums over up to half a million rows, also of products that all have one sign, where roundings add up. A thread adds
+    the rows of its group, T H over the groups of all CTAs (4 an SM, of 16 or 8 groups; twice as many are allowed for, since
+    groups differ by a token), then up to 16, 19 and 32 parts. A sum of n additions in a row is off by n 2^-24 of the
+    terms' sizes, and 2^-19 of them for the products."""
+    g = torch.Generator().manual_seed(T + one_sign)
+    q, k = (torch.randn(T, h, D, generator=g).to(dtype).cuda() for h in (H, Hk))
+    w = torch.ones(D, device="cuda")
+    dq, dk = (torch.randn(x.shape, generator=g).to(dtype).cuda() for x in (q, k))
+    if one_sign:
+        dq, dk = dq.abs() * q.sign(), dk.abs() * k.sign()
+    freqs = cp.rope_frequencies(0)
+    got = cp.qk_norm_rope_backward(dq, dk, q, k, w, w, freqs)[2:]
+    for x, dy, dw, h in ((q, dq, got[0], H), (k, dk, got[1], Hk)):
+        xd, gd = x.double(), dy.double()
+        xhat = xd / torch.sqrt((xd * xd).mean(-1, keepdim=True) + EPS)
+        want, size = (gd * xhat).flatten(0, 1).sum(0), (gd * xhat).abs().flatten(0, 1).sum(0)
+        chain = 2 * T * h / (4 * 132 * (128 // (D // 8))) + 100
+        assert ((dw.double() - want).abs() <= (chain * 2.0 ** -24 + 2.0 ** -19) * size + 2.0 ** -24 * want.abs()).all()

@@ -392,3 +392,38 @@ def test_wide_tables(cuda):
     top = 448 * 2.0 ** -7
     err = (wide[:rows].float() - near[:rows].float()).abs()
     assert (err <= 2.0 ** -7 * near[:rows].float().abs() + 2.0 ** -9 * top).all()
+
+
+def test_a_step_with_chunks_and_trees(cuda):
+    """Trees first, chunks of prompts behind them: one call for all where they are alike, and the trees' part of the tables
+    for the verification and the compaction."""
+    g = torch.Generator().manual_seed(11)
+    H, hkv, D, V, page, pages = 8, 2, 64, 200, 16, 60
+    sizes, drafted = [13, 5, 40, 90], 2  # two trees; chunks of 40 and of 90 tokens
+    B, T, n = len(sizes), sum(sizes), sum(sizes[:2])
+    cache = cp.new_cache(pages, hkv, D, page_size=page)
+    table, ring = ints([[0] * 12] * B), torch.arange(pages, dtype=torch.int32, device="cuda")
+    lens, state = ints([0] * B), ints([0, pages])
+    for it in range(2):
+        cu = [sum(sizes[:i]) for i in range(B + 1)]
+        parents = [p for i in range(drafted) for p in do.tree(sizes[i], 10 * it + i)]
+        parents += [i - 1 for m in sizes[drafted:] for i in range(m)]  # (a chunk of up to 64 tokens is a row)
+        q, k, v = torch.randn(T, H + 2 * hkv, D, generator=g).to(BF16).cuda().split([H, hkv, hkv], 1)
+        before = lens.tolist()
+        st = cp.page_tables(lens, ints(sizes), table, ring, state, page_size=page, max_tokens=T)
+        tree = cp.tree_tables(ints(parents), st.cu_q, st.seq_lens)
+        cp.cache_append(k, v, st.slots, *cache)
+        got = cp.paged_attention(q, *cache, table, st.seq_lens, st.cu_q, max_q=max(sizes), tree=tree)
+        c = dict(q=q.cpu(), k=cache[0].cpu(), v=cache[1].cpu(), ks=cache[2].cpu(), vs=cache[3].cpu(), table=table.tolist(),
+                 lens=st.seq_lens.tolist(), cu=cu, parents=parents)
+        check(c, got)
+        p = torch.softmax(torch.randn(n, V, generator=g), 1)
+        tokens, u = torch.randint(0, V, (n,), generator=g).tolist(), torch.rand(n, generator=g)
+        part = st.cu_q[:drafted + 1]
+        done = cp.verify_drafts(p.cuda(), ints(tokens), ints(parents[:n]), part, u.cuda(), max_tokens=9)
+        counts, toks, path = do.verify(p, tokens, parents[:n], cu[:drafted + 1], u, None, 9)
+        assert done.counts.tolist() == counts and done.tokens.tolist() == toks and done.path.tolist() == path
+        keep = cp.cache_compact(done.path, done.counts, part, st.seq_lens[:drafted], table[:drafted], *cache, st.slots)
+        keep = torch.cat([keep, st.seq_lens[drafted:]])
+        lens, state = cp.release_pages(None, st.seq_lens, table, ring, st.free_state, page_size=page, keep_lens=keep)
+        assert lens.tolist() == [b + (counts[i] if i < drafted else sizes[i]) for i, b in enumerate(before)]
