@@ -178,8 +178,10 @@ __device__ __forceinline__ double shfl_up(double x, int d) { return __shfl_up_sy
 // Measured, fp32: 64 trees of up to 25 nodes over 131,072 entries, drafts drawn at random, 28.5 us,
 // where the rows that tokens are drawn from take 10 at the rate of a copy: some 4 us to the first pass
 // (offsets, nodes, their probabilities), 3 to 4 a pass, up to five passes one behind another in a
-// request; one chain of five drafts over 32,000 entries 5.0. An entry costs a conversion and two 64-bit
-// operations; with single entries a load and a maximum in 64 bits the trees took 102 us.
+// request; one chain of five drafts over 32,000 entries 5.0. An entry of a row costs a conversion, one of the
+// target's two 64-bit operations beside; with single entries a load and a maximum in 64 bits the trees took
+// 102 us. Rows whose width or address is no multiple of four entries are read entry by entry: 27.5 us over
+// 131,072 entries are 35.9 over 131,073, and 15.5 over 50,256 are 17.7 over 50,257.
 template <int T, bool DRAFTS, bool VEC>
 __global__ void __launch_bounds__(kVerifyMostThreads, 1) verify_kernel(const VerifyArgs a) {
   __shared__ double s_sum[kVerifyMostChunks];  // of this CTA's chunks

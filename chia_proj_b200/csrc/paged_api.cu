@@ -206,7 +206,10 @@ constexpr int64_t kTiledRows = 56;
 // goes by the rows that there are, the tiled kernel's by the requests. Split and tiled, us, D 128,
 // 8 K/V heads, all requests alike: 8 x 4096 keys, 64 rows 64, 68, 72 rows 76, 69; 32 x 2048, 64 rows
 // 120, 114, 80 rows 145, 114. Sizes spread from one node up to 80 rows (30 in the mean) 32, 53, to
-// 96 rows 45, 53.
+// 96 rows 45, 53. The mean says little where requests are very unequal, padding among them. Split
+// (the rule's choice) and tiled (that without trees): a tree of 64 nodes beside 63 single tokens, group
+// 4, 4096 keys 137, 340; a chunk of 512 beside them 336, 381; but that chunk over 32,768 keys beside 1024
+// of the others 1429, 437; 8 trees of 64 nodes, group 8, in a batch padded to 64 392, 115 (118 unpadded).
 constexpr int64_t kTreeRows = 65;
 struct SplitPlan {
   bool tiled;

@@ -151,12 +151,15 @@ __device__ __noinline__ void nan_channels(const PagedArgs &a, const uint8_t *v_c
 }
 
 // TREE: requests of up to kTreeNodes queries are trees of drafted tokens, as in the split kernel.
-// Measured (D 128, e4m3, bf16, 8 K/V heads): 8 x 64 nodes of 64 heads over 4,096 keys 119 us, 16 x 25
-// of 32 over 16,000 323, 32 x 1 to 64 of 64 over up to 16,384 keys, capped, 314. A tile takes 2,400
-// to 3,500 cycles whatever its rows: 1,140 of the conversion, 700 of waits for copies, 1,700 to 2,150
-// of the softmax. Tried for units of up to 128 rows: both halves of the softmax warps with the same
-// rows, a key tile each by turns, joined at the end: 291 and 300 us on 16 x 25 nodes, 337 and 330
-// capped; warps without rows that do no arithmetic: 325 and 314 capped.
+// Measured (D 128, e4m3, bf16, 8 K/V heads): 8 x 64 nodes of 64 heads over 4,096 keys 118 us, 16 x 25
+// of 32 over 16,000 313 to 323, 32 x 1 to 64 of 64 over up to 16,384 keys, capped, 315. A tile takes
+// 2,400 to 3,500 cycles where its unit has up to 128 rows (1,140 of the conversion, 700 of waits for
+// copies, 1,700 to 2,150 of the softmax), up to 5,000 in a full unit with capped scores; the line
+// counts them alike, so the CTA with most full units is the last: 123 tiles of 5,000 cycles are 313
+// us. Tried for units of up to 128 rows: both halves of the softmax warps with the same rows, a key
+// tile each by turns, joined at the end: 291 us on 16 x 25 nodes, where warps without rows that did no
+// arithmetic took 300; capped 337 and 330. Without that skipping, as it is now, the capped trees took
+// 314 us for 325 and the 16 x 25 nodes 313 to 323 for 300.
 template <int D, int CT, int KIND, bool BF16, bool TREE>
 __global__ void __launch_bounds__(kTiledThreads, 1)
 paged_tiled_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,

@@ -183,7 +183,7 @@ __device__ __forceinline__ RopeVals rope_weights(const RopeArgs &a, const void *
 // Cosines and sines of four angles, turns in units of 2^-64. The nearest quarter turn goes to a
 // choice of signs and sides; what is left, |x| <= pi / 4, to the Taylor polynomials
 //   sin x = x - x^3/3! + .. + x^9/9!,  cos x = 1 - x^2/2! + .. + x^10/10!
-// whose next terms are 2^-29 and 2^-30.
+// whose next terms are 2^-29 and 2^-33.
 __device__ __forceinline__ void rope_angles(const uint64_t (&turn)[4], uint64_t (&cos)[2], uint64_t (&sin)[2]) {
   float c[4], s[4];
 #pragma unroll

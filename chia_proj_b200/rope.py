@@ -51,9 +51,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     ``q`` ``[T, H, D]``, ``k`` ``[T, H_kv, D]`` with ``positions`` ``[T]``, or ``[B, H, S, D]``, ``[B, H_kv, S, D]`` with
     ``[S]`` or ``[B, S]`` (int32; ``None``: 0, 1, ...); bf16, fp16 or fp32, ``D`` 64 or 128. Views of a fused projection
     are taken as they are (strides that are multiples of 8 elements, unit last stride); outputs have their order of
-    dimensions. ``q_weight``, ``k_weight`` ``[D]`` (bf16, fp16 or fp32; ``None``: ones, without the offset). Pair ``i`` is
+    dimensions. ``q_weight``, ``k_weight`` ``[D]`` (bf16, fp16 or fp32; ``None``: ones, without the offset; the rows are
+    normed all the same). Pair ``i`` is
     channels ``i`` and ``i + rot / 2``, or neighbours with ``interleaved``. ``freqs``: ``rope_frequencies``; an empty one
-    turns nothing. Computed in 32 bits and rounded once. Differentiable in ``q``, ``k`` and the weights, once; only the inputs are kept for the backward pass.
+    turns nothing. Computed in 32 bits and rounded once. Differentiable in ``q``, ``k`` and the weights, once
+    (a second derivative is an error); only the inputs are kept for the backward pass.
     """
     r = N.binding().qk_norm_rope(q, k, q_weight, k_weight, freqs, positions, eps, interleaved, weight_offset)
     if type(r) is int:

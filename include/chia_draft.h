@@ -61,8 +61,9 @@ CHIA_API int chia_tree_tables(const chia_tree_params_t *params, void *stream);
  * score modifications likewise). The workspace is that of chia_paged_attn.
  * positions and ancestors are those of chia_tree_tables; a position outside of its
  * request's tokens counts as the nearest inside. The words may hold any nodes of
- * the request. Requests of more than CHIA_TREE_NODES queries are served as by
- * chia_paged_attn. */
+ * the request. Requests of more than CHIA_TREE_NODES queries see what they see in
+ * chia_paged_attn. The kernel is chosen for the call, by the mean number of rows of a
+ * request: padding (requests without tokens) counts in it. */
 CHIA_API int chia_tree_attn(const chia_paged_params_t *params, const int32_t *positions,
                             const uint64_t *ancestors, void *stream);
 
@@ -108,7 +109,10 @@ typedef struct chia_verify_params {
  * out_tokens[b]: the accepted tokens, then the drawn one; path[b]: node 0, then the
  * accepted nodes; counts[b] of each, -1 behind them. counts[b] is 0 for a request
  * without tokens. A request of more than CHIA_TREE_NODES tokens is reported and
- * gets 0; a parent or token out of range is reported, its node never accepted. */
+ * gets 0; a parent or token out of range is reported, its node never accepted. A
+ * request of fewer is a tree whatever it holds: with chunks of prompts in a step, pass
+ * the offsets of the trees alone. Rows are read four entries at a time where their
+ * addresses are multiples of that. */
 CHIA_API int chia_verify_drafts(const chia_verify_params_t *params, void *stream);
 
 /* -------------------------------------------------------------- compaction */
